@@ -23,10 +23,13 @@
 extern "C" {
 #endif
 
-#define SWARP_ABI_VERSION 16
+#define SWARP_ABI_VERSION 17
 
 #define SWARP_F32 0
 #define SWARP_F64 1
+/* 16-bit scalars: heads and parameters of the policy update only (below) */
+#define SWARP_BF16 2
+#define SWARP_F16 3
 
 /* desc->integrator (the reference's Integrator, swarp/dynamics/base.py:97-101) */
 #define SWARP_EULER 0
@@ -396,6 +399,129 @@ int swarp_edge_index_noalloc(int32_t n_envs, int32_t n_agents, int32_t max_neigh
  * quaternion (0, 0, 0, 1) per agent.  `buf` must be 16-byte aligned.  Replaces the zero
  * and identity tensors of fill_state_defaults (swarp/interop/autograd.py:48-68). */
 int swarp_state_defaults(int32_t dtype, int64_t n, void *buf, void *stream);
+
+/* ------------------------------------------------------------------ the policy update
+ * What follows a rollout when a policy is trained on it: advantages, the clipped policy
+ * loss with its gradient, and the optimizer step.  Own operators of this build: the
+ * reference trains with torch operations (its swarp/rl package). */
+
+/* Generalised advantage estimation of T steps of N columns (one per env and agent):
+ *   n_t = 0 where terminated, final_values_t where truncated and final_values is set, else
+ *         V_{t+1};   d_t = r_t + gamma n_t - V_t;
+ *   A_t = d_t + (terminated or truncated ? 0 : gamma lam A_{t+1}),  A_T = 0;  R_t = A_t + V_t.
+ * Values of a step that is not read (V_{t+1} or final_values_t where the flags say so) may be
+ * anything, NaN included. */
+typedef struct swarp_gae {
+    int32_t dtype;            /* SWARP_F32 or SWARP_F64 */
+    int32_t rows;             /* 0: time first, arrays [T,N]; 1: time last, arrays [N,T] */
+    int64_t steps, columns;   /* T >= 0, N >= 0 */
+    int64_t group;            /* consecutive columns that share their flags (N a multiple) */
+    double gamma, lam;
+    const void *rewards;      /* [T,N] or [N,T] */
+    const void *values;       /* [T+1,N] or [N,T+1] */
+    const uint8_t *terminated, *truncated; /* [T,N/group] or [N/group,T], nonzero = true; NULL:
+                                              never */
+    const void *final_values; /* as rewards; NULL: a truncated step reads V_{t+1} */
+    void *advantages, *returns;            /* as rewards; written by swarp_gae_fwd */
+    const void *adj_advantages, *adj_returns; /* as rewards, NULL = zero; read by
+                                                 swarp_gae_bwd */
+    void *adj_rewards, *adj_values, *adj_final_values; /* as rewards, values, final_values;
+                                                          written by swarp_gae_bwd (NULL = not
+                                                          wanted) */
+} swarp_gae_t;
+int swarp_gae_fwd(const swarp_gae_t *a, void *stream);
+int swarp_gae_bwd(const swarp_gae_t *a, void *stream);
+
+/* The clipped policy loss of `rows` decisions, and its gradient.  With lp the log-probability
+ * of the action taken, q = ref_logp (old_logp where that is NULL), A the advantage and
+ * H the entropy of a decision:
+ *   rho = exp(lp - old_logp);  s = -min(rho A, clamp(rho, 1 - clip_low, 1 + clip_high) A);
+ *   kl = exp(q - lp) - 1 - (q - lp);   l = s + kl_coef kl - entropy_coef H;
+ *   loss = w sum of l over the decisions whose mask is set, w = 1 / max(1, their number) or 1.
+ * A masked decision's other inputs are not read into any result: its logp is 0, its gradient
+ * rows are zero.
+ * Categorical head: decision r has the logits at head + (r / inner) outer_stride
+ * + (r % inner) inner_stride (in elements), `width` of them; -inf is an action that is not
+ * open.  A decision whose logits hold NaN or +inf or only -inf, or whose action is outside
+ * [0, width), has a NaN logp, loss and gradient row.
+ * Gaussian head: mean and actions [rows, width], log_std [width] (shared_std) or [rows, width],
+ * width <= 64; lp and H are sums over the width dimensions. */
+typedef struct swarp_policy {
+    int32_t dtype;            /* of the heads and their gradients; everything else that is not
+                                 an integer is float, or double with SWARP_F64 */
+    int32_t sum;              /* 1: loss is the sum, 0: the mean */
+    int32_t width;            /* actions of a categorical head, dimensions of a Gaussian one */
+    int32_t actions32;        /* categorical: actions are int32 (0: int64) */
+    int32_t shared_std;
+    int32_t skip_unit;        /* 1: nothing is written where *scale is 1 (see swarp_policy_*) */
+    int64_t rows;
+    int64_t inner, outer_stride, inner_stride;
+    double clip_low, clip_high, kl_coef, entropy_coef;
+    const void *head;         /* logits, or mean */
+    const void *log_std;
+    const void *actions;      /* [rows] integers, or [rows, width] */
+    const void *old_logp, *advantages; /* [rows] */
+    const void *ref_logp;     /* [rows] or NULL */
+    const uint8_t *mask;      /* [rows], nonzero = counts; NULL: all count */
+    void *logp;               /* [rows] or NULL */
+    void *loss;               /* [1], set together with stats, or NULL */
+    void *stats;              /* [3]: the means over the counted decisions of the entropy, the
+                                 kl and whether the clip was active; or NULL */
+    void *d_head;             /* [rows, width] contiguous, or NULL: no gradient */
+    void *d_log_std;          /* as log_std, or NULL */
+    const void *scale;        /* [1] on the device: the gradients are times this; NULL: 1 */
+    void *work;               /* swarp_policy_work_bytes(rows, width) bytes, 16-byte aligned */
+    uint64_t work_bytes;
+} swarp_policy_t;
+/* A forward with the gradient writes logp, stats and the gradients for an upstream gradient of
+ * 1.  The backward is the same call with logp, loss and stats NULL, scale the upstream gradient and
+ * skip_unit = 1 into the same buffers: where the upstream gradient is 1 they are right as they
+ * stand, else they are computed again with it.  Which it is, the device decides. */
+uint64_t swarp_policy_work_bytes(int64_t rows, int32_t width);
+int swarp_categorical_loss(const swarp_policy_t *a, void *stream);
+int swarp_gaussian_loss(const swarp_policy_t *a, void *stream);
+
+/* One tensor of an optimizer step: n elements, whose moments start at element `slot` (a
+ * multiple of SWARP_ADAMW_GROUP) of the flat state. */
+#define SWARP_ADAMW_GROUP 256
+typedef struct swarp_tensor {
+    void *param;
+    const void *grad;
+    int64_t n, slot;
+    int32_t param_dtype, grad_dtype; /* SWARP_F32, _BF16 or _F16; grad_dtype is param_dtype or
+                                        SWARP_F32 */
+} swarp_tensor_t;
+
+/* AdamW with decoupled weight decay, t = step >= 1, g scaled by *grad_scale where that is set:
+ *   m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2;
+ *   p = (1 - lr weight_decay) p - lr / (1 - beta1^t) m / (sqrt(v / (1 - beta2^t)) + eps).
+ * Flat state of `state_len` elements, zero before the first step.  bits = 32: exp_avg and
+ * exp_avg_sq are float.  bits = 8: they are uint8 codes with one uint8 base per group of 256:
+ * a code is the top of the float's bits -- (sign,) exponent counted from the base, three of
+ * mantissa; exponents reach 15 below the group's largest for m, 31 for v -- rounded up or down
+ * at random by the element's place and `seed` (give every step another one), so that sums of
+ * small changes are not lost.  A v above zero never becomes zero.
+ * 16-bit parameters: with `master` (float, flat like the state) p is its nearest; without it
+ * (SWARP_BF16 only) p itself is rounded at random. */
+typedef struct swarp_adamw {
+    int32_t bits;
+    uint32_t seed;
+    int64_t step, state_len;
+    double lr, beta1, beta2, eps, weight_decay;
+    void *exp_avg, *exp_avg_sq;
+    uint8_t *avg_base, *sq_base;
+    float *master;
+    const float *grad_scale;  /* [1] on the device, or NULL */
+} swarp_adamw_t;
+int swarp_adamw(const swarp_adamw_t *a, const swarp_tensor_t *tensors, int32_t n_tensors,
+                void *stream);
+/* 8-bit moments as the floats they stand for: avg and sq [state_len]. */
+int swarp_adamw_unpack(const swarp_adamw_t *a, float *avg, float *sq, void *stream);
+/* norm_scale[0]: the 2-norm of all gradients; norm_scale[1]: min(1, max_norm / (norm + 1e-6)),
+ * which swarp_adamw takes as grad_scale.  work: SWARP_NORM_WORK bytes, 16-byte aligned. */
+#define SWARP_NORM_WORK 16384
+int swarp_grad_norm(const swarp_tensor_t *tensors, int32_t n_tensors, double max_norm,
+                    float *norm_scale, void *work, void *stream);
 
 #ifdef __cplusplus
 }

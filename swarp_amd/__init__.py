@@ -6,6 +6,9 @@ bicycle / quadrotor agents) and its adjoint run as hand-written HIP kernels in
 PyTorch-facing host side with the reference's API (``Stepper``, ``TorchState``,
 ``warp_step``, ``rollout``, ``GradRing``, ``NeighborGrid``, the config classes, and the
 ``World`` / ``Environment`` / ``make("navigation", ...)`` surface that calls the step).
+
+Beside the step stand the operators a policy is trained with on it: ``gae``,
+``categorical_policy_loss``, ``gaussian_policy_loss`` and ``AdamW``.
 """
 
 from .autograd import GradRing, StepGradSlot, TorchState, fill_state_defaults, rollout, warp_step
@@ -29,11 +32,15 @@ from .config import (
 )
 from .environment import Environment, make
 from .neighbors import NeighborGrid
+from .optim import AdamW, AdamWState, adamw_state, adamw_step, grad_norm
+from .policy import Advantages, PolicyLoss, categorical_policy_loss, gae, gaussian_policy_loss
 from .scenarios import SCENARIOS, NavigationScenario, Scenario, make_scenario
 from .stepper import AgentParams, Stepper, build_agent_params
 from .world import World
 
 __all__ = [
+    "AdamW", "AdamWState", "Advantages", "PolicyLoss", "adamw_state", "adamw_step",
+    "categorical_policy_loss", "gae", "gaussian_policy_loss", "grad_norm",
     "AgentConfig", "AgentParams", "AgentShape", "ControlMode", "DynamicsModel", "Environment",
     "GradRing", "Integrator", "MODEL_ACTION_DIM", "NUM_PARAMS", "NavigationScenario",
     "NeighborGrid", "ObstacleKind", "per_env_float_template", "ObstacleShape", "Obstacles", "PARAM_FIELDS", "SCENARIOS",

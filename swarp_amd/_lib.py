@@ -13,8 +13,8 @@ from pathlib import Path
 
 import torch
 
-ABI_VERSION = 16
-F32, F64 = 0, 1
+ABI_VERSION = 17
+F32, F64, BF16, F16 = 0, 1, 2, 3
 EULER, RK4 = 0, 1
 LISTS_BRUTE, LISTS_GRID = 0, 1
 WIDE_MAX_AGENTS = 4096
@@ -115,6 +115,67 @@ class SwarpNav(ctypes.Structure):
     ]
 
 
+class SwarpGae(ctypes.Structure):
+    """Mirror of ``swarp_gae_t``."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int32), ("rows", ctypes.c_int32),
+        ("steps", ctypes.c_int64), ("columns", ctypes.c_int64), ("group", ctypes.c_int64),
+        ("gamma", ctypes.c_double), ("lam", ctypes.c_double),
+        ("rewards", ctypes.c_void_p), ("values", ctypes.c_void_p),
+        ("terminated", ctypes.c_void_p), ("truncated", ctypes.c_void_p),
+        ("final_values", ctypes.c_void_p),
+        ("advantages", ctypes.c_void_p), ("returns", ctypes.c_void_p),
+        ("adj_advantages", ctypes.c_void_p), ("adj_returns", ctypes.c_void_p),
+        ("adj_rewards", ctypes.c_void_p), ("adj_values", ctypes.c_void_p),
+        ("adj_final_values", ctypes.c_void_p),
+    ]
+
+
+class SwarpPolicy(ctypes.Structure):
+    """Mirror of ``swarp_policy_t``."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int32), ("sum", ctypes.c_int32), ("width", ctypes.c_int32),
+        ("actions32", ctypes.c_int32), ("shared_std", ctypes.c_int32),
+        ("skip_unit", ctypes.c_int32),
+        ("rows", ctypes.c_int64), ("inner", ctypes.c_int64),
+        ("outer_stride", ctypes.c_int64), ("inner_stride", ctypes.c_int64),
+        ("clip_low", ctypes.c_double), ("clip_high", ctypes.c_double),
+        ("kl_coef", ctypes.c_double), ("entropy_coef", ctypes.c_double),
+        ("head", ctypes.c_void_p), ("log_std", ctypes.c_void_p), ("actions", ctypes.c_void_p),
+        ("old_logp", ctypes.c_void_p), ("advantages", ctypes.c_void_p),
+        ("ref_logp", ctypes.c_void_p), ("mask", ctypes.c_void_p), ("logp", ctypes.c_void_p),
+        ("loss", ctypes.c_void_p), ("stats", ctypes.c_void_p), ("d_head", ctypes.c_void_p),
+        ("d_log_std", ctypes.c_void_p), ("scale", ctypes.c_void_p), ("work", ctypes.c_void_p),
+        ("work_bytes", ctypes.c_uint64),
+    ]
+
+
+class SwarpTensor(ctypes.Structure):
+    """Mirror of ``swarp_tensor_t``."""
+
+    _fields_ = [
+        ("param", ctypes.c_void_p), ("grad", ctypes.c_void_p),
+        ("n", ctypes.c_int64), ("slot", ctypes.c_int64),
+        ("param_dtype", ctypes.c_int32), ("grad_dtype", ctypes.c_int32),
+    ]
+
+
+class SwarpAdamW(ctypes.Structure):
+    """Mirror of ``swarp_adamw_t``."""
+
+    _fields_ = [
+        ("bits", ctypes.c_int32), ("seed", ctypes.c_uint32),
+        ("step", ctypes.c_int64), ("state_len", ctypes.c_int64),
+        ("lr", ctypes.c_double), ("beta1", ctypes.c_double), ("beta2", ctypes.c_double),
+        ("eps", ctypes.c_double), ("weight_decay", ctypes.c_double),
+        ("exp_avg", ctypes.c_void_p), ("exp_avg_sq", ctypes.c_void_p),
+        ("avg_base", ctypes.c_void_p), ("sq_base", ctypes.c_void_p),
+        ("master", ctypes.c_void_p), ("grad_scale", ctypes.c_void_p),
+    ]
+
+
 #: Exported entry points and their ctypes signatures.
 SIGNATURES = {
     "swarp_abi_version": ([], ctypes.c_int),
@@ -206,6 +267,24 @@ SIGNATURES = {
     "swarp_edge_index_noalloc": (
         [ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p,
          ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p],
+        ctypes.c_int,
+    ),
+    "swarp_gae_fwd": ([ctypes.POINTER(SwarpGae), ctypes.c_void_p], ctypes.c_int),
+    "swarp_gae_bwd": ([ctypes.POINTER(SwarpGae), ctypes.c_void_p], ctypes.c_int),
+    "swarp_policy_work_bytes": ([ctypes.c_int64, ctypes.c_int32], ctypes.c_uint64),
+    "swarp_categorical_loss": ([ctypes.POINTER(SwarpPolicy), ctypes.c_void_p], ctypes.c_int),
+    "swarp_gaussian_loss": ([ctypes.POINTER(SwarpPolicy), ctypes.c_void_p], ctypes.c_int),
+    "swarp_adamw": (
+        [ctypes.POINTER(SwarpAdamW), ctypes.POINTER(SwarpTensor), ctypes.c_int32, ctypes.c_void_p],
+        ctypes.c_int,
+    ),
+    "swarp_adamw_unpack": (
+        [ctypes.POINTER(SwarpAdamW), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p],
+        ctypes.c_int,
+    ),
+    "swarp_grad_norm": (
+        [ctypes.POINTER(SwarpTensor), ctypes.c_int32, ctypes.c_double, ctypes.c_void_p,
+         ctypes.c_void_p, ctypes.c_void_p],
         ctypes.c_int,
     ),
     "swarp_state_defaults": (

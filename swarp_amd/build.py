@@ -1,9 +1,9 @@
 """Build libswarp_hip.so in-tree with hipcc for gfx950.
 
 ``python -m swarp_amd.build`` (or ``__graft_entry__.build()``) compiles the units under
-``swarp_amd/csrc`` -- the host side ``swarp_hip.hip`` and one object per kernel family
-and scalar type (``k_*.hip`` with ``SWARP_T`` = float / double) -- in parallel, then links
-them into ``swarp_amd/libswarp_hip.so``.  ``--incremental`` recompiles only the objects
+``swarp_amd/csrc`` -- the host side ``swarp_hip.hip``, the radius graph, the policy update
+(``gae.hip``, ``policy.hip``, ``adamw.hip``) and one object per kernel family and scalar
+type (``k_*.hip`` with ``SWARP_T`` = float / double) -- in parallel, then links them into ``swarp_amd/libswarp_hip.so``.  ``--incremental`` recompiles only the objects
 whose sources, headers (from the compiler's dependency files) or flags changed.
 
 Floating-point flags are part of the contract with the parity tests:
@@ -41,7 +41,10 @@ DTYPES = (("f32", "float", "1"), ("f64", "double", "0"))
 def units() -> list[tuple[str, Path, list[str]]]:
     out = [("swarp_hip", CSRC / "swarp_hip.hip", []),
            ("coo", CSRC / "coo.hip", []),
-           ("coo_noalloc", CSRC / "coo_noalloc.hip", [])]
+           ("coo_noalloc", CSRC / "coo_noalloc.hip", []),
+           ("gae", CSRC / "gae.hip", []),
+           ("policy", CSRC / "policy.hip", []),
+           ("adamw", CSRC / "adamw.hip", [])]
     for fam in FAMILIES:
         for tag, ctype, is32 in DTYPES:
             out.append((f"{fam}.{tag}", CSRC / f"{fam}.hip",

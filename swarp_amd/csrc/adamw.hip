@@ -1,0 +1,383 @@
+// adamw.hip -- an AdamW step over many tensors (swarp_adamw), its 8-bit moments as floats
+// (swarp_adamw_unpack) and the norm of all gradients (swarp_grad_norm).
+//
+// The tensors of a launch travel in its arguments, up to MOST_TENSORS of them; a workgroup finds
+// its own from a running count of chunks.
+//
+// 8-bit moments.  A group of 256 elements shares a base; a code is the float's bits from the
+// third bit of the mantissa up, less the base's exponent: all integer work, the same on any
+// machine.  beta2 = 0.999 moves v by a thousandth a step, and a code's step is an eighth: rounded
+// to nearest, v would never fall and hardly rise.  Rounded up or down at random in proportion
+// (16 random bits from the element's place and the step's seed), its mean is right.
+#include <math.h>
+
+#include "learn.hpp"
+
+namespace {
+
+using namespace learn;
+
+constexpr int GROUP = SWARP_ADAMW_GROUP;
+constexpr int BLOCK = GROUP;
+constexpr int CHUNK = 16 * GROUP;        // elements of a workgroup
+constexpr int MOST_TENSORS = 64;         // of a launch
+constexpr int NORM_BLOCKS = 1024;
+
+struct Tensors {
+    void *param[MOST_TENSORS];
+    const void *grad[MOST_TENSORS];
+    int64_t n[MOST_TENSORS], slot[MOST_TENSORS];
+    uint32_t first[MOST_TENSORS];  // the tensor's first chunk
+    int count;
+};
+
+// The tensor of chunk `c`.
+__device__ __forceinline__ int tensor_of(const Tensors &t, uint32_t c)
+{
+    int lo = 0, hi = t.count;
+    while (hi - lo > 1) {
+        const int m = (lo + hi) / 2;
+        if (t.first[m] <= c) lo = m;
+        else hi = m;
+    }
+    return lo;
+}
+
+struct Step {
+    float b1, a1, b2, a2;     // beta1, 1 - beta1, beta2, 1 - beta2
+    float lr_t, v_t, eps, keep;  // lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t), eps, 1 - lr wd
+    uint32_t seed;
+    void *m, *v;
+    uint8_t *m_base, *v_base;
+    float *master;
+    const float *scale;
+};
+
+// One round of multiply and shift; the multipliers here and below are the odd integers at 2^32
+// times the fractional parts of sqrt(3), sqrt(7), the golden ratio and sqrt(5).
+__device__ __forceinline__ uint32_t mix(uint32_t x)
+{
+    x *= 0xBB67AE85u;
+    x ^= x >> 15;
+    x *= 0xA54FF53Bu;
+    return x ^ (x >> 16);
+}
+// 32 random bits of element i of the flat state.
+__device__ __forceinline__ uint32_t random_of(uint64_t i, uint32_t seed)
+{
+    return mix((uint32_t)i * 0x9E3779B1u + seed + (uint32_t)(i >> 32) * 0x3C6EF373u);
+}
+
+__device__ __forceinline__ uint32_t bits_of(float x) { return (uint32_t)__float_as_int(x); }
+__device__ __forceinline__ float float_of(uint32_t b) { return __int_as_float((int)b); }
+
+// The base of a group whose largest magnitude has the bits `most`: the exponent `reach` below
+// that of the magnitude rounded up to a code.
+__device__ __forceinline__ uint32_t base_of(uint32_t most, uint32_t reach)
+{
+    const uint32_t e = (most + 0xfffffu) >> 23;
+    return e > reach ? e - reach : 0;
+}
+__device__ __forceinline__ uint32_t magnitude(float x)
+{
+    const uint32_t m = bits_of(x) & 0x7fffffffu;
+    return m < 0x7ff00000u ? m : 0x7ff00000u;
+}
+__device__ __forceinline__ uint32_t encode(uint32_t mag, uint32_t base, uint32_t r16)
+{
+    const uint32_t k = (mag + (r16 << 4 | 8u)) >> 20, low = base << 3;
+    return k > low ? k - low : 0;
+}
+__device__ __forceinline__ float decode(uint32_t q, uint32_t base)
+{
+    return q ? float_of((q + (base << 3)) << 20) : 0.0f;
+}
+__device__ __forceinline__ float decode_m(uint32_t c, uint32_t base)
+{
+    const float x = decode(c & 127u, base);
+    return float_of(bits_of(x) | (c & 128u) << 24);
+}
+
+__device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t *red)
+{
+    v = wave_max(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    for (int w = 0; w < BLOCK / 64; ++w) v = red[w] > v ? red[w] : v;
+    return v;
+}
+
+__device__ __forceinline__ void put(float *p, float x, uint32_t) { *p = x; }
+__device__ __forceinline__ void put(f16 *p, float x, uint32_t) { *p = (f16)x; }
+// bfloat16 without a master: at random, in proportion; infinities and NaN are cut
+__device__ __forceinline__ void put(bf16 *p, float x, uint32_t r)
+{
+    const uint32_t b = bits_of(x);
+    const bool finite = (b & 0x7f800000u) != 0x7f800000u;
+    *p = finite ? __builtin_bit_cast(bf16, (uint16_t)((b + (mix(r) & 0xffffu)) >> 16)) : (bf16)x;
+}
+
+// A workgroup takes a chunk of a tensor, a thread an element of each of its groups.
+template <typename P, typename G, int BITS>
+__global__ __launch_bounds__(BLOCK) void k_adamw(const Step s, const Tensors t)
+{
+    __shared__ uint32_t red[2][BLOCK / 64];
+    const int k = tensor_of(t, blockIdx.x);
+    P *const param = (P *)t.param[k];
+    const G *const grad = (const G *)t.grad[k];
+    const int64_t n = t.n[k], slot = t.slot[k];
+    const int64_t begin = (int64_t)(blockIdx.x - t.first[k]) * CHUNK;
+    const float scale = s.scale ? *s.scale : 1.0f;
+    for (int64_t i0 = begin; i0 < begin + CHUNK && i0 < n; i0 += GROUP) {
+        const int64_t i = i0 + threadIdx.x, j = slot + i, q = (slot + i0) / GROUP;
+        const bool in = i < n;
+        float g = in ? (float)grad[i] : 0.0f, m = 0, v = 0, w = 0;
+        if (BITS == 8) {
+            m = decode_m(((const uint8_t *)s.m)[j], s.m_base[q]);
+            v = decode(((const uint8_t *)s.v)[j], s.v_base[q]);
+        } else if (in) {
+            m = ((const float *)s.m)[j];
+            v = ((const float *)s.v)[j];
+        }
+        if (in) w = s.master ? s.master[j] : (float)param[i];
+        if (s.scale) g = g * scale;
+        m = m * s.b1 + g * s.a1;
+        v = v * s.b2 + g * g * s.a2;
+        w = w * s.keep - s.lr_t * (m / (sqrtf(v) * s.v_t + s.eps));
+        const uint32_t r = random_of((uint64_t)j, s.seed);
+        if (BITS == 8) {
+            const uint32_t mm = in ? magnitude(m) : 0, vm = in ? magnitude(v) : 0;
+            const uint32_t mb = base_of(block_max(mm, red[0]), 15), vb = base_of(block_max(vm, red[1]), 31);
+            uint32_t mc = encode(mm, mb, r >> 16), vc = encode(vm, vb, r & 0xffffu);
+            vc = vc == 0 && vm > 0 ? 1 : vc;
+            ((uint8_t *)s.m)[j] = (uint8_t)(in ? mc | (bits_of(m) >> 24 & 128u) : 0);
+            ((uint8_t *)s.v)[j] = (uint8_t)(in ? vc : 0);
+            if (threadIdx.x == 0) {
+                s.m_base[q] = (uint8_t)mb;
+                s.v_base[q] = (uint8_t)vb;
+            }
+        } else if (in) {
+            ((float *)s.m)[j] = m;
+            ((float *)s.v)[j] = v;
+        }
+        if (!in) continue;
+        if (s.master) {
+            s.master[j] = w;
+            param[i] = (P)w;
+        } else {
+            put(param + i, w, r);
+        }
+    }
+}
+
+__global__ __launch_bounds__(BLOCK) void k_unpack(int64_t groups, const uint8_t *m, const uint8_t *v,
+                                                  const uint8_t *m_base, const uint8_t *v_base,
+                                                  float *avg, float *sq)
+{
+    for (int64_t q = blockIdx.x; q < groups; q += gridDim.x) {
+        const int64_t j = q * GROUP + threadIdx.x;
+        avg[j] = decode_m(m[j], m_base[q]);
+        sq[j] = decode(v[j], v_base[q]);
+    }
+}
+
+template <typename G>
+__global__ __launch_bounds__(BLOCK) void k_norm(const Tensors t, uint32_t chunks, double *sums, int set)
+{
+    __shared__ double red[BLOCK / 64];
+    double s = 0;
+    for (uint32_t c = blockIdx.x; c < chunks; c += gridDim.x) {
+        const int k = tensor_of(t, c);
+        const G *const grad = (const G *)t.grad[k];
+        const int64_t begin = (int64_t)(c - t.first[k]) * CHUNK;
+        const int64_t end = begin + CHUNK < t.n[k] ? begin + CHUNK : t.n[k];
+        float part = 0;
+        for (int64_t i = begin + threadIdx.x; i < end; i += BLOCK) {
+            const float g = (float)grad[i];
+            part += g * g;
+        }
+        s += part;
+    }
+    s = wave_sum(s);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < BLOCK / 64; ++w) s += red[w];
+        sums[blockIdx.x] = (int)blockIdx.x < set ? sums[blockIdx.x] + s : s;
+    }
+}
+
+__global__ __launch_bounds__(BLOCK) void k_norm_finish(int blocks, const double *sums, float most, float *out)
+{
+    __shared__ double red[BLOCK / 64];
+    double s = 0;
+    for (int b = threadIdx.x; b < blocks; b += BLOCK) s += sums[b];
+    s = wave_sum(s);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < BLOCK / 64; ++w) s += red[w];
+        const float norm = (float)sqrt(s);
+        const float c = most / (norm + 1e-6f);
+        out[0] = norm;
+        out[1] = c > 1.0f ? 1.0f : c;
+    }
+}
+
+// ------------------------------------------------------------------------------ host side
+
+int check(const swarp_adamw_t *a)
+{
+    if (!a) return fail("arguments must be set");
+    if (a->bits != 32 && a->bits != 8) return fail("bits must be 32 or 8");
+    if (a->state_len < 0 || a->state_len % GROUP) return fail("state_len must be a multiple of 256");
+    if (a->state_len && (!a->exp_avg || !a->exp_avg_sq)) return fail("the moments must be set");
+    if (((uintptr_t)a->exp_avg | (uintptr_t)a->exp_avg_sq | (uintptr_t)a->master) & 15u)
+        return fail("the state must be 16-byte aligned");
+    if (a->bits == 8 && a->state_len && (!a->avg_base || !a->sq_base))
+        return fail("8-bit moments need their bases");
+    return 0;
+}
+
+int check(const swarp_tensor_t *t, int n)
+{
+    if (n < 0 || (n && !t)) return fail("tensors must be set");
+    for (int k = 0; k < n; ++k) {
+        if (t[k].n < 0 || t[k].n > (int64_t)CHUNK << 30) return fail("a tensor's size is out of range");
+        if (t[k].n && !t[k].grad) return fail("a tensor has no gradient");
+        const int d = t[k].grad_dtype;
+        if (d != SWARP_F32 && d != SWARP_BF16 && d != SWARP_F16)
+            return fail("gradients are float32, bfloat16 or float16");
+    }
+    return 0;
+}
+
+// Fills the table with the tensors from `k` on that `take` accepts, as many as it holds;
+// returns where to go on.
+template <typename Take>
+int fill(Tensors &t, uint32_t &chunks, const swarp_tensor_t *x, int n, int k, Take take)
+{
+    t.count = 0;
+    chunks = 0;
+    for (; k < n && t.count < MOST_TENSORS; ++k) {
+        if (x[k].n == 0 || !take(x[k])) continue;
+        const uint64_t c = (uint64_t)((x[k].n + CHUNK - 1) / CHUNK);
+        if (chunks + c > 0x7fffffffu) break;
+        t.param[t.count] = x[k].param;
+        t.grad[t.count] = x[k].grad;
+        t.n[t.count] = x[k].n;
+        t.slot[t.count] = x[k].slot;
+        t.first[t.count] = chunks;
+        chunks += (uint32_t)c;
+        ++t.count;
+    }
+    return k;
+}
+
+template <typename P, typename G>
+void steps(const Step &s, int bits, const swarp_tensor_t *x, int n, int pd, int gd, hipStream_t st)
+{
+    Tensors t;
+    uint32_t chunks;
+    for (int k = 0; k < n;) {
+        k = fill(t, chunks, x, n, k, [&](const swarp_tensor_t &y) { return y.param_dtype == pd && y.grad_dtype == gd; });
+        if (!t.count) continue;
+        if (bits == 8)
+            hipLaunchKernelGGL((k_adamw<P, G, 8>), dim3(chunks), dim3(BLOCK), 0, st, s, t);
+        else
+            hipLaunchKernelGGL((k_adamw<P, G, 32>), dim3(chunks), dim3(BLOCK), 0, st, s, t);
+    }
+}
+
+}  // namespace
+
+extern "C" {
+
+int swarp_adamw(const swarp_adamw_t *a, const swarp_tensor_t *tensors, int32_t n_tensors, void *stream)
+{
+    swarp::set_error("");
+    if (check(a) || check(tensors, n_tensors)) return -1;
+    if (a->step < 1) return fail("step must be >= 1");
+    for (int k = 0; k < n_tensors; ++k) {
+        const swarp_tensor_t &x = tensors[k];
+        if (x.n == 0) continue;
+        if (!x.param) return fail("a tensor has no parameter");
+        if (x.param_dtype != SWARP_F32 && x.param_dtype != SWARP_BF16 && x.param_dtype != SWARP_F16)
+            return fail("parameters are float32, bfloat16 or float16");
+        if (x.grad_dtype != x.param_dtype && x.grad_dtype != SWARP_F32)
+            return fail("a gradient has its parameter's type, or float32");
+        if (x.param_dtype == SWARP_F16 && !a->master) return fail("float16 parameters need a master copy");
+        if (x.slot < 0 || x.slot % GROUP || x.slot > a->state_len || (x.n + GROUP - 1) / GROUP > (a->state_len - x.slot) / GROUP)
+            return fail("a tensor's slot is outside the state");
+    }
+    Step s;
+    const double c1 = 1.0 - pow(a->beta1, (double)a->step), c2 = 1.0 - pow(a->beta2, (double)a->step);
+    s.b1 = (float)a->beta1;
+    s.a1 = (float)(1.0 - a->beta1);
+    s.b2 = (float)a->beta2;
+    s.a2 = (float)(1.0 - a->beta2);
+    s.lr_t = (float)(a->lr / c1);
+    s.v_t = (float)(1.0 / sqrt(c2));
+    s.eps = (float)a->eps;
+    s.keep = (float)(1.0 - a->lr * a->weight_decay);
+    s.seed = a->seed;
+    s.m = a->exp_avg;
+    s.v = a->exp_avg_sq;
+    s.m_base = a->avg_base;
+    s.v_base = a->sq_base;
+    s.master = a->master;
+    s.scale = a->grad_scale;
+    hipStream_t st = (hipStream_t)stream;
+    const int b = a->bits, n = n_tensors;
+    steps<float, float>(s, b, tensors, n, SWARP_F32, SWARP_F32, st);
+    steps<bf16, bf16>(s, b, tensors, n, SWARP_BF16, SWARP_BF16, st);
+    steps<bf16, float>(s, b, tensors, n, SWARP_BF16, SWARP_F32, st);
+    steps<f16, f16>(s, b, tensors, n, SWARP_F16, SWARP_F16, st);
+    steps<f16, float>(s, b, tensors, n, SWARP_F16, SWARP_F32, st);
+    return launched();
+}
+
+int swarp_adamw_unpack(const swarp_adamw_t *a, float *avg, float *sq, void *stream)
+{
+    swarp::set_error("");
+    if (check(a)) return -1;
+    if (a->bits != 8) return fail("only 8-bit moments are unpacked");
+    if (a->state_len == 0) return 0;
+    if (!avg || !sq) return fail("pointer arguments must be set");
+    const int64_t groups = a->state_len / GROUP;
+    hipLaunchKernelGGL(k_unpack, dim3((unsigned)(groups < 16384 ? groups : 16384)), dim3(BLOCK), 0,
+                       (hipStream_t)stream, groups, (const uint8_t *)a->exp_avg,
+                       (const uint8_t *)a->exp_avg_sq, (const uint8_t *)a->avg_base,
+                       (const uint8_t *)a->sq_base, avg, sq);
+    return launched();
+}
+
+int swarp_grad_norm(const swarp_tensor_t *tensors, int32_t n_tensors, double max_norm,
+                    float *norm_scale, void *work, void *stream)
+{
+    swarp::set_error("");
+    if (check(tensors, n_tensors)) return -1;
+    if (!norm_scale || !work || (uintptr_t)work & 15u) return fail("norm_scale and aligned work must be set");
+    hipStream_t st = (hipStream_t)stream;
+    double *const sums = (double *)work;
+    Tensors t;
+    uint32_t chunks;
+    int blocks = 0;  // sums set so far: a launch adds to those and sets the others of its grid
+    for (int d : {SWARP_F32, SWARP_BF16, SWARP_F16})
+        for (int k = 0; k < n_tensors;) {
+            k = fill(t, chunks, tensors, n_tensors, k, [&](const swarp_tensor_t &y) { return y.grad_dtype == d; });
+            if (!t.count) continue;
+            const int grid = (int)(chunks < NORM_BLOCKS ? chunks : NORM_BLOCKS);
+            const dim3 g(grid), b(BLOCK);
+            if (d == SWARP_F32) hipLaunchKernelGGL((k_norm<float>), g, b, 0, st, t, chunks, sums, blocks);
+            else if (d == SWARP_BF16) hipLaunchKernelGGL((k_norm<bf16>), g, b, 0, st, t, chunks, sums, blocks);
+            else hipLaunchKernelGGL((k_norm<f16>), g, b, 0, st, t, chunks, sums, blocks);
+            blocks = grid > blocks ? grid : blocks;
+        }
+    hipLaunchKernelGGL(k_norm_finish, dim3(1), dim3(BLOCK), 0, st, blocks, (const double *)sums,
+                       (float)max_norm, norm_scale);
+    return launched();
+}
+
+}  // extern "C"
