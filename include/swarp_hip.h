@@ -453,7 +453,8 @@ typedef struct swarp_policy {
     int32_t width;            /* actions of a categorical head, dimensions of a Gaussian one */
     int32_t actions32;        /* categorical: actions are int32 (0: int64) */
     int32_t shared_std;
-    int32_t skip_unit;        /* 1: nothing is written where *scale is 1 (see swarp_policy_*) */
+    int32_t skip_unit;        /* 1: nothing is written where *scale is 1 (see below) */
+    int32_t counted;          /* 1: work holds the mask's counts from an earlier call */
     int64_t rows;
     int64_t inner, outer_stride, inner_stride;
     double clip_low, clip_high, kl_coef, entropy_coef;
@@ -473,9 +474,9 @@ typedef struct swarp_policy {
     void *work;               /* swarp_policy_work_bytes(rows, width) bytes, 16-byte aligned */
     uint64_t work_bytes;
 } swarp_policy_t;
-/* A forward with the gradient writes logp, stats and the gradients for an upstream gradient of
- * 1.  The backward is the same call with logp, loss and stats NULL, scale the upstream gradient and
- * skip_unit = 1 into the same buffers: where the upstream gradient is 1 they are right as they
+/* A forward with the gradient writes logp, loss, stats and the gradients for an upstream
+ * gradient of 1.  The backward is the same call on the same work with logp, loss and stats NULL,
+ * counted = 1, scale the upstream gradient and skip_unit = 1 into the same buffers: where the upstream gradient is 1 they are right as they
  * stand, else they are computed again with it.  Which it is, the device decides. */
 uint64_t swarp_policy_work_bytes(int64_t rows, int32_t width);
 int swarp_categorical_loss(const swarp_policy_t *a, void *stream);

@@ -138,7 +138,7 @@ class SwarpPolicy(ctypes.Structure):
     _fields_ = [
         ("dtype", ctypes.c_int32), ("sum", ctypes.c_int32), ("width", ctypes.c_int32),
         ("actions32", ctypes.c_int32), ("shared_std", ctypes.c_int32),
-        ("skip_unit", ctypes.c_int32),
+        ("skip_unit", ctypes.c_int32), ("counted", ctypes.c_int32),
         ("rows", ctypes.c_int64), ("inner", ctypes.c_int64),
         ("outer_stride", ctypes.c_int64), ("inner_stride", ctypes.c_int64),
         ("clip_low", ctypes.c_double), ("clip_high", ctypes.c_double),

@@ -18,6 +18,7 @@ constexpr int BLOCK = 256;
 constexpr int MOST_BLOCKS = 2048;   // of a loss kernel: each leaves one row of sums
 constexpr int COUNTERS = 256;       // blocks that count the mask
 constexpr int MOST_DIMS = 64;       // of a Gaussian head
+constexpr int FEW_ROWS = 256;       // fewer rows than compute units: long ones are split
 constexpr double HALF_LOG_2PI = 0.91893853320467274178;
 
 template <typename A> struct Row {  // what every decision has, and the loss's constants
@@ -33,49 +34,67 @@ template <typename A> struct Row {  // what every decision has, and the loss's c
     const A *scale;
 };
 
-// Weight of a counted decision in the gradient: the same in every thread of the block.
-template <typename A> __device__ A weight_of(const Row<A> &r)
+// Decisions that count, at least 1: the same in every thread of the block.
+template <typename A> __device__ double counted(const Row<A> &r)
 {
-    if (r.sum) return A(1);
-    if (!r.mask) return A(1) / (A)r.rows;
+    if (!r.mask) return r.rows > 1 ? (double)r.rows : 1.0;
     __shared__ double count;
     if (threadIdx.x < 64) {
-        double c = 0;
+        int64_t c = 0;
         for (int i = threadIdx.x; i < r.n_counts; i += 64) c += r.counts[i];
         c = wave_sum(c);
-        if (threadIdx.x == 0) count = c;
+        if (threadIdx.x == 0) count = c > 1 ? (double)c : 1.0;
     }
     __syncthreads();
-    return A(1) / (A)(count > 1 ? count : 1);
+    return count;
 }
+// Weight of a decision in the gradient.
+template <typename A> __device__ A weight_of(const Row<A> &r) { return r.sum ? A(1) : (A)(1.0 / counted(r)); }
 
 template <typename A> struct Terms {
     A loss, ent, kl, clipped;
 };
 
-__device__ __forceinline__ float exp_of(float x) { return expf(x); }
+// exp and log of the accumulation types.  float: the hardware's base-2 functions, whose error is
+// an ulp of the result; arguments are differences of a few units, which the product with log2(e)
+// rounds by half an ulp more.
+constexpr float LOG2E = 1.44269504088896340736f;
+constexpr double LN_2 = 0.69314718055994530942;
+__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * LOG2E); }
 __device__ __forceinline__ double exp_of(double x) { return exp(x); }
-__device__ __forceinline__ float expm1_of(float x) { return expm1f(x); }
-__device__ __forceinline__ double expm1_of(double x) { return expm1(x); }
-__device__ __forceinline__ float log_of(float x) { return logf(x); }
-__device__ __forceinline__ double log_of(double x) { return log(x); }
 
-// One decision's terms added to `t`; returns g.
-template <typename A>
-__device__ __forceinline__ A decide(const Row<A> &r, int64_t i, A lp, A H, Terms<A> &t)
+// expm1(e) - e, without the cancellation of small e (the series to e^9 / 9! below 1/2).
+template <typename A> __device__ __forceinline__ A kl_of(A e)
+{
+    A s = A(1) / A(362880);
+    s = s * e + A(1) / A(40320);
+    s = s * e + A(1) / A(5040);
+    s = s * e + A(1) / A(720);
+    s = s * e + A(1) / A(120);
+    s = s * e + A(1) / A(24);
+    s = s * e + A(1) / A(6);
+    s = s * e + A(0.5);
+    const bool small = sizeof(A) == 4 && e < A(0.5) && e > A(-0.5);
+    return small ? s * e * e : (sizeof(A) == 4 ? exp_of(e) - A(1) - e : (A)(expm1((double)e) - (double)e));
+}
+
+// One decision's terms added to `t`; returns g.  lp may be wider than A: its differences to the
+// old and the reference log-probability are then rounded once.
+template <typename A, typename L>
+__device__ __forceinline__ A decide(const Row<A> &r, int64_t i, L lp, A H, Terms<A> &t)
 {
     const A old = r.old[i], adv = r.adv[i];
-    const A rho = exp_of(lp - old);
+    const A rho = exp_of((A)(lp - (L)old));
     const A bounded = rho < r.lo ? r.lo : (rho > r.hi ? r.hi : rho);
     const A first = rho * adv, second = bounded * adv;
     const bool clipped = second < first;
-    const A e = (r.ref ? r.ref[i] : old) - lp;
-    const A em = expm1_of(e), kl = em - e;
+    const A e = (A)((L)(r.ref ? r.ref[i] : old) - lp);
+    const A kl = kl_of(e);
     A l = clipped ? -second : -first;
     A g = clipped ? A(0) : -first;
     if (r.klc != A(0)) {
         l += r.klc * kl;
-        g -= r.klc * em;
+        g -= r.klc * (kl + e);
     }
     if (r.entc != A(0)) l -= r.entc * H;
     t.loss += l;
@@ -86,9 +105,9 @@ __device__ __forceinline__ A decide(const Row<A> &r, int64_t i, A lp, A H, Terms
 }
 
 // The block's sums of its threads' terms to row blockIdx.x of `sums`.
-template <typename A> __device__ void leave_sums(const Terms<A> &t, double *sums)
+template <int THREADS, typename A> __device__ void leave_sums(const Terms<A> &t, double *sums)
 {
-    __shared__ double red[BLOCK / 64][4];
+    __shared__ double red[THREADS / 64][4];
     const double v[4] = {(double)t.loss, (double)t.ent, (double)t.kl, (double)t.clipped};
     for (int k = 0; k < 4; ++k) {
         const double s = wave_sum(v[k]);
@@ -97,7 +116,7 @@ template <typename A> __device__ void leave_sums(const Terms<A> &t, double *sums
     __syncthreads();
     if (threadIdx.x < 4) {
         double s = 0;
-        for (int w = 0; w < BLOCK / 64; ++w) s += red[w][threadIdx.x];
+        for (int w = 0; w < THREADS / 64; ++w) s += red[w][threadIdx.x];
         sums[4 * (int64_t)blockIdx.x + threadIdx.x] = s;
     }
 }
@@ -117,75 +136,643 @@ __global__ __launch_bounds__(BLOCK) void k_count(int64_t rows, const uint8_t *ma
     }
 }
 
+// ------------------------------------------------------------------------ categorical head
+//
+// A row of logits is read once, held in registers as it came (of its own type) while its maximum,
+// its sums and its gradient are formed, and the gradient is written once.  Work is in base 2: with
+// m the maximum, z = (x - m) log2(e), s = sum 2^z, q = sum 2^z z:
+//   log2 p = z - log2 s;  H = (log2 s - q / s) ln 2;  dl/dx = 2^z (c1 z + c2) + g [j = a],
+//   c1 = entropy_coef ln 2 / s,  c2 = (entropy_coef (H - ln s) - g) / s.
+// The difference comes first: logits at the type's lowest value neither overflow nor differ from
+// each other.  z is held above a number that 2^z makes 0, in the products alone: 0 times -inf is
+// no NaN, and a NaN logit still is one through 2^z.
+
 struct Logits {
     int64_t inner, outer_stride, inner_stride;
-    int width, actions32;
+    int width, actions32, flat;
+    int splits, part;    // of a row that goes to several workgroups: parts, elements of one
     const void *x, *actions;
     void *d;
+    void *parts;         // [rows][splits][3]: max, sum, q of a part
 };
 
-template <typename T>
-__global__ __launch_bounds__(BLOCK) void k_categorical(const Row<typename Acc<T>::type> r, const Logits g)
+// VEC neighbouring elements, 16 bytes; rows start at any element.
+template <typename T, int N> struct __attribute__((packed, aligned(sizeof(T)))) Span {
+    T e[N];
+};
+
+// The same where they lie on 16 bytes (in LDS).
+template <typename T, int N> struct __align__(16) Line {
+    Span<T, N> s;
+};
+
+template <typename A> struct Base2;
+template <> struct Base2<float> {
+    static __device__ __forceinline__ float z(float x, float m) { return (x - m) * LOG2E; }
+    static __device__ __forceinline__ float exp(float z) { return __builtin_amdgcn_exp2f(z); }
+    static __device__ __forceinline__ float log(float s) { return __builtin_amdgcn_logf(s); }
+    static __device__ __forceinline__ float floor(float z) { return fmaxf(z, -2000.0f); }
+};
+template <> struct Base2<double> {
+    static constexpr double L = 1.44269504088896340736;
+    static __device__ __forceinline__ double z(double x, double m) { return (x - m) * L; }
+    static __device__ __forceinline__ double exp(double z) { return exp2(z); }
+    static __device__ __forceinline__ double log(double s) { return log2(s); }
+    static __device__ __forceinline__ double floor(double z) { return fmax(z, -2000.0); }
+};
+
+__device__ __forceinline__ int64_t start_of(const Logits &g, int64_t i)
+{
+    if (g.flat) return i * g.inner_stride;
+    const uint64_t o = (uint64_t)i / (uint64_t)g.inner;
+    return (int64_t)o * g.outer_stride + (i - (int64_t)o * g.inner) * g.inner_stride;
+}
+__device__ __forceinline__ int64_t action_of(const Logits &g, int64_t i)
+{
+    return g.actions32 ? (int64_t)((const int32_t *)g.actions)[i] : ((const int64_t *)g.actions)[i];
+}
+
+// What the gradient of a row needs.
+template <typename A> struct Slope {
+    A m, c1, c2, gw;
+    int64_t at;
+};
+
+// The row's terms from its sums; `lp` is its log-probability.
+template <typename A>
+__device__ __forceinline__ Slope<A> slope_of(const Row<A> &r, const Logits &g, int64_t i, A m, A s, A q,
+                                             A xa, int64_t at, A w, Terms<A> &t, A &lp)
+{
+    typedef Base2<A> B;
+    const bool in = at >= 0 && at < g.width;
+    const A ls = B::log(s), inv = A(1) / s;
+    const A H = (ls - q * inv) * A(LN_2);
+    lp = in ? (xa - m) - ls * A(LN_2) : A(NAN);
+    const A gw = decide(r, i, lp, in ? H : A(NAN), t) * w;
+    const A ew = r.entc * w;
+    return {m, ew * A(LN_2) * inv, (ew * (H - ls * A(LN_2)) - gw) * inv, in ? gw : A(NAN), in ? at : -1};
+}
+
+template <typename A> __device__ __forceinline__ A max_of(A a, A b) { return a > b ? a : b; }
+__device__ __forceinline__ float fma_of(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
+__device__ __forceinline__ double fma_of(double a, double b, double c) { return __builtin_fma(a, b, c); }
+
+// Elements of a 32-bit word (two words, for double) and back.
+template <typename T> struct Words;
+template <> struct Words<float> {
+    static constexpr uint32_t LOW = 0xff800000u, LOW_HI = LOW;  // -inf
+    static __device__ __forceinline__ float get(const uint32_t (&w)[4], int k) { return __int_as_float((int)w[k]); }
+    static __device__ __forceinline__ void set(uint32_t (&w)[4], const float (&y)[4])
+    {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] = (uint32_t)__float_as_int(y[k]);
+    }
+};
+template <> struct Words<double> {
+    static constexpr uint32_t LOW = 0, LOW_HI = 0xfff00000u;
+    static __device__ __forceinline__ double get(const uint32_t (&w)[4], int k)
+    {
+        return __longlong_as_double((long long)((uint64_t)w[2 * k + 1] << 32 | w[2 * k]));
+    }
+    static __device__ __forceinline__ void set(uint32_t (&w)[4], const double (&y)[2])
+    {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const uint64_t b = (uint64_t)__double_as_longlong(y[k]);
+            w[2 * k] = (uint32_t)b;
+            w[2 * k + 1] = (uint32_t)(b >> 32);
+        }
+    }
+};
+template <> struct Words<bf16> {
+    static constexpr uint32_t LOW = 0xff80ff80u, LOW_HI = LOW;
+    static __device__ __forceinline__ float get(const uint32_t (&w)[4], int k)
+    {
+        return __int_as_float((int)(k & 1 ? w[k / 2] & 0xffff0000u : w[k / 2] << 16));
+    }
+    static __device__ __forceinline__ void set(uint32_t (&w)[4], const float (&y)[8])
+    {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] = __builtin_bit_cast(uint32_t, Span<bf16, 2>{{(bf16)y[2 * k], (bf16)y[2 * k + 1]}});
+    }
+};
+template <> struct Words<f16> {
+    static constexpr uint32_t LOW = 0xfc00fc00u, LOW_HI = LOW;
+    static __device__ __forceinline__ float get(const uint32_t (&w)[4], int k)
+    {
+        return (float)__builtin_bit_cast(f16, (uint16_t)(w[k / 2] >> 16 * (k & 1)));
+    }
+    static __device__ __forceinline__ void set(uint32_t (&w)[4], const float (&y)[8])
+    {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] = __builtin_bit_cast(uint32_t, Span<f16, 2>{{(f16)y[2 * k], (f16)y[2 * k + 1]}});
+    }
+};
+
+// LANES threads hold a row of at most LANES * E elements, E a multiple of VEC: thread `lane` the
+// spans lane, lane + LANES, ..., as the words they came in (as elements they would take a register
+// each).  The last, short span is read and written in pieces; its length is the same for every
+// row, so only scalar branches choose them.
+template <typename T, int LANES, int E> struct Held {
+    typedef typename Acc<T>::type A;
+    typedef Base2<A> B;
+    static constexpr int VEC = 16 / sizeof(T), NV = E / VEC;
+    struct Raw {
+        uint32_t w[4];
+    };
+    uint32_t v[NV][4];
+
+    __device__ __forceinline__ void fill(uint32_t lo, uint32_t hi)
+    {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            v[i][0] = v[i][2] = lo;
+            v[i][1] = v[i][3] = hi;
+        }
+    }
+    __device__ __forceinline__ void take(int i, const Raw &y)
+    {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[i][k] = y.w[k];
+    }
+    __device__ __forceinline__ Raw give(int i) const { return Raw{{v[i][0], v[i][1], v[i][2], v[i][3]}}; }
+
+    template <int N> static __device__ __forceinline__ Raw piece(const T *x)
+    {
+        Span<T, VEC> d;
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) d.e[k] = (T)(-INFINITY);
+        const Span<T, N> y = *(const Span<T, N> *)x;
+#pragma unroll
+        for (int k = 0; k < N; ++k) d.e[k] = y.e[k];
+        return __builtin_bit_cast(Raw, d);
+    }
+    template <int N> __device__ __forceinline__ void piece_out(int i, T *x) const
+    {
+        const Span<T, VEC> s = __builtin_bit_cast(Span<T, VEC>, give(i));
+        Span<T, N> y;
+#pragma unroll
+        for (int k = 0; k < N; ++k) y.e[k] = s.e[k];
+        *(Span<T, N> *)x = y;
+    }
+
+    // width >= VEC: a thread without a span of its own reads the row's first, so that every load is
+    // in flight at once and into its own registers.
+    __device__ __forceinline__ void load(const T *x, int width, int lane)
+    {
+        // (the offsets are formed here, row by row, and not kept in registers from row to row)
+        if constexpr (E > 16) asm volatile("" : "+v"(lane));
+        const int full = width / VEC, rem = width % VEC;
+        Raw last = {{Words<T>::LOW, Words<T>::LOW_HI, Words<T>::LOW, Words<T>::LOW_HI}};
+        if (rem && lane == full % LANES) {
+            const T *const y = x + full * VEC;
+            switch (rem) {
+            case 1: last = piece<1>(y); break;
+            case 2: if constexpr (VEC > 2) last = piece<2>(y); break;
+            case 3: if constexpr (VEC > 2) last = piece<3>(y); break;
+            case 4: if constexpr (VEC > 4) last = piece<4>(y); break;
+            case 5: if constexpr (VEC > 4) last = piece<5>(y); break;
+            case 6: if constexpr (VEC > 4) last = piece<6>(y); break;
+            default: if constexpr (VEC > 4) last = piece<7>(y); break;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const uint32_t at = lane < full - i * LANES ? (uint32_t)(i * LANES + lane) * VEC : 0u;
+            take(i, __builtin_bit_cast(Raw, *(const Span<T, VEC> *)(x + at)));
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int left = full - i * LANES;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t low = k & 1 ? Words<T>::LOW_HI : Words<T>::LOW;
+                v[i][k] = lane < left ? v[i][k] : (lane == left ? last.w[k] : low);
+            }
+        }
+    }
+    __device__ __forceinline__ A most() const
+    {
+        A m = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) {
+                m = max_of(Words<T>::get(v[i], k), m);  // (passes a NaN over: the sums hold it)
+            }
+            in_turn();
+        }
+        return m;
+    }
+    __device__ __forceinline__ void sums(A m, A &s, A &q)
+    {
+        forget();
+        s = q = 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) {
+                const A z = B::z(Words<T>::get(v[i], k), m), e = B::exp(z);
+                s += e;
+                q = fma_of(e, B::floor(z), q);
+            }
+            in_turn();
+        }
+    }
+    // Up to 16 elements a thread the compiler keeps what it has of a logit from one use to the next
+    // (as a float, z, 2^z).  More would not fit the registers: there each use starts from the
+    // words as they were loaded, which the compiler is not to see through, one span after the
+    // other.
+    __device__ __forceinline__ void forget()
+    {
+        if constexpr (E > 16) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) asm volatile("" : "+v"(v[i][0]), "+v"(v[i][1]), "+v"(v[i][2]), "+v"(v[i][3]));
+        }
+    }
+    static __device__ __forceinline__ void in_turn()
+    {
+        if constexpr (E > 16) __builtin_amdgcn_sched_barrier(0);
+    }
+    // The gradient row to d.
+    __device__ __forceinline__ void slope(const Slope<A> &c, T *d, int width, int lane)
+    {
+        const int full = width / VEC, rem = width % VEC;
+        forget();
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            A y[VEC];
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) {
+                const A z = B::z(Words<T>::get(v[i], k), c.m);
+                y[k] = B::exp(z) * fma_of(c.c1, B::floor(z), c.c2);
+            }
+            if (c.at >= 0 && (int)c.at / VEC - i * LANES == lane) {
+                const int at = (int)c.at % VEC;
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) y[k] += k == at ? c.gw : A(0);
+            }
+            if (c.at < 0) {
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) y[k] = c.gw;
+            }
+            Words<T>::set(v[i], y);
+            put(d, lane, i, full, rem);
+            in_turn();
+        }
+    }
+    __device__ __forceinline__ void zero(T *d, int width, int lane)
+    {
+        const int full = width / VEC, rem = width % VEC;
+        fill(0, 0);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) put(d, lane, i, full, rem);
+    }
+    __device__ __forceinline__ void put(T *d, int lane, int i, int full, int rem) const
+    {
+        T *const y = d + i * LANES * VEC + (uint32_t)(lane * VEC);
+        const int left = full - i * LANES;
+        if (lane < left) *(Span<T, VEC> *)y = __builtin_bit_cast(Span<T, VEC>, give(i));
+        if (rem && full / LANES == i && lane == left) {
+            switch (rem) {
+            case 1: piece_out<1>(i, y); break;
+            case 2: if constexpr (VEC > 2) piece_out<2>(i, y); break;
+            case 3: if constexpr (VEC > 2) piece_out<3>(i, y); break;
+            case 4: if constexpr (VEC > 4) piece_out<4>(i, y); break;
+            case 5: if constexpr (VEC > 4) piece_out<5>(i, y); break;
+            case 6: if constexpr (VEC > 4) piece_out<6>(i, y); break;
+            default: if constexpr (VEC > 4) piece_out<7>(i, y); break;
+            }
+        }
+    }
+};
+
+// Sums and maxima over LANES neighbouring threads of a wave.
+template <int LANES, typename A> __device__ __forceinline__ A lanes_sum(A v)
+{
+#pragma unroll
+    for (int d = LANES / 2; d > 0; d >>= 1) v += __shfl_xor(v, d, 64);
+    return v;
+}
+template <int LANES, typename A> __device__ __forceinline__ A lanes_max(A v)
+{
+#pragma unroll
+    for (int d = LANES / 2; d > 0; d >>= 1) {
+        const A y = __shfl_xor(v, d, 64);
+        v = y > v ? y : v;
+    }
+    return v;
+}
+
+template <typename A> __device__ __forceinline__ void add(Terms<A> &t, const Terms<A> &x)
+{
+    t.loss += x.loss;
+    t.ent += x.ent;
+    t.kl += x.kl;
+    t.clipped += x.clipped;
+}
+
+// The upstream gradient, and whether there is nothing to do.
+template <typename A> __device__ __forceinline__ bool upstream(const Row<A> &r, A &g)
+{
+    g = r.scale ? *r.scale : A(1);
+    return r.scale && r.skip_unit && g == A(1);
+}
+
+// Rows of 33 to 2048 elements: LANES threads of a wave a row.
+template <typename T, int LANES, int E>
+__global__ __launch_bounds__(BLOCK) void k_cat_lanes(const Row<typename Acc<T>::type> r, const Logits g)
 {
     typedef typename Acc<T>::type A;
-    A up1 = A(1);
-    if (r.scale) {
-        up1 = *r.scale;
-        if (r.skip_unit && up1 == A(1)) return;
-    }
+    A up1;
+    if (upstream(r, up1)) return;
     const A w = weight_of(r) * up1;
-    const int lane = threadIdx.x & 63;
-    const int64_t waves = (int64_t)gridDim.x * (BLOCK / 64);
+    const int lane = threadIdx.x % LANES;
+    constexpr int ROWS = BLOCK / LANES;
     Terms<A> t = {};
-    for (int64_t i = (int64_t)blockIdx.x * (BLOCK / 64) + (threadIdx.x >> 6); i < r.rows; i += waves) {
-        const T *x = (const T *)g.x + (i / g.inner) * g.outer_stride + (i % g.inner) * g.inner_stride;
-        T *d = g.d ? (T *)g.d + i * g.width : nullptr;
+    for (int64_t i0 = (int64_t)blockIdx.x * ROWS; i0 < r.rows; i0 += (int64_t)gridDim.x * ROWS) {
+        // (a wave's last rows may be past the end: its threads stay for the sums over lanes)
+        const int64_t i = i0 + threadIdx.x / LANES < r.rows ? i0 + threadIdx.x / LANES : r.rows - 1;
+        const bool mine = i0 + threadIdx.x / LANES < r.rows;
+        const bool on = mine && (!r.mask || r.mask[i]);
+        const T *const x = (const T *)g.x + start_of(g, i);
+        const int64_t at = action_of(g, i);
+        const bool in = at >= 0 && at < g.width;
+        Held<T, LANES, E> h;
+        if (on) h.load(x, g.width, lane);
+        else h.fill(0, 0);
+        const A xa = up(x[in ? at : 0]);
+        const A m = lanes_max<LANES>(h.most());
+        A s, q, lp;
+        h.sums(m, s, q);
+        s = lanes_sum<LANES>(s);
+        q = lanes_sum<LANES>(q);
+        if (!mine) continue;
+        Terms<A> x1 = {};
+        const Slope<A> c = slope_of(r, g, i, m, s, q, xa, at, w, x1, lp);
+        if (lane == 0) {
+            if (on) add(t, x1);
+            if (r.logp) r.logp[i] = on ? lp : A(0);
+        }
+        if (!g.d) continue;
+        T *const d = (T *)g.d + i * g.width;
+        if (on) h.slope(c, d, g.width, lane);
+        else h.zero(d, g.width, lane);
+    }
+    if (r.sums) leave_sums<BLOCK>(t, r.sums);
+}
+
+// Sum or maximum over a workgroup; `red` is used again only after another barrier.
+template <int THREADS, typename A> __device__ __forceinline__ A block_max(A v, A *red)
+{
+    v = wave_max(v);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = lanes_max<THREADS / 64>(red[threadIdx.x % (THREADS / 64)]);
+    return v;
+}
+template <int THREADS, typename A> __device__ __forceinline__ void block_sums(A &s, A &q, A (*red)[2])
+{
+    s = wave_sum(s);
+    q = wave_sum(q);
+    if ((threadIdx.x & 63) == 0) {
+        red[threadIdx.x >> 6][0] = s;
+        red[threadIdx.x >> 6][1] = q;
+    }
+    __syncthreads();
+    s = lanes_sum<THREADS / 64>(red[threadIdx.x % (THREADS / 64)][0]);
+    q = lanes_sum<THREADS / 64>(red[threadIdx.x % (THREADS / 64)][1]);
+}
+
+// Longer rows, up to THREADS * E elements: a workgroup a row.
+template <typename T, int THREADS, int E>
+__global__ __launch_bounds__(THREADS, E * sizeof(T) >= 256 ? 4 : 1) void k_cat_block(const Row<typename Acc<T>::type> r, const Logits g)
+{
+    typedef typename Acc<T>::type A;
+    __shared__ A red_m[THREADS / 64], red_s[THREADS / 64][2];
+    A up1;
+    if (upstream(r, up1)) return;
+    const A w = weight_of(r) * up1;
+    const int lane = threadIdx.x;
+    Terms<A> t = {};
+    for (int64_t i = blockIdx.x; i < r.rows; i += gridDim.x) {
+        T *const d = g.d ? (T *)g.d + i * g.width : nullptr;
+        Held<T, THREADS, E> h;
         if (r.mask && !r.mask[i]) {
             if (r.logp && lane == 0) r.logp[i] = A(0);
-            if (d)
-                for (int j = lane; j < g.width; j += 64) d[j] = (T)A(0);
+            if (d) h.zero(d, g.width, lane);
             continue;
         }
-        const int64_t at = g.actions32 ? (int64_t)((const int32_t *)g.actions)[i]
-                                       : ((const int64_t *)g.actions)[i];
-        A m = -INFINITY;
-        for (int j = lane; j < g.width; j += 64) m = up(x[j]) > m ? up(x[j]) : m;
-        m = wave_max(m);
-        A s = 0, q = 0;
-        for (int j = lane; j < g.width; j += 64) {
-            A z = up(x[j]) - m;
-            z = z < A(-1000) ? A(-1000) : z;  // (-inf: no term; NaN stays)
-            const A e = exp_of(z);
-            s += e;
-            q += e * z;
-        }
-        s = wave_sum(s);
-        q = wave_sum(q);
-        const A ls = log_of(s), H = ls - q / s;
+        const T *const x = (const T *)g.x + start_of(g, i);
+        const int64_t at = action_of(g, i);
         const bool in = at >= 0 && at < g.width;
-        const A lp = in ? (up(x[in ? at : 0]) - m) - ls : A(NAN);
-        Terms<A> mine = {};
-        const A gl = decide(r, i, lp, H + (in ? A(0) : A(NAN)), mine);
+        h.load(x, g.width, lane);
+        const A xa = up(x[in ? at : 0]);
+        // (each buffer's next use lies behind the other's barrier)
+        const A m = block_max<THREADS>(h.most(), red_m);
+        A s, q, lp;
+        h.sums(m, s, q);
+        block_sums<THREADS>(s, q, red_s);
+        Terms<A> x1 = {};
+        const Slope<A> c = slope_of(r, g, i, m, s, q, xa, at, w, x1, lp);
         if (lane == 0) {
+            add(t, x1);
             if (r.logp) r.logp[i] = lp;
-            t.loss += mine.loss;
-            t.ent += mine.ent;
-            t.kl += mine.kl;
-            t.clipped += mine.clipped;
         }
-        if (!d) continue;
-        const A gw = gl * w + (in ? A(0) : A(NAN)), ew = r.entc * w;
-        for (int j = lane; j < g.width; j += 64) {
-            A z = up(x[j]) - m;
-            z = z < A(-1000) ? A(-1000) : z;
-            const A p = exp_of(z) / s;
-            A v = p * (ew * (z - ls + H) - gw);
-            if (j == at) v += gw;
-            d[j] = (T)v;
+        if (d) h.slope(c, d, g.width, lane);
+    }
+    if (r.sums) leave_sums<THREADS>(t, r.sums);
+}
+
+// Rows too long for a workgroup's registers, or too few of them to fill the card: parts of up to
+// PART elements, a workgroup a part; first each part's maximum and sums, then every part of a row
+// joins them and writes its share of the gradient (its second reading comes from the caches).
+constexpr int PART = 8192;
+
+template <typename T>
+__global__ __launch_bounds__(BLOCK) void k_cat_parts(const Row<typename Acc<T>::type> r, const Logits g)
+{
+    typedef typename Acc<T>::type A;
+    __shared__ A red_m[BLOCK / 64], red_s[BLOCK / 64][2];
+    A up1;
+    if (upstream(r, up1)) return;
+    const int64_t units = r.rows * g.splits;
+    for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+        const int64_t i = u / g.splits;
+        const int part = (int)(u - i * g.splits), j = part * g.part;
+        if (r.mask && !r.mask[i]) continue;
+        const int n = g.width - j < g.part ? g.width - j : g.part;
+        Held<T, BLOCK, PART / BLOCK> h;
+        const T *const x = (const T *)g.x + start_of(g, i);
+        h.load(x + j, n, threadIdx.x);
+        const A m = block_max<BLOCK>(h.most(), red_m);
+        A s, q;
+        h.sums(m == A(-INFINITY) ? A(0) : m, s, q);  // (nothing open here: sums of 0)
+        block_sums<BLOCK>(s, q, red_s);
+        if (threadIdx.x == 0) {
+            A *const p = (A *)g.parts + 3 * u;
+            p[0] = m;
+            p[1] = s;
+            p[2] = q;
         }
     }
-    if (r.sums) leave_sums(t, r.sums);
 }
+
+template <typename T>
+__global__ __launch_bounds__(BLOCK) void k_cat_join(const Row<typename Acc<T>::type> r, const Logits g)
+{
+    typedef typename Acc<T>::type A;
+    typedef Base2<A> B;
+    A up1;
+    if (upstream(r, up1)) return;
+    const A w = weight_of(r) * up1;
+    const int64_t per = g.d ? g.splits : 1, units = r.rows * per;
+    Terms<A> t = {};
+    for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+        const int64_t i = u / per;
+        const int part = (int)(u - i * per), j = part * g.part;
+        const int n = g.width - j < g.part ? g.width - j : g.part;
+        T *const d = g.d ? (T *)g.d + i * g.width + j : nullptr;
+        Held<T, BLOCK, PART / BLOCK> h;
+        if (r.mask && !r.mask[i]) {
+            if (part == 0 && r.logp && threadIdx.x == 0) r.logp[i] = A(0);
+            if (d) h.zero(d, n, threadIdx.x);
+            continue;
+        }
+        const T *const x = (const T *)g.x + start_of(g, i);
+        if (d) h.load(x + j, n, threadIdx.x);
+        const int64_t at = action_of(g, i);
+        const bool in = at >= 0 && at < g.width;
+        const A xa = up(x[in ? at : 0]);
+        const A *const p = (const A *)g.parts + 3 * i * g.splits;
+        A m = -INFINITY, s = 0, q = 0;
+        for (int k = 0; k < g.splits; ++k) m = p[3 * k] > m ? p[3 * k] : m;
+        for (int k = 0; k < g.splits; ++k) {
+            const A dm = B::z(p[3 * k], m), f = B::exp(dm);
+            s += f * p[3 * k + 1];
+            q += f * (p[3 * k + 2] + B::floor(dm) * p[3 * k + 1]);
+        }
+        Terms<A> x1 = {};
+        A lp;
+        Slope<A> c = slope_of(r, g, i, m, s, q, xa, at, w, x1, lp);
+        if (part == 0 && threadIdx.x == 0) {
+            add(t, x1);
+            if (r.logp) r.logp[i] = lp;
+        }
+        if (!d) continue;
+        if (in) c.at = at >= j && at < j + n ? at - j : PART;  // (PART: in another part)
+        h.slope(c, d, n, threadIdx.x);
+    }
+    if (r.sums) leave_sums<BLOCK>(t, r.sums);
+}
+
+// Rows of up to N <= 32 elements: a thread a row.  A workgroup's rows lie next to each other in
+// memory (where the caller's strides say so) and pass through LDS both ways, so that memory sees
+// whole lines; a row's place there has an odd length, which spreads the threads over the banks.
+template <typename T, int N>
+__global__ __launch_bounds__(BLOCK) void k_cat_rows(const Row<typename Acc<T>::type> r, const Logits g)
+{
+    typedef typename Acc<T>::type A;
+    typedef Base2<A> B;
+    constexpr int VEC = 16 / sizeof(T);
+    __align__(16) __shared__ T tile[BLOCK * (N + 1)];
+    A up1;
+    if (upstream(r, up1)) return;
+    const A w = weight_of(r) * up1;
+    const int V = g.width, S = V | 1, tid = threadIdx.x;
+    const bool packed = g.flat && g.inner_stride == V;
+    Terms<A> t = {};
+    for (int64_t i0 = (int64_t)blockIdx.x * BLOCK; i0 < r.rows; i0 += (int64_t)gridDim.x * BLOCK) {
+        const int rows = r.rows - i0 < BLOCK ? (int)(r.rows - i0) : BLOCK, n = rows * V;
+        const int64_t i = i0 + tid;
+        const bool mine = tid < rows;
+        T *const own = tile + tid * S;
+        if (packed) {
+            const T *const x = (const T *)g.x + i0 * V;
+            for (int e = tid * VEC; e < n; e += BLOCK * VEC) {
+                if (e + VEC <= n) {
+                    const Span<T, VEC> y = *(const Span<T, VEC> *)(x + e);
+                    if (S == V) {
+                        ((Line<T, VEC> *)(tile + e))->s = y;
+                    } else {
+                        int row = e / V, col = e - row * V;
+#pragma unroll
+                        for (int k = 0; k < VEC; ++k) {
+                            tile[row * S + col] = y.e[k];
+                            if (++col == V) col = 0, ++row;
+                        }
+                    }
+                } else {
+                    for (int k = e; k < n; ++k) tile[k / V * S + k % V] = x[k];
+                }
+            }
+        } else if (mine) {
+            const T *const x = (const T *)g.x + start_of(g, i);
+            for (int k = 0; k < V; ++k) own[k] = x[k];
+        }
+        __syncthreads();
+        const bool on = mine && (!r.mask || r.mask[i]);
+        if (on) {
+            const int64_t at = action_of(g, i);
+            const bool in = at >= 0 && at < V;
+            A z[N], m = -INFINITY, s = 0, q = 0, lp;
+#pragma unroll
+            for (int k = 0; k < N; ++k)
+                if (k < V) {
+                    z[k] = up(own[k]);
+                    m = z[k] > m ? z[k] : m;
+                }
+            const A xa = up(own[in ? at : 0]);
+#pragma unroll
+            for (int k = 0; k < N; ++k)
+                if (k < V) {
+                    const A e = B::exp(B::z(z[k], m));
+                    z[k] = B::z(z[k], m);
+                    s += e;
+                    q = fma_of(e, B::floor(z[k]), q);
+                }
+            const Slope<A> c = slope_of(r, g, i, m, s, q, xa, at, w, t, lp);
+            if (r.logp) r.logp[i] = lp;
+            if (g.d) {
+#pragma unroll
+                for (int k = 0; k < N; ++k)
+                    if (k < V) own[k] = (T)(c.at < 0 ? c.gw : B::exp(z[k]) * fma_of(c.c1, B::floor(z[k]), c.c2) + (k == c.at ? c.gw : A(0)));
+            }
+        } else if (mine) {
+            if (r.logp) r.logp[i] = A(0);
+            for (int k = 0; k < V; ++k) own[k] = (T)0.0f;
+        }
+        __syncthreads();
+        if (!g.d) continue;
+        T *const d = (T *)g.d + i0 * V;
+        for (int e = tid * VEC; e < n; e += BLOCK * VEC) {
+            if (e + VEC <= n) {
+                Span<T, VEC> y;
+                if (S == V) {
+                    y = ((const Line<T, VEC> *)(tile + e))->s;
+                } else {
+                    int row = e / V, col = e - row * V;
+#pragma unroll
+                    for (int k = 0; k < VEC; ++k) {
+                        y.e[k] = tile[row * S + col];
+                        if (++col == V) col = 0, ++row;
+                    }
+                }
+                *(Span<T, VEC> *)(d + e) = y;
+            } else {
+                for (int k = e; k < n; ++k) d[k] = tile[k / V * S + k % V];
+            }
+        }
+        __syncthreads();
+    }
+    if (r.sums) leave_sums<BLOCK>(t, r.sums);
+}
+
+// ------------------------------------------------------------------------- Gaussian head
+//
+// z, its products and the gradient are in the head's accumulation type; log-probabilities are
+// summed in double, which costs nothing beside the memory and leaves the ratio to the old
+// policy, a small difference of sums of up to 64 terms, its last digits.
 
 struct Normal {
     int width, shared_std;
@@ -193,123 +780,170 @@ struct Normal {
     void *d_mean, *d_log_std;
 };
 
-// One thread per decision.
-template <typename T>
-__global__ __launch_bounds__(BLOCK) void k_gaussian(const Row<typename Acc<T>::type> r, const Normal g)
+// The block's sums of the shared deviations' gradient, D of them a thread, to its row of std_sums.
+template <int D, typename A> __device__ void leave_std(const A (&v)[D], double *out)
 {
-    typedef typename Acc<T>::type A;
-    A up1 = A(1);
-    if (r.scale) {
-        up1 = *r.scale;
-        if (r.skip_unit && up1 == A(1)) return;
+    __shared__ double red[BLOCK / 64][D];
+#pragma unroll
+    for (int k = 0; k < D; ++k) {
+        const double s = wave_sum((double)v[k]);
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6][k] = s;
     }
-    const A w = weight_of(r) * up1;
-    const int D = g.width;
-    const T *mean = (const T *)g.mean, *ls = (const T *)g.log_std;
-    const A *act = (const A *)g.actions;
-    T *dm = (T *)g.d_mean, *dl = (T *)g.d_log_std;
-    __shared__ double red[BLOCK / 64];
-    Terms<A> t = {};
-    for (int64_t i0 = (int64_t)blockIdx.x * BLOCK; i0 < r.rows; i0 += (int64_t)gridDim.x * BLOCK) {
-        const int64_t i = i0 + threadIdx.x;
-        const bool on = i < r.rows && (!r.mask || r.mask[i]);
-        if (i >= r.rows) continue;
-        if (!on) {
-            if (r.logp) r.logp[i] = A(0);
-            for (int d = 0; d < D; ++d) {
-                if (dm) dm[i * D + d] = (T)A(0);
-                if (dl && !g.shared_std) dl[i * D + d] = (T)A(0);
-            }
-            continue;
-        }
-        A lp = 0, H = 0;
-        for (int d = 0; d < D; ++d) {
-            const A l = up(ls[g.shared_std ? d : i * D + d]);
-            const A z = (act[i * D + d] - up(mean[i * D + d])) * exp_of(-l);
-            lp += A(-0.5) * z * z - l - A(HALF_LOG_2PI);
-            H += l + A(HALF_LOG_2PI + 0.5);
-        }
-        const A gl = decide(r, i, lp, H, t) * w;
-        if (r.logp) r.logp[i] = lp;
-        for (int d = 0; d < D; ++d) {
-            const A l = up(ls[g.shared_std ? d : i * D + d]), inv = exp_of(-l);
-            const A z = (act[i * D + d] - up(mean[i * D + d])) * inv;
-            if (dm) dm[i * D + d] = (T)(gl * z * inv);
-            if (dl && !g.shared_std) dl[i * D + d] = (T)(gl * (z * z - A(1)) - r.entc * w);
-        }
-    }
-    if (r.sums) leave_sums(t, r.sums);
-    if (!r.std_sums) return;
-    // the shared deviations' gradient, dimension by dimension
-    for (int d = 0; d < D; ++d) {
-        const A l = up(ls[d]), inv = exp_of(-l);
+    __syncthreads();
+    if (threadIdx.x < D) {
         double s = 0;
-        for (int64_t i = (int64_t)blockIdx.x * BLOCK + threadIdx.x; i < r.rows;
-             i += (int64_t)gridDim.x * BLOCK) {
-            if (r.mask && !r.mask[i]) continue;
-            A lp = 0;
-            for (int k = 0; k < D; ++k) {
-                const A lk = up(ls[k]);
-                const A zk = (act[i * D + k] - up(mean[i * D + k])) * exp_of(-lk);
-                lp += A(-0.5) * zk * zk - lk - A(HALF_LOG_2PI);
-            }
-            Terms<A> none = {};
-            const A gl = decide(r, i, lp, A(0), none) * w;
-            const A z = (act[i * D + d] - up(mean[i * D + d])) * inv;
-            s += (double)(gl * (z * z - A(1)) - r.entc * w);
-        }
-        s = wave_sum(s);
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            for (int k = 1; k < BLOCK / 64; ++k) s += red[k];
-            r.std_sums[(int64_t)blockIdx.x * D + d] = s;
-        }
+        for (int w = 0; w < BLOCK / 64; ++w) s += red[w][threadIdx.x];
+        out[(int64_t)blockIdx.x * D + threadIdx.x] = s;
     }
 }
 
-// One block: the blocks' sums to the loss and the means, and to the shared deviations' gradient.
-template <typename T>
-__global__ __launch_bounds__(BLOCK) void k_finish(const Row<typename Acc<T>::type> r, int blocks, int D,
-                                                  typename Acc<T>::type *loss,
-                                                  typename Acc<T>::type *stats, T *d_log_std)
+// Up to four dimensions: a thread a decision.
+template <typename T, int D, bool SHARED>
+__global__ __launch_bounds__(BLOCK) void k_gauss_rows(const Row<typename Acc<T>::type> r, const Normal g)
 {
     typedef typename Acc<T>::type A;
+    A up1;
+    if (upstream(r, up1)) return;
+    const A w = weight_of(r) * up1;
+    const Span<T, D> *mean = (const Span<T, D> *)g.mean, *ls = (const Span<T, D> *)g.log_std;
+    const Span<A, D> *act = (const Span<A, D> *)g.actions;
+    Span<T, D> *dm = (Span<T, D> *)g.d_mean, *dl = (Span<T, D> *)g.d_log_std;
+    Terms<A> t = {};
+    A std_sum[D] = {};
+    Span<T, D> l0;
+    if (SHARED) l0 = ls[0];
+    for (int64_t i = (int64_t)blockIdx.x * BLOCK + threadIdx.x; i < r.rows; i += (int64_t)gridDim.x * BLOCK) {
+        const bool on = !r.mask || r.mask[i];
+        Span<T, D> om, ol;
+        if (!on) {
+#pragma unroll
+            for (int k = 0; k < D; ++k) om.e[k] = (T)0.0f;
+            ol = om;
+            if (r.logp) r.logp[i] = A(0);
+        } else {
+            const Span<T, D> mu = mean[i], lv = SHARED ? l0 : ls[i];
+            const Span<A, D> a = act[i];
+            A z[D], inv[D], H = 0;
+            double lp = 0;
+#pragma unroll
+            for (int k = 0; k < D; ++k) {
+                const A l = up(lv.e[k]);
+                inv[k] = exp_of(-l);
+                z[k] = (a.e[k] - up(mu.e[k])) * inv[k];
+                lp += -0.5 * (double)(z[k] * z[k]) - (double)l - HALF_LOG_2PI;
+                H += l + A(HALF_LOG_2PI + 0.5);
+            }
+            const A gl = decide(r, i, lp, H, t) * w;
+            if (r.logp) r.logp[i] = (A)lp;
+#pragma unroll
+            for (int k = 0; k < D; ++k) {
+                om.e[k] = (T)(gl * z[k] * inv[k]);
+                const A y = gl * (z[k] * z[k] - A(1)) - r.entc * w;
+                if (SHARED) std_sum[k] += y;
+                else ol.e[k] = (T)y;
+            }
+        }
+        if (dm) dm[i] = om;
+        if (!SHARED && dl) dl[i] = ol;
+    }
+    if (r.sums) leave_sums<BLOCK>(t, r.sums);
+    if (SHARED && r.std_sums) leave_std<D>(std_sum, r.std_sums);
+}
+
+// More dimensions: LANES threads a decision, a thread a dimension.
+template <typename T, int LANES>
+__global__ __launch_bounds__(BLOCK) void k_gauss_lanes(const Row<typename Acc<T>::type> r, const Normal g)
+{
+    typedef typename Acc<T>::type A;
+    __shared__ double red[BLOCK / LANES][LANES];
+    A up1;
+    if (upstream(r, up1)) return;
+    const A w = weight_of(r) * up1;
+    constexpr int ROWS = BLOCK / LANES;
+    const int D = g.width, k = threadIdx.x % LANES, row = threadIdx.x / LANES;
+    const bool dim = k < D;
+    const T *mean = (const T *)g.mean, *ls = (const T *)g.log_std;
+    const A *act = (const A *)g.actions;
+    T *dm = (T *)g.d_mean, *dl = (T *)g.d_log_std;
+    Terms<A> t = {};
+    A std_sum = 0;
+    const A l0 = g.shared_std && dim ? up(ls[k]) : A(0);
+    for (int64_t i0 = (int64_t)blockIdx.x * ROWS; i0 < r.rows; i0 += (int64_t)gridDim.x * ROWS) {
+        const int64_t i = i0 + row, j = i * D + k;
+        const bool mine = i < r.rows, on = mine && (!r.mask || r.mask[i]);
+        A z = 0, inv = 0, h = 0;
+        double lp = 0;
+        if (on && dim) {
+            const A l = g.shared_std ? l0 : up(ls[j]);
+            inv = exp_of(-l);
+            z = (act[j] - up(mean[j])) * inv;
+            lp = -0.5 * (double)(z * z) - (double)l - HALF_LOG_2PI;
+            h = l + A(HALF_LOG_2PI + 0.5);
+        }
+        lp = lanes_sum<LANES>(lp);
+        h = lanes_sum<LANES>(h);
+        if (!mine) continue;
+        A om = 0, ol = 0;
+        if (on) {
+            Terms<A> x1 = {};
+            const A gl = decide(r, i, lp, h, x1) * w;
+            if (k == 0) add(t, x1);
+            om = gl * z * inv;
+            ol = gl * (z * z - A(1)) - r.entc * w;
+            if (dim) std_sum += ol;
+        }
+        if (k == 0 && r.logp) r.logp[i] = on ? (A)lp : A(0);
+        if (dim && dm) dm[j] = (T)om;
+        if (dim && dl && !g.shared_std) dl[j] = (T)ol;
+    }
+    if (r.sums) leave_sums<BLOCK>(t, r.sums);
+    if (!r.std_sums) return;
+    red[row][k] = (double)std_sum;
+    __syncthreads();
+    if (threadIdx.x < D) {
+        double s = 0;
+        for (int q = 0; q < ROWS; ++q) s += red[q][threadIdx.x];
+        r.std_sums[(int64_t)blockIdx.x * D + threadIdx.x] = s;
+    }
+}
+
+// One workgroup joins what the others left: sums of the columns of v [blocks][W], W <= 64, in
+// threads below W.  `red`: FINISH doubles.
+constexpr int FINISH = 1024;
+__device__ __forceinline__ double columns(const double *v, int blocks, int W, double *red)
+{
+    const int groups = FINISH / W, g = threadIdx.x / W, c = threadIdx.x - g * W;
+    double s = 0;
+    if (g < groups)
+        for (int b = g; b < blocks; b += groups) s += v[(int64_t)b * W + c];
+    __syncthreads();
+    red[threadIdx.x] = s;
+    __syncthreads();
+    for (int n = groups; n > 1;) {
+        const int h = (n + 1) / 2;
+        if (g < n - h) red[threadIdx.x] += red[threadIdx.x + h * W];
+        __syncthreads();
+        n = h;
+    }
+    return red[threadIdx.x];
+}
+
+template <typename T>
+__global__ __launch_bounds__(FINISH) void k_finish(const Row<typename Acc<T>::type> r, int blocks, int D,
+                                                   typename Acc<T>::type *loss,
+                                                   typename Acc<T>::type *stats, T *d_log_std)
+{
+    typedef typename Acc<T>::type A;
+    __shared__ double red[FINISH];
     if (r.scale && r.skip_unit && *r.scale == A(1)) return;
-    __shared__ double red[BLOCK];
-    __shared__ double n;
-    if (threadIdx.x == 0) {
-        double c = (double)r.rows;
-        if (r.mask) {
-            c = 0;
-            for (int i = 0; i < r.n_counts; ++i) c += r.counts[i];
-        }
-        n = c > 1 ? c : 1;
-    }
     if (stats) {
-        const int k = threadIdx.x & 3;
-        double s = 0;
-        for (int b = threadIdx.x >> 2; b < blocks; b += BLOCK / 4) s += r.sums[4 * (int64_t)b + k];
-        red[threadIdx.x] = s;
-        __syncthreads();
-        if (threadIdx.x < 4) {
-            for (int b = 1; b < BLOCK / 4; ++b) s += red[4 * b + k];
-            if (k == 0) *loss = (A)(r.sum ? s : s / n);
-            else stats[k - 1] = (A)(s / n);
-        }
+        const double n = counted(r), s = columns(r.sums, blocks, 4, red);
+        if (threadIdx.x == 0) *loss = (A)(r.sum ? s : s / n);
+        else if (threadIdx.x < 4) stats[threadIdx.x - 1] = (A)(s / n);
     }
-    if (!d_log_std) return;
-    for (int d = 0; d < D; ++d) {
-        double s = 0;
-        for (int b = threadIdx.x; b < blocks; b += BLOCK) s += r.std_sums[(int64_t)b * D + d];
-        __syncthreads();
-        red[threadIdx.x] = s;
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            for (int b = 1; b < BLOCK; ++b) s += red[b];
-            d_log_std[d] = (T)(A)s;
-        }
+    if (d_log_std) {
+        const double s = columns(r.std_sums, blocks, D, red);
+        if (threadIdx.x < D) d_log_std[threadIdx.x] = (T)(A)s;
     }
 }
 
@@ -317,6 +951,13 @@ __global__ __launch_bounds__(BLOCK) void k_finish(const Row<typename Acc<T>::typ
 
 uint64_t sums_bytes() { return (uint64_t)MOST_BLOCKS * 4 * sizeof(double); }
 uint64_t counts_bytes() { return (uint64_t)COUNTERS * sizeof(int32_t); }
+// Elements of a part: the largest multiple of `vec` up to PART that leaves none shorter than vec.
+int part_of(int width, int vec)
+{
+    int n = PART;
+    while (width % n && width % n < vec) n -= vec;
+    return n;
+}
 
 int check(const swarp_policy_t *a)
 {
@@ -363,38 +1004,120 @@ template <typename A> void count(const swarp_policy_t *a, Row<A> &r, hipStream_t
     if (!a->mask) return;
     const int64_t want = (a->rows + 8 * BLOCK - 1) / (8 * BLOCK);
     r.n_counts = (int)(want < 1 ? 1 : want > COUNTERS ? COUNTERS : want);
+    if (a->counted) return;
     hipLaunchKernelGGL(k_count, dim3(r.n_counts), dim3(BLOCK), 0, st, a->rows, a->mask,
                        (int32_t *)r.counts);
 }
 
 int blocks_for(int64_t units) { return (int)(units < 1 ? 1 : units > MOST_BLOCKS ? MOST_BLOCKS : units); }
 
+template <typename T, int LANES, int E>
+int cat_lanes(const Row<typename Acc<T>::type> &r, const Logits &g, hipStream_t st)
+{
+    const int blocks = blocks_for((r.rows + BLOCK / LANES - 1) / (BLOCK / LANES));
+    hipLaunchKernelGGL((k_cat_lanes<T, LANES, E>), dim3(blocks), dim3(BLOCK), 0, st, r, g);
+    return blocks;
+}
+template <typename T, int THREADS, int E>
+int cat_block(const Row<typename Acc<T>::type> &r, const Logits &g, hipStream_t st)
+{
+    const int blocks = blocks_for(r.rows);
+    hipLaunchKernelGGL((k_cat_block<T, THREADS, E>), dim3(blocks), dim3(THREADS), 0, st, r, g);
+    return blocks;
+}
+template <typename T, int N>
+int cat_rows(const Row<typename Acc<T>::type> &r, const Logits &g, hipStream_t st)
+{
+    const int blocks = blocks_for((r.rows + BLOCK - 1) / BLOCK);
+    hipLaunchKernelGGL((k_cat_rows<T, N>), dim3(blocks), dim3(BLOCK), 0, st, r, g);
+    return blocks;
+}
+template <typename T> int cat_parts(const Row<typename Acc<T>::type> &r, Logits g, void *parts, hipStream_t st)
+{
+    g.parts = parts;
+    g.part = part_of(g.width, 16 / sizeof(T));
+    g.splits = (g.width + g.part - 1) / g.part;
+    const int blocks = blocks_for(r.rows * g.splits);
+    hipLaunchKernelGGL((k_cat_parts<T>), dim3(blocks), dim3(BLOCK), 0, st, r, g);
+    hipLaunchKernelGGL((k_cat_join<T>), dim3(blocks), dim3(BLOCK), 0, st, r, g);
+    return blocks;
+}
+
 template <typename T> void categorical(const swarp_policy_t *a, hipStream_t st)
 {
     Row<typename Acc<T>::type> r = row_of<T>(a);
     count(a, r, st);
-    const int blocks = blocks_for((a->rows + BLOCK / 64 - 1) / (BLOCK / 64));
-    const Logits g = {a->inner, a->outer_stride, a->inner_stride, a->width, a->actions32,
-                      a->head, a->actions, a->d_head};
-    hipLaunchKernelGGL((k_categorical<T>), dim3(blocks), dim3(BLOCK), 0, st, r, g);
+    const int V = a->width;
+    Logits g = {a->inner, a->outer_stride, a->inner_stride, V, a->actions32, a->inner >= a->rows, 1, PART,
+                a->head, a->actions, a->d_head, nullptr};
+    void *const parts = (char *)a->work + sums_bytes() + counts_bytes() + MOST_BLOCKS * sizeof(double) * MOST_DIMS;
+    int blocks = 0;
+    if constexpr (sizeof(T) < 8) {
+        if (V <= 8) blocks = cat_rows<T, 8>(r, g, st);
+        else if (V <= 16) blocks = cat_rows<T, 16>(r, g, st);
+        else if (V <= 32) blocks = cat_rows<T, 32>(r, g, st);
+    }
+    if (blocks) {
+    } else if (V <= 64) blocks = cat_lanes<T, 4, 16>(r, g, st);
+    else if (V <= 128) blocks = cat_lanes<T, 8, 16>(r, g, st);
+    else if (V <= 256) blocks = cat_lanes<T, 16, 16>(r, g, st);
+    else if (V <= 512) blocks = cat_lanes<T, 32, 16>(r, g, st);
+    else if (V <= 1024) blocks = cat_lanes<T, 64, 16>(r, g, st);
+    else if (V <= 2048) blocks = cat_lanes<T, 64, 32>(r, g, st);
+    else if (V <= 4096) blocks = cat_block<T, 256, 16>(r, g, st);
+    else if (V <= 8192) blocks = cat_block<T, 256, 32>(r, g, st);
+    else if (r.rows < FEW_ROWS || V > 65536 || sizeof(T) == 8) blocks = cat_parts<T>(r, g, parts, st);
+    else if constexpr (sizeof(T) < 8) {
+        if (V <= 16384) blocks = cat_block<T, 256, 64>(r, g, st);
+        else if (V <= 32768) blocks = cat_block<T, 512, 64>(r, g, st);
+        else if constexpr (sizeof(T) == 2) blocks = cat_block<T, 512, 128>(r, g, st);
+        else blocks = cat_block<T, 1024, 64>(r, g, st);
+    }
     if (a->stats)
-        hipLaunchKernelGGL((k_finish<T>), dim3(1), dim3(BLOCK), 0, st, r, blocks, 0,
+        hipLaunchKernelGGL((k_finish<T>), dim3(1), dim3(FINISH), 0, st, r, blocks, 0,
                            (typename Acc<T>::type *)a->loss, (typename Acc<T>::type *)a->stats,
                            (T *)nullptr);
+}
+
+template <typename T, int D> int gauss_rows(const Row<typename Acc<T>::type> &r, const Normal &g, hipStream_t st)
+{
+    const int blocks = blocks_for((r.rows + BLOCK - 1) / BLOCK);
+    if (g.shared_std)
+        hipLaunchKernelGGL((k_gauss_rows<T, D, true>), dim3(blocks), dim3(BLOCK), 0, st, r, g);
+    else
+        hipLaunchKernelGGL((k_gauss_rows<T, D, false>), dim3(blocks), dim3(BLOCK), 0, st, r, g);
+    return blocks;
+}
+template <typename T, int LANES>
+int gauss_lanes(const Row<typename Acc<T>::type> &r, const Normal &g, hipStream_t st)
+{
+    const int blocks = blocks_for((r.rows + BLOCK / LANES - 1) / (BLOCK / LANES));
+    hipLaunchKernelGGL((k_gauss_lanes<T, LANES>), dim3(blocks), dim3(BLOCK), 0, st, r, g);
+    return blocks;
 }
 
 template <typename T> void gaussian(const swarp_policy_t *a, hipStream_t st)
 {
     Row<typename Acc<T>::type> r = row_of<T>(a);
     count(a, r, st);
-    const int blocks = blocks_for((a->rows + BLOCK - 1) / BLOCK);
     const bool shared = a->shared_std && a->d_log_std;
     if (shared) r.std_sums = (double *)((char *)a->work + sums_bytes() + counts_bytes());
     const Normal g = {a->width, a->shared_std, a->head, a->log_std, a->actions, a->d_head,
                       a->d_log_std};
-    hipLaunchKernelGGL((k_gaussian<T>), dim3(blocks), dim3(BLOCK), 0, st, r, g);
+    int blocks;
+    switch (a->width) {
+    case 1: blocks = gauss_rows<T, 1>(r, g, st); break;
+    case 2: blocks = gauss_rows<T, 2>(r, g, st); break;
+    case 3: blocks = gauss_rows<T, 3>(r, g, st); break;
+    case 4: blocks = gauss_rows<T, 4>(r, g, st); break;
+    default:
+        blocks = a->width <= 8    ? gauss_lanes<T, 8>(r, g, st)
+                 : a->width <= 16 ? gauss_lanes<T, 16>(r, g, st)
+                 : a->width <= 32 ? gauss_lanes<T, 32>(r, g, st)
+                                  : gauss_lanes<T, 64>(r, g, st);
+    }
     if (a->stats || shared)
-        hipLaunchKernelGGL((k_finish<T>), dim3(1), dim3(BLOCK), 0, st, r, blocks, a->width,
+        hipLaunchKernelGGL((k_finish<T>), dim3(1), dim3(FINISH), 0, st, r, blocks, a->width,
                            (typename Acc<T>::type *)a->loss, (typename Acc<T>::type *)a->stats,
                            shared ? (T *)a->d_log_std : nullptr);
 }
@@ -403,7 +1126,7 @@ template <typename T> void gaussian(const swarp_policy_t *a, hipStream_t st)
 template <typename T> void nothing(const swarp_policy_t *a, hipStream_t st)
 {
     const Row<typename Acc<T>::type> r = row_of<T>(a);
-    hipLaunchKernelGGL((k_finish<T>), dim3(1), dim3(BLOCK), 0, st, r, 0, a->width,
+    hipLaunchKernelGGL((k_finish<T>), dim3(1), dim3(FINISH), 0, st, r, 0, a->width,
                        (typename Acc<T>::type *)a->loss, (typename Acc<T>::type *)a->stats,
                        a->shared_std ? (T *)a->d_log_std : (T *)nullptr);
 }
@@ -422,9 +1145,13 @@ extern "C" {
 
 uint64_t swarp_policy_work_bytes(int64_t rows, int32_t width)
 {
-    (void)rows;
-    const uint64_t dims = width < MOST_DIMS ? (width < 1 ? 1 : width) : MOST_DIMS;
-    return sums_bytes() + counts_bytes() + MOST_BLOCKS * dims * sizeof(double);
+    uint64_t n = sums_bytes() + counts_bytes() + MOST_BLOCKS * sizeof(double) * MOST_DIMS;
+    if (width > PART && rows > 0) {  // whichever type the call has
+        const int part = part_of(width, 2), p4 = part_of(width, 4), p8 = part_of(width, 8);
+        const int least = part < p4 ? (part < p8 ? part : p8) : (p4 < p8 ? p4 : p8);
+        n += (uint64_t)rows * ((width - 1) / least + 1) * 3 * sizeof(double);
+    }
+    return n;
 }
 
 int swarp_categorical_loss(const swarp_policy_t *a, void *stream)

@@ -167,19 +167,16 @@ def gae(rewards: torch.Tensor, values: torch.Tensor, terminated: torch.Tensor | 
     values = _same(values, "values", (*batch, T + 1) if last else (T + 1, *batch), dtype, dev)
     if final_values is not None:
         final_values = _same(final_values, "final_values", shape, dtype, dev)
-    group, flags = 1, []
-    for name, f in (("terminated", terminated), ("truncated", truncated)):
-        if f is None:
-            flags.append(None)
-            continue
-        k = f.dim() - 1
-        lead = batch[:max(k, 0)]
-        f = _same(f, name, (*lead, T) if last else (T, *lead), torch.bool, dev)
-        flags.append(f)
-        group = math.prod(batch[k:])
-    if None not in flags and flags[0].shape != flags[1].shape:
-        raise ValueError(f"terminated {list(flags[0].shape)} and truncated {list(flags[1].shape)} "
-                         "must have the same shape")
+    if terminated is not None and truncated is not None and terminated.shape != truncated.shape:
+        raise ValueError(f"terminated {list(terminated.shape)} and truncated "
+                         f"{list(truncated.shape)} must have the same shape")
+    group, flags = 1, [terminated, truncated]
+    for n, name in enumerate(("terminated", "truncated")):
+        if flags[n] is not None:
+            k = max(flags[n].dim() - 1, 0)
+            lead = batch[:k]
+            flags[n] = _same(flags[n], name, (*lead, T) if last else (T, *lead), torch.bool, dev)
+            group = math.prod(batch[k:])
     scan = _Scan(int(last), T, math.prod(batch), max(group, 1), float(gamma), float(lam))
     inputs = (rewards, values, final_values)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs):
@@ -203,29 +200,39 @@ class _Loss(NamedTuple):
     sum: bool
 
 
-def _loss_call(c: _Loss, head, log_std, actions, old, adv, ref, mask, logp=None, loss=None,
-               stats=None, d_head=None, d_log_std=None, scale=None, skip_unit=0) -> None:
-    lib = _lib.load()
-    dev = head.device
-    nbytes = lib.swarp_policy_work_bytes(c.rows, c.width)
-    work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+def _loss_args(c: _Loss, head, log_std, actions, old, adv, ref, mask):
+    """The C arguments of a call, without its results, and the work memory they point to."""
+    nbytes = _lib.load().swarp_policy_work_bytes(c.rows, c.width)
+    work = torch.empty(nbytes, dtype=torch.uint8, device=head.device)
     a = _lib.SwarpPolicy(
         dtype=_CODES[head.dtype], sum=c.sum, width=c.width,
-        actions32=actions.dtype == torch.int32, skip_unit=skip_unit,
+        actions32=actions.dtype == torch.int32,
         shared_std=log_std is not None and log_std.dim() == 1 and head.dim() > 1,
         rows=c.rows, inner=c.strides[0], outer_stride=c.strides[1], inner_stride=c.strides[2],
         clip_low=c.clip[0], clip_high=c.clip[1], kl_coef=c.kl_coef, entropy_coef=c.entropy_coef,
         head=head.data_ptr(), log_std=_ptr(log_std), actions=actions.data_ptr(),
         old_logp=old.data_ptr(), advantages=adv.data_ptr(), ref_logp=_ptr(ref), mask=_ptr(mask),
-        logp=_ptr(logp), loss=_ptr(loss), stats=_ptr(stats), d_head=_ptr(d_head),
-        d_log_std=_ptr(d_log_std), scale=_ptr(scale), work=work.data_ptr(), work_bytes=nbytes)
+        work=work.data_ptr(), work_bytes=nbytes)
+    return a, work
+
+
+def _loss_launch(c: _Loss, a: _lib.SwarpPolicy, dev) -> None:
+    lib = _lib.load()
     call = lib.swarp_gaussian_loss if c.gaussian else lib.swarp_categorical_loss
     with _guard(dev):
         _lib.check(call(ctypes.byref(a), _lib.stream_of(dev)))
 
 
-def _results(head, old):
-    return old.new_empty(()), old.new_empty(3), torch.empty_like(old)
+def _loss_forward(c: _Loss, head, log_std, rest, made=(None, None)):
+    """(loss, stats, logp) of a call, its arguments and its work memory; ``made`` are gradient
+    buffers to fill on the way."""
+    a, work = _loss_args(c, head, log_std, *rest)
+    old = rest[1]
+    loss, stats, logp = old.new_empty(()), old.new_empty(3), torch.empty_like(old)
+    a.logp, a.loss, a.stats = logp.data_ptr(), loss.data_ptr(), stats.data_ptr()
+    a.d_head, a.d_log_std = _ptr(made[0]), _ptr(made[1])
+    _loss_launch(c, a, head.device)
+    return loss, stats, logp, a, work
 
 
 def _buffers(head, log_std, need):
@@ -252,10 +259,8 @@ class _LossFn(torch.autograd.Function):
         ctx.made = None
         if head.dtype != torch.float16:
             ctx.made = _buffers(head, log_std, ctx.need)
-        loss, stats, logp = _results(head, rest[1])
-        d = ctx.made or (None, None)
-        _loss_call(c, head, log_std, *rest, logp=logp, loss=loss, stats=stats, d_head=d[0],
-                   d_log_std=d[1])
+        loss, stats, logp, *ctx.call = _loss_forward(c, head, log_std, rest,
+                                                     ctx.made or (None, None))
         ctx.save_for_backward(head, log_std, *rest)
         ctx.mark_non_differentiable(stats, logp)
         return loss, stats, logp
@@ -265,11 +270,14 @@ class _LossFn(torch.autograd.Function):
     def backward(ctx, g, *_):
         if g is None:
             return (None,) * 8
-        head, log_std, *rest = ctx.saved_tensors
+        head, log_std = ctx.saved_tensors[:2]  # (unchanged since, or this raises)
         made, ctx.made = ctx.made, None  # handed out once: the caller may change them
         d = made or _buffers(head, log_std, ctx.need)
-        _loss_call(ctx.c, head, log_std, *rest, d_head=d[0], d_log_std=d[1], scale=g,
-                   skip_unit=made is not None)
+        a = ctx.call[0]
+        a.logp = a.loss = a.stats = None
+        a.d_head, a.d_log_std, a.scale = _ptr(d[0]), _ptr(d[1]), g.data_ptr()
+        a.skip_unit, a.counted = made is not None, 1
+        _loss_launch(ctx.c, a, head.device)
         return None, *d, *(None,) * 5
 
 
@@ -300,8 +308,7 @@ def _evaluate(c: _Loss, head, log_std, *rest) -> PolicyLoss:
                                     or (log_std is not None and log_std.requires_grad)):
         loss, stats, logp = _LossFn.apply(c, head, log_std, *rest)
     else:
-        loss, stats, logp = _results(head, rest[1])
-        _loss_call(c, head, log_std, *rest, logp=logp, loss=loss, stats=stats)
+        loss, stats, logp = _loss_forward(c, head, log_std, rest)[:3]
     return PolicyLoss(loss, logp, *stats.unbind(0))
 
 
