@@ -71,13 +71,8 @@ __device__ __forceinline__ uint32_t random_of(uint64_t i, uint32_t seed)
 __device__ __forceinline__ uint32_t bits_of(float x) { return (uint32_t)__float_as_int(x); }
 __device__ __forceinline__ float float_of(uint32_t b) { return __int_as_float((int)b); }
 
-// The base of a group whose largest magnitude has the bits `most`: the exponent `reach` below
-// that of the magnitude rounded up to a code.
-__device__ __forceinline__ uint32_t base_of(uint32_t most, uint32_t reach)
-{
-    const uint32_t e = (most + 0xfffffu) >> 23;
-    return e > reach ? e - reach : 0;
-}
+// The base of a group whose largest magnitude, rounded up to a code, has the exponent e.
+__device__ __forceinline__ uint32_t base_of(uint32_t e, uint32_t reach) { return e > reach ? e - reach : 0; }
 __device__ __forceinline__ uint32_t magnitude(float x)
 {
     const uint32_t m = bits_of(x) & 0x7fffffffu;
@@ -98,87 +93,165 @@ __device__ __forceinline__ float decode_m(uint32_t c, uint32_t base)
     return float_of(bits_of(x) | (c & 128u) << 24);
 }
 
-__device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t *red)
+// Both exponents of a group's largest magnitudes, rounded up to a code: one reduction over the wave
+// for the two, as halves of a word.
+typedef unsigned short Pair __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ Pair wave_max(Pair e)
 {
-    v = wave_max(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    for (int w = 0; w < BLOCK / 64; ++w) v = red[w] > v ? red[w] : v;
-    return v;
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1)
+        e = __builtin_elementwise_max(e, __builtin_bit_cast(Pair, __shfl_xor(__builtin_bit_cast(int, e), d, 64)));
+    return e;
+}
+__device__ __forceinline__ uint32_t exponent(uint32_t mag) { return (mag + 0xfffffu) >> 23; }
+
+// A parameter without a master copy: bfloat16 at random, in proportion (infinities and NaN are
+// cut).
+template <typename P> __device__ __forceinline__ P rounded(float x, uint32_t r)
+{
+    if constexpr (sizeof(P) == 2 && __is_same(P, bf16)) {
+        const uint32_t b = bits_of(x);
+        const bool finite = (b & 0x7f800000u) != 0x7f800000u;
+        return finite ? __builtin_bit_cast(bf16, (uint16_t)((b + (mix(r) & 0xffffu)) >> 16)) : (bf16)x;
+    } else {
+        return (P)x;
+    }
 }
 
-__device__ __forceinline__ void put(float *p, float x, uint32_t) { *p = x; }
-__device__ __forceinline__ void put(f16 *p, float x, uint32_t) { *p = (f16)x; }
-// bfloat16 without a master: at random, in proportion; infinities and NaN are cut
-__device__ __forceinline__ void put(bf16 *p, float x, uint32_t r)
+template <typename T, int N> struct __attribute__((packed, aligned(sizeof(T)))) Span {
+    T e[N];
+};
+// Elements i .. i + 3 of n, those there are; 0 for the others.
+template <typename T> __device__ __forceinline__ void get(float (&x)[4], const T *p, int64_t i, int64_t n)
 {
-    const uint32_t b = bits_of(x);
-    const bool finite = (b & 0x7f800000u) != 0x7f800000u;
-    *p = finite ? __builtin_bit_cast(bf16, (uint16_t)((b + (mix(r) & 0xffffu)) >> 16)) : (bf16)x;
+    if (i + 4 <= n) {
+        const Span<T, 4> y = *(const Span<T, 4> *)(p + i);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = (float)y.e[k];
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = i + k < n ? (float)p[i + k] : 0.0f;
+    }
 }
 
-// A workgroup takes a chunk of a tensor, a thread an element of each of its groups.
+// A workgroup takes a chunk of a tensor, a wave four groups of it, a thread four neighbouring
+// elements of each group: all loads of the four groups are in flight before the first is used,
+// and a group's largest exponents are found without LDS or barriers.
+constexpr int WAVE_GROUPS = CHUNK / GROUP / (BLOCK / 64);
+
 template <typename P, typename G, int BITS>
 __global__ __launch_bounds__(BLOCK) void k_adamw(const Step s, const Tensors t)
 {
-    __shared__ uint32_t red[2][BLOCK / 64];
     const int k = tensor_of(t, blockIdx.x);
     P *const param = (P *)t.param[k];
     const G *const grad = (const G *)t.grad[k];
     const int64_t n = t.n[k], slot = t.slot[k];
-    const int64_t begin = (int64_t)(blockIdx.x - t.first[k]) * CHUNK;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t begin = (int64_t)(blockIdx.x - t.first[k]) * CHUNK + wave * (WAVE_GROUPS * GROUP);
     const float scale = s.scale ? *s.scale : 1.0f;
-    for (int64_t i0 = begin; i0 < begin + CHUNK && i0 < n; i0 += GROUP) {
-        const int64_t i = i0 + threadIdx.x, j = slot + i, q = (slot + i0) / GROUP;
-        const bool in = i < n;
-        float g = in ? (float)grad[i] : 0.0f, m = 0, v = 0, w = 0;
+    float g[WAVE_GROUPS][4], m[WAVE_GROUPS][4], v[WAVE_GROUPS][4], w[WAVE_GROUPS][4];
+    uint32_t mc[WAVE_GROUPS], vc[WAVE_GROUPS], mb[WAVE_GROUPS], vb[WAVE_GROUPS];
+#pragma unroll
+    for (int u = 0; u < WAVE_GROUPS; ++u) {
+        const int64_t i0 = begin + u * GROUP, i = i0 + 4 * lane, j = slot + i;
+        if (i0 >= n) break;
+        get(g[u], grad, i, n);
         if (BITS == 8) {
-            m = decode_m(((const uint8_t *)s.m)[j], s.m_base[q]);
-            v = decode(((const uint8_t *)s.v)[j], s.v_base[q]);
-        } else if (in) {
-            m = ((const float *)s.m)[j];
-            v = ((const float *)s.v)[j];
-        }
-        if (in) w = s.master ? s.master[j] : (float)param[i];
-        if (s.scale) g = g * scale;
-        m = m * s.b1 + g * s.a1;
-        v = v * s.b2 + g * g * s.a2;
-        w = w * s.keep - s.lr_t * (m / (sqrtf(v) * s.v_t + s.eps));
-        const uint32_t r = random_of((uint64_t)j, s.seed);
-        if (BITS == 8) {
-            const uint32_t mm = in ? magnitude(m) : 0, vm = in ? magnitude(v) : 0;
-            const uint32_t mb = base_of(block_max(mm, red[0]), 15), vb = base_of(block_max(vm, red[1]), 31);
-            uint32_t mc = encode(mm, mb, r >> 16), vc = encode(vm, vb, r & 0xffffu);
-            vc = vc == 0 && vm > 0 ? 1 : vc;
-            ((uint8_t *)s.m)[j] = (uint8_t)(in ? mc | (bits_of(m) >> 24 & 128u) : 0);
-            ((uint8_t *)s.v)[j] = (uint8_t)(in ? vc : 0);
-            if (threadIdx.x == 0) {
-                s.m_base[q] = (uint8_t)mb;
-                s.v_base[q] = (uint8_t)vb;
-            }
-        } else if (in) {
-            ((float *)s.m)[j] = m;
-            ((float *)s.v)[j] = v;
-        }
-        if (!in) continue;
-        if (s.master) {
-            s.master[j] = w;
-            param[i] = (P)w;
+            mc[u] = *(const uint32_t *)((const uint8_t *)s.m + j);
+            vc[u] = *(const uint32_t *)((const uint8_t *)s.v + j);
+            mb[u] = s.m_base[(slot + i0) / GROUP];
+            vb[u] = s.v_base[(slot + i0) / GROUP];
         } else {
-            put(param + i, w, r);
+            // (the state goes on to the end of the group)
+            const float4 a = *(const float4 *)((const float *)s.m + j), b = *(const float4 *)((const float *)s.v + j);
+            m[u][0] = a.x, m[u][1] = a.y, m[u][2] = a.z, m[u][3] = a.w;
+            v[u][0] = b.x, v[u][1] = b.y, v[u][2] = b.z, v[u][3] = b.w;
+        }
+        if (s.master) {
+            const float4 a = *(const float4 *)(s.master + j);
+            w[u][0] = a.x, w[u][1] = a.y, w[u][2] = a.z, w[u][3] = a.w;
+        } else {
+            get(w[u], param, i, n);
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < WAVE_GROUPS; ++u) {
+        const int64_t i0 = begin + u * GROUP, i = i0 + 4 * lane, j = slot + i;
+        if (i0 >= n) break;
+        uint32_t r[4];
+        Pair top = {0, 0};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (BITS == 8) {
+                m[u][e] = decode_m(mc[u] >> 8 * e & 255u, mb[u]);
+                v[u][e] = decode(vc[u] >> 8 * e & 255u, vb[u]);
+            }
+            const float x = s.scale ? g[u][e] * scale : g[u][e];
+            m[u][e] = m[u][e] * s.b1 + x * s.a1;
+            v[u][e] = v[u][e] * s.b2 + x * x * s.a2;
+            w[u][e] = w[u][e] * s.keep - s.lr_t * (m[u][e] / (sqrtf(v[u][e]) * s.v_t + s.eps));
+            r[e] = random_of((uint64_t)(j + e), s.seed);
+            if (BITS == 8 && i + e < n) {
+                const Pair y = {(unsigned short)exponent(magnitude(m[u][e])), (unsigned short)exponent(magnitude(v[u][e]))};
+                top = __builtin_elementwise_max(top, y);
+            }
+        }
+        if (BITS == 8) {
+            top = wave_max(top);
+            const uint32_t mbase = base_of(top.x, 15), vbase = base_of(top.y, 31);
+            uint32_t a = 0, b = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t vm = magnitude(v[u][e]);
+                uint32_t x = encode(magnitude(m[u][e]), mbase, r[e] >> 16) | (bits_of(m[u][e]) >> 24 & 128u);
+                uint32_t y = encode(vm, vbase, r[e] & 0xffffu);
+                y = y == 0 && vm > 0 ? 1 : y;
+                if (i + e >= n) x = y = 0;
+                a |= x << 8 * e;
+                b |= y << 8 * e;
+            }
+            *(uint32_t *)((uint8_t *)s.m + j) = a;
+            *(uint32_t *)((uint8_t *)s.v + j) = b;
+            if (lane == 0) {
+                s.m_base[(slot + i0) / GROUP] = (uint8_t)mbase;
+                s.v_base[(slot + i0) / GROUP] = (uint8_t)vbase;
+            }
+        } else {
+            *(float4 *)((float *)s.m + j) = make_float4(m[u][0], m[u][1], m[u][2], m[u][3]);
+            *(float4 *)((float *)s.v + j) = make_float4(v[u][0], v[u][1], v[u][2], v[u][3]);
+        }
+        if (s.master) *(float4 *)(s.master + j) = make_float4(w[u][0], w[u][1], w[u][2], w[u][3]);
+        Span<P, 4> o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (s.master) o.e[e] = (P)w[u][e];
+            else o.e[e] = rounded<P>(w[u][e], r[e]);
+        }
+        if (i + 4 <= n) {
+            *(Span<P, 4> *)(param + i) = o;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (i + e < n) param[i + e] = o.e[e];
         }
     }
 }
 
+// A thread writes four neighbouring elements of each moment, so that a wave writes whole lines.
 __global__ __launch_bounds__(BLOCK) void k_unpack(int64_t groups, const uint8_t *m, const uint8_t *v,
                                                   const uint8_t *m_base, const uint8_t *v_base,
                                                   float *avg, float *sq)
 {
-    for (int64_t q = blockIdx.x; q < groups; q += gridDim.x) {
-        const int64_t j = q * GROUP + threadIdx.x;
-        avg[j] = decode_m(m[j], m_base[q]);
-        sq[j] = decode(v[j], v_base[q]);
+    const int lane = threadIdx.x & 63;
+    for (int64_t q = (int64_t)blockIdx.x * (BLOCK / 64) + (threadIdx.x >> 6); q < groups;
+         q += (int64_t)gridDim.x * (BLOCK / 64)) {
+        const int64_t j = q * GROUP + 4 * lane;
+        const uint32_t a = *(const uint32_t *)(m + j), b = *(const uint32_t *)(v + j);
+        const uint32_t mb = m_base[q], vb = v_base[q];
+        *(float4 *)(avg + j) = make_float4(decode_m(a & 255u, mb), decode_m(a >> 8 & 255u, mb),
+                                           decode_m(a >> 16 & 255u, mb), decode_m(a >> 24, mb));
+        *(float4 *)(sq + j) = make_float4(decode(b & 255u, vb), decode(b >> 8 & 255u, vb),
+                                          decode(b >> 16 & 255u, vb), decode(b >> 24, vb));
     }
 }
 
@@ -193,9 +266,12 @@ __global__ __launch_bounds__(BLOCK) void k_norm(const Tensors t, uint32_t chunks
         const int64_t begin = (int64_t)(c - t.first[k]) * CHUNK;
         const int64_t end = begin + CHUNK < t.n[k] ? begin + CHUNK : t.n[k];
         float part = 0;
-        for (int64_t i = begin + threadIdx.x; i < end; i += BLOCK) {
-            const float g = (float)grad[i];
-            part += g * g;
+#pragma unroll
+        for (int u = 0; u < CHUNK / (4 * BLOCK); ++u) {
+            const int64_t i = begin + (u * BLOCK + threadIdx.x) * 4;
+            float g[4];
+            get(g, grad, i, end);
+            part += g[0] * g[0] + g[1] * g[1] + (g[2] * g[2] + g[3] * g[3]);
         }
         s += part;
     }
@@ -345,8 +421,9 @@ int swarp_adamw_unpack(const swarp_adamw_t *a, float *avg, float *sq, void *stre
     if (a->bits != 8) return fail("only 8-bit moments are unpacked");
     if (a->state_len == 0) return 0;
     if (!avg || !sq) return fail("pointer arguments must be set");
+    if (((uintptr_t)avg | (uintptr_t)sq) & 15u) return fail("avg and sq must be 16-byte aligned");
     const int64_t groups = a->state_len / GROUP;
-    hipLaunchKernelGGL(k_unpack, dim3((unsigned)(groups < 16384 ? groups : 16384)), dim3(BLOCK), 0,
+    hipLaunchKernelGGL(k_unpack, dim3((unsigned)(groups < 65536 ? (groups + 3) / 4 : 16384)), dim3(BLOCK), 0,
                        (hipStream_t)stream, groups, (const uint8_t *)a->exp_avg,
                        (const uint8_t *)a->exp_avg_sq, (const uint8_t *)a->avg_base,
                        (const uint8_t *)a->sq_base, avg, sq);
