@@ -453,8 +453,7 @@ typedef struct swarp_policy {
     int32_t width;            /* actions of a categorical head, dimensions of a Gaussian one */
     int32_t actions32;        /* categorical: actions are int32 (0: int64) */
     int32_t shared_std;
-    int32_t skip_unit;        /* 1: nothing is written where *scale is 1 (see below) */
-    int32_t counted;          /* 1: work holds the mask's counts from an earlier call */
+    int32_t skip_unit, counted; /* 0 (set by the _bwd calls) */
     int64_t rows;
     int64_t inner, outer_stride, inner_stride;
     double clip_low, clip_high, kl_coef, entropy_coef;
@@ -470,17 +469,22 @@ typedef struct swarp_policy {
                                  kl and whether the clip was active; or NULL */
     void *d_head;             /* [rows, width] contiguous, or NULL: no gradient */
     void *d_log_std;          /* as log_std, or NULL */
-    const void *scale;        /* [1] on the device: the gradients are times this; NULL: 1 */
+    const void *scale;        /* NULL (set by the _bwd calls) */
     void *work;               /* swarp_policy_work_bytes(rows, width) bytes, 16-byte aligned */
     uint64_t work_bytes;
 } swarp_policy_t;
-/* A forward with the gradient writes logp, loss, stats and the gradients for an upstream
- * gradient of 1.  The backward is the same call on the same work with logp, loss and stats NULL,
- * counted = 1, scale the upstream gradient and skip_unit = 1 into the same buffers: where the upstream gradient is 1 they are right as they
- * stand, else they are computed again with it.  Which it is, the device decides. */
+/* A forward with d_head or d_log_std writes logp, loss, stats and the gradients for an upstream
+ * gradient of 1.  The _bwd calls, on the arguments and the work of a forward, write the gradients
+ * for the upstream gradient *scale.  With skip_unit = 1 the buffers hold what the forward wrote:
+ * where *scale is 1 they are right as they stand, else they are computed again with it.  Which it
+ * is, the device decides. */
 uint64_t swarp_policy_work_bytes(int64_t rows, int32_t width);
 int swarp_categorical_loss(const swarp_policy_t *a, void *stream);
 int swarp_gaussian_loss(const swarp_policy_t *a, void *stream);
+int swarp_categorical_loss_bwd(const swarp_policy_t *a, int32_t skip_unit, const void *scale,
+                               void *stream);
+int swarp_gaussian_loss_bwd(const swarp_policy_t *a, int32_t skip_unit, const void *scale,
+                            void *stream);
 
 /* One tensor of an optimizer step: n elements, whose moments start at element `slot` (a
  * multiple of SWARP_ADAMW_GROUP) of the flat state. */

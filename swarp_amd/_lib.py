@@ -274,6 +274,14 @@ SIGNATURES = {
     "swarp_policy_work_bytes": ([ctypes.c_int64, ctypes.c_int32], ctypes.c_uint64),
     "swarp_categorical_loss": ([ctypes.POINTER(SwarpPolicy), ctypes.c_void_p], ctypes.c_int),
     "swarp_gaussian_loss": ([ctypes.POINTER(SwarpPolicy), ctypes.c_void_p], ctypes.c_int),
+    "swarp_categorical_loss_bwd": (
+        [ctypes.POINTER(SwarpPolicy), ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p],
+        ctypes.c_int,
+    ),
+    "swarp_gaussian_loss_bwd": (
+        [ctypes.POINTER(SwarpPolicy), ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p],
+        ctypes.c_int,
+    ),
     "swarp_adamw": (
         [ctypes.POINTER(SwarpAdamW), ctypes.POINTER(SwarpTensor), ctypes.c_int32, ctypes.c_void_p],
         ctypes.c_int,

@@ -62,10 +62,12 @@ __device__ __forceinline__ uint32_t mix(uint32_t x)
     x *= 0xA54FF53Bu;
     return x ^ (x >> 16);
 }
-// 32 random bits of element i of the flat state.
-__device__ __forceinline__ uint32_t random_of(uint64_t i, uint32_t seed)
+// 32 random bits of element i of the flat state are mix(place_of(i, seed)); i + 1 of the same 2^32
+// is a PLACE further.
+constexpr uint32_t PLACE = 0x9E3779B1u;
+__device__ __forceinline__ uint32_t place_of(uint64_t i, uint32_t seed)
 {
-    return mix((uint32_t)i * 0x9E3779B1u + seed + (uint32_t)(i >> 32) * 0x3C6EF373u);
+    return (uint32_t)i * PLACE + seed + (uint32_t)(i >> 32) * 0x3C6EF373u;
 }
 
 __device__ __forceinline__ uint32_t bits_of(float x) { return (uint32_t)__float_as_int(x); }
@@ -80,12 +82,12 @@ __device__ __forceinline__ uint32_t magnitude(float x)
 }
 __device__ __forceinline__ uint32_t encode(uint32_t mag, uint32_t base, uint32_t r16)
 {
-    const uint32_t k = (mag + (r16 << 4 | 8u)) >> 20, low = base << 3;
-    return k > low ? k - low : 0;
+    const int k = (int)((mag + (r16 << 4 | 8u)) >> 20) - (int)(base << 3);
+    return (uint32_t)(k > 0 ? k : 0);
 }
 __device__ __forceinline__ float decode(uint32_t q, uint32_t base)
 {
-    return q ? float_of((q + (base << 3)) << 20) : 0.0f;
+    return float_of(((q + (base << 3)) << 20) & (q ? 0xffffffffu : 0u));
 }
 __device__ __forceinline__ float decode_m(uint32_t c, uint32_t base)
 {
@@ -105,14 +107,12 @@ __device__ __forceinline__ Pair wave_max(Pair e)
 }
 __device__ __forceinline__ uint32_t exponent(uint32_t mag) { return (mag + 0xfffffu) >> 23; }
 
-// A parameter without a master copy: bfloat16 at random, in proportion (infinities and NaN are
-// cut).
+// A parameter without a master copy: bfloat16 at random, in proportion (a NaN stays one).
 template <typename P> __device__ __forceinline__ P rounded(float x, uint32_t r)
 {
-    if constexpr (sizeof(P) == 2 && __is_same(P, bf16)) {
-        const uint32_t b = bits_of(x);
-        const bool finite = (b & 0x7f800000u) != 0x7f800000u;
-        return finite ? __builtin_bit_cast(bf16, (uint16_t)((b + (mix(r) & 0xffffu)) >> 16)) : (bf16)x;
+    if constexpr (__is_same(P, bf16)) {
+        const uint32_t b = x != x ? 0x7fc00000u : bits_of(x);
+        return __builtin_bit_cast(bf16, (uint16_t)((b + (mix(r) & 0xffffu)) >> 16));
     } else {
         return (P)x;
     }
@@ -137,6 +137,12 @@ template <typename T> __device__ __forceinline__ void get(float (&x)[4], const T
 // A workgroup takes a chunk of a tensor, a wave four groups of it, a thread four neighbouring
 // elements of each group: all loads of the four groups are in flight before the first is used,
 // and a group's largest exponents are found without LDS or barriers.
+struct Yes {
+    constexpr operator bool() const { return true; }
+};
+struct No {
+    constexpr operator bool() const { return false; }
+};
 constexpr int WAVE_GROUPS = CHUNK / GROUP / (BLOCK / 64);
 
 template <typename P, typename G, int BITS>
@@ -174,14 +180,15 @@ __global__ __launch_bounds__(BLOCK) void k_adamw(const Step s, const Tensors t)
             get(w[u], param, i, n);
         }
     }
-#pragma unroll
-    for (int u = 0; u < WAVE_GROUPS; ++u) {
+    // One group, whose last elements may be past the tensor's end where it is not `whole`.
+    const auto one = [&](int u, auto whole) {
         const int64_t i0 = begin + u * GROUP, i = i0 + 4 * lane, j = slot + i;
-        if (i0 >= n) break;
         uint32_t r[4];
         Pair top = {0, 0};
+        const uint32_t place = place_of((uint64_t)j, s.seed);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
+            const bool in = whole || i + e < n;
             if (BITS == 8) {
                 m[u][e] = decode_m(mc[u] >> 8 * e & 255u, mb[u]);
                 v[u][e] = decode(vc[u] >> 8 * e & 255u, vb[u]);
@@ -189,11 +196,14 @@ __global__ __launch_bounds__(BLOCK) void k_adamw(const Step s, const Tensors t)
             const float x = s.scale ? g[u][e] * scale : g[u][e];
             m[u][e] = m[u][e] * s.b1 + x * s.a1;
             v[u][e] = v[u][e] * s.b2 + x * x * s.a2;
-            w[u][e] = w[u][e] * s.keep - s.lr_t * (m[u][e] / (sqrtf(v[u][e]) * s.v_t + s.eps));
-            r[e] = random_of((uint64_t)(j + e), s.seed);
-            if (BITS == 8 && i + e < n) {
+            // (the root and the quotient to an ulp or two: a fraction of an update that is itself a
+            // thousandth of the parameter; the moments, which accumulate, are exact)
+            const float den = __builtin_amdgcn_sqrtf(v[u][e]) * s.v_t + s.eps;
+            w[u][e] = w[u][e] * s.keep - s.lr_t * (m[u][e] * __builtin_amdgcn_rcpf(den));
+            r[e] = mix(place + (uint32_t)e * PLACE);
+            if (BITS == 8) {
                 const Pair y = {(unsigned short)exponent(magnitude(m[u][e])), (unsigned short)exponent(magnitude(v[u][e]))};
-                top = __builtin_elementwise_max(top, y);
+                if (in) top = __builtin_elementwise_max(top, y);
             }
         }
         if (BITS == 8) {
@@ -203,12 +213,13 @@ __global__ __launch_bounds__(BLOCK) void k_adamw(const Step s, const Tensors t)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const uint32_t vm = magnitude(v[u][e]);
-                uint32_t x = encode(magnitude(m[u][e]), mbase, r[e] >> 16) | (bits_of(m[u][e]) >> 24 & 128u);
-                uint32_t y = encode(vm, vbase, r[e] & 0xffffu);
-                y = y == 0 && vm > 0 ? 1 : y;
-                if (i + e >= n) x = y = 0;
-                a |= x << 8 * e;
-                b |= y << 8 * e;
+                const uint32_t x = encode(magnitude(m[u][e]), mbase, r[e] >> 16) | (bits_of(m[u][e]) >> 24 & 128u);
+                const uint32_t c = encode(vm, vbase, r[e] & 0xffffu), least = vm > 0 ? 1u : 0u;
+                const uint32_t y = c > least ? c : least;
+                if (whole || i + e < n) {
+                    a |= x << 8 * e;
+                    b |= y << 8 * e;
+                }
             }
             *(uint32_t *)((uint8_t *)s.m + j) = a;
             *(uint32_t *)((uint8_t *)s.v + j) = b;
@@ -220,20 +231,29 @@ __global__ __launch_bounds__(BLOCK) void k_adamw(const Step s, const Tensors t)
             *(float4 *)((float *)s.m + j) = make_float4(m[u][0], m[u][1], m[u][2], m[u][3]);
             *(float4 *)((float *)s.v + j) = make_float4(v[u][0], v[u][1], v[u][2], v[u][3]);
         }
-        if (s.master) *(float4 *)(s.master + j) = make_float4(w[u][0], w[u][1], w[u][2], w[u][3]);
         Span<P, 4> o;
+        if (s.master) {
+            *(float4 *)(s.master + j) = make_float4(w[u][0], w[u][1], w[u][2], w[u][3]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if (s.master) o.e[e] = (P)w[u][e];
-            else o.e[e] = rounded<P>(w[u][e], r[e]);
+            for (int e = 0; e < 4; ++e) o.e[e] = (P)w[u][e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o.e[e] = rounded<P>(w[u][e], r[e]);
         }
-        if (i + 4 <= n) {
+        if (whole || i + 4 <= n) {
             *(Span<P, 4> *)(param + i) = o;
         } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 if (i + e < n) param[i + e] = o.e[e];
         }
+    };
+#pragma unroll
+    for (int u = 0; u < WAVE_GROUPS; ++u) {
+        const int64_t i0 = begin + u * GROUP;
+        if (i0 >= n) break;
+        if (i0 + GROUP <= n) one(u, Yes());
+        else one(u, No());
     }
 }
 

@@ -192,7 +192,8 @@ __device__ __forceinline__ int64_t action_of(const Logits &g, int64_t i)
     return g.actions32 ? (int64_t)((const int32_t *)g.actions)[i] : ((const int64_t *)g.actions)[i];
 }
 
-// What the gradient of a row needs.
+// What the gradient of a row needs; `at`: where its action lies, below 0 if nowhere (its terms are
+// NaN then, and so are c2 and the row).
 template <typename A> struct Slope {
     A m, c1, c2, gw;
     int64_t at;
@@ -210,10 +211,11 @@ __device__ __forceinline__ Slope<A> slope_of(const Row<A> &r, const Logits &g, i
     lp = in ? (xa - m) - ls * A(LN_2) : A(NAN);
     const A gw = decide(r, i, lp, in ? H : A(NAN), t) * w;
     const A ew = r.entc * w;
-    return {m, ew * A(LN_2) * inv, (ew * (H - ls * A(LN_2)) - gw) * inv, in ? gw : A(NAN), in ? at : -1};
+    return {m, ew * A(LN_2) * inv, (ew * (H - ls * A(LN_2)) - gw) * inv, gw, in ? at : -1};
 }
 
-template <typename A> __device__ __forceinline__ A max_of(A a, A b) { return a > b ? a : b; }
+// The larger of x and m; m where x is NaN.
+template <typename A> __device__ __forceinline__ A max_of(A x, A m) { return x > m ? x : m; }
 __device__ __forceinline__ float fma_of(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
 __device__ __forceinline__ double fma_of(double a, double b, double c) { return __builtin_fma(a, b, c); }
 
@@ -350,6 +352,7 @@ template <typename T, int LANES, int E> struct Held {
                 v[i][k] = lane < left ? v[i][k] : (lane == left ? last.w[k] : low);
             }
         }
+        forget();
     }
     __device__ __forceinline__ A most() const
     {
@@ -411,10 +414,6 @@ template <typename T, int LANES, int E> struct Held {
                 const int at = (int)c.at % VEC;
 #pragma unroll
                 for (int k = 0; k < VEC; ++k) y[k] += k == at ? c.gw : A(0);
-            }
-            if (c.at < 0) {
-#pragma unroll
-                for (int k = 0; k < VEC; ++k) y[k] = c.gw;
             }
             Words<T>::set(v[i], y);
             put(d, lane, i, full, rem);
@@ -546,7 +545,7 @@ template <int THREADS, typename A> __device__ __forceinline__ void block_sums(A 
 
 // Longer rows, up to THREADS * E elements: a workgroup a row.
 template <typename T, int THREADS, int E>
-__global__ __launch_bounds__(THREADS, E * sizeof(T) >= 256 ? 4 : 1) void k_cat_block(const Row<typename Acc<T>::type> r, const Logits g)
+__global__ __launch_bounds__(THREADS, sizeof(T) < 8 && E * sizeof(T) >= 256 ? 4 : 1) void k_cat_block(const Row<typename Acc<T>::type> r, const Logits g)
 {
     typedef typename Acc<T>::type A;
     __shared__ A red_m[THREADS / 64], red_s[THREADS / 64][2];
@@ -720,7 +719,7 @@ __global__ __launch_bounds__(BLOCK) void k_cat_rows(const Row<typename Acc<T>::t
             for (int k = 0; k < N; ++k)
                 if (k < V) {
                     z[k] = up(own[k]);
-                    m = z[k] > m ? z[k] : m;
+                    m = max_of(z[k], m);
                 }
             const A xa = up(own[in ? at : 0]);
 #pragma unroll
@@ -736,7 +735,9 @@ __global__ __launch_bounds__(BLOCK) void k_cat_rows(const Row<typename Acc<T>::t
             if (g.d) {
 #pragma unroll
                 for (int k = 0; k < N; ++k)
-                    if (k < V) own[k] = (T)(c.at < 0 ? c.gw : B::exp(z[k]) * fma_of(c.c1, B::floor(z[k]), c.c2) + (k == c.at ? c.gw : A(0)));
+                    if (k < V) own[k] = (T)(B::exp(z[k]) * fma_of(c.c1, B::floor(z[k]), c.c2));
+                const A za = B::z(xa, m);
+                if (in) own[at] = (T)(B::exp(za) * fma_of(c.c1, B::floor(za), c.c2) + c.gw);
             }
         } else if (mine) {
             if (r.logp) r.logp[i] = A(0);
@@ -1179,6 +1180,30 @@ int swarp_gaussian_loss(const swarp_policy_t *a, void *stream)
     if (!a->log_std) return fail("pointer arguments must be set");
     FOR_DTYPE(gaussian, a, st)
     return launched();
+}
+
+static int backward(const swarp_policy_t *a, int32_t skip_unit, const void *scale, swarp_policy_t &b)
+{
+    swarp::set_error("");
+    if (!a || !scale) return fail("arguments must be set");
+    b = *a;
+    b.logp = b.loss = b.stats = nullptr;
+    b.scale = scale;
+    b.skip_unit = skip_unit;
+    b.counted = 1;
+    return 0;
+}
+
+int swarp_categorical_loss_bwd(const swarp_policy_t *a, int32_t skip_unit, const void *scale, void *stream)
+{
+    swarp_policy_t b;
+    return backward(a, skip_unit, scale, b) ? -1 : swarp_categorical_loss(&b, stream);
+}
+
+int swarp_gaussian_loss_bwd(const swarp_policy_t *a, int32_t skip_unit, const void *scale, void *stream)
+{
+    swarp_policy_t b;
+    return backward(a, skip_unit, scale, b) ? -1 : swarp_gaussian_loss(&b, stream);
 }
 
 }  // extern "C"

@@ -54,9 +54,9 @@ def _on_gpu(t: torch.Tensor, what: str) -> None:
                            f"got a tensor on {t.device}")
 
 
-def _same(t: torch.Tensor, name: str, shape, dtype, device) -> torch.Tensor:
+def _same(t: torch.Tensor, name: str, shape: torch.Size, dtype, device) -> torch.Tensor:
     """``t``, contiguous, after checking its shape, type and device."""
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name} must be {list(shape)}; got {list(t.shape)}")
     if t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}; got {t.dtype}")
@@ -72,63 +72,51 @@ def _ptr(t: torch.Tensor | None):
 # ----------------------------------------------------------------------------- advantages
 
 
-class _Scan(NamedTuple):
-    rows: int
-    steps: int
-    columns: int
-    group: int
-    gamma: float
-    lam: float
-
-
-def _scan_args(scan: _Scan, dtype, rewards, values, term, trunc, final) -> _lib.SwarpGae:
+def _scan_args(rows, steps, columns, group, gamma, lam, rewards, values, final, term,
+               trunc) -> _lib.SwarpGae:
     return _lib.SwarpGae(
-        dtype=_CODES[dtype], rows=scan.rows, steps=scan.steps, columns=scan.columns,
-        group=scan.group, gamma=scan.gamma, lam=scan.lam, rewards=_ptr(rewards),
-        values=_ptr(values), terminated=_ptr(term), truncated=_ptr(trunc),
-        final_values=_ptr(final))
+        dtype=_CODES[rewards.dtype], rows=rows, steps=steps, columns=columns, group=group,
+        gamma=gamma, lam=lam, rewards=rewards.data_ptr(), values=values.data_ptr(),
+        terminated=_ptr(term), truncated=_ptr(trunc), final_values=_ptr(final))
 
 
-def _gae_forward(scan: _Scan, rewards, values, final, term, trunc):
+def _gae_forward(a: _lib.SwarpGae, rewards: torch.Tensor, stream: int):
     adv, ret = torch.empty_like(rewards), torch.empty_like(rewards)
-    a = _scan_args(scan, rewards.dtype, rewards, values, term, trunc, final)
     a.advantages, a.returns = adv.data_ptr(), ret.data_ptr()
     with _guard(rewards.device):
-        _lib.check(_lib.load().swarp_gae_fwd(ctypes.byref(a), _lib.stream_of(rewards.device)))
+        _lib.check(_lib.load().swarp_gae_fwd(ctypes.byref(a), stream))
     return adv, ret
 
 
 class _GaeFn(torch.autograd.Function):
-    """The scan as one autograd node; it is linear, so only the flags are kept."""
+    """The scan as one autograd node; it is linear, so only the flags are kept.  autograd runs the
+    backward with the forward's device and stream current."""
 
     @staticmethod
-    def forward(ctx, scan: _Scan, rewards, values, final, term, trunc):
+    def forward(ctx, a: _lib.SwarpGae, stream: int, rewards, values, final, term, trunc):
         ctx.set_materialize_grads(False)
-        ctx.scan = scan
-        ctx.final = final is not None
+        ctx.a, ctx.stream = a, stream
         ctx.like = (rewards.shape, values.shape)
         ctx.save_for_backward(term, trunc)
-        return _gae_forward(scan, rewards, values, final, term, trunc)
+        return _gae_forward(a, rewards, stream)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g_adv, g_ret):
         if g_adv is None and g_ret is None:
-            return (None,) * 6
-        term, trunc = ctx.saved_tensors
+            return (None,) * 7
+        term, trunc = ctx.saved_tensors  # (unchanged since, or this raises)
         g_adv, g_ret = (None if g is None else g.contiguous() for g in (g_adv, g_ret))
         ref = g_adv if g_adv is not None else g_ret
-        need = ctx.needs_input_grad
-        d_r = ref.new_empty(ctx.like[0]) if need[1] else None
-        d_v = ref.new_empty(ctx.like[1]) if need[2] else None
-        d_f = ref.new_empty(ctx.like[0]) if ctx.final and need[3] else None
-        # a final-value buffer is only looked at for being there: the adjoint reads no values
-        a = _scan_args(ctx.scan, ref.dtype, None, None, term, trunc, ref if ctx.final else None)
+        need, (r_shape, v_shape) = ctx.needs_input_grad, ctx.like
+        a = ctx.a  # whose final_values is only looked at for being there
+        d_r = ref.new_empty(r_shape) if need[2] else None
+        d_v = ref.new_empty(v_shape) if need[3] else None
+        d_f = ref.new_empty(r_shape) if a.final_values and need[4] else None
         a.adj_advantages, a.adj_returns = _ptr(g_adv), _ptr(g_ret)
         a.adj_rewards, a.adj_values, a.adj_final_values = _ptr(d_r), _ptr(d_v), _ptr(d_f)
-        with _guard(ref.device):
-            _lib.check(_lib.load().swarp_gae_bwd(ctypes.byref(a), _lib.stream_of(ref.device)))
-        return None, d_r, d_v, d_f, None, None
+        _lib.check(_lib.load().swarp_gae_bwd(ctypes.byref(a), ctx.stream))
+        return None, None, d_r, d_v, d_f, None, None
 
 
 def gae(rewards: torch.Tensor, values: torch.Tensor, terminated: torch.Tensor | None = None,
@@ -161,10 +149,13 @@ def gae(rewards: torch.Tensor, values: torch.Tensor, terminated: torch.Tensor | 
     if not (0.0 <= gamma <= 1.0 and 0.0 <= lam <= 1.0):
         raise ValueError(f"gamma and lam must lie in [0, 1]; got {gamma} and {lam}")
     last = time_dim != 0 and nd > 1
-    shape = tuple(rewards.shape)
+    shape = rewards.shape
     T, batch = (shape[-1], shape[:-1]) if last else (shape[0], shape[1:])
+
+    def timed(steps, lead):
+        return torch.Size((*lead, steps) if last else (steps, *lead))
     rewards = _same(rewards, "rewards", shape, dtype, dev)
-    values = _same(values, "values", (*batch, T + 1) if last else (T + 1, *batch), dtype, dev)
+    values = _same(values, "values", timed(T + 1, batch), dtype, dev)
     if final_values is not None:
         final_values = _same(final_values, "final_values", shape, dtype, dev)
     if terminated is not None and truncated is not None and terminated.shape != truncated.shape:
@@ -174,65 +165,31 @@ def gae(rewards: torch.Tensor, values: torch.Tensor, terminated: torch.Tensor | 
     for n, name in enumerate(("terminated", "truncated")):
         if flags[n] is not None:
             k = max(flags[n].dim() - 1, 0)
-            lead = batch[:k]
-            flags[n] = _same(flags[n], name, (*lead, T) if last else (T, *lead), torch.bool, dev)
+            flags[n] = _same(flags[n], name, timed(T, batch[:k]), torch.bool, dev)
             group = math.prod(batch[k:])
-    scan = _Scan(int(last), T, math.prod(batch), max(group, 1), float(gamma), float(lam))
     inputs = (rewards, values, final_values)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs):
-        return Advantages(*_GaeFn.apply(scan, *inputs, *flags))
-    return Advantages(*_gae_forward(scan, *inputs, *flags))
+    a = _scan_args(int(last), T, math.prod(batch), max(group, 1), gamma, lam, *inputs, *flags)
+    stream = _lib.stream_of(dev)
+    if torch.is_grad_enabled() and (rewards.requires_grad or values.requires_grad or (
+            final_values is not None and final_values.requires_grad)):
+        return Advantages(*_GaeFn.apply(a, stream, *inputs, *flags))
+    return Advantages(*_gae_forward(a, rewards, stream))
 
 
 # ------------------------------------------------------------------------- policy losses
 
 
-class _Loss(NamedTuple):
-    """The constants of a call (everything that is not a tensor)."""
-
-    gaussian: bool
-    rows: int
-    width: int
-    strides: tuple[int, int, int]
-    clip: tuple[float, float]
-    kl_coef: float
-    entropy_coef: float
-    sum: bool
-
-
-def _loss_args(c: _Loss, head, log_std, actions, old, adv, ref, mask):
-    """The C arguments of a call, without its results, and the work memory they point to."""
-    nbytes = _lib.load().swarp_policy_work_bytes(c.rows, c.width)
-    work = torch.empty(nbytes, dtype=torch.uint8, device=head.device)
-    a = _lib.SwarpPolicy(
-        dtype=_CODES[head.dtype], sum=c.sum, width=c.width,
-        actions32=actions.dtype == torch.int32,
-        shared_std=log_std is not None and log_std.dim() == 1 and head.dim() > 1,
-        rows=c.rows, inner=c.strides[0], outer_stride=c.strides[1], inner_stride=c.strides[2],
-        clip_low=c.clip[0], clip_high=c.clip[1], kl_coef=c.kl_coef, entropy_coef=c.entropy_coef,
-        head=head.data_ptr(), log_std=_ptr(log_std), actions=actions.data_ptr(),
-        old_logp=old.data_ptr(), advantages=adv.data_ptr(), ref_logp=_ptr(ref), mask=_ptr(mask),
-        work=work.data_ptr(), work_bytes=nbytes)
-    return a, work
-
-
-def _loss_launch(c: _Loss, a: _lib.SwarpPolicy, dev) -> None:
-    lib = _lib.load()
-    call = lib.swarp_gaussian_loss if c.gaussian else lib.swarp_categorical_loss
-    with _guard(dev):
-        _lib.check(call(ctypes.byref(a), _lib.stream_of(dev)))
-
-
-def _loss_forward(c: _Loss, head, log_std, rest, made=(None, None)):
-    """(loss, stats, logp) of a call, its arguments and its work memory; ``made`` are gradient
-    buffers to fill on the way."""
-    a, work = _loss_args(c, head, log_std, *rest)
-    old = rest[1]
+def _loss_forward(call, a: _lib.SwarpPolicy, head, old, stream: int):
+    """(loss, stats, logp) of a call, and its work memory."""
+    dev = head.device
+    nbytes = _lib.load().swarp_policy_work_bytes(a.rows, a.width)
+    work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     loss, stats, logp = old.new_empty(()), old.new_empty(3), torch.empty_like(old)
     a.logp, a.loss, a.stats = logp.data_ptr(), loss.data_ptr(), stats.data_ptr()
-    a.d_head, a.d_log_std = _ptr(made[0]), _ptr(made[1])
-    _loss_launch(c, a, head.device)
-    return loss, stats, logp, a, work
+    a.work, a.work_bytes = work.data_ptr(), nbytes
+    with _guard(dev):
+        _lib.check(call(ctypes.byref(a), stream))
+    return loss, stats, logp, work
 
 
 def _buffers(head, log_std, need):
@@ -252,15 +209,15 @@ class _LossFn(torch.autograd.Function):
     """
 
     @staticmethod
-    def forward(ctx, c: _Loss, head, log_std, *rest):
+    def forward(ctx, calls, a: _lib.SwarpPolicy, stream: int, head, log_std, *rest):
         ctx.set_materialize_grads(False)
-        ctx.c = c
-        ctx.need = ctx.needs_input_grad[1:3]
+        ctx.call = (calls[1], a, stream)
+        ctx.need = ctx.needs_input_grad[3:5]
         ctx.made = None
         if head.dtype != torch.float16:
             ctx.made = _buffers(head, log_std, ctx.need)
-        loss, stats, logp, *ctx.call = _loss_forward(c, head, log_std, rest,
-                                                     ctx.made or (None, None))
+            a.d_head, a.d_log_std = _ptr(ctx.made[0]), _ptr(ctx.made[1])
+        loss, stats, logp, ctx.work = _loss_forward(calls[0], a, head, rest[1], stream)
         ctx.save_for_backward(head, log_std, *rest)
         ctx.mark_non_differentiable(stats, logp)
         return loss, stats, logp
@@ -269,16 +226,18 @@ class _LossFn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, g, *_):
         if g is None:
-            return (None,) * 8
-        head, log_std = ctx.saved_tensors[:2]  # (unchanged since, or this raises)
+            return (None,) * 10
+        saved = ctx.saved_tensors  # (unchanged since, or this raises)
+        call, a, stream = ctx.call
         made, ctx.made = ctx.made, None  # handed out once: the caller may change them
-        d = made or _buffers(head, log_std, ctx.need)
-        a = ctx.call[0]
-        a.logp = a.loss = a.stats = None
-        a.d_head, a.d_log_std, a.scale = _ptr(d[0]), _ptr(d[1]), g.data_ptr()
-        a.skip_unit, a.counted = made is not None, 1
-        _loss_launch(ctx.c, a, head.device)
-        return None, *d, *(None,) * 5
+        if made is None:
+            d = _buffers(saved[0], saved[1], ctx.need)
+            a.d_head, a.d_log_std = _ptr(d[0]), _ptr(d[1])
+            _lib.check(call(ctypes.byref(a), 0, g.data_ptr(), stream))
+            return None, None, None, *d, None, None, None, None, None
+        # (autograd runs this with the forward's device and stream current)
+        _lib.check(call(ctypes.byref(a), 1, g.data_ptr(), stream))
+        return None, None, None, *made, None, None, None, None, None
 
 
 def _clip_of(clip) -> tuple[float, float]:
@@ -303,12 +262,27 @@ def _per_row(lead, dtype, dev, old_logp, advantages, ref_logp, mask):
     return (*out, mask)
 
 
-def _evaluate(c: _Loss, head, log_std, *rest) -> PolicyLoss:
+def _evaluate(gaussian: bool, width: int, strides, clip, coefs, head, log_std, actions, old, adv,
+              ref, mask) -> PolicyLoss:
+    lib = _lib.load()
+    stream = _lib.stream_of(head.device)
+    (low, high), (kl_c, ent_c, total) = clip, coefs
+    a = _lib.SwarpPolicy(
+        dtype=_CODES[head.dtype], sum=total, width=width,
+        actions32=actions.dtype == torch.int32,
+        shared_std=gaussian and log_std.dim() == 1 and head.dim() > 1,
+        rows=old.numel(), inner=strides[0], outer_stride=strides[1], inner_stride=strides[2],
+        clip_low=low, clip_high=high, kl_coef=kl_c, entropy_coef=ent_c,
+        head=head.data_ptr(), log_std=_ptr(log_std), actions=actions.data_ptr(),
+        old_logp=old.data_ptr(), advantages=adv.data_ptr(), ref_logp=_ptr(ref), mask=_ptr(mask))
+    calls = ((lib.swarp_gaussian_loss, lib.swarp_gaussian_loss_bwd) if gaussian else
+             (lib.swarp_categorical_loss, lib.swarp_categorical_loss_bwd))
     if torch.is_grad_enabled() and (head.requires_grad
-                                    or (log_std is not None and log_std.requires_grad)):
-        loss, stats, logp = _LossFn.apply(c, head, log_std, *rest)
+                                    or (gaussian and log_std.requires_grad)):
+        loss, stats, logp = _LossFn.apply(calls, a, stream, head, log_std, actions, old, adv, ref,
+                                          mask)
     else:
-        loss, stats, logp = _loss_forward(c, head, log_std, rest)[:3]
+        loss, stats, logp = _loss_forward(calls[0], a, head, old, stream)[:3]
     return PolicyLoss(loss, logp, *stats.unbind(0))
 
 
@@ -323,6 +297,8 @@ def _coefs(kl_coef, entropy_coef, reduction):
 def _row_strides(x: torch.Tensor):
     """(inner, outer stride, inner stride) of the rows of ``x [*lead, V]``, or None where two
     levels of strides do not reach them."""
+    if x.is_contiguous():
+        return max(x.numel() // x.shape[-1], 1), 0, x.shape[-1]
     if x.shape[-1] > 1 and x.stride(-1) != 1:
         return None
     dims: list[list[int]] = []  # [size, stride], outermost first, neighbours merged
@@ -375,18 +351,17 @@ def categorical_policy_loss(
         raise ValueError(f"logits must be [*lead, V] with V >= 1; got {list(logits.shape)}")
     if actions.dtype not in (torch.int64, torch.int32):
         raise TypeError(f"actions must be int64 or int32; got {actions.dtype}")
-    lead, dev = tuple(logits.shape[:-1]), logits.device
+    lead, dev = logits.shape[:-1], logits.device
     wide = torch.float64 if logits.dtype == torch.float64 else torch.float32
     actions = _same(actions, "actions", lead, actions.dtype, dev)
     rest = _per_row(lead, wide, dev, old_logp, advantages, ref_logp, mask)
     low_high = _clip_of(clip)
-    kl_c, ent_c, total = _coefs(kl_coef, entropy_coef, reduction)
+    coefs = _coefs(kl_coef, entropy_coef, reduction)
     strides = _row_strides(logits)
     if strides is None:
         logits = logits.contiguous()
         strides = _row_strides(logits)
-    c = _Loss(False, math.prod(lead), logits.shape[-1], strides, low_high, kl_c, ent_c, total)
-    return _evaluate(c, logits, None, actions, *rest)
+    return _evaluate(False, logits.shape[-1], strides, low_high, coefs, logits, None, actions, *rest)
 
 
 def gaussian_policy_loss(
@@ -409,7 +384,7 @@ def gaussian_policy_loss(
         raise TypeError(f"mean must be float32, float64, bfloat16 or float16; got {mean.dtype}")
     if mean.dim() < 1 or not 1 <= mean.shape[-1] <= 64:
         raise ValueError(f"mean must be [*lead, D] with 1 <= D <= 64; got {list(mean.shape)}")
-    D, lead, dev = mean.shape[-1], tuple(mean.shape[:-1]), mean.device
+    D, lead, dev = mean.shape[-1], mean.shape[:-1], mean.device
     if log_std.dtype != mean.dtype:
         raise TypeError(f"log_std must be {mean.dtype} as mean is; got {log_std.dtype}")
     if log_std.device != dev:
@@ -425,6 +400,6 @@ def gaussian_policy_loss(
     if actions.requires_grad:
         raise ValueError("actions requires grad, but the loss treats it as a constant: detach it")
     rest = _per_row(lead, wide, dev, old_logp, advantages, ref_logp, mask)
-    kl_c, ent_c, total = _coefs(kl_coef, entropy_coef, reduction)
-    c = _Loss(True, math.prod(lead), D, (1, 0, 0), _clip_of(clip), kl_c, ent_c, total)
-    return _evaluate(c, mean.contiguous(), log_std.contiguous(), actions, *rest)
+    coefs = _coefs(kl_coef, entropy_coef, reduction)
+    return _evaluate(True, D, (1, 0, 0), _clip_of(clip), coefs, mean.contiguous(),
+                     log_std.contiguous(), actions, *rest)

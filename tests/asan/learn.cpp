@@ -207,12 +207,9 @@ template <typename T> int check_cat(int outer, int inner, int V, int pad, bool m
     a.work_bytes = wb;
     if (swarp_categorical_loss(&a, nullptr)) return printf("cat refused: %s\n", swarp::message.c_str()), 1;
     // the backward with an upstream gradient of -2 into another buffer
-    a.logp = a.loss = a.stats = nullptr;
     a.d_head = d2.p;
     scale[0] = (A)-2;
-    a.scale = scale.p;
-    a.skip_unit = a.counted = 1;
-    if (swarp_categorical_loss(&a, nullptr)) return printf("cat refused: %s\n", swarp::message.c_str()), 1;
+    if (swarp_categorical_loss_bwd(&a, 1, scale.p, nullptr)) return printf("cat refused: %s\n", swarp::message.c_str()), 1;
     double L = 0, E = 0, K = 0, C = 0, err = 0, gerr = 0, top = 0;
     std::vector<double> want((size_t)n * V, 0.0);
     for (int64_t i = 0; i < n; ++i) {
