@@ -279,6 +279,12 @@ template <typename T, int LANES, int E> struct Held {
     typedef typename Acc<T>::type A;
     typedef Base2<A> B;
     static constexpr int VEC = 16 / sizeof(T), NV = E / VEC;
+    // Few logits a thread: the compiler keeps what it has of one from one use to the next (as a
+    // float, z, 2^z), which saves the second 2^z.  More would not fit the registers: there each use
+    // starts from the words as they were loaded, which the compiler is not to see through, one
+    // span after the other.  (200 M bfloat16 logits in rows of 1000, 32 a thread: kept 166 us, not
+    // kept 188; float32 is the same to 2 %.)
+    static constexpr bool KEEP = E <= (sizeof(T) == 2 ? 32 : 16);
     struct Raw {
         uint32_t w[4];
     };
@@ -323,7 +329,7 @@ template <typename T, int LANES, int E> struct Held {
     __device__ __forceinline__ void load(const T *x, int width, int lane)
     {
         // (the offsets are formed here, row by row, and not kept in registers from row to row)
-        if constexpr (E > 16) asm volatile("" : "+v"(lane));
+        if constexpr (!KEEP) asm volatile("" : "+v"(lane));
         const int full = width / VEC, rem = width % VEC;
         Raw last = {{Words<T>::LOW, Words<T>::LOW_HI, Words<T>::LOW, Words<T>::LOW_HI}};
         if (rem && lane == full % LANES) {
@@ -382,20 +388,16 @@ template <typename T, int LANES, int E> struct Held {
             in_turn();
         }
     }
-    // Up to 16 elements a thread the compiler keeps what it has of a logit from one use to the next
-    // (as a float, z, 2^z).  More would not fit the registers: there each use starts from the
-    // words as they were loaded, which the compiler is not to see through, one span after the
-    // other.
     __device__ __forceinline__ void forget()
     {
-        if constexpr (E > 16) {
+        if constexpr (!KEEP) {
 #pragma unroll
             for (int i = 0; i < NV; ++i) asm volatile("" : "+v"(v[i][0]), "+v"(v[i][1]), "+v"(v[i][2]), "+v"(v[i][3]));
         }
     }
     static __device__ __forceinline__ void in_turn()
     {
-        if constexpr (E > 16) __builtin_amdgcn_sched_barrier(0);
+        if constexpr (!KEEP) __builtin_amdgcn_sched_barrier(0);
     }
     // The gradient row to d.
     __device__ __forceinline__ void slope(const Slope<A> &c, T *d, int width, int lane)
@@ -665,7 +667,8 @@ __global__ __launch_bounds__(BLOCK) void k_cat_join(const Row<typename Acc<T>::t
     if (r.sums) leave_sums<BLOCK>(t, r.sums);
 }
 
-// Rows of up to N <= 32 elements: a thread a row.  A workgroup's rows lie next to each other in
+// Rows of N - 3 to N <= 32 elements, N a multiple of 4 (so that only the last three ask whether they
+// are there): a thread a row.  A workgroup's rows lie next to each other in
 // memory (where the caller's strides say so) and pass through LDS both ways, so that memory sees
 // whole lines; a row's place there has an odd length, which spreads the threads over the banks.
 template <typename T, int N>
@@ -716,26 +719,26 @@ __global__ __launch_bounds__(BLOCK) void k_cat_rows(const Row<typename Acc<T>::t
             const bool in = at >= 0 && at < V;
             A z[N], m = -INFINITY, s = 0, q = 0, lp;
 #pragma unroll
-            for (int k = 0; k < N; ++k)
-                if (k < V) {
-                    z[k] = up(own[k]);
-                    m = max_of(z[k], m);
-                }
+            for (int k = 0; k < N; ++k) {
+                // (a place past the row is another's, and read in vain)
+                z[k] = up(own[k]);
+                if (k > N - 4) z[k] = k < V ? z[k] : A(-INFINITY);
+                m = max_of(z[k], m);
+            }
             const A xa = up(own[in ? at : 0]);
 #pragma unroll
-            for (int k = 0; k < N; ++k)
-                if (k < V) {
-                    const A e = B::exp(B::z(z[k], m));
-                    z[k] = B::z(z[k], m);
-                    s += e;
-                    q = fma_of(e, B::floor(z[k]), q);
-                }
+            for (int k = 0; k < N; ++k) {
+                z[k] = B::z(z[k], m);
+                const A e = B::exp(z[k]);
+                s += e;
+                q = fma_of(e, B::floor(z[k]), q);
+            }
             const Slope<A> c = slope_of(r, g, i, m, s, q, xa, at, w, t, lp);
             if (r.logp) r.logp[i] = lp;
             if (g.d) {
 #pragma unroll
                 for (int k = 0; k < N; ++k)
-                    if (k < V) own[k] = (T)(B::exp(z[k]) * fma_of(c.c1, B::floor(z[k]), c.c2));
+                    if (k <= N - 4 || k < V) own[k] = (T)(B::exp(z[k]) * fma_of(c.c1, B::floor(z[k]), c.c2));
                 const A za = B::z(xa, m);
                 if (in) own[at] = (T)(B::exp(za) * fma_of(c.c1, B::floor(za), c.c2) + c.gw);
             }
@@ -1053,19 +1056,31 @@ template <typename T> void categorical(const swarp_policy_t *a, hipStream_t st)
                 a->head, a->actions, a->d_head, nullptr};
     void *const parts = (char *)a->work + sums_bytes() + counts_bytes() + MOST_BLOCKS * sizeof(double) * MOST_DIMS;
     int blocks = 0;
+    // A thread's share of a short row.  What a decision costs beside its logits is paid by every
+    // lane of its row, so 16-bit logits, of which a line holds twice as many, go 32 to a thread:
+    // 200 M bfloat16 ones in rows of 250 take 192 us, 16 to a thread 237; 100 M float32 ones 178 and
+    // 169.
+    constexpr int E = sizeof(T) == 2 ? 32 : 16;
     if constexpr (sizeof(T) < 8) {
-        if (V <= 8) blocks = cat_rows<T, 8>(r, g, st);
-        else if (V <= 16) blocks = cat_rows<T, 16>(r, g, st);
-        else if (V <= 32) blocks = cat_rows<T, 32>(r, g, st);
+        switch ((V + 3) / 4) {
+        case 1: blocks = cat_rows<T, 4>(r, g, st); break;
+        case 2: blocks = cat_rows<T, 8>(r, g, st); break;
+        case 3: blocks = cat_rows<T, 12>(r, g, st); break;
+        case 4: blocks = cat_rows<T, 16>(r, g, st); break;
+        case 5: blocks = cat_rows<T, 20>(r, g, st); break;
+        case 6: blocks = cat_rows<T, 24>(r, g, st); break;
+        case 7: blocks = cat_rows<T, 28>(r, g, st); break;
+        case 8: blocks = cat_rows<T, 32>(r, g, st); break;
+        }
     }
     if (blocks) {
-    } else if (V <= 64) blocks = cat_lanes<T, 4, 16>(r, g, st);
-    else if (V <= 128) blocks = cat_lanes<T, 8, 16>(r, g, st);
-    else if (V <= 256) blocks = cat_lanes<T, 16, 16>(r, g, st);
-    else if (V <= 512) blocks = cat_lanes<T, 32, 16>(r, g, st);
-    else if (V <= 1024) blocks = cat_lanes<T, 64, 16>(r, g, st);
+    } else if (V <= 64) blocks = cat_lanes<T, 64 / E, E>(r, g, st);
+    else if (V <= 128) blocks = cat_lanes<T, 128 / E, E>(r, g, st);
+    else if (V <= 256) blocks = cat_lanes<T, 256 / E, E>(r, g, st);
+    else if (V <= 512) blocks = cat_lanes<T, 512 / E, E>(r, g, st);
+    else if (V <= 1024) blocks = cat_lanes<T, 1024 / E, E>(r, g, st);
     else if (V <= 2048) blocks = cat_lanes<T, 64, 32>(r, g, st);
-    else if (V <= 4096) blocks = cat_block<T, 256, 16>(r, g, st);
+    else if (V <= 4096) blocks = cat_block<T, 4096 / E, E>(r, g, st);
     else if (V <= 8192) blocks = cat_block<T, 256, 32>(r, g, st);
     else if (r.rows < FEW_ROWS || V > 65536 || sizeof(T) == 8) blocks = cat_parts<T>(r, g, parts, st);
     else if constexpr (sizeof(T) < 8) {
