@@ -19,7 +19,7 @@ using namespace learn;
 
 constexpr int GROUP = SWARP_ADAMW_GROUP;
 constexpr int BLOCK = GROUP;
-constexpr int CHUNK = 16 * GROUP;        // elements of a workgroup
+constexpr int CHUNK = 8 * GROUP;         // elements of a workgroup
 constexpr int MOST_TENSORS = 64;         // of a launch
 constexpr int NORM_BLOCKS = 1024;
 
@@ -87,7 +87,8 @@ __device__ __forceinline__ uint32_t encode(uint32_t mag, uint32_t base, uint32_t
 }
 __device__ __forceinline__ float decode(uint32_t q, uint32_t base)
 {
-    return float_of(((q + (base << 3)) << 20) & (q ? 0xffffffffu : 0u));
+    const uint32_t b = (q + (base << 3)) << 20;
+    return float_of(q ? b : 0u);
 }
 __device__ __forceinline__ float decode_m(uint32_t c, uint32_t base)
 {
@@ -121,22 +122,27 @@ template <typename P> __device__ __forceinline__ P rounded(float x, uint32_t r)
 template <typename T, int N> struct __attribute__((packed, aligned(sizeof(T)))) Span {
     T e[N];
 };
-// Elements i .. i + 3 of n, those there are; 0 for the others.
-template <typename T> __device__ __forceinline__ void get(float (&x)[4], const T *p, int64_t i, int64_t n)
+// The four elements from p[i] on, those below n; 0 for the others.
+template <typename T> __device__ __forceinline__ void get(float (&x)[4], const T *p, uint32_t i, int64_t n)
 {
-    if (i + 4 <= n) {
+    if ((int64_t)i + 4 <= n) {
         const Span<T, 4> y = *(const Span<T, 4> *)(p + i);
 #pragma unroll
         for (int k = 0; k < 4; ++k) x[k] = (float)y.e[k];
     } else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) x[k] = i + k < n ? (float)p[i + k] : 0.0f;
+        for (int k = 0; k < 4; ++k) x[k] = (int64_t)i + k < n ? (float)p[i + k] : 0.0f;
     }
 }
 
-// A workgroup takes a chunk of a tensor, a wave four groups of it, a thread four neighbouring
-// elements of each group: all loads of the four groups are in flight before the first is used,
-// and a group's largest exponents are found without LDS or barriers.
+// A workgroup takes a chunk of a tensor, a wave two groups of it, a thread four neighbouring
+// elements of each group: all loads of both groups are in flight before the first is used, and a
+// group's largest exponents are found without LDS or barriers.  (100 M float32 parameters with two
+// groups a wave 490 us, with four 504; 150 M bfloat16 with 8-bit moments 378 and 405.)
+// What bounds it: 32-bit moments, memory: 28 bytes a parameter at 5.7 TB/s.  8-bit ones, the
+// vector units, which are busy 0.9 of the time: some 80 instructions a parameter, the random
+// bits' multiplications, the root and the reciprocal at a quarter of the rate; 10 bytes a
+// parameter at 4.0 TB/s.
 struct Yes {
     constexpr operator bool() const { return true; }
 };
@@ -152,43 +158,44 @@ __global__ __launch_bounds__(BLOCK) void k_adamw(const Step s, const Tensors t)
     P *const param = (P *)t.param[k];
     const G *const grad = (const G *)t.grad[k];
     const int64_t n = t.n[k], slot = t.slot[k];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int wave = threadIdx.x >> 6;
+    const uint32_t at = 4 * (threadIdx.x & 63);
     const int64_t begin = (int64_t)(blockIdx.x - t.first[k]) * CHUNK + wave * (WAVE_GROUPS * GROUP);
     const float scale = s.scale ? *s.scale : 1.0f;
     float g[WAVE_GROUPS][4], m[WAVE_GROUPS][4], v[WAVE_GROUPS][4], w[WAVE_GROUPS][4];
     uint32_t mc[WAVE_GROUPS], vc[WAVE_GROUPS], mb[WAVE_GROUPS], vb[WAVE_GROUPS];
 #pragma unroll
     for (int u = 0; u < WAVE_GROUPS; ++u) {
-        const int64_t i0 = begin + u * GROUP, i = i0 + 4 * lane, j = slot + i;
+        const int64_t i0 = begin + u * GROUP, j0 = slot + i0;
         if (i0 >= n) break;
-        get(g[u], grad, i, n);
+        get(g[u], grad + i0, at, n - i0);
         if (BITS == 8) {
-            mc[u] = *(const uint32_t *)((const uint8_t *)s.m + j);
-            vc[u] = *(const uint32_t *)((const uint8_t *)s.v + j);
-            mb[u] = s.m_base[(slot + i0) / GROUP];
-            vb[u] = s.v_base[(slot + i0) / GROUP];
+            mc[u] = *(const uint32_t *)((const uint8_t *)s.m + j0 + at);
+            vc[u] = *(const uint32_t *)((const uint8_t *)s.v + j0 + at);
+            mb[u] = s.m_base[j0 / GROUP];
+            vb[u] = s.v_base[j0 / GROUP];
         } else {
             // (the state goes on to the end of the group)
-            const float4 a = *(const float4 *)((const float *)s.m + j), b = *(const float4 *)((const float *)s.v + j);
+            const float4 a = *(const float4 *)((const float *)s.m + j0 + at);
+            const float4 b = *(const float4 *)((const float *)s.v + j0 + at);
             m[u][0] = a.x, m[u][1] = a.y, m[u][2] = a.z, m[u][3] = a.w;
             v[u][0] = b.x, v[u][1] = b.y, v[u][2] = b.z, v[u][3] = b.w;
         }
         if (s.master) {
-            const float4 a = *(const float4 *)(s.master + j);
+            const float4 a = *(const float4 *)(s.master + j0 + at);
             w[u][0] = a.x, w[u][1] = a.y, w[u][2] = a.z, w[u][3] = a.w;
         } else {
-            get(w[u], param, i, n);
+            get(w[u], param + i0, at, n - i0);
         }
     }
     // One group, whose last elements may be past the tensor's end where it is not `whole`.
     const auto one = [&](int u, auto whole) {
-        const int64_t i0 = begin + u * GROUP, i = i0 + 4 * lane, j = slot + i;
-        uint32_t r[4];
-        Pair top = {0, 0};
-        const uint32_t place = place_of((uint64_t)j, s.seed);
+        const int64_t i0 = begin + u * GROUP, j0 = slot + i0;
+        const int left = whole ? GROUP : (int)(n - i0);
+        uint32_t r[4], mt = 0, vt = 0;
+        const uint32_t place = place_of((uint64_t)j0, s.seed) + at * PLACE;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const bool in = whole || i + e < n;
             if (BITS == 8) {
                 m[u][e] = decode_m(mc[u] >> 8 * e & 255u, mb[u]);
                 v[u][e] = decode(vc[u] >> 8 * e & 255u, vb[u]);
@@ -198,54 +205,55 @@ __global__ __launch_bounds__(BLOCK) void k_adamw(const Step s, const Tensors t)
             v[u][e] = v[u][e] * s.b2 + x * x * s.a2;
             // (the root and the quotient to an ulp or two: a fraction of an update that is itself a
             // thousandth of the parameter; the moments, which accumulate, are exact)
-            const float den = __builtin_amdgcn_sqrtf(v[u][e]) * s.v_t + s.eps;
-            w[u][e] = w[u][e] * s.keep - s.lr_t * (m[u][e] * __builtin_amdgcn_rcpf(den));
+            const float den = __builtin_fmaf(__builtin_amdgcn_sqrtf(v[u][e]), s.v_t, s.eps);
+            w[u][e] = __builtin_fmaf(-s.lr_t, m[u][e] * __builtin_amdgcn_rcpf(den), w[u][e] * s.keep);
             r[e] = mix(place + (uint32_t)e * PLACE);
-            if (BITS == 8) {
-                const Pair y = {(unsigned short)exponent(magnitude(m[u][e])), (unsigned short)exponent(magnitude(v[u][e]))};
-                if (in) top = __builtin_elementwise_max(top, y);
+            if (BITS == 8 && (whole || (int)at + e < left)) {
+                const uint32_t a = magnitude(m[u][e]), b = magnitude(v[u][e]);
+                mt = a > mt ? a : mt;
+                vt = b > vt ? b : vt;
             }
         }
         if (BITS == 8) {
-            top = wave_max(top);
+            const Pair top = wave_max(Pair{(unsigned short)exponent(mt), (unsigned short)exponent(vt)});
             const uint32_t mbase = base_of(top.x, 15), vbase = base_of(top.y, 31);
             uint32_t a = 0, b = 0;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const uint32_t vm = magnitude(v[u][e]);
                 const uint32_t x = encode(magnitude(m[u][e]), mbase, r[e] >> 16) | (bits_of(m[u][e]) >> 24 & 128u);
-                const uint32_t c = encode(vm, vbase, r[e] & 0xffffu), least = vm > 0 ? 1u : 0u;
+                const uint32_t c = encode(vm, vbase, r[e] & 0xffffu), least = vm < 1u ? vm : 1u;
                 const uint32_t y = c > least ? c : least;
-                if (whole || i + e < n) {
+                if (whole || (int)at + e < left) {
                     a |= x << 8 * e;
                     b |= y << 8 * e;
                 }
             }
-            *(uint32_t *)((uint8_t *)s.m + j) = a;
-            *(uint32_t *)((uint8_t *)s.v + j) = b;
-            if (lane == 0) {
-                s.m_base[(slot + i0) / GROUP] = (uint8_t)mbase;
-                s.v_base[(slot + i0) / GROUP] = (uint8_t)vbase;
+            *(uint32_t *)((uint8_t *)s.m + j0 + at) = a;
+            *(uint32_t *)((uint8_t *)s.v + j0 + at) = b;
+            if (at == 0) {
+                s.m_base[j0 / GROUP] = (uint8_t)mbase;
+                s.v_base[j0 / GROUP] = (uint8_t)vbase;
             }
         } else {
-            *(float4 *)((float *)s.m + j) = make_float4(m[u][0], m[u][1], m[u][2], m[u][3]);
-            *(float4 *)((float *)s.v + j) = make_float4(v[u][0], v[u][1], v[u][2], v[u][3]);
+            *(float4 *)((float *)s.m + j0 + at) = make_float4(m[u][0], m[u][1], m[u][2], m[u][3]);
+            *(float4 *)((float *)s.v + j0 + at) = make_float4(v[u][0], v[u][1], v[u][2], v[u][3]);
         }
         Span<P, 4> o;
         if (s.master) {
-            *(float4 *)(s.master + j) = make_float4(w[u][0], w[u][1], w[u][2], w[u][3]);
+            *(float4 *)(s.master + j0 + at) = make_float4(w[u][0], w[u][1], w[u][2], w[u][3]);
 #pragma unroll
             for (int e = 0; e < 4; ++e) o.e[e] = (P)w[u][e];
         } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e) o.e[e] = rounded<P>(w[u][e], r[e]);
         }
-        if (whole || i + 4 <= n) {
-            *(Span<P, 4> *)(param + i) = o;
+        if (whole || (int)at + 4 <= left) {
+            *(Span<P, 4> *)(param + i0 + at) = o;
         } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (i + e < n) param[i + e] = o.e[e];
+                if ((int)at + e < left) param[i0 + at + e] = o.e[e];
         }
     };
 #pragma unroll
@@ -290,7 +298,7 @@ __global__ __launch_bounds__(BLOCK) void k_norm(const Tensors t, uint32_t chunks
         for (int u = 0; u < CHUNK / (4 * BLOCK); ++u) {
             const int64_t i = begin + (u * BLOCK + threadIdx.x) * 4;
             float g[4];
-            get(g, grad, i, end);
+            get(g, grad + begin, (uint32_t)(i - begin), end - begin);
             part += g[0] * g[0] + g[1] * g[1] + (g[2] * g[2] + g[3] * g[3]);
         }
         s += part;
