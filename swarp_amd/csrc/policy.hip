@@ -63,9 +63,11 @@ constexpr double LN_2 = 0.69314718055994530942;
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * LOG2E); }
 __device__ __forceinline__ double exp_of(double x) { return exp(x); }
 
-// expm1(e) - e, without the cancellation of small e (the series to e^9 / 9! below 1/2).
+// expm1(e) - e, without the cancellation of small e (the series to e^9 / 9! below 1/2) and without
+// inf - inf where the action taken has no probability left (beside e^80, e is nothing).
 template <typename A> __device__ __forceinline__ A kl_of(A e)
 {
+    if (e > A(80)) return exp_of(e);
     A s = A(1) / A(362880);
     s = s * e + A(1) / A(40320);
     s = s * e + A(1) / A(5040);
@@ -324,8 +326,9 @@ template <typename T, int LANES, int E> struct Held {
         *(Span<T, N> *)x = y;
     }
 
-    // width >= VEC: a thread without a span of its own reads the row's first, so that every load is
-    // in flight at once and into its own registers.
+    // A thread without a span of its own reads the row's first, so that every load is in flight at
+    // once and into its own registers.  The row has a whole span: all but a double's of one element
+    // are wider (33 logits and up of the smaller types; parts are cut so).
     __device__ __forceinline__ void load(const T *x, int width, int lane)
     {
         // (the offsets are formed here, row by row, and not kept in registers from row to row)
@@ -347,7 +350,8 @@ template <typename T, int LANES, int E> struct Held {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const uint32_t at = lane < full - i * LANES ? (uint32_t)(i * LANES + lane) * VEC : 0u;
-            take(i, __builtin_bit_cast(Raw, *(const Span<T, VEC> *)(x + at)));
+            if (sizeof(T) < 8 || full > 0) take(i, __builtin_bit_cast(Raw, *(const Span<T, VEC> *)(x + at)));
+            else take(i, last);
         }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
@@ -1040,7 +1044,7 @@ template <typename T> int cat_parts(const Row<typename Acc<T>::type> &r, Logits 
 {
     g.parts = parts;
     g.part = part_of(g.width, 16 / sizeof(T));
-    g.splits = (g.width + g.part - 1) / g.part;
+    g.splits = (g.width - 1) / g.part + 1;
     const int blocks = blocks_for(r.rows * g.splits);
     hipLaunchKernelGGL((k_cat_parts<T>), dim3(blocks), dim3(BLOCK), 0, st, r, g);
     hipLaunchKernelGGL((k_cat_join<T>), dim3(blocks), dim3(BLOCK), 0, st, r, g);

@@ -347,8 +347,8 @@ def categorical_policy_loss(
     _on_gpu(logits, "categorical_policy_loss")
     if logits.dtype not in _CODES:
         raise TypeError(f"logits must be float32, float64, bfloat16 or float16; got {logits.dtype}")
-    if logits.dim() < 1 or logits.shape[-1] < 1:
-        raise ValueError(f"logits must be [*lead, V] with V >= 1; got {list(logits.shape)}")
+    if logits.dim() < 1 or not 1 <= logits.shape[-1] < 1 << 31:
+        raise ValueError(f"logits must be [*lead, V] with 1 <= V < 2^31; got {list(logits.shape)}")
     if actions.dtype not in (torch.int64, torch.int32):
         raise TypeError(f"actions must be int64 or int32; got {actions.dtype}")
     lead, dev = logits.shape[:-1], logits.device

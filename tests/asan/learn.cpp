@@ -423,6 +423,8 @@ int main()
         fails += check_cat<learn::bf16>(2, 7, V, V % 2, V % 3 == 0, true, V > 2, 1, 2e-6, 6e-3);
     for (int V : {3, 33, 600}) fails += check_cat<learn::f16>(2, 3, V, 3, true, true, true, 0, 2e-6, 2e-3);
     for (int V : {2, 30, 300}) fails += check_cat<double>(2, 3, V, 1, true, true, true, 0, 1e-13, 1e-13);
+    for (int V : {1, 3}) fails += check_cat<double>(1, 3, V, 0, false, true, false, 0, 1e-13, 1e-13);
+    for (int V : {8193, 8195}) fails += check_cat<double>(1, 1, V, 0, false, true, true, 0, 1e-12, 1e-12);
     for (int V : {4100, 8200, 20001}) {
         fails += check_cat<float>(1, 2, V, 1, false, true, true, 1, 3e-6, 3e-6);
         fails += check_cat<learn::bf16>(1, 2, V, 0, true, false, false, 0, 3e-6, 6e-3);
