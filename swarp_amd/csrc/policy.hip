@@ -278,6 +278,38 @@ template <> struct Words<f16> {
     }
 };
 
+// The largest of many elements, word by word.  16-bit ones by twos, as integers: the largest signed
+// one is the answer if it is not negative; if all are negative, the smallest unsigned one is (the
+// magnitudes are then in that order).
+template <typename T> struct Most {
+    typedef typename Acc<T>::type A;
+    A m = -INFINITY;
+    __device__ __forceinline__ void add(const uint32_t (&w)[4], int k)
+    {
+        if (k < (int)(16 / sizeof(T))) m = max_of(Words<T>::get(w, k), m);
+    }
+    __device__ __forceinline__ A value() const { return m; }
+};
+template <typename T> struct Most16 {
+    typedef short I2 __attribute__((ext_vector_type(2)));
+    typedef unsigned short U2 __attribute__((ext_vector_type(2)));
+    I2 i = {-32768, -32768};
+    U2 u = {65535, 65535};
+    __device__ __forceinline__ void add(const uint32_t (&w)[4], int k)
+    {
+        i = __builtin_elementwise_max(i, __builtin_bit_cast(I2, w[k]));
+        u = __builtin_elementwise_min(u, __builtin_bit_cast(U2, w[k]));
+    }
+    __device__ __forceinline__ float value() const
+    {
+        const short a = i.x > i.y ? i.x : i.y;
+        const unsigned short b = u.x < u.y ? u.x : u.y;
+        return (float)__builtin_bit_cast(T, (unsigned short)(a >= 0 ? (unsigned short)a : b));
+    }
+};
+template <> struct Most<bf16> : Most16<bf16> {};
+template <> struct Most<f16> : Most16<f16> {};
+
 // LANES threads hold a row of at most LANES * E elements, E a multiple of VEC: thread `lane` the
 // spans lane, lane + LANES, ..., as the words they came in (as elements they would take a register
 // each).  The last, short span is read and written in pieces; its length is the same for every
@@ -296,9 +328,15 @@ template <typename T, int LANES, int E> struct Held {
         uint32_t w[4];
     };
     uint32_t v[NV][4];
+    int spans;  // of the row
+
+    // Whether any thread has a span i: the same for the whole workgroup, so that what a row leaves
+    // empty costs nothing.
+    __device__ __forceinline__ bool used(int i) const { return KEEP || i * LANES < spans; }
 
     __device__ __forceinline__ void fill(uint32_t lo, uint32_t hi)
     {
+        spans = 0;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             v[i][0] = v[i][2] = lo;
@@ -339,6 +377,7 @@ template <typename T, int LANES, int E> struct Held {
         // (the offsets are formed here, row by row, and not kept in registers from row to row)
         if constexpr (!KEEP) asm volatile("" : "+v"(lane));
         const int full = width / VEC, rem = width % VEC;
+        spans = full + (rem != 0);
         Raw last = {{Words<T>::LOW, Words<T>::LOW_HI, Words<T>::LOW, Words<T>::LOW_HI}};
         if (rem && lane == full % LANES) {
             const T *const y = x + full * VEC;
@@ -371,16 +410,16 @@ template <typename T, int LANES, int E> struct Held {
     }
     __device__ __forceinline__ A most() const
     {
-        A m = -INFINITY;
+        // (a NaN may be passed over or come out: the sums hold it either way)
+        Most<T> m;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
+            if (!used(i)) break;
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) {
-                m = max_of(Words<T>::get(v[i], k), m);  // (passes a NaN over: the sums hold it)
-            }
+            for (int k = 0; k < 4; ++k) m.add(v[i], k);
             in_turn();
         }
-        return m;
+        return m.value();
     }
     __device__ __forceinline__ void sums(A m, A &s, A &q)
     {
@@ -388,6 +427,7 @@ template <typename T, int LANES, int E> struct Held {
         s = q = 0;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
+            if (!used(i)) break;
 #pragma unroll
             for (int k = 0; k < VEC; ++k) {
                 const A z = B::z(Words<T>::get(v[i], k), m), e = B::exp(z);
@@ -415,6 +455,7 @@ template <typename T, int LANES, int E> struct Held {
         forget();
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
+            if (!used(i)) break;
             A y[VEC];
 #pragma unroll
             for (int k = 0; k < VEC; ++k) {
@@ -490,11 +531,12 @@ template <typename A> __device__ __forceinline__ bool upstream(const Row<A> &r, 
 }
 
 // Rows of 33 to 2048 elements (a double's: of any number up to that): LANES threads of a wave a row.
-// What bounds it: memory from rows of 250 on (800 MB of bfloat16 logits and gradients in 165 to
-// 190 us, of float32 in 152 to 169); below, what each row costs beside its logits (rows of 50:
-// 284 and 247 us).
+// What bounds it: memory from rows of 250 on (800 MB of bfloat16 logits and gradients in 156 to
+// 189 us, of float32 in 152 to 169); below, what each row costs beside its logits (rows of 50:
+// 282 and 247 us).  16-bit rows are held to four waves a SIMD: 133 registers instead of 128 cost
+// rows of 1000 16 us.
 template <typename T, int LANES, int E>
-__global__ __launch_bounds__(BLOCK) void k_cat_lanes(const Row<typename Acc<T>::type> r, const Logits g)
+__global__ __launch_bounds__(BLOCK, sizeof(T) == 2 ? 4 : 1) void k_cat_lanes(const Row<typename Acc<T>::type> r, const Logits g)
 {
     typedef typename Acc<T>::type A;
     A up1;
@@ -559,9 +601,9 @@ template <int THREADS, typename A> __device__ __forceinline__ void block_sums(A 
 
 // Longer rows, up to THREADS * E elements: a workgroup a row.  Where a thread holds 256 bytes of
 // logits the registers are limited to four waves a SIMD, so that two workgroups of 512 share a
-// compute unit and one loads while the other computes: 8184 rows of 50001 bfloat16 logits in 440 us
-// (1.64 GB, which a copy moves in 346; vector units busy 0.62 of the time); as 1024 threads of 64
-// logits each, one workgroup a unit, 547 us.
+// compute unit and one loads while the other computes: 8184 rows of 50001 bfloat16 logits in 412 us
+// (1.64 GB, which a copy moves in 346; the vector units are busy 0.6 of the time, which the two
+// overlap in part); as 1024 threads of 64 logits each, one workgroup a unit, 547 us.
 template <typename T, int THREADS, int E>
 __global__ __launch_bounds__(THREADS, sizeof(T) < 8 && E * sizeof(T) >= 256 ? 4 : 1) void k_cat_block(const Row<typename Acc<T>::type> r, const Logits g)
 {
@@ -686,34 +728,46 @@ __global__ __launch_bounds__(BLOCK) void k_cat_join(const Row<typename Acc<T>::t
     if (r.sums) leave_sums<BLOCK>(t, r.sums);
 }
 
+// A wave's LDS instructions are executed in their order: between its writes and the reads of other
+// lanes only the compiler is to be held.
+__device__ __forceinline__ void wave_lds()
+{
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // Rows of N - 3 to N <= 32 elements, N a multiple of 4 (so that only the last three ask whether they
-// are there): a thread a row.  A workgroup's rows lie next to each other in
+// are there): a thread a row.  A wave's rows lie next to each other in
 // memory (where the caller's strides say so) and pass through LDS both ways, so that memory sees
 // whole lines; a row's place there has an odd length, which spreads the threads over the banks.
-// What bounds it: 4.1 M rows of 25 bfloat16 logits take 139 us (491 MB, which a copy moves in 104):
-// the vector units are busy 0.43 of the time, the rest is the chain load, barrier, row, barrier,
-// store with five waves a SIMD; keeping 2^z or forming it again measured the same.
+// A wave has 64 rows of its own and waits for no other (with the workgroup's 256 rows between
+// barriers 4.1 M rows of 25 bfloat16 logits took 139 us, now 130).
+// What bounds it: those are 491 MB, which a copy moves in 104 us; the vector units are busy half the
+// time, the rest is the chain load, LDS, row, LDS, store with four waves a SIMD.  Keeping 2^z or
+// forming it again measured the same, fetching the next rows ahead took more registers than it gave.
 template <typename T, int N>
 __global__ __launch_bounds__(BLOCK) void k_cat_rows(const Row<typename Acc<T>::type> r, const Logits g)
 {
     typedef typename Acc<T>::type A;
     typedef Base2<A> B;
     constexpr int VEC = 16 / sizeof(T);
-    __align__(16) __shared__ T tile[BLOCK * (N + 1)];
+    __align__(16) __shared__ T tiles[BLOCK * (N + 1)];
     A up1;
     if (upstream(r, up1)) return;
     const A w = weight_of(r) * up1;
-    const int V = g.width, S = V | 1, tid = threadIdx.x;
+    const int V = g.width, S = V | 1, tid = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    T *const tile = tiles + wave * (64 * (N + 1));
     const bool packed = g.flat && g.inner_stride == V;
     Terms<A> t = {};
-    for (int64_t i0 = (int64_t)blockIdx.x * BLOCK; i0 < r.rows; i0 += (int64_t)gridDim.x * BLOCK) {
-        const int rows = r.rows - i0 < BLOCK ? (int)(r.rows - i0) : BLOCK, n = rows * V;
+    for (int64_t i0 = (int64_t)blockIdx.x * BLOCK + wave * 64; i0 < r.rows; i0 += (int64_t)gridDim.x * BLOCK) {
+        const int rows = r.rows - i0 < 64 ? (int)(r.rows - i0) : 64, n = rows * V;
         const int64_t i = i0 + tid;
         const bool mine = tid < rows;
         T *const own = tile + tid * S;
         if (packed) {
             const T *const x = (const T *)g.x + i0 * V;
-            for (int e = tid * VEC; e < n; e += BLOCK * VEC) {
+            for (int e = tid * VEC; e < n; e += 64 * VEC) {
                 if (e + VEC <= n) {
                     const Span<T, VEC> y = *(const Span<T, VEC> *)(x + e);
                     if (S == V) {
@@ -734,7 +788,7 @@ __global__ __launch_bounds__(BLOCK) void k_cat_rows(const Row<typename Acc<T>::t
             const T *const x = (const T *)g.x + start_of(g, i);
             for (int k = 0; k < V; ++k) own[k] = x[k];
         }
-        __syncthreads();
+        wave_lds();
         const bool on = mine && (!r.mask || r.mask[i]);
         if (on) {
             const int64_t at = action_of(g, i);
@@ -768,10 +822,10 @@ __global__ __launch_bounds__(BLOCK) void k_cat_rows(const Row<typename Acc<T>::t
             if (r.logp) r.logp[i] = A(0);
             for (int k = 0; k < V; ++k) own[k] = (T)0.0f;
         }
-        __syncthreads();
+        wave_lds();
         if (!g.d) continue;
         T *const d = (T *)g.d + i0 * V;
-        for (int e = tid * VEC; e < n; e += BLOCK * VEC) {
+        for (int e = tid * VEC; e < n; e += 64 * VEC) {
             if (e + VEC <= n) {
                 Span<T, VEC> y;
                 if (S == V) {
@@ -789,7 +843,7 @@ __global__ __launch_bounds__(BLOCK) void k_cat_rows(const Row<typename Acc<T>::t
                 for (int k = e; k < n; ++k) d[k] = tile[k / V * S + k % V];
             }
         }
-        __syncthreads();
+        wave_lds();
     }
     if (r.sums) leave_sums<BLOCK>(t, r.sums);
 }

@@ -56,6 +56,8 @@ def _on_gpu(t: torch.Tensor, what: str) -> None:
 
 def _same(t: torch.Tensor, name: str, shape: torch.Size, dtype, device) -> torch.Tensor:
     """``t``, contiguous, after checking its shape, type and device."""
+    if (t.shape == shape and t.dtype is dtype and t.device == device and t.is_contiguous()):
+        return t
     if t.shape != shape:
         raise ValueError(f"{name} must be {list(shape)}; got {list(t.shape)}")
     if t.dtype != dtype:
@@ -194,8 +196,8 @@ def _loss_forward(call, a: _lib.SwarpPolicy, head, old, stream: int):
 
 def _buffers(head, log_std, need):
     """Gradient buffers of the heads that want one."""
-    return (torch.empty(head.shape, dtype=head.dtype, device=head.device) if need[0] else None,
-            torch.empty_like(log_std) if log_std is not None and need[1] else None)
+    return (torch.empty_like(head, memory_format=torch.contiguous_format) if need[0] else None,
+            torch.empty_like(log_std) if need[1] else None)
 
 
 class _LossFn(torch.autograd.Function):
