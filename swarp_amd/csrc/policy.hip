@@ -878,7 +878,7 @@ template <int D, typename A> __device__ void leave_std(const A (&v)[D], double *
 }
 
 // Up to four dimensions: a thread a decision.  What bounds it: memory; 8.2 M decisions of two
-// dimensions in 51 us (295 MB: 5.7 TB/s, part of it from the last cache).
+// dimensions in 50 us (295 MB: 5.9 TB/s, part of it from the last cache).
 template <typename T, int D, bool SHARED>
 __global__ __launch_bounds__(BLOCK) void k_gauss_rows(const Row<typename Acc<T>::type> r, const Normal g)
 {
@@ -1135,7 +1135,7 @@ template <typename T> void categorical(const swarp_policy_t *a, hipStream_t st)
     int blocks = 0;
     // A thread's share of a short row.  What a decision costs beside its logits is paid by every
     // lane of its row, so 16-bit logits, of which a line holds twice as many, go 32 to a thread:
-    // 200 M bfloat16 ones in rows of 250 take 192 us, 16 to a thread 237; 100 M float32 ones 178 and
+    // 200 M bfloat16 ones in rows of 250 take 189 us, 16 to a thread 237; 100 M float32 ones 178 and
     // 169.
     constexpr int E = sizeof(T) == 2 ? 32 : 16;
     if constexpr (sizeof(T) < 8) {
