@@ -602,8 +602,8 @@ template <int THREADS, typename A> __device__ __forceinline__ void block_sums(A 
 // Longer rows, up to THREADS * E elements: a workgroup a row.  Where a thread holds 256 bytes of
 // logits the registers are limited to four waves a SIMD, so that two workgroups of 512 share a
 // compute unit and one loads while the other computes: 8184 rows of 50001 bfloat16 logits in 412 us
-// (1.64 GB, which a copy moves in 346; the vector units are busy 0.6 of the time, which the two
-// overlap in part); as 1024 threads of 64 logits each, one workgroup a unit, 547 us.
+// (1.64 GB, which a copy moves in 346; the vector units are busy 0.54 of the time, which the
+// two overlap in part); as 1024 threads of 64 logits each, one workgroup a unit, 547 us.
 template <typename T, int THREADS, int E>
 __global__ __launch_bounds__(THREADS, sizeof(T) < 8 && E * sizeof(T) >= 256 ? 4 : 1) void k_cat_block(const Row<typename Acc<T>::type> r, const Logits g)
 {
