@@ -104,11 +104,11 @@ def _check_state(s: AdamWState, dev) -> None:
 
 
 def _table(params, grads, dev):
-    """The C table of the tensors that have a gradient, the tensors it points into, and the
-    state's length."""
+    """The C table of the tensors that have a gradient, the gradients made for it, the state's
+    length, and whether two of the tensors start at one place."""
     n = len(params)
     table = (_lib.SwarpTensor * max(n, 1))()
-    at, count, keep = 0, 0, []
+    at, count, keep, starts = 0, 0, [], set()
     for k in range(n):
         p, g = params[k], grads[k]
         size = p.numel()
@@ -128,11 +128,13 @@ def _table(params, grads, dev):
                 g = g.contiguous()
                 keep.append(g)
             t = table[count]
-            t.param, t.grad, t.n, t.slot = p.data_ptr(), g.data_ptr(), size, at
+            start = p.data_ptr()
+            starts.add(start)
+            t.param, t.grad, t.n, t.slot = start, g.data_ptr(), size, at
             t.param_dtype, t.grad_dtype = _CODES[p.dtype], _CODES[g.dtype]
             count += 1
         at += -(-size // GROUP) * GROUP
-    return table, count, keep, at
+    return table, count, keep, at, len(starts) < count
 
 
 def _norm_of(table, count, max_norm: float, dev) -> torch.Tensor:
@@ -159,7 +161,7 @@ def grad_norm(grads: Sequence[torch.Tensor | None],
     _check_norm(max_norm)
     dev = grads[0].device
     _on_gpu(grads[0], "grad_norm")
-    table, count, keep, _ = _table(grads, grads, dev)
+    table, count, keep, *_ = _table(grads, grads, dev)
     with _guard(dev):
         out = _norm_of(table, count, max_norm, dev)
     return out[0], out[1]
@@ -197,7 +199,9 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor | No
             raise ValueError("give max_grad_norm or grad_scale, not both")
     dev = params[0].device
     _on_gpu(params[0], "adamw_step")
-    table, count, keep, n = _table(params, grads, dev)
+    table, count, keep, n, twice = _table(params, grads, dev)
+    if twice:
+        raise ValueError("a parameter is listed twice: its updates would race")
     _check_state(state, dev)
     if state.exp_avg.numel() != n:
         raise ValueError(f"the state holds {state.exp_avg.numel()} elements, these parameters "
@@ -216,12 +220,16 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor | No
             norm = _norm_of(table, count, max_grad_norm, dev)
             a.grad_scale = norm.data_ptr() + 4
         _lib.check(_lib.load().swarp_adamw(ctypes.byref(a), table, count, _lib.stream_of(dev)))
+    # autograd then refuses a backward through what a graph saved of them before
+    torch.autograd.graph.increment_version(
+        [p for p, g in zip(params, grads) if g is not None and not p.is_inference()])
     return None if norm is None else norm[0]
 
 
 class AdamW(torch.optim.Optimizer):
     """AdamW over the parameter groups (one launch per group and 64 tensors), as
-    :func:`adamw_step`.
+    :func:`adamw_step`.  Steps are counted by group: a parameter whose first gradient comes late
+    is corrected for the steps that its group has taken.
 
     ``bits`` (32 or 8) is the width of the moments.  ``master`` keeps a float32 copy of 16-bit
     parameters (default: where a group holds float16 ones); after changing such parameters by
@@ -241,6 +249,10 @@ class AdamW(torch.optim.Optimizer):
         self._states: dict[int, AdamWState] = {}  # by group
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps,
                                       weight_decay=weight_decay))
+
+    def __getstate__(self) -> dict:  # (what a copy or a pickle takes along)
+        own = ("bits", "master", "max_grad_norm", "seed", "last_grad_norm", "_steps", "_states")
+        return super().__getstate__() | {name: getattr(self, name) for name in own}
 
     def _state_of(self, k: int) -> AdamWState:
         params = self.param_groups[k]["params"]

@@ -2,6 +2,7 @@
 float64, at the sizes and masks where they can go wrong, their gradients against the formula's and
 against differences, and their refusals."""
 
+import copy
 import math
 
 import pytest
@@ -709,6 +710,32 @@ def test_adamw_optimizer_and_its_state():
         AdamW(a.parameters(), bits=32).load_state_dict(one.state_dict())
 
 
+def test_adamw_is_seen_by_autograd():
+    w, idle = (torch.ones(300, device=DEV, requires_grad=True) for _ in range(2))
+    loss = (w * w * idle).sum()
+    before = idle._version
+    adamw_step([w, idle], [torch.ones_like(w), None], adamw_state([w, idle]), 1)
+    assert idle._version == before
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+def test_adamw_optimizer_is_copied_whole():
+    p = torch.nn.Parameter(torch.ones(300, device=DEV))
+    one = AdamW([p], bits=8, max_grad_norm=1.0, seed=3)
+    p.grad = torch.linspace(-1, 1, 300, device=DEV)
+    one.step()
+    two = copy.deepcopy(one)
+    q = two.param_groups[0]["params"][0]
+    q.grad = p.grad.clone()
+    one.step()
+    two.step()
+    assert q is not p and torch.equal(p, q)
+    assert torch.equal(one.last_grad_norm, two.last_grad_norm)
+    for a, b in zip(one._states[0][:4], two._states[0][:4]):
+        assert torch.equal(a, b)
+
+
 def test_adamw_refuses():
     p, g = [torch.zeros(4, device=DEV)], [torch.zeros(4, device=DEV)]
     s = adamw_state(p)
@@ -716,6 +743,8 @@ def test_adamw_refuses():
         adamw_step(p, [], s, 1)
     with pytest.raises(ValueError, match="step"):
         adamw_step(p, g, s, 0)
+    with pytest.raises(ValueError, match="twice"):
+        adamw_step([p[0], p[0].view(2, 2)], [g[0], g[0].view(2, 2)], adamw_state(p + p), 1)
     with pytest.raises(ValueError, match="betas"):
         adamw_step(p, g, s, 1, betas=(1.0, 0.9))
     with pytest.raises(TypeError, match="parameter 0"):

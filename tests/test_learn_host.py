@@ -2,6 +2,7 @@
 and that nothing computes on the CPU."""
 
 import ctypes
+import pickle
 import subprocess
 from pathlib import Path
 
@@ -114,3 +115,10 @@ def test_state_layout():
     assert s.master.dtype == torch.float32
     opt = AdamW([torch.nn.Parameter(torch.zeros(3))])
     assert opt.step() is None and opt.state_dict()["steps"] == {}
+
+
+def test_a_copied_optimizer_keeps_its_settings():
+    one = AdamW([torch.nn.Parameter(torch.zeros(3))], lr=2e-3, bits=8, max_grad_norm=0.5, seed=7)
+    two = pickle.loads(pickle.dumps(one))
+    assert (two.bits, two.max_grad_norm, two.seed, two.master) == (8, 0.5, 7, None)
+    assert two.param_groups[0]["lr"] == 2e-3 and two.step() is None
