@@ -421,7 +421,8 @@ typedef struct swarp_gae {
     const void *values;       /* [T+1,N] or [N,T+1] */
     const uint8_t *terminated, *truncated; /* [T,N/group] or [N/group,T], nonzero = true; NULL:
                                               never */
-    const void *final_values; /* as rewards; NULL: a truncated step reads V_{t+1} */
+    const void *final_values; /* as rewards; NULL: a truncated step reads V_{t+1}.  swarp_gae_bwd
+                                 only asks whether it is set */
     void *advantages, *returns;            /* as rewards; written by swarp_gae_fwd */
     const void *adj_advantages, *adj_returns; /* as rewards, NULL = zero; read by
                                                  swarp_gae_bwd */

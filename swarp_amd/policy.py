@@ -71,6 +71,16 @@ def _ptr(t: torch.Tensor | None):
     return None if t is None else t.data_ptr()
 
 
+def _like(t: torch.Tensor | None):
+    return None if t is None else (t.shape, t.dtype, t.device)
+
+
+def _as_saved(t: torch.Tensor | None, like) -> torch.Tensor | None:
+    """A saved tensor whose ``_like`` was ``like``, contiguous: a saved-tensor hook may have given
+    back another one (a checkpoint's recomputation, a copy from the host)."""
+    return None if t is None else _same(t, "a saved tensor", *like)
+
+
 # ----------------------------------------------------------------------------- advantages
 
 
@@ -98,7 +108,7 @@ class _GaeFn(torch.autograd.Function):
     def forward(ctx, a: _lib.SwarpGae, stream: int, rewards, values, final, term, trunc):
         ctx.set_materialize_grads(False)
         ctx.a, ctx.stream = a, stream
-        ctx.like = (rewards.shape, values.shape)
+        ctx.like = (rewards.shape, values.shape, _like(term), _like(trunc))
         ctx.save_for_backward(term, trunc)
         return _gae_forward(a, rewards, stream)
 
@@ -107,14 +117,20 @@ class _GaeFn(torch.autograd.Function):
     def backward(ctx, g_adv, g_ret):
         if g_adv is None and g_ret is None:
             return (None,) * 7
-        term, trunc = ctx.saved_tensors  # (unchanged since, or this raises)
+        r_shape, v_shape, *flags = ctx.like
+        # (unchanged since, or this raises; not the forward's memory where a hook packed them)
+        term, trunc = (_as_saved(t, like) for t, like in zip(ctx.saved_tensors, flags))
         g_adv, g_ret = (None if g is None else g.contiguous() for g in (g_adv, g_ret))
         ref = g_adv if g_adv is not None else g_ret
-        need, (r_shape, v_shape) = ctx.needs_input_grad, ctx.like
-        a = ctx.a  # whose final_values is only looked at for being there
+        need = ctx.needs_input_grad
+        a = _lib.SwarpGae.from_buffer_copy(ctx.a)
+        a.rewards = a.values = a.advantages = a.returns = None  # (read by the forward alone)
+        a.terminated, a.truncated = _ptr(term), _ptr(trunc)
         d_r = ref.new_empty(r_shape) if need[2] else None
         d_v = ref.new_empty(v_shape) if need[3] else None
         d_f = ref.new_empty(r_shape) if a.final_values and need[4] else None
+        if a.final_values:  # (only looked at for being set: an address that is alive)
+            a.final_values = ref.data_ptr()
         a.adj_advantages, a.adj_returns = _ptr(g_adv), _ptr(g_ret)
         a.adj_rewards, a.adj_values, a.adj_final_values = _ptr(d_r), _ptr(d_v), _ptr(d_f)
         _lib.check(_lib.load().swarp_gae_bwd(ctypes.byref(a), ctx.stream))
@@ -200,13 +216,36 @@ def _buffers(head, log_std, need):
             torch.empty_like(log_std) if need[1] else None)
 
 
+def _relocated(a: _lib.SwarpPolicy, saved, like):
+    """A copy of a forward's arguments that reads the saved tensors where they now lie; the head,
+    the deviations, and all that has to stay until the launch."""
+    head, log_std, *rest = saved
+    shape, dtype, dev = like[0]
+    if head.shape != shape or head.dtype != dtype or head.device != dev:
+        raise RuntimeError(f"a saved head came back as {list(head.shape)} {head.dtype} on "
+                           f"{head.device}; it was {list(shape)} {dtype} on {dev}")
+    strides = _row_strides(head) if log_std is None else None
+    if strides is None:
+        head = head.contiguous()
+        strides = (1, 0, 0) if log_std is not None else _row_strides(head)
+    log_std = _as_saved(log_std, like[1])
+    rest = [_as_saved(t, x) for t, x in zip(rest, like[2:])]
+    a = _lib.SwarpPolicy.from_buffer_copy(a)
+    a.inner, a.outer_stride, a.inner_stride = strides
+    a.head, a.log_std = head.data_ptr(), _ptr(log_std)
+    a.actions, a.old_logp, a.advantages, a.ref_logp, a.mask = (_ptr(t) for t in rest)
+    a.logp = a.loss = a.stats = None  # (of the forward alone)
+    return a, head, log_std, rest
+
+
 class _LossFn(torch.autograd.Function):
     """A policy loss as one autograd node.
 
     The forward leaves the gradients for an upstream gradient of 1 behind, while a head's row is
     at hand: a training step then reads the heads once and writes their gradients once.  The
     backward hands them out; where the upstream gradient is not 1 (the device looks) it computes
-    them again with it, so each is rounded once.  float16 gradients are left to the backward:
+    them again with it, so each is rounded once, from the tensors that autograd kept: under a
+    checkpoint or a packing hook the forward's own are gone.  float16 gradients are left to the backward:
     without the loss scale that comes with it they would vanish.
     """
 
@@ -220,6 +259,7 @@ class _LossFn(torch.autograd.Function):
             ctx.made = _buffers(head, log_std, ctx.need)
             a.d_head, a.d_log_std = _ptr(ctx.made[0]), _ptr(ctx.made[1])
         loss, stats, logp, ctx.work = _loss_forward(calls[0], a, head, rest[1], stream)
+        ctx.like = [_like(t) for t in (head, log_std, *rest)]
         ctx.save_for_backward(head, log_std, *rest)
         ctx.mark_non_differentiable(stats, logp)
         return loss, stats, logp
@@ -229,17 +269,15 @@ class _LossFn(torch.autograd.Function):
     def backward(ctx, g, *_):
         if g is None:
             return (None,) * 10
-        saved = ctx.saved_tensors  # (unchanged since, or this raises)
         call, a, stream = ctx.call
+        # (unchanged since, or this raises)
+        a, head, log_std, keep = _relocated(a, ctx.saved_tensors, ctx.like)
         made, ctx.made = ctx.made, None  # handed out once: the caller may change them
-        if made is None:
-            d = _buffers(saved[0], saved[1], ctx.need)
-            a.d_head, a.d_log_std = _ptr(d[0]), _ptr(d[1])
-            _lib.check(call(ctypes.byref(a), 0, g.data_ptr(), stream))
-            return None, None, None, *d, None, None, None, None, None
+        d = _buffers(head, log_std, ctx.need) if made is None else made
+        a.d_head, a.d_log_std = _ptr(d[0]), _ptr(d[1])
         # (autograd runs this with the forward's device and stream current)
-        _lib.check(call(ctypes.byref(a), 1, g.data_ptr(), stream))
-        return None, None, None, *made, None, None, None, None, None
+        _lib.check(call(ctypes.byref(a), int(made is not None), g.data_ptr(), stream))
+        return None, None, None, *d, None, None, None, None, None
 
 
 def _clip_of(clip) -> tuple[float, float]:
