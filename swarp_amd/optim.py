@@ -232,8 +232,8 @@ class AdamW(torch.optim.Optimizer):
     is corrected for the steps that its group has taken.
 
     ``bits`` (32 or 8) is the width of the moments.  ``master`` keeps a float32 copy of 16-bit
-    parameters (default: where a group holds float16 ones); after changing such parameters by
-    other means call :meth:`sync_master`.  ``max_grad_norm`` clips the norm over all groups;
+    parameters (default: where a group holds float16 ones, or the state that is loaded has one);
+    after changing such parameters by other means call :meth:`sync_master`.  ``max_grad_norm`` clips the norm over all groups;
     ``last_grad_norm`` is what it was, on the device."""
 
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
@@ -254,13 +254,17 @@ class AdamW(torch.optim.Optimizer):
         own = ("bits", "master", "max_grad_norm", "seed", "last_grad_norm", "_steps", "_states")
         return super().__getstate__() | {name: getattr(self, name) for name in own}
 
+    def _master_of(self, k: int) -> bool | None:
+        """Whether group ``k`` keeps a master copy; None: it was left open, and nothing needs one."""
+        if self.master is None and any(p.dtype == torch.float16
+                                       for p in self.param_groups[k]["params"]):
+            return True
+        return self.master
+
     def _state_of(self, k: int) -> AdamWState:
-        params = self.param_groups[k]["params"]
         if k not in self._states:
-            master = self.master
-            if master is None:
-                master = any(p.dtype == torch.float16 for p in params)
-            self._states[k] = adamw_state(params, bits=self.bits, master=master)
+            self._states[k] = adamw_state(self.param_groups[k]["params"], bits=self.bits,
+                                          master=bool(self._master_of(k)))
         return self._states[k]
 
     @torch.no_grad()
@@ -321,6 +325,10 @@ class AdamW(torch.optim.Optimizer):
             if s.bits != self.bits:
                 raise ValueError(f"group {k}: moments of {s.bits} bits, this optimizer keeps "
                                  f"{self.bits}")
+            keeps = self._master_of(k)
+            if keeps is not None and keeps != (s.master is not None):
+                raise ValueError(f"group {k}: the state has {'no' if keeps else 'a'} master copy, "
+                                 f"this optimizer keeps {'one' if keeps else 'none'}")
             states[k] = s
         for g, new in zip(self.param_groups, state["groups"]):
             g.update(new)

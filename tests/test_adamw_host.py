@@ -1,0 +1,43 @@
+"""The optimizer around the AdamW step, without a GPU: what it loads, takes, refuses and tells its
+hooks."""
+
+import pytest
+import torch
+
+from swarp_amd import AdamW
+
+
+def params(dtype=torch.bfloat16, n=300):
+    return [torch.nn.Parameter(torch.ones(n, dtype=dtype))]
+
+
+def saved(dtype=torch.bfloat16, **kw):
+    """The state dictionary of an optimizer that has its state."""
+    opt = AdamW(params(dtype), **kw)
+    opt._state_of(0)
+    return opt.state_dict()
+
+
+def test_a_loaded_state_has_the_master_that_the_optimizer_keeps():
+    without, having = saved(), saved(master=True)
+    with pytest.raises(ValueError, match="no master copy"):
+        AdamW(params(), master=True).load_state_dict(without)
+    with pytest.raises(ValueError, match="a master copy"):
+        AdamW(params(), master=False).load_state_dict(having)
+    with pytest.raises(ValueError, match="no master copy"):  # which float16 needs
+        AdamW(params(torch.float16)).load_state_dict(without)
+    for kw, state in (({"master": True}, having), ({"master": False}, without), ({}, without),
+                      ({}, having)):
+        opt = AdamW(params(), **kw)
+        opt.load_state_dict(state)
+        assert (opt._states[0].master is None) == (state is without)
+    opt = AdamW(params(torch.float16))
+    opt.load_state_dict(saved(torch.float16))
+    assert opt._states[0].master is not None
+
+
+def test_a_refused_state_leaves_the_optimizer_as_it_was():
+    opt = AdamW(params(), master=True, seed=4)
+    with pytest.raises(ValueError):
+        opt.load_state_dict(saved(seed=9, lr=1.0))
+    assert opt.seed == 4 and not opt._states and opt.param_groups[0]["lr"] == 1e-3
