@@ -285,10 +285,11 @@ class AdamW(torch.optim.Optimizer):
             if all(x is None for x in grads):
                 continue
             g = self.param_groups[k]
-            t = self._steps[k] = self._steps.get(k, 0) + 1
+            t = self._steps.get(k, 0) + 1
             adamw_step(params, grads, self._state_of(k), t, lr=float(g["lr"]),
                        betas=g["betas"], eps=g["eps"], weight_decay=g["weight_decay"],
                        grad_scale=scale, seed=self.seed + 0x51ED * t + k)
+            self._steps[k] = t  # (a step that was refused is none)
         return loss
 
     @torch.no_grad()

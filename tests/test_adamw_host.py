@@ -41,3 +41,12 @@ def test_a_refused_state_leaves_the_optimizer_as_it_was():
     with pytest.raises(ValueError):
         opt.load_state_dict(saved(seed=9, lr=1.0))
     assert opt.seed == 4 and not opt._states and opt.param_groups[0]["lr"] == 1e-3
+
+
+def test_a_step_that_is_refused_is_not_counted():
+    opt = AdamW(params(torch.float32))
+    opt.param_groups[0]["params"][0].grad = torch.ones(300)
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="HIP device"):
+            opt.step()
+    assert opt.state_dict()["steps"] == {}
