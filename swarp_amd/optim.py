@@ -9,6 +9,7 @@ tensor's at a multiple of 256 elements, so that a step is one launch over up to 
 from __future__ import annotations
 
 import ctypes
+import operator
 from typing import Iterable, NamedTuple, Sequence
 
 import torch
@@ -105,10 +106,10 @@ def _check_state(s: AdamWState, dev) -> None:
 
 def _table(params, grads, dev):
     """The C table of the tensors that have a gradient, the gradients made for it, the state's
-    length, and whether two of the tensors start at one place."""
+    length, and whether two of the tensors share memory."""
     n = len(params)
     table = (_lib.SwarpTensor * max(n, 1))()
-    at, count, keep, starts = 0, 0, [], set()
+    at, count, keep, starts, ends = 0, 0, [], [], []
     for k in range(n):
         p, g = params[k], grads[k]
         size = p.numel()
@@ -129,12 +130,16 @@ def _table(params, grads, dev):
                 keep.append(g)
             t = table[count]
             start = p.data_ptr()
-            starts.add(start)
+            starts.append(start)
+            ends.append(start + size * p.element_size())
             t.param, t.grad, t.n, t.slot = start, g.data_ptr(), size, at
             t.param_dtype, t.grad_dtype = _CODES[p.dtype], _CODES[g.dtype]
             count += 1
         at += -(-size // GROUP) * GROUP
-    return table, count, keep, at, len(starts) < count
+    # (spans are apart if, each list in order, every one ends before the next begins)
+    starts.sort()
+    ends.sort()
+    return table, count, keep, at, any(map(operator.lt, starts[1:], ends))
 
 
 def _norm_of(table, count, max_norm: float, dev) -> torch.Tensor:
@@ -199,9 +204,10 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor | No
             raise ValueError("give max_grad_norm or grad_scale, not both")
     dev = params[0].device
     _on_gpu(params[0], "adamw_step")
-    table, count, keep, n, twice = _table(params, grads, dev)
-    if twice:
-        raise ValueError("a parameter is listed twice: its updates would race")
+    table, count, keep, n, shared = _table(params, grads, dev)
+    if shared:
+        raise ValueError("two parameters share memory, or one is listed twice: their updates "
+                         "would race")
     _check_state(state, dev)
     if state.exp_avg.numel() != n:
         raise ValueError(f"the state holds {state.exp_avg.numel()} elements, these parameters "

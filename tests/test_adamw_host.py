@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from swarp_amd import AdamW
+from swarp_amd.optim import _table
 
 
 def params(dtype=torch.bfloat16, n=300):
@@ -50,3 +51,21 @@ def test_a_step_that_is_refused_is_not_counted():
         with pytest.raises(RuntimeError, match="HIP device"):
             opt.step()
     assert opt.state_dict()["steps"] == {}
+
+
+def test_parameters_that_share_memory_are_found():
+    b = torch.zeros(1000)
+
+    def shared(*spans):
+        p = [b[lo:hi] for lo, hi in spans]
+        return _table(p, [torch.zeros_like(x) for x in p], b.device)[4]
+    assert shared((0, 300), (100, 400)) and shared((100, 400), (0, 300))
+    assert shared((0, 1000), (10, 20), (30, 40)) and shared((5, 6), (5, 6))
+    assert shared((0, 10), (20, 30), (29, 40), (50, 60))
+    assert not shared((0, 300), (300, 400)) and not shared((500, 1000), (0, 1), (1, 500))
+    assert not shared((0, 10)) and not shared((0, 0), (0, 10), (5, 5))
+    h = b.view(torch.bfloat16)
+    assert _table([b[:10], h[19:30]], [torch.zeros(10), torch.zeros(11).bfloat16()], b.device)[4]
+    assert not _table([b[:10], h[20:30]], [torch.zeros(10), torch.zeros(10).bfloat16()], b.device)[4]
+    # one without a gradient is not touched
+    assert not _table([b[:300], b[100:400]], [torch.zeros(300), None], b.device)[4]

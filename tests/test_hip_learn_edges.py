@@ -8,7 +8,7 @@ import pytest
 import torch
 from torch.utils.checkpoint import checkpoint
 
-from swarp_amd import categorical_policy_loss, gae, gaussian_policy_loss
+from swarp_amd import adamw_state, adamw_step, categorical_policy_loss, gae, gaussian_policy_loss
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -112,3 +112,17 @@ def test_gae_under_hooks_and_checkpoints(last, way):
     taken = poison(ends[0], ends[0], r)
     got = torch.autograd.grad(out, x, up)
     assert all(torch.equal(a, b) for a, b in zip(got, want)), len(taken)
+
+
+# ------------------------------------------------------------------------------ refusals
+
+
+def test_overlapping_parameters_are_refused():
+    b = torch.zeros(1000, device=DEV)
+    p = [b[:300], b[100:400]]
+    with pytest.raises(ValueError, match="share memory"):
+        adamw_step(p, [torch.ones_like(x) for x in p], adamw_state(p), 1)
+    assert not b.any()
+    p = [b[:300], b[300:400]]
+    adamw_step(p, [torch.ones_like(x) for x in p], adamw_state(p), 1)
+    assert bool(b[:400].all()) and not b[400:].any()
