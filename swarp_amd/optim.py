@@ -15,7 +15,7 @@ from typing import Iterable, NamedTuple, Sequence
 import torch
 
 from . import _lib
-from .policy import _CODES, _guard, _on_gpu, _ptr
+from .policy import _CODES, _guard, _on_gpu, _plain, _ptr
 
 GROUP = 256  # elements that share an exponent in an 8-bit moment
 _PARAMS = (torch.float32, torch.bfloat16, torch.float16)
@@ -98,7 +98,8 @@ def _check_state(s: AdamWState, dev) -> None:
         want["master"] = (n, torch.float32)
     for name, (k, dtype) in want.items():
         t = getattr(s, name)
-        if t is None or t.numel() != k or t.dtype != dtype or not t.is_contiguous():
+        if (t is None or t.numel() != k or t.dtype != dtype or not t.is_contiguous()
+                or t.is_neg()):
             raise ValueError(f"state.{name} must be a contiguous {dtype} tensor of {k} elements")
         if t.device != dev:
             raise ValueError(f"state.{name} is on {t.device}, the parameters on {dev}")
@@ -118,15 +119,15 @@ def _table(params, grads, dev):
                 raise TypeError(f"parameter {k}: float32, bfloat16 or float16; got {p.dtype}")
             if p.device != dev or g.device != dev:
                 raise ValueError(f"parameter {k} and its gradient must be on {dev}")
-            if not p.is_contiguous():
-                raise ValueError(f"parameter {k} must be contiguous")
+            if not p.is_contiguous() or p.is_neg():
+                raise ValueError(f"parameter {k} must be contiguous, and no negated view")
             if g.shape != p.shape or g.layout != torch.strided:
                 raise ValueError(f"gradient {k} must be a dense {list(p.shape)}; got "
                                  f"{list(g.shape)}")
             if g.dtype != p.dtype and g.dtype != torch.float32:
                 raise TypeError(f"gradient {k} must be {p.dtype} or float32; got {g.dtype}")
-            if not g.is_contiguous():
-                g = g.contiguous()
+            if not g.is_contiguous() or g.is_neg():
+                g = _plain(g)
                 keep.append(g)
             t = table[count]
             start = p.data_ptr()
@@ -160,7 +161,7 @@ def grad_norm(grads: Sequence[torch.Tensor | None],
     """``(norm, scale)``, float32 scalars on the device: the 2-norm of all ``grads`` together (in
     a fixed order: the same bits every time) and ``min(1, max_norm / (norm + 1e-6))``, which
     :func:`adamw_step` takes as ``grad_scale``.  No host synchronisation."""
-    grads = [g.contiguous() for g in grads if g is not None]
+    grads = [_plain(g) for g in grads if g is not None]
     if not grads:
         raise ValueError("no gradients")
     _check_norm(max_norm)
@@ -217,6 +218,8 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor | No
     if grad_scale is not None and (grad_scale.numel() != 1 or grad_scale.dtype != torch.float32
                                    or grad_scale.device != dev):
         raise ValueError(f"grad_scale must be one float32 on {dev}")
+    if grad_scale is not None:
+        grad_scale = _plain(grad_scale)
     a = _state_args(state)
     a.seed, a.step, a.lr, a.beta1, a.beta2 = seed & 0xFFFFFFFF, step, lr, betas[0], betas[1]
     a.eps, a.weight_decay, a.grad_scale = eps, weight_decay, _ptr(grad_scale)

@@ -56,7 +56,8 @@ def _on_gpu(t: torch.Tensor, what: str) -> None:
 
 def _same(t: torch.Tensor, name: str, shape: torch.Size, dtype, device) -> torch.Tensor:
     """``t``, contiguous, after checking its shape, type and device."""
-    if (t.shape == shape and t.dtype is dtype and t.device == device and t.is_contiguous()):
+    if (t.shape == shape and t.dtype is dtype and t.device == device and t.is_contiguous()
+            and not t.is_neg()):
         return t
     if t.shape != shape:
         raise ValueError(f"{name} must be {list(shape)}; got {list(t.shape)}")
@@ -64,7 +65,13 @@ def _same(t: torch.Tensor, name: str, shape: torch.Size, dtype, device) -> torch
         raise TypeError(f"{name} must be {dtype}; got {t.dtype}")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, the others on {device}")
-    return t if t.is_contiguous() else t.contiguous()
+    return _plain(t)
+
+
+def _plain(t: torch.Tensor) -> torch.Tensor:
+    """``t``, contiguous, with the values that its memory holds: a negated view (the imaginary part
+    of a conjugate) reads the others' storage with its sign kept aside."""
+    return (t.resolve_neg() if t.is_neg() else t).contiguous()
 
 
 def _ptr(t: torch.Tensor | None):
@@ -120,7 +127,7 @@ class _GaeFn(torch.autograd.Function):
         r_shape, v_shape, *flags = ctx.like
         # (unchanged since, or this raises; not the forward's memory where a hook packed them)
         term, trunc = (_as_saved(t, like) for t, like in zip(ctx.saved_tensors, flags))
-        g_adv, g_ret = (None if g is None else g.contiguous() for g in (g_adv, g_ret))
+        g_adv, g_ret = (None if g is None else _plain(g) for g in (g_adv, g_ret))
         ref = g_adv if g_adv is not None else g_ret
         need = ctx.needs_input_grad
         a = _lib.SwarpGae.from_buffer_copy(ctx.a)
@@ -224,9 +231,9 @@ def _relocated(a: _lib.SwarpPolicy, saved, like):
     if head.shape != shape or head.dtype != dtype or head.device != dev:
         raise RuntimeError(f"a saved head came back as {list(head.shape)} {head.dtype} on "
                            f"{head.device}; it was {list(shape)} {dtype} on {dev}")
-    strides = _row_strides(head) if log_std is None else None
+    strides = _row_strides(head) if log_std is None and not head.is_neg() else None
     if strides is None:
-        head = head.contiguous()
+        head = _plain(head)
         strides = (1, 0, 0) if log_std is not None else _row_strides(head)
     log_std = _as_saved(log_std, like[1])
     rest = [_as_saved(t, x) for t, x in zip(rest, like[2:])]
@@ -275,6 +282,7 @@ class _LossFn(torch.autograd.Function):
         made, ctx.made = ctx.made, None  # handed out once: the caller may change them
         d = _buffers(head, log_std, ctx.need) if made is None else made
         a.d_head, a.d_log_std = _ptr(d[0]), _ptr(d[1])
+        g = _plain(g)
         # (autograd runs this with the forward's device and stream current)
         _lib.check(call(ctypes.byref(a), int(made is not None), g.data_ptr(), stream))
         return None, None, None, *d, None, None, None, None, None
@@ -397,9 +405,9 @@ def categorical_policy_loss(
     rest = _per_row(lead, wide, dev, old_logp, advantages, ref_logp, mask)
     low_high = _clip_of(clip)
     coefs = _coefs(kl_coef, entropy_coef, reduction)
-    strides = _row_strides(logits)
+    strides = None if logits.is_neg() else _row_strides(logits)
     if strides is None:
-        logits = logits.contiguous()
+        logits = _plain(logits)
         strides = _row_strides(logits)
     return _evaluate(False, logits.shape[-1], strides, low_high, coefs, logits, None, actions, *rest)
 
@@ -441,5 +449,5 @@ def gaussian_policy_loss(
         raise ValueError("actions requires grad, but the loss treats it as a constant: detach it")
     rest = _per_row(lead, wide, dev, old_logp, advantages, ref_logp, mask)
     coefs = _coefs(kl_coef, entropy_coef, reduction)
-    return _evaluate(True, D, (1, 0, 0), _clip_of(clip), coefs, mean.contiguous(),
-                     log_std.contiguous(), actions, *rest)
+    return _evaluate(True, D, (1, 0, 0), _clip_of(clip), coefs, _plain(mean),
+                     _plain(log_std), actions, *rest)

@@ -1,12 +1,15 @@
-"""What the backwards of ``gae`` and the policy losses hand to the library, without a GPU: the
-library is a stand-in that notes its arguments.  Under a saved-tensor hook or a checkpoint the
-forward's own tensors are gone by then, so the addresses have to be those that autograd gives back."""
+"""What ``gae``, the policy losses and AdamW hand to the library, without a GPU: the library is a
+stand-in that notes its arguments.  Under a saved-tensor hook or a checkpoint the forward's own
+tensors are gone when the backward runs, so the addresses have to be those that autograd gives
+back; and what a kernel reads at an address has to be what the tensor reads."""
+
+import ctypes
 
 import pytest
 import torch
 from torch.utils.checkpoint import checkpoint
 
-from swarp_amd import _lib, policy
+from swarp_amd import _lib, adamw_state, adamw_step, grad_norm, optim, policy
 
 POINTERS = {"head", "log_std", "actions", "old_logp", "advantages", "ref_logp", "mask"}
 
@@ -16,14 +19,17 @@ class Library:
 
     def __init__(self):
         self.calls = []
+        self.look = None  # called within each call, while its memory is alive
 
     def __getattr__(self, name):
         if name == "swarp_policy_work_bytes":
             return lambda rows, width: 64
 
         def call(arg, *rest):
-            a = arg._obj
+            a = arg._obj if hasattr(arg, "_obj") else arg
             self.calls.append((name, type(a).from_buffer_copy(a), rest))
+            if self.look is not None:
+                self.look(a, rest)
             return 0
         return call
 
@@ -33,7 +39,8 @@ def library(monkeypatch):
     lib = Library()
     monkeypatch.setattr(_lib, "load", lambda: lib)
     monkeypatch.setattr(_lib, "stream_of", lambda device: 0)
-    monkeypatch.setattr(policy, "_on_gpu", lambda t, what: None)
+    for module in (policy, optim):
+        monkeypatch.setattr(module, "_on_gpu", lambda t, what: None)
     return lib
 
 
@@ -151,3 +158,71 @@ def test_the_scan_reads_what_the_hook_gives_back(library, last):
     gone = hook.addresses() | {ends.data_ptr()}
     assert a.terminated not in gone and a.truncated not in gone and a.terminated != a.truncated
     assert a.final_values == a.adj_advantages  # (alive; only looked at for being set)
+
+
+def neg(t):
+    """-t as a view that keeps its sign aside, as ``torch.conj`` makes them."""
+    return torch._neg_view(t)
+
+
+def floats(address, n):
+    return list((ctypes.c_float * n).from_address(address))
+
+
+def test_negated_views_are_handed_over_as_they_read(library):
+    x = torch.arange(1.0, 13.0)
+    seen = {}
+
+    def look(a, rest):
+        for name, _ in a._fields_:
+            if getattr(a, name) and name in ("rewards", "values", "final_values", "head", "log_std",
+                                             "old_logp", "advantages", "ref_logp"):
+                seen[name] = floats(getattr(a, name), 2)
+        if len(rest) == 3:
+            seen["scale"] = floats(rest[1], 1)
+    library.look = look
+    h = neg(x.view(6, 2)).detach().requires_grad_(True)
+    policy.gae(neg(x[:4]), neg(x[:5]), None, None, neg(x[:4]))
+    assert all(seen[k] == [-1.0, -2.0] for k in ("rewards", "values", "final_values"))
+    loss = policy.categorical_policy_loss(h, torch.zeros(6, dtype=torch.int64), neg(x[:6]), x[:6],
+                                          neg(x[:6])).loss
+    want = {"head": [-1.0, -2.0], "old_logp": [-1.0, -2.0], "ref_logp": [-1.0, -2.0]}
+    assert {k: seen[k] for k in want} == want
+    loss.backward(neg(torch.tensor(3.0)))
+    assert {k: seen[k] for k in want} == want and seen["scale"] == [-3.0]
+    seen.clear()
+    policy.gaussian_policy_loss(h, neg(x[:2]), neg(x.view(6, 2)), x[:6], neg(x[:6])).loss.backward()
+    assert seen["head"] == seen["log_std"] == seen["advantages"] == [-1.0, -2.0]
+    with Packed(neg):
+        loss = policy.categorical_policy_loss(h, torch.zeros(6, dtype=torch.int64), x[:6], x[:6]).loss
+    loss.backward()
+    assert seen["head"] == [1.0, 2.0] and seen["old_logp"] == [-1.0, -2.0]
+
+
+def test_the_adjoint_of_the_scan_reads_negated_gradients(library):
+    seen = []
+    library.look = lambda a, rest: seen.append(a.adj_advantages and floats(a.adj_advantages, 2))
+    r = torch.zeros(3, requires_grad=True)
+    out = policy.gae(r, torch.zeros(4))
+    torch.autograd.backward(out.advantages, neg(torch.tensor([1.0, 2.0, 3.0])))
+    assert seen[-1] == [-1.0, -2.0]
+
+
+def test_adamw_and_negated_views(library):
+    p, g = [torch.ones(2)], [neg(torch.tensor([1.0, 2.0]))]
+    seen = []
+
+    def look(a, rest):
+        table = rest[0] if isinstance(a, _lib.SwarpAdamW) else a
+        seen.append(floats(table[0].grad, 2))
+        if isinstance(a, _lib.SwarpAdamW) and a.grad_scale:
+            seen.append(floats(a.grad_scale, 1))
+    library.look = look
+    adamw_step(p, g, adamw_state(p), 1, grad_scale=neg(torch.tensor([0.5])))
+    grad_norm(g)
+    assert seen == [[-1.0, -2.0], [-0.5], [-1.0, -2.0]]
+    with pytest.raises(ValueError, match="negated"):
+        adamw_step([neg(p[0])], g, adamw_state(p), 1)
+    s = adamw_state(p)
+    with pytest.raises(ValueError, match="exp_avg"):
+        adamw_step(p, g, s._replace(exp_avg=neg(s.exp_avg)), 1)
