@@ -16,6 +16,7 @@ import math
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -52,6 +53,16 @@ def _on_gpu(t: torch.Tensor, what: str) -> None:
     if not t.is_cuda:
         raise RuntimeError(f"{what}: swarp_amd computes on the HIP device only (no CPU fallback); "
                            f"got a tensor on {t.device}")
+
+
+def _no_tangents(what: str, *tensors: torch.Tensor | None) -> None:
+    """Refuses dual tensors, whose tangents the kernels would drop."""
+    if forward_ad._current_level < 0:  # (no forward-mode derivative is being taken)
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{what} has no forward-mode derivative; it is "
+                                      "differentiated backward")
 
 
 def _same(t: torch.Tensor, name: str, shape: torch.Size, dtype, device) -> torch.Tensor:
@@ -193,6 +204,7 @@ def gae(rewards: torch.Tensor, values: torch.Tensor, terminated: torch.Tensor | 
             flags[n] = _same(flags[n], name, timed(T, batch[:k]), torch.bool, dev)
             group = math.prod(batch[k:])
     inputs = (rewards, values, final_values)
+    _no_tangents("gae", *inputs)
     a = _scan_args(int(last), T, math.prod(batch), max(group, 1), gamma, lam, *inputs, *flags)
     stream = _lib.stream_of(dev)
     if torch.is_grad_enabled() and (rewards.requires_grad or values.requires_grad or (
@@ -312,6 +324,7 @@ def _per_row(lead, dtype, dev, old_logp, advantages, ref_logp, mask):
 
 def _evaluate(gaussian: bool, width: int, strides, clip, coefs, head, log_std, actions, old, adv,
               ref, mask) -> PolicyLoss:
+    _no_tangents("the policy loss", head, log_std, actions, old, adv, ref)
     lib = _lib.load()
     stream = _lib.stream_of(head.device)
     (low, high), (kl_c, ent_c, total) = clip, coefs

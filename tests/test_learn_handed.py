@@ -7,6 +7,7 @@ import ctypes
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 from torch.utils.checkpoint import checkpoint
 
 from swarp_amd import _lib, adamw_state, adamw_step, grad_norm, optim, policy
@@ -226,3 +227,30 @@ def test_adamw_and_negated_views(library):
     s = adamw_state(p)
     with pytest.raises(ValueError, match="exp_avg"):
         adamw_step(p, g, s._replace(exp_avg=neg(s.exp_avg)), 1)
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_derivatives_are_refused(library, grad):
+    """A tangent is not dropped in silence, whichever input has it."""
+    def dual(*s):
+        return forward_ad.make_dual(torch.zeros(*s), torch.ones(*s))
+    act = torch.zeros(6, dtype=torch.int64)
+    z = torch.zeros(6)
+    with forward_ad.dual_level():
+        h = torch.zeros(6, 2, requires_grad=grad)
+        calls = [lambda: policy.gae(dual(3), torch.zeros(4, requires_grad=grad)),
+                 lambda: policy.gae(torch.zeros(3, requires_grad=grad), dual(4)),
+                 lambda: policy.gae(z[:3], torch.zeros(4), None, None, dual(3)),
+                 lambda: policy.categorical_policy_loss(dual(6, 2), act, z, z),
+                 lambda: policy.categorical_policy_loss(h, act, dual(6), z),
+                 lambda: policy.categorical_policy_loss(h, act, z, dual(6)),
+                 lambda: policy.categorical_policy_loss(h, act, z, z, dual(6)),
+                 lambda: policy.gaussian_policy_loss(dual(6, 2), torch.zeros(2), h.detach(), z, z),
+                 lambda: policy.gaussian_policy_loss(h, dual(2), h.detach(), z, z),
+                 lambda: policy.gaussian_policy_loss(h, torch.zeros(2), dual(6, 2), z, z)]
+        for call in calls:
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        assert not library.calls
+        policy.gae(z[:3], torch.zeros(4))  # nothing dual: as ever
+    assert len(library.calls) == 1
