@@ -101,7 +101,8 @@ __device__ __forceinline__ A decide(const Row<A> &r, int64_t i, L lp, A H, Terms
     A g = clipped ? A(0) : -first;
     if (r.klc != A(0)) {
         l += r.klc * kl;
-        g -= r.klc * (kl + e);
+        // (exp(e) - 1; a reference that forbids the action makes kl infinite, this -1)
+        g -= r.klc * (e < A(-80) ? A(-1) : kl + e);
     }
     if (r.entc != A(0)) l -= r.entc * H;
     t.loss += l;

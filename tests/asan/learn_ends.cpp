@@ -1,0 +1,158 @@
+// The kernels of the policy update on the host under the sanitizers, at the ends of the number
+// range: one case a run, named by the argument.  All outputs start as NaN, and a comparison that
+// meets one fails, so an element that is never written shows.
+#include <math.h>
+#include <stdio.h>
+#include <string.h>
+
+#include <string>
+#include <vector>
+
+#include "learn.hpp"
+
+// device functions of the GPU build that the host build has by other names
+inline float __builtin_amdgcn_exp2f(float x) { return exp2f(x); }
+inline float __builtin_amdgcn_logf(float x) { return log2f(x); }
+inline void __builtin_amdgcn_sched_barrier(int) {}
+struct alignas(16) float4 {
+    float x, y, z, w;
+};
+inline float4 make_float4(float x, float y, float z, float w) { return {x, y, z, w}; }
+
+namespace g {
+#include "gae.hip"
+}
+namespace p {
+#include "policy.hip"
+}
+namespace o {
+#include "adamw.hip"
+}
+
+namespace swarp {
+std::string message;
+int set_error(const char *m)
+{
+    message = m;
+    return m[0] ? -1 : 0;
+}
+}  // namespace swarp
+
+namespace {
+
+template <typename T> struct Code;
+template <> struct Code<float> { static constexpr int value = SWARP_F32; };
+template <> struct Code<double> { static constexpr int value = SWARP_F64; };
+template <> struct Code<learn::bf16> { static constexpr int value = SWARP_BF16; };
+template <> struct Code<learn::f16> { static constexpr int value = SWARP_F16; };
+
+// 1 and a line where got is not within tol of want; infinities have to be the same, and a NaN
+// meets only a NaN that is wanted.
+int differs(const char *what, double got, double want, double tol)
+{
+    const bool same = isnan(want) ? isnan(got) : isinf(want) ? got == want : fabs(got - want) <= tol;
+    if (!same) printf("%s: %.17g, not %.17g (within %g)\n", what, got, want, tol);
+    return !same;
+}
+
+// A policy loss over `n` decisions and its gradients for an upstream gradient of 1.
+template <typename T> struct Loss {
+    typedef typename learn::Acc<T>::type A;
+    int n, width;
+    bool gauss, shared;
+    std::vector<T> head, std, d_head, d_std;
+    std::vector<A> old, adv, ref, logp, loss, stats, taken;
+    std::vector<int64_t> actions;
+    std::vector<uint8_t> mask;
+    std::vector<double> work;
+    swarp_policy_t a = {};
+
+    Loss(int n, int width, bool gauss = false, bool shared = false)
+        : n(n), width(width), gauss(gauss), shared(shared), head((size_t)n * width, (T)0.0f),
+          std(!gauss ? 0 : shared ? width : (size_t)n * width, (T)0.0f),
+          d_head((size_t)n * width, (T)NAN), d_std(std.size(), (T)NAN), old(n, A(-1)), adv(n, A(1)),
+          logp(n, A(NAN)), loss(1, A(NAN)), stats(3, A(NAN)), taken(gauss ? (size_t)n * width : 0, A(0)),
+          actions(n, 0), work(swarp_policy_work_bytes(n, width) / 8, NAN)
+    {
+        a.dtype = Code<T>::value;
+        a.width = width;
+        a.shared_std = shared;
+        a.rows = n;
+        a.inner = n;
+        a.inner_stride = width;
+        a.clip_low = 0.2;
+        a.clip_high = 0.3;
+    }
+    int run()
+    {
+        a.head = head.data();
+        a.log_std = gauss ? std.data() : nullptr;
+        a.actions = gauss ? (const void *)taken.data() : (const void *)actions.data();
+        a.old_logp = old.data();
+        a.advantages = adv.data();
+        a.ref_logp = ref.empty() ? nullptr : ref.data();
+        a.mask = mask.empty() ? nullptr : mask.data();
+        a.logp = logp.data();
+        a.loss = loss.data();
+        a.stats = stats.data();
+        a.d_head = d_head.data();
+        a.d_log_std = gauss ? d_std.data() : nullptr;
+        a.work = work.data();
+        a.work_bytes = work.size() * 8;
+        const int rc = gauss ? swarp_gaussian_loss(&a, nullptr) : swarp_categorical_loss(&a, nullptr);
+        if (rc) printf("refused: %s\n", swarp::message.c_str());
+        return rc != 0;
+    }
+};
+
+// A reference that forbids the action taken: the loss is infinite, its slope along the
+// log-probability g = -rho A + kl_coef (as exp(e) is 0), and the gradients are that times the
+// head's.  Uniform logits, a unit Gaussian at its mean: rho = 1 with the old log-probability.
+template <typename T> int forbidden(double tol)
+{
+    const double klc = 0.25;
+    int bad = 0;
+    for (int V : {3, 40, 4100}) {
+        Loss<T> c(4, V);
+        c.a.kl_coef = klc;
+        c.ref.assign(4, (typename Loss<T>::A)(-log(V)));
+        c.old = c.ref;
+        c.ref[1] = -INFINITY;
+        c.actions = {0, V - 1, 1, 0};
+        bad += c.run();
+        bad += differs("loss", c.loss[0], INFINITY, 0) + differs("kl", c.stats[1], INFINITY, 0);
+        for (int i = 0; i < 4; ++i)
+            for (int j = 0; j < V; ++j) {
+                const double gi = i == 1 ? -1 + klc : -1;
+                bad += differs("d_logits", (double)c.d_head[(size_t)i * V + j],
+                               gi * ((j == c.actions[i]) - 1.0 / V) / 4, tol);
+            }
+    }
+    for (int D : {2, 6})
+        for (int shared = 0; shared < 2; ++shared) {
+            Loss<T> c(3, D, true, shared);
+            c.a.kl_coef = klc;
+            c.taken.assign(c.taken.size(), 1);  // z = 1: dl/dmu = g, dl/dls = 0
+            c.ref.assign(3, (typename Loss<T>::A)(D * (-0.5 - 0.5 * log(2 * M_PI))));
+            c.old = c.ref;
+            c.ref[2] = -INFINITY;
+            bad += c.run();
+            bad += differs("loss", c.loss[0], INFINITY, 0);
+            for (size_t k = 0; k < c.d_head.size(); ++k)
+                bad += differs("d_mean", (double)c.d_head[k], (k / D == 2 ? -1 + klc : -1) / 3, tol);
+            for (size_t k = 0; k < c.d_std.size(); ++k) bad += differs("d_log_std", (double)c.d_std[k], 0, tol);
+        }
+    return bad;
+}
+
+}  // namespace
+
+int main(int argc, char **argv)
+{
+    const std::string what = argc > 1 ? argv[1] : "";
+    int bad = -1;
+    // a few roundings of terms of size 1: 16 of the type's
+    if (what == "forbidden") bad = forbidden<float>(0x1p-20) + forbidden<double>(0x1p-48) + forbidden<learn::f16>(0x1p-9);
+    printf("%s: %d wrong\n", what.c_str(), bad);
+    return bad != 0;
+}

@@ -126,3 +126,29 @@ def test_overlapping_parameters_are_refused():
     p = [b[:300], b[300:400]]
     adamw_step(p, [torch.ones_like(x) for x in p], adamw_state(p), 1)
     assert bool(b[:400].all()) and not b[400:].any()
+
+
+# ------------------------------------------------------------- ends of the number range
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64, torch.bfloat16])
+@pytest.mark.parametrize("V", [3, 40, 4100, 9000])
+def test_a_reference_that_forbids_the_action(V, dtype):
+    """The loss is infinite, its slope along the log-probability is -rho A + kl_coef."""
+    wide = torch.float64 if dtype == torch.float64 else torch.float32
+    x = torch.zeros(4, V, device=DEV, dtype=dtype, requires_grad=True)
+    act = torch.tensor([0, V - 1, 1, 0], device=DEV)
+    old = torch.full((4,), -math.log(V), device=DEV, dtype=wide)
+    ref = old.clone()
+    ref[1] = -math.inf
+    r = categorical_policy_loss(x, act, old, torch.ones_like(old), ref, kl_coef=0.25)
+    r.loss.backward()
+    assert float(r.loss) == math.inf and float(r.kl) == math.inf
+    slope = torch.tensor([-1.0, -0.75, -1.0, -1.0], device=DEV, dtype=torch.float64)
+    want = torch.full((4, V), -1 / V, device=DEV, dtype=torch.float64)
+    want[torch.arange(4), act] += 1
+    want *= slope[:, None] / 4
+    # rho is off by a rounding of log V (9.1 at most), a handful more; one to the head's type
+    tol = 16 * 2.0 ** (-53 if dtype == torch.float64 else -24) + (
+        2.0 ** -8 * want.abs() if dtype == torch.bfloat16 else 0.0)
+    assert bool(((x.grad.double() - want).abs() <= tol).all())
