@@ -145,6 +145,27 @@ template <typename T> int forbidden(double tol)
     return bad;
 }
 
+// The KL term of a decision whose log-probability is exactly 0 (its only action), for reference
+// log-probabilities e of all sizes: e^2 / 2 + e^3 / 6 + ..., to a few roundings of itself.
+template <typename T> int kl(double least, double most, double tol)
+{
+    int bad = 0;
+    for (double size = least; size <= most; size *= 20)
+        for (double e : {size, -size}) {
+            Loss<T> c(1, 1);
+            c.a.kl_coef = 1;
+            c.adv[0] = 0;
+            c.ref.assign(1, (typename Loss<T>::A)e);
+            long double want = 0, term = 1, x = c.ref[0];
+            for (int k = 1; k < 60; ++k) {
+                term *= x / k;
+                if (k > 1) want += term;
+            }
+            bad += c.run() + differs("kl", c.stats[1], (double)want, tol * (double)want);
+        }
+    return bad;
+}
+
 }  // namespace
 
 int main(int argc, char **argv)
@@ -153,6 +174,8 @@ int main(int argc, char **argv)
     int bad = -1;
     // a few roundings of terms of size 1: 16 of the type's
     if (what == "forbidden") bad = forbidden<float>(0x1p-20) + forbidden<double>(0x1p-48) + forbidden<learn::f16>(0x1p-9);
+    // 16 roundings; above 1/2 the difference from e loses a digit in four, and float's exp two more
+    if (what == "kl") bad = kl<float>(1e-15, 0.5, 0x1p-20) + kl<double>(1e-17, 3.0, 0x1p-49);
     printf("%s: %d wrong\n", what.c_str(), bad);
     return bad != 0;
 }

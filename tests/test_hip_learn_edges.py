@@ -3,6 +3,7 @@ or computed again, derivatives and views that it does not read, overlapping para
 the ends of the number range."""
 
 import math
+from fractions import Fraction
 
 import pytest
 import torch
@@ -152,3 +153,22 @@ def test_a_reference_that_forbids_the_action(V, dtype):
     tol = 16 * 2.0 ** (-53 if dtype == torch.float64 else -24) + (
         2.0 ** -8 * want.abs() if dtype == torch.bfloat16 else 0.0)
     assert bool(((x.grad.double() - want).abs() <= tol).all())
+
+
+def test_the_kl_term_of_small_differences():
+    """With one action the log-probability is 0, and e the reference's: the mean of
+    exp(e) - 1 - e to 16 roundings of itself, in float64 down to where e^2 is lost beside e."""
+    for dtype, sizes in ((torch.float64, (1e-17, 1e-12, 1e-10, 1e-8, 1e-6, 1e-3, 0.1, 0.49, 0.6, 2.0)),
+                         (torch.float32, (1e-12, 1e-8, 1e-4, 0.1, 0.49))):
+        for e in (s * sign for s in sizes for sign in (1, -1)):
+            ref = torch.full((1,), e, device=DEV, dtype=dtype)
+            e = Fraction(float(ref))
+            want, term = Fraction(0), Fraction(1)
+            for k in range(1, 40):
+                term *= e / k
+                want += term if k > 1 else 0
+            z = torch.zeros(1, device=DEV, dtype=dtype)
+            r = categorical_policy_loss(z[:, None], z.long(), z, z, ref, kl_coef=1.0)
+            tol = 16 * 2.0 ** (-53 if dtype == torch.float64 else -24)
+            assert abs(float(r.kl) - float(want)) <= tol * float(want), (dtype, float(e))
+            assert float(r.loss) == float(r.kl)
