@@ -25,7 +25,7 @@ using namespace learn;
 
 template <typename T> struct Args {
     int64_t steps, columns, group;
-    T gamma, carry;  // gamma, gamma * lam
+    T gamma, carry, carries;  // gamma, gamma * lam, the product of a stretch's SEG such factors
     const T *r, *v, *fin;
     const uint8_t *term, *trunc;
     T *adv, *ret;
@@ -34,18 +34,28 @@ template <typename T> struct Args {
     int has_fin;
 };
 
-// x -> a + c x, and one such map after another.
+// x -> a + c x, and one such map after another.  An end of an episode is a factor of -0, which
+// stops NaN and infinities too; every other factor is +0 (lam = 0) or above, and a product of such
+// ones that would underflow is held at the smallest number, so that what is not finite reaches
+// as far through a scan as it does step by step.
 template <typename T> struct Map {
     T a, c;
 };
+__device__ __forceinline__ bool ends(float c) { return (uint32_t)__float_as_int(c) == 0x80000000u; }
+__device__ __forceinline__ bool ends(double c) { return (uint64_t)__double_as_longlong(c) == (uint64_t)1 << 63; }
+constexpr float least(float) { return 0x1p-149f; }
+constexpr double least(double) { return 0x1p-1074; }
+template <typename T> __host__ __device__ __forceinline__ T product(T f, T c)
+{
+    return f > T(0) && c > T(0) && !(f * c > T(0)) ? least(T(0)) : f * c;
+}
 template <typename T> __device__ __forceinline__ Map<T> after(const Map<T> &f, const Map<T> &first)
 {
-    // (a factor of 0 cuts what came before, NaN and infinities with it)
-    return {f.c == T(0) ? f.a : f.a + f.c * first.a, f.c == T(0) ? T(0) : f.c * first.c};
+    return {ends(f.c) ? f.a : f.a + f.c * first.a, ends(f.c) ? f.c : product(f.c, first.c)};
 }
 template <typename T> __device__ __forceinline__ T apply(const Map<T> &f, T x)
 {
-    return f.c == T(0) ? f.a : f.a + f.c * x;
+    return ends(f.c) ? f.a : f.a + f.c * x;
 }
 
 constexpr int SEG = 8;       // steps of a stretch
@@ -56,26 +66,27 @@ template <typename T, int N> struct __attribute__((packed, aligned(sizeof(T)))) 
     T e[N];
 };
 
-// A stretch of steps t0 .. t0 + SEG - 1 of one column; those outside 0 .. L - 1 do nothing.
-// q: two bits a step, terminated and truncated.
+// A stretch of steps t0 .. t0 + SEG - 1 of one column.  One that reaches past the first or the last
+// step is the last in the recurrence's order: nothing is done with its map, and of its steps out
+// there nothing is stored.  q: two bits a step, terminated and truncated.
 template <typename T> struct Stretch {
     T x[SEG], y[SEG + 1];
     uint32_t q;
 
+    __device__ __forceinline__ T factor(const Args<T> &a) const { return q & (1u << 2 * SEG) - 1u ? T(-0.0) : a.carries; }
     // Advantages: x holds the rewards, y the values; leaves x the d_t.
     template <typename Fin> __device__ __forceinline__ Map<T> rewards(const Args<T> &a, int64_t t0, Fin fin)
     {
-        Map<T> m = {T(0), T(1)};
+        T A = T(0);
 #pragma unroll
         for (int k = SEG - 1; k >= 0; --k) {
             const uint32_t e = q >> 2 * k & 3u;
             T next = y[k + 1];
             if (a.has_fin && e == 2u && t0 + k >= 0) next = fin(k);
             x[k] = x[k] + (e & 1u ? T(0) : a.gamma * next) - y[k];
-            const Map<T> s = after(Map<T>{x[k], e ? T(0) : a.carry}, m);
-            m = t0 + k >= 0 ? s : m;
+            A = e ? x[k] : x[k] + a.carry * A;
         }
-        return m;
+        return {A, factor(a)};
     }
     // ... and with A of the step behind carried in, x the advantages, y the returns.
     __device__ __forceinline__ void advantages(const Args<T> &a, T in)
@@ -88,16 +99,15 @@ template <typename T> struct Stretch {
         }
     }
     // The adjoint: x holds gA, y gR (both 0 past the end); q begins one step earlier.
-    __device__ __forceinline__ Map<T> adjoints(const Args<T> &a, int64_t t0)
+    __device__ __forceinline__ Map<T> adjoints(const Args<T> &a)
     {
-        Map<T> m = {T(0), T(1)};
+        T G = T(0);
 #pragma unroll
         for (int k = 0; k < SEG; ++k) {
             x[k] += y[k];
-            const Map<T> s = after(Map<T>{x[k], q >> 2 * k & 3u ? T(0) : a.carry}, m);
-            m = t0 + k < a.steps ? s : m;
+            G = q >> 2 * k & 3u ? x[k] : x[k] + a.carry * G;
         }
-        return m;
+        return {G, factor(a)};
     }
     // ... and with G of the step before carried in, x the adjoints of the rewards, y those of the
     // values (of step L, too, where the stretch reaches it), z those of the final values.
@@ -226,7 +236,7 @@ template <typename T> __global__ __launch_bounds__(64 * MOST_WAVES) void k_gae_b
 #pragma unroll
             for (int k = 0; k <= SEG; ++k) s.q |= (uint32_t)((te[k] ? 1 : 0) | (tr[k] ? 2 : 0)) << 2 * k;
             if (t0 == 0) s.q |= 1u;  // (nothing comes before the first step)
-            m = s.adjoints(a, t0);
+            m = s.adjoints(a);
         }
         join_waves(m, maps, carry, in);
         if (t0 < L && mine) {
@@ -372,7 +382,7 @@ __global__ __launch_bounds__(ROWS_BLOCK) void k_gae_bwd_rows(const Args<T> a, in
                 s.q |= (uint32_t)((te[k] ? 1 : 0) | (tr[k] ? 2 : 0)) << 2 * (k + 1);
                 s.y[k] = gr[k];
             }
-            m = s.adjoints(a, t0);
+            m = s.adjoints(a);
         }
         join_lanes(m, per, totals, carry, in);
         if (some) {
@@ -401,7 +411,9 @@ template <typename T> Args<T> args_of(const swarp_gae_t *a)
     k.columns = a->columns;
     k.group = a->group;
     k.gamma = (T)a->gamma;
-    k.carry = (T)(a->gamma * a->lam);
+    k.carry = (T)(a->gamma * a->lam) + T(0);  // (no -0)
+    k.carries = k.carry;
+    for (int i = 1; i < SEG; ++i) k.carries = product(k.carries, k.carry);
     k.r = (const T *)a->rewards;
     k.v = (const T *)a->values;
     k.fin = (const T *)a->final_values;

@@ -166,6 +166,53 @@ template <typename T> int kl(double least, double most, double tol)
     return bad;
 }
 
+// What is not finite reaches back (the adjoint: on) to the next end of an episode and no further,
+// wherever the stretches of the scan lie, with lam = 0 and with factors whose product underflows.
+template <typename T> int cut(int rows, double lam, T seed)
+{
+    const int L = 300, N = 2;
+    const double carry = (double)(T)(0.5 * lam);
+    std::vector<T> r((size_t)L * N, T(0)), v((size_t)(L + 1) * N, T(0)), adv(r.size(), T(NAN)), ret(adv), d_r(adv),
+        d_v(v.size(), T(NAN)), up(r.size(), T(1));
+    std::vector<uint8_t> te(r.size(), 0);
+    auto at = [&](int t, int n) { return rows ? (size_t)n * L + t : (size_t)t * N + n; };
+    for (size_t i = 0; i < r.size(); ++i) r[i] = T(0.25) * T(i % 7);
+    r[at(290, 0)] = r[at(150, 1)] = seed;
+    up[at(3, 0)] = up[at(200, 1)] = seed;
+    te[at(9, 0)] = te[at(277, 0)] = te[at(100, 1)] = te[at(201, 1)] = 1;
+    swarp_gae_t a = {};
+    a.dtype = Code<T>::value;
+    a.rows = rows;
+    a.steps = L;
+    a.columns = N;
+    a.group = 1;
+    a.gamma = 0.5;
+    a.lam = lam;
+    a.rewards = r.data();
+    a.values = v.data();
+    a.terminated = te.data();
+    a.advantages = adv.data();
+    a.returns = ret.data();
+    a.adj_advantages = up.data();
+    a.adj_rewards = d_r.data();
+    a.adj_values = d_v.data();
+    if (swarp_gae_fwd(&a, nullptr) || swarp_gae_bwd(&a, nullptr)) return printf("refused\n"), 1;
+    int bad = 0;
+    const double tol = 16 * (sizeof(T) == 4 ? 0x1p-24 : 0x1p-53) * 4;  // of values up to 4
+    for (int n = 0; n < N; ++n) {
+        double A = 0, G = 0;
+        for (int t = L - 1; t >= 0; --t) {
+            A = te[at(t, n)] ? (double)r[at(t, n)] : (double)r[at(t, n)] + carry * A;
+            bad += differs("advantage", adv[at(t, n)], A, tol) + differs("return", ret[at(t, n)], A, tol);
+        }
+        for (int t = 0; t < L; ++t) {
+            G = t == 0 || te[at(t - 1, n)] ? (double)up[at(t, n)] : (double)up[at(t, n)] + carry * G;
+            bad += differs("d_rewards", d_r[at(t, n)], G, tol);
+        }
+    }
+    return bad;
+}
+
 }  // namespace
 
 int main(int argc, char **argv)
@@ -176,6 +223,13 @@ int main(int argc, char **argv)
     if (what == "forbidden") bad = forbidden<float>(0x1p-20) + forbidden<double>(0x1p-48) + forbidden<learn::f16>(0x1p-9);
     // 16 roundings; above 1/2 the difference from e loses a digit in four, and float's exp two more
     if (what == "kl") bad = kl<float>(1e-15, 0.5, 0x1p-20) + kl<double>(1e-17, 3.0, 0x1p-49);
+    if (what == "cut") {
+        bad = 0;
+        for (int rows = 0; rows < 2; ++rows)
+            for (double lam : {0.0, -0.0, 0.04, 1e-7, 0.9})
+                for (double seed : {(double)NAN, (double)INFINITY, -(double)INFINITY})
+                    bad += cut<float>(rows, lam, (float)seed) + cut<double>(rows, lam, seed);
+    }
     printf("%s: %d wrong\n", what.c_str(), bad);
     return bad != 0;
 }

@@ -172,3 +172,35 @@ def test_the_kl_term_of_small_differences():
             tol = 16 * 2.0 ** (-53 if dtype == torch.float64 else -24)
             assert abs(float(r.kl) - float(want)) <= tol * float(want), (dtype, float(e))
             assert float(r.loss) == float(r.kl)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
+@pytest.mark.parametrize("last", [False, True])
+@pytest.mark.parametrize("lam", [0.0, 0.04, 1e-7, 0.9])
+def test_what_is_not_finite_reaches_the_next_end(lam, last, dtype):
+    """... and no further, wherever a stretch of the scan begins: A_t = d_t + gamma lam A_{t+1},
+    whose product with 0 is NaN, and whose factors' product underflows over a long way."""
+    T, N = 2500, 6
+    r = torch.randint(-4, 5, (T, N), generator=gen(1), device=DEV).to(dtype)
+    for n, x in enumerate((math.nan, math.inf, -math.inf) * 2):
+        r[2300 - 7 * n, n] = x
+    te = torch.zeros(T, N, dtype=torch.bool, device=DEV)
+    te[1003, :3] = te[2400, 1] = True
+    want, a, h = torch.empty(T, N, dtype=torch.float64), torch.zeros(N, dtype=torch.float64), te.cpu()
+    # (as the call rounds it)
+    carry = float(torch.tensor(0.5 * lam, dtype=dtype))
+    for t in reversed(range(T)):
+        a = torch.where(h[t], r[t].cpu().double(), r[t].cpu().double() + carry * a)
+        want[t] = a
+    v = torch.zeros(T + 1, N, device=DEV, dtype=dtype)
+    if last:
+        r, v, te = (t.T.contiguous() for t in (r, v, te))
+    got = gae(r, v, te, gamma=0.5, lam=lam, time_dim=-1 if last else 0).advantages
+    got = (got.T if last else got).cpu().double()
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(torch.isinf(got), torch.isinf(want))
+    ok = torch.isfinite(want)
+    # sums of at most 4 / (1 - 0.45)
+    assert float((got - want)[ok].abs().max()) <= 64 * 2.0 ** (-24 if dtype == torch.float32 else -53) * 8
+    ok = torch.isinf(want)
+    assert torch.equal(got[ok], want[ok])
