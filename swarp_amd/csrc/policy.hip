@@ -68,18 +68,29 @@ constexpr double LN_2 = 0.69314718055994530942;
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * LOG2E); }
 __device__ __forceinline__ double exp_of(double x) { return exp(x); }
 
-constexpr double factorial(int k) { return k < 2 ? 1.0 : k * factorial(k - 1); }
-
 // expm1(e) - e, without the cancellation of small e (below 1/2 the series to e^9 / 9! in float, to
 // e^15 / 15! in double: the next term is below a tenth of the last digit) and without inf - inf
 // where the action taken has no probability left (beside e^80, e is nothing).
 template <typename A> __device__ __forceinline__ A kl_of(A e)
 {
     if (e > A(80)) return exp_of(e);
-    constexpr int TERMS = sizeof(A) == 4 ? 9 : 15;
-    A s = A(1) / A(factorial(TERMS));
-#pragma unroll
-    for (int k = TERMS - 1; k >= 2; --k) s = s * e + A(1) / A(factorial(k));
+    A s = A(1) / A(362880);
+    if constexpr (sizeof(A) == 8) {
+        s = A(1) / A(1307674368000);
+        s = s * e + A(1) / A(87178291200);
+        s = s * e + A(1) / A(6227020800);
+        s = s * e + A(1) / A(479001600);
+        s = s * e + A(1) / A(39916800);
+        s = s * e + A(1) / A(3628800);
+        s = s * e + A(1) / A(362880);
+    }
+    s = s * e + A(1) / A(40320);
+    s = s * e + A(1) / A(5040);
+    s = s * e + A(1) / A(720);
+    s = s * e + A(1) / A(120);
+    s = s * e + A(1) / A(24);
+    s = s * e + A(1) / A(6);
+    s = s * e + A(0.5);
     const bool small = e < A(0.5) && e > A(-0.5);
     return small ? s * e * e : (sizeof(A) == 4 ? exp_of(e) - A(1) - e : (A)(expm1((double)e) - (double)e));
 }
