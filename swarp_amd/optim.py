@@ -18,7 +18,7 @@ from . import _lib
 from .policy import _CODES, _guard, _on_gpu, _plain, _ptr
 
 GROUP = 256  # elements that share an exponent in an 8-bit moment
-_PARAMS = (torch.float32, torch.bfloat16, torch.float16)
+_PARAMS = {torch.float32: 4, torch.bfloat16: 2, torch.float16: 2}  # and the bytes of each
 
 
 class AdamWState(NamedTuple):
@@ -108,33 +108,33 @@ def _check_state(s: AdamWState, dev) -> None:
 def _table(params, grads, dev):
     """The C table of the tensors that have a gradient, the gradients made for it, the state's
     length, and whether two of the tensors share memory."""
-    n = len(params)
-    table = (_lib.SwarpTensor * max(n, 1))()
+    table = (_lib.SwarpTensor * max(len(params), 1))()
     at, count, keep, starts, ends = 0, 0, [], [], []
-    for k in range(n):
-        p, g = params[k], grads[k]
+    index = -1 if dev.index is None else dev.index  # (which the CPU's tensors say, too)
+    for k, (p, g) in enumerate(zip(params, grads)):
         size = p.numel()
         if g is not None and size:
-            if p.dtype not in _PARAMS:
-                raise TypeError(f"parameter {k}: float32, bfloat16 or float16; got {p.dtype}")
-            if p.device != dev or g.device != dev:
+            dtype, g_dtype = p.dtype, g.dtype
+            if dtype not in _PARAMS:
+                raise TypeError(f"parameter {k}: float32, bfloat16 or float16; got {dtype}")
+            if p.get_device() != index or g.get_device() != index:
                 raise ValueError(f"parameter {k} and its gradient must be on {dev}")
             if not p.is_contiguous() or p.is_neg():
                 raise ValueError(f"parameter {k} must be contiguous, and no negated view")
             if g.shape != p.shape or g.layout != torch.strided:
                 raise ValueError(f"gradient {k} must be a dense {list(p.shape)}; got "
                                  f"{list(g.shape)}")
-            if g.dtype != p.dtype and g.dtype != torch.float32:
-                raise TypeError(f"gradient {k} must be {p.dtype} or float32; got {g.dtype}")
+            if g_dtype is not dtype and g_dtype != torch.float32:
+                raise TypeError(f"gradient {k} must be {dtype} or float32; got {g_dtype}")
             if not g.is_contiguous() or g.is_neg():
                 g = _plain(g)
                 keep.append(g)
             t = table[count]
             start = p.data_ptr()
             starts.append(start)
-            ends.append(start + size * p.element_size())
+            ends.append(start + size * _PARAMS[dtype])
             t.param, t.grad, t.n, t.slot = start, g.data_ptr(), size, at
-            t.param_dtype, t.grad_dtype = _CODES[p.dtype], _CODES[g.dtype]
+            t.param_dtype, t.grad_dtype = _CODES[dtype], _CODES[g_dtype]
             count += 1
         at += -(-size // GROUP) * GROUP
     # (spans are apart if, each list in order, every one ends before the next begins)

@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import math
 from typing import NamedTuple
 
@@ -42,10 +43,13 @@ class PolicyLoss(NamedTuple):
     clip_fraction: torch.Tensor  # share of counted decisions whose ratio the clip held
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _guard(device: torch.device):
     """Makes ``device`` current for the launches inside, where it is not."""
     if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
+        return _HERE
     return torch.cuda.device(device)
 
 
@@ -57,8 +61,6 @@ def _on_gpu(t: torch.Tensor, what: str) -> None:
 
 def _no_tangents(what: str, *tensors: torch.Tensor | None) -> None:
     """Refuses dual tensors, whose tangents the kernels would drop."""
-    if forward_ad._current_level < 0:  # (no forward-mode derivative is being taken)
-        return
     for t in tensors:
         if t is not None and forward_ad.unpack_dual(t).tangent is not None:
             raise NotImplementedError(f"{what} has no forward-mode derivative; it is "
@@ -89,14 +91,14 @@ def _ptr(t: torch.Tensor | None):
     return None if t is None else t.data_ptr()
 
 
-def _like(t: torch.Tensor | None):
-    return None if t is None else (t.shape, t.dtype, t.device)
+def _differentiable_once(backward):
+    """``once_differentiable``, at no cost where no second derivative can be asked for."""
+    guarded = once_differentiable(backward)
 
-
-def _as_saved(t: torch.Tensor | None, like) -> torch.Tensor | None:
-    """A saved tensor whose ``_like`` was ``like``, contiguous: a saved-tensor hook may have given
-    back another one (a checkpoint's recomputation, a copy from the host)."""
-    return None if t is None else _same(t, "a saved tensor", *like)
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
 
 
 # ----------------------------------------------------------------------------- advantages
@@ -126,24 +128,33 @@ class _GaeFn(torch.autograd.Function):
     def forward(ctx, a: _lib.SwarpGae, stream: int, rewards, values, final, term, trunc):
         ctx.set_materialize_grads(False)
         ctx.a, ctx.stream = a, stream
-        ctx.like = (rewards.shape, values.shape, _like(term), _like(trunc))
+        ctx.like = (rewards.shape, values.shape, None if term is None else term.shape,
+                    None if trunc is None else trunc.shape)
         ctx.save_for_backward(term, trunc)
         return _gae_forward(a, rewards, stream)
 
     @staticmethod
-    @once_differentiable
+    @_differentiable_once
     def backward(ctx, g_adv, g_ret):
         if g_adv is None and g_ret is None:
             return (None,) * 7
         r_shape, v_shape, *flags = ctx.like
-        # (unchanged since, or this raises; not the forward's memory where a hook packed them)
-        term, trunc = (_as_saved(t, like) for t, like in zip(ctx.saved_tensors, flags))
-        g_adv, g_ret = (None if g is None else _plain(g) for g in (g_adv, g_ret))
+        if g_adv is not None:
+            g_adv = _plain(g_adv)
+        if g_ret is not None:
+            g_ret = _plain(g_ret)
         ref = g_adv if g_adv is not None else g_ret
         need = ctx.needs_input_grad
         a = _lib.SwarpGae.from_buffer_copy(ctx.a)
         a.rewards = a.values = a.advantages = a.returns = None  # (read by the forward alone)
-        a.terminated, a.truncated = _ptr(term), _ptr(trunc)
+        # (unchanged since, or this raises; not the forward's memory where a hook packed them)
+        term, trunc = ctx.saved_tensors
+        if term is not None and not (term.data_ptr() == a.terminated and term.is_contiguous()):
+            term = _same(term, "a saved tensor", flags[0], torch.bool, ref.device)
+            a.terminated = term.data_ptr()
+        if trunc is not None and not (trunc.data_ptr() == a.truncated and trunc.is_contiguous()):
+            trunc = _same(trunc, "a saved tensor", flags[1], torch.bool, ref.device)
+            a.truncated = trunc.data_ptr()
         d_r = ref.new_empty(r_shape) if need[2] else None
         d_v = ref.new_empty(v_shape) if need[3] else None
         d_f = ref.new_empty(r_shape) if a.final_values and need[4] else None
@@ -204,7 +215,8 @@ def gae(rewards: torch.Tensor, values: torch.Tensor, terminated: torch.Tensor | 
             flags[n] = _same(flags[n], name, timed(T, batch[:k]), torch.bool, dev)
             group = math.prod(batch[k:])
     inputs = (rewards, values, final_values)
-    _no_tangents("gae", *inputs)
+    if forward_ad._current_level >= 0:  # (a forward-mode derivative is being taken)
+        _no_tangents("gae", *inputs)
     a = _scan_args(int(last), T, math.prod(batch), max(group, 1), gamma, lam, *inputs, *flags)
     stream = _lib.stream_of(dev)
     if torch.is_grad_enabled() and (rewards.requires_grad or values.requires_grad or (
@@ -216,10 +228,15 @@ def gae(rewards: torch.Tensor, values: torch.Tensor, terminated: torch.Tensor | 
 # ------------------------------------------------------------------------- policy losses
 
 
+@functools.lru_cache(maxsize=256)
+def _work_bytes(lib, rows: int, width: int) -> int:
+    return lib.swarp_policy_work_bytes(rows, width)
+
+
 def _loss_forward(call, a: _lib.SwarpPolicy, head, old, stream: int):
     """(loss, stats, logp) of a call, and its work memory."""
     dev = head.device
-    nbytes = _lib.load().swarp_policy_work_bytes(a.rows, a.width)
+    nbytes = _work_bytes(_lib.load(), a.rows, a.width)
     work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     loss, stats, logp = old.new_empty(()), old.new_empty(3), torch.empty_like(old)
     a.logp, a.loss, a.stats = logp.data_ptr(), loss.data_ptr(), stats.data_ptr()
@@ -232,29 +249,48 @@ def _loss_forward(call, a: _lib.SwarpPolicy, head, old, stream: int):
 def _buffers(head, log_std, need):
     """Gradient buffers of the heads that want one."""
     return (torch.empty_like(head, memory_format=torch.contiguous_format) if need[0] else None,
-            torch.empty_like(log_std) if need[1] else None)
+            torch.empty_like(log_std, memory_format=torch.contiguous_format) if need[1] else None)
 
 
-def _relocated(a: _lib.SwarpPolicy, saved, like):
-    """A copy of a forward's arguments that reads the saved tensors where they now lie; the head,
-    the deviations, and all that has to stay until the launch."""
-    head, log_std, *rest = saved
-    shape, dtype, dev = like[0]
+def _unmoved(a: _lib.SwarpPolicy, strides, head, log_std, actions, old, adv, ref, mask) -> bool:
+    """Whether saved tensors lie where and as the forward read them.  (Without a hook they do.  What
+    a hook gives back has the values, size and type of what it took, but may be laid otherwise.
+    Written out: this is on the path of every training step.)"""
+    return (head.data_ptr() == a.head and head.stride() == strides and not head.is_neg()
+            and old.data_ptr() == a.old_logp and old.is_contiguous() and not old.is_neg()
+            and adv.data_ptr() == a.advantages and adv.is_contiguous() and not adv.is_neg()
+            and actions.data_ptr() == a.actions and actions.is_contiguous() and not actions.is_neg()
+            and (log_std is None or log_std.data_ptr() == a.log_std and log_std.is_contiguous()
+                 and not log_std.is_neg())
+            and (ref is None or ref.data_ptr() == a.ref_logp and ref.is_contiguous()
+                 and not ref.is_neg())
+            and (mask is None or mask.data_ptr() == a.mask and mask.is_contiguous()))
+
+
+def _relocated(a: _lib.SwarpPolicy, like, head, log_std, actions, *rows):
+    """A copy of a forward's arguments that reads saved tensors where they now lie, and all that has
+    to stay until the launch."""
+    shape, _, dtype, act = like
+    dev, lead = rows[0].device, shape[:-1]
     if head.shape != shape or head.dtype != dtype or head.device != dev:
         raise RuntimeError(f"a saved head came back as {list(head.shape)} {head.dtype} on "
                            f"{head.device}; it was {list(shape)} {dtype} on {dev}")
-    strides = _row_strides(head) if log_std is None and not head.is_neg() else None
+    gaussian = log_std is not None
+    strides = None if gaussian or head.is_neg() else _row_strides(head)
     if strides is None:
         head = _plain(head)
-        strides = (1, 0, 0) if log_std is not None else _row_strides(head)
-    log_std = _as_saved(log_std, like[1])
-    rest = [_as_saved(t, x) for t, x in zip(rest, like[2:])]
+        strides = (1, 0, 0) if gaussian else _row_strides(head)
+    if gaussian:
+        log_std = _same(log_std, "a saved tensor", shape[-1:] if a.shared_std else shape, dtype, dev)
+    wide = torch.float64 if dtype is torch.float64 else torch.float32
+    rest = [t if t is None else _same(t, "a saved tensor", s, kind, dev) for t, s, kind in
+            zip((actions, *rows), (shape if gaussian else lead, lead, lead, lead, lead),
+                (act, wide, wide, wide, torch.bool))]
     a = _lib.SwarpPolicy.from_buffer_copy(a)
     a.inner, a.outer_stride, a.inner_stride = strides
     a.head, a.log_std = head.data_ptr(), _ptr(log_std)
     a.actions, a.old_logp, a.advantages, a.ref_logp, a.mask = (_ptr(t) for t in rest)
-    a.logp = a.loss = a.stats = None  # (of the forward alone)
-    return a, head, log_std, rest
+    return a, (head, log_std, rest)
 
 
 class _LossFn(torch.autograd.Function):
@@ -278,23 +314,30 @@ class _LossFn(torch.autograd.Function):
             ctx.made = _buffers(head, log_std, ctx.need)
             a.d_head, a.d_log_std = _ptr(ctx.made[0]), _ptr(ctx.made[1])
         loss, stats, logp, ctx.work = _loss_forward(calls[0], a, head, rest[1], stream)
-        ctx.like = [_like(t) for t in (head, log_std, *rest)]
+        ctx.like = head.shape, head.stride(), head.dtype, rest[0].dtype
         ctx.save_for_backward(head, log_std, *rest)
         ctx.mark_non_differentiable(stats, logp)
         return loss, stats, logp
 
     @staticmethod
-    @once_differentiable
+    @_differentiable_once
     def backward(ctx, g, *_):
         if g is None:
             return (None,) * 10
+        saved = ctx.saved_tensors  # (unchanged since, or this raises)
         call, a, stream = ctx.call
-        # (unchanged since, or this raises)
-        a, head, log_std, keep = _relocated(a, ctx.saved_tensors, ctx.like)
+        keep = None
+        if not _unmoved(a, ctx.like[1], *saved):
+            a, keep = _relocated(a, ctx.like, *saved)
+        if g.is_neg():
+            g = g.resolve_neg()
         made, ctx.made = ctx.made, None  # handed out once: the caller may change them
-        d = _buffers(head, log_std, ctx.need) if made is None else made
-        a.d_head, a.d_log_std = _ptr(d[0]), _ptr(d[1])
-        g = _plain(g)
+        if made is None:
+            d = _buffers(saved[0], saved[1], ctx.need)
+            a = _lib.SwarpPolicy.from_buffer_copy(a)
+            a.d_head, a.d_log_std = _ptr(d[0]), _ptr(d[1])
+        else:
+            d = made  # (where the forward's arguments say)
         # (autograd runs this with the forward's device and stream current)
         _lib.check(call(ctypes.byref(a), int(made is not None), g.data_ptr(), stream))
         return None, None, None, *d, None, None, None, None, None
@@ -307,24 +350,28 @@ def _clip_of(clip) -> tuple[float, float]:
     return float(low), float(high)
 
 
+def _constant(t: torch.Tensor, name: str, shape, dtype, dev) -> torch.Tensor:
+    t = _same(t, name, shape, dtype, dev)
+    if t.requires_grad:
+        raise ValueError(f"{name} requires grad, but the loss treats it as a constant: detach it")
+    return t
+
+
 def _per_row(lead, dtype, dev, old_logp, advantages, ref_logp, mask):
     """The per-decision inputs, checked."""
-    out = []
-    for name, t in (("old_logp", old_logp), ("advantages", advantages), ("ref_logp", ref_logp)):
-        if t is not None:
-            t = _same(t, name, lead, dtype, dev)
-            if t.requires_grad:
-                raise ValueError(f"{name} requires grad, but the loss treats it as a constant: "
-                                 "detach it")
-        out.append(t)
+    old_logp = _constant(old_logp, "old_logp", lead, dtype, dev)
+    advantages = _constant(advantages, "advantages", lead, dtype, dev)
+    if ref_logp is not None:
+        ref_logp = _constant(ref_logp, "ref_logp", lead, dtype, dev)
     if mask is not None:
         mask = _same(mask, "mask", lead, torch.bool, dev)
-    return (*out, mask)
+    return old_logp, advantages, ref_logp, mask
 
 
 def _evaluate(gaussian: bool, width: int, strides, clip, coefs, head, log_std, actions, old, adv,
               ref, mask) -> PolicyLoss:
-    _no_tangents("the policy loss", head, log_std, actions, old, adv, ref)
+    if forward_ad._current_level >= 0:
+        _no_tangents("the policy loss", head, log_std, actions, old, adv, ref)
     lib = _lib.load()
     stream = _lib.stream_of(head.device)
     (low, high), (kl_c, ent_c, total) = clip, coefs
@@ -457,9 +504,7 @@ def gaussian_policy_loss(
             raise ValueError(f"log_std {list(log_std.shape)} does not broadcast to mean "
                              f"{list(mean.shape)}") from None
     wide = torch.float64 if mean.dtype == torch.float64 else torch.float32
-    actions = _same(actions, "actions", mean.shape, wide, dev)
-    if actions.requires_grad:
-        raise ValueError("actions requires grad, but the loss treats it as a constant: detach it")
+    actions = _constant(actions, "actions", mean.shape, wide, dev)
     rest = _per_row(lead, wide, dev, old_logp, advantages, ref_logp, mask)
     coefs = _coefs(kl_coef, entropy_coef, reduction)
     return _evaluate(True, D, (1, 0, 0), _clip_of(clip), coefs, _plain(mean),

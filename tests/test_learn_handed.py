@@ -254,3 +254,17 @@ def test_forward_mode_derivatives_are_refused(library, grad):
         assert not library.calls
         policy.gae(z[:3], torch.zeros(4))  # nothing dual: as ever
     assert len(library.calls) == 1
+
+
+def test_a_second_derivative_is_refused(library):
+    """... as ``once_differentiable`` does: where the upstream gradient is to be differentiated."""
+    head = torch.randn(6, 2, requires_grad=True)
+    up = torch.ones((), requires_grad=True)
+    g, = torch.autograd.grad(loss_of("cat", head, None, 6), head, up, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()
+    r = torch.zeros(3, requires_grad=True)
+    g, = torch.autograd.grad(policy.gae(r, torch.zeros(4)).advantages, r, up.expand(3),
+                             create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()
