@@ -151,6 +151,14 @@ def _norm_of(table, count, max_norm: float, dev) -> torch.Tensor:
     return out
 
 
+def _check_rates(lr, betas, eps, weight_decay) -> None:
+    if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
+        raise ValueError(f"betas must lie in [0, 1); got {betas}")
+    if not (lr >= 0.0 and eps >= 0.0 and weight_decay >= 0.0):
+        raise ValueError("lr, eps and weight_decay must be >= 0; got "
+                         f"{lr}, {eps} and {weight_decay}")
+
+
 def _check_norm(max_norm: float) -> None:
     if not max_norm > 0:
         raise ValueError(f"the largest norm must be > 0; got {max_norm}")
@@ -195,10 +203,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor | No
         raise ValueError("no parameters")
     if step < 1:
         raise ValueError(f"step counts from 1; got {step}")
-    if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
-        raise ValueError(f"betas must lie in [0, 1); got {betas}")
-    if not (lr >= 0.0 and eps >= 0.0 and weight_decay >= 0.0):
-        raise ValueError("lr, eps and weight_decay must be >= 0")
+    _check_rates(lr, betas, eps, weight_decay)
     if max_grad_norm is not None:
         _check_norm(max_grad_norm)
         if grad_scale is not None:
@@ -258,6 +263,11 @@ class AdamW(torch.optim.Optimizer):
         self._states: dict[int, AdamWState] = {}  # by group
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps,
                                       weight_decay=weight_decay))
+
+    def add_param_group(self, param_group: dict) -> None:
+        rates = self.defaults | param_group
+        _check_rates(*(rates[name] for name in ("lr", "betas", "eps", "weight_decay")))
+        super().add_param_group(param_group)
 
     def __getstate__(self) -> dict:  # (what a copy or a pickle takes along)
         own = ("bits", "master", "max_grad_norm", "seed", "last_grad_norm", "_steps", "_states")
@@ -340,6 +350,8 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError(f"group {k}: the state has {'no' if keeps else 'a'} master copy, "
                                  f"this optimizer keeps {'one' if keeps else 'none'}")
             states[k] = s
+        for new in state["groups"]:
+            _check_rates(*(new[name] for name in ("lr", "betas", "eps", "weight_decay")))
         for g, new in zip(self.param_groups, state["groups"]):
             g.update(new)
         self._states, self._steps, self.seed = states, dict(state["steps"]), state["seed"]

@@ -69,3 +69,25 @@ def test_parameters_that_share_memory_are_found():
     assert not _table([b[:10], h[20:30]], [torch.zeros(10), torch.zeros(10).bfloat16()], b.device)[4]
     # one without a gradient is not touched
     assert not _table([b[:300], b[100:400]], [torch.zeros(300), None], b.device)[4]
+
+
+@pytest.mark.parametrize("rates", [{"lr": -1.0}, {"betas": (2.0, 2.0)}, {"betas": (0.9, 1.0)},
+                                   {"eps": -1e-8}, {"weight_decay": -0.1}, {"lr": float("nan")}])
+def test_rates_are_refused_when_they_are_given(rates):
+    """... to the constructor, in a group, in a group that is added later, in a loaded state."""
+    with pytest.raises(ValueError, match="lr, eps|betas"):
+        AdamW(params(), **rates)
+    with pytest.raises(ValueError, match="lr, eps|betas"):
+        AdamW([{"params": params()}, {"params": params(), **rates}])
+    opt = AdamW(params())
+    with pytest.raises(ValueError, match="lr, eps|betas"):
+        opt.add_param_group({"params": params(), **rates})
+    assert len(opt.param_groups) == 1
+    opt.add_param_group({"params": params(), "lr": 0.5})
+    assert [g["lr"] for g in opt.param_groups] == [1e-3, 0.5]
+    state = AdamW(params()).state_dict()
+    state["groups"][0] |= rates
+    opt = AdamW(params(), seed=3)
+    with pytest.raises(ValueError, match="lr, eps|betas"):
+        opt.load_state_dict(state)
+    assert opt.param_groups[0]["lr"] == 1e-3 and opt.seed == 3
