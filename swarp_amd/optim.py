@@ -320,15 +320,29 @@ class AdamW(torch.optim.Optimizer):
                 for p, a in zip(params, _slots(p.numel() for p in params)[0]):
                     s.master[a:a + p.numel()] = p.reshape(-1)
 
+    def _hooks(self, when: str) -> list:
+        """What was registered by ``register_state_dict_pre_hook`` and its like."""
+        return list(getattr(self, f"_optimizer_{when}_hooks", {}).values())
+
     def state_dict(self) -> dict:
         """Hyperparameters, step count and the flat states of the groups."""
-        return {"steps": dict(self._steps), "seed": self.seed,
-                "groups": [{k: v for k, v in g.items() if k != "params"}
-                           for g in self.param_groups],
-                "states": {k: dict(s._asdict()) for k, s in self._states.items()}}
+        for hook in self._hooks("state_dict_pre"):
+            hook(self)
+        state = {"steps": dict(self._steps), "seed": self.seed,
+                 "groups": [{k: v for k, v in g.items() if k != "params"}
+                            for g in self.param_groups],
+                 "states": {k: dict(s._asdict()) for k, s in self._states.items()}}
+        for hook in self._hooks("state_dict_post"):
+            changed = hook(self, state)
+            state = state if changed is None else changed
+        return state
 
     @torch.no_grad()
     def load_state_dict(self, state: dict) -> None:
+        state = dict(state)  # (the caller's own stays as it is)
+        for hook in self._hooks("load_state_dict_pre"):
+            changed = hook(self, state)
+            state = state if changed is None else changed
         if len(state["groups"]) != len(self.param_groups):
             raise ValueError(f"{len(state['groups'])} parameter groups in the state, "
                              f"{len(self.param_groups)} here")
@@ -355,3 +369,5 @@ class AdamW(torch.optim.Optimizer):
         for g, new in zip(self.param_groups, state["groups"]):
             g.update(new)
         self._states, self._steps, self.seed = states, dict(state["steps"]), state["seed"]
+        for hook in self._hooks("load_state_dict_post"):
+            hook(self)

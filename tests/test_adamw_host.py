@@ -1,6 +1,8 @@
 """The optimizer around the AdamW step, without a GPU: what it loads, takes, refuses and tells its
 hooks."""
 
+import pickle
+
 import pytest
 import torch
 
@@ -91,3 +93,32 @@ def test_rates_are_refused_when_they_are_given(rates):
     with pytest.raises(ValueError, match="lr, eps|betas"):
         opt.load_state_dict(state)
     assert opt.param_groups[0]["lr"] == 1e-3 and opt.seed == 3
+
+
+def test_hooks_are_called():
+    """Those of the state dictionary, of its loading (which may replace it) and of a step."""
+    said = []
+    opt = AdamW(params(), seed=3)
+    opt.register_state_dict_pre_hook(lambda o: said.append(("pre", o is opt)))
+    opt.register_state_dict_post_hook(lambda o, s: {**s, "note": "kept"})
+    gone = opt.register_state_dict_post_hook(lambda o, s: said.append("gone"))
+    gone.remove()
+    state = opt.state_dict()
+    assert state["note"] == "kept" and said == [("pre", True)]
+
+    two = AdamW(params(), seed=4)
+    two.register_load_state_dict_pre_hook(lambda o, s: {**s, "seed": 8})
+    two.register_load_state_dict_pre_hook(lambda o, s: s.pop("note") and None)
+    two.register_load_state_dict_post_hook(lambda o: said.append(o.seed))
+    two.load_state_dict(state)
+    assert two.seed == 8 and said[-1] == 8 and state["seed"] == 3 and state["note"] == "kept"
+    opt.register_step_pre_hook(lambda o, args, kwargs: said.append("step"))
+    opt.register_step_post_hook(lambda o, args, kwargs: said.append("stepped"))
+    opt.step()
+    assert said[-2:] == ["step", "stepped"]
+    # a copy is an optimizer like another
+    three = pickle.loads(pickle.dumps(AdamW(params(), seed=5)))
+    assert three.state_dict()["seed"] == 5
+    three.register_state_dict_pre_hook(lambda o: said.append("copy"))
+    three.state_dict()
+    assert said[-1] == "copy"
