@@ -39,6 +39,7 @@ class AdamWState(NamedTuple):
         """Both moments as flat float32 (the state's own tensors where they are)."""
         if self.bits == 32:
             return self.exp_avg, self.exp_avg_sq
+        _on_gpu(self.exp_avg, "AdamWState.moments")
         _check_state(self, self.exp_avg.device)
         m = torch.empty(self.exp_avg.shape, device=self.exp_avg.device)
         v = torch.empty_like(m)

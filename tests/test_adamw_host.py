@@ -6,7 +6,7 @@ import pickle
 import pytest
 import torch
 
-from swarp_amd import AdamW
+from swarp_amd import AdamW, adamw_state
 from swarp_amd.optim import _table
 
 
@@ -122,3 +122,13 @@ def test_hooks_are_called():
     three.register_state_dict_pre_hook(lambda o: said.append("copy"))
     three.state_dict()
     assert said[-1] == "copy"
+
+
+def test_moments_of_a_state_in_host_memory():
+    """32-bit ones are the state's own; 8-bit ones are unpacked by a kernel, which is not handed
+    host addresses."""
+    p = params(torch.float32)
+    s = adamw_state(p)
+    assert s.moments()[0] is s.exp_avg
+    with pytest.raises(RuntimeError, match="HIP device"):
+        adamw_state(p, bits=8).moments()
