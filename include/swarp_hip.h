@@ -488,7 +488,8 @@ int swarp_gaussian_loss_bwd(const swarp_policy_t *a, int32_t skip_unit, const vo
                             void *stream);
 
 /* One tensor of an optimizer step: n elements, whose moments start at element `slot` (a
- * multiple of SWARP_ADAMW_GROUP) of the flat state. */
+ * multiple of SWARP_ADAMW_GROUP) of the flat state.  A step takes at most 2^35 - 2048
+ * elements a tensor. */
 #define SWARP_ADAMW_GROUP 256
 typedef struct swarp_tensor {
     void *param;

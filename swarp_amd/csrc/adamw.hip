@@ -21,6 +21,7 @@ constexpr int GROUP = SWARP_ADAMW_GROUP;
 constexpr int BLOCK = GROUP;
 constexpr int CHUNK = 8 * GROUP;         // elements of a workgroup
 constexpr int MOST_TENSORS = 64;         // of a launch
+constexpr uint32_t MOST_CHUNKS = (1u << 24) - 1;  // of a step's launch: below 2^32 threads
 constexpr int NORM_BLOCKS = 1024;
 
 struct Tensors {
@@ -357,17 +358,17 @@ int check(const swarp_tensor_t *t, int n)
     return 0;
 }
 
-// Fills the table with the tensors from `k` on that `take` accepts, as many as it holds;
-// returns where to go on.
+// Fills the table with the tensors from `k` on that `take` accepts, as many as it holds and `most`
+// chunks (none has more by itself); returns where to go on.
 template <typename Take>
-int fill(Tensors &t, uint32_t &chunks, const swarp_tensor_t *x, int n, int k, Take take)
+int fill(Tensors &t, uint32_t &chunks, const swarp_tensor_t *x, int n, int k, uint32_t most, Take take)
 {
     t.count = 0;
     chunks = 0;
     for (; k < n && t.count < MOST_TENSORS; ++k) {
         if (x[k].n == 0 || !take(x[k])) continue;
         const uint64_t c = (uint64_t)((x[k].n + CHUNK - 1) / CHUNK);
-        if (chunks + c > 0x7fffffffu) break;
+        if (chunks + c > most) break;
         t.param[t.count] = x[k].param;
         t.grad[t.count] = x[k].grad;
         t.n[t.count] = x[k].n;
@@ -385,7 +386,7 @@ void steps(const Step &s, int bits, const swarp_tensor_t *x, int n, int pd, int 
     Tensors t;
     uint32_t chunks;
     for (int k = 0; k < n;) {
-        k = fill(t, chunks, x, n, k, [&](const swarp_tensor_t &y) { return y.param_dtype == pd && y.grad_dtype == gd; });
+        k = fill(t, chunks, x, n, k, MOST_CHUNKS, [&](const swarp_tensor_t &y) { return y.param_dtype == pd && y.grad_dtype == gd; });
         if (!t.count) continue;
         if (bits == 8)
             hipLaunchKernelGGL((k_adamw<P, G, 8>), dim3(chunks), dim3(BLOCK), 0, st, s, t);
@@ -407,6 +408,7 @@ int swarp_adamw(const swarp_adamw_t *a, const swarp_tensor_t *tensors, int32_t n
         const swarp_tensor_t &x = tensors[k];
         if (x.n == 0) continue;
         if (!x.param) return fail("a tensor has no parameter");
+        if (x.n > (int64_t)CHUNK * MOST_CHUNKS) return fail("a tensor's size is out of range");
         if (x.param_dtype != SWARP_F32 && x.param_dtype != SWARP_BF16 && x.param_dtype != SWARP_F16)
             return fail("parameters are float32, bfloat16 or float16");
         if (x.grad_dtype != x.param_dtype && x.grad_dtype != SWARP_F32)
@@ -471,7 +473,7 @@ int swarp_grad_norm(const swarp_tensor_t *tensors, int32_t n_tensors, double max
     int blocks = 0;  // sums set so far: a launch adds to those and sets the others of its grid
     for (int d : {SWARP_F32, SWARP_BF16, SWARP_F16})
         for (int k = 0; k < n_tensors;) {
-            k = fill(t, chunks, tensors, n_tensors, k, [&](const swarp_tensor_t &y) { return y.grad_dtype == d; });
+            k = fill(t, chunks, tensors, n_tensors, k, 0x7fffffffu, [&](const swarp_tensor_t &y) { return y.grad_dtype == d; });
             if (!t.count) continue;
             const int grid = (int)(chunks < NORM_BLOCKS ? chunks : NORM_BLOCKS);
             const dim3 g(grid), b(BLOCK);

@@ -1,12 +1,13 @@
 """The optimizer around the AdamW step, without a GPU: what it loads, takes, refuses and tells its
 hooks."""
 
+import ctypes
 import pickle
 
 import pytest
 import torch
 
-from swarp_amd import AdamW, adamw_state
+from swarp_amd import AdamW, _lib, adamw_state
 from swarp_amd.optim import _table
 
 
@@ -132,3 +133,13 @@ def test_moments_of_a_state_in_host_memory():
     assert s.moments()[0] is s.exp_avg
     with pytest.raises(RuntimeError, match="HIP device"):
         adamw_state(p, bits=8).moments()
+
+
+def test_a_tensor_too_large_for_a_launch_is_refused_before_any():
+    """2^35 elements are 2^24 workgroups of 256 threads, one thread more than a launch has: refused
+    with the arguments, not by the runtime when other tensors of the step are already written."""
+    lib, n = _lib.load(), 1 << 35
+    s = _lib.SwarpAdamW(bits=32, state_len=n, step=1, exp_avg=256, exp_avg_sq=512)
+    t = (_lib.SwarpTensor * 1)(_lib.SwarpTensor(param=64, grad=64, n=n, slot=0))
+    assert lib.swarp_adamw(ctypes.byref(s), t, 1, None) != 0
+    assert b"out of range" in lib.swarp_last_error()
