@@ -48,6 +48,7 @@ struct Step {
     float b1, a1, b2, a2;     // beta1, 1 - beta1, beta2, 1 - beta2
     float lr_t, v_t, eps, keep;  // lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t), eps, 1 - lr wd
     uint32_t seed;
+    int careful;  // whether the root of a v below the smallest normal number counts beside eps
     void *m, *v;
     uint8_t *m_base, *v_base;
     float *master;
@@ -204,9 +205,24 @@ __global__ __launch_bounds__(BLOCK) void k_adamw(const Step s, const Tensors t)
             const float x = s.scale ? g[u][e] * scale : g[u][e];
             m[u][e] = m[u][e] * s.b1 + x * s.a1;
             v[u][e] = v[u][e] * s.b2 + x * x * s.a2;
-            // (the root and the quotient to an ulp or two: a fraction of an update that is itself a
-            // thousandth of the parameter; the moments, which accumulate, are exact)
-            const float den = __builtin_fmaf(__builtin_amdgcn_sqrtf(v[u][e]), s.v_t, s.eps);
+        }
+        // (the root and the quotient to an ulp or two: a fraction of an update that is itself a
+        // thousandth of the parameter; the moments, which accumulate, are exact.  The instruction
+        // takes a v below the smallest normal number for 0: one it matters for is scaled)
+        float root[4];
+        if (s.careful) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const bool tiny = v[u][e] < 0x1p-96f;
+                root[e] = __builtin_amdgcn_sqrtf(tiny ? v[u][e] * 0x1p32f : v[u][e]) * (tiny ? 0x1p-16f : 1.0f);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) root[e] = __builtin_amdgcn_sqrtf(v[u][e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float den = __builtin_fmaf(root[e], s.v_t, s.eps);
             w[u][e] = __builtin_fmaf(-s.lr_t, m[u][e] * __builtin_amdgcn_rcpf(den), w[u][e] * s.keep);
             r[e] = mix(place + (uint32_t)e * PLACE);
             if (BITS == 8 && (whole || (int)at + e < left)) {
@@ -426,6 +442,7 @@ int swarp_adamw(const swarp_adamw_t *a, const swarp_tensor_t *tensors, int32_t n
     s.lr_t = (float)(a->lr / c1);
     s.v_t = (float)(1.0 / sqrt(c2));
     s.eps = (float)a->eps;
+    s.careful = s.v_t * 0x1p-63f > s.eps * 0x1p-25f;
     s.keep = (float)(1.0 - a->lr * a->weight_decay);
     s.seed = a->seed;
     s.m = a->exp_avg;

@@ -204,3 +204,26 @@ def test_what_is_not_finite_reaches_the_next_end(lam, last, dtype):
     assert float((got - want)[ok].abs().max()) <= 64 * 2.0 ** (-24 if dtype == torch.float32 else -53) * 8
     ok = torch.isinf(want)
     assert torch.equal(got[ok], want[ok])
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-8])
+@pytest.mark.parametrize("size", [1.0, 1e-10, 1e-18, 3e-21])
+def test_adamw_where_second_moments_are_small(size, eps):
+    """The update from the moments that the step stored, in float64: with eps = 0 and second moments
+    down to below the smallest normal float.  A root and a reciprocal of an ulp or two each, three
+    products: 8 roundings of the update, and those of the parameter."""
+    n = 3000
+    g = torch.randn(n, generator=gen(2), device=DEV) * size
+    g = torch.where(g.abs() < 0.1 * size, 0.1 * size, g)
+    p = [torch.zeros(n, device=DEV)]
+    state = adamw_state(p)
+    for t in (1, 2, 3):
+        before = p[0].double()
+        adamw_step(p, [g * t], state, t, lr=0.5, betas=(0.5, 0.75), eps=eps, weight_decay=0.0)
+        m, v = (x[:n].double() for x in state.moments())
+        assert bool((v > 0).all())
+        update = 0.5 * (m / (1 - 0.5 ** t)) / ((v / (1 - 0.75 ** t)).sqrt() + eps)
+        want = before - update
+        tol = 2.0 ** -24 * (8 * update.abs() + want.abs())
+        err = (p[0].double() - want).abs()
+        assert bool((err <= tol).all()), float((err / tol).max())
