@@ -41,7 +41,7 @@ class AdamWState(NamedTuple):
             return self.exp_avg, self.exp_avg_sq
         _on_gpu(self.exp_avg, "AdamWState.moments")
         _check_state(self, self.exp_avg.device)
-        m = torch.empty(self.exp_avg.shape, device=self.exp_avg.device)
+        m = torch.empty(self.exp_avg.shape, device=self.exp_avg.device, dtype=torch.float32)
         v = torch.empty_like(m)
         a = _state_args(self)
         with _guard(m.device):
@@ -75,7 +75,7 @@ def adamw_state(params: Sequence[torch.Tensor], *, bits: int = 32,
             for _ in range(2)]
     copy = None
     if master:
-        copy = torch.zeros(n, device=dev)
+        copy = torch.zeros(n, device=dev, dtype=torch.float32)
         for p, a in zip(params, at):
             copy[a:a + p.numel()] = p.detach().reshape(-1)
     return AdamWState(torch.zeros(n, **z), torch.zeros(n, **z), *base, copy)
@@ -145,7 +145,7 @@ def _table(params, grads, dev):
 
 
 def _norm_of(table, count, max_norm: float, dev) -> torch.Tensor:
-    out = torch.empty(2, device=dev)
+    out = torch.empty(2, device=dev, dtype=torch.float32)
     work = torch.empty(16384, device=dev, dtype=torch.uint8)
     _lib.check(_lib.load().swarp_grad_norm(table, count, max_norm, out.data_ptr(),
                                            work.data_ptr(), _lib.stream_of(dev)))

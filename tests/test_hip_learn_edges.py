@@ -9,7 +9,8 @@ import pytest
 import torch
 from torch.utils.checkpoint import checkpoint
 
-from swarp_amd import adamw_state, adamw_step, categorical_policy_loss, gae, gaussian_policy_loss
+from swarp_amd import (adamw_state, adamw_step, categorical_policy_loss, gae,
+                       gaussian_policy_loss, grad_norm)
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -127,6 +128,23 @@ def test_overlapping_parameters_are_refused():
     p = [b[:300], b[300:400]]
     adamw_step(p, [torch.ones_like(x) for x in p], adamw_state(p), 1)
     assert bool(b[:400].all()) and not b[400:].any()
+
+
+def test_the_default_type_changes_nothing():
+    g = [torch.randn(700, generator=gen(4), device=DEV)]
+
+    def run():
+        p = [torch.ones(700, device=DEV, dtype=torch.bfloat16)]
+        state = adamw_state(p, bits=8, master=True)
+        norm = adamw_step(p, g, state, 1, max_grad_norm=0.5)
+        return (norm, *p, state.master, *state.moments(), *grad_norm(g, 0.5))
+    want = run()
+    torch.set_default_dtype(torch.float64)
+    try:
+        got = run()
+    finally:
+        torch.set_default_dtype(torch.float32)
+    assert all(torch.equal(a, b) and a.dtype == b.dtype for a, b in zip(got, want))
 
 
 # ------------------------------------------------------------- ends of the number range

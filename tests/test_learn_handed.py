@@ -268,3 +268,23 @@ def test_a_second_derivative_is_refused(library):
                              create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         g.sum().backward()
+
+
+@pytest.mark.parametrize("default", [torch.float64, torch.bfloat16])
+def test_the_default_type_is_not_taken_for_float32(library, default):
+    """What the kernels write as float32 is float32, whatever torch makes by default."""
+    torch.set_default_dtype(default)
+    try:
+        p = [torch.zeros(300, dtype=torch.float32)]
+        assert adamw_state(p, master=True).master.dtype == torch.float32
+        assert all(x.dtype == torch.float32 for x in adamw_state(p).moments())
+        assert all(x.dtype == torch.float32 for x in adamw_state(p, bits=8).moments())
+        assert all(x.dtype == torch.float32 for x in grad_norm(p))
+        assert adamw_step(p, p, adamw_state(p), 1, max_grad_norm=1.0).dtype == torch.float32
+        out = policy.gae(p[0], torch.zeros(301, dtype=torch.float32))
+        assert all(x.dtype == torch.float32 for x in out)
+        z = p[0][:6]
+        out = policy.categorical_policy_loss(z[:, None], z.long(), z, z)
+        assert all(x.dtype == torch.float32 for x in out)
+    finally:
+        torch.set_default_dtype(torch.float32)
