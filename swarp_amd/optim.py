@@ -144,11 +144,15 @@ def _table(params, grads, dev):
     return table, count, keep, at, any(map(operator.lt, starts[1:], ends))
 
 
+_SUMS = 4096  # float32 of work memory of the norm, which its results lie behind
+
+
 def _norm_of(table, count, max_norm: float, dev) -> torch.Tensor:
-    out = torch.empty(2, device=dev, dtype=torch.float32)
-    work = torch.empty(16384, device=dev, dtype=torch.uint8)
-    _lib.check(_lib.load().swarp_grad_norm(table, count, max_norm, out.data_ptr(),
-                                           work.data_ptr(), _lib.stream_of(dev)))
+    """The norm and the scale, as elements ``_SUMS`` and ``_SUMS + 1``."""
+    out = torch.empty(_SUMS + 2, device=dev, dtype=torch.float32)
+    work = out.data_ptr()
+    _lib.check(_lib.load().swarp_grad_norm(table, count, max_norm, work + 4 * _SUMS, work,
+                                           _lib.stream_of(dev)))
     return out
 
 
@@ -179,7 +183,7 @@ def grad_norm(grads: Sequence[torch.Tensor | None],
     table, count, keep, *_ = _table(grads, grads, dev)
     with _guard(dev):
         out = _norm_of(table, count, max_norm, dev)
-    return out[0], out[1]
+    return out[_SUMS], out[_SUMS + 1]
 
 
 def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor | None],
@@ -219,7 +223,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor | No
     if state.exp_avg.numel() != n:
         raise ValueError(f"the state holds {state.exp_avg.numel()} elements, these parameters "
                          f"take {n}")
-    if state.master is None and any(p.dtype == torch.float16 for p in params):
+    if state.master is None and torch.float16 in [p.dtype for p in params]:
         raise ValueError("float16 parameters need a master copy (adamw_state(..., master=True))")
     if grad_scale is not None and (grad_scale.numel() != 1 or grad_scale.dtype != torch.float32
                                    or grad_scale.device != dev):
@@ -233,12 +237,12 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor | No
     with _guard(dev):
         if max_grad_norm is not None:
             norm = _norm_of(table, count, max_grad_norm, dev)
-            a.grad_scale = norm.data_ptr() + 4
+            a.grad_scale = norm.data_ptr() + 4 * (_SUMS + 1)
         _lib.check(_lib.load().swarp_adamw(ctypes.byref(a), table, count, _lib.stream_of(dev)))
     # autograd then refuses a backward through what a graph saved of them before
     torch.autograd.graph.increment_version(
         [p for p, g in zip(params, grads) if g is not None and not p.is_inference()])
-    return None if norm is None else norm[0]
+    return None if norm is None else norm[_SUMS]
 
 
 class AdamW(torch.optim.Optimizer):
