@@ -5,6 +5,8 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <algorithm>
+#include <random>
 #include <string>
 #include <vector>
 
@@ -213,6 +215,87 @@ template <typename T> int cut(int rows, double lam, T seed)
     return bad;
 }
 
+// Every gradient element against plain loops, the forward's and those of a backward with an
+// upstream gradient of -2: remainders of spans, -inf logits, masked decisions that hold NaN.
+std::mt19937 rng(5);
+double uni() { return std::uniform_real_distribution<double>(0, 1)(rng); }
+double nrm() { return std::normal_distribution<double>(0, 1)(rng); }
+
+template <typename T> int gradients(int n, int width, bool gauss, bool shared, double tol)
+{
+    typedef typename learn::Acc<T>::type A;
+    const double klc = 0.1, entc = 0.05;
+    Loss<T> c(n, width, gauss, shared);
+    c.a.kl_coef = klc;
+    c.a.entropy_coef = entc;
+    c.ref.resize(n);
+    c.mask.resize(n);
+    double count = 0;
+    for (T &x : c.head) x = (T)(float)nrm();
+    for (T &x : c.std) x = (T)(float)(0.2 * nrm());
+    for (A &x : c.taken) x = (A)nrm();
+    for (int i = 0; i < n; ++i) {
+        c.mask[i] = i == 0 || uni() < 0.7;
+        count += c.mask[i];
+        c.actions[i] = c.mask[i] ? (int64_t)(uni() * width) : -100;
+        c.adv[i] = c.mask[i] ? (A)nrm() : (A)NAN;
+        for (int j = 0; j < width && !gauss; ++j)
+            if (!c.mask[i]) c.head[(size_t)i * width + j] = (T)NAN;
+            else if (j != c.actions[i] && uni() < 0.2) c.head[(size_t)i * width + j] = (T)-INFINITY;
+    }
+    std::vector<double> want(c.head.size(), 0.0), wants(c.std.size(), 0.0);
+    double top = 0, tops = 0;
+    for (int i = 0; i < n; ++i) {
+        if (!c.mask[i]) continue;
+        const T *row = &c.head[(size_t)i * width];
+        double lp = 0, m = -INFINITY, s = 0, H = 0;
+        for (int j = 0; j < width && !gauss; ++j) m = fmax(m, (double)row[j]);
+        for (int j = 0; j < width && !gauss; ++j) s += exp((double)row[j] - m);
+        for (int j = 0; j < width; ++j) {
+            if (gauss) {
+                const double l = (double)c.std[shared ? j : (size_t)i * width + j], z = ((double)c.taken[(size_t)i * width + j] - (double)row[j]) * exp(-l);
+                lp += -0.5 * z * z - l - 0.5 * log(2 * M_PI);
+            } else {
+                const double l = (double)row[j] - m - log(s);
+                if (exp(l) > 0) H -= exp(l) * l;
+                if (j == c.actions[i]) lp = l;
+            }
+        }
+        // (ratios away from the clip's bounds)
+        c.old[i] = (A)(lp - (i % 3 == 0 ? 0.05 : i % 3 == 1 ? 0.5 : -0.5));
+        c.ref[i] = (A)(lp + 0.3 * nrm());
+        const double rho = exp(lp - (double)c.old[i]), b = fmin(fmax(rho, 0.8), 1.3), adv = c.adv[i];
+        const double g = ((b * adv < rho * adv ? 0 : -rho * adv) - klc * expm1((double)c.ref[i] - lp)) / count;
+        for (int j = 0; j < width; ++j) {
+            double &y = want[(size_t)i * width + j];
+            if (gauss) {
+                const size_t k = shared ? j : (size_t)i * width + j;
+                const double l = (double)c.std[k], z = ((double)c.taken[(size_t)i * width + j] - (double)row[j]) * exp(-l);
+                y = g * z * exp(-l);
+                wants[k] += g * (z * z - 1) - entc / count;
+            } else {
+                const double l = (double)row[j] - m - log(s), pj = exp(l);
+                y = g * ((j == c.actions[i]) - pj) + (pj > 0 ? entc * pj * (l + H) / count : 0);
+            }
+            top = fmax(top, fabs(y));
+        }
+    }
+    for (double y : wants) tops = fmax(tops, fabs(y));
+    char what[64];
+    snprintf(what, sizeof what, "%s %d: %d x %d shared %d", gauss ? "gauss" : "cat", Code<T>::value, n, width, shared);
+    int bad = c.run();
+    for (int pass = 0; pass < 2; ++pass) {
+        const double up = pass ? -2 : 1;
+        for (size_t k = 0; k < want.size(); ++k) bad += differs(what, (double)c.d_head[k], up * want[k], tol * 2 * top);
+        for (size_t k = 0; k < wants.size(); ++k) bad += differs(what, (double)c.d_std[k], up * wants[k], tol * 2 * tops);
+        std::fill(c.d_head.begin(), c.d_head.end(), (T)NAN);
+        std::fill(c.d_std.begin(), c.d_std.end(), (T)NAN);
+        A scale = A(-2);
+        if (!pass) bad += gauss ? swarp_gaussian_loss_bwd(&c.a, pass, &scale, nullptr) : swarp_categorical_loss_bwd(&c.a, pass, &scale, nullptr);
+    }
+    return bad;
+}
+
 }  // namespace
 
 int main(int argc, char **argv)
@@ -229,6 +312,19 @@ int main(int argc, char **argv)
             for (double lam : {0.0, -0.0, 0.04, 1e-7, 0.9})
                 for (double seed : {(double)NAN, (double)INFINITY, -(double)INFINITY})
                     bad += cut<float>(rows, lam, (float)seed) + cut<double>(rows, lam, seed);
+    }
+    if (what == "gradients") {
+        bad = 0;
+        // float: log-probabilities of up to 12 to a few roundings, which the ratio takes whole;
+        // 16-bit heads: half a step of the type and that
+        for (int V : {3, 9, 33, 100, 2049, 8200}) bad += gradients<float>(7, V, false, false, 6e-6);
+        for (int V : {5, 40, 129, 4100}) bad += gradients<learn::bf16>(5, V, false, false, 5e-3);
+        bad += gradients<learn::f16>(5, 37, false, false, 1e-3) + gradients<double>(5, 30, false, false, 1e-14 * 8);
+        for (int shared = 0; shared < 2; ++shared) {
+            bad += gradients<float>(70, 2, true, shared, 6e-6) + gradients<float>(21, 5, true, shared, 1.2e-5);
+            bad += gradients<learn::bf16>(33, 3, true, shared, 5e-3) + gradients<learn::f16>(19, 9, true, shared, 1e-3);
+            bad += gradients<double>(11, 17, true, shared, 1e-14 * 8);
+        }
     }
     printf("%s: %d wrong\n", what.c_str(), bad);
     return bad != 0;

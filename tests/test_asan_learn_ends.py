@@ -29,7 +29,7 @@ def exe():
     return exe
 
 
-@pytest.mark.parametrize("case", ["forbidden", "kl", "cut"])
+@pytest.mark.parametrize("case", ["forbidden", "kl", "cut", "gradients"])
 def test_at_the_ends_of_the_range(exe, case):
     r = subprocess.run([str(exe), case], capture_output=True, text=True, timeout=600, cwd="/tmp")
     assert r.returncode == 0 and f"{case}: 0 wrong" in r.stdout, r.stdout[:3000] + r.stderr[-3000:]
