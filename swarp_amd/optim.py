@@ -13,9 +13,10 @@ import operator
 from typing import Iterable, NamedTuple, Sequence
 
 import torch
+from torch.compiler import is_dynamo_compiling
 
 from . import _lib
-from .policy import _CODES, _guard, _on_gpu, _plain, _ptr
+from .policy import _CODES, _guard, _on_gpu, _plain, _ptr, _untraced
 
 GROUP = 256  # elements that share an exponent in an 8-bit moment
 _PARAMS = {torch.float32: 4, torch.bfloat16: 2, torch.float16: 2}  # and the bytes of each
@@ -37,6 +38,8 @@ class AdamWState(NamedTuple):
 
     def moments(self) -> tuple[torch.Tensor, torch.Tensor]:
         """Both moments as flat float32 (the state's own tensors where they are)."""
+        if is_dynamo_compiling():
+            return _untraced(AdamWState.moments)(self)
         if self.bits == 32:
             return self.exp_avg, self.exp_avg_sq
         _on_gpu(self.exp_avg, "AdamWState.moments")
@@ -174,6 +177,8 @@ def grad_norm(grads: Sequence[torch.Tensor | None],
     """``(norm, scale)``, float32 scalars on the device: the 2-norm of all ``grads`` together (in
     a fixed order: the same bits every time) and ``min(1, max_norm / (norm + 1e-6))``, which
     :func:`adamw_step` takes as ``grad_scale``.  No host synchronisation."""
+    if is_dynamo_compiling():
+        return _untraced(grad_norm)(grads, max_norm)
     grads = [_plain(g) for g in grads if g is not None]
     if not grads:
         raise ValueError("no gradients")
@@ -201,6 +206,10 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor | No
     random, in proportion: an update below half a step is not lost on average.  ``seed`` is where
     those random numbers come from: give each step another one.
     """
+    if is_dynamo_compiling():
+        return _untraced(adamw_step)(
+            params, grads, state, step, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay,
+            max_grad_norm=max_grad_norm, grad_scale=grad_scale, seed=seed)
     params, grads = list(params), list(grads)
     if len(params) != len(grads):
         raise ValueError(f"{len(params)} parameters, {len(grads)} gradients")
@@ -291,8 +300,13 @@ class AdamW(torch.optim.Optimizer):
                                           master=bool(self._master_of(k)))
         return self._states[k]
 
-    @torch.no_grad()
     def step(self, closure=None):
+        return self._step(closure)
+
+    @torch.no_grad()
+    def _step(self, closure):
+        if is_dynamo_compiling():
+            return _untraced(AdamW._step)(self, closure)
         loss = None
         if closure is not None:
             with torch.enable_grad():

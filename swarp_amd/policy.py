@@ -19,6 +19,7 @@ from typing import NamedTuple
 import torch
 from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
+from torch.compiler import is_dynamo_compiling
 
 from . import _lib
 
@@ -70,7 +71,7 @@ def _no_tangents(what: str, *tensors: torch.Tensor | None) -> None:
 def _same(t: torch.Tensor, name: str, shape: torch.Size, dtype, device) -> torch.Tensor:
     """``t``, contiguous, after checking its shape, type and device."""
     if (t.shape == shape and t.dtype is dtype and t.device == device and t.is_contiguous()
-            and not t.is_neg()):
+            and (dtype is torch.bool or not t.is_neg())):
         return t
     if t.shape != shape:
         raise ValueError(f"{name} must be {list(shape)}; got {list(t.shape)}")
@@ -89,6 +90,17 @@ def _plain(t: torch.Tensor) -> torch.Tensor:
 
 def _ptr(t: torch.Tensor | None):
     return None if t is None else t.data_ptr()
+
+
+_UNTRACED: dict = {}
+
+
+def _untraced(fn):
+    """``fn`` as torch.compile leaves it alone, with all that it calls: the graph breaks there.
+    (Made when it is first wanted: it imports the compiler.)"""
+    if fn not in _UNTRACED:
+        _UNTRACED[fn] = torch.compiler.disable(fn)
+    return _UNTRACED[fn]
 
 
 def _differentiable_once(backward):
@@ -185,6 +197,9 @@ def gae(rewards: torch.Tensor, values: torch.Tensor, terminated: torch.Tensor | 
     Gradients flow to ``rewards``, ``values`` and ``final_values`` (lambda-returns that are
     differentiated through a rollout); detach them for the usual constant targets.
     """
+    if is_dynamo_compiling():
+        return _untraced(gae)(rewards, values, terminated, truncated, final_values, gamma=gamma,
+                              lam=lam, time_dim=time_dim)
     _on_gpu(rewards, "gae")
     dtype, dev, nd = rewards.dtype, rewards.device, rewards.dim()
     if dtype not in (torch.float32, torch.float64):
@@ -201,7 +216,8 @@ def gae(rewards: torch.Tensor, values: torch.Tensor, terminated: torch.Tensor | 
 
     def timed(steps, lead):
         return torch.Size((*lead, steps) if last else (steps, *lead))
-    rewards = _same(rewards, "rewards", shape, dtype, dev)
+    if not rewards.is_contiguous() or rewards.is_neg():
+        rewards = _plain(rewards)
     values = _same(values, "values", timed(T + 1, batch), dtype, dev)
     if final_values is not None:
         final_values = _same(final_values, "final_values", shape, dtype, dev)
@@ -452,6 +468,10 @@ def categorical_policy_loss(
 
     Gradients flow to ``logits`` alone (:class:`PolicyLoss`).
     """
+    if is_dynamo_compiling():
+        return _untraced(categorical_policy_loss)(
+            logits, actions, old_logp, advantages, ref_logp, mask, clip=clip, kl_coef=kl_coef,
+            entropy_coef=entropy_coef, reduction=reduction)
     _on_gpu(logits, "categorical_policy_loss")
     if logits.dtype not in _CODES:
         raise TypeError(f"logits must be float32, float64, bfloat16 or float16; got {logits.dtype}")
@@ -487,6 +507,10 @@ def gaussian_policy_loss(
     ``ref_logp`` float32 (float64 with a float64 head); ``D <= 64``.  ``logp`` and the entropy are
     sums over the dimensions.  Gradients flow to ``mean`` and ``log_std``.
     """
+    if is_dynamo_compiling():
+        return _untraced(gaussian_policy_loss)(
+            mean, log_std, actions, old_logp, advantages, ref_logp, mask, clip=clip,
+            kl_coef=kl_coef, entropy_coef=entropy_coef, reduction=reduction)
     _on_gpu(mean, "gaussian_policy_loss")
     if mean.dtype not in _CODES:
         raise TypeError(f"mean must be float32, float64, bfloat16 or float16; got {mean.dtype}")

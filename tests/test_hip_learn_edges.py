@@ -9,7 +9,7 @@ import pytest
 import torch
 from torch.utils.checkpoint import checkpoint
 
-from swarp_amd import (adamw_state, adamw_step, categorical_policy_loss, gae,
+from swarp_amd import (AdamW, adamw_state, adamw_step, categorical_policy_loss, gae,
                        gaussian_policy_loss, grad_norm)
 
 pytestmark = pytest.mark.gpu
@@ -145,6 +145,87 @@ def test_the_default_type_changes_nothing():
     finally:
         torch.set_default_dtype(torch.float32)
     assert all(torch.equal(a, b) and a.dtype == b.dtype for a, b in zip(got, want))
+
+
+# --------------------------------------------------------------- without gradients, compiled
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("V", [9, 50, 3000, 20000])
+def test_losses_without_gradients(V, dtype):
+    """The values of a call whose inputs need no gradient, or under no_grad, are those of one that
+    leaves gradients, to the last bit (rows that are split have them formed in other workgroups,
+    whose sums are joined in another order: there to 16 roundings)."""
+    g = gen(V)
+    x = (torch.randn(5, V, generator=g, device=DEV) * 2).to(dtype)
+    act = torch.randint(0, V, (5,), generator=g, device=DEV)
+    old, adv, ref = (torch.randn(5, generator=g, device=DEV) - 3 for _ in range(3))
+    mask = torch.tensor([True, False, True, True, True], device=DEV)
+    std = (torch.randn(5, 7, generator=g, device=DEV) * 0.2).to(dtype)
+
+    def cat(x):
+        return categorical_policy_loss(x, act, old, adv, ref, mask, kl_coef=0.1, entropy_coef=0.1)
+
+    def gauss(x):
+        return gaussian_policy_loss(x, std, x.detach().float() + 0.1, old, adv, ref, mask, kl_coef=0.1,
+                                    entropy_coef=0.1)
+    for f, head in ((cat, x), (gauss, x[:, :7].contiguous())):
+        want = f(head.clone().requires_grad_(True))
+        with torch.no_grad():
+            under = f(head.clone().requires_grad_(True))
+        for got in (f(head), under):
+            assert not any(t.requires_grad for t in got)
+            for a, b in zip(got, want):
+                if V > 8192 and f is cat:
+                    assert bool(((a - b).abs() <= 16 * 2.0 ** -24 * b.abs()).all())
+                else:
+                    assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("backend", ["eager", "inductor"])
+def test_compiled_callers(backend):
+    """torch.compile runs functions that call the operators, with the same results: the graph
+    breaks at them."""
+    g = gen(8)
+    r, v = torch.randn(20, 30, generator=g, device=DEV), torch.randn(21, 30, generator=g, device=DEV)
+    x = torch.randn(30, 9, generator=g, device=DEV, requires_grad=True)
+    act = torch.randint(0, 9, (30,), generator=g, device=DEV)
+
+    def cat(x):
+        adv = gae(r * 2, v).advantages[0] + 0
+        return categorical_policy_loss(x * 2, act, adv - 3, adv, entropy_coef=0.1).loss * 4
+
+    def gauss(x):
+        adv = gae(r * 2, v).advantages[0] + 0
+        return gaussian_policy_loss(x * 2, x[0] * 0.5, x.detach(), adv - 9, adv).loss * 4
+
+    def step(x):
+        p = [x.detach() * 2]
+        state = adamw_state(p, bits=8)
+        norm = adamw_step(p, [x.detach() * 4], state, 1, max_grad_norm=1.0)
+        return (p[0], norm * 2, *grad_norm(p), *state.moments())
+    for f in (cat, gauss):
+        want, compiled = f(x), torch.compile(f, backend=backend)
+        dwant, = torch.autograd.grad(want, x, retain_graph=True)
+        for _ in range(2):
+            got = compiled(x)
+            assert torch.equal(want, got) and torch.equal(torch.autograd.grad(got, x)[0], dwant)
+    want, compiled = step(x), torch.compile(step, backend=backend)
+    for _ in range(2):
+        assert all(torch.equal(a, b) for a, b in zip(compiled(x), want))
+
+
+def test_compiled_optimizer():
+    def go(wrap):
+        p = torch.nn.Parameter(torch.ones(300, device=DEV))
+        opt = AdamW([p], lr=0.1, max_grad_norm=0.5)
+        step = wrap(opt.step)
+        for k in range(3):
+            p.grad = torch.linspace(-1, k, 300, device=DEV)
+            step()
+        return p.detach(), opt.last_grad_norm, opt.state_dict()["steps"]
+    want, got = go(lambda f: f), go(lambda f: torch.compile(f, backend="eager"))
+    assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1]) and want[2] == got[2] == {0: 3}
 
 
 # ------------------------------------------------------------- ends of the number range
