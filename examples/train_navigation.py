@@ -67,27 +67,27 @@ def train(head: str = "gaussian", bits: int = 32, n_envs: int = 1024, n_agents: 
     """Mean reward per step of every iteration."""
     torch.manual_seed(seed)
     env = Environment(NavigationScenario(n_agents=n_agents, world_size=1.0), n_envs=n_envs,
-                      device=device, dt=0.1, max_steps=100, seed=seed, auto_reset=True,
-                      clone_outputs=True)
+                      device=device, dt=0.1, max_steps=100, seed=seed, clone_outputs=True)
     policy = Policy(env.obs_dim, env.act_dim, head).to(device)
     opt = AdamW(policy.parameters(), lr=lr, bits=bits, max_grad_norm=0.5, seed=seed)
     obs = env.reset(seed=seed)
     history = []
     for it in range(iterations):
-        keep = {k: [] for k in ("obs", "choice", "logp", "value", "reward", "term", "trunc")}
+        keep = {k: [] for k in ("obs", "choice", "logp", "value", "reward", "term", "trunc", "next")}
         for _ in range(steps):
             choice, action, logp, value = policy.act(obs)
             new_obs, reward, terminated, truncated, _ = env.step(action)
-            for k, v in zip(keep, (obs, choice, logp, value, reward, terminated, truncated)):
+            for k, v in zip(keep, (obs, choice, logp, value, reward, terminated, truncated,
+                                   new_obs)):
                 keep[k].append(v)
-            obs = new_obs
+            # (envs whose episode ended begin another; what they ended in is kept above)
+            obs = env.reset_at(terminated | truncated).clone()
         roll = {k: torch.stack(v) for k, v in keep.items()}
         with torch.no_grad():
             last = policy(obs)[1]
-            # (the observation an episode ends in is replaced by the reset's: its own value, the
-            # one before it, stands in at time limits)
+            # at a time limit the return goes on with the value of what the episode ended in
             adv, returns = gae(roll["reward"], torch.cat([roll["value"], last[None]]), roll["term"],
-                               roll["trunc"], roll["value"], gamma=0.99, lam=0.95)
+                               roll["trunc"], policy(roll["next"])[1], gamma=0.99, lam=0.95)
             adv = (adv - adv.mean()) / (adv.std() + 1e-6)
         for _ in range(epochs):
             opt.zero_grad(set_to_none=True)
