@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import operator
+import struct
 from typing import Iterable, NamedTuple, Sequence
 
 import torch
@@ -19,6 +20,7 @@ from . import _lib
 from .policy import _CODES, _guard, _on_gpu, _plain, _ptr, _untraced
 
 GROUP = 256  # elements that share an exponent in an 8-bit moment
+_ROW = struct.Struct("QQqqii")  # a ``SwarpTensor``, written in one call
 _PARAMS = {torch.float32: 4, torch.bfloat16: 2, torch.float16: 2}  # and the bytes of each
 
 
@@ -112,9 +114,12 @@ def _check_state(s: AdamWState, dev) -> None:
 def _table(params, grads, dev):
     """The C table of the tensors that have a gradient, the gradients made for it, the state's
     length, and whether two of the tensors share memory."""
-    table = (_lib.SwarpTensor * max(len(params), 1))()
+    rows, write, wide = bytearray(_ROW.size * max(len(params), 1)), _ROW.pack_into, _ROW.size
     at, count, keep, starts, ends = 0, 0, [], [], []
     index = -1 if dev.index is None else dev.index  # (which the CPU's tensors say, too)
+    # (asked of all at once: a step's host time goes by what is asked of each)
+    neg = torch.Tensor.is_neg
+    negated = any(map(neg, params)) or any(map(neg, [g for g in grads if g is not None]))
     for k, (p, g) in enumerate(zip(params, grads)):
         size = p.numel()
         if g is not None and size:
@@ -123,27 +128,27 @@ def _table(params, grads, dev):
                 raise TypeError(f"parameter {k}: float32, bfloat16 or float16; got {dtype}")
             if p.get_device() != index or g.get_device() != index:
                 raise ValueError(f"parameter {k} and its gradient must be on {dev}")
-            if not p.is_contiguous() or p.is_neg():
+            if not p.is_contiguous() or negated and p.is_neg():
                 raise ValueError(f"parameter {k} must be contiguous, and no negated view")
             if g.shape != p.shape or g.layout != torch.strided:
                 raise ValueError(f"gradient {k} must be a dense {list(p.shape)}; got "
                                  f"{list(g.shape)}")
             if g_dtype is not dtype and g_dtype != torch.float32:
                 raise TypeError(f"gradient {k} must be {dtype} or float32; got {g_dtype}")
-            if not g.is_contiguous() or g.is_neg():
+            if not g.is_contiguous() or negated and g.is_neg():
                 g = _plain(g)
                 keep.append(g)
-            t = table[count]
             start = p.data_ptr()
             starts.append(start)
             ends.append(start + size * _PARAMS[dtype])
-            t.param, t.grad, t.n, t.slot = start, g.data_ptr(), size, at
-            t.param_dtype, t.grad_dtype = _CODES[dtype], _CODES[g_dtype]
+            write(rows, count * wide, start, g.data_ptr(), size, at, _CODES[dtype],
+                  _CODES[g_dtype])
             count += 1
         at += -(-size // GROUP) * GROUP
     # (spans are apart if, each list in order, every one ends before the next begins)
     starts.sort()
     ends.sort()
+    table = (_lib.SwarpTensor * max(len(params), 1)).from_buffer(rows)
     return table, count, keep, at, any(map(operator.lt, starts[1:], ends))
 
 
