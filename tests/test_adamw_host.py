@@ -143,3 +143,6 @@ def test_a_tensor_too_large_for_a_launch_is_refused_before_any():
     t = (_lib.SwarpTensor * 1)(_lib.SwarpTensor(param=64, grad=64, n=n, slot=0))
     assert lib.swarp_adamw(ctypes.byref(s), t, 1, None) != 0
     assert b"out of range" in lib.swarp_last_error()
+    # (a call that is accepted clears the message)
+    a = _lib.SwarpGae(dtype=0, steps=0, columns=4, group=1)
+    assert lib.swarp_gae_fwd(ctypes.byref(a), None) == 0 and lib.swarp_last_error() == b""
