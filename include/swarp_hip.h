@@ -410,7 +410,7 @@ int swarp_state_defaults(int32_t dtype, int64_t n, void *buf, void *stream);
  *         V_{t+1};   d_t = r_t + gamma n_t - V_t;
  *   A_t = d_t + (terminated or truncated ? 0 : gamma lam A_{t+1}),  A_T = 0;  R_t = A_t + V_t.
  * Values of a step that is not read (V_{t+1} or final_values_t where the flags say so) may be
- * anything, NaN included. */
+ * anything, NaN included; what else is not finite reaches back to the next end. */
 typedef struct swarp_gae {
     int32_t dtype;            /* SWARP_F32 or SWARP_F64 */
     int32_t rows;             /* 0: time first, arrays [T,N]; 1: time last, arrays [N,T] */
@@ -439,6 +439,7 @@ int swarp_gae_bwd(const swarp_gae_t *a, void *stream);
  *   rho = exp(lp - old_logp);  s = -min(rho A, clamp(rho, 1 - clip_low, 1 + clip_high) A);
  *   kl = exp(q - lp) - 1 - (q - lp);   l = s + kl_coef kl - entropy_coef H;
  *   loss = w sum of l over the decisions whose mask is set, w = 1 / max(1, their number) or 1.
+ * (where q is -inf kl is infinite and its derivative to lp +1)
  * A masked decision's other inputs are not read into any result: its logp is 0, its gradient
  * rows are zero.
  * Categorical head: decision r has the logits at head + (r / inner) outer_stride

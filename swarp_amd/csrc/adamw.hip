@@ -141,10 +141,11 @@ template <typename T> __device__ __forceinline__ void get(float (&x)[4], const T
 // elements of each group: all loads of both groups are in flight before the first is used, and a
 // group's largest exponents are found without LDS or barriers.  (100 M float32 parameters with two
 // groups a wave 490 us, with four 504; 150 M bfloat16 with 8-bit moments 378 and 405.)
-// What bounds it: 32-bit moments, memory: 28 bytes a parameter at 5.7 TB/s.  8-bit ones, the
-// vector units, which are busy 0.9 of the time: some 80 instructions a parameter, the random
-// bits' multiplications, the root and the reciprocal at a quarter of the rate; 10 bytes a
-// parameter at 4.0 TB/s.
+// What bounds it: 32-bit moments, memory: 28 bytes a parameter at 5.6 TB/s (100 M in 490 to 504 us,
+// by the card).  8-bit ones, the vector units, which are busy 0.9 of the time: some 80 instructions a
+// parameter, the random bits' multiplications, the root and the reciprocal at a quarter of the
+// rate; 10 bytes a parameter at 3.9 TB/s.  100 M bfloat16 parameters with 32-bit moments take 414 us,
+// with a master copy 526; float16 ones with a master copy and 8-bit moments 324.
 struct Yes {
     constexpr operator bool() const { return true; }
 };

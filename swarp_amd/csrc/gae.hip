@@ -14,9 +14,10 @@
 //   Time last: the threads of a wave (of 1 to 4, by the length) have consecutive stretches of one
 //   column, joined by a scan over the lanes; a column's arrays are read in spans of SEG steps,
 //   which start anywhere (a column of values is one longer than one of rewards).
-// What bounds it: many columns, memory: 32 x 16000 x 16 float32 in 24.5 us, 132 MB at 5.4 TB/s (a
-// thread that walks its column alone: 52 us).  Few, the latency of two tiles' loads and scans: 96
-// columns of 4095 steps in 10 us, their adjoint in 10 (alone: 3 ms each).
+// What bounds it: many columns, memory: 32 x 16000 x 16 float32 in 24 us, 132 MB at 5.5 TB/s (a
+// thread that walks its column alone: 52 us), its adjoint in 30; half as many columns of float64 in
+// 26 and 27.  Few, the latency of two tiles' loads and scans: 96 columns of 4095 steps in 10 us,
+// their adjoint in 10 (alone: 3 ms each), 13 and 12 in float64.
 #include "learn.hpp"
 
 namespace {

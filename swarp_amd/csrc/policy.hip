@@ -545,7 +545,7 @@ template <typename A> __device__ __forceinline__ bool upstream(const Row<A> &r, 
 // What bounds it: memory from rows of 250 on (800 MB of bfloat16 logits and gradients in 156 to
 // 189 us, of float32 in 152 to 169); below, what each row costs beside its logits (rows of 50:
 // 282 and 247 us).  16-bit rows are held to four waves a SIMD: 133 registers instead of 128 cost
-// rows of 1000 16 us.
+// rows of 1000 16 us.  (Rows of 32 and 64 lanes pay 16 bytes of scratch a thread for that.)
 template <typename T, int LANES, int E>
 __global__ __launch_bounds__(BLOCK, sizeof(T) == 2 ? 4 : 1) void k_cat_lanes(const Row<typename Acc<T>::type> r, const Logits g)
 {

@@ -40,7 +40,7 @@ class PolicyLoss(NamedTuple):
     loss: torch.Tensor           # scalar
     logp: torch.Tensor           # log-probability of each action taken (0 where masked)
     entropy: torch.Tensor        # mean entropy of the counted decisions
-    kl: torch.Tensor             # mean of exp(q - logp) - 1 - (q - logp), q the reference's
+    kl: torch.Tensor             # mean of exp(q - logp) - 1 - (q - logp), q = ref_logp or old_logp
     clip_fraction: torch.Tensor  # share of counted decisions whose ratio the clip held
 
 
@@ -194,8 +194,12 @@ def gae(rewards: torch.Tensor, values: torch.Tensor, terminated: torch.Tensor | 
 
         delta_t = r_t + gamma next_t - V_t;   A_t = delta_t + gamma lam A_{t+1} (0 across an end)
 
+    An end stops NaN and infinities as well, and nothing else does: ``0 * NaN`` is NaN with
+    ``lam=0`` too.
+
     Gradients flow to ``rewards``, ``values`` and ``final_values`` (lambda-returns that are
-    differentiated through a rollout); detach them for the usual constant targets.
+    differentiated through a rollout), once, and backward only; detach them for the usual constant
+    targets.
     """
     if is_dynamo_compiling():
         return _untraced(gae)(rewards, values, terminated, truncated, final_values, gamma=gamma,
@@ -460,13 +464,17 @@ def categorical_policy_loss(
         -min(ratio A, clamp(ratio, 1 - low, 1 + high) A)
             + kl_coef (exp(q - logp) - 1 - (q - logp)) - entropy_coef H
 
-    averaged (``"mean"``) or summed over the decisions that count.  ``clip`` is the bound on both
+    averaged (``"mean"``) or summed over the decisions that count.  The KL term estimates the
+    divergence of this policy from the reference as far as the actions are this policy's; they are
+    the old policy's, so with ``q = old_logp`` it agrees with either divergence of the two to second
+    order in their difference, and is exact for neither.  ``clip`` is the bound on both
     sides, or ``(low, high)``.  Logits of -inf are actions that are not open.  What a masked
     decision holds is not looked at, its action included; with no decision that counts the loss
-    and its gradients are 0.  A decision that counts with NaN or +inf among its logits, with all
+    and its gradients are 0.  An action that the reference forbids (``ref_logp`` of -inf) makes the
+    KL term infinite, its gradient that of ``+kl_coef logp``.  A decision that counts with NaN or +inf among its logits, with all
     of them -inf, or with an action outside ``[0, V)`` makes the loss NaN.
 
-    Gradients flow to ``logits`` alone (:class:`PolicyLoss`).
+    Gradients flow to ``logits`` alone (:class:`PolicyLoss`), once, and backward only.
     """
     if is_dynamo_compiling():
         return _untraced(categorical_policy_loss)(
