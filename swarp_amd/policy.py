@@ -320,8 +320,8 @@ class _LossFn(torch.autograd.Function):
     at hand: a training step then reads the heads once and writes their gradients once.  The
     backward hands them out; where the upstream gradient is not 1 (the device looks) it computes
     them again with it, so each is rounded once, from the tensors that autograd kept: under a
-    checkpoint or a packing hook the forward's own are gone.  float16 gradients are left to the backward:
-    without the loss scale that comes with it they would vanish.
+    checkpoint or a packing hook the forward's own are gone.  float16 gradients are left to the
+    backward: without the loss scale that comes with it they would vanish.
     """
 
     @staticmethod
