@@ -23,7 +23,7 @@
 extern "C" {
 #endif
 
-#define SWARP_ABI_VERSION 17
+#define SWARP_ABI_VERSION 18
 
 #define SWARP_F32 0
 #define SWARP_F64 1
@@ -530,6 +530,79 @@ int swarp_adamw_unpack(const swarp_adamw_t *a, float *avg, float *sq, void *stre
 #define SWARP_NORM_WORK 16384
 int swarp_grad_norm(const swarp_tensor_t *tensors, int32_t n_tensors, double max_norm,
                     float *norm_scale, void *work, void *stream);
+
+/* ------------------------------------------------------------------ a policy with memory */
+
+/* Softmax cross entropy of a linear head, without its logits.  Per row i that counts, with its
+ * target t:
+ *   z_j = hidden_i . weight_j + bias_j;  logp_i = z_t - log sum_j exp(z_j);
+ *   loss = -w sum of logp over the rows that count, w = 1 / their number or 1 (0 if none counts).
+ * Row r of `hidden` lies at (r / inner) outer_stride + (r % inner) inner_stride (in elements).  A
+ * masked row is not read; its logp is 0, its gradient zero.  A row that counts with a target outside
+ * [0, width), with NaN or +inf among its logits, or with all of them -inf, makes the loss NaN.
+ * Where d_hidden, d_weight or d_bias is set the call also leaves the gradients of the summed loss
+ * there, in float, d_hidden with the rows that count moved together; swarp_linear_ce_bwd turns them
+ * into the caller's.  The work memory holds the exponentials of at most 1 GiB of rows (or of 256
+ * rows) at a time, and copies of hidden and weight; the backward does not need it. */
+typedef struct swarp_linear_ce {
+    int32_t dtype;            /* of hidden, weight, bias: SWARP_F32, _BF16 or _F16 */
+    int32_t sum;              /* 1: loss is the sum, 0: the mean */
+    int32_t targets32;        /* targets are int32 (0: int64) */
+    int32_t dim, width;       /* 1 to 65536, 1 to 2^21 */
+    int64_t rows;             /* below 2^31 */
+    int64_t inner, outer_stride, inner_stride; /* inner >= 1 */
+    const void *hidden;
+    const void *weight;       /* [width, dim] */
+    const void *bias;         /* [width] or NULL */
+    const void *targets;      /* [rows] */
+    const uint8_t *mask;      /* [rows], nonzero = counts; NULL: all count */
+    int32_t *place;           /* [rows + 1], with a mask: where each row's gradient lies (-1: none),
+                                 and how many count */
+    float *logp;              /* [rows] */
+    float *loss;              /* [1] */
+    float *d_hidden;          /* [rows, dim], [width, dim], [width], or NULL */
+    float *d_weight, *d_bias;
+    void *work;               /* swarp_linear_ce_work_bytes() bytes, 256-byte aligned */
+    uint64_t work_bytes;
+} swarp_linear_ce_t;
+uint64_t swarp_linear_ce_work_bytes(const swarp_linear_ce_t *a);
+int swarp_linear_ce(const swarp_linear_ce_t *a, void *stream);
+/* d_hidden [rows, dim], d_weight and d_bias of `dtype` (NULL: not wanted) for the upstream gradient
+ * *scale (float, on the device), from what a call with the same arguments left: rounded once. */
+int swarp_linear_ce_bwd(const swarp_linear_ce_t *a, const void *scale, void *d_hidden, void *d_weight,
+                        void *d_bias, void *stream);
+
+/* Linear attention with a decay for each head, along a rollout.  Per batch entry and head, with
+ * the state S [dk, dv] and a step's q, k [dk], v [dv]:
+ *   S_t = (starts_t ? 0 : exp(log_decay) S_{t-1}) + k_t v_t^T;   out_t = scale q_t S_t.
+ * log_decay is not above 0.  An episode that starts stops what came before, NaN and infinities too,
+ * and a step does not look at later ones.  Element (t, b, h, i) of q, k, v lies at
+ * t stride[0] + b stride[1] + h stride[2] + i; of the others at ((t batch + b) heads + h) d + i. */
+typedef struct swarp_decay {
+    int32_t dtype;            /* of q, k, v, out and their gradients: SWARP_F32, _BF16 or _F16 */
+    int32_t heads, dk, dv;    /* 1 <= dk, dv <= 128 */
+    int64_t steps, batch;
+    int64_t group;            /* consecutive batch entries that share their starts */
+    int64_t q_stride[3], k_stride[3], v_stride[3]; /* elements */
+    double scale;
+    const float *log_decay;   /* [heads] */
+    const void *q, *k, *v;
+    const uint8_t *starts;    /* [steps, batch / group], nonzero = an episode starts; NULL: none */
+    const float *state;       /* [batch, heads, dk, dv] before the first step; NULL: zero */
+    void *out;                /* [steps, batch, heads, dv] */
+    float *state_out;         /* as state, after the last step, or NULL; may be `state` */
+    const void *adj_out;      /* as out, and as state_out, or NULL (zero); read by the _bwd call */
+    const float *adj_state;
+    void *d_q, *d_k, *d_v;    /* [steps, batch, heads, dk or dv], or NULL */
+    float *d_state;           /* as state, or NULL */
+    void *work;               /* swarp_decay_work_bytes() bytes, 256-byte aligned */
+    uint64_t work_bytes;
+} swarp_decay_t;
+uint64_t swarp_decay_work_bytes(const swarp_decay_t *a);
+int swarp_decay_fwd(const swarp_decay_t *a, void *stream);
+int swarp_decay_bwd(const swarp_decay_t *a, void *stream);
+/* One step (steps = 1): state_out is written, `state` itself as a rule.  No work memory. */
+int swarp_decay_step(const swarp_decay_t *a, void *stream);
 
 #ifdef __cplusplus
 }

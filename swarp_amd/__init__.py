@@ -31,6 +31,7 @@ from .config import (
     per_env_float_template,
 )
 from .environment import Environment, make
+from .imitation import LinearCrossEntropy, linear_cross_entropy
 from .neighbors import NeighborGrid
 from .optim import AdamW, AdamWState, adamw_state, adamw_step, grad_norm
 from .policy import Advantages, PolicyLoss, categorical_policy_loss, gae, gaussian_policy_loss
@@ -41,6 +42,7 @@ from .world import World
 __all__ = [
     "AdamW", "AdamWState", "Advantages", "PolicyLoss", "adamw_state", "adamw_step",
     "categorical_policy_loss", "gae", "gaussian_policy_loss", "grad_norm",
+    "LinearCrossEntropy", "linear_cross_entropy",
     "AgentConfig", "AgentParams", "AgentShape", "ControlMode", "DynamicsModel", "Environment",
     "GradRing", "Integrator", "MODEL_ACTION_DIM", "NUM_PARAMS", "NavigationScenario",
     "NeighborGrid", "ObstacleKind", "per_env_float_template", "ObstacleShape", "Obstacles", "PARAM_FIELDS", "SCENARIOS",

@@ -13,7 +13,7 @@ from pathlib import Path
 
 import torch
 
-ABI_VERSION = 17
+ABI_VERSION = 18
 F32, F64, BF16, F16 = 0, 1, 2, 3
 EULER, RK4 = 0, 1
 LISTS_BRUTE, LISTS_GRID = 0, 1
@@ -176,6 +176,40 @@ class SwarpAdamW(ctypes.Structure):
     ]
 
 
+class SwarpLinearCe(ctypes.Structure):
+    """Mirror of ``swarp_linear_ce_t``."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int32), ("sum", ctypes.c_int32), ("targets32", ctypes.c_int32),
+        ("dim", ctypes.c_int32), ("width", ctypes.c_int32),
+        ("rows", ctypes.c_int64), ("inner", ctypes.c_int64),
+        ("outer_stride", ctypes.c_int64), ("inner_stride", ctypes.c_int64),
+        ("hidden", ctypes.c_void_p), ("weight", ctypes.c_void_p), ("bias", ctypes.c_void_p),
+        ("targets", ctypes.c_void_p), ("mask", ctypes.c_void_p), ("place", ctypes.c_void_p),
+        ("logp", ctypes.c_void_p), ("loss", ctypes.c_void_p), ("d_hidden", ctypes.c_void_p),
+        ("d_weight", ctypes.c_void_p), ("d_bias", ctypes.c_void_p), ("work", ctypes.c_void_p),
+        ("work_bytes", ctypes.c_uint64),
+    ]
+
+
+class SwarpDecay(ctypes.Structure):
+    """Mirror of ``swarp_decay_t``."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int32), ("heads", ctypes.c_int32), ("dk", ctypes.c_int32),
+        ("dv", ctypes.c_int32), ("steps", ctypes.c_int64), ("batch", ctypes.c_int64),
+        ("group", ctypes.c_int64), ("q_stride", ctypes.c_int64 * 3),
+        ("k_stride", ctypes.c_int64 * 3), ("v_stride", ctypes.c_int64 * 3),
+        ("scale", ctypes.c_double), ("log_decay", ctypes.c_void_p),
+        ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+        ("starts", ctypes.c_void_p), ("state", ctypes.c_void_p), ("out", ctypes.c_void_p),
+        ("state_out", ctypes.c_void_p), ("adj_out", ctypes.c_void_p),
+        ("adj_state", ctypes.c_void_p), ("d_q", ctypes.c_void_p), ("d_k", ctypes.c_void_p),
+        ("d_v", ctypes.c_void_p), ("d_state", ctypes.c_void_p), ("work", ctypes.c_void_p),
+        ("work_bytes", ctypes.c_uint64),
+    ]
+
+
 #: Exported entry points and their ctypes signatures.
 SIGNATURES = {
     "swarp_abi_version": ([], ctypes.c_int),
@@ -295,6 +329,17 @@ SIGNATURES = {
          ctypes.c_void_p, ctypes.c_void_p],
         ctypes.c_int,
     ),
+    "swarp_linear_ce_work_bytes": ([ctypes.POINTER(SwarpLinearCe)], ctypes.c_uint64),
+    "swarp_linear_ce": ([ctypes.POINTER(SwarpLinearCe), ctypes.c_void_p], ctypes.c_int),
+    "swarp_linear_ce_bwd": (
+        [ctypes.POINTER(SwarpLinearCe), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+         ctypes.c_void_p, ctypes.c_void_p],
+        ctypes.c_int,
+    ),
+    "swarp_decay_work_bytes": ([ctypes.POINTER(SwarpDecay)], ctypes.c_uint64),
+    "swarp_decay_fwd": ([ctypes.POINTER(SwarpDecay), ctypes.c_void_p], ctypes.c_int),
+    "swarp_decay_bwd": ([ctypes.POINTER(SwarpDecay), ctypes.c_void_p], ctypes.c_int),
+    "swarp_decay_step": ([ctypes.POINTER(SwarpDecay), ctypes.c_void_p], ctypes.c_int),
     "swarp_state_defaults": (
         [ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p],
         ctypes.c_int,

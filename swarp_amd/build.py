@@ -2,7 +2,8 @@
 
 ``python -m swarp_amd.build`` (or ``__graft_entry__.build()``) compiles the units under
 ``swarp_amd/csrc`` -- the host side ``swarp_hip.hip``, the radius graph, the policy update
-(``gae.hip``, ``policy.hip``, ``adamw.hip``) and one object per kernel family and scalar
+(``gae.hip``, ``policy.hip``, ``adamw.hip``, ``linear_ce.hip``,
+``decay.hip``) and one object per kernel family and scalar
 type (``k_*.hip`` with ``SWARP_T`` = float / double) -- in parallel, then links them into ``swarp_amd/libswarp_hip.so``.  ``--incremental`` recompiles only the objects
 whose sources, headers (from the compiler's dependency files) or flags changed.
 
@@ -44,7 +45,9 @@ def units() -> list[tuple[str, Path, list[str]]]:
            ("coo_noalloc", CSRC / "coo_noalloc.hip", []),
            ("gae", CSRC / "gae.hip", []),
            ("policy", CSRC / "policy.hip", []),
-           ("adamw", CSRC / "adamw.hip", [])]
+           ("adamw", CSRC / "adamw.hip", []),
+           ("linear_ce", CSRC / "linear_ce.hip", []),
+           ("decay", CSRC / "decay.hip", [])]
     for fam in FAMILIES:
         for tag, ctype, is32 in DTYPES:
             out.append((f"{fam}.{tag}", CSRC / f"{fam}.hip",

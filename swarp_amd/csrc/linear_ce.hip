@@ -1,0 +1,770 @@
+// linear_ce.hip -- softmax cross entropy of a linear head, from the hidden states and the head's
+// weight, without the logits (swarp_linear_ce).
+//
+// Per decision i with the hidden state h, target t and the head's rows W_j (and biases b_j):
+//   z_j = h W_j + b_j;   logp = z_t - log sum_j exp z_j;   loss = -w sum of logp;
+//   G_ij = p_ij - [j = t];   d h_i = w G_i W,  d W = w G^T h,  d b = w sum_i G_i.
+//
+// Three matrix products of 2 rows dim width operations each: the logits, which are formed tile by
+// tile in the matrix cores' registers and leave them as exponentials, and the two gradients, which
+// need all of a row's exponentials.  Those are kept for as many rows as 1 GiB holds (a piece), in
+// the heads' type; then comes the next piece.  They are relative to the target's logit, which is
+// known beforehand (one dot product a row):
+//   E_ij = exp(z_j - z_t),  s_i = sum_j E_ij,  logp = -log s_i,  G_ij = E_ij / s_i - [j = t],
+// so that a tile of them can be written before the row's sum is known; 1 / s_i goes into the rows of
+// d h and into h beside E^T.  Where some logit of a piece is above its target's by more than REACH
+// the piece is done again, relative to the rows' maxima (the kernels of that second pass are always
+// launched, look at a flag, and mostly end).  float16 has not the range for that: there the sums
+// come first, and the exponentials, relative to them, from a second product.
+//
+// Decisions whose mask is not set are left out of the products: the rows that count are gathered
+// first, and every kernel goes by their number on the device.
+#include <math.h>
+
+#include "matrix.hpp"
+
+namespace {
+
+using namespace mat;
+using learn::fail;
+using learn::launched;
+using learn::up;
+using learn::wave_sum;
+
+constexpr int BLOCK = 256;
+constexpr float LOG2E = 1.44269504088896340736f;
+constexpr float LN_2 = 0.69314718055994530942f;
+constexpr float REACH = 40.0f;        // e^40 times 2^21 logits, times any weight, is far from overflow
+constexpr int F16_BITS = 14;          // float16 exponentials are kept times 2^14: 2^-38 is not lost
+constexpr int COUNT_ROWS = 4096;      // rows of the mask that one workgroup counts
+constexpr uint64_t PIECE = 1ull << 30;  // bytes of exponentials at a time
+
+__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * LOG2E); }
+__device__ __forceinline__ float log_of(float x) { return __builtin_amdgcn_logf(x) * LN_2; }
+
+// What every kernel of a call may read.  Rows are the counted ones, in order; `n_on` of them.
+struct Call {
+    int64_t rows;             // of the call; at most as many count
+    int64_t inner, outer_stride, inner_stride;
+    int dim, width;
+    int dim_p;                // elements of a padded row of h and W
+    int64_t wide;             // elements of a row of E
+    int64_t tall;             // elements of a row of E^T and of h^T
+    int64_t first;            // row that the piece starts with
+    int piece;                // rows that it has room for
+    int targets32, sum;
+    const void *hidden, *weight, *bias, *targets;
+    const int32_t *index;     // which rows count, or NULL: all
+    const int32_t *n_on;      // how many, or NULL: all
+    float *logp, *loss;
+    // of all rows
+    void *h;
+    float *z_t, *ref, *top;   // target's logit; what E is relative to; largest logit
+    float *inv, *inv_h;       // 1 / s; what h is multiplied by beside E^T
+    double *sums;             // of logp, one for 64 rows
+    // of the piece
+    int32_t *flag;
+    float2 *parts;            // [n_parts][piece]: largest logit and sum of a part of a row
+    int n_parts;
+    void *e, *et, *ht;
+    const void *w, *wt;       // padded weight, its transpose
+};
+
+// Rows of the piece that count.
+__device__ __forceinline__ int rows_of(const Call &c)
+{
+    const int64_t n = (c.n_on ? (int64_t)*c.n_on : c.rows) - c.first;
+    return (int)(n < 0 ? 0 : n < c.piece ? n : c.piece);
+}
+
+// ------------------------------------------------------------------ which rows count
+
+__global__ __launch_bounds__(BLOCK) void k_count(int64_t rows, const uint8_t *mask, int32_t *counts)
+{
+    __shared__ int red[BLOCK / 64];
+    int n = 0;
+    for (int k = threadIdx.x; k < COUNT_ROWS; k += BLOCK) {
+        const int64_t i = (int64_t)blockIdx.x * COUNT_ROWS + k;
+        n += i < rows && mask[i];
+    }
+    n = wave_sum(n);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = n;
+    __syncthreads();
+    if (threadIdx.x == 0) counts[blockIdx.x] = red[0] + red[1] + red[2] + red[3];
+}
+
+// index[j] is the j-th row that counts, place[i] the j of row i or -1; logp of the others is 0.
+__global__ __launch_bounds__(BLOCK) void k_place(int64_t rows, const uint8_t *mask, const int32_t *counts,
+                                                 int32_t *index, int32_t *place, int32_t *n_on, float *logp)
+{
+    __shared__ int red[BLOCK / 64];
+    int before = 0;
+    for (int k = threadIdx.x; k < (int)blockIdx.x; k += BLOCK) before += counts[k];
+    before = wave_sum(before);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = before;
+    __syncthreads();
+    int at = red[0] + red[1] + red[2] + red[3];
+    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    for (int k = 0; k < COUNT_ROWS; k += BLOCK) {
+        const int64_t i = (int64_t)blockIdx.x * COUNT_ROWS + k + threadIdx.x;
+        const bool on = i < rows && mask[i];
+        const uint64_t votes = __ballot(on);
+        __syncthreads();
+        if (lane == 0) red[w] = __popcll(votes);
+        __syncthreads();
+        int j = at + __popcll(votes & ((1ull << lane) - 1));
+        for (int v = 0; v < w; ++v) j += red[v];
+        if (on) index[j] = (int32_t)i;
+        if (i < rows) {
+            place[i] = on ? j : -1;
+            if (!on) logp[i] = 0.0f;
+        }
+        at += red[0] + red[1] + red[2] + red[3];
+    }
+    if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) *n_on = at;
+}
+
+// ------------------------------------------------------------------ rows made ready
+
+// Row i of the hidden states, padded with zeros, and its target's logit (NaN if there is no such
+// target).  A wave a row.
+template <typename T> __global__ __launch_bounds__(BLOCK) void k_rows(const Call c)
+{
+    const int lane = threadIdx.x & 63;
+    const int64_t n = c.n_on ? *c.n_on : c.rows;
+    for (int64_t j = (int64_t)blockIdx.x * (BLOCK / 64) + (threadIdx.x >> 6); j < n;
+         j += (int64_t)gridDim.x * (BLOCK / 64)) {
+        const int64_t i = c.index ? c.index[j] : j;
+        const uint64_t o = (uint64_t)i / (uint64_t)c.inner;
+        const T *const x = (const T *)c.hidden + (int64_t)o * c.outer_stride + (i - (int64_t)o * c.inner) * c.inner_stride;
+        const int64_t t = c.targets32 ? (int64_t)((const int32_t *)c.targets)[i] : ((const int64_t *)c.targets)[i];
+        const bool in = t >= 0 && t < c.width;
+        const T *const w = (const T *)c.weight + (in ? t : 0) * c.dim;
+        T *const h = (T *)c.h + j * c.dim_p;
+        float z = 0.0f;
+        for (int k = lane; k < c.dim_p; k += 64) {
+            T v = (T)0.0f;
+            if (k < c.dim) {
+                v = x[k];
+                z = __builtin_fmaf(up(v), up(w[k]), z);
+            }
+            h[k] = v;
+        }
+        z = wave_sum(z);
+        if (lane == 0) {
+            if (c.bias) z += up(((const T *)c.bias)[in ? t : 0]);
+            z = in ? z : NAN;
+            c.z_t[j] = z;
+            c.ref[j] = z;
+        }
+    }
+}
+
+__global__ void k_clear(int32_t *flag) { *flag = 0; }
+
+// out [rows][pitch] = in [rows][n], the rest zero.
+template <typename T>
+__global__ __launch_bounds__(BLOCK) void k_pad(const T *in, int64_t rows, int n, T *out, int pitch)
+{
+    const int64_t all = rows * pitch;
+    for (int64_t k = (int64_t)blockIdx.x * BLOCK + threadIdx.x; k < all; k += (int64_t)gridDim.x * BLOCK) {
+        const int64_t r = k / pitch;
+        const int i = (int)(k - r * pitch);
+        out[k] = i < n ? in[r * n + i] : (T)0.0f;
+    }
+}
+
+// out [n][pitch] = in [rows][in_pitch] transposed, zero for rows past `rows` (up to `pitch`), each
+// row times scale[row] where that is set.  With `piece` the rows are the piece's.
+template <typename T>
+__global__ __launch_bounds__(BLOCK) void k_transpose(const T *in, int64_t rows, int64_t in_pitch, int64_t n, T *out,
+                                                     int64_t pitch, const float *scale, const Call c, int piece)
+{
+    __shared__ float tile[64][65];
+    if (piece) {
+        rows = rows_of(c);
+        const int64_t end = (rows + 63) / 64 * 64;  // (whole steps: nothing reads more)
+        pitch = c.tall;
+        if ((int64_t)blockIdx.x * 64 >= end) return;
+    }
+    const int64_t r0 = (int64_t)blockIdx.x * 64, c0 = (int64_t)blockIdx.y * 64;
+    const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
+    for (int k = y; k < 64; k += 4) {
+        float v = 0.0f;
+        if (r0 + k < rows && c0 + x < n) {
+            v = up(in[(r0 + k) * in_pitch + c0 + x]);
+            if (scale) v *= scale[r0 + k];
+        }
+        tile[k][x] = v;
+    }
+    __syncthreads();
+    for (int k = y; k < 64; k += 4)
+        if (c0 + k < n && r0 + x < pitch) out[(c0 + k) * pitch + r0 + x] = (T)tile[x][k];
+}
+
+// ------------------------------------------------------------------ logits
+
+// A tile of logits, width along the tile's rows and decisions along its columns, so that a lane has
+// many logits of one decision.  Leaves the largest and the sum of the exponentials of each wave's
+// part of a row; with STORE relative to ref[row], and the exponentials themselves; else the sum is
+// relative to the part's largest.  With `again` only where the piece's flag is set.
+template <typename T, typename C, bool STORE>
+__global__ __launch_bounds__(C::THREADS) void k_logits(const Call c, int nm, int nn, int again)
+{
+    extern __shared__ __align__(16) char lds[];
+    if (again && !*c.flag) return;
+    const int rows = rows_of(c);
+    int tm, tn;
+    tile_of(blockIdx.x, gridDim.x, nm, nn, tm, tn);
+    const int v0 = tm * C::BM, r0 = tn * C::BN;
+    if (r0 >= rows) return;
+    C t;
+    t.clear();
+    const int64_t pitch = (int64_t)c.dim_p * sizeof(T);
+    const Operand a = {(const char *)c.w + v0 * pitch, pitch, c.width - v0};
+    const Operand b = {(const char *)c.h + (c.first + r0) * pitch, pitch, rows - r0};
+    t.run(lds, a, b, 0, c.dim_p / C::KE);
+
+    const int lane = threadIdx.x & 63, w = C::wave(), wm = w / C::WN, wn = w % C::WN;
+    float *const bias = (float *)lds;
+    for (int k = threadIdx.x; k < C::BM; k += C::THREADS)
+        bias[k] = c.bias && v0 + k < c.width ? up(((const T *)c.bias)[v0 + k]) : 0.0f;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < C::TN; ++j) {
+        const int row = r0 + (wn * C::TN + j) * 32 + acc_col(lane);
+        const bool mine = row < rows;
+        float m = -INFINITY, s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int k = (wm * C::TM + i) * 32 + acc_row(r, lane);
+                const float z = v0 + k < c.width ? t.acc[i][j][r] + bias[k] : -INFINITY;
+                t.acc[i][j][r] = z;
+                m = z > m ? z : m;
+            }
+        const float ref = STORE ? c.ref[c.first + (mine ? row : 0)] : (m == -INFINITY ? 0.0f : m);
+#pragma unroll
+        for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float e = exp_of(t.acc[i][j][r] - ref);
+                s += e;
+                t.acc[i][j][r] = e;
+            }
+        if constexpr (STORE) {
+            T *const out = (T *)c.e + (int64_t)row * c.wide;
+            if (mine) {
+#pragma unroll
+                for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int64_t v = v0 + (wm * C::TM + i) * 32 + acc_row(r, lane);
+                        if (v < c.wide) out[v] = (T)(v < c.width ? t.acc[i][j][r] : 0.0f);
+                    }
+            }
+            s += __shfl_xor(s, 32, 64);
+            const float y = __shfl_xor(m, 32, 64);
+            m = y > m ? y : m;
+        } else {
+            const float ms = __shfl_xor(m, 32, 64), ss = __shfl_xor(s, 32, 64);
+            const float hi = ms > m ? ms : m, at = hi == -INFINITY ? 0.0f : hi;
+            s = (m == -INFINITY && s == 0.0f ? 0.0f : s * exp_of(m - at)) +
+                (ms == -INFINITY && ss == 0.0f ? 0.0f : ss * exp_of(ms - at));
+            m = hi;
+        }
+        if (lane < 32 && mine) c.parts[(int64_t)(tm * C::WM + wm) * c.piece + row] = make_float2(m, s);
+    }
+}
+
+// How a row's parts are joined.
+enum { SUMS = 0,     // from parts relative to their largest: logp; ref becomes what E is made with
+       KEPT = 1,     // from parts relative to ref, which E is too: logp, 1 / s, E at the target
+       KEPT2 = 2,    // the same after a second pass
+       NORMED = 3 }; // E is there, normalised: E at the target
+
+template <typename T> __global__ __launch_bounds__(BLOCK) void k_join(const Call c, int how)
+{
+    __shared__ float red[2][4][64];
+    __shared__ double total[64];
+    if (how == KEPT2 && !*c.flag) return;
+    const int rows = rows_of(c), lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int row = blockIdx.x * 64 + lane;
+    const bool mine = row < rows;
+    const int64_t j = c.first + (mine ? row : 0);
+    if (blockIdx.x * 64 >= rows) return;
+    const float ref = c.ref[j], zt = c.z_t[j];
+    float s = 0.0f, m = -INFINITY;
+    if (how != NORMED && mine) {
+        for (int k = w; k < c.n_parts; k += 4) {
+            const float2 p = c.parts[(int64_t)k * c.piece + row];
+            if (how == SUMS) {
+                const float hi = p.x > m ? p.x : m, at = hi == -INFINITY ? 0.0f : hi;
+                s = s * (m == -INFINITY ? 1.0f : exp_of(m - at)) + p.y * (p.x == -INFINITY ? 1.0f : exp_of(p.x - at));
+                m = hi;
+            } else {
+                s += p.y;
+                m = p.x > m ? p.x : m;
+            }
+        }
+    }
+    red[0][w][lane] = m;
+    red[1][w][lane] = s;
+    __syncthreads();
+    if (w) return;
+    float hi = m;
+    for (int k = 1; k < 4; ++k) hi = red[0][k][lane] > hi ? red[0][k][lane] : hi;
+    s = 0.0f;
+    for (int k = 0; k < 4; ++k) {
+        const float mk = red[0][k][lane];
+        s += red[1][k][lane] * (how == SUMS && mk != -INFINITY ? exp_of(mk - hi) : 1.0f);
+    }
+    const int64_t i = c.index ? c.index[j] : j;
+    float logp = 0.0f, unit = s;  // the exponentials' sum as E has them
+    if (how == SUMS) {
+        // (no logit above -inf: NaN)
+        const float lse = hi == -INFINITY ? NAN : hi + log_of(s);
+        logp = (zt - hi) - log_of(s);
+        if (hi == -INFINITY) logp = NAN;
+        if (mine) c.ref[j] = sizeof(T) == 2 ? lse - F16_BITS * LN_2 : lse;
+    } else if (how == NORMED) {
+        unit = (float)(1 << F16_BITS);
+    } else {
+        logp = (zt - ref) - log_of(s);
+        if (hi == -INFINITY) logp = NAN;
+        if (how == KEPT && mine) {
+            if (hi - ref > REACH || ref == -INFINITY) *c.flag = 1;
+            c.top[j] = hi;
+        }
+    }
+    if (mine && how != SUMS) {
+        // (a float16 h times 2^-14 would lose its digits: there the product is multiplied)
+        const bool none = how == NORMED ? zt != zt : hi == -INFINITY;
+        c.inv[j] = none ? NAN : 1.0f / unit;
+        c.inv_h[j] = none ? NAN : how == NORMED ? 1.0f : 1.0f / unit;
+        if (c.e) {
+            const int64_t t = c.targets32 ? (int64_t)((const int32_t *)c.targets)[i] : ((const int64_t *)c.targets)[i];
+            if (t >= 0 && t < c.width)
+                ((T *)c.e)[(int64_t)row * c.wide + t] = (T)(exp_of(zt - ref) - unit);
+        }
+    }
+    if (how != NORMED) {
+        if (mine) c.logp[i] = logp;
+        total[lane] = mine ? (double)logp : 0.0;
+        if (lane == 0) {
+            double sum = 0;
+            for (int k = 0; k < 64; ++k) sum += total[k];
+            c.sums[c.first / 64 + blockIdx.x] = sum;
+        }
+    }
+}
+
+// What a second pass is relative to.
+__global__ __launch_bounds__(BLOCK) void k_again(const Call c)
+{
+    const int row = blockIdx.x * BLOCK + threadIdx.x;
+    if (*c.flag && row < rows_of(c)) c.ref[c.first + row] = c.top[c.first + row];
+}
+
+// ------------------------------------------------------------------ products of the gradients
+
+// out [m][n] (+)= scale[m] sum_k A[m][k] B[n][k], split along k over gridDim.y; the splits leave
+// their sums behind each other.
+struct Product {
+    const void *a, *b;
+    int64_t a_pitch, b_pitch;  // bytes
+    int64_t m, n;              // rows of A and of B
+    int steps;                 // of k
+    int rows_m, rows_k;        // 1: m, or k, goes by the piece's rows
+    int add;
+    float times;
+    const float *scale;        // of the rows of A, or NULL
+    float *out;                // [m][n], or [splits][m][n]
+};
+
+template <typename T, typename C> __global__ __launch_bounds__(C::THREADS) void k_product(const Call c, const Product p, int nm, int nn)
+{
+    extern __shared__ __align__(16) char lds[];
+    const int rows = rows_of(c);
+    const int64_t M = p.rows_m ? rows : p.m;
+    int tm, tn;
+    tile_of(blockIdx.x, gridDim.x, nm, nn, tm, tn);
+    const int64_t m0 = (int64_t)tm * C::BM, n0 = (int64_t)tn * C::BN;
+    if (m0 >= M) return;
+    int steps = p.rows_k ? (rows + C::KE - 1) / C::KE : p.steps;
+    const int each = (steps + gridDim.y - 1) / gridDim.y, first = each * blockIdx.y;
+    steps = first + each < steps ? first + each : steps;
+    C t;
+    t.clear();
+    const Operand a = {(const char *)p.a + m0 * p.a_pitch, p.a_pitch, (int)(M - m0 < C::BM ? M - m0 : C::BM)};
+    const Operand b = {(const char *)p.b + n0 * p.b_pitch, p.b_pitch, (int)(p.n - n0 < C::BN ? p.n - n0 : C::BN)};
+    t.run(lds, a, b, first, steps);
+    const int lane = threadIdx.x & 63, w = C::wave(), wm = w / C::WN, wn = w % C::WN;
+    float *const out = p.out + (gridDim.y > 1 ? (int64_t)blockIdx.y * p.m * p.n : 0);
+    const bool whole = gridDim.y == 1;
+#pragma unroll
+    for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int64_t m = m0 + (wm * C::TM + i) * 32 + acc_row(r, lane);
+            if (m >= M) continue;
+            const float f = !whole ? 1.0f : p.scale ? p.times * p.scale[m] : p.times;
+#pragma unroll
+            for (int j = 0; j < C::TN; ++j) {
+                const int64_t n = n0 + (wn * C::TN + j) * 32 + acc_col(lane);
+                if (n >= p.n) continue;
+                float *const y = out + m * p.n + n;
+                *y = f * t.acc[i][j][r] + (whole && p.add ? *y : 0.0f);
+            }
+        }
+}
+
+__global__ __launch_bounds__(BLOCK) void k_splits(const Call c, const Product p, const float *parts, int splits)
+{
+    const int64_t all = (p.rows_m ? (int64_t)rows_of(c) : p.m) * p.n;
+    for (int64_t k = (int64_t)blockIdx.x * BLOCK + threadIdx.x; k < all; k += (int64_t)gridDim.x * BLOCK) {
+        float s = 0.0f;
+        for (int i = 0; i < splits; ++i) s += parts[(int64_t)i * p.m * p.n + k];
+        s *= p.scale ? p.times * p.scale[k / p.n] : p.times;
+        p.out[k] = s + (p.add ? p.out[k] : 0.0f);
+    }
+}
+
+// d b (+)= sum_i inv_i E_ij: a workgroup takes 64 columns, its waves every fourth row.
+template <typename T> __global__ __launch_bounds__(BLOCK) void k_bias(const Call c, float *out, int add)
+{
+    __shared__ float red[4][64];
+    const int rows = rows_of(c), lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int64_t v = (int64_t)blockIdx.x * 64 + lane;
+    float s = 0.0f;
+    if (v < c.width)
+        for (int r = w; r < rows; r += 4) s = __builtin_fmaf(c.inv[c.first + r], up(((const T *)c.e)[(int64_t)r * c.wide + v]), s);
+    red[w][lane] = s;
+    __syncthreads();
+    if (w == 0 && v < c.width) {
+        s = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
+        out[v] = s + (add ? out[v] : 0.0f);
+    }
+}
+
+__global__ __launch_bounds__(BLOCK) void k_loss(const Call c)
+{
+    __shared__ double red[BLOCK / 64];
+    const int64_t n = c.n_on ? *c.n_on : c.rows;
+    double s = 0;
+    for (int64_t k = threadIdx.x; k < (n + 63) / 64; k += BLOCK) s += c.sums[k];
+    s = wave_sum(s);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        s = (red[0] + red[1]) + (red[2] + red[3]);
+        *c.loss = (float)(n ? -s * (c.sum ? 1.0 : 1.0 / (double)n) : 0.0);
+    }
+}
+
+// The gradients as the caller has them: times the upstream gradient and the weight of a decision,
+// rounded once.  place: of the rows that count, or NULL.
+template <typename T>
+__global__ __launch_bounds__(BLOCK) void k_give(const float *from, T *to, int64_t n, int dim, const int32_t *place,
+                                                const int32_t *n_on, int64_t rows, int sum, const float *up1)
+{
+    const double count = n_on ? (double)*n_on : (double)rows;
+    const float f = (float)((double)*up1 * (sum || count < 1 ? 1.0 : 1.0 / count));
+    for (int64_t k = (int64_t)blockIdx.x * BLOCK + threadIdx.x; k < n; k += (int64_t)gridDim.x * BLOCK) {
+        int64_t at = k;
+        if (place) {
+            const int64_t i = k / dim, j = place[i];
+            at = j < 0 ? -1 : j * dim + (k - i * dim);
+        }
+        to[k] = at < 0 ? (T)0.0f : (T)(f * from[at]);
+    }
+}
+
+// ------------------------------------------------------------------ host
+
+template <typename T> struct Tiles;
+template <> struct Tiles<bf16> { typedef Tile<bf16, 4, 2, 2, 4> Wide; typedef Tile<bf16, 2, 1, 4, 1> Few; };
+template <> struct Tiles<f16> { typedef Tile<f16, 4, 2, 2, 4> Wide; typedef Tile<f16, 2, 1, 4, 1> Few; };
+template <> struct Tiles<float> { typedef Tile<float, 2, 2, 2, 2> Wide; typedef Tile<float, 2, 1, 4, 1> Few; };
+constexpr int FEW = 32;            // rows of a Few tile
+
+int64_t up_to(int64_t n, int64_t k) { return (n + k - 1) / k * k; }
+
+// Where everything lies in the work memory.
+struct Plan {
+    int size;                 // bytes of an element
+    int64_t dim_p, wide, tall, piece, n_parts;
+    bool few, pad_w, grad;
+    int split_h, split_w;
+    uint64_t index, counts, h, z_t, ref, top, inv, inv_h, sums, flag, parts, e, et, ht, w, wt, split, bytes;
+};
+
+int splits_of(int64_t tiles, int64_t steps)
+{
+    // fill the chip where the output alone does not: at least 8 steps each
+    int64_t s = tiles < 192 ? (256 + tiles - 1) / tiles : 1;
+    if (s > steps / 8) s = steps / 8;
+    return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+}
+
+Plan plan_of(const swarp_linear_ce_t *a)
+{
+    Plan p = {};
+    p.size = a->dtype == SWARP_F32 ? 4 : 2;
+    const int64_t ke = STEP / p.size, V = a->width, N = a->rows < 1 ? 1 : a->rows, D = a->dim;
+    const bool dh = a->d_hidden, dw = a->d_weight;
+    p.grad = dh || dw || a->d_bias;
+    p.dim_p = up_to(D, ke);
+    p.wide = up_to(V, ke);
+    p.few = N <= FEW;
+    const int64_t bm = p.few || p.size == 2 ? 256 : 128, wm = p.few ? 4 : 2;
+    p.n_parts = (V + bm - 1) / bm * wm;
+    // (a piece's parts of sums stay below its exponentials)
+    int64_t piece = p.grad ? (int64_t)(PIECE / (uint64_t)(p.wide * p.size)) : (int64_t)(PIECE / 8 / (uint64_t)p.n_parts);
+    piece = piece / 256 * 256;
+    if (piece < 256) piece = 256;
+    if (piece > up_to(N, 256)) piece = up_to(N, 256);
+    p.piece = piece;
+    p.tall = up_to(piece, 64);
+    p.pad_w = p.dim_p != D || ((uintptr_t)a->weight & 15);
+    const int64_t t = p.size == 2 ? 256 : 128;
+    p.split_h = splits_of(((piece + t - 1) / t) * ((D + t - 1) / t), p.wide / ke);
+    p.split_w = splits_of(((V + t - 1) / t) * ((D + t - 1) / t), p.tall / ke);
+    uint64_t at = 0;
+    auto room = [&](bool need, uint64_t bytes) {
+        const uint64_t here = at;
+        if (need) at += (bytes + 255) / 256 * 256;
+        return here;
+    };
+    p.flag = room(true, 4);
+    p.index = room(a->mask, 4 * N);
+    p.counts = room(a->mask, 4 * (N / COUNT_ROWS + 1));
+    p.h = room(true, (uint64_t)N * p.dim_p * p.size);
+    p.z_t = room(true, 4 * N);
+    p.ref = room(true, 4 * N);
+    p.top = room(true, 4 * N);
+    p.inv = room(true, 4 * N);
+    p.inv_h = room(true, 4 * N);
+    p.sums = room(true, 8 * (N / 64 + 1));
+    p.parts = room(true, 8ull * p.n_parts * piece);
+    p.w = room(p.pad_w, (uint64_t)V * p.dim_p * p.size);
+    p.e = room(p.grad, (uint64_t)piece * p.wide * p.size);
+    p.et = room(dw, (uint64_t)V * p.tall * p.size);
+    p.ht = room(dw, (uint64_t)D * p.tall * p.size);
+    p.wt = room(dh, (uint64_t)D * p.wide * p.size);
+    uint64_t s = dh && p.split_h > 1 ? 4ull * p.split_h * piece * D : 0;
+    const uint64_t s2 = dw && p.split_w > 1 ? 4ull * p.split_w * V * D : 0;
+    p.split = room(true, s > s2 ? s : s2);
+    p.bytes = at;
+    return p;
+}
+
+int blocks_of(int64_t n) { return (int)(n < 1 ? 1 : n > 4096 ? 4096 : n); }
+
+template <typename K> bool lds_limit(K kernel, int bytes)
+{
+    return hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess;
+}
+
+template <typename T, typename C, bool STORE> bool logits(const Call &c, int again, hipStream_t st)
+{
+    static const bool ok = lds_limit(k_logits<T, C, STORE>, C::LDS);
+    const int nm = (c.width + C::BM - 1) / C::BM, nn = (c.piece + C::BN - 1) / C::BN;
+    hipLaunchKernelGGL((k_logits<T, C, STORE>), dim3(nm * nn), dim3(C::THREADS), C::LDS, st, c, nm, nn, again);
+    return ok;
+}
+template <typename T, bool STORE> bool logits(const Call &c, bool few, int again, hipStream_t st)
+{
+    return few ? logits<T, typename Tiles<T>::Few, STORE>(c, again, st)
+               : logits<T, typename Tiles<T>::Wide, STORE>(c, again, st);
+}
+
+template <typename T> bool product(const Call &c, Product p, int splits, float *parts, hipStream_t st)
+{
+    typedef typename Tiles<T>::Wide C;
+    static const bool ok = lds_limit(k_product<T, C>, C::LDS);
+    const int64_t nm = ((p.rows_m ? c.piece : p.m) + C::BM - 1) / C::BM, nn = (p.n + C::BN - 1) / C::BN;
+    float *const out = p.out;
+    if (splits > 1) p.out = parts;
+    hipLaunchKernelGGL((k_product<T, C>), dim3(nm * nn, splits), dim3(C::THREADS), C::LDS, st, c, p, (int)nm, (int)nn);
+    if (splits > 1) {
+        p.out = out;
+        hipLaunchKernelGGL(k_splits, dim3(blocks_of(p.m * p.n / BLOCK)), dim3(BLOCK), 0, st, c, p, parts, splits);
+    }
+    return ok;
+}
+
+template <typename T> int run(const swarp_linear_ce_t *a, hipStream_t st)
+{
+    const Plan p = plan_of(a);
+    char *const mem = (char *)a->work;
+    Call c = {};
+    c.rows = a->rows;
+    c.inner = a->inner;
+    c.outer_stride = a->outer_stride;
+    c.inner_stride = a->inner_stride;
+    c.dim = a->dim;
+    c.width = a->width;
+    c.dim_p = (int)p.dim_p;
+    c.wide = p.wide;
+    c.tall = p.tall;
+    c.piece = (int)p.piece;
+    c.targets32 = a->targets32;
+    c.sum = a->sum;
+    c.hidden = a->hidden;
+    c.weight = a->weight;
+    c.bias = a->bias;
+    c.targets = a->targets;
+    c.logp = a->logp;
+    c.loss = a->loss;
+    c.h = mem + p.h;
+    c.z_t = (float *)(mem + p.z_t);
+    c.ref = (float *)(mem + p.ref);
+    c.top = (float *)(mem + p.top);
+    c.inv = (float *)(mem + p.inv);
+    c.inv_h = (float *)(mem + p.inv_h);
+    c.sums = (double *)(mem + p.sums);
+    c.flag = (int32_t *)(mem + p.flag);
+    c.parts = (float2 *)(mem + p.parts);
+    c.n_parts = (int)p.n_parts;
+    c.w = p.pad_w ? mem + p.w : (const char *)a->weight;
+    c.e = p.grad ? mem + p.e : nullptr;
+    c.et = mem + p.et;
+    c.ht = mem + p.ht;
+    c.wt = mem + p.wt;
+    if (a->mask && a->rows) {
+        c.index = (int32_t *)(mem + p.index);
+        c.n_on = a->place + a->rows;
+        int32_t *const counts = (int32_t *)(mem + p.counts);
+        const int blocks = (int)((a->rows + COUNT_ROWS - 1) / COUNT_ROWS);
+        hipLaunchKernelGGL(k_count, dim3(blocks), dim3(BLOCK), 0, st, a->rows, a->mask, counts);
+        hipLaunchKernelGGL(k_place, dim3(blocks), dim3(BLOCK), 0, st, a->rows, a->mask, counts, (int32_t *)c.index,
+                           a->place, (int32_t *)c.n_on, a->logp);
+    }
+    hipLaunchKernelGGL((k_rows<T>), dim3(blocks_of((a->rows + 3) / 4)), dim3(BLOCK), 0, st, c);
+    if (p.pad_w)
+        hipLaunchKernelGGL((k_pad<T>), dim3(blocks_of(c.width * p.dim_p / BLOCK)), dim3(BLOCK), 0, st,
+                           (const T *)a->weight, (int64_t)c.width, c.dim, (T *)c.w, c.dim_p);
+    if (a->d_hidden)
+        hipLaunchKernelGGL((k_transpose<T>), dim3((c.width + 63) / 64, (c.dim + 63) / 64), dim3(BLOCK), 0, st,
+                           (const T *)a->weight, (int64_t)c.width, (int64_t)c.dim, (int64_t)c.dim, (T *)c.wt, c.wide,
+                           (const float *)nullptr, c, 0);
+    bool ok = true;
+    // (without a row too: the gradients are zeros)
+    for (int64_t first = 0, n = 0; n == 0 || first < a->rows; first += p.piece, ++n) {
+        c.first = first;
+        const dim3 joins((unsigned)((p.piece + 63) / 64)), block(BLOCK);
+        if (!p.grad) {
+            ok &= logits<T, false>(c, p.few, 0, st);
+            hipLaunchKernelGGL((k_join<T>), joins, block, 0, st, c, SUMS);
+            continue;
+        }
+        if (a->dtype == SWARP_F16) {
+            ok &= logits<T, false>(c, p.few, 0, st);
+            hipLaunchKernelGGL((k_join<T>), joins, block, 0, st, c, SUMS);
+            ok &= logits<T, true>(c, p.few, 0, st);
+            hipLaunchKernelGGL((k_join<T>), joins, block, 0, st, c, NORMED);
+        } else {
+            hipLaunchKernelGGL(k_clear, dim3(1), dim3(1), 0, st, c.flag);
+            ok &= logits<T, true>(c, p.few, 0, st);
+            hipLaunchKernelGGL((k_join<T>), joins, block, 0, st, c, KEPT);
+            hipLaunchKernelGGL(k_again, dim3((unsigned)((p.piece + BLOCK - 1) / BLOCK)), block, 0, st, c);
+            ok &= logits<T, true>(c, p.few, 1, st);
+            hipLaunchKernelGGL((k_join<T>), joins, block, 0, st, c, KEPT2);
+        }
+        float *const parts = (float *)(mem + p.split);
+        const int ke = STEP / sizeof(T);
+        if (a->d_hidden) {
+            const Product y = {c.e, c.wt, (int64_t)(c.wide * sizeof(T)), (int64_t)(c.wide * sizeof(T)), p.piece, c.dim,
+                               (int)(c.wide / ke), 1, 0, 0, 1.0f, c.inv + first, a->d_hidden + first * c.dim};
+            ok &= product<T>(c, y, p.split_h, parts, st);
+        }
+        if (a->d_weight) {
+            hipLaunchKernelGGL((k_transpose<T>), dim3((unsigned)(c.tall / 64), (c.width + 63) / 64), block, 0, st,
+                               (const T *)c.e, (int64_t)0, c.wide, (int64_t)c.width, (T *)c.et, c.tall,
+                               (const float *)nullptr, c, 1);
+            hipLaunchKernelGGL((k_transpose<T>), dim3((unsigned)(c.tall / 64), (c.dim + 63) / 64), block, 0, st,
+                               (const T *)c.h + first * c.dim_p, (int64_t)0, (int64_t)c.dim_p, (int64_t)c.dim, (T *)c.ht,
+                               c.tall, (const float *)(c.inv_h + first), c, 1);
+            const Product y = {c.et, c.ht, (int64_t)(c.tall * sizeof(T)), (int64_t)(c.tall * sizeof(T)), c.width, c.dim,
+                               0, 0, 1, n > 0, a->dtype == SWARP_F16 ? 1.0f / (1 << F16_BITS) : 1.0f, nullptr, a->d_weight};
+            ok &= product<T>(c, y, p.split_w, parts, st);
+        }
+        if (a->d_bias)
+            hipLaunchKernelGGL((k_bias<T>), dim3((c.width + 63) / 64), block, 0, st, c, a->d_bias, n > 0);
+    }
+    hipLaunchKernelGGL(k_loss, dim3(1), dim3(BLOCK), 0, st, c);
+    const int rc = launched();
+    return ok ? rc : fail("the LDS of the matrix products was refused");
+}
+
+int check(const swarp_linear_ce_t *a)
+{
+    swarp::set_error("");
+    if (!a) return fail("arguments must be set");
+    if (a->dtype != SWARP_F32 && a->dtype != SWARP_BF16 && a->dtype != SWARP_F16) return fail("unknown dtype");
+    if (a->rows < 0 || a->rows >= 1ll << 31 || a->dim < 1 || a->dim > 65536 || a->width < 1 || a->width > 1 << 21)
+        return fail("bad sizes");
+    return 0;
+}
+
+template <typename T> void give(const swarp_linear_ce_t *a, const float *scale, void *h, void *w, void *b, hipStream_t st)
+{
+    const int32_t *const n_on = a->mask && a->rows ? a->place + a->rows : nullptr;
+    const int64_t nh = a->rows * a->dim, nw = (int64_t)a->width * a->dim;
+    if (h && nh)
+        hipLaunchKernelGGL((k_give<T>), dim3(blocks_of(nh / BLOCK)), dim3(BLOCK), 0, st, (const float *)a->d_hidden, (T *)h,
+                           nh, a->dim, (const int32_t *)(a->mask ? a->place : nullptr), n_on, a->rows, a->sum, scale);
+    if (w)
+        hipLaunchKernelGGL((k_give<T>), dim3(blocks_of(nw / BLOCK)), dim3(BLOCK), 0, st, (const float *)a->d_weight, (T *)w,
+                           nw, a->dim, (const int32_t *)nullptr, n_on, a->rows, a->sum, scale);
+    if (b)
+        hipLaunchKernelGGL((k_give<T>), dim3(blocks_of(a->width / BLOCK)), dim3(BLOCK), 0, st, (const float *)a->d_bias,
+                           (T *)b, (int64_t)a->width, 1, (const int32_t *)nullptr, n_on, a->rows, a->sum, scale);
+}
+
+}  // namespace
+
+extern "C" {
+
+uint64_t swarp_linear_ce_work_bytes(const swarp_linear_ce_t *a)
+{
+    if (check(a)) return 0;
+    return plan_of(a).bytes;
+}
+
+int swarp_linear_ce(const swarp_linear_ce_t *a, void *stream)
+{
+    if (check(a)) return -1;
+    if (!a->loss) return fail("loss must be set");
+    if (!a->work || a->work_bytes < plan_of(a).bytes) return fail("work must be set, swarp_linear_ce_work_bytes() long");
+    if ((uintptr_t)a->work & 255u) return fail("work must be 256-byte aligned");
+    if (!a->weight || a->inner < 1 || (a->rows && (!a->hidden || !a->targets || !a->logp)))
+        return fail("pointer arguments must be set");
+    if (a->rows && a->mask && !a->place) return fail("a mask needs place");
+    hipStream_t st = (hipStream_t)stream;
+    switch (a->dtype) {
+    case SWARP_F32: return run<float>(a, st);
+    case SWARP_BF16: return run<bf16>(a, st);
+    default: return run<f16>(a, st);
+    }
+}
+
+int swarp_linear_ce_bwd(const swarp_linear_ce_t *a, const void *scale, void *d_hidden, void *d_weight, void *d_bias,
+                        void *stream)
+{
+    if (check(a)) return -1;
+    if (!scale || (d_hidden && !a->d_hidden) || (d_weight && !a->d_weight) || (d_bias && !a->d_bias))
+        return fail("pointer arguments must be set");
+    if (a->rows && a->mask && !a->place) return fail("a mask needs place");
+    hipStream_t st = (hipStream_t)stream;
+    switch (a->dtype) {
+    case SWARP_F32: give<float>(a, (const float *)scale, d_hidden, d_weight, d_bias, st); break;
+    case SWARP_BF16: give<bf16>(a, (const float *)scale, d_hidden, d_weight, d_bias, st); break;
+    default: give<f16>(a, (const float *)scale, d_hidden, d_weight, d_bias, st); break;
+    }
+    return launched();
+}
+
+}  // extern "C"

@@ -1,0 +1,155 @@
+"""The loss of imitation, and the log-probabilities of a wide head: softmax cross entropy of a linear
+head over action bins or the tokens of a vocabulary, computed from the hidden states and the head's
+weight by hand-written kernels that never hold the logits of all decisions.
+
+In the manner of the policy losses: HIP tensors only, every launch on torch's current stream, shapes
+and types checked before any launch, no host synchronisation.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import NamedTuple
+
+import torch
+from torch.autograd import forward_ad
+from torch.compiler import is_dynamo_compiling
+
+from . import _lib
+from .policy import (_CODES, _differentiable_once, _guard, _no_tangents, _on_gpu, _plain, _ptr,
+                     _row_strides, _same, _untraced)
+
+_MOST_DIM, _MOST_WIDTH = 65536, 1 << 21
+
+
+class LinearCrossEntropy(NamedTuple):
+    """Result of :func:`linear_cross_entropy`.  Gradients flow from ``loss`` only."""
+
+    loss: torch.Tensor  # scalar, float32
+    logp: torch.Tensor  # log-probability of each target (0 where masked), float32
+
+
+def _forward(a: _lib.SwarpLinearCe, hidden: torch.Tensor, lead, wants, stream: int):
+    """The call: (loss, logp), and what its backward reads."""
+    dev = hidden.device
+    f32 = dict(dtype=torch.float32, device=dev)
+    loss, logp = torch.empty((), **f32), torch.empty(lead, **f32)
+    grads = [torch.empty(shape, **f32) if want else None for want, shape in
+             zip(wants, ((a.rows, a.dim), (a.width, a.dim), (a.width,)))]
+    place = torch.empty(a.rows + 1, dtype=torch.int32, device=dev) if a.mask else None
+    a.loss, a.logp, a.place = loss.data_ptr(), logp.data_ptr(), _ptr(place)
+    a.d_hidden, a.d_weight, a.d_bias = (_ptr(g) for g in grads)
+    lib = _lib.load()
+    nbytes = lib.swarp_linear_ce_work_bytes(ctypes.byref(a))
+    work = torch.empty(nbytes + 255, dtype=torch.uint8, device=dev)
+    a.work, a.work_bytes = (work.data_ptr() + 255) // 256 * 256, nbytes
+    with _guard(dev):
+        _lib.check(lib.swarp_linear_ce(ctypes.byref(a), stream))
+    return loss, logp, grads, place
+
+
+class _LinearCeFn(torch.autograd.Function):
+    """The loss as one autograd node.  The forward leaves the gradients of the summed loss behind in
+    float32, while the exponentials are at hand; the backward multiplies them by the upstream
+    gradient and rounds them, once, to the type of what they belong to."""
+
+    @staticmethod
+    def forward(ctx, a: _lib.SwarpLinearCe, stream: int, hidden, weight, bias, lead):
+        ctx.set_materialize_grads(False)
+        loss, logp, grads, place = _forward(a, hidden, lead, ctx.needs_input_grad[2:5], stream)
+        ctx.a, ctx.shapes, ctx.dtype, ctx.stream = a, (hidden.shape, weight.shape), hidden.dtype, stream
+        ctx.save_for_backward(*grads, place)
+        ctx.mark_non_differentiable(logp)
+        return loss, logp
+
+    @staticmethod
+    @_differentiable_once
+    def backward(ctx, g, *_):
+        if g is None:
+            return (None,) * 6
+        *grads, place = ctx.saved_tensors
+        dev, a = g.device, _lib.SwarpLinearCe.from_buffer_copy(ctx.a)
+        # (they may have been packed and lie elsewhere by now)
+        kept = [t if t is None else _same(t, "a saved tensor", t.shape, t.dtype, dev)
+                for t in (*grads, place)]
+        a.d_hidden, a.d_weight, a.d_bias, a.place = (_ptr(t) for t in kept)
+        shapes = (*ctx.shapes, ctx.shapes[1][:1])
+        out = [t if t is None else torch.empty(s, dtype=ctx.dtype, device=dev)
+               for t, s in zip(kept, shapes)]
+        g = _plain(g)
+        _lib.check(_lib.load().swarp_linear_ce_bwd(
+            ctypes.byref(a), g.data_ptr(), *(_ptr(t) for t in out), _lib.stream_of(dev)))
+        return None, None, *out, None
+
+
+def linear_cross_entropy(
+    hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor,
+    bias: torch.Tensor | None = None, mask: torch.Tensor | None = None, *,
+    reduction: str = "mean",
+) -> LinearCrossEntropy:
+    """Softmax cross entropy of the head ``hidden @ weight.T + bias`` with ``targets``: the loss of
+    imitating recorded actions or tokens, with its gradient, and the targets' log-probabilities,
+    which under ``torch.no_grad()`` are what :func:`categorical_policy_loss` takes as ``old_logp``
+    or ``ref_logp``.  The logits of all decisions are never in memory.
+
+    ``hidden [*lead, D]`` (float32, bfloat16, float16; any strides over ``lead``, so a sequence
+    model's ``hidden[:, :-1]`` is read where it lies), ``weight [V, D]`` and ``bias [V]`` of the same
+    type, ``targets [*lead]`` (int64 or int32), ``mask [*lead]`` (bool: which decisions count).
+    ``D`` up to 65536, ``V`` up to 2^21.
+
+        logp = z[target] - log sum exp z,   loss = -mean (or sum) of logp over what counts
+
+    Products and sums are in float32, whatever the type; exponentials go into the gradients' products
+    in the type of ``hidden``.  What a masked decision holds is not looked at, its target included
+    (-100); with no decision that counts the loss and its gradients are 0.  A bias of -inf is an
+    action that is not open.  A decision that counts with NaN or +inf among its logits, with all of
+    them -inf, or with a target outside ``[0, V)`` makes the loss NaN.
+
+    Gradients flow to ``hidden``, ``weight`` and ``bias``, once, and backward only.  A loss with
+    float16 heads should be scaled, as mixed precision does.  A call needs, beside copies of
+    ``hidden`` and ``weight``, up to 1 GiB of work memory where gradients are wanted, and float32
+    buffers for them until the backward.
+    """
+    if is_dynamo_compiling():
+        return _untraced(linear_cross_entropy)(hidden, weight, targets, bias, mask,
+                                               reduction=reduction)
+    _on_gpu(hidden, "linear_cross_entropy")
+    dtype, dev = hidden.dtype, hidden.device
+    if dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise TypeError(f"hidden must be float32, bfloat16 or float16; got {dtype}")
+    if hidden.dim() < 1 or not 1 <= hidden.shape[-1] <= _MOST_DIM:
+        raise ValueError(f"hidden must be [*lead, D] with 1 <= D <= {_MOST_DIM}; got "
+                         f"{list(hidden.shape)}")
+    D, lead = hidden.shape[-1], hidden.shape[:-1]
+    if weight.dim() != 2 or weight.shape[1] != D or not 1 <= weight.shape[0] <= _MOST_WIDTH:
+        raise ValueError(f"weight must be [V, {D}] with 1 <= V <= {_MOST_WIDTH}; got "
+                         f"{list(weight.shape)}")
+    V = weight.shape[0]
+    if lead.numel() >= 1 << 31:
+        raise ValueError(f"at most 2^31 - 1 decisions; got {lead.numel()}")
+    if targets.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"targets must be int64 or int32; got {targets.dtype}")
+    if reduction not in ("mean", "sum"):
+        raise ValueError(f'reduction must be "mean" or "sum"; got {reduction!r}')
+    weight = _same(weight, "weight", torch.Size((V, D)), dtype, dev)
+    targets = _same(targets, "targets", lead, targets.dtype, dev)
+    if bias is not None:
+        bias = _same(bias, "bias", torch.Size((V,)), dtype, dev)
+    if mask is not None:
+        mask = _same(mask, "mask", lead, torch.bool, dev)
+    if forward_ad._current_level >= 0:
+        _no_tangents("linear_cross_entropy", hidden, weight, bias)
+    strides = None if hidden.is_neg() else _row_strides(hidden)
+    if strides is None:
+        hidden = _plain(hidden)
+        strides = _row_strides(hidden)
+    a = _lib.SwarpLinearCe(
+        dtype=_CODES[dtype], sum=reduction == "sum", targets32=targets.dtype == torch.int32,
+        dim=D, width=V, rows=targets.numel(), inner=strides[0], outer_stride=strides[1],
+        inner_stride=strides[2], hidden=hidden.data_ptr(), weight=weight.data_ptr(),
+        bias=_ptr(bias), targets=targets.data_ptr(), mask=_ptr(mask))
+    stream = _lib.stream_of(dev)
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad or (
+            bias is not None and bias.requires_grad)):
+        return LinearCrossEntropy(*_LinearCeFn.apply(a, stream, hidden, weight, bias, lead))
+    return LinearCrossEntropy(*_forward(a, hidden, lead, (False,) * 3, stream)[:2])
