@@ -32,6 +32,7 @@ from .config import (
 )
 from .environment import Environment, make
 from .imitation import LinearCrossEntropy, linear_cross_entropy
+from .memory import DecayAttention, decay_attention, decay_attention_step
 from .neighbors import NeighborGrid
 from .optim import AdamW, AdamWState, adamw_state, adamw_step, grad_norm
 from .policy import Advantages, PolicyLoss, categorical_policy_loss, gae, gaussian_policy_loss
@@ -42,7 +43,8 @@ from .world import World
 __all__ = [
     "AdamW", "AdamWState", "Advantages", "PolicyLoss", "adamw_state", "adamw_step",
     "categorical_policy_loss", "gae", "gaussian_policy_loss", "grad_norm",
-    "LinearCrossEntropy", "linear_cross_entropy",
+    "DecayAttention", "LinearCrossEntropy", "decay_attention", "decay_attention_step",
+    "linear_cross_entropy",
     "AgentConfig", "AgentParams", "AgentShape", "ControlMode", "DynamicsModel", "Environment",
     "GradRing", "Integrator", "MODEL_ACTION_DIM", "NUM_PARAMS", "NavigationScenario",
     "NeighborGrid", "ObstacleKind", "per_env_float_template", "ObstacleShape", "Obstacles", "PARAM_FIELDS", "SCENARIOS",
