@@ -590,7 +590,8 @@ typedef struct swarp_decay {
     const uint8_t *starts;    /* [steps, batch / group], nonzero = an episode starts; NULL: none */
     const float *state;       /* [batch, heads, dk, dv] before the first step; NULL: zero */
     void *out;                /* [steps, batch, heads, dv] */
-    float *state_out;         /* as state, after the last step, or NULL; may be `state` */
+    float *state_out;         /* as state, after the last step, or NULL; not `state`
+                                 itself but in swarp_decay_step */
     const void *adj_out;      /* as out, and as state_out, or NULL (zero); read by the _bwd call */
     const float *adj_state;
     void *d_q, *d_k, *d_v;    /* [steps, batch, heads, dk or dv], or NULL */
@@ -598,7 +599,7 @@ typedef struct swarp_decay {
     void *work;               /* swarp_decay_work_bytes() bytes, 256-byte aligned */
     uint64_t work_bytes;
 } swarp_decay_t;
-uint64_t swarp_decay_work_bytes(const swarp_decay_t *a);
+uint64_t swarp_decay_work_bytes(const swarp_decay_t *a); /* of either call */
 int swarp_decay_fwd(const swarp_decay_t *a, void *stream);
 int swarp_decay_bwd(const swarp_decay_t *a, void *stream);
 /* One step (steps = 1): state_out is written, `state` itself as a rule.  No work memory. */

@@ -13,6 +13,9 @@
 //   dk_i = scale sum_{t >= i} lambda^(t-i) (v_i do_t) q_t + ...     backwards, (v, do, q), state dS^T
 //   dv_i = scale sum_{t >= i} lambda^(t-i) (k_i q_t) do_t + ...     backwards, (k, q, do), state dS
 // so that one kernel does all four; below, q, k and v are a scan's own parts.
+//
+// Where there are few heads the steps are cut into segments: one kernel finds the state that each
+// would end with if none entered, a second joins them, a third does the segments, each from its state.
 #include <math.h>
 
 #include "learn.hpp"
@@ -43,89 +46,125 @@ struct Scan {
     int back;                            // from the last step to the first
     int slices;                          // of 32 columns of v
     float score, grow, carry;            // factors of the scores, of k v^T in the state, of q S in the output
-    const float *state;                  // element (i, j) at i si + j sj of a head's
-    float *state_out;
+    const float *state;                  // before the first step, or NULL; element (i, j) at i si + j sj of a head's
+    float *state_out;                    // after the last, or NULL
     int si, sj;
+    float *between;                      // [segments][batch heads][area]: states that segments end (k_scan<ENDS>)
+    int32_t *cut;                        // or start with (k_between); [segments][batch heads]: no state gets through
 };
 
 struct Call {
     Scan scan[3];
     int scans, slices;     // slices of all scans
-    int64_t units;         // waves: batch * heads * slices
+    int segments, chunks;  // of the steps, and chunks of a segment
+    int64_t units;         // waves: batch * heads * segments * slices
     int64_t steps, batch, group;
     int heads, area;       // area: dk dv of a state
     const float *log_decay;
     const uint8_t *starts;
+    uint8_t *wrong;        // [units]: something was not finite
 };
 
 // What a lane gives to a product of 32 x 32 over 16 k: row (or column) l % 32, the eight k from
-// 8 (l / 32) on.  bfloat16 goes into the matrix cores as it is, sums of it and what is rounded from
-// float as two or three terms; the others are multiplied in float (float16 has not the range for the
-// states).
+// 8 (l / 32) on.  bfloat16 goes into the matrix cores as it is, what is in float as a sum of
+// bfloat16 terms; the others are multiplied in float (float16 has not the range for the states).
 template <typename T> struct Part {
     float x[8];
-    static constexpr int TERMS = 1;
+    static constexpr bool TERMS = false;
 };
 template <> struct Part<bf16> {
     u32x4 w;
-    static constexpr int TERMS = 3;
+    static constexpr bool TERMS = true;
 };
 
-__device__ __forceinline__ void mma(f32x16 &acc, const Part<float> &a, const Part<float> &b)
+template <typename T> __device__ __forceinline__ void mma(f32x16 &acc, const Part<T> &a, const Part<T> &b)
 {
+    if constexpr (Part<T>::TERMS) {
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a.w), __builtin_bit_cast(bf16x8, b.w),
+                                                      acc, 0, 0, 0);
+    } else {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a.x[k], b.x[k], acc, 0, 0, 0);
-}
-__device__ __forceinline__ void mma(f32x16 &acc, const Part<f16> &a, const Part<f16> &b)
-{
-#pragma unroll
-    for (int k = 0; k < 8; ++k) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a.x[k], b.x[k], acc, 0, 0, 0);
-}
-__device__ __forceinline__ void mma(f32x16 &acc, const Part<bf16> &a, const Part<bf16> &b)
-{
-    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a.w), __builtin_bit_cast(bf16x8, b.w),
-                                                  acc, 0, 0, 0);
+        for (int k = 0; k < 8; ++k) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a.x[k], b.x[k], acc, 0, 0, 0);
+    }
 }
 
-template <typename T> __device__ __forceinline__ Part<T> part_of(const T (&e)[8])
+// Eight elements as they came from memory.
+template <typename T> struct Raw {
+    uint32_t w[2 * sizeof(T)];
+};
+template <typename T> __device__ __forceinline__ float element(const Raw<T> &r, int k)
+{
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, r.w[k]);
+    else if constexpr (Part<T>::TERMS) return __builtin_bit_cast(float, k & 1 ? r.w[k >> 1] & 0xffff0000u : r.w[k >> 1] << 16);
+    else return (float)__builtin_bit_cast(f16, (uint16_t)(r.w[k >> 1] >> 16 * (k & 1)));
+}
+template <typename T> __device__ __forceinline__ Part<T> part_of(const Raw<T> &r)
 {
     Part<T> p;
-    if constexpr (sizeof(p) == 16) p.w = __builtin_bit_cast(u32x4, *(const Span<T, 8> *)e);
+    if constexpr (Part<T>::TERMS) p.w = __builtin_bit_cast(u32x4, r);
     else {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) p.x[k] = (float)e[k];
+        for (int k = 0; k < 8; ++k) p.x[k] = element(r, k);
     }
     return p;
 }
 // The next term of x, which is left with what remains of it.
-template <typename T> __device__ __forceinline__ Part<T> term_of(float (&x)[8])
+template <typename T> __device__ __forceinline__ Part<T> term_of(float (&x)[8], bool more)
 {
     Part<T> p;
-    if constexpr (Part<T>::TERMS == 1) {
+    if constexpr (!Part<T>::TERMS) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) p.x[k] = x[k];
     } else {
-        T e[8];
+        Raw<T> r;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            e[k] = (T)x[k];
-            x[k] -= (float)e[k];
+        for (int k = 0; k < 4; ++k)
+            r.w[k] = __builtin_bit_cast(uint32_t, Span<bf16, 2>{{(bf16)x[2 * k], (bf16)x[2 * k + 1]}});
+        if (more) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[k] -= element(r, k);
         }
-        p = part_of<T>(e);
+        p = part_of(r);
     }
     return p;
 }
-
-// n elements of a row from x on, zero past them.
-template <typename T> __device__ __forceinline__ Part<T> row_of(const T *x, int n)
+// odd + 0 times what a part holds: not 0 where some of it is not finite.
+template <typename T> __device__ __forceinline__ float odd_of(const Part<T> &p, float odd)
 {
-    T e[8];
-    if (n >= 8) *(Span<T, 8> *)e = *(const Span<T, 8> *)x;
-    else {
+    if constexpr (Part<T>::TERMS) {
+        typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+        const bf16x2 none = {(bf16)0.0f, (bf16)0.0f};
 #pragma unroll
-        for (int k = 0; k < 8; ++k) e[k] = k < n ? x[k] : (T)0.0f;
+        for (int k = 0; k < 4; ++k)
+            odd = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, (uint32_t)p.w[k]), none, odd, false);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) odd = __builtin_fmaf(p.x[k], 0.0f, odd);
     }
-    return part_of<T>(e);
+    return odd;
+}
+
+// Elements at .. at + 7 of a row of n; past its end its last ones, or with `zero` zeros.  EIGHTS: n is a
+// multiple of 8.
+template <typename T, bool EIGHTS> __device__ __forceinline__ Raw<T> row_of(const T *x, int at, int n, bool zero)
+{
+    Raw<T> r;
+    if constexpr (EIGHTS) {
+        r = __builtin_bit_cast(Raw<T>, *(const Span<T, 8> *)(x + (at < n ? at : n - 8)));
+        if (zero) {
+#pragma unroll
+            for (int k = 0; k < (int)(2 * sizeof(T)); ++k) r.w[k] = at < n ? r.w[k] : 0;
+        }
+    } else {
+        Span<T, 8> e;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const T y = x[at + k < n ? at + k : n - 1];
+            e.e[k] = zero && at + k >= n ? (T)0.0f : y;
+        }
+        r = __builtin_bit_cast(Raw<T>, e);
+    }
+    return r;
 }
 
 // Row m of a 32 x 32 accumulator is what operand row m was; swapping two bits of the operand's
@@ -133,48 +172,97 @@ template <typename T> __device__ __forceinline__ Part<T> row_of(const T *x, int 
 // how it holds an operand: accumulators go into the next product as they are.
 __device__ __forceinline__ int swapped(int m) { return (m & 0x13) | (m & 4) << 1 | (m & 8) >> 1; }
 
-// One wave: one head of a batch entry, 32 columns of v, all steps.  The state's columns stay in its
-// registers; KT: 32s of dk.
-template <typename T, int KT> __global__ __launch_bounds__(BLOCK) void k_scan(const Call c)
+// Rows of a chunk in LDS, `pitch` elements apart, read as columns: lane l has column
+// col + swapped(l % 32), rows row + 8 (l / 32) + 0 .. 7.  16-bit elements come by the transposing read:
+// 16 lanes bring four rows of 16 elements, lane i keeps column i of them.
+template <typename T> __device__ __forceinline__ Part<T> column_of(const T *x, int pitch, int row, int col, int lane)
 {
-    const int64_t unit = (int64_t)blockIdx.x * WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int half = lane >> 5;
+    if constexpr (sizeof(T) == 2) {
+        typedef short s16x4 __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) s16x4 *Ptr;
+        const int four = lane & 3, at = (lane & 16) + 4 * ((four & 1) << 1 | four >> 1);
+        const T *const y = x + (row + 8 * half + ((lane & 15) >> 2)) * pitch + col + at;
+        Raw<T> r;
+        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)(uintptr_t)(y));
+        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)(uintptr_t)(y + 4 * pitch));
+        const uint64_t lo = __builtin_bit_cast(uint64_t, a), hi = __builtin_bit_cast(uint64_t, b);
+        r.w[0] = (uint32_t)lo;
+        r.w[1] = (uint32_t)(lo >> 32);
+        r.w[2] = (uint32_t)hi;
+        r.w[3] = (uint32_t)(hi >> 32);
+        return part_of(r);
+    } else {
+        const T *const y = x + (row + 8 * half) * pitch + col + swapped(lane & 31);
+        Part<T> p;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) p.x[k] = y[k * pitch];
+        return p;
+    }
+}
+template <typename T> __device__ __forceinline__ float element(const Part<T> &p, int k)
+{
+    if constexpr (Part<T>::TERMS) return element(__builtin_bit_cast(Raw<T>, p.w), k);
+    else return p.x[k];
+}
+
+// What a wave does: the outputs of a segment, or (ENDS) the state that it ends with if none enters.
+enum { OUTPUTS, ENDS };
+
+// One wave: one head of a batch entry, 32 columns of v, the steps of a segment.  The state's columns
+// stay in its registers; KT: 32s of dk.  A wave works alone: its part of the LDS holds the chunk's
+// rows of k and v, to be read as columns.
+template <typename T, int KT, int WHAT, bool EIGHTS>
+__global__ __launch_bounds__(BLOCK, KT < 4 && sizeof(T) == 2 ? 2 : 1) void k_scan(const Call c)
+{
+    constexpr int KP = 32 * KT + 16 / (int)sizeof(T), VP = 32 + 16 / (int)sizeof(T);
+    __shared__ __align__(16) T room[WAVES][32 * (KP + VP)];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t unit = (int64_t)blockIdx.x * WAVES + wave;
     if (unit >= c.units) return;
-    const int64_t bh = unit / c.slices, b = bh / c.heads;
-    const int h = (int)(bh - b * c.heads);
-    int slice = (int)(unit - bh * c.slices), which = 0;
+    T *const kx = room[wave], *const vx = kx + 32 * KP;
+    const int64_t part = unit / c.slices, bh = part / c.segments, b = bh / c.heads;
+    const int segment = (int)(part - bh * c.segments), h = (int)(bh - b * c.heads);
+    int slice = (int)(unit - part * c.slices), which = 0;
     while (slice >= c.scan[which].slices) slice -= c.scan[which++].slices;
     const Scan &s = c.scan[which];
     const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31, perm = swapped(col);
-    const int64_t steps = c.steps, last = s.back ? steps - 1 : 0, way = s.back ? -1 : 1;
-    const int64_t qt = way * s.qs[0], kt = way * s.ks[0], vt = way * s.vs[0], ot = way * s.os[0];
-    const T *const q = (const T *)s.q + b * s.qs[1] + h * s.qs[2] + last * s.qs[0];
-    const T *const k = (const T *)s.k + b * s.ks[1] + h * s.ks[2] + last * s.ks[0];
-    const T *const v = (const T *)s.v + b * s.vs[1] + h * s.vs[2] + last * s.vs[0];
-    T *const out = (T *)s.out + b * s.os[1] + h * s.os[2] + last * s.os[0];
-    const int dk = s.dk, dv = s.dv, j0 = 32 * slice, j = j0 + perm;
     const bool back = s.back;
+    const int64_t steps = c.steps, origin = back ? steps - 1 : 0, way = back ? -1 : 1;
+    const int64_t qt = way * s.qs[0], kt = way * s.ks[0], vt = way * s.vs[0], ot = way * s.os[0];
+    const int64_t begin = (int64_t)segment * c.chunks * CHUNK;
+    const int64_t end = begin + (int64_t)c.chunks * CHUNK < steps ? begin + (int64_t)c.chunks * CHUNK : steps;
+    const T *const q0 = (const T *)s.q + b * s.qs[1] + h * s.qs[2] + origin * s.qs[0];
+    const T *const k0 = (const T *)s.k + b * s.ks[1] + h * s.ks[2] + origin * s.ks[0];
+    const T *const v0 = (const T *)s.v + b * s.vs[1] + h * s.vs[2] + origin * s.vs[0];
+    const int dk = s.dk, dv = s.dv, j0 = 32 * slice, j = j0 + perm;
     const uint8_t *const starts = c.starts ? c.starts + b / c.group : nullptr;
     const int64_t groups = c.batch / c.group;
+    const bool ends = end == steps;  // the last segment
 
     // the state: element (32 t + 16 (r / 8) + 8 half + r % 8, j) in register r of tile t
     f32x16 S[KT];
+    const float *const from = WHAT == ENDS ? nullptr
+                              : segment    ? s.between + ((int64_t)segment * c.batch * c.heads + bh) * c.area
+                              : s.state    ? s.state + bh * c.area
+                                           : nullptr;
 #pragma unroll
     for (int t = 0; t < KT; ++t)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const int i = 32 * t + 16 * (r >> 3) + 8 * half + (r & 7);
-            S[t][r] = s.state && i < dk && j < dv ? s.state[bh * c.area + (int64_t)i * s.si + (int64_t)j * s.sj] : 0.0f;
+            S[t][r] = from && i < dk && j < dv ? from[(int64_t)i * s.si + (int64_t)j * s.sj] : 0.0f;
         }
-    // (a product with 0 is not 0 where the state is not finite)
-    auto finite = [&]() {
-        float z = 0.0f;
+    bool none = !from;  // the state is still zero
+    // 0 as long as all that is multiplied is finite: a product with 0 is not 0 where it is not, and the
+    // head is done again by k_exact
+    float odd = 0.0f;
+    if (from) {
 #pragma unroll
         for (int t = 0; t < KT; ++t)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) z = __builtin_fmaf(S[t][r], 0.0f, z);
-        return __ballot(!(z == 0.0f)) == 0;
-    };
-    bool plain = finite();
+            for (int r = 0; r < 16; ++r) odd = __builtin_fmaf(S[t][r], 0.0f, odd);
+    }
 
     // powers: of the decay between the steps of a lane's scores, of what a step leaves in the state
     float a2 = c.log_decay[h] * LOG2E;
@@ -187,11 +275,41 @@ template <typename T, int KT> __global__ __launch_bounds__(BLOCK) void k_scan(co
         D[r] = col >= i ? s.score * __builtin_amdgcn_exp2f(a2 * (float)(col - i)) : 0.0f;
     }
     const float w0 = s.carry * __builtin_amdgcn_exp2f(a2 * (float)(col + (back ? 0 : 1)));
+    const uint8_t *sp = starts ? starts + (back ? steps - (begin + col) : begin + col) * groups : nullptr;
+    T *op = (T *)s.out + b * s.os[1] + h * s.os[2] + origin * s.os[0] + (begin + col) * ot + j0 + 8 * half;
     float whole = 0.0f;
     int width = 0;  // of the chunk that u and whole are for
+    uint32_t any = 0;
 
-    for (int64_t c0 = 0; c0 < steps; c0 += CHUNK) {
-        const int L = (int)(steps - c0 < CHUNK ? steps - c0 : CHUNK);
+    // Rows as they lie in memory: q by lane, k by swapped lane, v by quarters of rows.  Where a row or a
+    // step is past the end the last one is read again: only q has to be zero past dk, what else it
+    // brings meets a zero (of q, of D, of u) or is not written.
+    Raw<T> qr[2 * KT], kr[2 * KT], vr[2];
+    const T *qp = q0 + (begin + col) * qt, *kp = k0 + (begin + perm) * kt, *vp = v0 + (begin + (lane >> 2)) * vt;
+    const int64_t qn = CHUNK * qt, kn = CHUNK * kt, vn = CHUNK * vt;
+    auto load = [&](int L) {
+        const T *x = qp, *y = kp, *z[2] = {vp, vp + 16 * vt};
+        if (L < CHUNK) {
+            x -= (col < L ? 0 : col - (L - 1)) * qt;
+            y -= (perm < L ? 0 : perm - (L - 1)) * kt;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) z[t] -= (16 * t + (lane >> 2) < L ? 0 : 16 * t + (lane >> 2) - (L - 1)) * vt;
+        }
+#pragma unroll
+        for (int t = 0; t < 2 * KT; ++t) {
+            if (WHAT == OUTPUTS) qr[t] = row_of<T, EIGHTS>(x, 16 * t + 8 * half, dk, 16 * t + 16 > dk);
+            kr[t] = row_of<T, EIGHTS>(y, 16 * t + 8 * half, dk, false);
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) vr[t] = row_of<T, EIGHTS>(z[t], j0 + 8 * (lane & 3), dv, false);
+        qp += qn;
+        kp += kn;
+        vp += vn;
+    };
+    if (begin < end) load((int)(end - begin < CHUNK ? end - begin : CHUNK));
+    for (int64_t c0 = begin; c0 < end; c0 += CHUNK) {
+        const int L = (int)(end - c0 < CHUNK ? end - c0 : CHUNK);
+        const bool more = c0 + CHUNK < end;
         if (L != width) {
             width = L;
 #pragma unroll
@@ -204,143 +322,221 @@ template <typename T, int KT> __global__ __launch_bounds__(BLOCK) void k_scan(co
         // steps that nothing before them enters
         uint32_t cut = 0;
         if (starts) {
-            const int64_t t = back ? steps - (c0 + col) : c0 + col;
-            cut = (uint32_t)__ballot(half == 0 && col < L && (!back || c0 + col > 0) && starts[t * groups]);
+            cut = (uint32_t)__ballot(half == 0 && col < L && (!back || c0 + col > 0) && *sp);
+            sp += CHUNK * way * groups;
+            any |= cut;
         }
-        const uint32_t upto = cut & (0xffffffffu >> (31 - col));
-        const int since = upto ? 31 - __clz(upto) : -1;               // first step that enters step `col`
-        const int kept = cut ? 31 - __clz(cut) : -1;                  // ... the leaving state
-
-        Part<T> qf[2 * KT], vf[2];
+        // the rows of k and v into LDS
+#pragma unroll
+        for (int t = 0; t < 2 * KT; ++t) *(Raw<T> *)(kx + perm * KP + 16 * t + 8 * half) = kr[t];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) *(Raw<T> *)(vx + (16 * t + (lane >> 2)) * VP + 8 * (lane & 3)) = vr[t];
+        Part<T> qf[2 * KT];
         f32x16 p = {};
-        const T *const qr = q + (c0 + (col < L ? col : 0)) * qt, *const kr = k + (c0 + (perm < L ? perm : 0)) * kt;
+        if (WHAT == OUTPUTS) {
 #pragma unroll
-        for (int x = 0; x < 2 * KT; ++x) {
-            const int at = 16 * x + 8 * half;
-            qf[x] = row_of<T>(qr + at, col < L ? dk - at : 0);
-            const Part<T> kf = row_of<T>(kr + at, perm < L ? dk - at : 0);
-            mma(p, kf, qf[x]);
-        }
-        float vx[16], odd = 0.0f;
-        {
-            T e[16];
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int i = 16 * (r >> 3) + 8 * half + (r & 7);
-                e[r] = i < L && j < dv ? v[(c0 + i) * vt + j] : (T)0.0f;
-                vx[r] = (float)e[r];
-                odd = __builtin_fmaf(vx[r], 0.0f, odd);
+            for (int t = 0; t < 2 * KT; ++t) {
+                qf[t] = part_of(qr[t]);
+                mma<T>(p, part_of(kr[t]), qf[t]);
             }
-            vf[0] = part_of<T>(*(const T(*)[8])e);
-            vf[1] = part_of<T>(*(const T(*)[8])(e + 8));
         }
-        // (a score is not finite wherever its q or k is not)
+        if (more) load((int)(end - c0 - CHUNK < CHUNK ? end - c0 - CHUNK : CHUNK));
+        Part<T> vf[2];
+        vf[0] = column_of<T>(vx, VP, 0, 0, lane);
+        vf[1] = column_of<T>(vx, VP, 16, 0, lane);
+        odd = odd_of<T>(vf[1], odd_of<T>(vf[0], odd));
+        Part<T> pf[2], pl[2];
+        if (WHAT == OUTPUTS) {
+            const uint32_t upto = cut & (0xffffffffu >> (31 - col));
+            const int since = upto ? 31 - __clz(upto) : 0;  // first step that enters step `col`
 #pragma unroll
-        for (int r = 0; r < 16; ++r) odd = __builtin_fmaf(p[r], 0.0f, odd);
-        Part<T> kc[KT][2];  // columns of k
-#pragma unroll
-        for (int t = 0; t < KT; ++t)
+            for (int r = 0; r < 16; ++r) p[r] *= D[r];
+            // (a score is not finite wherever its q or k is not)
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                T e[8];
+                float y[8];
 #pragma unroll
-                for (int r = 0; r < 8; ++r) {
-                    const int i = 16 * x + 8 * half + r;
-                    e[r] = i < L && 32 * t + perm < dk ? k[(c0 + i) * kt + 32 * t + perm] : (T)0.0f;
+                for (int r = 0; r < 8; ++r) y[r] = p[8 * x + r];
+                if (cut) {
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) {
+                        odd = __builtin_fmaf(y[r], 0.0f, odd);
+                        y[r] = 16 * x + 8 * half + r >= since ? y[r] : 0.0f;
+                    }
                 }
-                kc[t][x] = part_of<T>(e);
+                pf[x] = term_of<T>(y, true);
+                if (Part<T>::TERMS) pl[x] = term_of<T>(y, false);
+                odd = odd_of<T>(pf[x], odd);
             }
-        if (plain && __ballot(!(odd == 0.0f)) == 0) {
+        }
+        if (WHAT == OUTPUTS) {
             f32x16 o = {};
+            if (!none) {
 #pragma unroll
-            for (int x = 0; x < 2 * KT; ++x) {
-                float y[8];
+                for (int x = 0; x < 2 * KT; ++x) {
+                    float y[8];
 #pragma unroll
-                for (int r = 0; r < 8; ++r) y[r] = S[x >> 1][8 * (x & 1) + r];
+                    for (int r = 0; r < 8; ++r) y[r] = S[x >> 1][8 * (x & 1) + r];
+                    mma<T>(o, term_of<T>(y, true), qf[x]);
+                    if (Part<T>::TERMS) mma<T>(o, term_of<T>(y, false), qf[x]);
+                }
+                const float f = cut & (0xffffffffu >> (31 - col)) ? 0.0f : w0;
 #pragma unroll
-                for (int n = 0; n < (Part<T>::TERMS + 1) / 2; ++n) mma(o, term_of<T>(y), qf[x]);
+                for (int r = 0; r < 16; ++r) o[r] *= f;
             }
 #pragma unroll
-            for (int r = 0; r < 16; ++r) o[r] = since < 0 ? o[r] * w0 : 0.0f;
-#pragma unroll
             for (int x = 0; x < 2; ++x) {
-                float y[8];
-#pragma unroll
-                for (int r = 0; r < 8; ++r) {
-                    const int i = 16 * x + 8 * half + r;
-                    // (a select: a step that is not open may hold anything)
-                    y[r] = i <= col && i >= since ? p[8 * x + r] * D[8 * x + r] : 0.0f;
-                }
-#pragma unroll
-                for (int n = 0; n < (Part<T>::TERMS + 1) / 2; ++n) mma(o, vf[x], term_of<T>(y));
+                mma<T>(o, vf[x], pf[x]);
+                if (Part<T>::TERMS) mma<T>(o, vf[x], pl[x]);
             }
             if (col < L) {
-                T *const to = out + (c0 + col) * ot + j0;
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
-                    const int at = 16 * x + 8 * half, n = dv - j0 - at;
-                    T e[8];
+                    const int n = dv - j0 - 8 * half - 16 * x;
+                    Span<T, 8> e;
 #pragma unroll
-                    for (int r = 0; r < 8; ++r) e[r] = (T)o[8 * x + r];
-                    if (n >= 8) *(Span<T, 8> *)(to + at) = *(const Span<T, 8> *)e;
-                    else {
+                    for (int r = 0; r < 8; ++r) e.e[r] = (T)o[8 * x + r];
+                    if (EIGHTS ? n > 0 : n >= 8) *(Span<T, 8> *)(op + 16 * x) = e;
+                    else if constexpr (!EIGHTS) {
 #pragma unroll
                         for (int r = 0; r < 8; ++r)
-                            if (r < n) to[at + r] = e[r];
+                            if (r < n) op[16 * x + r] = e.e[r];
                     }
                 }
             }
-#pragma unroll
-            for (int t = 0; t < KT; ++t)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) S[t][r] = cut ? 0.0f : S[t][r] * whole;
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                float y[8];
-#pragma unroll
-                for (int r = 0; r < 8; ++r) y[r] = 16 * x + 8 * half + r >= kept ? vx[8 * x + r] * u[8 * x + r] : 0.0f;
-#pragma unroll
-                for (int n = 0; n < Part<T>::TERMS; ++n) {
-                    const Part<T> w = term_of<T>(y);
-#pragma unroll
-                    for (int t = 0; t < KT; ++t) mma(S[t], kc[t][x], w);
-                }
-            }
-        } else {
-            // something is not finite: step by step, as the definition has it
-            for (int i = 0; i < L; ++i) {
-                const float vi = j < dv ? (float)v[(c0 + i) * vt + j] : 0.0f;
-                const bool fresh = cut >> i & 1;
-                float o = 0.0f;
+        }
+        if (WHAT == ENDS || more || (ends && s.state_out)) {
+            const int kept = cut ? 31 - __clz(cut) : 0;  // first step that enters the leaving state
+            if (!none) {
+                const float f = cut ? 0.0f : whole;
 #pragma unroll
                 for (int t = 0; t < KT; ++t)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int at = 32 * t + 16 * (r >> 3) + 8 * half + (r & 7);
-                        if (at < dk) {
-                            const float kv = (float)k[(c0 + i) * kt + at] * vi * s.grow;
-                            const float y = fresh ? kv : __builtin_fmaf(back ? 1.0f : lambda, S[t][r], kv);
-                            o = __builtin_fmaf((float)q[(c0 + i) * qt + at], y, o);
-                            S[t][r] = back ? lambda * y : y;
-                        }
-                    }
-                o += __shfl_xor(o, 32, 64);
-                if (half == 0 && j < dv) out[(c0 + i) * ot + j] = (T)(o * s.carry);
+                    for (int r = 0; r < 16; ++r) S[t][r] *= f;
             }
-            plain = finite();
+            none = false;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                float y[8];
+#pragma unroll
+                for (int r = 0; r < 8; ++r) y[r] = element(vf[x], r) * u[8 * x + r];
+                if (cut) {
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) y[r] = 16 * x + 8 * half + r >= kept ? y[r] : 0.0f;
+                }
+                Part<T> w[3];
+                w[0] = term_of<T>(y, true);
+                if (Part<T>::TERMS) {
+                    w[1] = term_of<T>(y, true);
+                    w[2] = term_of<T>(y, false);
+                }
+#pragma unroll
+                for (int t = 0; t < KT; ++t) {
+                    const Part<T> kc = column_of<T>(kx, KP, 16 * x, 32 * t, lane);
+                    mma<T>(S[t], kc, w[0]);
+                    if (Part<T>::TERMS) {
+                        mma<T>(S[t], kc, w[1]);
+                        mma<T>(S[t], kc, w[2]);
+                    }
+                }
+            }
         }
+        op += CHUNK * ot;
     }
-    if (s.state_out) {
+    float *to = WHAT == ENDS        ? s.between + ((int64_t)segment * c.batch * c.heads + bh) * c.area
+                : ends && s.state_out ? s.state_out + bh * c.area
+                                      : nullptr;
+    if (to) {
         // (backwards: what an episode that starts with the first step leaves of the state before it)
-        const bool none = back && starts && steps > 0 && starts[0];
+        const bool clear = WHAT == OUTPUTS && back && starts && steps > 0 && starts[0];
 #pragma unroll
         for (int t = 0; t < KT; ++t)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const int i = 32 * t + 16 * (r >> 3) + 8 * half + (r & 7);
-                if (i < dk && j < dv)
-                    s.state_out[bh * c.area + (int64_t)i * s.si + (int64_t)j * s.sj] = none ? 0.0f : S[t][r];
+                if (i < dk && j < dv) to[(int64_t)i * s.si + (int64_t)j * s.sj] = clear ? 0.0f : S[t][r];
             }
+    }
+    if (WHAT == OUTPUTS) {
+        const bool wrong = __ballot(!(odd == 0.0f)) != 0;
+        if (lane == 0) c.wrong[unit] = wrong;
+    }
+    if (WHAT == ENDS && lane == 0) s.cut[(int64_t)segment * c.batch * c.heads + bh] = any != 0;
+}
+
+// The heads (and columns) where something was not finite, step by step, as the definition has it: what
+// a start or the order of the steps keeps from an output does not reach it as a product with 0.
+template <typename T, int KT> __global__ __launch_bounds__(BLOCK) void k_exact(const Call c, int64_t n)
+{
+    const int64_t unit = (int64_t)blockIdx.x * WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (unit >= n) return;
+    const int lane = threadIdx.x & 63, half = lane >> 5;
+    const int64_t bh = unit / c.slices, b = bh / c.heads;
+    const int h = (int)(bh - b * c.heads);
+    int slice = (int)(unit - bh * c.slices), which = 0;
+    bool wrong = false;
+    for (int i = lane; i < c.segments; i += 64) wrong |= c.wrong[(bh * c.segments + i) * c.slices + slice] != 0;
+    if (!__ballot(wrong)) return;
+    while (slice >= c.scan[which].slices) slice -= c.scan[which++].slices;
+    const Scan &s = c.scan[which];
+    const int j = 32 * slice + (lane & 31), dk = s.dk;
+    const bool back = s.back, mine = j < s.dv;
+    const uint8_t *const starts = c.starts ? c.starts + b / c.group : nullptr;
+    const int64_t groups = c.batch / c.group;
+    float S[KT * 16];
+#pragma unroll
+    for (int r = 0; r < 16 * KT; ++r) {
+        const int i = 2 * r + half;
+        S[r] = s.state && i < dk && mine ? s.state[bh * c.area + (int64_t)i * s.si + (int64_t)j * s.sj] : 0.0f;
+    }
+    const float lambda = __builtin_amdgcn_exp2f(c.log_decay[h] * LOG2E);
+    for (int64_t x = 0; x < c.steps; ++x) {
+        const int64_t t = back ? c.steps - 1 - x : x;
+        const T *const q = (const T *)s.q + t * s.qs[0] + b * s.qs[1] + h * s.qs[2];
+        const T *const k = (const T *)s.k + t * s.ks[0] + b * s.ks[1] + h * s.ks[2];
+        const float v = mine ? (float)((const T *)s.v)[t * s.vs[0] + b * s.vs[1] + h * s.vs[2] + j] * s.grow : 0.0f;
+        const bool fresh = starts && (back ? x > 0 && starts[(t + 1) * groups] : starts[t * groups]);
+        float o = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 16 * KT; ++r) {
+            const int i = 2 * r + half;
+            if (i < dk) {
+                const float kv = (float)k[i] * v;
+                const float y = fresh ? kv : __builtin_fmaf(back ? 1.0f : lambda, S[r], kv);
+                o = __builtin_fmaf((float)q[i], y, o);
+                S[r] = back ? lambda * y : y;
+            }
+        }
+        o += __shfl_xor(o, 32, 64);
+        if (half == 0 && mine) ((T *)s.out)[t * s.os[0] + b * s.os[1] + h * s.os[2] + j] = (T)(o * s.carry);
+    }
+    if (s.state_out && mine) {
+        const bool clear = back && starts && c.steps > 0 && starts[0];
+#pragma unroll
+        for (int r = 0; r < 16 * KT; ++r) {
+            const int i = 2 * r + half;
+            if (i < dk) s.state_out[bh * c.area + (int64_t)i * s.si + (int64_t)j * s.sj] = clear ? 0.0f : S[r];
+        }
+    }
+}
+
+// The states that segments end with if none enters become those that they start with.
+__global__ __launch_bounds__(BLOCK) void k_between(const Call c, int64_t n)
+{
+    const Scan &s = c.scan[blockIdx.y];
+    const int64_t heads = c.batch * c.heads;
+    for (int64_t x = (int64_t)blockIdx.x * BLOCK + threadIdx.x; x < n; x += (int64_t)gridDim.x * BLOCK) {
+        const int64_t bh = x / c.area;
+        float a2 = c.log_decay[bh % c.heads] * LOG2E;
+        a2 = a2 < -1e30f ? -1e30f : a2;
+        const float f = __builtin_amdgcn_exp2f(a2 * (float)((int64_t)c.chunks * CHUNK));
+        float now = s.state ? s.state[x] : 0.0f;
+        for (int i = 0; i < c.segments; ++i) {
+            float *const y = s.between + i * n + x;
+            const float end = *y;
+            *y = now;
+            now = s.cut[i * heads + bh] ? end : __builtin_fmaf(f, now, end);
+        }
     }
 }
 
@@ -391,9 +587,106 @@ void copy(int64_t (&to)[3], const int64_t *from)
     for (int i = 0; i < 3; ++i) to[i] = from[i];
 }
 
-Call call_of(const swarp_decay_t *a)
+// How the steps are cut: into as many segments as give the chip WANTED waves, of four chunks at
+// least; the states between them cost a second reading of k and v.
+constexpr int WANTED = 4096, LEAST_CHUNKS = 4, MOST_SEGMENTS = 256;
+
+struct Cuts {
+    int segments, chunks;
+};
+Cuts cuts_of(const swarp_decay_t *a, int slices)
+{
+    const int64_t waves = a->batch * a->heads * slices, chunks = (a->steps + CHUNK - 1) / CHUNK;
+    int64_t n = waves > 0 ? WANTED / waves : 1;
+    if (n > chunks / LEAST_CHUNKS) n = chunks / LEAST_CHUNKS;
+    if (n > MOST_SEGMENTS) n = MOST_SEGMENTS;
+    if (n < 2) return {1, (int)(chunks < 1 << 30 ? (chunks < 1 ? 1 : chunks) : 1 << 30)};
+    const int64_t each = (chunks + n - 1) / n;
+    return {(int)((chunks + each - 1) / each), (int)each};
+}
+int slices_of(const swarp_decay_t *a, bool back)
+{
+    const int k = (a->dk + 31) / 32, v = (a->dv + 31) / 32;
+    return back ? 2 * k + v : v;
+}
+uint64_t work_of(const swarp_decay_t *a, bool back)
+{
+    const int slices = slices_of(a, back);
+    const Cuts n = cuts_of(a, slices);
+    const uint64_t heads = (uint64_t)(a->batch * a->heads), scans = n.segments < 2 ? 0 : back ? 2 : 1;
+    return n.segments * heads * (scans * (4ull * a->dk * a->dv + 4) + slices) + 256;
+}
+
+template <typename T, int KT, int WHAT> void scan(const Call &c, bool eights, hipStream_t st)
+{
+    const dim3 grid((unsigned)((c.units + WAVES - 1) / WAVES));
+    const int64_t n = c.units / c.segments;
+    if (eights) hipLaunchKernelGGL((k_scan<T, KT, WHAT, true>), grid, dim3(BLOCK), 0, st, c);
+    else hipLaunchKernelGGL((k_scan<T, KT, WHAT, false>), grid, dim3(BLOCK), 0, st, c);
+    if (WHAT == OUTPUTS)
+        hipLaunchKernelGGL((k_exact<T, KT>), dim3((unsigned)((n + WAVES - 1) / WAVES)), dim3(BLOCK), 0, st, c, n);
+}
+template <typename T, int WHAT> void scan(Call &c, hipStream_t st)
+{
+    int kt = 0;
+    bool eights = true;
+    c.slices = 0;
+    for (int i = 0; i < c.scans; ++i) {
+        eights &= c.scan[i].dk % 8 == 0 && c.scan[i].dv % 8 == 0;
+        c.scan[i].slices = (c.scan[i].dv + 31) / 32;
+        c.slices += c.scan[i].slices;
+        if ((c.scan[i].dk + 31) / 32 > kt) kt = (c.scan[i].dk + 31) / 32;
+    }
+    c.units = c.batch * c.heads * c.segments * c.slices;
+    if (kt == 1) scan<T, 1, WHAT>(c, eights, st);
+    else if (kt == 2) scan<T, 2, WHAT>(c, eights, st);
+    else scan<T, 4, WHAT>(c, eights, st);
+}
+
+// `ends`: the scans whose states between segments are to be found first; the others have theirs.
+template <typename T> void launch(Call &c, const Call &ends, hipStream_t st)
+{
+    if (c.segments > 1) {
+        Call e = ends;
+        scan<T, ENDS>(e, st);
+        const int64_t n = c.batch * c.heads * c.area, blocks = (n + BLOCK - 1) / BLOCK;
+        hipLaunchKernelGGL(k_between, dim3((unsigned)(blocks < 4096 ? blocks : 4096), e.scans), dim3(BLOCK), 0, st, e, n);
+    }
+    scan<T, OUTPUTS>(c, st);
+}
+
+int launch(const swarp_decay_t *a, Call &c, const Call &ends, hipStream_t st)
+{
+    switch (a->dtype) {
+    case SWARP_F32: launch<float>(c, ends, st); break;
+    case SWARP_BF16: launch<bf16>(c, ends, st); break;
+    default: launch<f16>(c, ends, st); break;
+    }
+    return launched();
+}
+
+int work(const swarp_decay_t *a, bool back)
+{
+    if (!a->work || a->work_bytes < work_of(a, back)) return fail("work must be set, swarp_decay_work_bytes() long");
+    if ((uintptr_t)a->work & 255u) return fail("work must be 256-byte aligned");
+    return 0;
+}
+
+// Room for the states between a scan's segments, the n-th of the call.
+void between(const swarp_decay_t *a, const Call &c, Scan &s, int n, int scans)
+{
+    const int64_t heads = c.segments * a->batch * a->heads;
+    s.between = (float *)a->work + n * heads * c.area;
+    s.cut = (int32_t *)((float *)a->work + scans * heads * c.area) + n * heads;
+}
+
+Call call_of(const swarp_decay_t *a, bool back)
 {
     Call c = {};
+    const Cuts n = cuts_of(a, slices_of(a, back));
+    c.segments = n.segments;
+    c.chunks = n.chunks;
+    c.wrong = (uint8_t *)a->work + work_of(a, back) - n.segments * a->batch * a->heads * slices_of(a, back);
     c.steps = a->steps;
     c.batch = a->batch;
     c.group = a->group;
@@ -404,44 +697,24 @@ Call call_of(const swarp_decay_t *a)
     return c;
 }
 
-template <typename T> void launch(Call &c, hipStream_t st)
-{
-    int kt = 0;
-    c.slices = 0;
-    for (int i = 0; i < c.scans; ++i) {
-        c.scan[i].slices = (c.scan[i].dv + 31) / 32;
-        c.slices += c.scan[i].slices;
-        if ((c.scan[i].dk + 31) / 32 > kt) kt = (c.scan[i].dk + 31) / 32;
-    }
-    c.units = c.batch * c.heads * c.slices;
-    const dim3 grid((unsigned)((c.units + WAVES - 1) / WAVES));
-    if (kt == 1) hipLaunchKernelGGL((k_scan<T, 1>), grid, dim3(BLOCK), 0, st, c);
-    else if (kt == 2) hipLaunchKernelGGL((k_scan<T, 2>), grid, dim3(BLOCK), 0, st, c);
-    else hipLaunchKernelGGL((k_scan<T, 4>), grid, dim3(BLOCK), 0, st, c);
-}
-
-int launch(const swarp_decay_t *a, Call &c, hipStream_t st)
-{
-    switch (a->dtype) {
-    case SWARP_F32: launch<float>(c, st); break;
-    case SWARP_BF16: launch<bf16>(c, st); break;
-    default: launch<f16>(c, st); break;
-    }
-    return launched();
-}
-
 }  // namespace
 
 extern "C" {
 
-uint64_t swarp_decay_work_bytes(const swarp_decay_t *a) { return check(a) ? 0 : 256; }
+uint64_t swarp_decay_work_bytes(const swarp_decay_t *a)
+{
+    if (check(a)) return 0;
+    const uint64_t f = work_of(a, false), b = work_of(a, true);
+    return f > b ? f : b;
+}
 
 int swarp_decay_fwd(const swarp_decay_t *a, void *stream)
 {
     if (check(a)) return -1;
     if (!a->batch) return 0;
     if (!a->log_decay || (a->steps && (!a->q || !a->k || !a->v || !a->out))) return fail("pointer arguments must be set");
-    Call c = call_of(a);
+    if (work(a, false)) return -1;
+    Call c = call_of(a, false);
     Scan &s = c.scan[0];
     s.q = a->q;
     s.k = a->k;
@@ -460,7 +733,8 @@ int swarp_decay_fwd(const swarp_decay_t *a, void *stream)
     s.si = a->dv;
     s.sj = 1;
     c.scans = 1;
-    return launch(a, c, (hipStream_t)stream);
+    if (c.segments > 1) between(a, c, s, 0, 1);
+    return launch(a, c, c, (hipStream_t)stream);
 }
 
 int swarp_decay_bwd(const swarp_decay_t *a, void *stream)
@@ -470,7 +744,8 @@ int swarp_decay_bwd(const swarp_decay_t *a, void *stream)
     if (!a->log_decay || (a->steps && (!a->q || !a->k || !a->v || !a->adj_out)))
         return fail("pointer arguments must be set");
     if (!a->d_q != !a->d_k || !a->d_q != !a->d_v) return fail("d_q, d_k and d_v are set together");
-    Call c = call_of(a);
+    if (work(a, true)) return -1;
+    Call c = call_of(a, true);
     const float scale = (float)a->scale;
     Scan q = {}, k = {}, v = {};
     q.q = k.k = v.v = a->adj_out;
@@ -503,11 +778,21 @@ int swarp_decay_bwd(const swarp_decay_t *a, void *stream)
     v.state_out = a->d_state;
     q.si = k.si = v.sj = 1;
     q.sj = k.sj = v.si = a->dv;
+    Call ends = c;
+    if (c.segments > 1) {
+        // (the states of the k and the v scan are one matrix and its transpose)
+        between(a, c, q, 0, 2);
+        between(a, c, v, 1, 2);
+        k.between = v.between;
+        ends.scan[0] = q;
+        ends.scan[1] = v;
+        ends.scans = 2;
+    }
     c.scan[0] = q;
     c.scan[1] = k;
     c.scan[2] = v;
     c.scans = 3;
-    return launch(a, c, (hipStream_t)stream);
+    return launch(a, c, ends, (hipStream_t)stream);
 }
 
 int swarp_decay_step(const swarp_decay_t *a, void *stream)
