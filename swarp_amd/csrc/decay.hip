@@ -57,7 +57,8 @@ struct Call {
     Scan scan[3];
     int scans, slices;     // slices of all scans
     int segments, chunks;  // of the steps, and chunks of a segment
-    int64_t units;         // waves: batch * heads * segments * slices
+    int64_t units;         // batch * heads * segments * slices: what one state goes through
+    int64_t each;          // batch entries that a wave takes, one after the other
     int64_t steps, batch, group;
     int heads, area;       // area: dk dv of a state
     const float *log_decay;
@@ -144,12 +145,16 @@ template <typename T> __device__ __forceinline__ float odd_of(const Part<T> &p, 
     return odd;
 }
 
-// Elements at .. at + 7 of a row of n; past its end its last ones, or with `zero` zeros.  EIGHTS: n is a
-// multiple of 8.
-template <typename T, bool EIGHTS> __device__ __forceinline__ Raw<T> row_of(const T *x, int at, int n, bool zero)
+// How the heads' widths fit the tiles: FULL, dk the tiles' and dv a multiple of 32; EIGHTS, both
+// multiples of 8; ANY.
+enum { ANY, EIGHTS, FULL };
+
+// Elements at .. at + 7 of a row of n; past its end its last ones, or with `zero` zeros.
+template <typename T, int FIT> __device__ __forceinline__ Raw<T> row_of(const T *x, int at, int n, bool zero)
 {
     Raw<T> r;
-    if constexpr (EIGHTS) {
+    if constexpr (FIT == FULL) r = __builtin_bit_cast(Raw<T>, *(const Span<T, 8> *)(x + at));
+    else if constexpr (FIT == EIGHTS) {
         r = __builtin_bit_cast(Raw<T>, *(const Span<T, 8> *)(x + (at < n ? at : n - 8)));
         if (zero) {
 #pragma unroll
@@ -209,21 +214,27 @@ template <typename T> __device__ __forceinline__ float element(const Part<T> &p,
 // What a wave does: the outputs of a segment, or (ENDS) the state that it ends with if none enters.
 enum { OUTPUTS, ENDS };
 
-// One wave: one head of a batch entry, 32 columns of v, the steps of a segment.  The state's columns
-// stay in its registers; KT: 32s of dk.  A wave works alone: its part of the LDS holds the chunk's
-// rows of k and v, to be read as columns.
-template <typename T, int KT, int WHAT, bool EIGHTS>
-__global__ __launch_bounds__(BLOCK, KT < 4 && sizeof(T) == 2 ? 2 : 1) void k_scan(const Call c)
+// One wave: one head, 32 columns of v, the steps of a segment, for `each` batch entries in turn.  The
+// state's columns stay in its registers; KT: 32s of dk.  A wave works alone: its part of the LDS
+// holds the chunk's rows of k and v, to be read as columns.  The next chunk's rows (the next entry's
+// first ones) are on their way meanwhile.
+template <typename T, int KT, int WHAT, int FIT>
+__global__ __launch_bounds__(BLOCK, (KT + (WHAT == OUTPUTS)) * sizeof(T) < 10 ? 2 : 1) void k_scan(const Call c)
 {
     constexpr int KP = 32 * KT + 16 / (int)sizeof(T), VP = 32 + 16 / (int)sizeof(T);
     __shared__ __align__(16) T room[WAVES][32 * (KP + VP)];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t unit = (int64_t)blockIdx.x * WAVES + wave;
-    if (unit >= c.units) return;
     T *const kx = room[wave], *const vx = kx + 32 * KP;
-    const int64_t part = unit / c.slices, bh = part / c.segments, b = bh / c.heads;
-    const int segment = (int)(part - bh * c.segments), h = (int)(bh - b * c.heads);
-    int slice = (int)(unit - part * c.slices), which = 0;
+    // (neighbouring waves have neighbouring columns, then segments, then heads)
+    const uint32_t kinds = (uint32_t)(c.slices * c.heads * c.segments);
+    const int64_t number = (int64_t)blockIdx.x * WAVES + wave, span = number / kinds;
+    const uint32_t kind = (uint32_t)(number - span * kinds), lines = kind / (uint32_t)c.slices;
+    const int h = (int)(lines / (uint32_t)c.segments), segment = (int)(lines % (uint32_t)c.segments);
+    int64_t b = span * c.each;
+    const int64_t b_end = b + c.each < c.batch ? b + c.each : c.batch;
+    if (b >= b_end) return;
+    int slice = (int)(kind % (uint32_t)c.slices), which = 0;
+    const int whole_slice = slice;
     while (slice >= c.scan[which].slices) slice -= c.scan[which++].slices;
     const Scan &s = c.scan[which];
     const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31, perm = swapped(col);
@@ -232,42 +243,14 @@ __global__ __launch_bounds__(BLOCK, KT < 4 && sizeof(T) == 2 ? 2 : 1) void k_sca
     const int64_t qt = way * s.qs[0], kt = way * s.ks[0], vt = way * s.vs[0], ot = way * s.os[0];
     const int64_t begin = (int64_t)segment * c.chunks * CHUNK;
     const int64_t end = begin + (int64_t)c.chunks * CHUNK < steps ? begin + (int64_t)c.chunks * CHUNK : steps;
-    const T *const q0 = (const T *)s.q + b * s.qs[1] + h * s.qs[2] + origin * s.qs[0];
-    const T *const k0 = (const T *)s.k + b * s.ks[1] + h * s.ks[2] + origin * s.ks[0];
-    const T *const v0 = (const T *)s.v + b * s.vs[1] + h * s.vs[2] + origin * s.vs[0];
     const int dk = s.dk, dv = s.dv, j0 = 32 * slice, j = j0 + perm;
-    const uint8_t *const starts = c.starts ? c.starts + b / c.group : nullptr;
+    const uint32_t group = (uint32_t)c.group;
     const int64_t groups = c.batch / c.group;
     const bool ends = end == steps;  // the last segment
-
-    // the state: element (32 t + 16 (r / 8) + 8 half + r % 8, j) in register r of tile t
-    f32x16 S[KT];
-    const float *const from = WHAT == ENDS ? nullptr
-                              : segment    ? s.between + ((int64_t)segment * c.batch * c.heads + bh) * c.area
-                              : s.state    ? s.state + bh * c.area
-                                           : nullptr;
-#pragma unroll
-    for (int t = 0; t < KT; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int i = 32 * t + 16 * (r >> 3) + 8 * half + (r & 7);
-            S[t][r] = from && i < dk && j < dv ? from[(int64_t)i * s.si + (int64_t)j * s.sj] : 0.0f;
-        }
-    bool none = !from;  // the state is still zero
-    // 0 as long as all that is multiplied is finite: a product with 0 is not 0 where it is not, and the
-    // head is done again by k_exact
-    float odd = 0.0f;
-    if (from) {
-#pragma unroll
-        for (int t = 0; t < KT; ++t)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) odd = __builtin_fmaf(S[t][r], 0.0f, odd);
-    }
 
     // powers: of the decay between the steps of a lane's scores, of what a step leaves in the state
     float a2 = c.log_decay[h] * LOG2E;
     a2 = a2 < -1e30f ? -1e30f : a2;  // (-inf times 0 steps is no decay)
-    const float lambda = __builtin_amdgcn_exp2f(a2);
     float D[16], u[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
@@ -275,19 +258,26 @@ __global__ __launch_bounds__(BLOCK, KT < 4 && sizeof(T) == 2 ? 2 : 1) void k_sca
         D[r] = col >= i ? s.score * __builtin_amdgcn_exp2f(a2 * (float)(col - i)) : 0.0f;
     }
     const float w0 = s.carry * __builtin_amdgcn_exp2f(a2 * (float)(col + (back ? 0 : 1)));
-    const uint8_t *sp = starts ? starts + (back ? steps - (begin + col) : begin + col) * groups : nullptr;
-    T *op = (T *)s.out + b * s.os[1] + h * s.os[2] + origin * s.os[0] + (begin + col) * ot + j0 + 8 * half;
     float whole = 0.0f;
     int width = 0;  // of the chunk that u and whole are for
-    uint32_t any = 0;
 
-    // Rows as they lie in memory: q by lane, k by swapped lane, v by quarters of rows.  Where a row or a
-    // step is past the end the last one is read again: only q has to be zero past dk, what else it
-    // brings meets a zero (of q, of D, of u) or is not written.
+    // Rows as they lie in memory: q by lane, k by swapped lane, v by quarters of rows; and whether
+    // anything enters a lane's step.  Where a row or a step is past the end the last one is read
+    // again: only q has to be zero past dk, what else it brings meets a zero (of q, of D, of u) or is
+    // not written.
     Raw<T> qr[2 * KT], kr[2 * KT], vr[2];
-    const T *qp = q0 + (begin + col) * qt, *kp = k0 + (begin + perm) * kt, *vp = v0 + (begin + (lane >> 2)) * vt;
-    const int64_t qn = CHUNK * qt, kn = CHUNK * kt, vn = CHUNK * vt;
-    auto load = [&](int L) {
+    uint8_t sr = 0;
+    const T *qb = (const T *)s.q + h * s.qs[2] + origin * s.qs[0] + b * s.qs[1] + (begin + col) * qt;
+    const T *kb = (const T *)s.k + h * s.ks[2] + origin * s.ks[0] + b * s.ks[1] + (begin + perm) * kt;
+    const T *vb = (const T *)s.v + h * s.vs[2] + origin * s.vs[0] + b * s.vs[1] + (begin + (lane >> 2)) * vt;
+    T *ob = (T *)s.out + h * s.os[2] + origin * s.os[0] + b * s.os[1] + (begin + col) * ot + j0 + 8 * half;
+    const T *qp = qb, *kp = kb, *vp = vb;
+    auto starts_of = [&](int64_t b) {
+        return c.starts + (uint32_t)b / group + (back ? steps - (begin + col) : begin + col) * groups;
+    };
+    const uint8_t *sp = c.starts ? starts_of(b) : nullptr;
+    auto load = [&](int64_t c0) {
+        const int L = (int)(end - c0 < CHUNK ? end - c0 : CHUNK);
         const T *x = qp, *y = kp, *z[2] = {vp, vp + 16 * vt};
         if (L < CHUNK) {
             x -= (col < L ? 0 : col - (L - 1)) * qt;
@@ -297,225 +287,273 @@ __global__ __launch_bounds__(BLOCK, KT < 4 && sizeof(T) == 2 ? 2 : 1) void k_sca
         }
 #pragma unroll
         for (int t = 0; t < 2 * KT; ++t) {
-            if (WHAT == OUTPUTS) qr[t] = row_of<T, EIGHTS>(x, 16 * t + 8 * half, dk, 16 * t + 16 > dk);
-            kr[t] = row_of<T, EIGHTS>(y, 16 * t + 8 * half, dk, false);
+            if (WHAT == OUTPUTS) qr[t] = row_of<T, FIT>(x, 16 * t + 8 * half, dk, 16 * t + 16 > dk);
+            kr[t] = row_of<T, FIT>(y, 16 * t + 8 * half, dk, false);
         }
 #pragma unroll
-        for (int t = 0; t < 2; ++t) vr[t] = row_of<T, EIGHTS>(z[t], j0 + 8 * (lane & 3), dv, false);
-        qp += qn;
-        kp += kn;
-        vp += vn;
+        for (int t = 0; t < 2; ++t) vr[t] = row_of<T, FIT>(z[t], j0 + 8 * (lane & 3), dv, false);
+        if (sp) {
+            sr = 0;
+            if (col < L && (!back || c0 + col > 0)) sr = *sp;
+        }
     };
-    if (begin < end) load((int)(end - begin < CHUNK ? end - begin : CHUNK));
-    for (int64_t c0 = begin; c0 < end; c0 += CHUNK) {
-        const int L = (int)(end - c0 < CHUNK ? end - c0 : CHUNK);
-        const bool more = c0 + CHUNK < end;
-        if (L != width) {
-            width = L;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int i = 16 * (r >> 3) + 8 * half + (r & 7);
-                u[r] = i < L ? s.grow * __builtin_amdgcn_exp2f(a2 * (float)(L - 1 - i + (back ? 1 : 0))) : 0.0f;
-            }
-            whole = __builtin_amdgcn_exp2f(a2 * (float)L);
-        }
-        // steps that nothing before them enters
-        uint32_t cut = 0;
-        if (starts) {
-            cut = (uint32_t)__ballot(half == 0 && col < L && (!back || c0 + col > 0) && *sp);
-            sp += CHUNK * way * groups;
-            any |= cut;
-        }
-        // the rows of k and v into LDS
-#pragma unroll
-        for (int t = 0; t < 2 * KT; ++t) *(Raw<T> *)(kx + perm * KP + 16 * t + 8 * half) = kr[t];
-#pragma unroll
-        for (int t = 0; t < 2; ++t) *(Raw<T> *)(vx + (16 * t + (lane >> 2)) * VP + 8 * (lane & 3)) = vr[t];
-        Part<T> qf[2 * KT];
-        f32x16 p = {};
-        if (WHAT == OUTPUTS) {
-#pragma unroll
-            for (int t = 0; t < 2 * KT; ++t) {
-                qf[t] = part_of(qr[t]);
-                mma<T>(p, part_of(kr[t]), qf[t]);
-            }
-        }
-        if (more) load((int)(end - c0 - CHUNK < CHUNK ? end - c0 - CHUNK : CHUNK));
-        Part<T> vf[2];
-        vf[0] = column_of<T>(vx, VP, 0, 0, lane);
-        vf[1] = column_of<T>(vx, VP, 16, 0, lane);
-        odd = odd_of<T>(vf[1], odd_of<T>(vf[0], odd));
-        Part<T> pf[2], pl[2];
-        if (WHAT == OUTPUTS) {
-            const uint32_t upto = cut & (0xffffffffu >> (31 - col));
-            const int since = upto ? 31 - __clz(upto) : 0;  // first step that enters step `col`
-#pragma unroll
-            for (int r = 0; r < 16; ++r) p[r] *= D[r];
-            // (a score is not finite wherever its q or k is not)
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                float y[8];
-#pragma unroll
-                for (int r = 0; r < 8; ++r) y[r] = p[8 * x + r];
-                if (cut) {
-#pragma unroll
-                    for (int r = 0; r < 8; ++r) {
-                        odd = __builtin_fmaf(y[r], 0.0f, odd);
-                        y[r] = 16 * x + 8 * half + r >= since ? y[r] : 0.0f;
-                    }
-                }
-                pf[x] = term_of<T>(y, true);
-                if (Part<T>::TERMS) pl[x] = term_of<T>(y, false);
-                odd = odd_of<T>(pf[x], odd);
-            }
-        }
-        if (WHAT == OUTPUTS) {
-            f32x16 o = {};
-            if (!none) {
-#pragma unroll
-                for (int x = 0; x < 2 * KT; ++x) {
-                    float y[8];
-#pragma unroll
-                    for (int r = 0; r < 8; ++r) y[r] = S[x >> 1][8 * (x & 1) + r];
-                    mma<T>(o, term_of<T>(y, true), qf[x]);
-                    if (Part<T>::TERMS) mma<T>(o, term_of<T>(y, false), qf[x]);
-                }
-                const float f = cut & (0xffffffffu >> (31 - col)) ? 0.0f : w0;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) o[r] *= f;
-            }
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                mma<T>(o, vf[x], pf[x]);
-                if (Part<T>::TERMS) mma<T>(o, vf[x], pl[x]);
-            }
-            if (col < L) {
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const int n = dv - j0 - 8 * half - 16 * x;
-                    Span<T, 8> e;
-#pragma unroll
-                    for (int r = 0; r < 8; ++r) e.e[r] = (T)o[8 * x + r];
-                    if (EIGHTS ? n > 0 : n >= 8) *(Span<T, 8> *)(op + 16 * x) = e;
-                    else if constexpr (!EIGHTS) {
-#pragma unroll
-                        for (int r = 0; r < 8; ++r)
-                            if (r < n) op[16 * x + r] = e.e[r];
-                    }
-                }
-            }
-        }
-        if (WHAT == ENDS || more || (ends && s.state_out)) {
-            const int kept = cut ? 31 - __clz(cut) : 0;  // first step that enters the leaving state
-            if (!none) {
-                const float f = cut ? 0.0f : whole;
-#pragma unroll
-                for (int t = 0; t < KT; ++t)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) S[t][r] *= f;
-            }
-            none = false;
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                float y[8];
-#pragma unroll
-                for (int r = 0; r < 8; ++r) y[r] = element(vf[x], r) * u[8 * x + r];
-                if (cut) {
-#pragma unroll
-                    for (int r = 0; r < 8; ++r) y[r] = 16 * x + 8 * half + r >= kept ? y[r] : 0.0f;
-                }
-                Part<T> w[3];
-                w[0] = term_of<T>(y, true);
-                if (Part<T>::TERMS) {
-                    w[1] = term_of<T>(y, true);
-                    w[2] = term_of<T>(y, false);
-                }
-#pragma unroll
-                for (int t = 0; t < KT; ++t) {
-                    const Part<T> kc = column_of<T>(kx, KP, 16 * x, 32 * t, lane);
-                    mma<T>(S[t], kc, w[0]);
-                    if (Part<T>::TERMS) {
-                        mma<T>(S[t], kc, w[1]);
-                        mma<T>(S[t], kc, w[2]);
-                    }
-                }
-            }
-        }
-        op += CHUNK * ot;
-    }
-    float *to = WHAT == ENDS        ? s.between + ((int64_t)segment * c.batch * c.heads + bh) * c.area
-                : ends && s.state_out ? s.state_out + bh * c.area
-                                      : nullptr;
-    if (to) {
-        // (backwards: what an episode that starts with the first step leaves of the state before it)
-        const bool clear = WHAT == OUTPUTS && back && starts && steps > 0 && starts[0];
+    if (begin < end) load(begin);
+    for (; b < b_end; ++b) {
+        const int64_t bh = b * c.heads + h;
+        // the state: element (32 t + 16 (r / 8) + 8 half + r % 8, j) in register r of tile t
+        f32x16 S[KT];
+        const float *from = WHAT == ENDS ? nullptr
+                                  : segment    ? s.between + ((int64_t)segment * c.batch * c.heads + bh) * c.area
+                                  : s.state    ? s.state + bh * c.area
+                                               : nullptr;
+        int rest = dk - 8 * half;  // (worked out at the place, not kept in registers throughout)
+        asm volatile("" : "+v"(rest));
+        if (from) from += (int64_t)(8 * half) * s.si + (int64_t)j * s.sj;
 #pragma unroll
         for (int t = 0; t < KT; ++t)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const int i = 32 * t + 16 * (r >> 3) + 8 * half + (r & 7);
-                if (i < dk && j < dv) to[(int64_t)i * s.si + (int64_t)j * s.sj] = clear ? 0.0f : S[t][r];
+                const int i = 32 * t + 16 * (r >> 3) + (r & 7);
+                S[t][r] = from && (FIT == FULL || (i < rest && j < dv)) ? from[i * s.si] : 0.0f;
             }
+        bool none = !from;  // the state is still zero
+        // 0 as long as all that is multiplied is finite: a product with 0 is not 0 where it is not, and the
+        // head is done again by k_exact
+        float odd = 0.0f;
+        if (from) {
+#pragma unroll
+            for (int t = 0; t < KT; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) odd = __builtin_fmaf(S[t][r], 0.0f, odd);
+        }
+
+        uint32_t any = 0;
+        T *op = ob;
+        for (int64_t c0 = begin; c0 < end; c0 += CHUNK) {
+            const int L = (int)(end - c0 < CHUNK ? end - c0 : CHUNK);
+            const bool more = c0 + CHUNK < end;
+            if (L != width) {
+                width = L;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int i = 16 * (r >> 3) + 8 * half + (r & 7);
+                    u[r] = i < L ? s.grow * __builtin_amdgcn_exp2f(a2 * (float)(L - 1 - i + (back ? 1 : 0))) : 0.0f;
+                }
+                whole = __builtin_amdgcn_exp2f(a2 * (float)L);
+            }
+            // steps that nothing before them enters
+            const uint32_t cut = (uint32_t)__ballot(sr);
+            any |= cut;
+            // the rows of k and v into LDS
+#pragma unroll
+            for (int t = 0; t < 2 * KT; ++t) *(Raw<T> *)(kx + perm * KP + 16 * t + 8 * half) = kr[t];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) *(Raw<T> *)(vx + (16 * t + (lane >> 2)) * VP + 8 * (lane & 3)) = vr[t];
+            Part<T> qf[2 * KT];
+            f32x16 p = {};
+            if (WHAT == OUTPUTS) {
+#pragma unroll
+                for (int t = 0; t < 2 * KT; ++t) {
+                    qf[t] = part_of(qr[t]);
+                    mma<T>(p, part_of(kr[t]), qf[t]);
+                }
+            }
+            if (more) {
+                qp += CHUNK * qt;
+                kp += CHUNK * kt;
+                vp += CHUNK * vt;
+                if (sp) sp += CHUNK * way * groups;
+            } else {
+                qp = qb += s.qs[1];
+                kp = kb += s.ks[1];
+                vp = vb += s.vs[1];
+                if (sp) sp = starts_of(b + 1);
+            }
+            if (more || b + 1 < b_end) load(more ? c0 + CHUNK : begin);
+            Part<T> vf[2];
+            vf[0] = column_of<T>(vx, VP, 0, 0, lane);
+            vf[1] = column_of<T>(vx, VP, 16, 0, lane);
+            odd = odd_of<T>(vf[1], odd_of<T>(vf[0], odd));
+            Part<T> pf[2], pl[2];
+            if (WHAT == OUTPUTS) {
+                const uint32_t upto = cut & (0xffffffffu >> (31 - col));
+                const int since = upto ? 31 - __clz(upto) : 0;  // first step that enters step `col`
+#pragma unroll
+                for (int r = 0; r < 16; ++r) p[r] *= D[r];
+                // (a score is not finite wherever its q or k is not)
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    float y[8];
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) y[r] = p[8 * x + r];
+                    if (cut) {
+#pragma unroll
+                        for (int r = 0; r < 8; ++r) {
+                            odd = __builtin_fmaf(y[r], 0.0f, odd);
+                            y[r] = 16 * x + 8 * half + r >= since ? y[r] : 0.0f;
+                        }
+                    }
+                    pf[x] = term_of<T>(y, true);
+                    if (Part<T>::TERMS) pl[x] = term_of<T>(y, false);
+                    odd = odd_of<T>(pf[x], odd);
+                }
+            }
+            if (WHAT == OUTPUTS) {
+                f32x16 o = {};
+                if (!none) {
+#pragma unroll
+                    for (int x = 0; x < 2 * KT; ++x) {
+                        float y[8];
+#pragma unroll
+                        for (int r = 0; r < 8; ++r) y[r] = S[x >> 1][8 * (x & 1) + r];
+                        mma<T>(o, term_of<T>(y, true), qf[x]);
+                        if (Part<T>::TERMS) mma<T>(o, term_of<T>(y, false), qf[x]);
+                    }
+                    const float f = cut & (0xffffffffu >> (31 - col)) ? 0.0f : w0;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o[r] *= f;
+                }
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    mma<T>(o, vf[x], pf[x]);
+                    if (Part<T>::TERMS) mma<T>(o, vf[x], pl[x]);
+                }
+                if (col < L) {
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const int n = dv - j0 - 8 * half - 16 * x;
+                        Span<T, 8> e;
+#pragma unroll
+                        for (int r = 0; r < 8; ++r) e.e[r] = (T)o[8 * x + r];
+                        if (FIT == FULL || (FIT == EIGHTS ? n > 0 : n >= 8)) *(Span<T, 8> *)(op + 16 * x) = e;
+                        else if constexpr (FIT == ANY) {
+#pragma unroll
+                            for (int r = 0; r < 8; ++r)
+                                if (r < n) op[16 * x + r] = e.e[r];
+                        }
+                    }
+                }
+            }
+            if (WHAT == ENDS || more || (ends && s.state_out)) {
+                const int kept = cut ? 31 - __clz(cut) : 0;  // first step that enters the leaving state
+                if (!none) {
+                    const float f = cut ? 0.0f : whole;
+#pragma unroll
+                    for (int t = 0; t < KT; ++t)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) S[t][r] *= f;
+                }
+                none = false;
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    float y[8];
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) y[r] = element(vf[x], r) * u[8 * x + r];
+                    if (cut) {
+#pragma unroll
+                        for (int r = 0; r < 8; ++r) y[r] = 16 * x + 8 * half + r >= kept ? y[r] : 0.0f;
+                    }
+                    Part<T> w[3];
+                    w[0] = term_of<T>(y, true);
+                    if (Part<T>::TERMS) {
+                        w[1] = term_of<T>(y, true);
+                        w[2] = term_of<T>(y, false);
+                    }
+#pragma unroll
+                    for (int t = 0; t < KT; ++t) {
+                        const Part<T> kc = column_of<T>(kx, KP, 16 * x, 32 * t, lane);
+                        mma<T>(S[t], kc, w[0]);
+                        if (Part<T>::TERMS) {
+                            mma<T>(S[t], kc, w[1]);
+                            mma<T>(S[t], kc, w[2]);
+                        }
+                    }
+                }
+            }
+            op += CHUNK * ot;
+        }
+        ob += s.os[1];
+        float *to = WHAT == ENDS        ? s.between + ((int64_t)segment * c.batch * c.heads + bh) * c.area
+                    : ends && s.state_out ? s.state_out + bh * c.area
+                                          : nullptr;
+        if (to) {
+            to += (int64_t)(8 * half) * s.si + (int64_t)j * s.sj;
+            asm volatile("" : "+v"(rest));
+            // (backwards: what an episode that starts with the first step leaves of the state before it)
+            const bool clear = WHAT == OUTPUTS && back && c.starts && steps > 0 && c.starts[(uint32_t)b / group];
+#pragma unroll
+            for (int t = 0; t < KT; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int i = 32 * t + 16 * (r >> 3) + (r & 7);
+                    if (FIT == FULL || (i < rest && j < dv)) to[i * s.si] = clear ? 0.0f : S[t][r];
+                }
+        }
+        if (WHAT == OUTPUTS) {
+            const bool wrong = __ballot(!(odd == 0.0f)) != 0;
+            if (lane == 0) c.wrong[(bh * c.segments + segment) * c.slices + whole_slice] = wrong;
+        }
+        if (WHAT == ENDS && lane == 0) s.cut[(int64_t)segment * c.batch * c.heads + bh] = any != 0;
     }
-    if (WHAT == OUTPUTS) {
-        const bool wrong = __ballot(!(odd == 0.0f)) != 0;
-        if (lane == 0) c.wrong[unit] = wrong;
-    }
-    if (WHAT == ENDS && lane == 0) s.cut[(int64_t)segment * c.batch * c.heads + bh] = any != 0;
 }
 
 // The heads (and columns) where something was not finite, step by step, as the definition has it: what
 // a start or the order of the steps keeps from an output does not reach it as a product with 0.
 template <typename T, int KT> __global__ __launch_bounds__(BLOCK) void k_exact(const Call c, int64_t n)
 {
-    const int64_t unit = (int64_t)blockIdx.x * WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (unit >= n) return;
     const int lane = threadIdx.x & 63, half = lane >> 5;
-    const int64_t bh = unit / c.slices, b = bh / c.heads;
-    const int h = (int)(bh - b * c.heads);
-    int slice = (int)(unit - bh * c.slices), which = 0;
-    bool wrong = false;
-    for (int i = lane; i < c.segments; i += 64) wrong |= c.wrong[(bh * c.segments + i) * c.slices + slice] != 0;
-    if (!__ballot(wrong)) return;
-    while (slice >= c.scan[which].slices) slice -= c.scan[which++].slices;
-    const Scan &s = c.scan[which];
-    const int j = 32 * slice + (lane & 31), dk = s.dk;
-    const bool back = s.back, mine = j < s.dv;
-    const uint8_t *const starts = c.starts ? c.starts + b / c.group : nullptr;
-    const int64_t groups = c.batch / c.group;
-    float S[KT * 16];
-#pragma unroll
-    for (int r = 0; r < 16 * KT; ++r) {
-        const int i = 2 * r + half;
-        S[r] = s.state && i < dk && mine ? s.state[bh * c.area + (int64_t)i * s.si + (int64_t)j * s.sj] : 0.0f;
+    const int64_t first = ((int64_t)blockIdx.x * WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * 64;
+    uint64_t wrong = 0;
+    if (first + lane < n) {
+        const int64_t bh = (first + lane) / c.slices, at = bh * c.segments * c.slices + (first + lane - bh * c.slices);
+        for (int i = 0; i < c.segments; ++i) wrong |= c.wrong[at + (int64_t)i * c.slices];
     }
-    const float lambda = __builtin_amdgcn_exp2f(c.log_decay[h] * LOG2E);
-    for (int64_t x = 0; x < c.steps; ++x) {
-        const int64_t t = back ? c.steps - 1 - x : x;
-        const T *const q = (const T *)s.q + t * s.qs[0] + b * s.qs[1] + h * s.qs[2];
-        const T *const k = (const T *)s.k + t * s.ks[0] + b * s.ks[1] + h * s.ks[2];
-        const float v = mine ? (float)((const T *)s.v)[t * s.vs[0] + b * s.vs[1] + h * s.vs[2] + j] * s.grow : 0.0f;
-        const bool fresh = starts && (back ? x > 0 && starts[(t + 1) * groups] : starts[t * groups]);
-        float o = 0.0f;
+    wrong = __ballot(wrong != 0);
+    for (; wrong; wrong &= wrong - 1) {
+        const int64_t unit = first + __ffsll((unsigned long long)wrong) - 1;
+        const int64_t bh = unit / c.slices, b = bh / c.heads;
+        const int h = (int)(bh - b * c.heads);
+        int slice = (int)(unit - bh * c.slices), which = 0;
+        while (slice >= c.scan[which].slices) slice -= c.scan[which++].slices;
+        const Scan &s = c.scan[which];
+        const int j = 32 * slice + (lane & 31), dk = s.dk;
+        const bool back = s.back, mine = j < s.dv;
+        const uint8_t *const starts = c.starts ? c.starts + b / c.group : nullptr;
+        const int64_t groups = c.batch / c.group;
+        float S[KT * 16];
 #pragma unroll
         for (int r = 0; r < 16 * KT; ++r) {
             const int i = 2 * r + half;
-            if (i < dk) {
-                const float kv = (float)k[i] * v;
-                const float y = fresh ? kv : __builtin_fmaf(back ? 1.0f : lambda, S[r], kv);
-                o = __builtin_fmaf((float)q[i], y, o);
-                S[r] = back ? lambda * y : y;
-            }
+            S[r] = s.state && i < dk && mine ? s.state[bh * c.area + (int64_t)i * s.si + (int64_t)j * s.sj] : 0.0f;
         }
-        o += __shfl_xor(o, 32, 64);
-        if (half == 0 && mine) ((T *)s.out)[t * s.os[0] + b * s.os[1] + h * s.os[2] + j] = (T)(o * s.carry);
-    }
-    if (s.state_out && mine) {
-        const bool clear = back && starts && c.steps > 0 && starts[0];
+        const float lambda = __builtin_amdgcn_exp2f(c.log_decay[h] * LOG2E);
+        for (int64_t x = 0; x < c.steps; ++x) {
+            const int64_t t = back ? c.steps - 1 - x : x;
+            const T *const q = (const T *)s.q + t * s.qs[0] + b * s.qs[1] + h * s.qs[2];
+            const T *const k = (const T *)s.k + t * s.ks[0] + b * s.ks[1] + h * s.ks[2];
+            const float v = mine ? (float)((const T *)s.v)[t * s.vs[0] + b * s.vs[1] + h * s.vs[2] + j] * s.grow : 0.0f;
+            const bool fresh = starts && (back ? x > 0 && starts[(t + 1) * groups] : starts[t * groups]);
+            float o = 0.0f;
 #pragma unroll
-        for (int r = 0; r < 16 * KT; ++r) {
-            const int i = 2 * r + half;
-            if (i < dk) s.state_out[bh * c.area + (int64_t)i * s.si + (int64_t)j * s.sj] = clear ? 0.0f : S[r];
+            for (int r = 0; r < 16 * KT; ++r) {
+                const int i = 2 * r + half;
+                if (i < dk) {
+                    const float kv = (float)k[i] * v;
+                    const float y = fresh ? kv : __builtin_fmaf(back ? 1.0f : lambda, S[r], kv);
+                    o = __builtin_fmaf((float)q[i], y, o);
+                    S[r] = back ? lambda * y : y;
+                }
+            }
+            o += __shfl_xor(o, 32, 64);
+            if (half == 0 && mine) ((T *)s.out)[t * s.os[0] + b * s.os[1] + h * s.os[2] + j] = (T)(o * s.carry);
+        }
+        if (s.state_out && mine) {
+            const bool clear = back && starts && c.steps > 0 && starts[0];
+#pragma unroll
+            for (int r = 0; r < 16 * KT; ++r) {
+                const int i = 2 * r + half;
+                if (i < dk) s.state_out[bh * c.area + (int64_t)i * s.si + (int64_t)j * s.sj] = clear ? 0.0f : S[r];
+            }
         }
     }
 }
@@ -589,7 +627,8 @@ void copy(int64_t (&to)[3], const int64_t *from)
 
 // How the steps are cut: into as many segments as give the chip WANTED waves, of four chunks at
 // least; the states between them cost a second reading of k and v.
-constexpr int WANTED = 4096, LEAST_CHUNKS = 4, MOST_SEGMENTS = 256;
+constexpr int WANTED = 6144, LEAST_CHUNKS = 4, MOST_SEGMENTS = 256;
+constexpr int64_t MOST_WAVES = 8192;  // of a launch, about: beyond it a wave takes several entries in turn
 
 struct Cuts {
     int segments, chunks;
@@ -597,7 +636,7 @@ struct Cuts {
 Cuts cuts_of(const swarp_decay_t *a, int slices)
 {
     const int64_t waves = a->batch * a->heads * slices, chunks = (a->steps + CHUNK - 1) / CHUNK;
-    int64_t n = waves > 0 ? WANTED / waves : 1;
+    int64_t n = waves > 0 ? (WANTED + waves - 1) / waves : 1;
     if (n > chunks / LEAST_CHUNKS) n = chunks / LEAST_CHUNKS;
     if (n > MOST_SEGMENTS) n = MOST_SEGMENTS;
     if (n < 2) return {1, (int)(chunks < 1 << 30 ? (chunks < 1 ? 1 : chunks) : 1 << 30)};
@@ -617,30 +656,37 @@ uint64_t work_of(const swarp_decay_t *a, bool back)
     return n.segments * heads * (scans * (4ull * a->dk * a->dv + 4) + slices) + 256;
 }
 
-template <typename T, int KT, int WHAT> void scan(const Call &c, bool eights, hipStream_t st)
+template <typename T, int KT, int WHAT> void scan(const Call &c, int fit, hipStream_t st)
 {
-    const dim3 grid((unsigned)((c.units + WAVES - 1) / WAVES));
-    const int64_t n = c.units / c.segments;
-    if (eights) hipLaunchKernelGGL((k_scan<T, KT, WHAT, true>), grid, dim3(BLOCK), 0, st, c);
-    else hipLaunchKernelGGL((k_scan<T, KT, WHAT, false>), grid, dim3(BLOCK), 0, st, c);
+    const int64_t waves = (c.batch + c.each - 1) / c.each * c.heads * c.segments * c.slices, n = c.units / c.segments;
+    const dim3 grid((unsigned)((waves + WAVES - 1) / WAVES));
+    if (fit == FULL) hipLaunchKernelGGL((k_scan<T, KT, WHAT, FULL>), grid, dim3(BLOCK), 0, st, c);
+    else if (fit == EIGHTS) hipLaunchKernelGGL((k_scan<T, KT, WHAT, EIGHTS>), grid, dim3(BLOCK), 0, st, c);
+    else hipLaunchKernelGGL((k_scan<T, KT, WHAT, ANY>), grid, dim3(BLOCK), 0, st, c);
     if (WHAT == OUTPUTS)
-        hipLaunchKernelGGL((k_exact<T, KT>), dim3((unsigned)((n + WAVES - 1) / WAVES)), dim3(BLOCK), 0, st, c, n);
+        hipLaunchKernelGGL((k_exact<T, KT>), dim3((unsigned)((n + BLOCK - 1) / BLOCK)), dim3(BLOCK), 0, st, c, n);
 }
 template <typename T, int WHAT> void scan(Call &c, hipStream_t st)
 {
     int kt = 0;
-    bool eights = true;
     c.slices = 0;
     for (int i = 0; i < c.scans; ++i) {
-        eights &= c.scan[i].dk % 8 == 0 && c.scan[i].dv % 8 == 0;
         c.scan[i].slices = (c.scan[i].dv + 31) / 32;
         c.slices += c.scan[i].slices;
         if ((c.scan[i].dk + 31) / 32 > kt) kt = (c.scan[i].dk + 31) / 32;
     }
+    int fit = FULL;
+    for (int i = 0; i < c.scans; ++i) {
+        if (c.scan[i].dk != 32 * kt || c.scan[i].dv % 32) fit = fit < EIGHTS ? fit : EIGHTS;
+        if (c.scan[i].dk % 8 || c.scan[i].dv % 8) fit = ANY;
+    }
     c.units = c.batch * c.heads * c.segments * c.slices;
-    if (kt == 1) scan<T, 1, WHAT>(c, eights, st);
-    else if (kt == 2) scan<T, 2, WHAT>(c, eights, st);
-    else scan<T, 4, WHAT>(c, eights, st);
+    c.each = c.units / MOST_WAVES;
+    if (c.each < 1) c.each = 1;
+    if (kt == 1) scan<T, 1, WHAT>(c, fit, st);
+    else if (kt == 2) scan<T, 2, WHAT>(c, fit, st);
+    else if (kt == 3) scan<T, 3, WHAT>(c, fit, st);
+    else scan<T, 4, WHAT>(c, fit, st);
 }
 
 // `ends`: the scans whose states between segments are to be found first; the others have theirs.
