@@ -49,7 +49,6 @@ struct Call {
     int dim, width;
     int dim_p;                // elements of a padded row of h and W
     int64_t wide;             // elements of a row of E
-    int64_t tall;             // elements of a row of E^T and of h^T
     int64_t first;            // row that the piece starts with
     int piece;                // rows that it has room for
     int targets32, sum;
@@ -61,13 +60,14 @@ struct Call {
     void *h;
     float *z_t, *ref, *top;   // target's logit; what E is relative to; largest logit
     float *inv, *inv_h;       // 1 / s; what h is multiplied by beside E^T
-    double *sums;             // of logp, one for 64 rows
+    double *sums;             // of logp, one for `few` rows
+    int few;                  // rows of a workgroup that joins: 1 or 64
     // of the piece
     int32_t *flag;
     float2 *parts;            // [n_parts][piece]: largest logit and sum of a part of a row
     int n_parts;
-    void *e, *et, *ht;
-    const void *w, *wt;       // padded weight, its transpose
+    void *e, *hs;             // exponentials; h as it goes beside them
+    const void *w;            // padded weight
 };
 
 // Rows of the piece that count.
@@ -174,32 +174,16 @@ __global__ __launch_bounds__(BLOCK) void k_pad(const T *in, int64_t rows, int n,
     }
 }
 
-// out [n][pitch] = in [rows][in_pitch] transposed, zero for rows past `rows` (up to `pitch`), each
-// row times scale[row] where that is set.  With `piece` the rows are the piece's.
-template <typename T>
-__global__ __launch_bounds__(BLOCK) void k_transpose(const T *in, int64_t rows, int64_t in_pitch, int64_t n, T *out,
-                                                     int64_t pitch, const float *scale, const Call c, int piece)
+// The piece's rows of h times inv_h, which the weight's gradient is made of, and zeros up to a whole
+// step (where E has none).  A wave a row.
+template <typename T> __global__ __launch_bounds__(BLOCK) void k_scale(const Call c)
 {
-    __shared__ float tile[64][65];
-    if (piece) {
-        rows = rows_of(c);
-        const int64_t end = (rows + 63) / 64 * 64;  // (whole steps: nothing reads more)
-        pitch = c.tall;
-        if ((int64_t)blockIdx.x * 64 >= end) return;
+    const int rows = rows_of(c), all = (rows + 31) / 32 * 32, lane = threadIdx.x & 63;
+    for (int r = blockIdx.x * (BLOCK / 64) + (threadIdx.x >> 6); r < all; r += gridDim.x * (BLOCK / 64)) {
+        const T *const x = (const T *)c.h + (c.first + (r < rows ? r : 0)) * c.dim_p;
+        const float f = r < rows ? c.inv_h[c.first + r] : 0.0f;
+        for (int k = lane; k < c.dim_p; k += 64) ((T *)c.hs)[(int64_t)r * c.dim_p + k] = r < rows ? (T)(up(x[k]) * f) : (T)0.0f;
     }
-    const int64_t r0 = (int64_t)blockIdx.x * 64, c0 = (int64_t)blockIdx.y * 64;
-    const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
-    for (int k = y; k < 64; k += 4) {
-        float v = 0.0f;
-        if (r0 + k < rows && c0 + x < n) {
-            v = up(in[(r0 + k) * in_pitch + c0 + x]);
-            if (scale) v *= scale[r0 + k];
-        }
-        tile[k][x] = v;
-    }
-    __syncthreads();
-    for (int k = y; k < 64; k += 4)
-        if (c0 + k < n && r0 + x < pitch) out[(c0 + k) * pitch + r0 + x] = (T)tile[x][k];
 }
 
 // ------------------------------------------------------------------ logits
@@ -221,8 +205,8 @@ __global__ __launch_bounds__(C::THREADS) void k_logits(const Call c, int nm, int
     C t;
     t.clear();
     const int64_t pitch = (int64_t)c.dim_p * sizeof(T);
-    const Operand a = {(const char *)c.w + v0 * pitch, pitch, c.width - v0};
-    const Operand b = {(const char *)c.h + (c.first + r0) * pitch, pitch, rows - r0};
+    const Operand a = {(const char *)c.w + v0 * pitch, pitch, c.width - v0, 0};
+    const Operand b = {(const char *)c.h + (c.first + r0) * pitch, pitch, rows - r0, 0};
     t.run(lds, a, b, 0, c.dim_p / C::KE);
 
     const int lane = threadIdx.x & 63, w = C::wave(), wm = w / C::WN, wn = w % C::WN;
@@ -254,16 +238,6 @@ __global__ __launch_bounds__(C::THREADS) void k_logits(const Call c, int nm, int
                 t.acc[i][j][r] = e;
             }
         if constexpr (STORE) {
-            T *const out = (T *)c.e + (int64_t)row * c.wide;
-            if (mine) {
-#pragma unroll
-                for (int i = 0; i < C::TM; ++i)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int64_t v = v0 + (wm * C::TM + i) * 32 + acc_row(r, lane);
-                        if (v < c.wide) out[v] = (T)(v < c.width ? t.acc[i][j][r] : 0.0f);
-                    }
-            }
             s += __shfl_xor(s, 32, 64);
             const float y = __shfl_xor(m, 32, 64);
             m = y > m ? y : m;
@@ -276,6 +250,38 @@ __global__ __launch_bounds__(C::THREADS) void k_logits(const Call c, int nm, int
         }
         if (lane < 32 && mine) c.parts[(int64_t)(tm * C::WM + wm) * c.piece + row] = make_float2(m, s);
     }
+    if constexpr (STORE) {
+        // through LDS, so that a row's are written together: 32 decisions of a wave's columns at a time
+        constexpr int PITCH = C::TM * 32 + 16 / (int)sizeof(T), PIECES = C::TM * 32 * (int)sizeof(T) / 16;
+        static_assert(C::BM * 4 + C::WAVES * 32 * PITCH * (int)sizeof(T) <= C::LDS, "a wave's part of a tile fits");
+        T *const mine = (T *)(lds + C::BM * 4) + w * 32 * PITCH;
+        const int64_t v = v0 + wm * C::TM * 32;
+#pragma unroll
+        for (int j = 0; j < C::TN; ++j) {
+#pragma unroll
+            for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; r += 4) {
+                    // (columns past the last are 0, not exp(-inf - NaN))
+                    struct __attribute__((aligned(4 * sizeof(T)))) Four { T e[4]; } y;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int k = i * 32 + acc_row(r + q, lane);
+                        y.e[q] = (T)(v + k < c.width ? t.acc[i][j][r + q] : 0.0f);
+                    }
+                    *(Four *)(mine + acc_col(lane) * PITCH + i * 32 + acc_row(r, lane)) = y;
+                }
+            __builtin_amdgcn_wave_barrier();
+            const int row0 = r0 + (wn * C::TN + j) * 32;
+#pragma unroll
+            for (int k = 0; k < 32 * PIECES / 64; ++k) {
+                const int at = k * 64 + lane, r = at / PIECES, e = at % PIECES * (16 / (int)sizeof(T));
+                if (row0 + r < rows && v + e < c.wide)
+                    *(u32x4 *)((T *)c.e + (int64_t)(row0 + r) * c.wide + v + e) = *(const u32x4 *)(mine + r * PITCH + e);
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+    }
 }
 
 // How a row's parts are joined.
@@ -284,20 +290,22 @@ enum { SUMS = 0,     // from parts relative to their largest: logp; ref becomes 
        KEPT2 = 2,    // the same after a second pass
        NORMED = 3 }; // E is there, normalised: E at the target
 
-template <typename T> __global__ __launch_bounds__(BLOCK) void k_join(const Call c, int how)
+// A workgroup takes ROWS rows, its threads every (BLOCK / ROWS)-th part of one.
+template <typename T, int ROWS> __global__ __launch_bounds__(BLOCK) void k_join(const Call c, int how)
 {
-    __shared__ float red[2][4][64];
-    __shared__ double total[64];
+    constexpr int WAYS = BLOCK / ROWS;
+    __shared__ float red[2][WAYS][ROWS];
+    __shared__ double total[ROWS];
     if (how == KEPT2 && !*c.flag) return;
-    const int rows = rows_of(c), lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int row = blockIdx.x * 64 + lane;
+    const int rows = rows_of(c), lane = threadIdx.x % ROWS, w = threadIdx.x / ROWS;
+    const int row = blockIdx.x * ROWS + lane;
     const bool mine = row < rows;
     const int64_t j = c.first + (mine ? row : 0);
-    if (blockIdx.x * 64 >= rows) return;
+    if (blockIdx.x * ROWS >= rows) return;
     const float ref = c.ref[j], zt = c.z_t[j];
     float s = 0.0f, m = -INFINITY;
     if (how != NORMED && mine) {
-        for (int k = w; k < c.n_parts; k += 4) {
+        for (int k = w; k < c.n_parts; k += WAYS) {
             const float2 p = c.parts[(int64_t)k * c.piece + row];
             if (how == SUMS) {
                 const float hi = p.x > m ? p.x : m, at = hi == -INFINITY ? 0.0f : hi;
@@ -314,9 +322,9 @@ template <typename T> __global__ __launch_bounds__(BLOCK) void k_join(const Call
     __syncthreads();
     if (w) return;
     float hi = m;
-    for (int k = 1; k < 4; ++k) hi = red[0][k][lane] > hi ? red[0][k][lane] : hi;
+    for (int k = 1; k < WAYS; ++k) hi = red[0][k][lane] > hi ? red[0][k][lane] : hi;
     s = 0.0f;
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < WAYS; ++k) {
         const float mk = red[0][k][lane];
         s += red[1][k][lane] * (how == SUMS && mk != -INFINITY ? exp_of(mk - hi) : 1.0f);
     }
@@ -352,10 +360,10 @@ template <typename T> __global__ __launch_bounds__(BLOCK) void k_join(const Call
     if (how != NORMED) {
         if (mine) c.logp[i] = logp;
         total[lane] = mine ? (double)logp : 0.0;
-        if (lane == 0) {
+        if (lane == 0) {  // (w == 0: one wave at most)
             double sum = 0;
-            for (int k = 0; k < 64; ++k) sum += total[k];
-            c.sums[c.first / 64 + blockIdx.x] = sum;
+            for (int k = 0; k < ROWS; ++k) sum += total[k];
+            c.sums[c.first / ROWS + blockIdx.x] = sum;
         }
     }
 }
@@ -370,20 +378,21 @@ __global__ __launch_bounds__(BLOCK) void k_again(const Call c)
 // ------------------------------------------------------------------ products of the gradients
 
 // out [m][n] (+)= scale[m] sum_k A[m][k] B[n][k], split along k over gridDim.y; the splits leave
-// their sums behind each other.
+// their sums behind each other.  B lies along k ([k][n]), A too where AK ([k][m]).
 struct Product {
     const void *a, *b;
     int64_t a_pitch, b_pitch;  // bytes
     int64_t m, n;              // rows of A and of B
-    int steps;                 // of k
-    int rows_m, rows_k;        // 1: m, or k, goes by the piece's rows
+    int k;                     // how many there are
+    int rows_m, rows_k;        // 1: m, or k, is the piece's rows instead
     int add;
     float times;
     const float *scale;        // of the rows of A, or NULL
     float *out;                // [m][n], or [splits][m][n]
 };
 
-template <typename T, typename C> __global__ __launch_bounds__(C::THREADS) void k_product(const Call c, const Product p, int nm, int nn)
+template <typename T, typename C, bool AK>
+__global__ __launch_bounds__(C::THREADS) void k_product(const Call c, const Product p, int nm, int nn)
 {
     extern __shared__ __align__(16) char lds[];
     const int rows = rows_of(c);
@@ -392,14 +401,17 @@ template <typename T, typename C> __global__ __launch_bounds__(C::THREADS) void 
     tile_of(blockIdx.x, gridDim.x, nm, nn, tm, tn);
     const int64_t m0 = (int64_t)tm * C::BM, n0 = (int64_t)tn * C::BN;
     if (m0 >= M) return;
-    int steps = p.rows_k ? (rows + C::KE - 1) / C::KE : p.steps;
+    const int k = p.rows_k ? rows : p.k;
+    int steps = (k + C::KE - 1) / C::KE;
     const int each = (steps + gridDim.y - 1) / gridDim.y, first = each * blockIdx.y;
     steps = first + each < steps ? first + each : steps;
     C t;
     t.clear();
-    const Operand a = {(const char *)p.a + m0 * p.a_pitch, p.a_pitch, (int)(M - m0 < C::BM ? M - m0 : C::BM)};
-    const Operand b = {(const char *)p.b + n0 * p.b_pitch, p.b_pitch, (int)(p.n - n0 < C::BN ? p.n - n0 : C::BN)};
-    t.run(lds, a, b, first, steps);
+    const Operand a = {(const char *)p.a + (AK ? m0 * (int64_t)sizeof(T) : m0 * p.a_pitch), p.a_pitch,
+                       (int)(M - m0 < C::BM ? M - m0 : C::BM), k};
+    const Operand b = {(const char *)p.b + n0 * (int64_t)sizeof(T), p.b_pitch, (int)(p.n - n0 < C::BN ? p.n - n0 : C::BN),
+                       p.rows_k ? (k + 31) / 32 * 32 : k};  // (h beside E^T ends with zeros)
+    t.template run<AK, true>(lds, a, b, first, steps);
     const int lane = threadIdx.x & 63, w = C::wave(), wm = w / C::WN, wn = w % C::WN;
     float *const out = p.out + (gridDim.y > 1 ? (int64_t)blockIdx.y * p.m * p.n : 0);
     const bool whole = gridDim.y == 1;
@@ -453,7 +465,7 @@ __global__ __launch_bounds__(BLOCK) void k_loss(const Call c)
     __shared__ double red[BLOCK / 64];
     const int64_t n = c.n_on ? *c.n_on : c.rows;
     double s = 0;
-    for (int64_t k = threadIdx.x; k < (n + 63) / 64; k += BLOCK) s += c.sums[k];
+    for (int64_t k = threadIdx.x; k < (n + c.few - 1) / c.few; k += BLOCK) s += c.sums[k];
     s = wave_sum(s);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
     __syncthreads();
@@ -488,16 +500,17 @@ template <> struct Tiles<bf16> { typedef Tile<bf16, 4, 2, 2, 4> Wide; typedef Ti
 template <> struct Tiles<f16> { typedef Tile<f16, 4, 2, 2, 4> Wide; typedef Tile<f16, 2, 1, 4, 1> Few; };
 template <> struct Tiles<float> { typedef Tile<float, 2, 2, 2, 2> Wide; typedef Tile<float, 2, 1, 4, 1> Few; };
 constexpr int FEW = 32;            // rows of a Few tile
+constexpr int FEW_JOINED = 2048;   // fewer rows: a workgroup joins the parts of one
 
 int64_t up_to(int64_t n, int64_t k) { return (n + k - 1) / k * k; }
 
 // Where everything lies in the work memory.
 struct Plan {
     int size;                 // bytes of an element
-    int64_t dim_p, wide, tall, piece, n_parts;
+    int64_t dim_p, wide, piece, n_parts;
     bool few, pad_w, grad;
     int split_h, split_w;
-    uint64_t index, counts, h, z_t, ref, top, inv, inv_h, sums, flag, parts, e, et, ht, w, wt, split, bytes;
+    uint64_t index, counts, h, z_t, ref, top, inv, inv_h, sums, flag, parts, e, hs, w, split, bytes;
 };
 
 int splits_of(int64_t tiles, int64_t steps)
@@ -526,11 +539,10 @@ Plan plan_of(const swarp_linear_ce_t *a)
     if (piece < 256) piece = 256;
     if (piece > up_to(N, 256)) piece = up_to(N, 256);
     p.piece = piece;
-    p.tall = up_to(piece, 64);
     p.pad_w = p.dim_p != D || ((uintptr_t)a->weight & 15);
     const int64_t t = p.size == 2 ? 256 : 128;
     p.split_h = splits_of(((piece + t - 1) / t) * ((D + t - 1) / t), p.wide / ke);
-    p.split_w = splits_of(((V + t - 1) / t) * ((D + t - 1) / t), p.tall / ke);
+    p.split_w = splits_of(((V + t - 1) / t) * ((D + t - 1) / t), piece / ke);
     uint64_t at = 0;
     auto room = [&](bool need, uint64_t bytes) {
         const uint64_t here = at;
@@ -546,13 +558,11 @@ Plan plan_of(const swarp_linear_ce_t *a)
     p.top = room(true, 4 * N);
     p.inv = room(true, 4 * N);
     p.inv_h = room(true, 4 * N);
-    p.sums = room(true, 8 * (N / 64 + 1));
+    p.sums = room(true, 8 * (N / (piece < FEW_JOINED ? 1 : 64) + 1));
     p.parts = room(true, 8ull * p.n_parts * piece);
     p.w = room(p.pad_w, (uint64_t)V * p.dim_p * p.size);
     p.e = room(p.grad, (uint64_t)piece * p.wide * p.size);
-    p.et = room(dw, (uint64_t)V * p.tall * p.size);
-    p.ht = room(dw, (uint64_t)D * p.tall * p.size);
-    p.wt = room(dh, (uint64_t)D * p.wide * p.size);
+    p.hs = room(dw, (uint64_t)piece * p.dim_p * p.size);
     uint64_t s = dh && p.split_h > 1 ? 4ull * p.split_h * piece * D : 0;
     const uint64_t s2 = dw && p.split_w > 1 ? 4ull * p.split_w * V * D : 0;
     p.split = room(true, s > s2 ? s : s2);
@@ -580,19 +590,25 @@ template <typename T, bool STORE> bool logits(const Call &c, bool few, int again
                : logits<T, typename Tiles<T>::Wide, STORE>(c, again, st);
 }
 
-template <typename T> bool product(const Call &c, Product p, int splits, float *parts, hipStream_t st)
+template <typename T, bool AK> bool product(const Call &c, Product p, int splits, float *parts, hipStream_t st)
 {
     typedef typename Tiles<T>::Wide C;
-    static const bool ok = lds_limit(k_product<T, C>, C::LDS);
+    static const bool ok = lds_limit(k_product<T, C, AK>, C::LDS);
     const int64_t nm = ((p.rows_m ? c.piece : p.m) + C::BM - 1) / C::BM, nn = (p.n + C::BN - 1) / C::BN;
     float *const out = p.out;
     if (splits > 1) p.out = parts;
-    hipLaunchKernelGGL((k_product<T, C>), dim3(nm * nn, splits), dim3(C::THREADS), C::LDS, st, c, p, (int)nm, (int)nn);
+    hipLaunchKernelGGL((k_product<T, C, AK>), dim3(nm * nn, splits), dim3(C::THREADS), C::LDS, st, c, p, (int)nm, (int)nn);
     if (splits > 1) {
         p.out = out;
         hipLaunchKernelGGL(k_splits, dim3(blocks_of(p.m * p.n / BLOCK)), dim3(BLOCK), 0, st, c, p, parts, splits);
     }
     return ok;
+}
+
+template <typename T> void join(const Call &c, int how, hipStream_t st)
+{
+    if (c.few == 1) hipLaunchKernelGGL((k_join<T, 1>), dim3((unsigned)c.piece), dim3(BLOCK), 0, st, c, how);
+    else hipLaunchKernelGGL((k_join<T, 64>), dim3((unsigned)((c.piece + 63) / 64)), dim3(BLOCK), 0, st, c, how);
 }
 
 template <typename T> int run(const swarp_linear_ce_t *a, hipStream_t st)
@@ -608,7 +624,6 @@ template <typename T> int run(const swarp_linear_ce_t *a, hipStream_t st)
     c.width = a->width;
     c.dim_p = (int)p.dim_p;
     c.wide = p.wide;
-    c.tall = p.tall;
     c.piece = (int)p.piece;
     c.targets32 = a->targets32;
     c.sum = a->sum;
@@ -628,11 +643,10 @@ template <typename T> int run(const swarp_linear_ce_t *a, hipStream_t st)
     c.flag = (int32_t *)(mem + p.flag);
     c.parts = (float2 *)(mem + p.parts);
     c.n_parts = (int)p.n_parts;
+    c.few = p.piece < FEW_JOINED ? 1 : 64;
     c.w = p.pad_w ? mem + p.w : (const char *)a->weight;
     c.e = p.grad ? mem + p.e : nullptr;
-    c.et = mem + p.et;
-    c.ht = mem + p.ht;
-    c.wt = mem + p.wt;
+    c.hs = mem + p.hs;
     if (a->mask && a->rows) {
         c.index = (int32_t *)(mem + p.index);
         c.n_on = a->place + a->rows;
@@ -646,50 +660,41 @@ template <typename T> int run(const swarp_linear_ce_t *a, hipStream_t st)
     if (p.pad_w)
         hipLaunchKernelGGL((k_pad<T>), dim3(blocks_of(c.width * p.dim_p / BLOCK)), dim3(BLOCK), 0, st,
                            (const T *)a->weight, (int64_t)c.width, c.dim, (T *)c.w, c.dim_p);
-    if (a->d_hidden)
-        hipLaunchKernelGGL((k_transpose<T>), dim3((c.width + 63) / 64, (c.dim + 63) / 64), dim3(BLOCK), 0, st,
-                           (const T *)a->weight, (int64_t)c.width, (int64_t)c.dim, (int64_t)c.dim, (T *)c.wt, c.wide,
-                           (const float *)nullptr, c, 0);
     bool ok = true;
     // (without a row too: the gradients are zeros)
     for (int64_t first = 0, n = 0; n == 0 || first < a->rows; first += p.piece, ++n) {
         c.first = first;
-        const dim3 joins((unsigned)((p.piece + 63) / 64)), block(BLOCK);
+        const dim3 block(BLOCK);
         if (!p.grad) {
             ok &= logits<T, false>(c, p.few, 0, st);
-            hipLaunchKernelGGL((k_join<T>), joins, block, 0, st, c, SUMS);
+            join<T>(c, SUMS, st);
             continue;
         }
         if (a->dtype == SWARP_F16) {
             ok &= logits<T, false>(c, p.few, 0, st);
-            hipLaunchKernelGGL((k_join<T>), joins, block, 0, st, c, SUMS);
+            join<T>(c, SUMS, st);
             ok &= logits<T, true>(c, p.few, 0, st);
-            hipLaunchKernelGGL((k_join<T>), joins, block, 0, st, c, NORMED);
+            join<T>(c, NORMED, st);
         } else {
             hipLaunchKernelGGL(k_clear, dim3(1), dim3(1), 0, st, c.flag);
             ok &= logits<T, true>(c, p.few, 0, st);
-            hipLaunchKernelGGL((k_join<T>), joins, block, 0, st, c, KEPT);
+            join<T>(c, KEPT, st);
             hipLaunchKernelGGL(k_again, dim3((unsigned)((p.piece + BLOCK - 1) / BLOCK)), block, 0, st, c);
             ok &= logits<T, true>(c, p.few, 1, st);
-            hipLaunchKernelGGL((k_join<T>), joins, block, 0, st, c, KEPT2);
+            join<T>(c, KEPT2, st);
         }
         float *const parts = (float *)(mem + p.split);
-        const int ke = STEP / sizeof(T);
+        const int64_t pitch_e = c.wide * (int64_t)sizeof(T), pitch_h = c.dim_p * (int64_t)sizeof(T);
         if (a->d_hidden) {
-            const Product y = {c.e, c.wt, (int64_t)(c.wide * sizeof(T)), (int64_t)(c.wide * sizeof(T)), p.piece, c.dim,
-                               (int)(c.wide / ke), 1, 0, 0, 1.0f, c.inv + first, a->d_hidden + first * c.dim};
-            ok &= product<T>(c, y, p.split_h, parts, st);
+            const Product y = {c.e, c.w, pitch_e, pitch_h, p.piece, c.dim, c.width, 1, 0, 0, 1.0f, c.inv + first,
+                               a->d_hidden + first * c.dim};
+            ok &= product<T, false>(c, y, p.split_h, parts, st);
         }
         if (a->d_weight) {
-            hipLaunchKernelGGL((k_transpose<T>), dim3((unsigned)(c.tall / 64), (c.width + 63) / 64), block, 0, st,
-                               (const T *)c.e, (int64_t)0, c.wide, (int64_t)c.width, (T *)c.et, c.tall,
-                               (const float *)nullptr, c, 1);
-            hipLaunchKernelGGL((k_transpose<T>), dim3((unsigned)(c.tall / 64), (c.dim + 63) / 64), block, 0, st,
-                               (const T *)c.h + first * c.dim_p, (int64_t)0, (int64_t)c.dim_p, (int64_t)c.dim, (T *)c.ht,
-                               c.tall, (const float *)(c.inv_h + first), c, 1);
-            const Product y = {c.et, c.ht, (int64_t)(c.tall * sizeof(T)), (int64_t)(c.tall * sizeof(T)), c.width, c.dim,
-                               0, 0, 1, n > 0, a->dtype == SWARP_F16 ? 1.0f / (1 << F16_BITS) : 1.0f, nullptr, a->d_weight};
-            ok &= product<T>(c, y, p.split_w, parts, st);
+            hipLaunchKernelGGL((k_scale<T>), dim3(blocks_of(p.piece / 4)), block, 0, st, c);
+            const Product y = {c.e, c.hs, pitch_e, pitch_h, c.width, c.dim, 0, 0, 1, n > 0,
+                               a->dtype == SWARP_F16 ? 1.0f / (1 << F16_BITS) : 1.0f, nullptr, a->d_weight};
+            ok &= product<T, true>(c, y, p.split_w, parts, st);
         }
         if (a->d_bias)
             hipLaunchKernelGGL((k_bias<T>), dim3((c.width + 63) / 64), block, 0, st, c, a->d_bias, n > 0);

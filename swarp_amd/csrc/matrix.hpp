@@ -1,9 +1,10 @@
 // matrix.hpp -- tiles of matrix products in the matrix cores, for the units that need them
 // (linear_ce.hip).
 //
-// A workgroup forms BM x BN elements of A B^T from operands whose rows run along k (in bytes:
-// 64 of a row and operand a step, 32 elements of 16 bits or 16 of float).  Operands go from memory
-// to LDS without passing through registers, three steps ahead of their use, into STAGES buffers.
+// A workgroup forms BM x BN elements of A B^T, a step of k at a time: 64 bytes, 32 elements of 16
+// bits or 16 of float.  An operand's rows run along k, or (ALONG) its memory's rows are steps of k
+// and run along the rows of the product: no transposed copy is made of either.  Operands go from
+// memory to LDS without passing through registers, three steps ahead of their use, into STAGES buffers.
 #pragma once
 #include "learn.hpp"
 
@@ -53,21 +54,23 @@ __device__ __forceinline__ int acc_row(int r, int lane) { return (r & 3) + 8 * (
 __device__ __forceinline__ int acc_col(int lane) { return lane & 31; }
 
 // An operand of a tile: rows [0, rows) of `base`, `pitch` bytes apart (a multiple of 16, as `base`).
-// Rows past the last one read as the last one.
+// Rows past the last one read as the last one.  ALONG k: `base` has `steps` rows of k, those past the
+// last read as the last (the other operand is zero there), and `rows` elements in each, up to a
+// multiple of 16 bytes.
 struct Operand {
     const char *base;
     int64_t pitch;
-    int rows;
+    int rows, steps;
 };
 
 template <typename T, int TM_, int TN_, int WM_, int WN_> struct Tile {
     static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_;
     static constexpr int BM = 32 * TM * WM, BN = 32 * TN * WN;
     static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
-    static constexpr int GROUPS = (BM + BN) / 16;           // of 16 rows: one load of a wave
-    // every wave loads alike (the last ones bring B's last rows again, behind them)
+    static constexpr int GROUPS = (BM + BN) / 16;           // of 1 KiB: one load of a wave
+    // every wave loads alike (the last ones bring B's last part again, behind it)
     static constexpr int EACH = (GROUPS + WAVES - 1) / WAVES;
-    static constexpr int BYTES = EACH * WAVES * 16 * STEP;  // of a stage
+    static constexpr int BYTES = EACH * WAVES * 1024;       // of a stage
     static constexpr int LDS = STAGES * BYTES;
     static constexpr int KE = STEP / sizeof(T);             // elements of a step
     static_assert(LDS <= 160 * 1024, "stages fit the LDS");
@@ -83,48 +86,111 @@ template <typename T, int TM_, int TN_, int WM_, int WN_> struct Tile {
                               (uint32_t)__builtin_amdgcn_readfirstlane((int)x));
     }
 
-    // 16 rows of 64 bytes to LDS: lane l brings row l / 4, piece (l % 4) ^ (row / 2 % 4), which puts
-    // the pieces that a wave's reads want at once (8 rows, one piece) on different banks.
+    // 1 KiB to LDS, 16 bytes a lane, in the order of the lanes.
     static __device__ __forceinline__ void fetch(uint32_t lds, uint32_t offset, const char *base)
     {
         asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2"
                      :: "s"(lds), "v"(offset), "s"(base) : "memory", "m0");
     }
 
+    // How pieces lie in LDS: where a wave's reads want several at once they are on different banks.
+    // Rows along k: 64 bytes of a row, its 16-byte pieces exchanged by the row.
+    static __device__ __forceinline__ int mix_row(int row) { return row >> 1 & 3; }
+    // Steps of k: W * sizeof(T) bytes of one, its 32-byte units exchanged by the step.
+    template <int W> static __device__ __forceinline__ int mix_step(int k)
+    {
+        const int x = sizeof(T) == 2 ? (k & 3) | (k >> 1 & 4) : k & 4;
+        return x & (W * (int)sizeof(T) / 32 - 1);
+    }
+
+    // Where lane l of a load finds what belongs at place g of an operand's part of a stage; ALONG, steps
+    // of k past `most` read as that one.
+    template <int W, bool ALONG>
+    static __device__ __forceinline__ uint32_t source(const Operand &o, int g, int lane, int most)
+    {
+        if constexpr (!ALONG) {
+            const int r = g * 16 + (lane >> 2), row = r < o.rows ? r : o.rows - 1;
+            return (uint32_t)(row * o.pitch) + (((lane & 3) ^ mix_row(r)) << 4);
+        } else {
+            constexpr int PIECES = W * sizeof(T) / 16;      // of a step
+            const int at = g * 64 + lane, k = at / PIECES, slot = at % PIECES;
+            const int from = k < most ? k : most;
+            int piece = (((slot >> 1) ^ mix_step<W>(k)) << 1) | (slot & 1);
+            const int last = (o.rows * (int)sizeof(T) + 15) / 16 - 1;
+            piece = piece < last ? piece : last;
+            return (uint32_t)(from * (int)o.pitch) + (piece << 4);
+        }
+    }
+
+    // The part of a 32-row tile that starts at row m0 of an operand, half s of a step.
+    template <int W, bool ALONG> static __device__ __forceinline__ u32x4 part(const char *x, int m0, int s, int lane)
+    {
+        const int half = lane >> 5;
+        if constexpr (!ALONG) {
+            const int r = m0 + (lane & 31);
+            return *(const u32x4 *)(x + r * STEP + (((2 * s + half) ^ mix_row(r)) << 4));
+        } else if constexpr (sizeof(T) == 2) {
+            // the transposing read: 16 lanes bring four steps of 16 rows, lane i keeps row i of them
+            typedef short s16x4 __attribute__((ext_vector_type(4)));
+            typedef __attribute__((address_space(3))) s16x4 *Ptr;
+            const int k = 16 * s + 8 * half + (lane >> 2 & 3), unit = (m0 >> 4) + (lane >> 4 & 1);
+            const char *const y = x + k * (W * 2) + ((unit ^ mix_step<W>(k)) << 5) + ((lane & 3) << 3);
+            const uint64_t lo = __builtin_bit_cast(uint64_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)(uintptr_t)y));
+            const uint64_t hi = __builtin_bit_cast(uint64_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)(uintptr_t)(y + 4 * (W * 2))));
+            return (u32x4){(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+        } else {
+            const int k = 4 * (2 * s + half), m = m0 + (lane & 31);
+            const char *const y = x + k * (W * 4) + (((m >> 3) ^ mix_step<W>(k)) << 5) + ((m & 7) << 2);
+            return (u32x4){*(const uint32_t *)y, *(const uint32_t *)(y + W * 4), *(const uint32_t *)(y + W * 8),
+                           *(const uint32_t *)(y + W * 12)};
+        }
+    }
+
+    template <bool AK, bool BK>
+    static __device__ __forceinline__ uint32_t offset(const Operand &a, const Operand &b, int at, int lane, int most)
+    {
+        const int g = at < GROUPS ? at : GROUPS - 1;         // (A's places, then B's)
+        return g >= BM / 16 ? source<BN, BK>(b, g - BM / 16, lane, most) : source<BM, AK>(a, g, lane, most);
+    }
+
     // acc += A[., k] B[., k] for steps [first, last).
+    template <bool AK = false, bool BK = false>
     __device__ __forceinline__ void run(char *lds, const Operand &a, const Operand &b, int first, int last)
     {
         if (first >= last) return;
         const int lane = threadIdx.x & 63, w = wave();
+        constexpr int GA = BM / 16;
         uint32_t off[EACH];
-        const char *pa = uniform(a.base + (int64_t)first * STEP), *pb = uniform(b.base + (int64_t)first * STEP);
 #pragma unroll
         for (int e = 0; e < EACH; ++e) {
-            const int at = w * EACH + e, g = at < GROUPS ? at : GROUPS - 1;  // (A's groups, then B's)
-            const bool isb = g >= BM / 16;
-            const Operand &o = isb ? b : a;
-            const int r = (isb ? g - BM / 16 : g) * 16 + (lane >> 2);
-            const int row = r < o.rows ? r : o.rows - 1;
-            off[e] = (uint32_t)(row * o.pitch) + (((lane & 3) ^ (r >> 1 & 3)) << 4);
+            off[e] = offset<AK, BK>(a, b, w * EACH + e, lane, KE);
         }
+        const int64_t step_a = AK ? KE * a.pitch : STEP, step_b = BK ? KE * b.pitch : STEP;
+        const char *pa = uniform(a.base + first * step_a), *pb = uniform(b.base + first * step_b);
         const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
         const int n = __builtin_amdgcn_readfirstlane(last - first);
-        int ahead = 0;
+        int at = __builtin_amdgcn_readfirstlane(first), ahead = 0;
         auto load = [&](int stage) {
 #pragma unroll
-            for (int e = 0; e < EACH; ++e)
-                fetch(__builtin_amdgcn_readfirstlane(lds0 + stage * BYTES + (w * EACH + e) * 1024), off[e],
-                      w * EACH + e >= BM / 16 ? pb : pa);
+            for (int e = 0; e < EACH; ++e) {
+                const bool isb = w * EACH + e >= GA;
+                uint32_t o = off[e];
+                if constexpr (AK || BK) {
+                    const int most = (isb ? b.steps : a.steps) - 1 - at * KE;
+                    if ((isb ? BK : AK) && most < KE - 1) o = offset<AK, BK>(a, b, w * EACH + e, lane, most);
+                }
+                fetch(__builtin_amdgcn_readfirstlane(lds0 + stage * BYTES + (w * EACH + e) * 1024), o, isb ? pb : pa);
+            }
             // (past the end the last step is brought again, into a buffer that nothing reads)
             if (++ahead < n) {
-                pa += STEP;
-                pb += STEP;
+                pa += step_a;
+                pb += step_b;
+                ++at;
             }
         };
 #pragma unroll
         for (int s = 0; s < STAGES - 1; ++s) load(s);
         const int wm = w / WN, wn = w % WN;
-        const int ra = wm * TM * 32 + (lane & 31), rb = BM + wn * TN * 32 + (lane & 31);
         int stage = 0;
         for (int k = 0; k < n; ++k) {
             // this wave's part of step k has come; then everybody's has, and nobody reads step k - 1
@@ -136,13 +202,10 @@ template <typename T, int TM_, int TN_, int WM_, int WN_> struct Tile {
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
                 u32x4 fa[TM], fb[TN];
-                const int piece = 2 * s + (lane >> 5);
 #pragma unroll
-                for (int i = 0; i < TM; ++i)
-                    fa[i] = *(const u32x4 *)(x + (ra + 32 * i) * STEP + ((piece ^ (ra >> 1 & 3)) << 4));
+                for (int i = 0; i < TM; ++i) fa[i] = part<BM, AK>(x, (wm * TM + i) * 32, s, lane);
 #pragma unroll
-                for (int j = 0; j < TN; ++j)
-                    fb[j] = *(const u32x4 *)(x + (rb + 32 * j) * STEP + ((piece ^ (rb >> 1 & 3)) << 4));
+                for (int j = 0; j < TN; ++j) fb[j] = part<BN, BK>(x + BM * STEP, (wn * TN + j) * 32, s, lane);
 #pragma unroll
                 for (int i = 0; i < TM; ++i)
 #pragma unroll
