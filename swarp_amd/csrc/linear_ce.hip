@@ -377,8 +377,7 @@ __global__ __launch_bounds__(BLOCK) void k_again(const Call c)
 
 // ------------------------------------------------------------------ products of the gradients
 
-// out [m][n] (+)= scale[m] sum_k A[m][k] B[n][k], split along k over gridDim.y; the splits leave
-// their sums behind each other.  B lies along k ([k][n]), A too where AK ([k][m]).
+// out [m][n] (+)= scale[m] sum_k A[m][k] B[n][k].  B lies along k ([k][n]), A too where AK ([k][m]).
 struct Product {
     const void *a, *b;
     int64_t a_pitch, b_pitch;  // bytes
@@ -388,76 +387,170 @@ struct Product {
     int add;
     float times;
     const float *scale;        // of the rows of A, or NULL
-    float *out;                // [m][n], or [splits][m][n]
+    float *out;                // [m][n]
+    float *parts;              // sums of splits
 };
 
+// How a product's tiles go over the workgroups, one for each place on the chip: whole tiles in rounds,
+// one a workgroup, and what is left of the last round along k, into as many splits as end soonest.
+// (8184 decisions of 50001 logits, a quarter of them masked, 1024 wide: 96 tiles for 256 places.)
+struct Share {
+    int nm, nn, steps;
+    int64_t whole;        // tiles that a workgroup does alone
+    int rest, splits;     // of the others
+};
+
+// A step of a tile of 256 x 256 takes some 0.45 us, a tile's sums to memory and back (all chip) 0.1.
+constexpr float SPLIT_COST = 0.25f;  // of a split of one tile, in steps of a round
+
+template <typename C> __device__ __forceinline__ Share share_of(int64_t m, int64_t n, int steps, int places)
+{
+    Share s;
+    s.nm = (int)((m + C::BM - 1) / C::BM);
+    s.nn = (int)((n + C::BN - 1) / C::BN);
+    s.steps = steps;
+    const int64_t tiles = (int64_t)s.nm * s.nn;
+    s.rest = (int)(tiles % places);
+    s.whole = tiles - s.rest;
+    s.splits = 1;
+    float least = (float)steps;
+    constexpr int WAYS[] = {2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48, 64, 96, 128, 192, 256};
+    for (int w : WAYS) {
+        if (!s.rest || s.rest * w > 2 * places || w * 4 > steps) break;
+        const float cost = (float)((s.rest * w + places - 1) / places) * (float)((steps + w - 1) / w) + SPLIT_COST * (float)(s.rest * w);
+        if (cost < least) {
+            least = cost;
+            s.splits = w;
+        }
+    }
+    return s;
+}
+// The m and n of a tile: groups of eight rows of tiles share what they read of B while it is in L2.
+__device__ __forceinline__ void place_of(const Share &s, int64_t t, int &m, int &n)
+{
+    const int per = 8 * s.nn, group = (int)(t / per), first = group * 8, size = s.nm - first < 8 ? s.nm - first : 8;
+    const int at = (int)(t - (int64_t)group * per);
+    m = first + at % size;
+    n = at / size;
+}
+
 template <typename T, typename C, bool AK>
-__global__ __launch_bounds__(C::THREADS) void k_product(const Call c, const Product p, int nm, int nn)
+__global__ __launch_bounds__(C::THREADS, 2) void k_product(const Call c, const Product p)
 {
     extern __shared__ __align__(16) char lds[];
-    const int rows = rows_of(c);
+    const int rows = rows_of(c), places = gridDim.x;
     const int64_t M = p.rows_m ? rows : p.m;
-    int tm, tn;
-    tile_of(blockIdx.x, gridDim.x, nm, nn, tm, tn);
-    const int64_t m0 = (int64_t)tm * C::BM, n0 = (int64_t)tn * C::BN;
-    if (m0 >= M) return;
     const int k = p.rows_k ? rows : p.k;
-    int steps = (k + C::KE - 1) / C::KE;
-    const int each = (steps + gridDim.y - 1) / gridDim.y, first = each * blockIdx.y;
-    steps = first + each < steps ? first + each : steps;
-    C t;
-    t.clear();
-    const Operand a = {(const char *)p.a + (AK ? m0 * (int64_t)sizeof(T) : m0 * p.a_pitch), p.a_pitch,
-                       (int)(M - m0 < C::BM ? M - m0 : C::BM), k};
-    const Operand b = {(const char *)p.b + n0 * (int64_t)sizeof(T), p.b_pitch, (int)(p.n - n0 < C::BN ? p.n - n0 : C::BN),
-                       p.rows_k ? (k + 31) / 32 * 32 : k};  // (h beside E^T ends with zeros)
-    t.template run<AK, true>(lds, a, b, first, steps);
+    const Share s = share_of<C>(M, p.n, (k + C::KE - 1) / C::KE, places);
     const int lane = threadIdx.x & 63, w = C::wave(), wm = w / C::WN, wn = w % C::WN;
-    float *const out = p.out + (gridDim.y > 1 ? (int64_t)blockIdx.y * p.m * p.n : 0);
-    const bool whole = gridDim.y == 1;
-#pragma unroll
-    for (int i = 0; i < C::TM; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int64_t m = m0 + (wm * C::TM + i) * 32 + acc_row(r, lane);
-            if (m >= M) continue;
-            const float f = !whole ? 1.0f : p.scale ? p.times * p.scale[m] : p.times;
-#pragma unroll
-            for (int j = 0; j < C::TN; ++j) {
-                const int64_t n = n0 + (wn * C::TN + j) * 32 + acc_col(lane);
-                if (n >= p.n) continue;
-                float *const y = out + m * p.n + n;
-                *y = f * t.acc[i][j][r] + (whole && p.add ? *y : 0.0f);
-            }
+    // (workgroups go round the eight dies one by one: each die, with its own L2, has neighbouring tiles)
+    const int mine = places % 8 ? blockIdx.x : (blockIdx.x & 7) * (places / 8) + (blockIdx.x >> 3);
+    for (int64_t u = mine; u < s.whole + (int64_t)s.rest * s.splits; u += places) {
+        const bool whole = u < s.whole || s.splits == 1;
+        const int64_t part = u - s.whole;
+        int first = 0, last = s.steps, tm, tn;
+        if (!whole) {
+            const int each = (s.steps + s.splits - 1) / s.splits;
+            first = (int)(part / s.rest) * each;
+            last = first + each < s.steps ? first + each : s.steps;
         }
-}
-
-__global__ __launch_bounds__(BLOCK) void k_splits(const Call c, const Product p, const float *parts, int splits)
-{
-    const int64_t all = (p.rows_m ? (int64_t)rows_of(c) : p.m) * p.n;
-    for (int64_t k = (int64_t)blockIdx.x * BLOCK + threadIdx.x; k < all; k += (int64_t)gridDim.x * BLOCK) {
-        float s = 0.0f;
-        for (int i = 0; i < splits; ++i) s += parts[(int64_t)i * p.m * p.n + k];
-        s *= p.scale ? p.times * p.scale[k / p.n] : p.times;
-        p.out[k] = s + (p.add ? p.out[k] : 0.0f);
+        place_of(s, whole ? u : s.whole + part % s.rest, tm, tn);
+        const int64_t m0 = (int64_t)tm * C::BM, n0 = (int64_t)tn * C::BN;
+        C t;
+        t.clear();
+        const Operand a = {(const char *)p.a + (AK ? m0 * (int64_t)sizeof(T) : m0 * p.a_pitch), p.a_pitch,
+                           (int)(M - m0 < C::BM ? M - m0 : C::BM), k};
+        const Operand b = {(const char *)p.b + n0 * (int64_t)sizeof(T), p.b_pitch, (int)(p.n - n0 < C::BN ? p.n - n0 : C::BN),
+                           p.rows_k ? (k + 31) / 32 * 32 : k};  // (h beside E^T ends with zeros)
+        t.template run<AK, true>(lds, a, b, first, last);
+        // (where each element goes is worked out here, and not kept in registers from tile to tile)
+        int at = lane;
+        asm volatile("" : "+v"(at));
+        const int i0 = wm * C::TM * 32 + acc_row(0, at), j0 = wn * C::TN * 32 + acc_col(at);
+        if (whole) {
+            float *const out = p.out + (m0 + i0) * p.n + n0 + j0;
+#pragma unroll
+            for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int row = 32 * i + acc_row(r, 0);
+                    if (m0 + i0 + row >= M) continue;
+                    const float f = p.scale ? p.times * p.scale[m0 + i0 + row] : p.times;
+#pragma unroll
+                    for (int j = 0; j < C::TN; ++j)
+                        if (n0 + j0 + 32 * j < p.n) {
+                            float *const y = out + row * p.n + 32 * j;
+                            *y = f * t.acc[i][j][r] + (p.add ? *y : 0.0f);
+                        }
+                }
+        } else {
+            float *const sums = p.parts + part * (C::BM * C::BN) + i0 * C::BN + j0;
+#pragma unroll
+            for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+#pragma unroll
+                    for (int j = 0; j < C::TN; ++j) sums[(32 * i + acc_row(r, 0)) * C::BN + 32 * j] = t.acc[i][j][r];
+        }
     }
 }
 
-// d b (+)= sum_i inv_i E_ij: a workgroup takes 64 columns, its waves every fourth row.
-template <typename T> __global__ __launch_bounds__(BLOCK) void k_bias(const Call c, float *out, int add)
+// The tiles whose sums lie in splits.
+template <typename C> __global__ __launch_bounds__(BLOCK) void k_splits(const Call c, const Product p, int ke, int places)
 {
-    __shared__ float red[4][64];
+    const int rows = rows_of(c), k = p.rows_k ? rows : p.k;
+    const int64_t M = p.rows_m ? rows : p.m;
+    const Share s = share_of<C>(M, p.n, (k + ke - 1) / ke, places);
+    if (s.splits == 1) return;
+    constexpr int AREA = C::BM * C::BN;
+    for (int64_t x = (int64_t)blockIdx.x * BLOCK + threadIdx.x; x < (int64_t)s.rest * AREA; x += (int64_t)gridDim.x * BLOCK) {
+        const int at = (int)(x % AREA), i = (int)(x / AREA);
+        int tm, tn;
+        place_of(s, s.whole + i, tm, tn);
+        const int64_t m = (int64_t)tm * C::BM + at / C::BN, n = (int64_t)tn * C::BN + at % C::BN;
+        if (m >= M || n >= p.n) continue;
+        float y = 0.0f;
+        for (int w = 0; w < s.splits; ++w) y += p.parts[((int64_t)w * s.rest + i) * AREA + at];
+        float *const out = p.out + m * p.n + n;
+        *out = y * (p.scale ? p.times * p.scale[m] : p.times) + (p.add ? *out : 0.0f);
+    }
+}
+
+// d b = sum_i inv_i E_ij: a workgroup takes 64 lanes' 16 bytes of columns and one of BIAS_WAYS shares of
+// the rows, its waves every fourth of these; the shares are added by k_bias_sum.
+constexpr int BIAS_WAYS = 32;
+
+template <typename T> __global__ __launch_bounds__(BLOCK) void k_bias(const Call c, float *parts)
+{
+    constexpr int V = 16 / sizeof(T);
+    struct __align__(16) Line { T e[V]; };
+    __shared__ float red[4][64 * V];
     const int rows = rows_of(c), lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int64_t v = (int64_t)blockIdx.x * 64 + lane;
-    float s = 0.0f;
-    if (v < c.width)
-        for (int r = w; r < rows; r += 4) s = __builtin_fmaf(c.inv[c.first + r], up(((const T *)c.e)[(int64_t)r * c.wide + v]), s);
-    red[w][lane] = s;
+    const int each = (rows + BIAS_WAYS - 1) / BIAS_WAYS, first = each * blockIdx.y, last = first + each < rows ? first + each : rows;
+    const int64_t v = (int64_t)blockIdx.x * (64 * V) + lane * V;
+    float s[V] = {};
+    if (v < c.wide)
+        for (int r = first + w; r < last; r += 4) {
+            const Line y = *(const Line *)((const T *)c.e + (int64_t)r * c.wide + v);
+            const float f = c.inv[c.first + r];
+#pragma unroll
+            for (int k = 0; k < V; ++k) s[k] = __builtin_fmaf(f, up(y.e[k]), s[k]);
+        }
+#pragma unroll
+    for (int k = 0; k < V; ++k) red[w][lane * V + k] = s[k];
     __syncthreads();
-    if (w == 0 && v < c.width) {
-        s = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
-        out[v] = s + (add ? out[v] : 0.0f);
+    for (int k = threadIdx.x; k < 64 * V; k += BLOCK) {
+        const int64_t at = (int64_t)blockIdx.x * (64 * V) + k;
+        if (at < c.width) parts[(int64_t)blockIdx.y * c.width + at] = (red[0][k] + red[1][k]) + (red[2][k] + red[3][k]);
     }
+}
+__global__ __launch_bounds__(BLOCK) void k_bias_sum(int width, const float *parts, float *out, int add)
+{
+    const int v = blockIdx.x * BLOCK + threadIdx.x;
+    if (v >= width) return;
+    float s = 0.0f;
+    for (int k = 0; k < BIAS_WAYS; ++k) s += parts[(int64_t)k * width + v];
+    out[v] = s + (add ? out[v] : 0.0f);
 }
 
 __global__ __launch_bounds__(BLOCK) void k_loss(const Call c)
@@ -509,17 +602,11 @@ struct Plan {
     int size;                 // bytes of an element
     int64_t dim_p, wide, piece, n_parts;
     bool few, pad_w, grad;
-    int split_h, split_w;
-    uint64_t index, counts, h, z_t, ref, top, inv, inv_h, sums, flag, parts, e, hs, w, split, bytes;
+    uint64_t index, counts, h, z_t, ref, top, inv, inv_h, sums, flag, parts, e, hs, w, split, bias, bytes;
 };
 
-int splits_of(int64_t tiles, int64_t steps)
-{
-    // fill the chip where the output alone does not: at least 8 steps each
-    int64_t s = tiles < 192 ? (256 + tiles - 1) / tiles : 1;
-    if (s > steps / 8) s = steps / 8;
-    return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
-}
+// Workgroups of a product: one a compute unit with 128 KiB of LDS, two with 64.
+int places(int size) { return size == 2 ? 256 : 512; }
 
 Plan plan_of(const swarp_linear_ce_t *a)
 {
@@ -540,9 +627,6 @@ Plan plan_of(const swarp_linear_ce_t *a)
     if (piece > up_to(N, 256)) piece = up_to(N, 256);
     p.piece = piece;
     p.pad_w = p.dim_p != D || ((uintptr_t)a->weight & 15);
-    const int64_t t = p.size == 2 ? 256 : 128;
-    p.split_h = splits_of(((piece + t - 1) / t) * ((D + t - 1) / t), p.wide / ke);
-    p.split_w = splits_of(((V + t - 1) / t) * ((D + t - 1) / t), piece / ke);
     uint64_t at = 0;
     auto room = [&](bool need, uint64_t bytes) {
         const uint64_t here = at;
@@ -563,9 +647,9 @@ Plan plan_of(const swarp_linear_ce_t *a)
     p.w = room(p.pad_w, (uint64_t)V * p.dim_p * p.size);
     p.e = room(p.grad, (uint64_t)piece * p.wide * p.size);
     p.hs = room(dw, (uint64_t)piece * p.dim_p * p.size);
-    uint64_t s = dh && p.split_h > 1 ? 4ull * p.split_h * piece * D : 0;
-    const uint64_t s2 = dw && p.split_w > 1 ? 4ull * p.split_w * V * D : 0;
-    p.split = room(true, s > s2 ? s : s2);
+    // (twice as many splits as places, of whole tiles: share_of)
+    p.split = room(dh || dw, p.size == 2 ? 2ull * places(2) * 256 * 256 * 4 : 2ull * places(4) * 128 * 128 * 4);
+    p.bias = room(a->d_bias, 4ull * BIAS_WAYS * V);
     p.bytes = at;
     return p;
 }
@@ -590,18 +674,13 @@ template <typename T, bool STORE> bool logits(const Call &c, bool few, int again
                : logits<T, typename Tiles<T>::Wide, STORE>(c, again, st);
 }
 
-template <typename T, bool AK> bool product(const Call &c, Product p, int splits, float *parts, hipStream_t st)
+template <typename T, bool AK> bool product(const Call &c, const Product &p, hipStream_t st)
 {
     typedef typename Tiles<T>::Wide C;
     static const bool ok = lds_limit(k_product<T, C, AK>, C::LDS);
-    const int64_t nm = ((p.rows_m ? c.piece : p.m) + C::BM - 1) / C::BM, nn = (p.n + C::BN - 1) / C::BN;
-    float *const out = p.out;
-    if (splits > 1) p.out = parts;
-    hipLaunchKernelGGL((k_product<T, C, AK>), dim3(nm * nn, splits), dim3(C::THREADS), C::LDS, st, c, p, (int)nm, (int)nn);
-    if (splits > 1) {
-        p.out = out;
-        hipLaunchKernelGGL(k_splits, dim3(blocks_of(p.m * p.n / BLOCK)), dim3(BLOCK), 0, st, c, p, parts, splits);
-    }
+    const int n = places(sizeof(T));
+    hipLaunchKernelGGL((k_product<T, C, AK>), dim3(n), dim3(C::THREADS), C::LDS, st, c, p);
+    hipLaunchKernelGGL((k_splits<C>), dim3(1024), dim3(BLOCK), 0, st, c, p, C::KE, n);
     return ok;
 }
 
@@ -687,17 +766,22 @@ template <typename T> int run(const swarp_linear_ce_t *a, hipStream_t st)
         const int64_t pitch_e = c.wide * (int64_t)sizeof(T), pitch_h = c.dim_p * (int64_t)sizeof(T);
         if (a->d_hidden) {
             const Product y = {c.e, c.w, pitch_e, pitch_h, p.piece, c.dim, c.width, 1, 0, 0, 1.0f, c.inv + first,
-                               a->d_hidden + first * c.dim};
-            ok &= product<T, false>(c, y, p.split_h, parts, st);
+                               a->d_hidden + first * c.dim, parts};
+            ok &= product<T, false>(c, y, st);
         }
         if (a->d_weight) {
             hipLaunchKernelGGL((k_scale<T>), dim3(blocks_of(p.piece / 4)), block, 0, st, c);
             const Product y = {c.e, c.hs, pitch_e, pitch_h, c.width, c.dim, 0, 0, 1, n > 0,
-                               a->dtype == SWARP_F16 ? 1.0f / (1 << F16_BITS) : 1.0f, nullptr, a->d_weight};
-            ok &= product<T, true>(c, y, p.split_w, parts, st);
+                               a->dtype == SWARP_F16 ? 1.0f / (1 << F16_BITS) : 1.0f, nullptr, a->d_weight, parts};
+            ok &= product<T, true>(c, y, st);
         }
         if (a->d_bias)
-            hipLaunchKernelGGL((k_bias<T>), dim3((c.width + 63) / 64), block, 0, st, c, a->d_bias, n > 0);
+        {
+            float *const sums = (float *)(mem + p.bias);
+            const int per = 64 * 16 / sizeof(T);
+            hipLaunchKernelGGL((k_bias<T>), dim3((c.width + per - 1) / per, BIAS_WAYS), block, 0, st, c, sums);
+            hipLaunchKernelGGL(k_bias_sum, dim3((c.width + BLOCK - 1) / BLOCK), block, 0, st, c.width, sums, a->d_bias, (int)(n > 0));
+        }
     }
     hipLaunchKernelGGL(k_loss, dim3(1), dim3(BLOCK), 0, st, c);
     const int rc = launched();
