@@ -540,10 +540,11 @@ int swarp_grad_norm(const swarp_tensor_t *tensors, int32_t n_tensors, double max
  * Row r of `hidden` lies at (r / inner) outer_stride + (r % inner) inner_stride (in elements).  A
  * masked row is not read; its logp is 0, its gradient zero.  A row that counts with a target outside
  * [0, width), with NaN or +inf among its logits, or with all of them -inf, makes the loss NaN.
- * Where d_hidden, d_weight or d_bias is set the call also leaves the gradients of the summed loss
- * there, in float, d_hidden with the rows that count moved together; swarp_linear_ce_bwd turns them
- * into the caller's.  The work memory holds the exponentials of at most 1 GiB of rows (or of 256
- * rows) at a time, and copies of hidden and weight; the backward does not need it. */
+ * Where d_hidden, d_weight or d_bias is set the call also leaves the gradients there, for an upstream
+ * gradient of 1.  A head whose weight a workgroup's LDS holds (swarp_linear_ce_complete) is done in
+ * one kernel, and they are complete, of `dtype`.  Else they are float, d_hidden with the rows that
+ * count moved together; the work memory then holds the exponentials of at most 1 GiB of rows (or of
+ * 256 rows) at a time, copies of hidden and, where its rows are not whole steps of 64 bytes, weight. */
 typedef struct swarp_linear_ce {
     int32_t dtype;            /* of hidden, weight, bias: SWARP_F32, _BF16 or _F16 */
     int32_t sum;              /* 1: loss is the sum, 0: the mean */
@@ -556,8 +557,8 @@ typedef struct swarp_linear_ce {
     const void *bias;         /* [width] or NULL */
     const void *targets;      /* [rows] */
     const uint8_t *mask;      /* [rows], nonzero = counts; NULL: all count */
-    int32_t *place;           /* [rows + 1], with a mask: where each row's gradient lies (-1: none),
-                                 and how many count */
+    int32_t *place;           /* [rows + 1], with a mask and a gradient that is not complete: where
+                                 each row's lies (-1: none), and how many count */
     float *logp;              /* [rows] */
     float *loss;              /* [1] */
     float *d_hidden;          /* [rows, dim], [width, dim], [width], or NULL */
@@ -565,12 +566,16 @@ typedef struct swarp_linear_ce {
     void *work;               /* swarp_linear_ce_work_bytes() bytes, 256-byte aligned */
     uint64_t work_bytes;
 } swarp_linear_ce_t;
+int32_t swarp_linear_ce_complete(const swarp_linear_ce_t *a); /* 1 or 0, by dtype, dim and width */
 uint64_t swarp_linear_ce_work_bytes(const swarp_linear_ce_t *a);
 int swarp_linear_ce(const swarp_linear_ce_t *a, void *stream);
-/* d_hidden [rows, dim], d_weight and d_bias of `dtype` (NULL: not wanted) for the upstream gradient
- * *scale (float, on the device), from what a call with the same arguments left: rounded once. */
-int swarp_linear_ce_bwd(const swarp_linear_ce_t *a, const void *scale, void *d_hidden, void *d_weight,
-                        void *d_bias, void *stream);
+/* The gradients of `dtype` (NULL: not wanted) for the upstream gradient *scale (float, on the device),
+ * rounded once.  Of a complete head they are computed again, with `work`; with skip_unit = 1 the
+ * buffers hold what the call left, and only where *scale is not 1.  Else they come from the d_hidden,
+ * d_weight and d_bias that the call left; float ones may be those themselves (d_hidden without a
+ * mask). */
+int swarp_linear_ce_bwd(const swarp_linear_ce_t *a, int32_t skip_unit, const void *scale, void *d_hidden,
+                        void *d_weight, void *d_bias, void *stream);
 
 /* Linear attention with a decay for each head, along a rollout.  Per batch entry and head, with
  * the state S [dk, dv] and a step's q, k [dk], v [dv]:

@@ -331,9 +331,10 @@ SIGNATURES = {
     ),
     "swarp_linear_ce_work_bytes": ([ctypes.POINTER(SwarpLinearCe)], ctypes.c_uint64),
     "swarp_linear_ce": ([ctypes.POINTER(SwarpLinearCe), ctypes.c_void_p], ctypes.c_int),
+    "swarp_linear_ce_complete": ([ctypes.POINTER(SwarpLinearCe)], ctypes.c_int32),
     "swarp_linear_ce_bwd": (
-        [ctypes.POINTER(SwarpLinearCe), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
-         ctypes.c_void_p, ctypes.c_void_p],
+        [ctypes.POINTER(SwarpLinearCe), ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p,
+         ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p],
         ctypes.c_int,
     ),
     "swarp_decay_work_bytes": ([ctypes.POINTER(SwarpDecay)], ctypes.c_uint64),

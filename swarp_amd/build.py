@@ -3,7 +3,7 @@
 ``python -m swarp_amd.build`` (or ``__graft_entry__.build()``) compiles the units under
 ``swarp_amd/csrc`` -- the host side ``swarp_hip.hip``, the radius graph, the policy update
 (``gae.hip``, ``policy.hip``, ``adamw.hip``, ``linear_ce.hip``,
-``decay.hip``) and one object per kernel family and scalar
+``narrow_ce.hip``, ``decay.hip``) and one object per kernel family and scalar
 type (``k_*.hip`` with ``SWARP_T`` = float / double) -- in parallel, then links them into ``swarp_amd/libswarp_hip.so``.  ``--incremental`` recompiles only the objects
 whose sources, headers (from the compiler's dependency files) or flags changed.
 
@@ -47,6 +47,7 @@ def units() -> list[tuple[str, Path, list[str]]]:
            ("policy", CSRC / "policy.hip", []),
            ("adamw", CSRC / "adamw.hip", []),
            ("linear_ce", CSRC / "linear_ce.hip", []),
+           ("narrow_ce", CSRC / "narrow_ce.hip", []),
            ("decay", CSRC / "decay.hip", [])]
     for fam in FAMILIES:
         for tag, ctype, is32 in DTYPES:

@@ -22,6 +22,7 @@
 #include <math.h>
 
 #include "matrix.hpp"
+#include "narrow_ce.hpp"
 
 namespace {
 
@@ -36,7 +37,7 @@ constexpr float LOG2E = 1.44269504088896340736f;
 constexpr float LN_2 = 0.69314718055994530942f;
 constexpr float REACH = 40.0f;        // e^40 times 2^21 logits, times any weight, is far from overflow
 constexpr int F16_BITS = 14;          // float16 exponentials are kept times 2^14: 2^-38 is not lost
-constexpr int COUNT_ROWS = 4096;      // rows of the mask that one workgroup counts
+using narrow::COUNT_ROWS;
 constexpr uint64_t PIECE = 1ull << 30;  // bytes of exponentials at a time
 
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * LOG2E); }
@@ -59,7 +60,7 @@ struct Call {
     // of all rows
     void *h;
     float *z_t, *ref, *top;   // target's logit; what E is relative to; largest logit
-    float *inv, *inv_h;       // 1 / s; what h is multiplied by beside E^T
+    float *inv, *inv_h;       // weight / s; what h is multiplied by beside E^T
     double *sums;             // of logp, one for `few` rows
     int few;                  // rows of a workgroup that joins: 1 or 64
     // of the piece
@@ -75,6 +76,13 @@ __device__ __forceinline__ int rows_of(const Call &c)
 {
     const int64_t n = (c.n_on ? (int64_t)*c.n_on : c.rows) - c.first;
     return (int)(n < 0 ? 0 : n < c.piece ? n : c.piece);
+}
+
+// Weight of a row in the loss.
+__device__ __forceinline__ float weight_of(const Call &c)
+{
+    const int64_t n = c.n_on ? (int64_t)*c.n_on : c.rows;
+    return c.sum || n < 1 ? 1.0f : (float)(1.0 / (double)n);
 }
 
 // ------------------------------------------------------------------ which rows count
@@ -349,8 +357,9 @@ template <typename T, int ROWS> __global__ __launch_bounds__(BLOCK) void k_join(
     if (mine && how != SUMS) {
         // (a float16 h times 2^-14 would lose its digits: there the product is multiplied)
         const bool none = how == NORMED ? zt != zt : hi == -INFINITY;
-        c.inv[j] = none ? NAN : 1.0f / unit;
-        c.inv_h[j] = none ? NAN : how == NORMED ? 1.0f : 1.0f / unit;
+        const float f = weight_of(c) / unit;
+        c.inv[j] = none ? NAN : f;
+        c.inv_h[j] = none ? NAN : how == NORMED ? 1.0f : f;
         if (c.e) {
             const int64_t t = c.targets32 ? (int64_t)((const int32_t *)c.targets)[i] : ((const int64_t *)c.targets)[i];
             if (t >= 0 && t < c.width)
@@ -385,7 +394,8 @@ struct Product {
     int k;                     // how many there are
     int rows_m, rows_k;        // 1: m, or k, is the piece's rows instead
     int add;
-    float times;
+    float times;               // with `weigh` times the rows' weight
+    int weigh;
     const float *scale;        // of the rows of A, or NULL
     float *out;                // [m][n]
     float *parts;              // sums of splits
@@ -442,6 +452,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void k_product(const Call c, const P
     const int64_t M = p.rows_m ? rows : p.m;
     const int k = p.rows_k ? rows : p.k;
     const Share s = share_of<C>(M, p.n, (k + C::KE - 1) / C::KE, places);
+    const float times = p.weigh ? p.times * weight_of(c) : p.times;
     const int lane = threadIdx.x & 63, w = C::wave(), wm = w / C::WN, wn = w % C::WN;
     // (workgroups go round the eight dies one by one: each die, with its own L2, has neighbouring tiles)
     const int mine = places % 8 ? blockIdx.x : (blockIdx.x & 7) * (places / 8) + (blockIdx.x >> 3);
@@ -475,7 +486,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void k_product(const Call c, const P
                 for (int r = 0; r < 16; ++r) {
                     const int row = 32 * i + acc_row(r, 0);
                     if (m0 + i0 + row >= M) continue;
-                    const float f = p.scale ? p.times * p.scale[m0 + i0 + row] : p.times;
+                    const float f = p.scale ? times * p.scale[m0 + i0 + row] : times;
 #pragma unroll
                     for (int j = 0; j < C::TN; ++j)
                         if (n0 + j0 + 32 * j < p.n) {
@@ -502,6 +513,7 @@ template <typename C> __global__ __launch_bounds__(BLOCK) void k_splits(const Ca
     const int64_t M = p.rows_m ? rows : p.m;
     const Share s = share_of<C>(M, p.n, (k + ke - 1) / ke, places);
     if (s.splits == 1) return;
+    const float times = p.weigh ? p.times * weight_of(c) : p.times;
     constexpr int AREA = C::BM * C::BN;
     for (int64_t x = (int64_t)blockIdx.x * BLOCK + threadIdx.x; x < (int64_t)s.rest * AREA; x += (int64_t)gridDim.x * BLOCK) {
         const int at = (int)(x % AREA), i = (int)(x / AREA);
@@ -512,7 +524,7 @@ template <typename C> __global__ __launch_bounds__(BLOCK) void k_splits(const Ca
         float y = 0.0f;
         for (int w = 0; w < s.splits; ++w) y += p.parts[((int64_t)w * s.rest + i) * AREA + at];
         float *const out = p.out + m * p.n + n;
-        *out = y * (p.scale ? p.times * p.scale[m] : p.times) + (p.add ? *out : 0.0f);
+        *out = y * (p.scale ? times * p.scale[m] : times) + (p.add ? *out : 0.0f);
     }
 }
 
@@ -568,14 +580,14 @@ __global__ __launch_bounds__(BLOCK) void k_loss(const Call c)
     }
 }
 
-// The gradients as the caller has them: times the upstream gradient and the weight of a decision,
-// rounded once.  place: of the rows that count, or NULL.
+// The gradients as the caller has them: times the upstream gradient, rounded once; in place (floats) only
+// where that is not 1.  place: of the rows that count, or NULL.
 template <typename T>
 __global__ __launch_bounds__(BLOCK) void k_give(const float *from, T *to, int64_t n, int dim, const int32_t *place,
-                                                const int32_t *n_on, int64_t rows, int sum, const float *up1)
+                                                const float *up1)
 {
-    const double count = n_on ? (double)*n_on : (double)rows;
-    const float f = (float)((double)*up1 * (sum || count < 1 ? 1.0 : 1.0 / count));
+    const float f = *up1;
+    if ((const void *)from == (const void *)to && f == 1.0f) return;
     for (int64_t k = (int64_t)blockIdx.x * BLOCK + threadIdx.x; k < n; k += (int64_t)gridDim.x * BLOCK) {
         int64_t at = k;
         if (place) {
@@ -765,14 +777,15 @@ template <typename T> int run(const swarp_linear_ce_t *a, hipStream_t st)
         float *const parts = (float *)(mem + p.split);
         const int64_t pitch_e = c.wide * (int64_t)sizeof(T), pitch_h = c.dim_p * (int64_t)sizeof(T);
         if (a->d_hidden) {
-            const Product y = {c.e, c.w, pitch_e, pitch_h, p.piece, c.dim, c.width, 1, 0, 0, 1.0f, c.inv + first,
+            const Product y = {c.e, c.w, pitch_e, pitch_h, p.piece, c.dim, c.width, 1, 0, 0, 1.0f, 0, c.inv + first,
                                a->d_hidden + first * c.dim, parts};
             ok &= product<T, false>(c, y, st);
         }
         if (a->d_weight) {
             hipLaunchKernelGGL((k_scale<T>), dim3(blocks_of(p.piece / 4)), block, 0, st, c);
             const Product y = {c.e, c.hs, pitch_e, pitch_h, c.width, c.dim, 0, 0, 1, n > 0,
-                               a->dtype == SWARP_F16 ? 1.0f / (1 << F16_BITS) : 1.0f, nullptr, a->d_weight, parts};
+                               a->dtype == SWARP_F16 ? 1.0f / (1 << F16_BITS) : 1.0f, a->dtype == SWARP_F16, nullptr,
+                               a->d_weight, parts};
             ok &= product<T, true>(c, y, st);
         }
         if (a->d_bias)
@@ -800,39 +813,50 @@ int check(const swarp_linear_ce_t *a)
 
 template <typename T> void give(const swarp_linear_ce_t *a, const float *scale, void *h, void *w, void *b, hipStream_t st)
 {
-    const int32_t *const n_on = a->mask && a->rows ? a->place + a->rows : nullptr;
     const int64_t nh = a->rows * a->dim, nw = (int64_t)a->width * a->dim;
     if (h && nh)
         hipLaunchKernelGGL((k_give<T>), dim3(blocks_of(nh / BLOCK)), dim3(BLOCK), 0, st, (const float *)a->d_hidden, (T *)h,
-                           nh, a->dim, (const int32_t *)(a->mask ? a->place : nullptr), n_on, a->rows, a->sum, scale);
+                           nh, a->dim, (const int32_t *)(a->mask ? a->place : nullptr), scale);
     if (w)
         hipLaunchKernelGGL((k_give<T>), dim3(blocks_of(nw / BLOCK)), dim3(BLOCK), 0, st, (const float *)a->d_weight, (T *)w,
-                           nw, a->dim, (const int32_t *)nullptr, n_on, a->rows, a->sum, scale);
+                           nw, a->dim, (const int32_t *)nullptr, scale);
     if (b)
         hipLaunchKernelGGL((k_give<T>), dim3(blocks_of(a->width / BLOCK)), dim3(BLOCK), 0, st, (const float *)a->d_bias,
-                           (T *)b, (int64_t)a->width, 1, (const int32_t *)nullptr, n_on, a->rows, a->sum, scale);
+                           (T *)b, (int64_t)a->width, 1, (const int32_t *)nullptr, scale);
+}
+
+// Of a call without gradients, or of one with them.
+uint64_t work_of(const swarp_linear_ce_t *a) { return narrow::fits(a) ? narrow::work_bytes(a) : plan_of(a).bytes; }
+
+int ready(const swarp_linear_ce_t *a)
+{
+    if (!a->work || a->work_bytes < work_of(a)) return fail("work must be set, swarp_linear_ce_work_bytes() long");
+    if ((uintptr_t)a->work & 255u) return fail("work must be 256-byte aligned");
+    if (!a->weight || a->inner < 1 || (a->rows && (!a->hidden || !a->targets))) return fail("pointer arguments must be set");
+    return 0;
 }
 
 }  // namespace
 
 extern "C" {
 
+int32_t swarp_linear_ce_complete(const swarp_linear_ce_t *a) { return !check(a) && narrow::fits(a); }
+
 uint64_t swarp_linear_ce_work_bytes(const swarp_linear_ce_t *a)
 {
     if (check(a)) return 0;
-    return plan_of(a).bytes;
+    return work_of(a);
 }
 
 int swarp_linear_ce(const swarp_linear_ce_t *a, void *stream)
 {
     if (check(a)) return -1;
     if (!a->loss) return fail("loss must be set");
-    if (!a->work || a->work_bytes < plan_of(a).bytes) return fail("work must be set, swarp_linear_ce_work_bytes() long");
-    if ((uintptr_t)a->work & 255u) return fail("work must be 256-byte aligned");
-    if (!a->weight || a->inner < 1 || (a->rows && (!a->hidden || !a->targets || !a->logp)))
-        return fail("pointer arguments must be set");
-    if (a->rows && a->mask && !a->place) return fail("a mask needs place");
+    if (ready(a)) return -1;
+    if (a->rows && !a->logp) return fail("pointer arguments must be set");
     hipStream_t st = (hipStream_t)stream;
+    if (narrow::fits(a)) return narrow::run(a, 0, nullptr, a->d_hidden, a->d_weight, a->d_bias, st);
+    if (a->rows && a->mask && !a->place) return fail("a mask needs place");
     switch (a->dtype) {
     case SWARP_F32: return run<float>(a, st);
     case SWARP_BF16: return run<bf16>(a, st);
@@ -840,14 +864,21 @@ int swarp_linear_ce(const swarp_linear_ce_t *a, void *stream)
     }
 }
 
-int swarp_linear_ce_bwd(const swarp_linear_ce_t *a, const void *scale, void *d_hidden, void *d_weight, void *d_bias,
-                        void *stream)
+int swarp_linear_ce_bwd(const swarp_linear_ce_t *a, int32_t skip_unit, const void *scale, void *d_hidden, void *d_weight,
+                        void *d_bias, void *stream)
 {
     if (check(a)) return -1;
-    if (!scale || (d_hidden && !a->d_hidden) || (d_weight && !a->d_weight) || (d_bias && !a->d_bias))
+    if (!scale) return fail("pointer arguments must be set");
+    hipStream_t st = (hipStream_t)stream;
+    if (narrow::fits(a))
+        return ready(a) ? -1 : narrow::run(a, skip_unit, (const float *)scale, d_hidden, d_weight, d_bias, st);
+    if ((d_hidden && !a->d_hidden) || (d_weight && !a->d_weight) || (d_bias && !a->d_bias))
         return fail("pointer arguments must be set");
     if (a->rows && a->mask && !a->place) return fail("a mask needs place");
-    hipStream_t st = (hipStream_t)stream;
+    if (a->dtype != SWARP_F32 && ((d_hidden && d_hidden == a->d_hidden) || (d_weight && d_weight == a->d_weight) ||
+                                  (d_bias && d_bias == a->d_bias)))
+        return fail("only float gradients are scaled in place");
+    if (a->mask && d_hidden && d_hidden == a->d_hidden) return fail("the rows that count are moved, not in place");
     switch (a->dtype) {
     case SWARP_F32: give<float>(a, (const float *)scale, d_hidden, d_weight, d_bias, st); break;
     case SWARP_BF16: give<bf16>(a, (const float *)scale, d_hidden, d_weight, d_bias, st); break;
@@ -857,3 +888,12 @@ int swarp_linear_ce_bwd(const swarp_linear_ce_t *a, const void *scale, void *d_h
 }
 
 }  // extern "C"
+
+namespace narrow {
+
+void count(int64_t rows, const uint8_t *mask, int32_t *counts, hipStream_t st)
+{
+    hipLaunchKernelGGL(k_count, dim3((unsigned)counts_of(rows)), dim3(BLOCK), 0, st, rows, mask, counts);
+}
+
+}  // namespace narrow

@@ -20,6 +20,7 @@ from .policy import (_CODES, _differentiable_once, _guard, _no_tangents, _on_gpu
                      _row_strides, _same, _untraced)
 
 _MOST_DIM, _MOST_WIDTH = 65536, 1 << 21
+_TYPES = {code: dtype for dtype, code in _CODES.items()}
 
 
 class LinearCrossEntropy(NamedTuple):
@@ -29,36 +30,58 @@ class LinearCrossEntropy(NamedTuple):
     logp: torch.Tensor  # log-probability of each target (0 where masked), float32
 
 
-def _forward(a: _lib.SwarpLinearCe, hidden: torch.Tensor, lead, wants, stream: int):
-    """The call: (loss, logp), and what its backward reads."""
-    dev = hidden.device
+def _call(a: _lib.SwarpLinearCe, dev, lead, wants, complete: bool, stream: int):
+    """The call: (loss, logp), the gradients that it leaves, where their rows lie, its work memory."""
     f32 = dict(dtype=torch.float32, device=dev)
     loss, logp = torch.empty((), **f32), torch.empty(lead, **f32)
-    grads = [torch.empty(shape, **f32) if want else None for want, shape in
+    kind = _TYPES[a.dtype] if complete else torch.float32
+    grads = [torch.empty(shape, dtype=kind, device=dev) if want else None for want, shape in
              zip(wants, ((a.rows, a.dim), (a.width, a.dim), (a.width,)))]
-    place = torch.empty(a.rows + 1, dtype=torch.int32, device=dev) if a.mask else None
+    place = None
+    if a.mask and not complete:
+        place = torch.empty(a.rows + 1, dtype=torch.int32, device=dev)
     a.loss, a.logp, a.place = loss.data_ptr(), logp.data_ptr(), _ptr(place)
     a.d_hidden, a.d_weight, a.d_bias = (_ptr(g) for g in grads)
-    lib = _lib.load()
-    nbytes = lib.swarp_linear_ce_work_bytes(ctypes.byref(a))
+    work = _work(a, dev)
+    with _guard(dev):
+        _lib.check(_lib.load().swarp_linear_ce(ctypes.byref(a), stream))
+    return loss, logp, grads, place, work
+
+
+def _work(a: _lib.SwarpLinearCe, dev):
+    nbytes = _lib.load().swarp_linear_ce_work_bytes(ctypes.byref(a))
     work = torch.empty(nbytes + 255, dtype=torch.uint8, device=dev)
     a.work, a.work_bytes = (work.data_ptr() + 255) // 256 * 256, nbytes
-    with _guard(dev):
-        _lib.check(lib.swarp_linear_ce(ctypes.byref(a), stream))
-    return loss, logp, grads, place
+    return work
 
 
 class _LinearCeFn(torch.autograd.Function):
-    """The loss as one autograd node.  The forward leaves the gradients of the summed loss behind in
-    float32, while the exponentials are at hand; the backward multiplies them by the upstream
-    gradient and rounds them, once, to the type of what they belong to."""
+    """The loss as one autograd node.  The forward leaves gradients for an upstream gradient of 1
+    behind, while the exponentials are at hand.
+
+    16-bit ones of a wide head are kept in float32, and the backward multiplies them by the upstream
+    gradient and rounds them, once.  The others are handed out, once; where the upstream gradient is
+    not 1 (the device looks) those of a wide head are multiplied by it and those of a narrow one
+    computed again with it.  float16 ones of a narrow head are left to the backward: without the loss
+    scale that comes with it they would vanish.  A second backward computes them again."""
 
     @staticmethod
-    def forward(ctx, a: _lib.SwarpLinearCe, stream: int, hidden, weight, bias, lead):
+    def forward(ctx, a: _lib.SwarpLinearCe, stream: int, complete: bool, hidden, weight, bias,
+                targets, mask):
         ctx.set_materialize_grads(False)
-        loss, logp, grads, place = _forward(a, hidden, lead, ctx.needs_input_grad[2:5], stream)
-        ctx.a, ctx.shapes, ctx.dtype, ctx.stream = a, (hidden.shape, weight.shape), hidden.dtype, stream
-        ctx.save_for_backward(*grads, place)
+        ctx.need = ctx.needs_input_grad[3:6]
+        ctx.complete, ctx.like = complete, (hidden.shape, weight.shape, weight.shape[:1])
+        late = complete and hidden.dtype == torch.float16
+        loss, logp, grads, place, work = _call(a, hidden.device, targets.shape,
+                                               (False,) * 3 if late else ctx.need, complete, stream)
+        ctx.a, ctx.dtype = a, hidden.dtype
+        ctx.kept = not complete and hidden.dtype != torch.float32
+        if ctx.kept:
+            ctx.save_for_backward(*grads, place)
+        else:
+            ctx.made = None if late else (grads, place)
+            ctx.work = work if complete else None
+            ctx.save_for_backward(hidden, weight, bias, targets, mask)
         ctx.mark_non_differentiable(logp)
         return loss, logp
 
@@ -66,20 +89,51 @@ class _LinearCeFn(torch.autograd.Function):
     @_differentiable_once
     def backward(ctx, g, *_):
         if g is None:
-            return (None,) * 6
-        *grads, place = ctx.saved_tensors
+            return (None,) * 8
+        saved = ctx.saved_tensors  # (unchanged since, or this raises)
         dev, a = g.device, _lib.SwarpLinearCe.from_buffer_copy(ctx.a)
-        # (they may have been packed and lie elsewhere by now)
-        kept = [t if t is None else _same(t, "a saved tensor", t.shape, t.dtype, dev)
-                for t in (*grads, place)]
-        a.d_hidden, a.d_weight, a.d_bias, a.place = (_ptr(t) for t in kept)
-        shapes = (*ctx.shapes, ctx.shapes[1][:1])
-        out = [t if t is None else torch.empty(s, dtype=ctx.dtype, device=dev)
-               for t, s in zip(kept, shapes)]
-        g = _plain(g)
-        _lib.check(_lib.load().swarp_linear_ce_bwd(
-            ctypes.byref(a), g.data_ptr(), *(_ptr(t) for t in out), _lib.stream_of(dev)))
-        return None, None, *out, None
+        g, stream = _plain(g), _lib.stream_of(dev)
+        if ctx.kept:
+            # (they may have been packed and lie elsewhere by now)
+            *grads, place = (t if t is None else _plain(t) for t in saved)
+            out = [t if t is None else torch.empty(s, dtype=ctx.dtype, device=dev)
+                   for t, s in zip(grads, ctx.like)]
+            first = 0
+        else:
+            keep = _point(a, *saved)
+            made, ctx.made = ctx.made, None  # handed out once: the caller may change them
+            first = int(made is not None)
+            if made is not None:
+                grads, place = made
+            elif ctx.complete:
+                grads, place = [torch.empty(s, dtype=ctx.dtype, device=dev) if n else None
+                                for n, s in zip(ctx.need, ctx.like)], None
+            else:
+                _, _, grads, place, work = _call(a, dev, saved[3].shape, ctx.need, False, stream)
+            out = list(grads)
+            if place is not None and grads[0] is not None:
+                out[0] = torch.empty(ctx.like[0], dtype=ctx.dtype, device=dev)
+        a.d_hidden, a.d_weight, a.d_bias = (_ptr(t) for t in grads)
+        a.place = _ptr(place)
+        _lib.check(_lib.load().swarp_linear_ce_bwd(ctypes.byref(a), first, g.data_ptr(),
+                                                   *(_ptr(t) for t in out), stream))
+        out = [t if t is None else t.view(s) for t, s in zip(out, ctx.like)]
+        return None, None, None, *out, None, None
+
+
+def _point(a: _lib.SwarpLinearCe, hidden, weight, bias, targets, mask):
+    """The inputs into the arguments, wherever they lie; what has to stay until the launch."""
+    strides = None if hidden.is_neg() else _row_strides(hidden)
+    if strides is None:
+        hidden = _plain(hidden)
+        strides = _row_strides(hidden)
+    weight, targets = _plain(weight), _plain(targets)
+    bias = None if bias is None else _plain(bias)
+    mask = None if mask is None else mask.contiguous()
+    a.inner, a.outer_stride, a.inner_stride = strides
+    a.hidden, a.weight, a.bias = hidden.data_ptr(), weight.data_ptr(), _ptr(bias)
+    a.targets, a.mask = targets.data_ptr(), _ptr(mask)
+    return hidden, weight, bias, targets, mask
 
 
 def linear_cross_entropy(
@@ -139,17 +193,16 @@ def linear_cross_entropy(
         mask = _same(mask, "mask", lead, torch.bool, dev)
     if forward_ad._current_level >= 0:
         _no_tangents("linear_cross_entropy", hidden, weight, bias)
-    strides = None if hidden.is_neg() else _row_strides(hidden)
-    if strides is None:
-        hidden = _plain(hidden)
-        strides = _row_strides(hidden)
     a = _lib.SwarpLinearCe(
         dtype=_CODES[dtype], sum=reduction == "sum", targets32=targets.dtype == torch.int32,
-        dim=D, width=V, rows=targets.numel(), inner=strides[0], outer_stride=strides[1],
-        inner_stride=strides[2], hidden=hidden.data_ptr(), weight=weight.data_ptr(),
-        bias=_ptr(bias), targets=targets.data_ptr(), mask=_ptr(mask))
+        dim=D, width=V, rows=targets.numel())
+    keep = _point(a, hidden, weight, bias, targets, mask)
     stream = _lib.stream_of(dev)
+    complete = bool(_lib.load().swarp_linear_ce_complete(ctypes.byref(a)))
     if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad or (
             bias is not None and bias.requires_grad)):
-        return LinearCrossEntropy(*_LinearCeFn.apply(a, stream, hidden, weight, bias, lead))
-    return LinearCrossEntropy(*_forward(a, hidden, lead, (False,) * 3, stream)[:2])
+        return LinearCrossEntropy(*_LinearCeFn.apply(a, stream, complete, hidden, weight, bias,
+                                                     targets, mask))
+    loss, logp = _call(a, dev, lead, (False,) * 3, complete, stream)[:2]
+    del keep
+    return LinearCrossEntropy(loss, logp)

@@ -38,7 +38,7 @@ def test_linear_ce_refuses_before_any_launch():
     lib = _lib.load()
 
     def args(**kw):
-        base = dict(dtype=0, dim=8, width=10, rows=4, inner=4, inner_stride=8, hidden=256, weight=256,
+        base = dict(dtype=0, dim=8, width=100, rows=4, inner=4, inner_stride=8, hidden=256, weight=256,
                     targets=256, logp=256, loss=256)
         return _lib.SwarpLinearCe(**{**base, **kw})
 
@@ -62,8 +62,24 @@ def test_linear_ce_refuses_before_any_launch():
     a.work_bytes = lib.swarp_linear_ce_work_bytes(ctypes.byref(a))
     refused(call(a), "place")
     a = args(d_hidden=256)
-    refused(lib.swarp_linear_ce_bwd(ctypes.byref(a), None, 256, None, None, None), "pointer")
-    refused(lib.swarp_linear_ce_bwd(ctypes.byref(a), 256, None, 256, None, None), "pointer")
+
+    def back(a, *p):
+        return lib.swarp_linear_ce_bwd(ctypes.byref(a), 1, *p, None)
+    refused(back(a, None, 256, None, None), "pointer")
+    refused(back(a, 256, None, 256, None), "pointer")
+    refused(back(args(d_weight=256, dtype=2), 256, None, 256, None), "in place")
+    refused(back(args(d_hidden=256, mask=256, place=256), 256, 256, None, None), "in place")
+    refused(back(args(d_hidden=256, mask=256), 256, 512, None, None), "place")
+    # a head that fits a workgroup is complete, and its backward computes again
+    for dim, width, one in ((128, 32, 1), (129, 32, 0), (64, 64, 1), (65, 33, 0), (64, 65, 0)):
+        assert lib.swarp_linear_ce_complete(ctypes.byref(args(dim=dim, width=width))) == one
+    assert lib.swarp_linear_ce_complete(ctypes.byref(args(dtype=1, width=9))) == 0
+    a = args(width=9)
+    refused(call(a), "work")
+    refused(back(a, 256, 256, None, None), "work")
+    a.work, a.work_bytes = 256, lib.swarp_linear_ce_work_bytes(ctypes.byref(a))
+    a.weight = None
+    refused(back(a, 256, 256, None, None), "pointer")
     # gradients need room for the exponentials, a mask for its list
     grad = args(rows=5000, width=40000, d_weight=256)
     plain = args(rows=5000, width=40000)
