@@ -426,8 +426,76 @@ __global__ __launch_bounds__(BLOCK) void k_between(const Call c, int64_t n)
     }
 }
 
-// One step: a thread a column of v, all of dk in turn; the state is read and written once.
-template <typename T> __global__ __launch_bounds__(BLOCK) void k_step(const swarp_decay_t a, int64_t n)
+// One step: the state is read and written once, which is all that counts.  A wave a head; a lane has
+// four columns of every (64 / LANES)-th row, LANES of them a row.
+template <typename T, int LANES> __global__ __launch_bounds__(BLOCK) void k_step(const swarp_decay_t a, int64_t heads)
+{
+    constexpr int ROWS = 64 / LANES, AHEAD = 4;  // rows of a wave at once, and how many times that are under way
+    struct __attribute__((packed, aligned(4))) Four { float e[4]; };
+    const int lane = threadIdx.x & 63, i0 = lane / LANES, j = lane % LANES * 4;
+    const int dk = a.dk, dv = a.dv;
+    const bool mine = j < dv;
+    const int64_t step = (int64_t)gridDim.x * WAVES;
+    for (int64_t bh = (int64_t)blockIdx.x * WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); bh < heads; bh += step) {
+        const int64_t b = (uint32_t)bh / (uint32_t)a.heads;  // (at most 2^31 heads)
+        const int h = (int)(bh - b * a.heads);
+        const T *const q = (const T *)a.q + b * a.q_stride[1] + h * a.q_stride[2];
+        const T *const k = (const T *)a.k + b * a.k_stride[1] + h * a.k_stride[2];
+        const T *const v = (const T *)a.v + b * a.v_stride[1] + h * a.v_stride[2];
+        // (lane l brings elements l and l + 64 of q and k)
+        const int l0 = lane < dk ? lane : dk - 1, l1 = lane + 64 < dk ? lane + 64 : dk - 1;
+        const float q0 = (float)q[l0], q1 = (float)q[l1], k0 = (float)k[l0], k1 = (float)k[l1];
+        float vj[4], o[4] = {};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) vj[c] = mine && j + c < dv ? (float)v[j + c] : 0.0f;
+        const bool fresh = !a.state || (a.starts && a.starts[(uint32_t)b / (uint32_t)a.group]);
+        const float lambda = __builtin_amdgcn_exp2f(a.log_decay[h] * LOG2E);
+        const float *const from = a.state + bh * dk * dv + j;
+        float *const to = a.state_out + bh * dk * dv + j;
+#pragma unroll 1
+        for (int r0 = 0; r0 < dk; r0 += ROWS * AHEAD) {
+            Four s[AHEAD];
+#pragma unroll
+            for (int x = 0; x < AHEAD; ++x) {
+                const int i = r0 + x * ROWS + i0;
+                s[x] = {};
+                if (mine && i < dk && !fresh) s[x] = *(const Four *)(from + i * dv);
+            }
+#pragma unroll
+            for (int x = 0; x < AHEAD; ++x) {
+                const int i = r0 + x * ROWS + i0;
+                float ki = __shfl(k0, i & 63, 64), qi = __shfl(q0, i & 63, 64);
+                if (dk > 64) {  // (the same for all lanes)
+                    const float k2 = __shfl(k1, i & 63, 64), q2 = __shfl(q1, i & 63, 64);
+                    ki = i < 64 ? ki : k2;
+                    qi = i < 64 ? qi : q2;
+                }
+                if (mine && i < dk) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const float kv = ki * vj[c];
+                        s[x].e[c] = fresh ? kv : __builtin_fmaf(lambda, s[x].e[c], kv);
+                        o[c] = __builtin_fmaf(qi, s[x].e[c], o[c]);
+                    }
+                    *(Four *)(to + i * dv) = s[x];
+                }
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int d = LANES; d < 64; d <<= 1) o[c] += __shfl_xor(o[c], d, 64);
+        if (i0 == 0 && mine) {
+            T *const y = (T *)a.out + bh * dv + j;
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                if (j + c < dv) y[c] = (T)(o[c] * (float)a.scale);
+        }
+    }
+}
+
+// The same where dv is no multiple of four: a thread a column of v, all of dk in turn.
+template <typename T> __global__ __launch_bounds__(BLOCK) void k_step_any(const swarp_decay_t a, int64_t n)
 {
     for (int64_t x = (int64_t)blockIdx.x * BLOCK + threadIdx.x; x < n; x += (int64_t)gridDim.x * BLOCK) {
         const int64_t bh = x / a.dv, b = bh / a.heads;
@@ -591,6 +659,20 @@ Call call_of(const swarp_decay_t *a, bool back)
     return c;
 }
 
+template <typename T> void step(const swarp_decay_t *a, hipStream_t st)
+{
+    const int64_t heads = a->batch * a->heads, n = heads * a->dv;
+    auto blocks = [](int64_t n, int64_t each) { return dim3((unsigned)((n + each - 1) / each < 16384 ? (n + each - 1) / each : 16384)); };
+    const dim3 grid = blocks(heads, WAVES), block(BLOCK);
+    if (a->dv % 4) hipLaunchKernelGGL((k_step_any<T>), blocks(n, BLOCK), block, 0, st, *a, n);
+    else if (a->dv <= 4) hipLaunchKernelGGL((k_step<T, 1>), grid, block, 0, st, *a, heads);
+    else if (a->dv <= 8) hipLaunchKernelGGL((k_step<T, 2>), grid, block, 0, st, *a, heads);
+    else if (a->dv <= 16) hipLaunchKernelGGL((k_step<T, 4>), grid, block, 0, st, *a, heads);
+    else if (a->dv <= 32) hipLaunchKernelGGL((k_step<T, 8>), grid, block, 0, st, *a, heads);
+    else if (a->dv <= 64) hipLaunchKernelGGL((k_step<T, 16>), grid, block, 0, st, *a, heads);
+    else hipLaunchKernelGGL((k_step<T, 32>), grid, block, 0, st, *a, heads);
+}
+
 }  // namespace
 
 extern "C" {
@@ -697,12 +779,10 @@ int swarp_decay_step(const swarp_decay_t *a, void *stream)
     if (!a->log_decay || !a->q || !a->k || !a->v || !a->out || !a->state_out)
         return fail("pointer arguments must be set");
     hipStream_t st = (hipStream_t)stream;
-    const int64_t n = a->batch * a->heads * a->dv;
-    const dim3 grid((unsigned)((n + BLOCK - 1) / BLOCK < 16384 ? (n + BLOCK - 1) / BLOCK : 16384));
     switch (a->dtype) {
-    case SWARP_F32: hipLaunchKernelGGL((k_step<float>), grid, dim3(BLOCK), 0, st, *a, n); break;
-    case SWARP_BF16: hipLaunchKernelGGL((k_step<bf16>), grid, dim3(BLOCK), 0, st, *a, n); break;
-    default: hipLaunchKernelGGL((k_step<f16>), grid, dim3(BLOCK), 0, st, *a, n); break;
+    case SWARP_F32: step<float>(a, st); break;
+    case SWARP_BF16: step<bf16>(a, st); break;
+    default: step<f16>(a, st); break;
     }
     return launched();
 }
