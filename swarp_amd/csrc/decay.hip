@@ -51,7 +51,7 @@ struct Call {
     int scans, slices;     // slices of all scans
     int segments, chunks;  // of the steps, and chunks of a segment
     int64_t units;         // batch * heads * segments * slices: what one state goes through
-    int64_t each;          // batch entries that a wave takes, one after the other
+    int64_t spans;         // a wave takes every spans-th batch entry: those at work at once are neighbours
     int64_t steps, batch, group;
     int heads, area;       // area: dk dv of a state
     const float *log_decay;
@@ -62,7 +62,7 @@ struct Call {
 // What a wave does: the outputs of a segment, or (ENDS) the state that it ends with if none enters.
 enum { OUTPUTS, ENDS };
 
-// One wave: one head, 32 columns of v, the steps of a segment, for `each` batch entries in turn.  The
+// One wave: one head, 32 columns of v, the steps of a segment, for some batch entries in turn.  The
 // state's columns stay in its registers; KT: 32s of dk.  A wave works alone: its part of the LDS
 // holds the chunk's rows of k and v, to be read as columns.  The next chunk's rows (the next entry's
 // first ones) are on their way meanwhile.
@@ -78,9 +78,8 @@ __global__ __launch_bounds__(BLOCK, (KT + (WHAT == OUTPUTS)) * sizeof(T) < 10 ? 
     const int64_t number = (int64_t)blockIdx.x * WAVES + wave, span = number / kinds;
     const uint32_t kind = (uint32_t)(number - span * kinds), lines = kind / (uint32_t)c.slices;
     const int h = (int)(lines / (uint32_t)c.segments), segment = (int)(lines % (uint32_t)c.segments);
-    int64_t b = span * c.each;
-    const int64_t b_end = b + c.each < c.batch ? b + c.each : c.batch;
-    if (b >= b_end) return;
+    int64_t b = span;
+    if (b >= c.spans) return;
     int slice = (int)(kind % (uint32_t)c.slices), which = 0;
     const int whole_slice = slice;
     while (slice >= c.scan[which].slices) slice -= c.scan[which++].slices;
@@ -146,7 +145,7 @@ __global__ __launch_bounds__(BLOCK, (KT + (WHAT == OUTPUTS)) * sizeof(T) < 10 ? 
         }
     };
     if (begin < end) load(begin);
-    for (; b < b_end; ++b) {
+    for (; b < c.batch; b += c.spans) {
         const int64_t bh = b * c.heads + h;
         // the state: element (32 t + 16 (r / 8) + 8 half + r % 8, j) in register r of tile t
         f32x16 S[KT];
@@ -212,12 +211,12 @@ __global__ __launch_bounds__(BLOCK, (KT + (WHAT == OUTPUTS)) * sizeof(T) < 10 ? 
                 vp += CHUNK * vt;
                 if (sp) sp += CHUNK * way * groups;
             } else {
-                qp = qb += s.qs[1];
-                kp = kb += s.ks[1];
-                vp = vb += s.vs[1];
-                if (sp) sp = starts_of(b + 1);
+                qp = qb += c.spans * s.qs[1];
+                kp = kb += c.spans * s.ks[1];
+                vp = vb += c.spans * s.vs[1];
+                if (sp) sp = starts_of(b + c.spans);
             }
-            if (more || b + 1 < b_end) load(more ? c0 + CHUNK : begin);
+            if (more || b + c.spans < c.batch) load(more ? c0 + CHUNK : begin);
             Part<T> vf[2];
             vf[0] = column_of<T>(vx, VP, 0, 0, lane);
             vf[1] = column_of<T>(vx, VP, 16, 0, lane);
@@ -320,7 +319,7 @@ __global__ __launch_bounds__(BLOCK, (KT + (WHAT == OUTPUTS)) * sizeof(T) < 10 ? 
             }
             op += CHUNK * ot;
         }
-        ob += s.os[1];
+        ob += c.spans * s.os[1];
         float *to = WHAT == ENDS        ? s.between + ((int64_t)segment * c.batch * c.heads + bh) * c.area
                     : ends && s.state_out ? s.state_out + bh * c.area
                                           : nullptr;
@@ -543,7 +542,7 @@ void copy(int64_t (&to)[3], const int64_t *from)
 
 // How the steps are cut: into as many segments as give the chip WANTED waves, of four chunks at
 // least; the states between them cost a second reading of k and v.
-constexpr int WANTED = 6144, LEAST_CHUNKS = 4, MOST_SEGMENTS = 256;
+constexpr int WANTED = 4096, LEAST_CHUNKS = 4, MOST_SEGMENTS = 256;
 constexpr int64_t MOST_WAVES = 8192;  // of a launch, about: beyond it a wave takes several entries in turn
 
 struct Cuts {
@@ -552,7 +551,7 @@ struct Cuts {
 Cuts cuts_of(const swarp_decay_t *a, int slices)
 {
     const int64_t waves = a->batch * a->heads * slices, chunks = (a->steps + CHUNK - 1) / CHUNK;
-    int64_t n = waves > 0 ? (WANTED + waves - 1) / waves : 1;
+    int64_t n = waves > 0 ? WANTED / waves : 1;
     if (n > chunks / LEAST_CHUNKS) n = chunks / LEAST_CHUNKS;
     if (n > MOST_SEGMENTS) n = MOST_SEGMENTS;
     if (n < 2) return {1, (int)(chunks < 1 << 30 ? (chunks < 1 ? 1 : chunks) : 1 << 30)};
@@ -574,7 +573,7 @@ uint64_t work_of(const swarp_decay_t *a, bool back)
 
 template <typename T, int KT, int WHAT> void scan(const Call &c, int fit, hipStream_t st)
 {
-    const int64_t waves = (c.batch + c.each - 1) / c.each * c.heads * c.segments * c.slices, n = c.units / c.segments;
+    const int64_t waves = c.spans * c.heads * c.segments * c.slices, n = c.units / c.segments;
     const dim3 grid((unsigned)((waves + WAVES - 1) / WAVES));
     if (fit == FULL) hipLaunchKernelGGL((k_scan<T, KT, WHAT, FULL>), grid, dim3(BLOCK), 0, st, c);
     else if (fit == EIGHTS) hipLaunchKernelGGL((k_scan<T, KT, WHAT, EIGHTS>), grid, dim3(BLOCK), 0, st, c);
@@ -597,8 +596,8 @@ template <typename T, int WHAT> void scan(Call &c, hipStream_t st)
         if (c.scan[i].dk % 8 || c.scan[i].dv % 8) fit = ANY;
     }
     c.units = c.batch * c.heads * c.segments * c.slices;
-    c.each = c.units / MOST_WAVES;
-    if (c.each < 1) c.each = 1;
+    const int64_t kinds = (int64_t)c.heads * c.segments * c.slices, spans = MOST_WAVES / kinds;
+    c.spans = spans < 1 ? 1 : spans < c.batch ? spans : c.batch;
     if (kt == 1) scan<T, 1, WHAT>(c, fit, st);
     else if (kt == 2) scan<T, 2, WHAT>(c, fit, st);
     else if (kt == 3) scan<T, 3, WHAT>(c, fit, st);
