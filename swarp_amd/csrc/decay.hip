@@ -37,21 +37,22 @@ struct Scan {
     int64_t qs[3], ks[3], vs[3], os[3];  // elements: step, batch, head
     int dk, dv;                          // of this scan
     int back;                            // from the last step to the first
-    int slices;                          // of 32 columns of v
+    int slices, first;                   // of 32 columns of v; where they lie among those of all scans
+    int64_t spans;                       // k_together: a workgroup takes every spans-th four heads
     float score, grow, carry;            // factors of the scores, of k v^T in the state, of q S in the output
     const float *state;                  // before the first step, or NULL; element (i, j) at i si + j sj of a head's
     float *state_out;                    // after the last, or NULL
     int si, sj;
-    float *between;                      // [segments][batch heads][area]: states that segments end (k_scan<ENDS>)
+    float *between;                      // [segments][batch heads][area]: states that segments end with (ENDS)
     int32_t *cut;                        // or start with (k_between); [segments][batch heads]: no state gets through
 };
 
 struct Call {
     Scan scan[3];
     int scans, slices;     // slices of all scans
+    int64_t spans;         // k_alone: a wave takes every spans-th batch entry: those at work at once are neighbours
     int segments, chunks;  // of the steps, and chunks of a segment
     int64_t units;         // batch * heads * segments * slices: what one state goes through
-    int64_t spans;         // a wave takes every spans-th batch entry: those at work at once are neighbours
     int64_t steps, batch, group;
     int heads, area;       // area: dk dv of a state
     const float *log_decay;
@@ -62,12 +63,208 @@ struct Call {
 // What a wave does: the outputs of a segment, or (ENDS) the state that it ends with if none enters.
 enum { OUTPUTS, ENDS };
 
+// What a wave keeps of a head from chunk to chunk: the state's columns -- element
+// (32 t + 16 (r / 8) + 8 half + r % 8, j) in register r of tile t --, whether it is still zero, and a number
+// that is 0 as long as all that was multiplied is finite: a product with 0 is not 0 where it is not, and
+// the head is done again by k_exact.
+template <int KT> struct Kept {
+    f32x16 S[KT];
+    bool none;
+    float odd;
+};
+// Powers of a head's decay: between the steps of a lane's scores, from the state to a lane's step, from a
+// step to the leaving state, and over the chunk.
+struct Powers {
+    float D[16], w0, u[16], whole;
+    int width;  // of the chunk that u and whole are for
+
+    __device__ __forceinline__ void set(const Scan &s, float a2, int col, int half)
+    {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int i = 16 * (r >> 3) + 8 * half + (r & 7);
+            D[r] = col >= i ? s.score * __builtin_amdgcn_exp2f(a2 * (float)(col - i)) : 0.0f;
+        }
+        w0 = s.carry * __builtin_amdgcn_exp2f(a2 * (float)(col + (s.back ? 0 : 1)));
+        width = 0;
+    }
+    __device__ __forceinline__ void over(const Scan &s, float a2, int half, int L)
+    {
+        if (L == width) return;
+        width = L;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int i = 16 * (r >> 3) + 8 * half + (r & 7);
+            u[r] = i < L ? s.grow * __builtin_amdgcn_exp2f(a2 * (float)(L - 1 - i + (s.back ? 1 : 0))) : 0.0f;
+        }
+        whole = __builtin_amdgcn_exp2f(a2 * (float)L);
+    }
+};
+__device__ __forceinline__ float decay_of(const Call &c, int h)
+{
+    const float a2 = c.log_decay[h] * LOG2E;
+    return a2 < -1e30f ? -1e30f : a2;  // (-inf times 0 steps is no decay)
+}
+
+// The state that enters a segment; and the one that leaves it, if it is wanted.
+template <int KT, int WHAT, int FIT>
+__device__ __forceinline__ void enter(const Call &c, const Scan &s, int64_t bh, int segment, bool at_work, int half, int j, Kept<KT> &w)
+{
+    const float *from = WHAT == ENDS || !at_work ? nullptr
+                        : segment                ? s.between + ((int64_t)segment * c.batch * c.heads + bh) * c.area
+                        : s.state                ? s.state + bh * c.area
+                                                 : nullptr;
+    int rest = s.dk - 8 * half;  // (worked out at the place, not kept in registers throughout)
+    asm volatile("" : "+v"(rest));
+    if (from) from += (int64_t)(8 * half) * s.si + (int64_t)j * s.sj;
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int i = 32 * t + 16 * (r >> 3) + (r & 7);
+            w.S[t][r] = from && (FIT == FULL || (i < rest && j < s.dv)) ? from[i * s.si] : 0.0f;
+        }
+    w.none = !from;
+    w.odd = 0.0f;
+    if (from) {
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) w.odd = __builtin_fmaf(w.S[t][r], 0.0f, w.odd);
+    }
+}
+template <int KT, int WHAT, int FIT>
+__device__ __forceinline__ void leave(const Call &c, const Scan &s, int64_t bh, int segment, bool ends, int lane, int j, int slice,
+                                      const Kept<KT> &w, bool any)
+{
+    const int half = lane >> 5;
+    float *to = WHAT == ENDS        ? s.between + ((int64_t)segment * c.batch * c.heads + bh) * c.area
+                : ends && s.state_out ? s.state_out + bh * c.area
+                                      : nullptr;
+    if (to) {
+        int rest = s.dk - 8 * half;
+        asm volatile("" : "+v"(rest));
+        to += (int64_t)(8 * half) * s.si + (int64_t)j * s.sj;
+        // (backwards: what an episode that starts with the first step leaves of the state before it)
+        const bool clear = WHAT == OUTPUTS && s.back && c.starts && c.steps > 0 &&
+                           c.starts[(uint32_t)bh / (uint32_t)c.heads / (uint32_t)c.group];
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int i = 32 * t + 16 * (r >> 3) + (r & 7);
+                if (FIT == FULL || (i < rest && j < s.dv)) to[i * s.si] = clear ? 0.0f : w.S[t][r];
+            }
+    }
+    if (WHAT == OUTPUTS) {
+        const bool wrong = __ballot(!(w.odd == 0.0f)) != 0;
+        if (lane == 0) c.wrong[(bh * c.segments + segment) * c.slices + s.first + slice] = wrong;
+    } else if (lane == 0) s.cut[(int64_t)segment * c.batch * c.heads + bh] = any;
+}
+
+// A chunk of a head: from its scores p, q's parts and the rows of k and v in LDS, the outputs o of 32
+// columns from j0 on (lane: step; register: column, as the state's rows) and the state after it.
+template <typename T, int KT, int WHAT>
+__device__ __forceinline__ void chunk(Kept<KT> &w, const Powers &f, const Part<T> (&qf)[2 * KT], f32x16 p, const T *kx, int kp,
+                                      const T *vx, int vp, int j0, uint32_t cut, bool goes_on, int lane, f32x16 &o)
+{
+    const int half = lane >> 5, col = lane & 31;
+    f32x16(&S)[KT] = w.S;
+    bool &none = w.none;
+    float &odd = w.odd;
+    Part<T> vf[2];
+    vf[0] = column_of<T>(vx, vp, 0, j0, lane);
+    vf[1] = column_of<T>(vx, vp, 16, j0, lane);
+    odd = odd_of<T>(vf[1], odd_of<T>(vf[0], odd));
+    Part<T> pf[2], pl[2];
+    if (WHAT == OUTPUTS) {
+        const uint32_t upto = cut & (0xffffffffu >> (31 - col));
+        const int since = upto ? 31 - __clz(upto) : 0;  // first step that enters step `col`
+#pragma unroll
+        for (int r = 0; r < 16; ++r) p[r] *= f.D[r];
+        // (a score is not finite wherever its q or k is not)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            float y[8];
+#pragma unroll
+            for (int r = 0; r < 8; ++r) y[r] = p[8 * x + r];
+            if (cut) {
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                    odd = __builtin_fmaf(y[r], 0.0f, odd);
+                    y[r] = 16 * x + 8 * half + r >= since ? y[r] : 0.0f;
+                }
+            }
+            pf[x] = term_of<T>(y, true);
+            if (Part<T>::TERMS) pl[x] = term_of<T>(y, false);
+            odd = odd_of<T>(pf[x], odd);
+        }
+    }
+    if (WHAT == OUTPUTS) {
+        o = {};
+        if (!none) {
+#pragma unroll
+            for (int x = 0; x < 2 * KT; ++x) {
+                float y[8];
+#pragma unroll
+                for (int r = 0; r < 8; ++r) y[r] = S[x >> 1][8 * (x & 1) + r];
+                mma<T>(o, term_of<T>(y, true), qf[x]);
+                if (Part<T>::TERMS) mma<T>(o, term_of<T>(y, false), qf[x]);
+            }
+            const float g = cut & (0xffffffffu >> (31 - col)) ? 0.0f : f.w0;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[r] *= g;
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            mma<T>(o, vf[x], pf[x]);
+            if (Part<T>::TERMS) mma<T>(o, vf[x], pl[x]);
+        }
+    }
+    if (goes_on) {
+        const int kept = cut ? 31 - __clz(cut) : 0;  // first step that enters the leaving state
+        if (!none) {
+            const float g = cut ? 0.0f : f.whole;
+#pragma unroll
+            for (int t = 0; t < KT; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) S[t][r] *= g;
+        }
+        none = false;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            float y[8];
+#pragma unroll
+            for (int r = 0; r < 8; ++r) y[r] = element(vf[x], r) * f.u[8 * x + r];
+            if (cut) {
+#pragma unroll
+                for (int r = 0; r < 8; ++r) y[r] = 16 * x + 8 * half + r >= kept ? y[r] : 0.0f;
+            }
+            Part<T> z[3];
+            z[0] = term_of<T>(y, true);
+            if (Part<T>::TERMS) {
+                z[1] = term_of<T>(y, true);
+                z[2] = term_of<T>(y, false);
+            }
+#pragma unroll
+            for (int t = 0; t < KT; ++t) {
+                const Part<T> kc = column_of<T>(kx, kp, 16 * x, 32 * t, lane);
+                mma<T>(S[t], kc, z[0]);
+                if (Part<T>::TERMS) {
+                    mma<T>(S[t], kc, z[1]);
+                    mma<T>(S[t], kc, z[2]);
+                }
+            }
+        }
+    }
+}
+
 // One wave: one head, 32 columns of v, the steps of a segment, for some batch entries in turn.  The
 // state's columns stay in its registers; KT: 32s of dk.  A wave works alone: its part of the LDS
 // holds the chunk's rows of k and v, to be read as columns.  The next chunk's rows (the next entry's
 // first ones) are on their way meanwhile.
 template <typename T, int KT, int WHAT, int FIT>
-__global__ __launch_bounds__(BLOCK, (KT + (WHAT == OUTPUTS)) * sizeof(T) < 10 ? 2 : 1) void k_scan(const Call c)
+__global__ __launch_bounds__(BLOCK, (KT + (WHAT == OUTPUTS)) * sizeof(T) < 10 ? 2 : 1) void k_alone(const Call c)
 {
     constexpr int KP = 32 * KT + 16 / (int)sizeof(T), VP = 32 + 16 / (int)sizeof(T);
     __shared__ __align__(16) T room[WAVES][32 * (KP + VP)];
@@ -81,7 +278,6 @@ __global__ __launch_bounds__(BLOCK, (KT + (WHAT == OUTPUTS)) * sizeof(T) < 10 ? 
     int64_t b = span;
     if (b >= c.spans) return;
     int slice = (int)(kind % (uint32_t)c.slices), which = 0;
-    const int whole_slice = slice;
     while (slice >= c.scan[which].slices) slice -= c.scan[which++].slices;
     const Scan &s = c.scan[which];
     const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31, perm = swapped(col);
@@ -95,18 +291,9 @@ __global__ __launch_bounds__(BLOCK, (KT + (WHAT == OUTPUTS)) * sizeof(T) < 10 ? 
     const int64_t groups = c.batch / c.group;
     const bool ends = end == steps;  // the last segment
 
-    // powers: of the decay between the steps of a lane's scores, of what a step leaves in the state
-    float a2 = c.log_decay[h] * LOG2E;
-    a2 = a2 < -1e30f ? -1e30f : a2;  // (-inf times 0 steps is no decay)
-    float D[16], u[16];
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        const int i = 16 * (r >> 3) + 8 * half + (r & 7);
-        D[r] = col >= i ? s.score * __builtin_amdgcn_exp2f(a2 * (float)(col - i)) : 0.0f;
-    }
-    const float w0 = s.carry * __builtin_amdgcn_exp2f(a2 * (float)(col + (back ? 0 : 1)));
-    float whole = 0.0f;
-    int width = 0;  // of the chunk that u and whole are for
+    const float a2 = decay_of(c, h);
+    Powers f;
+    f.set(s, a2, col, half);
 
     // Rows as they lie in memory: q by lane, k by swapped lane, v by quarters of rows; and whether
     // anything enters a lane's step.  Where a row or a step is past the end the last one is read
@@ -147,47 +334,14 @@ __global__ __launch_bounds__(BLOCK, (KT + (WHAT == OUTPUTS)) * sizeof(T) < 10 ? 
     if (begin < end) load(begin);
     for (; b < c.batch; b += c.spans) {
         const int64_t bh = b * c.heads + h;
-        // the state: element (32 t + 16 (r / 8) + 8 half + r % 8, j) in register r of tile t
-        f32x16 S[KT];
-        const float *from = WHAT == ENDS ? nullptr
-                                  : segment    ? s.between + ((int64_t)segment * c.batch * c.heads + bh) * c.area
-                                  : s.state    ? s.state + bh * c.area
-                                               : nullptr;
-        int rest = dk - 8 * half;  // (worked out at the place, not kept in registers throughout)
-        asm volatile("" : "+v"(rest));
-        if (from) from += (int64_t)(8 * half) * s.si + (int64_t)j * s.sj;
-#pragma unroll
-        for (int t = 0; t < KT; ++t)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int i = 32 * t + 16 * (r >> 3) + (r & 7);
-                S[t][r] = from && (FIT == FULL || (i < rest && j < dv)) ? from[i * s.si] : 0.0f;
-            }
-        bool none = !from;  // the state is still zero
-        // 0 as long as all that is multiplied is finite: a product with 0 is not 0 where it is not, and the
-        // head is done again by k_exact
-        float odd = 0.0f;
-        if (from) {
-#pragma unroll
-            for (int t = 0; t < KT; ++t)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) odd = __builtin_fmaf(S[t][r], 0.0f, odd);
-        }
-
+        Kept<KT> w;
+        enter<KT, WHAT, FIT>(c, s, bh, segment, true, half, j, w);
         uint32_t any = 0;
         T *op = ob;
         for (int64_t c0 = begin; c0 < end; c0 += CHUNK) {
             const int L = (int)(end - c0 < CHUNK ? end - c0 : CHUNK);
             const bool more = c0 + CHUNK < end;
-            if (L != width) {
-                width = L;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int i = 16 * (r >> 3) + 8 * half + (r & 7);
-                    u[r] = i < L ? s.grow * __builtin_amdgcn_exp2f(a2 * (float)(L - 1 - i + (back ? 1 : 0))) : 0.0f;
-                }
-                whole = __builtin_amdgcn_exp2f(a2 * (float)L);
-            }
+            f.over(s, a2, half, L);
             // steps that nothing before them enters
             const uint32_t cut = (uint32_t)__ballot(sr);
             any |= cut;
@@ -217,130 +371,196 @@ __global__ __launch_bounds__(BLOCK, (KT + (WHAT == OUTPUTS)) * sizeof(T) < 10 ? 
                 if (sp) sp = starts_of(b + c.spans);
             }
             if (more || b + c.spans < c.batch) load(more ? c0 + CHUNK : begin);
-            Part<T> vf[2];
-            vf[0] = column_of<T>(vx, VP, 0, 0, lane);
-            vf[1] = column_of<T>(vx, VP, 16, 0, lane);
-            odd = odd_of<T>(vf[1], odd_of<T>(vf[0], odd));
-            Part<T> pf[2], pl[2];
-            if (WHAT == OUTPUTS) {
-                const uint32_t upto = cut & (0xffffffffu >> (31 - col));
-                const int since = upto ? 31 - __clz(upto) : 0;  // first step that enters step `col`
-#pragma unroll
-                for (int r = 0; r < 16; ++r) p[r] *= D[r];
-                // (a score is not finite wherever its q or k is not)
+            f32x16 o;
+            chunk<T, KT, WHAT>(w, f, qf, p, kx, KP, vx, VP, 0, cut, WHAT == ENDS || more || (ends && s.state_out), lane, o);
+            if (WHAT == OUTPUTS && col < L) {
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
-                    float y[8];
+                    const int n = dv - j0 - 8 * half - 16 * x;
+                    Span<T, 8> e;
 #pragma unroll
-                    for (int r = 0; r < 8; ++r) y[r] = p[8 * x + r];
-                    if (cut) {
+                    for (int r = 0; r < 8; ++r) e.e[r] = (T)o[8 * x + r];
+                    if (FIT == FULL || (FIT == EIGHTS ? n > 0 : n >= 8)) *(Span<T, 8> *)(op + 16 * x) = e;
+                    else if constexpr (FIT == ANY) {
 #pragma unroll
-                        for (int r = 0; r < 8; ++r) {
-                            odd = __builtin_fmaf(y[r], 0.0f, odd);
-                            y[r] = 16 * x + 8 * half + r >= since ? y[r] : 0.0f;
-                        }
-                    }
-                    pf[x] = term_of<T>(y, true);
-                    if (Part<T>::TERMS) pl[x] = term_of<T>(y, false);
-                    odd = odd_of<T>(pf[x], odd);
-                }
-            }
-            if (WHAT == OUTPUTS) {
-                f32x16 o = {};
-                if (!none) {
-#pragma unroll
-                    for (int x = 0; x < 2 * KT; ++x) {
-                        float y[8];
-#pragma unroll
-                        for (int r = 0; r < 8; ++r) y[r] = S[x >> 1][8 * (x & 1) + r];
-                        mma<T>(o, term_of<T>(y, true), qf[x]);
-                        if (Part<T>::TERMS) mma<T>(o, term_of<T>(y, false), qf[x]);
-                    }
-                    const float f = cut & (0xffffffffu >> (31 - col)) ? 0.0f : w0;
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) o[r] *= f;
-                }
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    mma<T>(o, vf[x], pf[x]);
-                    if (Part<T>::TERMS) mma<T>(o, vf[x], pl[x]);
-                }
-                if (col < L) {
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const int n = dv - j0 - 8 * half - 16 * x;
-                        Span<T, 8> e;
-#pragma unroll
-                        for (int r = 0; r < 8; ++r) e.e[r] = (T)o[8 * x + r];
-                        if (FIT == FULL || (FIT == EIGHTS ? n > 0 : n >= 8)) *(Span<T, 8> *)(op + 16 * x) = e;
-                        else if constexpr (FIT == ANY) {
-#pragma unroll
-                            for (int r = 0; r < 8; ++r)
-                                if (r < n) op[16 * x + r] = e.e[r];
-                        }
-                    }
-                }
-            }
-            if (WHAT == ENDS || more || (ends && s.state_out)) {
-                const int kept = cut ? 31 - __clz(cut) : 0;  // first step that enters the leaving state
-                if (!none) {
-                    const float f = cut ? 0.0f : whole;
-#pragma unroll
-                    for (int t = 0; t < KT; ++t)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) S[t][r] *= f;
-                }
-                none = false;
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    float y[8];
-#pragma unroll
-                    for (int r = 0; r < 8; ++r) y[r] = element(vf[x], r) * u[8 * x + r];
-                    if (cut) {
-#pragma unroll
-                        for (int r = 0; r < 8; ++r) y[r] = 16 * x + 8 * half + r >= kept ? y[r] : 0.0f;
-                    }
-                    Part<T> w[3];
-                    w[0] = term_of<T>(y, true);
-                    if (Part<T>::TERMS) {
-                        w[1] = term_of<T>(y, true);
-                        w[2] = term_of<T>(y, false);
-                    }
-#pragma unroll
-                    for (int t = 0; t < KT; ++t) {
-                        const Part<T> kc = column_of<T>(kx, KP, 16 * x, 32 * t, lane);
-                        mma<T>(S[t], kc, w[0]);
-                        if (Part<T>::TERMS) {
-                            mma<T>(S[t], kc, w[1]);
-                            mma<T>(S[t], kc, w[2]);
-                        }
+                        for (int r = 0; r < 8; ++r)
+                            if (r < n) op[16 * x + r] = e.e[r];
                     }
                 }
             }
             op += CHUNK * ot;
         }
         ob += c.spans * s.os[1];
-        float *to = WHAT == ENDS        ? s.between + ((int64_t)segment * c.batch * c.heads + bh) * c.area
-                    : ends && s.state_out ? s.state_out + bh * c.area
-                                          : nullptr;
-        if (to) {
-            to += (int64_t)(8 * half) * s.si + (int64_t)j * s.sj;
-            asm volatile("" : "+v"(rest));
-            // (backwards: what an episode that starts with the first step leaves of the state before it)
-            const bool clear = WHAT == OUTPUTS && back && c.starts && steps > 0 && c.starts[(uint32_t)b / group];
+        leave<KT, WHAT, FIT>(c, s, bh, segment, ends, lane, j, slice, w, any != 0);
+    }
+}
+
+// The same for heads up to 32 wide: a workgroup brings the rows of its four heads into LDS together.
+// Heads and batch entries next to each other lie next to each other in memory, so that a load takes
+// few rows of many bytes.  (A rollout's steps are far apart: 32
+// rows a load are 32 pages, and translations then cost more than the bytes.)  Its outputs leave the
+// same way.  The next chunk's rows, or the next heads' first ones, are on their way meanwhile.
+template <typename T, int WHAT, int FIT>
+__global__ __launch_bounds__(BLOCK, 2) void k_together(const Call c)
+{
+    constexpr int PAD = 16 / (int)sizeof(T), P = 32 + PAD, ROOM = WAVES * 32 * P;
+    constexpr int EACH = 2;  // pieces of q, k or v that a thread brings
+    __shared__ __align__(16) T room[(WHAT == OUTPUTS ? 4 : 2) * ROOM];
+    T *const kx = room, *const vx = kx + ROOM, *const qx = vx + ROOM, *const ox = qx + ROOM;
+    const uint32_t index = blockIdx.x / (uint32_t)c.scans;
+    const Scan &s = c.scan[blockIdx.x % (uint32_t)c.scans];
+    const int segment = (int)(index % (uint32_t)c.segments);
+    int64_t group = index / (uint32_t)c.segments;     // of four heads
+    if (group >= s.spans) return;
+    const int mine = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t lines = c.batch * c.heads, groups = (lines + WAVES - 1) / WAVES;
+    const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31, perm = swapped(col);
+    const bool back = s.back;
+    const int64_t steps = c.steps, origin = back ? steps - 1 : 0, way = back ? -1 : 1;
+    const int64_t begin = (int64_t)segment * c.chunks * CHUNK;
+    const int64_t end = begin + (int64_t)c.chunks * CHUNK < steps ? begin + (int64_t)c.chunks * CHUNK : steps;
+    const int dk = s.dk, dv = s.dv;
+    const bool ends = end == steps;  // the last segment
+    // (a workgroup's next heads are a whole number of batch entries on: a wave's h is always the same)
+    const uint32_t line0 = (uint32_t)(group * WAVES + mine);
+    const int h = (int)(line0 % (uint32_t)c.heads);
+    const int64_t far = s.spans * WAVES / c.heads;
+
+    const float a2 = decay_of(c, h);
+    Powers f;
+    f.set(s, a2, col, half);
+
+    // A thread's pieces, of eight elements, in the order row, head, place.  Where a step is past the end
+    // the last one is read again: q is zero past dk, and what else that brings meets a zero (of q, of
+    // D, of u) or is not written.
+    struct Piece {
+        int row, head, at;
+    };
+    auto piece = [](int n) {
+        const int x = n * BLOCK + (int)threadIdx.x;
+        return Piece{x >> 4, x >> 2 & 3, 8 * (x & 3)};
+    };
+    auto entry = [&](const int64_t (&st)[3], const Piece &y) {  // (elements to a piece's first step)
+        const uint32_t line = (uint32_t)(group * WAVES + y.head);
+        const uint32_t b = line / (uint32_t)c.heads;
+        return (int64_t)b * st[1] + (int64_t)(line - b * (uint32_t)c.heads) * st[2] + (origin + way * (begin + y.row)) * st[0];
+    };
+    const T *qb[EACH], *kb[EACH], *vb[EACH];
+    T *ob[EACH];
 #pragma unroll
-            for (int t = 0; t < KT; ++t)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int i = 32 * t + 16 * (r >> 3) + (r & 7);
-                    if (FIT == FULL || (i < rest && j < dv)) to[i * s.si] = clear ? 0.0f : S[t][r];
-                }
-        }
+    for (int n = 0; n < EACH; ++n) {
         if (WHAT == OUTPUTS) {
-            const bool wrong = __ballot(!(odd == 0.0f)) != 0;
-            if (lane == 0) c.wrong[(bh * c.segments + segment) * c.slices + whole_slice] = wrong;
+            qb[n] = (const T *)s.q + entry(s.qs, piece(n));
+            ob[n] = (T *)s.out + entry(s.os, piece(n)) + piece(n).at;
         }
-        if (WHAT == ENDS && lane == 0) s.cut[(int64_t)segment * c.batch * c.heads + bh] = any != 0;
+        kb[n] = (const T *)s.k + entry(s.ks, piece(n));
+        vb[n] = (const T *)s.v + entry(s.vs, piece(n));
+    }
+    Raw<T> qr[EACH], kr[EACH], vr[EACH];
+    uint8_t sr = 0;  // whether nothing before it enters a lane's step
+    auto load = [&](int64_t c0, int64_t group, int64_t skip) {
+        const int L = (int)(end - c0 < CHUNK ? end - c0 : CHUNK);
+        const int64_t t = way * (c0 - begin);
+#pragma unroll
+        for (int n = 0; n < EACH; ++n) {
+            const Piece y = piece(n);
+            const int64_t yt = t - way * (y.row < L ? 0 : y.row - (L - 1));
+            if (group * WAVES + y.head < lines) {
+                if (WHAT == OUTPUTS) qr[n] = row_of<T, FIT>(qb[n] + skip * s.qs[1] + yt * s.qs[0], y.at, dk, true);
+                kr[n] = row_of<T, FIT>(kb[n] + skip * s.ks[1] + yt * s.ks[0], y.at, dk, false);
+                vr[n] = row_of<T, FIT>(vb[n] + skip * s.vs[1] + yt * s.vs[0], y.at, dv, false);
+            }
+        }
+        if (c.starts) {
+            sr = 0;
+            const int64_t line = group * WAVES + mine, x = c0 + col;
+            if (col < L && (!back || x > 0) && line < lines)
+                sr = c.starts[(back ? steps - x : x) * (c.batch / c.group) + (uint32_t)((uint32_t)line / (uint32_t)c.heads) / (uint32_t)c.group];
+        }
+    };
+#pragma unroll
+    for (int n = 0; n < EACH; ++n) {
+        qr[n] = {};
+        kr[n] = {};
+        vr[n] = {};
+    }
+    if (begin < end) load(begin, group, 0);
+    for (; group < groups; group += s.spans) {
+        const int64_t bh = group * WAVES + mine;
+        const bool at_work = bh < lines;  // (the same for a wave)
+        Kept<1> w;
+        enter<1, WHAT, FIT>(c, s, bh, segment, at_work, half, perm, w);
+        uint32_t any = 0;
+        for (int64_t c0 = begin; c0 < end; c0 += CHUNK) {
+            const int L = (int)(end - c0 < CHUNK ? end - c0 : CHUNK);
+            const bool more = c0 + CHUNK < end;
+            f.over(s, a2, half, L);
+            // steps that nothing before them enters
+            const uint32_t cut = (uint32_t)__ballot(sr);
+            any |= cut;
+            // rows into LDS
+#pragma unroll
+            for (int n = 0; n < EACH; ++n) {
+                const Piece y = piece(n);
+                const int at = (y.head * 32 + y.row) * P + y.at;
+                if (WHAT == OUTPUTS) *(Raw<T> *)(qx + at) = qr[n];
+                *(Raw<T> *)(kx + at) = kr[n];
+                *(Raw<T> *)(vx + at) = vr[n];
+            }
+            __syncthreads();
+            if (more) load(c0 + CHUNK, group, 0);
+            else if (group + s.spans < groups) load(begin, group + s.spans, far);
+            if (at_work) {
+                const T *const kw = kx + mine * 32 * P, *const vw = vx + mine * 32 * P;
+                Part<T> qf[2];
+                f32x16 p = {}, o;
+                if (WHAT == OUTPUTS) {
+                    const T *const qw = qx + (mine * 32 + col) * P + 8 * half, *const kr = kw + perm * P + 8 * half;
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        qf[t] = part_of(*(const Raw<T> *)(qw + 16 * t));
+                        mma<T>(p, part_of(*(const Raw<T> *)(kr + 16 * t)), qf[t]);
+                    }
+                }
+                chunk<T, 1, WHAT>(w, f, qf, p, kw, P, vw, P, 0, cut, WHAT == ENDS || more || (ends && s.state_out), lane, o);
+                if (WHAT == OUTPUTS) {
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        Span<T, 8> e;
+#pragma unroll
+                        for (int r = 0; r < 8; ++r) e.e[r] = (T)o[8 * x + r];
+                        *(Raw<T> *)(ox + (mine * 32 + col) * P + 16 * x + 8 * half) = __builtin_bit_cast(Raw<T>, e);
+                    }
+                }
+            }
+            __syncthreads();
+            if (WHAT == OUTPUTS) {
+#pragma unroll
+                for (int n = 0; n < EACH; ++n) {
+                    const Piece z = piece(n);
+                    if (z.row >= L || group * WAVES + z.head >= lines) continue;
+                    const Span<T, 8> e = __builtin_bit_cast(Span<T, 8>, *(const Raw<T> *)(ox + (z.head * 32 + z.row) * P + z.at));
+                    T *const to = ob[n] + way * (c0 - begin) * s.os[0];
+                    const int left = dv - z.at;
+                    if (FIT == FULL || (FIT == EIGHTS ? left > 0 : left >= 8)) *(Span<T, 8> *)to = e;
+                    else if constexpr (FIT == ANY) {
+#pragma unroll
+                        for (int r = 0; r < 8; ++r)
+                            if (r < left) to[r] = e.e[r];
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < EACH; ++n) {
+            if (WHAT == OUTPUTS) {
+                qb[n] += far * s.qs[1];
+                ob[n] += far * s.os[1];
+            }
+            kb[n] += far * s.ks[1];
+            vb[n] += far * s.vs[1];
+        }
+        if (at_work) leave<1, WHAT, FIT>(c, s, bh, segment, ends, lane, perm, 0, w, any != 0);
     }
 }
 
@@ -543,7 +763,7 @@ void copy(int64_t (&to)[3], const int64_t *from)
 // How the steps are cut: into as many segments as give the chip WANTED waves, of four chunks at
 // least; the states between them cost a second reading of k and v.
 constexpr int WANTED = 4096, LEAST_CHUNKS = 4, MOST_SEGMENTS = 256;
-constexpr int64_t MOST_WAVES = 8192;  // of a launch, about: beyond it a wave takes several entries in turn
+constexpr int64_t MOST_WAVES = 8192;  // of a launch, about: beyond it one takes several heads in turn
 
 struct Cuts {
     int segments, chunks;
@@ -571,22 +791,49 @@ uint64_t work_of(const swarp_decay_t *a, bool back)
     return n.segments * heads * (scans * (4ull * a->dk * a->dv + 4) + slices) + 256;
 }
 
-template <typename T, int KT, int WHAT> void scan(const Call &c, int fit, hipStream_t st)
+template <typename T, int KT, int WHAT> void alone(Call &c, int fit, hipStream_t st)
 {
-    const int64_t waves = c.spans * c.heads * c.segments * c.slices, n = c.units / c.segments;
-    const dim3 grid((unsigned)((waves + WAVES - 1) / WAVES));
-    if (fit == FULL) hipLaunchKernelGGL((k_scan<T, KT, WHAT, FULL>), grid, dim3(BLOCK), 0, st, c);
-    else if (fit == EIGHTS) hipLaunchKernelGGL((k_scan<T, KT, WHAT, EIGHTS>), grid, dim3(BLOCK), 0, st, c);
-    else hipLaunchKernelGGL((k_scan<T, KT, WHAT, ANY>), grid, dim3(BLOCK), 0, st, c);
-    if (WHAT == OUTPUTS)
-        hipLaunchKernelGGL((k_exact<T, KT>), dim3((unsigned)((n + BLOCK - 1) / BLOCK)), dim3(BLOCK), 0, st, c, n);
+    const int64_t kinds = (int64_t)c.heads * c.segments * c.slices, spans = MOST_WAVES / kinds;
+    c.spans = spans < 1 ? 1 : spans < c.batch ? spans : c.batch;
+    const dim3 grid((unsigned)((c.spans * kinds + WAVES - 1) / WAVES));
+    if (fit == FULL) hipLaunchKernelGGL((k_alone<T, KT, WHAT, FULL>), grid, dim3(BLOCK), 0, st, c);
+    else if (fit == EIGHTS) hipLaunchKernelGGL((k_alone<T, KT, WHAT, EIGHTS>), grid, dim3(BLOCK), 0, st, c);
+    else hipLaunchKernelGGL((k_alone<T, KT, WHAT, ANY>), grid, dim3(BLOCK), 0, st, c);
 }
+
+template <typename T, int WHAT> void together(Call &c, int fit, hipStream_t st)
+{
+    const int64_t lines = c.batch * c.heads, groups = (lines + WAVES - 1) / WAVES;
+    // (four times the spans must be a multiple of the call's heads, as far as there is more than one)
+    const int64_t whole = c.heads % 4 == 0 ? c.heads / 4 : c.heads % 2 == 0 ? c.heads / 2 : c.heads;
+    const int64_t want = MOST_WAVES / WAVES / (c.segments * c.scans), spans = want < whole ? whole : want / whole * whole;
+    for (int i = 0; i < c.scans; ++i) c.scan[i].spans = spans < groups ? spans : groups;
+    const dim3 grid((unsigned)(c.scan[0].spans * c.segments * c.scans));
+    if (fit == FULL) hipLaunchKernelGGL((k_together<T, WHAT, FULL>), grid, dim3(BLOCK), 0, st, c);
+    else if (fit == EIGHTS) hipLaunchKernelGGL((k_together<T, WHAT, EIGHTS>), grid, dim3(BLOCK), 0, st, c);
+    else hipLaunchKernelGGL((k_together<T, WHAT, ANY>), grid, dim3(BLOCK), 0, st, c);
+}
+
+template <typename T, int KT, int WHAT> void scan(Call &c, int fit, hipStream_t st)
+{
+    // Heads up to 32 wide go together: their rows are short (32 x 256000 x 2 heads of 32, forward and
+    // backward: 1.52 and 3.07 ms, alone 1.88 and 3.44); wider ones alone (4095 x 96 x 4 heads of 64: 0.28 and
+    // 0.88, together 0.29 and 1.11: barriers between waves that have much to do).
+    if (KT == 1 && c.slices == c.scans) together<T, WHAT>(c, fit, st);
+    else alone<T, KT, WHAT>(c, fit, st);
+    if (WHAT == OUTPUTS) {
+        const int64_t n = c.units / c.segments;
+        hipLaunchKernelGGL((k_exact<T, KT>), dim3((unsigned)((n + BLOCK - 1) / BLOCK)), dim3(BLOCK), 0, st, c, n);
+    }
+}
+
 template <typename T, int WHAT> void scan(Call &c, hipStream_t st)
 {
     int kt = 0;
     c.slices = 0;
     for (int i = 0; i < c.scans; ++i) {
         c.scan[i].slices = (c.scan[i].dv + 31) / 32;
+        c.scan[i].first = c.slices;
         c.slices += c.scan[i].slices;
         if ((c.scan[i].dk + 31) / 32 > kt) kt = (c.scan[i].dk + 31) / 32;
     }
@@ -596,8 +843,6 @@ template <typename T, int WHAT> void scan(Call &c, hipStream_t st)
         if (c.scan[i].dk % 8 || c.scan[i].dv % 8) fit = ANY;
     }
     c.units = c.batch * c.heads * c.segments * c.slices;
-    const int64_t kinds = (int64_t)c.heads * c.segments * c.slices, spans = MOST_WAVES / kinds;
-    c.spans = spans < 1 ? 1 : spans < c.batch ? spans : c.batch;
     if (kt == 1) scan<T, 1, WHAT>(c, fit, st);
     else if (kt == 2) scan<T, 2, WHAT>(c, fit, st);
     else if (kt == 3) scan<T, 3, WHAT>(c, fit, st);
