@@ -30,29 +30,37 @@ class LinearCrossEntropy(NamedTuple):
     logp: torch.Tensor  # log-probability of each target (0 where masked), float32
 
 
-def _call(a: _lib.SwarpLinearCe, dev, lead, wants, complete: bool, stream: int):
-    """The call: (loss, logp), the gradients that it leaves, where their rows lie, its work memory."""
-    f32 = dict(dtype=torch.float32, device=dev)
-    loss, logp = torch.empty((), **f32), torch.empty(lead, **f32)
+def _call(a: _lib.SwarpLinearCe, dev, lead, shapes, complete: bool, stream: int):
+    """The call: (loss, logp), the gradients that it leaves (of these shapes, or None), where their rows
+    lie, its work memory."""
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    logp = torch.empty(lead, dtype=torch.float32, device=dev)
     kind = _TYPES[a.dtype] if complete else torch.float32
-    grads = [torch.empty(shape, dtype=kind, device=dev) if want else None for want, shape in
-             zip(wants, ((a.rows, a.dim), (a.width, a.dim), (a.width,)))]
+    grads = [s if s is None else torch.empty(s, dtype=kind, device=dev) for s in shapes]
     place = None
     if a.mask and not complete:
         place = torch.empty(a.rows + 1, dtype=torch.int32, device=dev)
-    a.loss, a.logp, a.place = loss.data_ptr(), logp.data_ptr(), _ptr(place)
-    a.d_hidden, a.d_weight, a.d_bias = (_ptr(g) for g in grads)
-    work = _work(a, dev)
+        a.place = place.data_ptr()
+    a.loss, a.logp = loss.data_ptr(), logp.data_ptr()
+    a.d_hidden, a.d_weight, a.d_bias = map(_ptr, grads)
+    lib = _lib.load()
+    nbytes = lib.swarp_linear_ce_work_bytes(ctypes.byref(a))
+    work = torch.empty(nbytes + 255, dtype=torch.uint8, device=dev)
+    a.work, a.work_bytes = (work.data_ptr() + 255) // 256 * 256, nbytes
     with _guard(dev):
-        _lib.check(_lib.load().swarp_linear_ce(ctypes.byref(a), stream))
+        _lib.check(lib.swarp_linear_ce(ctypes.byref(a), stream))
     return loss, logp, grads, place, work
 
 
-def _work(a: _lib.SwarpLinearCe, dev):
-    nbytes = _lib.load().swarp_linear_ce_work_bytes(ctypes.byref(a))
-    work = torch.empty(nbytes + 255, dtype=torch.uint8, device=dev)
-    a.work, a.work_bytes = (work.data_ptr() + 255) // 256 * 256, nbytes
-    return work
+def _unmoved(a: _lib.SwarpLinearCe, strides, hidden, weight, bias, targets, mask) -> bool:
+    """Whether saved tensors lie where and as the forward read them (written out: this is on the path
+    of every training step)."""
+    return (hidden.data_ptr() == a.hidden and hidden.stride() == strides and not hidden.is_neg()
+            and weight.data_ptr() == a.weight and weight.is_contiguous() and not weight.is_neg()
+            and targets.data_ptr() == a.targets and targets.is_contiguous()
+            and (bias is None or bias.data_ptr() == a.bias and bias.is_contiguous()
+                 and not bias.is_neg())
+            and (mask is None or mask.data_ptr() == a.mask and mask.is_contiguous()))
 
 
 class _LinearCeFn(torch.autograd.Function):
@@ -69,12 +77,13 @@ class _LinearCeFn(torch.autograd.Function):
     def forward(ctx, a: _lib.SwarpLinearCe, stream: int, complete: bool, hidden, weight, bias,
                 targets, mask):
         ctx.set_materialize_grads(False)
-        ctx.need = ctx.needs_input_grad[3:6]
-        ctx.complete, ctx.like = complete, (hidden.shape, weight.shape, weight.shape[:1])
+        need = ctx.needs_input_grad
+        ctx.shapes = tuple(t.shape if n else None for t, n in zip((hidden, weight, bias), need[3:6]))
         late = complete and hidden.dtype == torch.float16
         loss, logp, grads, place, work = _call(a, hidden.device, targets.shape,
-                                               (False,) * 3 if late else ctx.need, complete, stream)
-        ctx.a, ctx.dtype = a, hidden.dtype
+                                               (None,) * 3 if late else ctx.shapes, complete, stream)
+        ctx.a, ctx.stream, ctx.complete = a, stream, complete
+        ctx.like = hidden.stride(), hidden.dtype
         ctx.kept = not complete and hidden.dtype != torch.float32
         if ctx.kept:
             ctx.save_for_backward(*grads, place)
@@ -91,33 +100,38 @@ class _LinearCeFn(torch.autograd.Function):
         if g is None:
             return (None,) * 8
         saved = ctx.saved_tensors  # (unchanged since, or this raises)
-        dev, a = g.device, _lib.SwarpLinearCe.from_buffer_copy(ctx.a)
-        g, stream = _plain(g), _lib.stream_of(dev)
+        a, first, keep = ctx.a, 0, None
+        if g.is_neg():
+            g = g.resolve_neg()
+        # (autograd runs this with the forward's device and stream current)
         if ctx.kept:
             # (they may have been packed and lie elsewhere by now)
-            *grads, place = (t if t is None else _plain(t) for t in saved)
-            out = [t if t is None else torch.empty(s, dtype=ctx.dtype, device=dev)
-                   for t, s in zip(grads, ctx.like)]
-            first = 0
+            *out, place = saved = [t if t is None else _plain(t) for t in saved]
+            a = _lib.SwarpLinearCe.from_buffer_copy(a)
+            a.d_hidden, a.d_weight, a.d_bias, a.place = map(_ptr, saved)
+            out = [t if t is None else torch.empty(t.shape, dtype=ctx.like[1], device=g.device)
+                   for t in out]
         else:
-            keep = _point(a, *saved)
             made, ctx.made = ctx.made, None  # handed out once: the caller may change them
-            first = int(made is not None)
+            if not _unmoved(a, ctx.like[0], *saved):
+                a = _lib.SwarpLinearCe.from_buffer_copy(a)
+                keep = _point(a, *saved)
             if made is not None:
-                grads, place = made
+                first, (out, place) = 1, made
             elif ctx.complete:
-                grads, place = [torch.empty(s, dtype=ctx.dtype, device=dev) if n else None
-                                for n, s in zip(ctx.need, ctx.like)], None
+                place = None
+                out = [s if s is None else torch.empty(s, dtype=ctx.like[1], device=g.device)
+                       for s in ctx.shapes]
             else:
-                _, _, grads, place, work = _call(a, dev, saved[3].shape, ctx.need, False, stream)
-            out = list(grads)
-            if place is not None and grads[0] is not None:
-                out[0] = torch.empty(ctx.like[0], dtype=ctx.dtype, device=dev)
-        a.d_hidden, a.d_weight, a.d_bias = (_ptr(t) for t in grads)
-        a.place = _ptr(place)
+                a = _lib.SwarpLinearCe.from_buffer_copy(a)
+                out, place, work = _call(a, g.device, saved[3].shape, ctx.shapes, False,
+                                         ctx.stream)[2:]
+                keep = keep, work
+            if place is not None and out[0] is not None:  # (its rows lie together)
+                out = [torch.empty(ctx.shapes[0], dtype=ctx.like[1], device=g.device), *out[1:]]
         _lib.check(_lib.load().swarp_linear_ce_bwd(ctypes.byref(a), first, g.data_ptr(),
-                                                   *(_ptr(t) for t in out), stream))
-        out = [t if t is None else t.view(s) for t, s in zip(out, ctx.like)]
+                                                   *map(_ptr, out), ctx.stream))
+        del keep
         return None, None, None, *out, None, None
 
 
@@ -203,6 +217,6 @@ def linear_cross_entropy(
             bias is not None and bias.requires_grad)):
         return LinearCrossEntropy(*_LinearCeFn.apply(a, stream, complete, hidden, weight, bias,
                                                      targets, mask))
-    loss, logp = _call(a, dev, lead, (False,) * 3, complete, stream)[:2]
+    loss, logp = _call(a, dev, lead, (None,) * 3, complete, stream)[:2]
     del keep
     return LinearCrossEntropy(loss, logp)
