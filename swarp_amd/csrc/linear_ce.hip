@@ -48,7 +48,8 @@ struct Call {
     int64_t rows;             // of the call; at most as many count
     int64_t inner, outer_stride, inner_stride;
     int dim, width;
-    int dim_p;                // elements of a padded row of h and W
+    int dim_p;                // elements of a padded row of h
+    int pitch_w;              // bytes of a row of W
     int64_t wide;             // elements of a row of E
     int64_t first;            // row that the piece starts with
     int piece;                // rows that it has room for
@@ -213,14 +214,14 @@ __global__ __launch_bounds__(C::THREADS) void k_logits(const Call c, int nm, int
     C t;
     t.clear();
     const int64_t pitch = (int64_t)c.dim_p * sizeof(T);
-    const Operand a = {(const char *)c.w + v0 * pitch, pitch, c.width - v0, 0};
-    const Operand b = {(const char *)c.h + (c.first + r0) * pitch, pitch, rows - r0, 0};
+    const Operand a = {(const char *)c.w + v0 * (int64_t)c.pitch_w, c.pitch_w, c.width - v0, c.pitch_w};
+    const Operand b = {(const char *)c.h + (c.first + r0) * pitch, pitch, rows - r0, (int)pitch};
     t.run(lds, a, b, 0, c.dim_p / C::KE);
 
     const int lane = threadIdx.x & 63, w = C::wave(), wm = w / C::WN, wn = w % C::WN;
     float *const bias = (float *)lds;
     for (int k = threadIdx.x; k < C::BM; k += C::THREADS)
-        bias[k] = c.bias && v0 + k < c.width ? up(((const T *)c.bias)[v0 + k]) : 0.0f;
+        bias[k] = v0 + k >= c.width ? -INFINITY : c.bias ? up(((const T *)c.bias)[v0 + k]) : 0.0f;
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < C::TN; ++j) {
@@ -232,9 +233,9 @@ __global__ __launch_bounds__(C::THREADS) void k_logits(const Call c, int nm, int
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const int k = (wm * C::TM + i) * 32 + acc_row(r, lane);
-                const float z = v0 + k < c.width ? t.acc[i][j][r] + bias[k] : -INFINITY;
-                t.acc[i][j][r] = z;
-                m = z > m ? z : m;
+                // (past the last column: -inf; a NaN is passed over here and shows in the sum)
+                t.acc[i][j][r] += bias[k];
+                m = fmaxf(m, t.acc[i][j][r]);
             }
         const float ref = STORE ? c.ref[c.first + (mine ? row : 0)] : (m == -INFINITY ? 0.0f : m);
 #pragma unroll
@@ -270,13 +271,9 @@ __global__ __launch_bounds__(C::THREADS) void k_logits(const Call c, int nm, int
             for (int i = 0; i < C::TM; ++i)
 #pragma unroll
                 for (int r = 0; r < 16; r += 4) {
-                    // (columns past the last are 0, not exp(-inf - NaN))
                     struct __attribute__((aligned(4 * sizeof(T)))) Four { T e[4]; } y;
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const int k = i * 32 + acc_row(r + q, lane);
-                        y.e[q] = (T)(v + k < c.width ? t.acc[i][j][r + q] : 0.0f);
-                    }
+                    for (int q = 0; q < 4; ++q) y.e[q] = (T)t.acc[i][j][r + q];
                     *(Four *)(mine + acc_col(lane) * PITCH + i * 32 + acc_row(r, lane)) = y;
                 }
             __builtin_amdgcn_wave_barrier();
@@ -470,7 +467,7 @@ __global__ __launch_bounds__(C::THREADS, 2) void k_product(const Call c, const P
         C t;
         t.clear();
         const Operand a = {(const char *)p.a + (AK ? m0 * (int64_t)sizeof(T) : m0 * p.a_pitch), p.a_pitch,
-                           (int)(M - m0 < C::BM ? M - m0 : C::BM), k};
+                           (int)(M - m0 < C::BM ? M - m0 : C::BM), AK ? k : (int)p.a_pitch};
         const Operand b = {(const char *)p.b + n0 * (int64_t)sizeof(T), p.b_pitch, (int)(p.n - n0 < C::BN ? p.n - n0 : C::BN),
                            p.rows_k ? (k + 31) / 32 * 32 : k};  // (h beside E^T ends with zeros)
         t.template run<AK, true>(lds, a, b, first, last);
@@ -636,9 +633,9 @@ Plan plan_of(const swarp_linear_ce_t *a)
     int64_t piece = p.grad ? (int64_t)(PIECE / (uint64_t)(p.wide * p.size)) : (int64_t)(PIECE / 8 / (uint64_t)p.n_parts);
     piece = piece / 256 * 256;
     if (piece < 256) piece = 256;
-    if (piece > up_to(N, 256)) piece = up_to(N, 256);
+    if (piece >= N) piece = up_to(N, N < 256 ? 32 : 256);
     p.piece = piece;
-    p.pad_w = p.dim_p != D || ((uintptr_t)a->weight & 15);
+    p.pad_w = D * p.size % 16 || ((uintptr_t)a->weight & 15);
     uint64_t at = 0;
     auto room = [&](bool need, uint64_t bytes) {
         const uint64_t here = at;
@@ -714,6 +711,7 @@ template <typename T> int run(const swarp_linear_ce_t *a, hipStream_t st)
     c.dim = a->dim;
     c.width = a->width;
     c.dim_p = (int)p.dim_p;
+    c.pitch_w = (int)((p.pad_w ? p.dim_p : a->dim) * p.size);
     c.wide = p.wide;
     c.piece = (int)p.piece;
     c.targets32 = a->targets32;
@@ -777,7 +775,7 @@ template <typename T> int run(const swarp_linear_ce_t *a, hipStream_t st)
         float *const parts = (float *)(mem + p.split);
         const int64_t pitch_e = c.wide * (int64_t)sizeof(T), pitch_h = c.dim_p * (int64_t)sizeof(T);
         if (a->d_hidden) {
-            const Product y = {c.e, c.w, pitch_e, pitch_h, p.piece, c.dim, c.width, 1, 0, 0, 1.0f, 0, c.inv + first,
+            const Product y = {c.e, c.w, pitch_e, c.pitch_w, p.piece, c.dim, c.width, 1, 0, 0, 1.0f, 0, c.inv + first,
                                a->d_hidden + first * c.dim, parts};
             ok &= product<T, false>(c, y, st);
         }

@@ -54,13 +54,13 @@ __device__ __forceinline__ int acc_row(int r, int lane) { return (r & 3) + 8 * (
 __device__ __forceinline__ int acc_col(int lane) { return lane & 31; }
 
 // An operand of a tile: rows [0, rows) of `base`, `pitch` bytes apart (a multiple of 16, as `base`).
-// Rows past the last one read as the last one.  ALONG k: `base` has `steps` rows of k, those past the
-// last read as the last (the other operand is zero there), and `rows` elements in each, up to a
-// multiple of 16 bytes.
+// Rows past the last one read as the last one, and 16-byte pieces of a row past `k` bytes as the last
+// of it.  ALONG k: `base` has `k` steps, those past the last read as the last, and `rows` elements in
+// each, up to a multiple of 16 bytes.  (What is read twice meets zeros in the other operand.)
 struct Operand {
     const char *base;
     int64_t pitch;
-    int rows, steps;
+    int rows, k;
 };
 
 template <typename T, int TM_, int TN_, int WM_, int WN_> struct Tile {
@@ -103,14 +103,15 @@ template <typename T, int TM_, int TN_, int WM_, int WN_> struct Tile {
         return x & (W * (int)sizeof(T) / 32 - 1);
     }
 
-    // Where lane l of a load finds what belongs at place g of an operand's part of a stage; ALONG, steps
-    // of k past `most` read as that one.
+    // Where lane l of a load finds what belongs at place g of an operand's part of a stage; steps of k
+    // (pieces of it, where rows run along k) past `most` read as that one.
     template <int W, bool ALONG>
     static __device__ __forceinline__ uint32_t source(const Operand &o, int g, int lane, int most)
     {
         if constexpr (!ALONG) {
             const int r = g * 16 + (lane >> 2), row = r < o.rows ? r : o.rows - 1;
-            return (uint32_t)(row * o.pitch) + (((lane & 3) ^ mix_row(r)) << 4);
+            const int piece = (lane & 3) ^ mix_row(r);
+            return (uint32_t)(row * o.pitch) + ((piece < most ? piece : most) << 4);
         } else {
             constexpr int PIECES = W * sizeof(T) / 16;      // of a step
             const int at = g * 64 + lane, k = at / PIECES, slot = at % PIECES;
@@ -175,10 +176,10 @@ template <typename T, int TM_, int TN_, int WM_, int WN_> struct Tile {
             for (int e = 0; e < EACH; ++e) {
                 const bool isb = w * EACH + e >= GA;
                 uint32_t o = off[e];
-                if constexpr (AK || BK) {
-                    const int most = (isb ? b.steps : a.steps) - 1 - at * KE;
-                    if ((isb ? BK : AK) && most < KE - 1) o = offset<AK, BK>(a, b, w * EACH + e, lane, most);
-                }
+                const int most_a = AK ? a.k - 1 - at * KE : (a.k >> 4) - 1 - at * (STEP / 16);
+                const int most_b = BK ? b.k - 1 - at * KE : (b.k >> 4) - 1 - at * (STEP / 16);
+                if ((isb ? most_b : most_a) < (isb ? (BK ? KE : STEP / 16) : (AK ? KE : STEP / 16)) - 1)
+                    o = offset<AK, BK>(a, b, w * EACH + e, lane, isb ? most_b : most_a);
                 fetch(__builtin_amdgcn_readfirstlane(lds0 + stage * BYTES + (w * EACH + e) * 1024), o, isb ? pb : pa);
             }
             // (past the end the last step is brought again, into a buffer that nothing reads)
@@ -197,20 +198,27 @@ template <typename T, int TM_, int TN_, int WM_, int WN_> struct Tile {
             asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"(EACH * (STAGES - 2)) : "memory");
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
-            load(stage == 0 ? STAGES - 1 : stage - 1);
+            // Both halves' parts are asked for before the first product: left to itself the compiler keeps
+            // one part at a time and waits for each.
             const char *const x = lds + stage * BYTES;
+            u32x4 fa[2][TM], fb[2][TN];
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
-                u32x4 fa[TM], fb[TN];
 #pragma unroll
-                for (int i = 0; i < TM; ++i) fa[i] = part<BM, AK>(x, (wm * TM + i) * 32, s, lane);
+                for (int j = 0; j < TN; ++j) fb[s][j] = part<BN, BK>(x + BM * STEP, (wn * TN + j) * 32, s, lane);
 #pragma unroll
-                for (int j = 0; j < TN; ++j) fb[j] = part<BN, BK>(x + BM * STEP, (wn * TN + j) * 32, s, lane);
+                for (int i = 0; i < TM; ++i) fa[s][i] = part<BM, AK>(x, (wm * TM + i) * 32, s, lane);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            load(stage == 0 ? STAGES - 1 : stage - 1);
+            __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
 #pragma unroll
                 for (int i = 0; i < TM; ++i)
 #pragma unroll
-                    for (int j = 0; j < TN; ++j) Mma<T>::add(acc[i][j], fa[i], fb[j]);
-            }
+                    for (int j = 0; j < TN; ++j) Mma<T>::add(acc[i][j], fa[s][i], fb[s][j]);
+            __builtin_amdgcn_s_setprio(0);
             stage = stage == STAGES - 1 ? 0 : stage + 1;
         }
         // nothing is in flight to the LDS, and nobody reads it, when this returns
