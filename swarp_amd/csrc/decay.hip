@@ -564,6 +564,249 @@ __global__ __launch_bounds__(BLOCK, 2) void k_together(const Call c)
     }
 }
 
+// All gradients of heads up to 32 wide over at most 32 steps, where one chunk is all: q, k, v and do are
+// read once.  As k_together a workgroup has four heads, whose rows it brings and writes together; a
+// wave then works on its head alone.  With the powers w_ti (0 across an end of an episode),
+//   dP_ti = w_ti (do_t v_i), P_ti = w_ti (q_t k_i):  dq = dP k,  dk = dP^T q,  dv = P^T do,
+// and with the state S0 before the first step and the gradient Z of the one after the last
+//   dq_t += lambda^(t+1) S0 do_t,  dk_i += lambda^(T-1-i) Z v_i,  dv_i += lambda^(T-1-i) Z^T k_i,
+//   d S0 = lambda^T Z + sum_t lambda^(t+1) q_t do_t^T.
+// dP is formed twice, with a lane's step that of dq and that of dk: either way it is the next product's
+// operand as it lies.
+template <typename T, int FIT> __global__ __launch_bounds__(BLOCK, 2) void k_short(const Call c, const Scan sq, const Scan sk, const Scan sv)
+{
+    constexpr int PAD = 16 / (int)sizeof(T), P = 32 + PAD, ROOM = WAVES * 32 * P, EACH = 2;
+    __shared__ __align__(16) T room[4 * ROOM];
+    const int mine = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t lines = c.batch * c.heads, groups = (lines + WAVES - 1) / WAVES;
+    int64_t group = blockIdx.x;
+    const int lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31, perm = swapped(col);
+    const int L = (int)c.steps, dk = sq.dv, dv = sq.dk;
+    const int h = (int)((uint32_t)(group * WAVES + mine) % (uint32_t)c.heads);
+    const float a2 = decay_of(c, h);
+    // powers from step i = register to step t = lane (D), from step i = lane to step t = register (E)
+    float D[16], E[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const int i = 16 * (r >> 3) + 8 * half + (r & 7);
+        D[r] = col >= i ? sq.score * __builtin_amdgcn_exp2f(a2 * (float)(col - i)) : 0.0f;
+        E[r] = i >= col && i < L ? sq.score * __builtin_amdgcn_exp2f(a2 * (float)(i - col)) : 0.0f;
+    }
+    const float first = sq.carry * __builtin_amdgcn_exp2f(a2 * (float)(col + 1)), last = __builtin_amdgcn_exp2f(a2 * (float)(L - 1 - col));
+
+    // pieces as in k_together: q, k, v, do in, dq, dk, dv out
+    struct Array {
+        const void *p;
+        const int64_t *st;
+        int n;
+    };
+    const Array in[4] = {{sk.v, sk.vs, dk}, {sq.v, sq.vs, dk}, {sq.k, sq.ks, dv}, {sq.q, sq.qs, dv}};
+    const Array to[3] = {{sv.out, sv.os, dv}, {sk.out, sk.os, dk}, {sq.out, sq.os, dk}};  // where q, k, v were
+    Raw<T> raw[4][EACH];
+    uint8_t sr = 0;
+    auto load = [&](int64_t group) {
+#pragma unroll
+        for (int n = 0; n < EACH; ++n) {
+            int x = n * BLOCK + (int)threadIdx.x;
+            asm volatile("" : "+v"(x));
+            const int row = (x >> 4) < L ? x >> 4 : L - 1, at = 8 * (x & 3);
+            const uint32_t line = (uint32_t)(group * WAVES + (x >> 2 & 3)), b = line / (uint32_t)c.heads;
+            if (line >= lines) continue;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const T *const y = (const T *)in[k].p + row * in[k].st[0] + b * in[k].st[1] + (line - b * (uint32_t)c.heads) * in[k].st[2];
+                // (q and do are zero past their ends: what k, v and columns bring there meets them)
+                raw[k][n] = row_of<T, FIT>(y, at, in[k].n, true);
+            }
+        }
+        const int64_t line = group * WAVES + mine;
+        sr = 0;
+        if (c.starts && col < L && line < lines)
+            sr = c.starts[col * (c.batch / c.group) + (uint32_t)line / (uint32_t)c.heads / (uint32_t)c.group];
+    };
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int n = 0; n < EACH; ++n) raw[k][n] = {};
+    load(group);
+    for (; group < groups; group += sq.spans) {
+        const int64_t bh = group * WAVES + mine;
+        // an episode starts with these steps: step t is entered from `since` on, step i enters up to `until`
+        const uint32_t cut = (uint32_t)__ballot(sr);
+#pragma unroll
+        for (int n = 0; n < EACH; ++n) {
+            const int x = n * BLOCK + (int)threadIdx.x, row = x >> 4;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                // (steps past the last are zeros)
+#pragma unroll
+                for (int w = 0; w < (int)(2 * sizeof(T)); ++w) raw[k][n].w[w] = row < L ? raw[k][n].w[w] : 0;
+                *(Raw<T> *)(room + k * ROOM + ((x >> 2 & 3) * 32 + row) * P + 8 * (x & 3)) = raw[k][n];
+            }
+        }
+        __syncthreads();
+        if (group + sq.spans < groups) load(group + sq.spans);
+        if (bh < lines) {
+            // (what follows from the lane is worked out here, and not kept in registers from head to head)
+            int lane = threadIdx.x & 63;
+            asm volatile("" : "+v"(lane));
+            const int half = lane >> 5, col = lane & 31, perm = swapped(col);
+            T *const qx = room + mine * 32 * P, *const kx = qx + ROOM, *const vx = kx + ROOM, *const ox = vx + ROOM;
+            auto rows = [&](const T *x, int row, Part<T> (&y)[2]) {
+                y[0] = part_of(*(const Raw<T> *)(x + row * P + 8 * half));
+                y[1] = part_of(*(const Raw<T> *)(x + row * P + 8 * half + 16));
+            };
+            const uint32_t upto = cut & (0xffffffffu >> (31 - col)), after = col < 31 ? cut >> (col + 1) << (col + 1) : 0;
+            const int since = upto ? 31 - __clz(upto) : 0, until = after ? __ffs((int)after) - 1 : 32;
+            float odd = 0.0f;
+            Part<T> a[2], b[2], hi[2], lo[2];
+            f32x16 p;
+            // scores of `a` (rows by swapped lane) and `b` (by lane), times their powers, as operands
+            auto scores = [&](const float (&w)[16], int from, int below) {
+                p = {};
+                mma<T>(p, a[0], b[0]);
+                mma<T>(p, a[1], b[1]);
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    float y[8];
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) {
+                        const int i = 16 * x + 8 * half + r;
+                        y[r] = p[8 * x + r] * w[8 * x + r];
+                        if (cut) {
+                            odd = __builtin_fmaf(y[r], 0.0f, odd);
+                            y[r] = i >= from && i < below ? y[r] : 0.0f;
+                        }
+                    }
+                    hi[x] = term_of<T>(y, true);
+                    if (Part<T>::TERMS) lo[x] = term_of<T>(y, false);
+                    odd = odd_of<T>(hi[x], odd);
+                }
+            };
+            auto times = [&](f32x16 &o, const T *x) {
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    const Part<T> z = column_of<T>(x, P, 16 * y, 0, lane);
+                    odd = odd_of<T>(z, odd);
+                    mma<T>(o, z, hi[y]);
+                    if (Part<T>::TERMS) mma<T>(o, z, lo[y]);
+                }
+            };
+            // o += M y for a state M: eight of its elements a lane, `step` apart, beside y's parts
+            auto state = [&](f32x16 &o, const float *m, int64_t lane_step, int64_t step, int across, int along, const Part<T> (&y)[2]) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    float z[8];
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) {
+                        const int i = 16 * x + 8 * half + r;
+                        z[r] = perm < across && i < along ? m[perm * lane_step + i * step] : 0.0f;
+                        odd = __builtin_fmaf(z[r], 0.0f, odd);
+                    }
+                    mma<T>(o, term_of<T>(z, true), y[x]);
+                    if (Part<T>::TERMS) mma<T>(o, term_of<T>(z, false), y[x]);
+                }
+            };
+            auto put = [&](T *x, const f32x16 &o) {
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    Span<T, 8> e;
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) e.e[r] = (T)o[8 * n + r];
+                    *(Raw<T> *)(x + col * P + 16 * n + 8 * half) = __builtin_bit_cast(Raw<T>, e);
+                }
+            };
+            f32x16 dq = {}, dk_ = {}, dv_ = {};
+            if (sq.state) {  // dq: S0 [dk][dv] do
+                rows(ox, col, b);
+                state(dq, sq.state + bh * c.area, dv, 1, dk, dv, b);
+                const float f = upto ? 0.0f : first;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) dq[r] *= f;
+            }
+            if (sk.state) {
+                const float *const z = sk.state + bh * c.area;
+                const float f = after ? 0.0f : last;
+                rows(vx, col, b);
+                state(dk_, z, dv, 1, dk, dv, b);
+                rows(kx, col, b);
+                state(dv_, z, 1, dv, dv, dk, b);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    dk_[r] *= f;
+                    dv_[r] *= f;
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            rows(vx, perm, a);
+            rows(ox, col, b);
+            scores(D, since, 32);
+            times(dq, kx);
+            __builtin_amdgcn_sched_barrier(0);
+            rows(ox, perm, a);
+            rows(vx, col, b);
+            scores(E, 0, until);
+            times(dk_, qx);
+            __builtin_amdgcn_sched_barrier(0);
+            put(vx, dq);  // (a wave has read what it needs of v: gradients take the rows' place)
+            rows(qx, perm, a);
+            rows(kx, col, b);
+            scores(E, 0, until);
+            times(dv_, ox);
+            __builtin_amdgcn_sched_barrier(0);
+            if (sv.state_out) {  // d S0: columns of q, and of do times their powers
+                f32x16 z = {};
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const Part<T> qc = column_of<T>(qx, P, 16 * x, 0, lane), oc = column_of<T>(ox, P, 16 * x, 0, lane);
+                    float y[8];
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) {
+                        const int t = 16 * x + 8 * half + r;
+                        const float w = cut & (0xffffffffu >> (31 - t)) ? 0.0f : sq.score * __builtin_amdgcn_exp2f(a2 * (float)(t + 1));
+                        y[r] = element(oc, r) * w;
+                    }
+#pragma unroll
+                    for (int n = 0; n < (Part<T>::TERMS ? 3 : 1); ++n) mma<T>(z, qc, term_of<T>(y, n < 2));
+                }
+                const float f = cut ? 0.0f : __builtin_amdgcn_exp2f(a2 * (float)L);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int i = 16 * (r >> 3) + 8 * half + (r & 7);
+                    const int64_t at = bh * c.area + i * dv + perm;
+                    if (i < dk && perm < dv) sv.state_out[at] = z[r] + (sk.state && !cut ? f * sk.state[at] : 0.0f);
+                }
+            }
+            const bool wrong = __ballot(!(odd == 0.0f)) != 0;
+            if (lane < 3) c.wrong[bh * 3 + lane] = wrong;
+            put(kx, dk_);
+            put(qx, dv_);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < EACH; ++n) {
+            int x = n * BLOCK + (int)threadIdx.x;
+            asm volatile("" : "+v"(x));
+            const int row = x >> 4, at = 8 * (x & 3);
+            const uint32_t line = (uint32_t)(group * WAVES + (x >> 2 & 3)), b = line / (uint32_t)c.heads;
+            if (row >= L || line >= lines) continue;
+#pragma unroll
+            for (int k = 0; k < 3; ++k) {
+                const Span<T, 8> e = __builtin_bit_cast(Span<T, 8>, *(const Raw<T> *)(room + k * ROOM + ((x >> 2 & 3) * 32 + row) * P + at));
+                T *const y = (T *)to[k].p + row * to[k].st[0] + b * to[k].st[1] + (line - b * (uint32_t)c.heads) * to[k].st[2] + at;
+                const int left = to[k].n - at;
+                if (FIT == FULL || (FIT == EIGHTS ? left > 0 : left >= 8)) *(Span<T, 8> *)y = e;
+                else if constexpr (FIT == ANY) {
+#pragma unroll
+                    for (int r = 0; r < 8; ++r)
+                        if (r < left) y[r] = e.e[r];
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
 // The heads (and columns) where something was not finite, step by step, as the definition has it: what
 // a start or the order of the steps keeps from an output does not reach it as a product with 0.
 template <typename T, int KT> __global__ __launch_bounds__(BLOCK) void k_exact(const Call c, int64_t n)
@@ -801,13 +1044,19 @@ template <typename T, int KT, int WHAT> void alone(Call &c, int fit, hipStream_t
     else hipLaunchKernelGGL((k_alone<T, KT, WHAT, ANY>), grid, dim3(BLOCK), 0, st, c);
 }
 
+// Workgroups of four heads each, of which each has the same h in every wave throughout: four times
+// their number is a multiple of the call's heads, as far as there is more than one group for each.
+int64_t spans_of(const Call &c, int64_t want)
+{
+    const int64_t groups = (c.batch * c.heads + WAVES - 1) / WAVES;
+    const int64_t whole = c.heads % 4 == 0 ? c.heads / 4 : c.heads % 2 == 0 ? c.heads / 2 : c.heads;
+    const int64_t n = want < whole ? whole : want / whole * whole;
+    return n < groups ? n : groups;
+}
+
 template <typename T, int WHAT> void together(Call &c, int fit, hipStream_t st)
 {
-    const int64_t lines = c.batch * c.heads, groups = (lines + WAVES - 1) / WAVES;
-    // (four times the spans must be a multiple of the call's heads, as far as there is more than one)
-    const int64_t whole = c.heads % 4 == 0 ? c.heads / 4 : c.heads % 2 == 0 ? c.heads / 2 : c.heads;
-    const int64_t want = MOST_WAVES / WAVES / (c.segments * c.scans), spans = want < whole ? whole : want / whole * whole;
-    for (int i = 0; i < c.scans; ++i) c.scan[i].spans = spans < groups ? spans : groups;
+    for (int i = 0; i < c.scans; ++i) c.scan[i].spans = spans_of(c, MOST_WAVES / WAVES / (c.segments * c.scans));
     const dim3 grid((unsigned)(c.scan[0].spans * c.segments * c.scans));
     if (fit == FULL) hipLaunchKernelGGL((k_together<T, WHAT, FULL>), grid, dim3(BLOCK), 0, st, c);
     else if (fit == EIGHTS) hipLaunchKernelGGL((k_together<T, WHAT, EIGHTS>), grid, dim3(BLOCK), 0, st, c);
@@ -819,7 +1068,14 @@ template <typename T, int KT, int WHAT> void scan(Call &c, int fit, hipStream_t 
     // Heads up to 32 wide go together: their rows are short (32 x 256000 x 2 heads of 32, forward and
     // backward: 1.52 and 3.07 ms, alone 1.88 and 3.44); wider ones alone (4095 x 96 x 4 heads of 64: 0.28 and
     // 0.88, together 0.29 and 1.11: barriers between waves that have much to do).
-    if (KT == 1 && c.slices == c.scans) together<T, WHAT>(c, fit, st);
+    if (KT == 1 && c.scans == 3 && c.slices == 3 && c.steps >= 1 && c.steps <= CHUNK) {
+        // One chunk, backward: all three at once.
+        c.scan[0].spans = spans_of(c, MOST_WAVES / WAVES);
+        const dim3 grid((unsigned)c.scan[0].spans);
+        if (fit == FULL) hipLaunchKernelGGL((k_short<T, FULL>), grid, dim3(BLOCK), 0, st, c, c.scan[0], c.scan[1], c.scan[2]);
+        else if (fit == EIGHTS) hipLaunchKernelGGL((k_short<T, EIGHTS>), grid, dim3(BLOCK), 0, st, c, c.scan[0], c.scan[1], c.scan[2]);
+        else hipLaunchKernelGGL((k_short<T, ANY>), grid, dim3(BLOCK), 0, st, c, c.scan[0], c.scan[1], c.scan[2]);
+    } else if (KT == 1 && c.slices == c.scans) together<T, WHAT>(c, fit, st);
     else alone<T, KT, WHAT>(c, fit, st);
     if (WHAT == OUTPUTS) {
         const int64_t n = c.units / c.segments;
