@@ -135,6 +135,11 @@ __global__ __launch_bounds__(BLOCK) void k_place(int64_t rows, const uint8_t *ma
 
 // ------------------------------------------------------------------ rows made ready
 
+// Eight neighbouring elements, anywhere.
+template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Eight {
+    T e[8];
+};
+
 // Row i of the hidden states, padded with zeros, and its target's logit (NaN if there is no such
 // target).  A wave a row.
 template <typename T> __global__ __launch_bounds__(BLOCK) void k_rows(const Call c)
@@ -151,13 +156,21 @@ template <typename T> __global__ __launch_bounds__(BLOCK) void k_rows(const Call
         const T *const w = (const T *)c.weight + (in ? t : 0) * c.dim;
         T *const h = (T *)c.h + j * c.dim_p;
         float z = 0.0f;
-        for (int k = lane; k < c.dim_p; k += 64) {
-            T v = (T)0.0f;
-            if (k < c.dim) {
-                v = x[k];
-                z = __builtin_fmaf(up(v), up(w[k]), z);
+        for (int k = lane * 8; k < c.dim_p; k += 64 * 8) {  // (a padded row is a multiple of eight)
+            Eight<T> v = {}, y = {};
+            if (k + 8 <= c.dim) {
+                v = *(const Eight<T> *)(x + k);
+                y = *(const Eight<T> *)(w + k);
+            } else {
+                for (int q = 0; q < 8; ++q)
+                    if (k + q < c.dim) {
+                        v.e[q] = x[k + q];
+                        y.e[q] = w[k + q];
+                    }
             }
-            h[k] = v;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) z = __builtin_fmaf(up(v.e[q]), up(y.e[q]), z);
+            *(Eight<T> *)(h + k) = v;
         }
         z = wave_sum(z);
         if (lane == 0) {
@@ -191,7 +204,12 @@ template <typename T> __global__ __launch_bounds__(BLOCK) void k_scale(const Cal
     for (int r = blockIdx.x * (BLOCK / 64) + (threadIdx.x >> 6); r < all; r += gridDim.x * (BLOCK / 64)) {
         const T *const x = (const T *)c.h + (c.first + (r < rows ? r : 0)) * c.dim_p;
         const float f = r < rows ? c.inv_h[c.first + r] : 0.0f;
-        for (int k = lane; k < c.dim_p; k += 64) ((T *)c.hs)[(int64_t)r * c.dim_p + k] = r < rows ? (T)(up(x[k]) * f) : (T)0.0f;
+        for (int k = lane * 8; k < c.dim_p; k += 64 * 8) {
+            Eight<T> v = *(const Eight<T> *)(x + k);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) v.e[q] = r < rows ? (T)(up(v.e[q]) * f) : (T)0.0f;
+            *(Eight<T> *)((T *)c.hs + (int64_t)r * c.dim_p + k) = v;
+        }
     }
 }
 
@@ -585,13 +603,25 @@ __global__ __launch_bounds__(BLOCK) void k_give(const float *from, T *to, int64_
 {
     const float f = *up1;
     if ((const void *)from == (const void *)to && f == 1.0f) return;
-    for (int64_t k = (int64_t)blockIdx.x * BLOCK + threadIdx.x; k < n; k += (int64_t)gridDim.x * BLOCK) {
-        int64_t at = k;
-        if (place) {
-            const int64_t i = k / dim, j = place[i];
-            at = j < 0 ? -1 : j * dim + (k - i * dim);
+    if (!place) {
+        struct __align__(16) F4 { float e[4]; };
+        struct __attribute__((aligned(4 * sizeof(T)))) T4 { T e[4]; };
+        for (int64_t k = ((int64_t)blockIdx.x * BLOCK + threadIdx.x) * 4; k < n; k += (int64_t)gridDim.x * BLOCK * 4) {
+            if (k + 4 <= n) {
+                const F4 x = *(const F4 *)(from + k);
+                T4 y;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) y.e[q] = (T)(f * x.e[q]);
+                *(T4 *)(to + k) = y;
+            } else {
+                for (int64_t q = k; q < n; ++q) to[q] = (T)(f * from[q]);
+            }
         }
-        to[k] = at < 0 ? (T)0.0f : (T)(f * from[at]);
+        return;
+    }
+    for (int64_t k = (int64_t)blockIdx.x * BLOCK + threadIdx.x; k < n; k += (int64_t)gridDim.x * BLOCK) {
+        const int64_t i = k / dim, j = place[i];
+        to[k] = j < 0 ? (T)0.0f : (T)(f * from[j * dim + (k - i * dim)]);
     }
 }
 
