@@ -6,8 +6,7 @@ magnitudes, `dz`; an exponential of a difference of two logits, relative to a su
 tree, is then off by 2 dz + 32 2^-24 of itself at most (the hardware's exp2 and log2 and what leads to
 them cost a few 2^-24 each, the argument's rounding 2^-24 times its magnitude, below 2^6 here).  A
 gradient is a sum of such weights times h or W: its magnitudes' sum times that error, times u for
-the weight's rounding to the type, times u again where h is multiplied by the row's 1 / s and rounded
-(the weight's gradient), and n 2^-24 for adding n terms; and u of itself, for the end."""
+the weight's rounding to the type, and n 2^-24 for adding n terms; and u of itself, for the end."""
 
 import math
 
@@ -70,7 +69,7 @@ def reference(h, w, t, b, m, up=1.0, reduction="mean"):
     dh = G @ wd
     out["hidden"] = (dh, tol(dh, (mag * err) @ wd.abs(), mag @ wd.abs(), V, 1))
     dw = G.t() @ hd
-    out["weight"] = (dw, tol(dw, (mag * err).t() @ hd.abs(), mag.t() @ hd.abs(), rows, 2))
+    out["weight"] = (dw, tol(dw, (mag * err).t() @ hd.abs(), mag.t() @ hd.abs(), rows, 1))
     db = G.sum(0)
     out["bias"] = (db, tol(db, (mag * err).sum(0), mag.sum(0), rows, 1))
     return out
@@ -185,6 +184,26 @@ def test_closed_actions_and_far_targets(dtype):
     assert float(got["loss"]) == math.inf and bool((got["logp"][t == 3] == -math.inf).all())
     want = reference(h, w, t, b, None, 64.0)
     close(got["hidden"], want["hidden"], "hidden")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,D,V", [(40, 64, 25), (300, 64, 300), (20, 64, 300)])
+def test_a_row_of_the_lowest_biases(rows, D, V, dtype):
+    """Beside the type's lowest value a logit vanishes: every action is as likely as another."""
+    h, w, t = inputs(rows, D, V, dtype, 21)[:3]
+    b = torch.full((V,), torch.finfo(dtype).min, dtype=dtype, device=DEV)
+    got = run(h, w, t, b, None)
+    # (hardware's exp2 and log2 and the sum's tree: the 32 2^-24 of the others)
+    assert float((got["logp"].double() + math.log(V)).abs().max()) <= (32 + 4 * math.log(V)) * F24
+    G = (1.0 / V - torch.nn.functional.one_hot(t, V).double()) / rows
+    mag, u = (1.0 / V + torch.nn.functional.one_hot(t, V).double()) / rows, half(dtype)
+
+    def tol(m, value, terms):
+        return m * (1.01 * u + (32 + terms) * F24) + (u + 4 * F24) * value.abs()
+    hd, wd = h.double(), w.double()
+    close(got["hidden"], (G @ wd, tol(mag @ wd.abs(), G @ wd, V)), "hidden")
+    close(got["weight"], (G.t() @ hd, tol(mag.t() @ hd.abs(), G.t() @ hd, rows)), "weight")
+    close(got["bias"], (G.sum(0), tol(mag.sum(0), G.sum(0), rows)), "bias")
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
