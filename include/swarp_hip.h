@@ -607,7 +607,8 @@ typedef struct swarp_decay {
 uint64_t swarp_decay_work_bytes(const swarp_decay_t *a); /* of either call */
 int swarp_decay_fwd(const swarp_decay_t *a, void *stream);
 int swarp_decay_bwd(const swarp_decay_t *a, void *stream);
-/* One step (steps = 1): state_out is written, `state` itself as a rule.  No work memory. */
+/* One step (steps = 1): state_out is written, `state` itself as a rule; q, k and v lie outside it.
+ * No work memory. */
 int swarp_decay_step(const swarp_decay_t *a, void *stream);
 
 #ifdef __cplusplus

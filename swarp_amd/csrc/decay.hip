@@ -1280,6 +1280,15 @@ int swarp_decay_step(const swarp_decay_t *a, void *stream)
     if (a->steps != 1) return fail("a step is one step");
     if (!a->log_decay || !a->q || !a->k || !a->v || !a->out || !a->state_out)
         return fail("pointer arguments must be set");
+    // (the state is changed while others still read q, k and v)
+    const uintptr_t size = a->dtype == SWARP_F32 ? 4 : 2, from = (uintptr_t)a->state_out;
+    const uintptr_t to = from + (uintptr_t)a->batch * a->heads * a->dk * a->dv * 4;
+    auto apart = [&](const void *x, const int64_t *stride, int d) {
+        const uintptr_t n = (uintptr_t)((a->batch - 1) * stride[1] + (a->heads - 1) * stride[2] + d) * size;
+        return (uintptr_t)x >= to || (uintptr_t)x + n <= from;
+    };
+    if (!apart(a->q, a->q_stride, a->dk) || !apart(a->k, a->k_stride, a->dk) || !apart(a->v, a->v_stride, a->dv))
+        return fail("q, k and v must not lie in the state");
     hipStream_t st = (hipStream_t)stream;
     switch (a->dtype) {
     case SWARP_F32: step<float>(a, st); break;

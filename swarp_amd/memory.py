@@ -239,6 +239,7 @@ def decay_attention_step(
     a.out = out.data_ptr()
     with _guard(q.device):
         _lib.check(_lib.load().swarp_decay_step(ctypes.byref(a), _lib.stream_of(q.device)))
-    torch.autograd.graph.increment_version(state)
+    if not state.is_inference():
+        torch.autograd.graph.increment_version(state)
     del keep
     return out

@@ -248,6 +248,31 @@ def test_strides(dtype):
         assert torch.equal(o1, decay_attention_step(*(t[0] for t in plain), ld, S2)) and torch.equal(S1, S2)
 
 
+def test_step_under_inference_mode():
+    q, k, v, ld, state, s = inputs(1, (3,), 2, 8, 8, torch.float32, 44, 0.3)
+    want = decay_attention(q, k, v, ld, state, s)
+    for own in (True, False):  # (a state of inference mode has no version to count)
+        with torch.inference_mode():
+            now = state.clone() if own else None
+        now = now if own else state.clone()
+        version = None if own else now._version
+        with torch.inference_mode():
+            out = decay_attention_step(q[0], k[0], v[0], ld, now, s[0])
+        assert torch.allclose(out, want.out[0], rtol=1e-5, atol=1e-5)
+        assert torch.allclose(now, want.state, rtol=1e-5, atol=1e-5)
+        assert own or now._version > version
+
+
+def test_step_with_parts_of_the_state():
+    state = torch.randn(4, 2, 8, 8, device=DEV)
+    q = torch.randn(4, 2, 8, device=DEV)
+    ld = torch.full((2,), -0.5, device=DEV)
+    with pytest.raises(RuntimeError, match="in the state"):
+        decay_attention_step(q, q, state[:, :, 3], ld, state)
+    both = torch.randn(4 * 2 * 8 + 4 * 2 * 8 * 8, device=DEV)  # beside each other
+    decay_attention_step(q, q, both[:64].view(4, 2, 8), ld, both[64:].view(4, 2, 8, 8))
+
+
 def test_empty_calls():
     for T, B in ((0, 3), (5, 0), (0, 0)):
         q, k, v, ld, state, s = inputs(T, (B,), 2, 8, 8, torch.float32, 1)

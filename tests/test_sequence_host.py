@@ -119,6 +119,13 @@ def test_decay_refuses_before_any_launch():
     refused(lib.swarp_decay_bwd(ctypes.byref(a), None), "together")
     refused(lib.swarp_decay_step(ctypes.byref(args(state_out=256)), None), "one step")
     refused(lib.swarp_decay_step(ctypes.byref(args(steps=1)), None), "pointer")
+    # the state: 4 x 2 x 8 x 8 floats from 1 << 20 on; q, k and v: 4 x 2 x 8
+    state, n = 1 << 20, 4 * 2 * 8 * 8 * 4
+    strides = {x + "_stride": (ctypes.c_int64 * 3)(0, 16, 8) for x in "qkv"}
+    for name in "qkv":
+        for at in (state, state - 4, state + n - 4, state - 4 * 2 * 8 * 4 + 4):
+            refused(lib.swarp_decay_step(ctypes.byref(args(steps=1, state_out=state, **strides, **{name: at})), None),
+                    "in the state")
 
 
 @pytest.fixture(autouse=True)
