@@ -17,11 +17,11 @@
 // the piece is done again, relative to the rows' maxima (the kernels of that second pass are always
 // launched, look at a flag, and mostly end).
 //
-// 16 bits: the sums come first and the exponentials, relative to them, from a second product, so that
-// beside E^T stands h itself and G is the one rounding before the gradients' own.  With one product
-// h / s is rounded too: 6138 decisions of 50001 logits, 1024 wide, bfloat16, took 2.24 ms then, not
-// 2.83, and had d W 2.9e-3 of its size off, not 1.7e-3, which is what its own rounding makes.
-// float16 has not the range for it either.
+// 16 bits: h / s beside E^T would be a second rounding of d W's terms (8 x 1023 decisions of 50001 logits,
+// 1024 wide, bfloat16, a quarter masked: 2.9e-3 of its size off, where its own rounding makes 1.7e-3),
+// and float16 has not the range.  So 24 bits of an exponential are kept, in two places, and become G,
+// normalised and rounded once, in a pass of their own (0.32 ms there: 5 bytes a logit at 4.8 TB/s), beside
+// which h stands as it is: 2.58 ms in all, and 2.83 with the sums from a product of their own instead.
 //
 // Decisions whose mask is not set are left out of the products: the rows that count are gathered
 // first, and every kernel goes by their number on the device.
@@ -44,15 +44,9 @@ constexpr float LN_2 = 0.69314718055994530942f;
 constexpr float REACH = 40.0f;        // e^40 times 2^21 logits, times any weight, is far from overflow
 constexpr int KEPT_BITS = 14;         // 16-bit exponentials are kept times 2^14: float16's 2^-38 is not lost
 using narrow::COUNT_ROWS;
-constexpr uint64_t PIECE = 1ull << 30;  // bytes of exponentials at a time
+constexpr uint64_t PIECE = 1ull << 30;  // bytes of exponentials at a time (but for their lower 8 bits)
 
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * LOG2E); }
-// An exponential times 2^KEPT_BITS over its row's sum: `hi` is the row's largest logit, `by` what the sum
-// is in the exponent.  (Not one number for both: beside a large logit the sum's part would be lost.)
-__device__ __forceinline__ float normed(float z, float hi, float by)
-{
-    return __builtin_amdgcn_exp2f(fmaf(z - hi, LOG2E, by));
-}
 __device__ __forceinline__ float log_of(float x) { return __builtin_amdgcn_logf(x) * LN_2; }
 
 // What every kernel of a call may read.  Rows are the counted ones, in order; `n_on` of them.
@@ -72,8 +66,9 @@ struct Call {
     float *logp, *loss;
     // of all rows
     void *h;
-    float *z_t, *ref, *top;   // target's logit; what E is relative to; largest logit (16 bits: `by` of normed())
-    float *inv, *inv_h;       // weight / s; what h is multiplied by beside E^T
+    float *z_t, *ref, *top;   // target's logit; what E is relative to; largest logit
+    float *inv, *inv_h;       // of d h's rows; what h, or E (16 bits), is multiplied by: k_scale, k_norm
+    int32_t *target;          // 16 bits: or -1
     double *sums;             // of logp, one for `few` rows
     int few;                  // rows of a workgroup that joins: 1 or 64
     // of the piece
@@ -81,6 +76,7 @@ struct Call {
     float2 *parts;            // [n_parts][piece]: largest logit and sum of a part of a row
     int n_parts;
     void *e, *hs;             // exponentials; h as it goes beside them
+    uint8_t *low;             // of a 24-bit exponential, the bits that E has not room for
     const void *w;            // padded weight
 };
 
@@ -215,7 +211,7 @@ template <typename T> __global__ __launch_bounds__(BLOCK) void k_scale(const Cal
     const int rows = rows_of(c), all = (rows + 31) / 32 * 32, lane = threadIdx.x & 63;
     for (int r = blockIdx.x * (BLOCK / 64) + (threadIdx.x >> 6); r < all; r += gridDim.x * (BLOCK / 64)) {
         const T *const x = (const T *)c.h + (c.first + (r < rows ? r : 0)) * c.dim_p;
-        const float f = r < rows ? c.inv_h[c.first + r] : 0.0f;
+        const float f = sizeof(T) == 2 ? 1.0f : r < rows ? c.inv_h[c.first + r] : 0.0f;
         for (int k = lane * 8; k < c.dim_p; k += 64 * 8) {
             Eight<T> v = *(const Eight<T> *)(x + k);
 #pragma unroll
@@ -267,15 +263,6 @@ __global__ __launch_bounds__(C::THREADS) void k_logits(const Call c, int nm, int
     for (int j = 0; j < C::TN; ++j) {
         const int row = r0 + (wn * C::TN + j) * 32 + acc_col(lane);
         const bool mine = row < rows;
-        if constexpr (STORE && sizeof(T) == 2) {
-            // (normalised, so that nothing is summed)
-            const float hi = c.ref[c.first + (mine ? row : 0)], by = c.top[c.first + (mine ? row : 0)];
-#pragma unroll
-            for (int i = 0; i < C::TM; ++i)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) t.acc[i][j][r] = normed(t.acc[i][j][r], hi, by);
-            continue;
-        }
         float m = -INFINITY, s = 0.0f;
 #pragma unroll
         for (int i = 0; i < C::TM; ++i)
@@ -306,8 +293,11 @@ __global__ __launch_bounds__(C::THREADS) void k_logits(const Call c, int nm, int
     if constexpr (STORE) {
         // through LDS, so that a row's are written together: 32 decisions of a wave's columns at a time
         constexpr int PITCH = C::TM * 32 + 16 / (int)sizeof(T), PIECES = C::TM * 32 * (int)sizeof(T) / 16;
-        static_assert(C::WAVES * 32 * PITCH * (int)sizeof(T) <= C::LDS, "a wave's part of a tile fits");
+        constexpr bool LOW = sizeof(T) == 2;
+        constexpr int PITCH_LOW = C::TM * 32 + 16;
+        static_assert(C::WAVES * 32 * (PITCH * (int)sizeof(T) + (LOW ? PITCH_LOW : 0)) <= C::LDS, "a wave's part of a tile fits");
         T *const mine = (T *)lds + w * 32 * PITCH;
+        uint8_t *const low = (uint8_t *)lds + C::WAVES * 32 * PITCH * sizeof(T) + w * 32 * PITCH_LOW;
         __syncthreads();  // (every wave has read its last operands)
         const int64_t v = v0 + wm * C::TM * 32;
 #pragma unroll
@@ -316,10 +306,23 @@ __global__ __launch_bounds__(C::THREADS) void k_logits(const Call c, int nm, int
             for (int i = 0; i < C::TM; ++i)
 #pragma unroll
                 for (int r = 0; r < 16; r += 4) {
-                    struct __attribute__((aligned(4 * sizeof(T)))) Four { T e[4]; } y;
+                    const int at = i * 32 + acc_row(r, lane);
+                    if constexpr (LOW) {
+                        // the upper 24 bits, rounded: 16 and 8
+                        uint32_t u[4];
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) y.e[q] = (T)t.acc[i][j][r + q];
-                    *(Four *)(mine + acc_col(lane) * PITCH + i * 32 + acc_row(r, lane)) = y;
+                        for (int q = 0; q < 4; ++q) {
+                            const float x = t.acc[i][j][r + q];  // (a vector's element has no address to cast from)
+                            u[q] = __builtin_bit_cast(uint32_t, x) + 0x80u;
+                        }
+                        const uint2 y = {__builtin_amdgcn_perm(u[1], u[0], 0x07060302u), __builtin_amdgcn_perm(u[3], u[2], 0x07060302u)};
+                        *(uint2 *)(mine + acc_col(lane) * PITCH + at) = y;
+                        const uint32_t a = __builtin_amdgcn_perm(u[1], u[0], 0x0c0c0501u), b = __builtin_amdgcn_perm(u[3], u[2], 0x05010c0cu);
+                        *(uint32_t *)(low + acc_col(lane) * PITCH_LOW + at) = a | b;
+                    } else {
+                        *(f32x4 *)(mine + acc_col(lane) * PITCH + at) =
+                            f32x4{t.acc[i][j][r], t.acc[i][j][r + 1], t.acc[i][j][r + 2], t.acc[i][j][r + 3]};
+                    }
                 }
             __builtin_amdgcn_wave_barrier();
             const int row0 = r0 + (wn * C::TN + j) * 32;
@@ -329,16 +332,24 @@ __global__ __launch_bounds__(C::THREADS) void k_logits(const Call c, int nm, int
                 if (row0 + r < rows && v + e < c.wide)
                     *(u32x4 *)((T *)c.e + (int64_t)(row0 + r) * c.wide + v + e) = *(const u32x4 *)(mine + r * PITCH + e);
             }
+            if constexpr (LOW) {
+                constexpr int LOWS = C::TM * 32 / 16;
+#pragma unroll
+                for (int k = 0; k < 32 * LOWS / 64; ++k) {
+                    const int at = k * 64 + lane, r = at / LOWS, e = at % LOWS * 16;
+                    if (row0 + r < rows && v + e < c.wide)
+                        *(u32x4 *)(c.low + (int64_t)(row0 + r) * c.wide + v + e) = *(const u32x4 *)(low + r * PITCH_LOW + e);
+                }
+            }
             __builtin_amdgcn_wave_barrier();
         }
     }
 }
 
 // How a row's parts are joined.
-enum { SUMS = 0,     // from parts relative to their largest: logp; ref becomes what E is made with
+enum { SUMS = 0,     // from parts relative to their largest: logp
        KEPT = 1,     // from parts relative to ref, which E is too: logp, 1 / s, E at the target
-       KEPT2 = 2,    // the same after a second pass
-       NORMED = 3 }; // E is there, normalised: E at the target
+       KEPT2 = 2 };  // the same after a second pass
 
 // A workgroup takes ROWS rows, its threads every (BLOCK / ROWS)-th part of one.
 template <typename T, int ROWS> __global__ __launch_bounds__(BLOCK) void k_join(const Call c, int how)
@@ -354,7 +365,7 @@ template <typename T, int ROWS> __global__ __launch_bounds__(BLOCK) void k_join(
     if (blockIdx.x * ROWS >= rows) return;
     const float ref = c.ref[j], zt = c.z_t[j];
     float s = 0.0f, m = -INFINITY;
-    if (how != NORMED && mine) {
+    if (mine) {
         for (int k = w; k < c.n_parts; k += WAYS) {
             const float2 p = c.parts[(int64_t)k * c.piece + row];
             if (how == SUMS) {
@@ -379,44 +390,35 @@ template <typename T, int ROWS> __global__ __launch_bounds__(BLOCK) void k_join(
         s += red[1][k][lane] * (how == SUMS && mk != -INFINITY ? exp_of(mk - hi) : 1.0f);
     }
     const int64_t i = c.index ? c.index[j] : j;
-    float logp = 0.0f, unit = s;  // the exponentials' sum as E has them
+    float logp;
     if (how == SUMS) {
         logp = (zt - hi) - log_of(s);
-        if (hi == -INFINITY) logp = NAN;  // (no logit above -inf)
-        if (mine) {
-            c.ref[j] = hi == -INFINITY ? NAN : hi;
-            c.top[j] = KEPT_BITS - __builtin_amdgcn_logf(s);
-        }
-    } else if (how == NORMED) {
-        unit = (float)(1 << KEPT_BITS);
     } else {
         logp = (zt - ref) - log_of(s);
-        if (hi == -INFINITY) logp = NAN;
         if (how == KEPT && mine) {
             if (hi - ref > REACH || ref == -INFINITY) *c.flag = 1;
             c.top[j] = hi;
         }
     }
+    const bool none = hi == -INFINITY;  // (no logit above -inf)
+    if (none) logp = NAN;
     if (mine && how != SUMS) {
-        // (a float16 h times 2^-14 would lose its digits: there the product is multiplied)
-        const bool none = how == NORMED ? zt != zt : hi == -INFINITY;
-        const float f = weight_of(c) / unit;
-        c.inv[j] = none ? NAN : f;
-        c.inv_h[j] = none ? NAN : how == NORMED ? 1.0f : f;
-        if (c.e) {
-            const int64_t t = c.targets32 ? (int64_t)((const int32_t *)c.targets)[i] : ((const int64_t *)c.targets)[i];
-            if (t >= 0 && t < c.width)
-                ((T *)c.e)[(int64_t)row * c.wide + t] = (T)((how == NORMED ? normed(zt, ref, c.top[j]) : exp_of(zt - ref)) - unit);
+        const int64_t t = c.targets32 ? (int64_t)((const int32_t *)c.targets)[i] : ((const int64_t *)c.targets)[i];
+        if constexpr (sizeof(T) == 4) {
+            c.inv[j] = c.inv_h[j] = none ? NAN : weight_of(c) / s;
+            if (t >= 0 && t < c.width) ((T *)c.e)[(int64_t)row * c.wide + t] = exp_of(zt - ref) - s;
+        } else {
+            c.inv[j] = weight_of(c) / (1 << KEPT_BITS);
+            c.inv_h[j] = none ? NAN : (1 << KEPT_BITS) / s;
+            c.target[j] = t >= 0 && t < c.width ? (int32_t)t : -1;
         }
     }
-    if (how != NORMED) {
-        if (mine) c.logp[i] = logp;
-        total[lane] = mine ? (double)logp : 0.0;
-        if (lane == 0) {  // (w == 0: one wave at most)
-            double sum = 0;
-            for (int k = 0; k < ROWS; ++k) sum += total[k];
-            c.sums[c.first / ROWS + blockIdx.x] = sum;
-        }
+    if (mine) c.logp[i] = logp;
+    total[lane] = mine ? (double)logp : 0.0;
+    if (lane == 0) {  // (w == 0: one wave at most)
+        double sum = 0;
+        for (int k = 0; k < ROWS; ++k) sum += total[k];
+        c.sums[c.first / ROWS + blockIdx.x] = sum;
     }
 }
 
@@ -425,6 +427,48 @@ __global__ __launch_bounds__(BLOCK) void k_again(const Call c)
 {
     const int row = blockIdx.x * BLOCK + threadIdx.x;
     if (*c.flag && row < rows_of(c)) c.ref[c.first + row] = c.top[c.first + row];
+}
+
+// 16 bits: G / weight times 2^KEPT_BITS, in E's place.  A thread takes eight neighbours at a time (a row is
+// of whole steps, so they are of one row), NORMS times, which it asks for ahead.
+constexpr int NORMS = 4;
+template <typename T> __global__ __launch_bounds__(BLOCK) void k_norm(const Call c)
+{
+    const uint32_t eights = (uint32_t)(c.wide / 8), n = (uint32_t)rows_of(c) * eights;  // (at most 2^26)
+    struct __attribute__((aligned(16))) Whole { uint16_t e[8]; };
+    struct __attribute__((aligned(8))) Low { uint8_t e[8]; };
+    Whole x[NORMS];
+    Low y[NORMS];
+    float f[NORMS];
+    int32_t t[NORMS];
+    const uint32_t first = blockIdx.x * NORMS * BLOCK + threadIdx.x;
+#pragma unroll
+    for (int k = 0; k < NORMS; ++k) {
+        const uint32_t at = first + k * BLOCK;
+        if (at >= n) break;
+        x[k] = ((const Whole *)c.e)[at];
+        y[k] = ((const Low *)c.low)[at];
+        const uint32_t row = at / eights;
+        f[k] = c.inv_h[c.first + row];
+        t[k] = c.target[c.first + row] - (int32_t)(at - row * eights) * 8;
+    }
+#pragma unroll
+    for (int k = 0; k < NORMS; ++k) {
+        const uint32_t at = first + k * BLOCK;
+        if (at >= n) break;
+        struct __attribute__((aligned(16))) { T e[8]; } z;
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+            z.e[q] = (T)(__builtin_bit_cast(float, (uint32_t)x[k].e[q] << 16 | (uint32_t)y[k].e[q] << 8) * f[k]);
+        if ((uint32_t)t[k] < 8u) {
+            const int64_t j = c.first + at / eights;
+            const T one = (T)(exp_of(c.z_t[j] - c.ref[j]) * f[k] - (1 << KEPT_BITS));
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+                if (q == t[k]) z.e[q] = one;
+        }
+        *(decltype(z) *)((Whole *)c.e + at) = z;
+    }
 }
 
 // ------------------------------------------------------------------ products of the gradients
@@ -669,7 +713,7 @@ struct Plan {
     int size;                 // bytes of an element
     int64_t dim_p, wide, piece, n_parts;
     bool few, pad_w, grad;
-    uint64_t index, counts, h, z_t, ref, top, inv, inv_h, sums, flag, parts, e, hs, w, split, bias, bytes;
+    uint64_t index, counts, h, z_t, ref, top, inv, inv_h, target, sums, flag, parts, e, low, hs, w, split, bias, bytes;
 };
 
 // Workgroups of a product: one a compute unit with 128 KiB of LDS, two with 64.
@@ -709,10 +753,12 @@ Plan plan_of(const swarp_linear_ce_t *a)
     p.top = room(true, 4 * N);
     p.inv = room(true, 4 * N);
     p.inv_h = room(true, 4 * N);
+    p.target = room(p.grad && p.size == 2, 4 * N);
     p.sums = room(true, 8 * (N / (piece < FEW_JOINED ? 1 : 64) + 1));
     p.parts = room(true, 8ull * p.n_parts * piece);
     p.w = room(p.pad_w, (uint64_t)V * p.dim_p * p.size);
     p.e = room(p.grad, (uint64_t)piece * p.wide * p.size);
+    p.low = room(p.grad && p.size == 2, (uint64_t)piece * p.wide);
     p.hs = room(dw, (uint64_t)piece * p.dim_p * p.size);
     // (twice as many splits as places, of whole tiles: share_of)
     p.split = room(dh || dw, p.size == 2 ? 2ull * places(2) * 256 * 256 * 4 : 2ull * places(4) * 128 * 128 * 4);
@@ -786,6 +832,7 @@ template <typename T> int run(const swarp_linear_ce_t *a, hipStream_t st)
     c.top = (float *)(mem + p.top);
     c.inv = (float *)(mem + p.inv);
     c.inv_h = (float *)(mem + p.inv_h);
+    c.target = (int32_t *)(mem + p.target);
     c.sums = (double *)(mem + p.sums);
     c.flag = (int32_t *)(mem + p.flag);
     c.parts = (float2 *)(mem + p.parts);
@@ -793,6 +840,7 @@ template <typename T> int run(const swarp_linear_ce_t *a, hipStream_t st)
     c.few = p.piece < FEW_JOINED ? 1 : 64;
     c.w = p.pad_w ? mem + p.w : (const char *)a->weight;
     c.e = p.grad ? mem + p.e : nullptr;
+    c.low = (uint8_t *)mem + p.low;
     c.hs = mem + p.hs;
     if (a->mask && a->rows) {
         c.index = (int32_t *)(mem + p.index);
@@ -817,18 +865,15 @@ template <typename T> int run(const swarp_linear_ce_t *a, hipStream_t st)
             join<T>(c, SUMS, st);
             continue;
         }
-        if (sizeof(T) == 2) {
-            ok &= logits<T, false>(c, p.few, 0, st);
-            join<T>(c, SUMS, st);
-            ok &= logits<T, true>(c, p.few, 0, st);
-            join<T>(c, NORMED, st);
-        } else {
-            hipLaunchKernelGGL(k_clear, dim3(1), dim3(1), 0, st, c.flag);
-            ok &= logits<T, true>(c, p.few, 0, st);
-            join<T>(c, KEPT, st);
-            hipLaunchKernelGGL(k_again, dim3((unsigned)((p.piece + BLOCK - 1) / BLOCK)), block, 0, st, c);
-            ok &= logits<T, true>(c, p.few, 1, st);
-            join<T>(c, KEPT2, st);
+        hipLaunchKernelGGL(k_clear, dim3(1), dim3(1), 0, st, c.flag);
+        ok &= logits<T, true>(c, p.few, 0, st);
+        join<T>(c, KEPT, st);
+        hipLaunchKernelGGL(k_again, dim3((unsigned)((p.piece + BLOCK - 1) / BLOCK)), block, 0, st, c);
+        ok &= logits<T, true>(c, p.few, 1, st);
+        join<T>(c, KEPT2, st);
+        if constexpr (sizeof(T) == 2) {
+            const int64_t n = p.piece * p.wide / 8, each = NORMS * BLOCK;
+            hipLaunchKernelGGL((k_norm<T>), dim3((unsigned)((n + each - 1) / each)), block, 0, st, c);
         }
         float *const parts = (float *)(mem + p.split);
         const int64_t pitch_e = c.wide * (int64_t)sizeof(T), pitch_h = c.dim_p * (int64_t)sizeof(T);

@@ -175,7 +175,7 @@ def linear_cross_entropy(
 
     Gradients flow to ``hidden``, ``weight`` and ``bias``, once, and backward only.  A loss with
     float16 heads should be scaled, as mixed precision does.  A call needs, beside copies of
-    ``hidden`` and ``weight``, up to 1 GiB of work memory where gradients are wanted, and float32
+    ``hidden`` and ``weight``, up to 1.5 GiB of work memory where gradients are wanted, and float32
     buffers for them until the backward.
     """
     if is_dynamo_compiling():
