@@ -71,8 +71,10 @@ struct Call {
     int32_t *target;          // 16 bits: or -1
     double *sums;             // of logp, one for `few` rows
     int few;                  // rows of a workgroup that joins: 1 or 64
+    int64_t pieces;
+    int normed;               // E becomes G in a pass of its own, and h stands beside it as it is
     // of the piece
-    int32_t *flag;
+    int32_t *flag;            // (of all of them, one behind the other)
     float2 *parts;            // [n_parts][piece]: largest logit and sum of a part of a row
     int n_parts;
     void *e, *hs;             // exponentials; h as it goes beside them
@@ -154,8 +156,13 @@ template <typename T> __global__ __launch_bounds__(BLOCK) void k_rows(const Call
 {
     const int lane = threadIdx.x & 63;
     const int64_t n = c.n_on ? *c.n_on : c.rows;
-    for (int64_t j = (int64_t)blockIdx.x * (BLOCK / 64) + (threadIdx.x >> 6); j < n;
+    for (int64_t k = (int64_t)blockIdx.x * BLOCK + threadIdx.x; k < c.pieces; k += (int64_t)gridDim.x * BLOCK) c.flag[k] = 0;
+    for (int64_t j = (int64_t)blockIdx.x * (BLOCK / 64) + (threadIdx.x >> 6); j < (n + 31) / 32 * 32;
          j += (int64_t)gridDim.x * (BLOCK / 64)) {
+        if (j >= n) {  // the last step of a product over the rows ends with zeros
+            for (int k = lane * 8; k < c.dim_p; k += 64 * 8) *(Eight<T> *)((T *)c.h + j * c.dim_p + k) = Eight<T>{};
+            continue;
+        }
         const int64_t i = c.index ? c.index[j] : j;
         const uint64_t o = (uint64_t)i / (uint64_t)c.inner;
         const T *const x = (const T *)c.hidden + (int64_t)o * c.outer_stride + (i - (int64_t)o * c.inner) * c.inner_stride;
@@ -190,8 +197,6 @@ template <typename T> __global__ __launch_bounds__(BLOCK) void k_rows(const Call
     }
 }
 
-__global__ void k_clear(int32_t *flag) { *flag = 0; }
-
 // out [rows][pitch] = in [rows][n], the rest zero.
 template <typename T>
 __global__ __launch_bounds__(BLOCK) void k_pad(const T *in, int64_t rows, int n, T *out, int pitch)
@@ -206,17 +211,17 @@ __global__ __launch_bounds__(BLOCK) void k_pad(const T *in, int64_t rows, int n,
 
 // The piece's rows of h times inv_h, which the weight's gradient is made of, and zeros up to a whole
 // step (where E has none).  A wave a row.
-template <typename T> __global__ __launch_bounds__(BLOCK) void k_scale(const Call c)
+__global__ __launch_bounds__(BLOCK) void k_scale(const Call c)
 {
     const int rows = rows_of(c), all = (rows + 31) / 32 * 32, lane = threadIdx.x & 63;
     for (int r = blockIdx.x * (BLOCK / 64) + (threadIdx.x >> 6); r < all; r += gridDim.x * (BLOCK / 64)) {
-        const T *const x = (const T *)c.h + (c.first + (r < rows ? r : 0)) * c.dim_p;
-        const float f = sizeof(T) == 2 ? 1.0f : r < rows ? c.inv_h[c.first + r] : 0.0f;
+        const float *const x = (const float *)c.h + (c.first + (r < rows ? r : 0)) * c.dim_p;
+        const float f = r < rows ? c.inv_h[c.first + r] : 0.0f;
         for (int k = lane * 8; k < c.dim_p; k += 64 * 8) {
-            Eight<T> v = *(const Eight<T> *)(x + k);
+            Eight<float> v = *(const Eight<float> *)(x + k);
 #pragma unroll
-            for (int q = 0; q < 8; ++q) v.e[q] = r < rows ? (T)(up(v.e[q]) * f) : (T)0.0f;
-            *(Eight<T> *)((T *)c.hs + (int64_t)r * c.dim_p + k) = v;
+            for (int q = 0; q < 8; ++q) v.e[q] = r < rows ? v.e[q] * f : 0.0f;
+            *(Eight<float> *)((float *)c.hs + (int64_t)r * c.dim_p + k) = v;
         }
     }
 }
@@ -268,7 +273,7 @@ __global__ __launch_bounds__(C::THREADS) void k_logits(const Call c, int nm, int
         for (int i = 0; i < C::TM; ++i)
 #pragma unroll
             for (int r = 0; r < 16; ++r) m = fmaxf(m, t.acc[i][j][r]);  // (a NaN is passed over here and shows in the sum)
-        const float ref = STORE ? c.ref[c.first + (mine ? row : 0)] : (m == -INFINITY ? 0.0f : m);
+        const float ref = STORE ? (again ? c.top : c.ref)[c.first + (mine ? row : 0)] : (m == -INFINITY ? 0.0f : m);
 #pragma unroll
         for (int i = 0; i < C::TM; ++i)
 #pragma unroll
@@ -363,7 +368,7 @@ template <typename T, int ROWS> __global__ __launch_bounds__(BLOCK) void k_join(
     const bool mine = row < rows;
     const int64_t j = c.first + (mine ? row : 0);
     if (blockIdx.x * ROWS >= rows) return;
-    const float ref = c.ref[j], zt = c.z_t[j];
+    const float ref = how == KEPT2 ? c.top[j] : c.ref[j], zt = c.z_t[j];
     float s = 0.0f, m = -INFINITY;
     if (mine) {
         for (int k = w; k < c.n_parts; k += WAYS) {
@@ -399,14 +404,15 @@ template <typename T, int ROWS> __global__ __launch_bounds__(BLOCK) void k_join(
             if (hi - ref > REACH || ref == -INFINITY) *c.flag = 1;
             c.top[j] = hi;
         }
+        if (how == KEPT2 && mine) c.ref[j] = ref;
     }
     const bool none = hi == -INFINITY;  // (no logit above -inf)
     if (none) logp = NAN;
     if (mine && how != SUMS) {
         const int64_t t = c.targets32 ? (int64_t)((const int32_t *)c.targets)[i] : ((const int64_t *)c.targets)[i];
-        if constexpr (sizeof(T) == 4) {
+        if (!c.normed) {
             c.inv[j] = c.inv_h[j] = none ? NAN : weight_of(c) / s;
-            if (t >= 0 && t < c.width) ((T *)c.e)[(int64_t)row * c.wide + t] = exp_of(zt - ref) - s;
+            if (t >= 0 && t < c.width) ((float *)c.e)[(int64_t)row * c.wide + t] = exp_of(zt - ref) - s;
         } else {
             c.inv[j] = weight_of(c) / (1 << KEPT_BITS);
             c.inv_h[j] = none ? NAN : (1 << KEPT_BITS) / s;
@@ -422,20 +428,13 @@ template <typename T, int ROWS> __global__ __launch_bounds__(BLOCK) void k_join(
     }
 }
 
-// What a second pass is relative to.
-__global__ __launch_bounds__(BLOCK) void k_again(const Call c)
-{
-    const int row = blockIdx.x * BLOCK + threadIdx.x;
-    if (*c.flag && row < rows_of(c)) c.ref[c.first + row] = c.top[c.first + row];
-}
-
-// 16 bits: G / weight times 2^KEPT_BITS, in E's place.  A thread takes eight neighbours at a time (a row is
-// of whole steps, so they are of one row), NORMS times, which it asks for ahead.
+// G / weight times 2^KEPT_BITS, in E's place.  A thread takes eight neighbours at a time (a row is of whole
+// steps, so they are of one row), NORMS times, which it asks for ahead.
 constexpr int NORMS = 4;
 template <typename T> __global__ __launch_bounds__(BLOCK) void k_norm(const Call c)
 {
     const uint32_t eights = (uint32_t)(c.wide / 8), n = (uint32_t)rows_of(c) * eights;  // (at most 2^26)
-    struct __attribute__((aligned(16))) Whole { uint16_t e[8]; };
+    struct __attribute__((aligned(16))) Whole { T e[8]; };
     struct __attribute__((aligned(8))) Low { uint8_t e[8]; };
     Whole x[NORMS];
     Low y[NORMS];
@@ -447,7 +446,7 @@ template <typename T> __global__ __launch_bounds__(BLOCK) void k_norm(const Call
         const uint32_t at = first + k * BLOCK;
         if (at >= n) break;
         x[k] = ((const Whole *)c.e)[at];
-        y[k] = ((const Low *)c.low)[at];
+        if constexpr (sizeof(T) == 2) y[k] = ((const Low *)c.low)[at];
         const uint32_t row = at / eights;
         f[k] = c.inv_h[c.first + row];
         t[k] = c.target[c.first + row] - (int32_t)(at - row * eights) * 8;
@@ -456,10 +455,18 @@ template <typename T> __global__ __launch_bounds__(BLOCK) void k_norm(const Call
     for (int k = 0; k < NORMS; ++k) {
         const uint32_t at = first + k * BLOCK;
         if (at >= n) break;
-        struct __attribute__((aligned(16))) { T e[8]; } z;
+        Whole z;
 #pragma unroll
-        for (int q = 0; q < 8; ++q)
-            z.e[q] = (T)(__builtin_bit_cast(float, (uint32_t)x[k].e[q] << 16 | (uint32_t)y[k].e[q] << 8) * f[k]);
+        for (int q = 0; q < 8; ++q) {
+            float p;
+            if constexpr (sizeof(T) == 2) {
+                const uint16_t hi = __builtin_bit_cast(uint16_t, x[k].e[q]);
+                p = __builtin_bit_cast(float, (uint32_t)hi << 16 | (uint32_t)y[k].e[q] << 8);
+            } else {
+                p = x[k].e[q];
+            }
+            z.e[q] = (T)(p * f[k]);
+        }
         if ((uint32_t)t[k] < 8u) {
             const int64_t j = c.first + at / eights;
             const T one = (T)(exp_of(c.z_t[j] - c.ref[j]) * f[k] - (1 << KEPT_BITS));
@@ -467,7 +474,7 @@ template <typename T> __global__ __launch_bounds__(BLOCK) void k_norm(const Call
             for (int q = 0; q < 8; ++q)
                 if (q == t[k]) z.e[q] = one;
         }
-        *(decltype(z) *)((Whole *)c.e + at) = z;
+        ((Whole *)c.e)[at] = z;
     }
 }
 
@@ -500,7 +507,7 @@ struct Share {
 // A step of a tile of 256 x 256 takes some 0.45 us, a tile's sums to memory and back (all chip) 0.1.
 constexpr float SPLIT_COST = 0.25f;  // of a split of one tile, in steps of a round
 
-template <typename C> __device__ __forceinline__ Share share_of(int64_t m, int64_t n, int steps, int places)
+template <typename C> __host__ __device__ __forceinline__ Share share_of(int64_t m, int64_t n, int steps, int places)
 {
     Share s;
     s.nm = (int)((m + C::BM - 1) / C::BM);
@@ -700,10 +707,12 @@ __global__ __launch_bounds__(BLOCK) void k_give(const float *from, T *to, int64_
 // ------------------------------------------------------------------ host
 
 template <typename T> struct Tiles;
-template <> struct Tiles<bf16> { typedef Tile<bf16, 4, 2, 2, 4> Wide; typedef Tile<bf16, 2, 1, 4, 1> Few; };
-template <> struct Tiles<f16> { typedef Tile<f16, 4, 2, 2, 4> Wide; typedef Tile<f16, 2, 1, 4, 1> Few; };
-template <> struct Tiles<float> { typedef Tile<float, 2, 2, 2, 2> Wide; typedef Tile<float, 2, 1, 4, 1> Few; };
+template <> struct Tiles<bf16> { typedef Tile<bf16, 4, 2, 2, 4> Wide; typedef Tile<bf16, 2, 1, 4, 1> Few; typedef Tile<bf16, 2, 2, 1, 4> Thin; };
+template <> struct Tiles<f16> { typedef Tile<f16, 4, 2, 2, 4> Wide; typedef Tile<f16, 2, 1, 4, 1> Few; typedef Tile<f16, 2, 2, 1, 4> Thin; };
+template <> struct Tiles<float> { typedef Tile<float, 2, 2, 2, 2> Wide; typedef Tile<float, 2, 1, 4, 1> Few; typedef Tile<float, 2, 2, 1, 4> Thin; };
 constexpr int FEW = 32;            // rows of a Few tile
+constexpr int THIN_MOST = 64;      // columns of a Thin one
+enum { WIDE, FEWER, THIN };
 constexpr int FEW_JOINED = 2048;   // fewer rows: a workgroup joins the parts of one
 
 int64_t up_to(int64_t n, int64_t k) { return (n + k - 1) / k * k; }
@@ -712,7 +721,9 @@ int64_t up_to(int64_t n, int64_t k) { return (n + k - 1) / k * k; }
 struct Plan {
     int size;                 // bytes of an element
     int64_t dim_p, wide, piece, n_parts;
-    bool few, pad_w, grad;
+    int shape;
+    int64_t pieces;
+    bool pad_w, grad, normed;
     uint64_t index, counts, h, z_t, ref, top, inv, inv_h, target, sums, flag, parts, e, low, hs, w, split, bias, bytes;
 };
 
@@ -728,8 +739,10 @@ Plan plan_of(const swarp_linear_ce_t *a)
     p.grad = dh || dw || a->d_bias;
     p.dim_p = up_to(D, ke);
     p.wide = up_to(V, ke);
-    p.few = N <= FEW;
-    const int64_t bm = p.few || p.size == 2 ? 256 : 128, wm = p.few ? 4 : 2;
+    p.shape = N <= FEW ? FEWER : V <= THIN_MOST ? THIN : WIDE;
+    const int64_t bm = p.shape == THIN ? 64 : p.shape == FEWER || p.size == 2 ? 256 : 128;
+    const int64_t wm = p.shape == THIN ? 1 : p.shape == FEWER ? 4 : 2;
+    p.normed = p.size == 2 || V < D;
     p.n_parts = (V + bm - 1) / bm * wm;
     // (a piece's parts of sums stay below its exponentials)
     int64_t piece = p.grad ? (int64_t)(PIECE / (uint64_t)(p.wide * p.size)) : (int64_t)(PIECE / 8 / (uint64_t)p.n_parts);
@@ -744,22 +757,23 @@ Plan plan_of(const swarp_linear_ce_t *a)
         if (need) at += (bytes + 255) / 256 * 256;
         return here;
     };
-    p.flag = room(true, 4);
+    p.pieces = (N + piece - 1) / piece;
+    p.flag = room(true, 4 * p.pieces);
     p.index = room(a->mask, 4 * N);
     p.counts = room(a->mask, 4 * (N / COUNT_ROWS + 1));
-    p.h = room(true, (uint64_t)N * p.dim_p * p.size);
+    p.h = room(true, (uint64_t)(N + 31) * p.dim_p * p.size);
     p.z_t = room(true, 4 * N);
     p.ref = room(true, 4 * N);
     p.top = room(true, 4 * N);
     p.inv = room(true, 4 * N);
     p.inv_h = room(true, 4 * N);
-    p.target = room(p.grad && p.size == 2, 4 * N);
+    p.target = room(p.grad && p.normed, 4 * N);
     p.sums = room(true, 8 * (N / (piece < FEW_JOINED ? 1 : 64) + 1));
     p.parts = room(true, 8ull * p.n_parts * piece);
     p.w = room(p.pad_w, (uint64_t)V * p.dim_p * p.size);
     p.e = room(p.grad, (uint64_t)piece * p.wide * p.size);
     p.low = room(p.grad && p.size == 2, (uint64_t)piece * p.wide);
-    p.hs = room(dw, (uint64_t)piece * p.dim_p * p.size);
+    p.hs = room(dw && !p.normed, (uint64_t)piece * p.dim_p * p.size);
     // (twice as many splits as places, of whole tiles: share_of)
     p.split = room(dh || dw, p.size == 2 ? 2ull * places(2) * 256 * 256 * 4 : 2ull * places(4) * 128 * 128 * 4);
     p.bias = room(a->d_bias, 4ull * BIAS_WAYS * V);
@@ -781,20 +795,30 @@ template <typename T, typename C, bool STORE> bool logits(const Call &c, int aga
     hipLaunchKernelGGL((k_logits<T, C, STORE>), dim3(nm * nn), dim3(C::THREADS), C::LDS, st, c, nm, nn, again);
     return ok;
 }
-template <typename T, bool STORE> bool logits(const Call &c, bool few, int again, hipStream_t st)
+template <typename T, bool STORE> bool logits(const Call &c, int shape, int again, hipStream_t st)
 {
-    return few ? logits<T, typename Tiles<T>::Few, STORE>(c, again, st)
-               : logits<T, typename Tiles<T>::Wide, STORE>(c, again, st);
+    switch (shape) {
+    case FEWER: return logits<T, typename Tiles<T>::Few, STORE>(c, again, st);
+    case THIN: return logits<T, typename Tiles<T>::Thin, STORE>(c, again, st);
+    default: return logits<T, typename Tiles<T>::Wide, STORE>(c, again, st);
+    }
 }
 
-template <typename T, bool AK> bool product(const Call &c, const Product &p, hipStream_t st)
+template <typename T, typename C, bool AK> bool product(const Call &c, const Product &p, int n, hipStream_t st)
 {
-    typedef typename Tiles<T>::Wide C;
     static const bool ok = lds_limit(k_product<T, C, AK>, C::LDS);
-    const int n = places(sizeof(T));
     hipLaunchKernelGGL((k_product<T, C, AK>), dim3(n), dim3(C::THREADS), C::LDS, st, c, p);
-    hipLaunchKernelGGL((k_splits<C>), dim3(1024), dim3(BLOCK), 0, st, c, p, C::KE, n);
+    const int64_t left = c.rows - c.first, rows = left < c.piece ? left : c.piece;
+    if (c.n_on || share_of<C>(p.rows_m ? rows : p.m, p.n, (int)(((p.rows_k ? rows : p.k) + C::KE - 1) / C::KE), n).splits > 1)
+        hipLaunchKernelGGL((k_splits<C>), dim3(1024), dim3(BLOCK), 0, st, c, p, C::KE, n);
     return ok;
+}
+template <typename T, bool AK> bool product(const Call &c, const Product &p, bool thin, hipStream_t st)
+{
+    if constexpr (AK) {
+        if (thin) return product<T, typename Tiles<T>::Thin, AK>(c, p, 512, st);
+    }
+    return product<T, typename Tiles<T>::Wide, AK>(c, p, places(sizeof(T)), st);
 }
 
 template <typename T> void join(const Call &c, int how, hipStream_t st)
@@ -835,6 +859,8 @@ template <typename T> int run(const swarp_linear_ce_t *a, hipStream_t st)
     c.target = (int32_t *)(mem + p.target);
     c.sums = (double *)(mem + p.sums);
     c.flag = (int32_t *)(mem + p.flag);
+    c.pieces = p.grad ? p.pieces : 0;
+    c.normed = p.normed;
     c.parts = (float2 *)(mem + p.parts);
     c.n_parts = (int)p.n_parts;
     c.few = p.piece < FEW_JOINED ? 1 : 64;
@@ -861,17 +887,16 @@ template <typename T> int run(const swarp_linear_ce_t *a, hipStream_t st)
         c.first = first;
         const dim3 block(BLOCK);
         if (!p.grad) {
-            ok &= logits<T, false>(c, p.few, 0, st);
+            ok &= logits<T, false>(c, p.shape, 0, st);
             join<T>(c, SUMS, st);
             continue;
         }
-        hipLaunchKernelGGL(k_clear, dim3(1), dim3(1), 0, st, c.flag);
-        ok &= logits<T, true>(c, p.few, 0, st);
+        c.flag = (int32_t *)(mem + p.flag) + n;
+        ok &= logits<T, true>(c, p.shape, 0, st);
         join<T>(c, KEPT, st);
-        hipLaunchKernelGGL(k_again, dim3((unsigned)((p.piece + BLOCK - 1) / BLOCK)), block, 0, st, c);
-        ok &= logits<T, true>(c, p.few, 1, st);
+        ok &= logits<T, true>(c, p.shape, 1, st);
         join<T>(c, KEPT2, st);
-        if constexpr (sizeof(T) == 2) {
+        if (c.normed) {
             const int64_t n = p.piece * p.wide / 8, each = NORMS * BLOCK;
             hipLaunchKernelGGL((k_norm<T>), dim3((unsigned)((n + each - 1) / each)), block, 0, st, c);
         }
@@ -880,14 +905,14 @@ template <typename T> int run(const swarp_linear_ce_t *a, hipStream_t st)
         if (a->d_hidden) {
             const Product y = {c.e, c.w, pitch_e, c.pitch_w, p.piece, c.dim, c.width, 1, 0, 0, 1.0f, 0, c.inv + first,
                                a->d_hidden + first * c.dim, parts};
-            ok &= product<T, false>(c, y, st);
+            ok &= product<T, false>(c, y, false, st);
         }
         if (a->d_weight) {
-            hipLaunchKernelGGL((k_scale<T>), dim3(blocks_of(p.piece / 4)), block, 0, st, c);
-            const Product y = {c.e, c.hs, pitch_e, pitch_h, c.width, c.dim, 0, 0, 1, n > 0,
-                               sizeof(T) == 2 ? 1.0f / (1 << KEPT_BITS) : 1.0f, sizeof(T) == 2, nullptr,
-                               a->d_weight, parts};
-            ok &= product<T, true>(c, y, st);
+            if (!c.normed) hipLaunchKernelGGL(k_scale, dim3(blocks_of(p.piece / 4)), block, 0, st, c);
+            const void *const h = c.normed ? (const char *)c.h + first * pitch_h : c.hs;
+            const Product y = {c.e, h, pitch_e, pitch_h, c.width, c.dim, 0, 0, 1, n > 0,
+                               c.normed ? 1.0f / (1 << KEPT_BITS) : 1.0f, c.normed, nullptr, a->d_weight, parts};
+            ok &= product<T, true>(c, y, p.shape == THIN, st);
         }
         if (a->d_bias)
         {

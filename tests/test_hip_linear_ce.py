@@ -94,7 +94,8 @@ def run(h, w, t, b, m, up=1.0, reduction="mean"):
 
 SHAPES = [(1, 1, 1), (1, 16, 2), (3, 5, 7), (32, 64, 31), (33, 32, 256), (64, 100, 257), (257, 33, 300),
           (300, 64, 25), (2560, 64, 9), (1000, 7, 40), (129, 256, 1000), (520, 96, 4099), (16, 520, 9001),
-          (4100, 40, 130), (96, 128, 20000)]
+          (4100, 40, 130), (96, 128, 20000), (300, 129, 33), (601, 200, 22), (2100, 520, 9), (77, 65, 64),
+          (70, 1261, 65)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
