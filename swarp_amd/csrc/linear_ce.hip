@@ -616,7 +616,13 @@ template <typename C> __global__ __launch_bounds__(BLOCK) void k_splits(const Ca
         const int64_t m = (int64_t)tm * C::BM + at / C::BN, n = (int64_t)tn * C::BN + at % C::BN;
         if (m >= M || n >= p.n) continue;
         float y = 0.0f;
-        for (int w = 0; w < s.splits; ++w) y += p.parts[((int64_t)w * s.rest + i) * AREA + at];
+        for (int w0 = 0; w0 < s.splits; w0 += 16) {  // (asked for together: there may be no other wave to wait for)
+            float part[16];
+#pragma unroll
+            for (int w = 0; w < 16; ++w) part[w] = w0 + w < s.splits ? p.parts[((int64_t)(w0 + w) * s.rest + i) * AREA + at] : 0.0f;
+#pragma unroll
+            for (int w = 0; w < 16; ++w) y += part[w];
+        }
         float *const out = p.out + m * p.n + n;
         *out = y * (p.scale ? times * p.scale[m] : times) + (p.add ? *out : 0.0f);
     }
