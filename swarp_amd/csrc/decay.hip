@@ -1174,6 +1174,14 @@ template <typename T> void step(const swarp_decay_t *a, hipStream_t st)
     else if (a->dv <= 64) hipLaunchKernelGGL((k_step<T, 16>), grid, block, 0, st, *a, heads);
     else hipLaunchKernelGGL((k_step<T, 32>), grid, block, 0, st, *a, heads);
 }
+void step_of(const swarp_decay_t *a, hipStream_t st)
+{
+    switch (a->dtype) {
+    case SWARP_F32: return step<float>(a, st);
+    case SWARP_BF16: return step<bf16>(a, st);
+    default: return step<f16>(a, st);
+    }
+}
 
 }  // namespace
 
@@ -1192,6 +1200,12 @@ int swarp_decay_fwd(const swarp_decay_t *a, void *stream)
     if (!a->batch) return 0;
     if (!a->log_decay || (a->steps && (!a->q || !a->k || !a->v || !a->out))) return fail("pointer arguments must be set");
     if (work(a, false)) return -1;
+    // One step is mostly its states: 13487 x 4 heads of 32, float32, 81 us, and 282 as a chunk of one step; 3000
+    // heads of 128, bfloat16, 79 and 132; 200000 of 4, float32, 82 and 1023.
+    if (a->steps == 1 && a->state_out && a->dv % 4 == 0) {
+        step_of(a, (hipStream_t)stream);
+        return launched();
+    }
     Call c = call_of(a, false);
     Scan &s = c.scan[0];
     s.q = a->q;
@@ -1289,12 +1303,7 @@ int swarp_decay_step(const swarp_decay_t *a, void *stream)
     };
     if (!apart(a->q, a->q_stride, a->dk) || !apart(a->k, a->k_stride, a->dk) || !apart(a->v, a->v_stride, a->dv))
         return fail("q, k and v must not lie in the state");
-    hipStream_t st = (hipStream_t)stream;
-    switch (a->dtype) {
-    case SWARP_F32: step<float>(a, st); break;
-    case SWARP_BF16: step<bf16>(a, st); break;
-    default: step<f16>(a, st); break;
-    }
+    step_of(a, (hipStream_t)stream);
     return launched();
 }
 
