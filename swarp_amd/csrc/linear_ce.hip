@@ -27,6 +27,8 @@
 // first, and every kernel goes by their number on the device.
 #include <math.h>
 
+#include <atomic>
+
 #include "matrix.hpp"
 #include "narrow_ce.hpp"
 
@@ -428,6 +430,17 @@ template <typename T, int ROWS> __global__ __launch_bounds__(BLOCK) void k_join(
     }
 }
 
+// An exponential as it is kept, and G / weight times 2^KEPT_BITS at row j's target (f: of its exponentials).
+__device__ __forceinline__ float exponential(float e, uint8_t) { return e; }
+template <typename T> __device__ __forceinline__ float exponential(T e, uint8_t low)
+{
+    return __builtin_bit_cast(float, (uint32_t)__builtin_bit_cast(uint16_t, e) << 16 | (uint32_t)low << 8);
+}
+__device__ __forceinline__ float one_of(const Call &c, int64_t j, float f)
+{
+    return exp_of(c.z_t[j] - c.ref[j]) * f - (1 << KEPT_BITS);
+}
+
 // G / weight times 2^KEPT_BITS, in E's place.  A thread takes eight neighbours at a time (a row is of whole
 // steps, so they are of one row), NORMS times, which it asks for ahead.
 constexpr int NORMS = 4;
@@ -457,19 +470,9 @@ template <typename T> __global__ __launch_bounds__(BLOCK) void k_norm(const Call
         if (at >= n) break;
         Whole z;
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
-            float p;
-            if constexpr (sizeof(T) == 2) {
-                const uint16_t hi = __builtin_bit_cast(uint16_t, x[k].e[q]);
-                p = __builtin_bit_cast(float, (uint32_t)hi << 16 | (uint32_t)y[k].e[q] << 8);
-            } else {
-                p = x[k].e[q];
-            }
-            z.e[q] = (T)(p * f[k]);
-        }
+        for (int q = 0; q < 8; ++q) z.e[q] = (T)(exponential(x[k].e[q], y[k].e[q]) * f[k]);
         if ((uint32_t)t[k] < 8u) {
-            const int64_t j = c.first + at / eights;
-            const T one = (T)(exp_of(c.z_t[j] - c.ref[j]) * f[k] - (1 << KEPT_BITS));
+            const T one = (T)one_of(c, c.first + at / eights, f[k]);
 #pragma unroll
             for (int q = 0; q < 8; ++q)
                 if (q == t[k]) z.e[q] = one;
@@ -628,7 +631,8 @@ template <typename C> __global__ __launch_bounds__(BLOCK) void k_splits(const Ca
     }
 }
 
-// d b = sum_i inv_i E_ij: a workgroup takes 64 lanes' 16 bytes of columns and one of BIAS_WAYS shares of
+// d b = sum_i inv_i E_ij, from E before it is rounded: where an action is as often right as it is likely the
+// sum is small beside its terms.  A workgroup takes 64 lanes' 16 bytes of columns and one of BIAS_WAYS shares of
 // the rows, its waves every fourth of these; the shares are added by k_bias_sum.
 constexpr int BIAS_WAYS = 32;
 
@@ -636,6 +640,7 @@ template <typename T> __global__ __launch_bounds__(BLOCK) void k_bias(const Call
 {
     constexpr int V = 16 / sizeof(T);
     struct __align__(16) Line { T e[V]; };
+    struct __align__(V) Low { uint8_t e[V]; };
     __shared__ float red[4][64 * V];
     const int rows = rows_of(c), lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int each = (rows + BIAS_WAYS - 1) / BIAS_WAYS, first = each * blockIdx.y, last = first + each < rows ? first + each : rows;
@@ -643,10 +648,15 @@ template <typename T> __global__ __launch_bounds__(BLOCK) void k_bias(const Call
     float s[V] = {};
     if (v < c.wide)
         for (int r = first + w; r < last; r += 4) {
-            const Line y = *(const Line *)((const T *)c.e + (int64_t)r * c.wide + v);
-            const float f = c.inv[c.first + r];
+            const int64_t j = c.first + r, at = (int64_t)r * c.wide + v;
+            const Line y = *(const Line *)((const T *)c.e + at);
+            Low low = {};
+            if constexpr (sizeof(T) == 2) low = *(const Low *)(c.low + at);
+            const float inv = c.inv[j], f = c.normed ? c.inv_h[j] : 1.0f;
+            const float one = c.normed ? one_of(c, j, f) : 0.0f;
+            const int64_t t = c.normed ? c.target[j] - v : -1;
 #pragma unroll
-            for (int k = 0; k < V; ++k) s[k] = __builtin_fmaf(f, up(y.e[k]), s[k]);
+            for (int k = 0; k < V; ++k) s[k] = __builtin_fmaf(inv, k == t ? one : exponential(y.e[k], low.e[k]) * f, s[k]);
         }
 #pragma unroll
     for (int k = 0; k < V; ++k) red[w][lane * V + k] = s[k];
@@ -789,14 +799,22 @@ Plan plan_of(const swarp_linear_ce_t *a)
 
 int blocks_of(int64_t n) { return (int)(n < 1 ? 1 : n > 4096 ? 4096 : n); }
 
-template <typename K> bool lds_limit(K kernel, int bytes)
+// A kernel may have more LDS than a launch without asking gives; once a device.
+bool lds_limit(const void *kernel, int bytes, std::atomic<uint64_t> &done)
 {
-    return hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess;
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess) return false;
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (done.load(std::memory_order_relaxed) & bit) return true;
+    if (hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess) return false;
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return true;
 }
 
 template <typename T, typename C, bool STORE> bool logits(const Call &c, int again, hipStream_t st)
 {
-    static const bool ok = lds_limit(k_logits<T, C, STORE>, C::LDS);
+    static std::atomic<uint64_t> done{0};
+    const bool ok = lds_limit((const void *)k_logits<T, C, STORE>, C::LDS, done);
     const int nm = (c.width + C::BM - 1) / C::BM, nn = (c.piece + C::BN - 1) / C::BN;
     hipLaunchKernelGGL((k_logits<T, C, STORE>), dim3(nm * nn), dim3(C::THREADS), C::LDS, st, c, nm, nn, again);
     return ok;
@@ -812,7 +830,8 @@ template <typename T, bool STORE> bool logits(const Call &c, int shape, int agai
 
 template <typename T, typename C, bool AK> bool product(const Call &c, const Product &p, int n, hipStream_t st)
 {
-    static const bool ok = lds_limit(k_product<T, C, AK>, C::LDS);
+    static std::atomic<uint64_t> done{0};
+    const bool ok = lds_limit((const void *)k_product<T, C, AK>, C::LDS, done);
     hipLaunchKernelGGL((k_product<T, C, AK>), dim3(n), dim3(C::THREADS), C::LDS, st, c, p);
     const int64_t left = c.rows - c.first, rows = left < c.piece ? left : c.piece;
     if (c.n_on || share_of<C>(p.rows_m ? rows : p.m, p.n, (int)(((p.rows_k ? rows : p.k) + C::KE - 1) / C::KE), n).splits > 1)
@@ -902,6 +921,12 @@ template <typename T> int run(const swarp_linear_ce_t *a, hipStream_t st)
         join<T>(c, KEPT, st);
         ok &= logits<T, true>(c, p.shape, 1, st);
         join<T>(c, KEPT2, st);
+        if (a->d_bias) {
+            float *const sums = (float *)(mem + p.bias);
+            const int per = 64 * 16 / sizeof(T);
+            hipLaunchKernelGGL((k_bias<T>), dim3((c.width + per - 1) / per, BIAS_WAYS), block, 0, st, c, sums);
+            hipLaunchKernelGGL(k_bias_sum, dim3((c.width + BLOCK - 1) / BLOCK), block, 0, st, c.width, sums, a->d_bias, (int)(n > 0));
+        }
         if (c.normed) {
             const int64_t n = p.piece * p.wide / 8, each = NORMS * BLOCK;
             hipLaunchKernelGGL((k_norm<T>), dim3((unsigned)((n + each - 1) / each)), block, 0, st, c);
@@ -919,13 +944,6 @@ template <typename T> int run(const swarp_linear_ce_t *a, hipStream_t st)
             const Product y = {c.e, h, pitch_e, pitch_h, c.width, c.dim, 0, 0, 1, n > 0,
                                c.normed ? 1.0f / (1 << KEPT_BITS) : 1.0f, c.normed, nullptr, a->d_weight, parts};
             ok &= product<T, true>(c, y, p.shape == THIN, st);
-        }
-        if (a->d_bias)
-        {
-            float *const sums = (float *)(mem + p.bias);
-            const int per = 64 * 16 / sizeof(T);
-            hipLaunchKernelGGL((k_bias<T>), dim3((c.width + per - 1) / per, BIAS_WAYS), block, 0, st, c, sums);
-            hipLaunchKernelGGL(k_bias_sum, dim3((c.width + BLOCK - 1) / BLOCK), block, 0, st, c.width, sums, a->d_bias, (int)(n > 0));
         }
     }
     hipLaunchKernelGGL(k_loss, dim3(1), dim3(BLOCK), 0, st, c);

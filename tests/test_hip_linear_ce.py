@@ -187,6 +187,21 @@ def test_closed_actions_and_far_targets(dtype):
     close(got["hidden"], want["hidden"], "hidden")
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,D,V", [(3, 583, 3), (3, 64, 3), (400, 130, 2), (4000, 40, 100)])
+def test_the_bias_gradient_is_summed_before_it_is_rounded(rows, D, V, dtype):
+    """Its terms cancel: their rounding to the type would be most of it.  Only the logits' own error and
+    the end's rounding are left, so the type's half step counts once, relative to the sum."""
+    h, w, t, b, m = inputs(rows, D, V, dtype, rows + V)
+    up = 1024.0 if dtype == torch.float16 else 1.0
+    value, tol = reference(h, w, t, b, m, up)["bias"]
+    p = torch.softmax(h.double() @ w.double().t() + b.double(), -1)
+    mag = (p + torch.nn.functional.one_hot(t, V)).sum(0) * up / rows
+    # (24 bits of an exponential are kept: 2^-17 of a half step, where the tolerance above has u)
+    tol = tol - mag * (1.01 * half(dtype) - 2.0 ** -16)
+    close(run(h, w, t, b, m, up)["bias"], (value, tol), "bias")
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("rows,D,V", [(40, 64, 25), (300, 64, 300), (20, 64, 300)])
 def test_a_row_of_the_lowest_biases(rows, D, V, dtype):
