@@ -361,7 +361,7 @@ enum { SUMS = 0,     // from parts relative to their largest: logp
 // A workgroup takes ROWS rows, its threads every (BLOCK / ROWS)-th part of one.
 template <typename T, int ROWS> __global__ __launch_bounds__(BLOCK) void k_join(const Call c, int how)
 {
-    constexpr int WAYS = BLOCK / ROWS;
+    constexpr int WAYS = BLOCK / ROWS, AHEAD = 8;
     __shared__ float red[2][WAYS][ROWS];
     __shared__ double total[ROWS];
     if (how == KEPT2 && !*c.flag) return;
@@ -373,16 +373,23 @@ template <typename T, int ROWS> __global__ __launch_bounds__(BLOCK) void k_join(
     const float ref = how == KEPT2 ? c.top[j] : c.ref[j], zt = c.z_t[j];
     float s = 0.0f, m = -INFINITY;
     if (mine) {
-        for (int k = w; k < c.n_parts; k += WAYS) {
-            const float2 p = c.parts[(int64_t)k * c.piece + row];
-            if (how == SUMS) {
-                const float hi = p.x > m ? p.x : m, at = hi == -INFINITY ? 0.0f : hi;
-                s = s * (m == -INFINITY ? 1.0f : exp_of(m - at)) + p.y * (p.x == -INFINITY ? 1.0f : exp_of(p.x - at));
-                m = hi;
-            } else {
-                s += p.y;
-                m = p.x > m ? p.x : m;
+        // (asked for together: a row's parts are few enough that latency is all of this)
+        for (int k0 = w; k0 < c.n_parts; k0 += AHEAD * WAYS) {
+            float2 p[AHEAD];
+#pragma unroll
+            for (int q = 0; q < AHEAD; ++q) {
+                const int k = k0 + q * WAYS;
+                p[q] = k < c.n_parts ? c.parts[(int64_t)k * c.piece + row] : make_float2(-INFINITY, 0.0f);
             }
+            float hi = m;
+#pragma unroll
+            for (int q = 0; q < AHEAD; ++q) hi = p[q].x > hi ? p[q].x : hi;
+            const float at = hi == -INFINITY ? 0.0f : hi;
+            if (how == SUMS) s *= m == -INFINITY ? 1.0f : exp_of(m - at);
+#pragma unroll
+            for (int q = 0; q < AHEAD; ++q)
+                s += how == SUMS ? p[q].y * (p[q].x == -INFINITY ? 1.0f : exp_of(p[q].x - at)) : p[q].y;
+            m = hi;
         }
     }
     red[0][w][lane] = m;
