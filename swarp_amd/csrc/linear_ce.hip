@@ -362,6 +362,7 @@ enum { SUMS = 0,     // from parts relative to their largest: logp
 template <typename T, int ROWS> __global__ __launch_bounds__(BLOCK) void k_join(const Call c, int how)
 {
     constexpr int WAYS = BLOCK / ROWS, AHEAD = 8;
+    auto of = [](float part, float all) { return part == -INFINITY ? 1.0f : exp_of(part - all); };
     __shared__ float red[2][WAYS][ROWS];
     __shared__ double total[ROWS];
     if (how == KEPT2 && !*c.flag) return;
@@ -385,23 +386,30 @@ template <typename T, int ROWS> __global__ __launch_bounds__(BLOCK) void k_join(
 #pragma unroll
             for (int q = 0; q < AHEAD; ++q) hi = p[q].x > hi ? p[q].x : hi;
             const float at = hi == -INFINITY ? 0.0f : hi;
-            if (how == SUMS) s *= m == -INFINITY ? 1.0f : exp_of(m - at);
+            if (how == SUMS) s *= of(m, at);
 #pragma unroll
             for (int q = 0; q < AHEAD; ++q)
-                s += how == SUMS ? p[q].y * (p[q].x == -INFINITY ? 1.0f : exp_of(p[q].x - at)) : p[q].y;
+                s += how == SUMS ? p[q].y * of(p[q].x, at) : p[q].y;
             m = hi;
         }
     }
     red[0][w][lane] = m;
     red[1][w][lane] = s;
     __syncthreads();
-    if (w) return;
     float hi = m;
-    for (int k = 1; k < WAYS; ++k) hi = red[0][k][lane] > hi ? red[0][k][lane] : hi;
-    s = 0.0f;
-    for (int k = 0; k < WAYS; ++k) {
-        const float mk = red[0][k][lane];
-        s += red[1][k][lane] * (how == SUMS && mk != -INFINITY ? exp_of(mk - hi) : 1.0f);
+    if constexpr (ROWS == 1) {
+        if (w >= 64) return;
+        for (int k = w + 64; k < WAYS; k += 64) hi = red[0][k][0] > hi ? red[0][k][0] : hi;
+        hi = learn::wave_max(hi);
+        s = 0.0f;
+        for (int k = w; k < WAYS; k += 64) s += red[1][k][0] * (how == SUMS ? of(red[0][k][0], hi) : 1.0f);
+        s = wave_sum(s);
+        if (w) return;
+    } else {
+        if (w) return;
+        for (int k = 1; k < WAYS; ++k) hi = red[0][k][lane] > hi ? red[0][k][lane] : hi;
+        s = 0.0f;
+        for (int k = 0; k < WAYS; ++k) s += red[1][k][lane] * (how == SUMS ? of(red[0][k][lane], hi) : 1.0f);
     }
     const int64_t i = c.index ? c.index[j] : j;
     float logp;
