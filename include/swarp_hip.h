@@ -544,7 +544,7 @@ int swarp_grad_norm(const swarp_tensor_t *tensors, int32_t n_tensors, double max
  * gradient of 1.  A head whose weight a workgroup's LDS holds (swarp_linear_ce_complete) is done in
  * one kernel, and they are complete, of `dtype`.  Else they are float, d_hidden with the rows that
  * count moved together; the work memory then holds the exponentials of at most 1 GiB of rows (or of
- * 256 rows) at a time, copies of hidden and, where its rows are not whole steps of 64 bytes, weight. */
+ * 256 rows; half as much again of 16-bit heads) at a time, copies of hidden and, where its rows are not whole steps of 64 bytes, weight. */
 typedef struct swarp_linear_ce {
     int32_t dtype;            /* of hidden, weight, bias: SWARP_F32, _BF16 or _F16 */
     int32_t sum;              /* 1: loss is the sum, 0: the mean */

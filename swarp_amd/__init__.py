@@ -8,7 +8,9 @@ PyTorch-facing host side with the reference's API (``Stepper``, ``TorchState``,
 ``World`` / ``Environment`` / ``make("navigation", ...)`` surface that calls the step).
 
 Beside the step stand the operators a policy is trained with on it: ``gae``,
-``categorical_policy_loss``, ``gaussian_policy_loss`` and ``AdamW``.
+``categorical_policy_loss``, ``gaussian_policy_loss`` and ``AdamW``; ``linear_cross_entropy``, the loss
+of a wide head or of imitation; and a policy's memory along an episode, ``decay_attention`` over a
+rollout and ``decay_attention_step`` while it acts.
 """
 
 from .autograd import GradRing, StepGradSlot, TorchState, fill_state_defaults, rollout, warp_step

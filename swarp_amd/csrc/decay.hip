@@ -14,7 +14,7 @@
 //   dv_i = scale sum_{t >= i} lambda^(t-i) (k_i q_t) do_t + ...     backwards, (k, q, do), state dS
 // so that one kernel does all four; below, q, k and v are a scan's own parts.
 //
-// Where there are few heads the steps are cut into segments: one kernel finds the state that each
+// Where there are fewer heads than SIMDs the steps are cut into segments: one kernel finds the state that each
 // would end with if none entered, a second joins them, a third does the segments, each from its state.
 #include <math.h>
 
@@ -263,6 +263,9 @@ __device__ __forceinline__ void chunk(Kept<KT> &w, const Powers &f, const Part<T
 // state's columns stay in its registers; KT: 32s of dk.  A wave works alone: its part of the LDS
 // holds the chunk's rows of k and v, to be read as columns.  The next chunk's rows (the next entry's
 // first ones) are on their way meanwhile.
+// What bounds it is one wave's chain through a chunk (rows to LDS, scores, output, state: some 40 products of
+// 32 x 32 x 16 behind one another, two waves a SIMD): 4095 steps of 384 heads of 64, bfloat16, forward and
+// backward 1.22 ms, 0.4 of it bytes; 1023 steps of 256 heads of 40 x 72, float32, 0.77 ms, 0.13 of it bytes.
 template <typename T, int KT, int WHAT, int FIT>
 __global__ __launch_bounds__(BLOCK, (KT + (WHAT == OUTPUTS)) * sizeof(T) < 10 ? 2 : 1) void k_alone(const Call c)
 {
@@ -400,6 +403,7 @@ __global__ __launch_bounds__(BLOCK, (KT + (WHAT == OUTPUTS)) * sizeof(T) < 10 ? 
 // few rows of many bytes.  (A rollout's steps are far apart: 32
 // rows a load are 32 pages, and translations then cost more than the bytes.)  Its outputs leave the
 // same way.  The next chunk's rows, or the next heads' first ones, are on their way meanwhile.
+// 32 steps of 512000 heads of 32, bfloat16: 6.3 GB in 1.5 ms, 4.2 TB/s.
 template <typename T, int WHAT, int FIT>
 __global__ __launch_bounds__(BLOCK, 2) void k_together(const Call c)
 {
@@ -573,6 +577,8 @@ __global__ __launch_bounds__(BLOCK, 2) void k_together(const Call c)
 //   d S0 = lambda^T Z + sum_t lambda^(t+1) q_t do_t^T.
 // dP is formed twice, with a lane's step that of dq and that of dk: either way it is the next product's
 // operand as it lies.
+// 32 steps of 512000 heads of 32, bfloat16: 1.74 ms for 7.3 GB; as three scans it was 3.1 ms for twice the bytes.
+// Bounds: the bytes, then what two waves a SIMD leave uncovered of the way from LDS to the products.
 template <typename T, int FIT> __global__ __launch_bounds__(BLOCK, 2) void k_short(const Call c, const Scan sq, const Scan sk, const Scan sv)
 {
     constexpr int PAD = 16 / (int)sizeof(T), P = 32 + PAD, ROOM = WAVES * 32 * P, EACH = 2;
@@ -889,7 +895,8 @@ __global__ __launch_bounds__(BLOCK) void k_between(const Call c, int64_t n)
 }
 
 // One step: the state is read and written once, which is all that counts.  A wave a head; a lane has
-// four columns of every (64 / LANES)-th row, LANES of them a row.
+// four columns of every (64 / LANES)-th row, LANES of them a row.  512000 heads of 32, bfloat16: 4.3 GB in
+// 0.81 ms, 5.4 TB/s (half of it written: above the rate of a copy).  Few heads: 4.5 us, a launch.
 template <typename T, int LANES> __global__ __launch_bounds__(BLOCK) void k_step(const swarp_decay_t a, int64_t heads)
 {
     constexpr int ROWS = 64 / LANES, AHEAD = 4;  // rows of a wave at once, and how many times that are under way
