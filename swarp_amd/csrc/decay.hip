@@ -901,9 +901,12 @@ template <typename T, int LANES> __global__ __launch_bounds__(BLOCK) void k_step
 {
     constexpr int ROWS = 64 / LANES, AHEAD = 4;  // rows of a wave at once, and how many times that are under way
     struct __attribute__((packed, aligned(4))) Four { float e[4]; };
-    const int lane = threadIdx.x & 63, i0 = lane / LANES, j = lane % LANES * 4;
+    const int lane = threadIdx.x & 63, i0 = lane / LANES, j4 = lane % LANES * 4;
     const int dk = a.dk, dv = a.dv;
-    const bool mine = j < dv;
+    const bool mine = j4 < dv;
+    // (the last four columns overlap those before them: a wave has read all of a row before it writes it, and
+    // writes the same there twice)
+    const int j = j4 < dv - 4 ? j4 : dv - 4;
     const int64_t step = (int64_t)gridDim.x * WAVES;
     for (int64_t bh = (int64_t)blockIdx.x * WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); bh < heads; bh += step) {
         const int64_t b = (uint32_t)bh / (uint32_t)a.heads;  // (at most 2^31 heads)
@@ -916,7 +919,7 @@ template <typename T, int LANES> __global__ __launch_bounds__(BLOCK) void k_step
         const float q0 = (float)q[l0], q1 = (float)q[l1], k0 = (float)k[l0], k1 = (float)k[l1];
         float vj[4], o[4] = {};
 #pragma unroll
-        for (int c = 0; c < 4; ++c) vj[c] = mine && j + c < dv ? (float)v[j + c] : 0.0f;
+        for (int c = 0; c < 4; ++c) vj[c] = mine ? (float)v[j + c] : 0.0f;
         const bool fresh = !a.state || (a.starts && a.starts[(uint32_t)b / (uint32_t)a.group]);
         const float lambda = __builtin_amdgcn_exp2f(a.log_decay[h] * LOG2E);
         const float *const from = a.state + bh * dk * dv + j;
@@ -957,13 +960,13 @@ template <typename T, int LANES> __global__ __launch_bounds__(BLOCK) void k_step
         if (i0 == 0 && mine) {
             T *const y = (T *)a.out + bh * dv + j;
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
-                if (j + c < dv) y[c] = (T)(o[c] * (float)a.scale);
+            for (int c = 0; c < 4; ++c) y[c] = (T)(o[c] * (float)a.scale);
         }
     }
 }
 
 // The same where dv is no multiple of four: a thread a column of v, all of dk in turn.
+// Few columns, not four: a thread one of them.
 template <typename T> __global__ __launch_bounds__(BLOCK) void k_step_any(const swarp_decay_t a, int64_t n)
 {
     for (int64_t x = (int64_t)blockIdx.x * BLOCK + threadIdx.x; x < n; x += (int64_t)gridDim.x * BLOCK) {
@@ -1173,7 +1176,8 @@ template <typename T> void step(const swarp_decay_t *a, hipStream_t st)
     const int64_t heads = a->batch * a->heads, n = heads * a->dv;
     auto blocks = [](int64_t n, int64_t each) { return dim3((unsigned)((n + each - 1) / each < 16384 ? (n + each - 1) / each : 16384)); };
     const dim3 grid = blocks(heads, WAVES), block(BLOCK);
-    if (a->dv % 4) hipLaunchKernelGGL((k_step_any<T>), blocks(n, BLOCK), block, 0, st, *a, n);
+    // (25068 heads of 112 x 86, bfloat16: 402 us, a thread a column 901; 100000 of 16 x 5, float32: 51 and 43)
+    if (a->dv < 6 && a->dv != 4) hipLaunchKernelGGL((k_step_any<T>), blocks(n, BLOCK), block, 0, st, *a, n);
     else if (a->dv <= 4) hipLaunchKernelGGL((k_step<T, 1>), grid, block, 0, st, *a, heads);
     else if (a->dv <= 8) hipLaunchKernelGGL((k_step<T, 2>), grid, block, 0, st, *a, heads);
     else if (a->dv <= 16) hipLaunchKernelGGL((k_step<T, 4>), grid, block, 0, st, *a, heads);
@@ -1209,7 +1213,7 @@ int swarp_decay_fwd(const swarp_decay_t *a, void *stream)
     if (work(a, false)) return -1;
     // One step is mostly its states: 13487 x 4 heads of 32, float32, 81 us, and 282 as a chunk of one step; 3000
     // heads of 128, bfloat16, 79 and 132; 200000 of 4, float32, 82 and 1023.
-    if (a->steps == 1 && a->state_out && a->dv % 4 == 0) {
+    if (a->steps == 1 && a->state_out && a->dv >= 4) {
         step_of(a, (hipStream_t)stream);
         return launched();
     }

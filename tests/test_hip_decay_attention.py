@@ -208,7 +208,8 @@ def test_step_equals_scan(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("batch,H,dk,dv", [((), 1, 1, 1), ((1,), 3, 128, 128), ((7,), 2, 64, 64), ((300,), 2, 32, 32), ((9,), 1, 17, 130 - 3), ((1000,), 1, 4, 4)])
+@pytest.mark.parametrize("batch,H,dk,dv", [((), 1, 1, 1), ((1,), 3, 128, 128), ((7,), 2, 64, 64), ((300,), 2, 32, 32), ((9,), 1, 17, 130 - 3), ((1000,), 1, 4, 4),
+                                           ((40,), 3, 33, 5), ((41,), 2, 65, 6), ((70,), 2, 32, 31), ((5, 3), 2, 9, 66)])
 def test_step(batch, H, dk, dv, dtype):
     q, k, v, ld, state, s = inputs(1, batch, H, dk, dv, dtype, dk + dv, 0.3)
     mine = state.clone()
