@@ -249,6 +249,23 @@ def test_strides(dtype):
         assert torch.equal(o1, decay_attention_step(*(t[0] for t in plain), ld, S2)) and torch.equal(S1, S2)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dk,dv", [(32, 32), (17, 31), (8, 3)])
+def test_a_scan_of_one_step(dk, dv, dtype):
+    """What a started episode's state held is not looked at; the state that was given stays."""
+    q, k, v, ld, state, s = inputs(1, (40, 3), 2, dk, dv, dtype, 45, 0.5)
+    s = s[..., 0]  # an env's, shared by its agents
+    want = both(q, k, v, ld, state, s, v * 0, state * 0, 0.7)
+    dirty = torch.where(s[0].view(40, 1, 1, 1, 1), math.nan, state)
+    kept = dirty.clone()
+    got = decay_attention(q, k, v, ld, dirty, s, scale=0.7)
+    check([got.out, got.state], want[:2], 1, dk, dv, dtype, "one step")
+    assert torch.equal(dirty.nan_to_num(7.0), kept.nan_to_num(7.0))
+    now = dirty.clone()
+    out = decay_attention_step(q[0], k[0], v[0], ld, now, s[0], scale=0.7)
+    check([out[None], now], want[:2], 1, dk, dv, dtype, "step")
+
+
 def test_step_under_inference_mode():
     q, k, v, ld, state, s = inputs(1, (3,), 2, 8, 8, torch.float32, 44, 0.3)
     want = decay_attention(q, k, v, ld, state, s)

@@ -286,6 +286,60 @@ def test_more_rows_than_a_piece_holds():
     close(got["weight"], (dw, mag * (2 * 2.0 ** -8 * 1.01 + 1e-5) + 2.0 ** -8 * dw.abs() + 1e-30), "weight")
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("far", [5, 600])
+def test_one_piece_of_several_starts_from_elsewhere(dtype, far):
+    """2^20 logits a row: 512 rows a piece of 16 bits, 256 of float32.  One row's target is e^-400."""
+    V, rows = 1 << 20, 601
+    h, w, t, b, _ = inputs(rows, 4, V, dtype, 9, spread=1.0)
+    t = torch.where(t == 77, 78, t)
+    t[far] = 77
+    b[77] = -400.0
+    got = run(h, w, t, b, None, reduction="sum")
+    u = half(dtype)
+    for part in (torch.arange(0, 30, device=DEV), torch.arange(590, rows, device=DEV)):
+        z = h[part].double() @ w.double().t() + b.double()
+        p = torch.softmax(z, -1)
+        one = torch.nn.functional.one_hot(t[part], V).double()
+        logp = torch.log_softmax(z, -1).gather(-1, t[part][:, None])[:, 0]
+        # (32 of the sum and the hardware's functions, 6 + 4 of a logit below 2^6, as above; 2^-24 of 400)
+        assert float((got["logp"][part] - logp).abs().max()) < 1e-4
+        dh, mag = (p - one) @ w.double(), (p + one) @ w.double().abs()
+        close(got["hidden"][part], (dh, mag * (1.01 * u + 1e-5) + (u + 4 * F24) * dh.abs() + 1e-30), "hidden")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,D,V", [(300, 64, 25), (20, 64, 300), (300, 200, 22), (260, 40, 300)])
+def test_graphs_of_every_shape(rows, D, V, dtype):
+    """Two graphs at once, each replayed three times with eager calls between."""
+    def one(seed):
+        h, w, t, b, m = inputs(rows, D, V, dtype, seed, True, 0.3)
+        x = [y.detach().clone().requires_grad_(True) for y in (h, w, b)]
+        run(h, w, t, b, m)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            r = linear_cross_entropy(x[0], x[1], t, x[2], m)
+            grads = torch.autograd.grad(r.loss, x)
+        return graph, x, t, m, r, grads
+    made = [one(60), one(61)]
+    for seed in (1, 2, 3):
+        new = []
+        for n, (graph, x, t, m, r, grads) in enumerate(made):
+            h2, _, t2, _, m2 = inputs(rows, D, V, dtype, 70 + 2 * seed + n, True, 0.25 * seed)
+            with torch.no_grad():
+                x[0].copy_(h2)
+                t.copy_(t2)
+                m.copy_(m2)
+            new.append((h2, t2, m2))
+        for graph, *_ in made:
+            graph.replay()
+        for (graph, x, t, m, r, grads), (h2, t2, m2) in zip(made, new):
+            want = run(h2, x[1].detach(), t2, x[2].detach(), m2)
+            assert torch.equal(r.loss, want["loss"]) and torch.equal(r.logp, want["logp"])
+            assert all(torch.equal(y, want[k]) for y, k in zip(grads, ("hidden", "weight", "bias")))
+
+
 def test_only_what_is_wanted():
     h, w, t, b, _ = inputs(90, 33, 70, torch.bfloat16, 6)
     full = run(h, w, t, b, None)
