@@ -384,7 +384,7 @@ __global__ __launch_bounds__(BLOCK, (KT + (WHAT == OUTPUTS)) * sizeof(T) < 10 ? 
 #pragma unroll
                     for (int r = 0; r < 8; ++r) e.e[r] = (T)o[8 * x + r];
                     if (FIT == FULL || (FIT == EIGHTS ? n > 0 : n >= 8)) *(Span<T, 8> *)(op + 16 * x) = e;
-                    else if constexpr (FIT == ANY) {
+                    else if constexpr (FIT <= ANY) {
 #pragma unroll
                         for (int r = 0; r < 8; ++r)
                             if (r < n) op[16 * x + r] = e.e[r];
@@ -547,7 +547,7 @@ __global__ __launch_bounds__(BLOCK, 2) void k_together(const Call c)
                     T *const to = ob[n] + way * (c0 - begin) * s.os[0];
                     const int left = dv - z.at;
                     if (FIT == FULL || (FIT == EIGHTS ? left > 0 : left >= 8)) *(Span<T, 8> *)to = e;
-                    else if constexpr (FIT == ANY) {
+                    else if constexpr (FIT <= ANY) {
 #pragma unroll
                         for (int r = 0; r < 8; ++r)
                             if (r < left) to[r] = e.e[r];
@@ -802,7 +802,7 @@ template <typename T, int FIT> __global__ __launch_bounds__(BLOCK, 2) void k_sho
                 T *const y = (T *)to[k].p + row * to[k].st[0] + b * to[k].st[1] + (line - b * (uint32_t)c.heads) * to[k].st[2] + at;
                 const int left = to[k].n - at;
                 if (FIT == FULL || (FIT == EIGHTS ? left > 0 : left >= 8)) *(Span<T, 8> *)y = e;
-                else if constexpr (FIT == ANY) {
+                else if constexpr (FIT <= ANY) {
 #pragma unroll
                     for (int r = 0; r < 8; ++r)
                         if (r < left) y[r] = e.e[r];
@@ -1053,7 +1053,8 @@ template <typename T, int KT, int WHAT> void alone(Call &c, int fit, hipStream_t
     const dim3 grid((unsigned)((c.spans * kinds + WAVES - 1) / WAVES));
     if (fit == FULL) hipLaunchKernelGGL((k_alone<T, KT, WHAT, FULL>), grid, dim3(BLOCK), 0, st, c);
     else if (fit == EIGHTS) hipLaunchKernelGGL((k_alone<T, KT, WHAT, EIGHTS>), grid, dim3(BLOCK), 0, st, c);
-    else hipLaunchKernelGGL((k_alone<T, KT, WHAT, ANY>), grid, dim3(BLOCK), 0, st, c);
+    else if (fit == ANY) hipLaunchKernelGGL((k_alone<T, KT, WHAT, ANY>), grid, dim3(BLOCK), 0, st, c);
+    else hipLaunchKernelGGL((k_alone<T, KT, WHAT, SHORT>), grid, dim3(BLOCK), 0, st, c);
 }
 
 // Workgroups of four heads each, of which each has the same h in every wave throughout: four times
@@ -1072,7 +1073,8 @@ template <typename T, int WHAT> void together(Call &c, int fit, hipStream_t st)
     const dim3 grid((unsigned)(c.scan[0].spans * c.segments * c.scans));
     if (fit == FULL) hipLaunchKernelGGL((k_together<T, WHAT, FULL>), grid, dim3(BLOCK), 0, st, c);
     else if (fit == EIGHTS) hipLaunchKernelGGL((k_together<T, WHAT, EIGHTS>), grid, dim3(BLOCK), 0, st, c);
-    else hipLaunchKernelGGL((k_together<T, WHAT, ANY>), grid, dim3(BLOCK), 0, st, c);
+    else if (fit == ANY) hipLaunchKernelGGL((k_together<T, WHAT, ANY>), grid, dim3(BLOCK), 0, st, c);
+    else hipLaunchKernelGGL((k_together<T, WHAT, SHORT>), grid, dim3(BLOCK), 0, st, c);
 }
 
 template <typename T, int KT, int WHAT> void scan(Call &c, int fit, hipStream_t st)
@@ -1086,7 +1088,8 @@ template <typename T, int KT, int WHAT> void scan(Call &c, int fit, hipStream_t 
         const dim3 grid((unsigned)c.scan[0].spans);
         if (fit == FULL) hipLaunchKernelGGL((k_short<T, FULL>), grid, dim3(BLOCK), 0, st, c, c.scan[0], c.scan[1], c.scan[2]);
         else if (fit == EIGHTS) hipLaunchKernelGGL((k_short<T, EIGHTS>), grid, dim3(BLOCK), 0, st, c, c.scan[0], c.scan[1], c.scan[2]);
-        else hipLaunchKernelGGL((k_short<T, ANY>), grid, dim3(BLOCK), 0, st, c, c.scan[0], c.scan[1], c.scan[2]);
+        else if (fit == ANY) hipLaunchKernelGGL((k_short<T, ANY>), grid, dim3(BLOCK), 0, st, c, c.scan[0], c.scan[1], c.scan[2]);
+        else hipLaunchKernelGGL((k_short<T, SHORT>), grid, dim3(BLOCK), 0, st, c, c.scan[0], c.scan[1], c.scan[2]);
     } else if (KT == 1 && c.slices == c.scans) together<T, WHAT>(c, fit, st);
     else alone<T, KT, WHAT>(c, fit, st);
     if (WHAT == OUTPUTS) {
@@ -1108,7 +1111,8 @@ template <typename T, int WHAT> void scan(Call &c, hipStream_t st)
     int fit = FULL;
     for (int i = 0; i < c.scans; ++i) {
         if (c.scan[i].dk != 32 * kt || c.scan[i].dv % 32) fit = fit < EIGHTS ? fit : EIGHTS;
-        if (c.scan[i].dk % 8 || c.scan[i].dv % 8) fit = ANY;
+        if (c.scan[i].dk % 8 || c.scan[i].dv % 8) fit = fit < ANY ? fit : ANY;
+        if (c.scan[i].dk < 8 || c.scan[i].dv < 8) fit = SHORT;
     }
     c.units = c.batch * c.heads * c.segments * c.slices;
     if (kt == 1) scan<T, 1, WHAT>(c, fit, st);

@@ -217,7 +217,7 @@ template <typename T, int VT, int KT, int FIT> __global__ __launch_bounds__(BLOC
 #pragma unroll
                         for (int r = 0; r < 8; ++r) e.e[r] = (T)(counts ? o[8 * x + r] * weight : 0.0f);
                         if (FIT == FULL || d + 8 <= D) *(Span<T, 8> *)to = e;
-                        else if constexpr (FIT == ANY) {
+                        else if constexpr (FIT <= ANY) {
 #pragma unroll
                             for (int r = 0; r < 8; ++r)
                                 if (d + r < D) to[r] = e.e[r];
@@ -338,7 +338,8 @@ template <typename T, int VT, int KT> void rows(const Head &c, int grid, hipStre
 {
     if (c.dim == 32 * KT) hipLaunchKernelGGL((k_rows<T, VT, KT, FULL>), dim3(grid), dim3(BLOCK), 0, st, c);
     else if (c.dim % 8 == 0) hipLaunchKernelGGL((k_rows<T, VT, KT, EIGHTS>), dim3(grid), dim3(BLOCK), 0, st, c);
-    else hipLaunchKernelGGL((k_rows<T, VT, KT, ANY>), dim3(grid), dim3(BLOCK), 0, st, c);
+    else if (c.dim >= 8) hipLaunchKernelGGL((k_rows<T, VT, KT, ANY>), dim3(grid), dim3(BLOCK), 0, st, c);
+    else if constexpr (KT == 1) hipLaunchKernelGGL((k_rows<T, VT, KT, SHORT>), dim3(grid), dim3(BLOCK), 0, st, c);
 }
 
 template <typename T> void call(const Head &c, int grid, hipStream_t st)

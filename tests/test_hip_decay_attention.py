@@ -83,7 +83,8 @@ def run(q, k, v, ld, state, starts, g_out, g_state, scale=None):
 SHAPES = [(1, (3,), 2, 5, 7), (2, (1,), 1, 1, 1), (31, (2, 3), 2, 32, 32), (32, (5,), 3, 16, 33), (33, (4,), 1, 64, 64),
           (65, (2,), 2, 40, 72), (100, (3,), 2, 128, 128), (64, (2,), 3, 31, 100), (130, (1,), 1, 127, 3),
           (257, (2, 2), 2, 64, 32), (1000, (1,), 1, 48, 65), (32, (7,), 3, 32, 32), (17, (3, 3), 1, 24, 9), (32, (41,), 5, 8, 32),
-          (8, (1,), 1, 32, 16), (40, (70,), 4, 32, 24), (96, (13,), 6, 11, 30)]
+          (8, (1,), 1, 32, 16), (40, (70,), 4, 32, 24), (96, (13,), 6, 11, 30),
+          (40, (3,), 2, 9, 15), (33, (2,), 1, 13, 122), (70, (3,), 2, 58, 23), (1, (5,), 3, 33, 6), (34, (2,), 2, 8, 127), (20, (9,), 2, 30, 29)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
