@@ -526,8 +526,10 @@ struct Share {
     int rest, splits;     // of the others
 };
 
-// A step of a tile of 256 x 256 takes some 0.45 us, a tile's sums to memory and back (all chip) 0.1.
-constexpr float SPLIT_COST = 0.25f;  // of a split of one tile, in steps of a round
+// What a split of one tile costs, in steps of a round: a step of 256 x 256 in 16 bits takes some 0.45 us, of 128 x 128
+// or 64 x 256 in float32 1, of 64 x 256 in 16 bits as long as of 256 x 256 (it waits for memory); a tile's
+// sums to memory and back 0.1 and 0.03 (all chip).
+template <typename C> constexpr float split_cost() { return (C::BM * C::BN == 256 * 256 ? 0.25f : 0.06f) * (C::KE == 32 ? 1.0f : 0.5f); }
 
 template <typename C> __host__ __device__ __forceinline__ Share share_of(int64_t m, int64_t n, int steps, int places)
 {
@@ -543,7 +545,7 @@ template <typename C> __host__ __device__ __forceinline__ Share share_of(int64_t
     constexpr int WAYS[] = {2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48, 64, 96, 128, 192, 256};
     for (int w : WAYS) {
         if (!s.rest || s.rest * w > 2 * places || w * 4 > steps) break;
-        const float cost = (float)((s.rest * w + places - 1) / places) * (float)((steps + w - 1) / w) + SPLIT_COST * (float)(s.rest * w);
+        const float cost = (float)((s.rest * w + places - 1) / places) * (float)((steps + w - 1) / w) + split_cost<C>() * (float)(s.rest * w);
         if (cost < least) {
             least = cost;
             s.splits = w;
