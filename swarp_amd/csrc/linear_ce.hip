@@ -747,12 +747,14 @@ __global__ __launch_bounds__(BLOCK) void k_give(const float *from, T *to, int64_
 // ------------------------------------------------------------------ host
 
 template <typename T> struct Tiles;
-template <> struct Tiles<bf16> { typedef Tile<bf16, 4, 2, 2, 4> Wide; typedef Tile<bf16, 2, 1, 4, 1> Few; typedef Tile<bf16, 2, 2, 1, 4> Thin; };
-template <> struct Tiles<f16> { typedef Tile<f16, 4, 2, 2, 4> Wide; typedef Tile<f16, 2, 1, 4, 1> Few; typedef Tile<f16, 2, 2, 1, 4> Thin; };
-template <> struct Tiles<float> { typedef Tile<float, 2, 2, 2, 2> Wide; typedef Tile<float, 2, 1, 4, 1> Few; typedef Tile<float, 2, 2, 1, 4> Thin; };
+template <> struct Tiles<bf16> { typedef Tile<bf16, 4, 2, 2, 4> Wide; typedef Tile<bf16, 2, 1, 4, 1> Few; typedef Tile<bf16, 2, 2, 1, 4> Thin; typedef Tile<bf16, 1, 1, 2, 1> Slim; };
+template <> struct Tiles<f16> { typedef Tile<f16, 4, 2, 2, 4> Wide; typedef Tile<f16, 2, 1, 4, 1> Few; typedef Tile<f16, 2, 2, 1, 4> Thin; typedef Tile<f16, 1, 1, 2, 1> Slim; };
+template <> struct Tiles<float> { typedef Tile<float, 2, 2, 2, 2> Wide; typedef Tile<float, 2, 1, 4, 1> Few; typedef Tile<float, 2, 2, 1, 4> Thin; typedef Tile<float, 1, 1, 2, 1> Slim; };
 constexpr int FEW = 32;            // rows of a Few tile
-constexpr int THIN_MOST = 64;      // columns of a Thin one (82305 x 1261 float32, 22 columns: 0.86 ms, 1.17 with Wide ones)
-enum { WIDE, FEWER, THIN };
+constexpr int THIN_MOST = 64;      // columns of a Thin one (82305 x 1261 float32, 22 columns: 0.77 ms, 1.17 with Wide ones)
+constexpr int SLIM_MOST = 64 * 256;  // rows of Slim tiles of logits (3205 x 2038 float32, 3 columns: 159 us, 253 with
+                                      // Thin ones, of 256 rows; 20000 rows: alike)
+enum { WIDE, FEWER, THIN, SLIM };
 constexpr int FEW_JOINED = 2048;   // fewer rows: a workgroup joins the parts of one
 
 int64_t up_to(int64_t n, int64_t k) { return (n + k - 1) / k * k; }
@@ -779,8 +781,8 @@ Plan plan_of(const swarp_linear_ce_t *a)
     p.grad = dh || dw || a->d_bias;
     p.dim_p = up_to(D, ke);
     p.wide = up_to(V, ke);
-    p.shape = N <= FEW ? FEWER : V <= THIN_MOST ? THIN : WIDE;
-    const int64_t bm = p.shape == THIN ? 64 : p.shape == FEWER || p.size == 2 ? 256 : 128;
+    p.shape = N <= FEW ? FEWER : V > THIN_MOST ? WIDE : N < SLIM_MOST ? SLIM : THIN;
+    const int64_t bm = p.shape >= THIN ? 64 : p.shape == FEWER || p.size == 2 ? 256 : 128;
     const int64_t wm = p.shape == THIN ? 1 : p.shape == FEWER ? 4 : 2;
     // (float32: what there is less of is multiplied, E or h)
     p.normed = p.size == 2 || V < D;
@@ -849,6 +851,7 @@ template <typename T, bool STORE> bool logits(const Call &c, int shape, int agai
     switch (shape) {
     case FEWER: return logits<T, typename Tiles<T>::Few, STORE>(c, again, st);
     case THIN: return logits<T, typename Tiles<T>::Thin, STORE>(c, again, st);
+    case SLIM: return logits<T, typename Tiles<T>::Slim, STORE>(c, again, st);
     default: return logits<T, typename Tiles<T>::Wide, STORE>(c, again, st);
     }
 }
@@ -968,7 +971,7 @@ template <typename T> int run(const swarp_linear_ce_t *a, hipStream_t st)
             const void *const h = c.normed ? (const char *)c.h + first * pitch_h : c.hs;
             const Product y = {c.e, h, pitch_e, pitch_h, c.width, c.dim, 0, 0, 1, n > 0,
                                c.normed ? 1.0f / (1 << KEPT_BITS) : 1.0f, c.normed, nullptr, a->d_weight, parts};
-            ok &= product<T, true>(c, y, p.shape == THIN, st);
+            ok &= product<T, true>(c, y, p.shape >= THIN, st);
         }
     }
     hipLaunchKernelGGL(k_loss, dim3(1), dim3(BLOCK), 0, st, c);
