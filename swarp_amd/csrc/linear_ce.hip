@@ -7,21 +7,22 @@
 //
 // Three matrix products of 2 rows dim width operations each: the logits, which are formed tile by
 // tile in the matrix cores' registers and leave them as exponentials, and the two gradients, which
-// need all of a row's exponentials.  Those are kept for as many rows as 1 GiB holds (a piece), in
-// the heads' type; then comes the next piece.
-//
-// float32: they are relative to the target's logit, which is known beforehand (one dot product a row):
+// need all of a row's exponentials.  Those are kept for as many rows as 1 GiB holds (a piece); then
+// comes the next piece.  They are relative to the target's logit, which is known beforehand (one dot
+// product a row):
 //   E_ij = exp(z_j - z_t),  s_i = sum_j E_ij,  logp = -log s_i,  G_ij = E_ij / s_i - [j = t],
-// so that a tile of them can be written before the row's sum is known; 1 / s_i goes into the rows of
-// d h and into h beside E^T.  Where some logit of a piece is above its target's by more than REACH
-// the piece is done again, relative to the rows' maxima (the kernels of that second pass are always
-// launched, look at a flag, and mostly end).
+// so that a tile of them can be written before the row's sum is known.  Where some logit of a piece is above
+// its target's by more than REACH the piece is done again, relative to the rows' maxima (the kernels of that
+// second pass are always launched, look at a flag, and mostly end).
+//
+// float32: 1 / s_i goes into the rows of d h and into E, or into h beside E^T, whichever is less.
 //
 // 16 bits: h / s beside E^T would be a second rounding of d W's terms (8 x 1023 decisions of 50001 logits,
 // 1024 wide, bfloat16, a quarter masked: 2.9e-3 of its size off, where its own rounding makes 1.7e-3),
 // and float16 has not the range.  So 24 bits of an exponential are kept, in two places, and become G,
 // normalised and rounded once, in a pass of their own (0.32 ms there: 5 bytes a logit at 4.8 TB/s), beside
-// which h stands as it is: 2.58 ms in all, and 2.83 with the sums from a product of their own instead.
+// which h stands as it is: 2.45 ms in all; it was 2.17 with the second rounding, and 2.83 with the sums from a
+// product of their own.
 //
 // Decisions whose mask is not set are left out of the products: the rows that count are gathered
 // first, and every kernel goes by their number on the device.
