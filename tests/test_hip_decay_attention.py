@@ -267,6 +267,27 @@ def test_a_scan_of_one_step(dk, dv, dtype):
     check([out[None], now], want[:2], 1, dk, dv, dtype, "step")
 
 
+def test_offsets_beyond_32_bits():
+    """2^31 + elements of q, k, v at once (one tensor, 4.3 GB).  What is 60 steps away weighs e^-180: the first
+    and the last steps are those of short calls."""
+    T, B, D, far = (1 << 20) + 77, 16, 128, 60
+    x = torch.randn(T, B, 1, D, generator=gen(46), device=DEV, dtype=torch.bfloat16).requires_grad_(True)
+    assert x.numel() > 1 << 31
+    ld = torch.full((1,), -3.0, device=DEV)
+    r = decay_attention(x, x.detach(), x.detach(), ld)
+    one = torch.ones((), device=DEV, dtype=torch.bfloat16).expand(r.out.shape)
+    d, = torch.autograd.grad(r.out, x, one)
+    for part in (slice(0, 3 * far), slice(T - 3 * far, T)):
+        y = x[part].detach().clone().requires_grad_(True)
+        want = decay_attention(y, y.detach(), y.detach(), ld)
+        w, = torch.autograd.grad(want.out, y, one[part])
+        keep = slice(0, far) if part.start == 0 else slice(-far, None)
+        # (chunks may begin elsewhere: products of 2^-8 halves' sums of 16 bits, and the end's rounding)
+        for got, wanted in ((r.out[part][keep], want.out[keep]), (d[part][keep], w[keep])):
+            assert float((got.float() - wanted.float()).abs().max()) <= 2.0 ** -7 * float(wanted.float().abs().max())
+    assert torch.allclose(r.state, want.state, rtol=1e-4, atol=1e-4 * float(want.state.abs().max()))
+
+
 def test_step_under_inference_mode():
     q, k, v, ld, state, s = inputs(1, (3,), 2, 8, 8, torch.float32, 44, 0.3)
     want = decay_attention(q, k, v, ld, state, s)

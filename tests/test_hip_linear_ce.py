@@ -340,6 +340,21 @@ def test_graphs_of_every_shape(rows, D, V, dtype):
             assert all(torch.equal(y, want[k]) for y, k in zip(grads, ("hidden", "weight", "bias")))
 
 
+@pytest.mark.parametrize("rows,D,V", [((1 << 24) + 33, 128, 9), ((1 << 21) + 33, 1032, 20)])
+def test_offsets_beyond_32_bits(rows, D, V):
+    """2^31 + elements of the hidden states; their last rows."""
+    g = gen(13)
+    h = torch.empty(rows, D, device=DEV, dtype=torch.bfloat16).normal_(generator=g)
+    w = torch.randn(V, D, generator=g, device=DEV).to(torch.bfloat16) / 16
+    t = torch.randint(0, V, (rows,), generator=g, device=DEV)
+    assert h.numel() > 1 << 31
+    got = run(h, w, t, None, None, reduction="sum")
+    part = slice(rows - 70, rows)
+    want = reference(h[part], w, t[part], None, None, reduction="sum")
+    close(got["logp"][part], want["logp"], "logp")
+    close(got["hidden"][part], want["hidden"], "hidden")
+
+
 def test_only_what_is_wanted():
     h, w, t, b, _ = inputs(90, 33, 70, torch.bfloat16, 6)
     full = run(h, w, t, b, None)
