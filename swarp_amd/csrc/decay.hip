@@ -65,8 +65,9 @@ enum { OUTPUTS, ENDS };
 
 // What a wave keeps of a head from chunk to chunk: the state's columns -- element
 // (32 t + 16 (r / 8) + 8 half + r % 8, j) in register r of tile t --, whether it is still zero, and a number
-// that is 0 as long as all that was multiplied is finite: a product with 0 is not 0 where it is not, and
-// the head is done again by k_exact.
+// that is 0 as long as its outputs and the state that it leaves are finite.  A product with 0 is not 0 where a
+// part, a score or the state (of finite parts, past the largest float) is not finite; that always shows
+// in an output of the chunk or in the leaving state, and the head is done again by k_exact.
 template <int KT> struct Kept {
     f32x16 S[KT];
     bool none;
@@ -126,16 +127,17 @@ __device__ __forceinline__ void enter(const Call &c, const Scan &s, int64_t bh, 
         }
     w.none = !from;
     w.odd = 0.0f;
-    if (from) {
+}
+// odd + 0 times what a tile holds: not 0 where some of it is not finite.
+__device__ __forceinline__ float odd_of(const f32x16 &x, float odd)
+{
 #pragma unroll
-        for (int t = 0; t < KT; ++t)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) w.odd = __builtin_fmaf(w.S[t][r], 0.0f, w.odd);
-    }
+    for (int r = 0; r < 16; ++r) odd = __builtin_fmaf(x[r], 0.0f, odd);
+    return odd;
 }
 template <int KT, int WHAT, int FIT>
 __device__ __forceinline__ void leave(const Call &c, const Scan &s, int64_t bh, int segment, bool ends, int lane, int j, int slice,
-                                      const Kept<KT> &w, bool any)
+                                      Kept<KT> &w, bool any)
 {
     const int half = lane >> 5;
     float *to = WHAT == ENDS        ? s.between + ((int64_t)segment * c.batch * c.heads + bh) * c.area
@@ -157,6 +159,10 @@ __device__ __forceinline__ void leave(const Call &c, const Scan &s, int64_t bh, 
             }
     }
     if (WHAT == OUTPUTS) {
+        if (to) {
+#pragma unroll
+            for (int t = 0; t < KT; ++t) w.odd = odd_of(w.S[t], w.odd);
+        }
         const bool wrong = __ballot(!(w.odd == 0.0f)) != 0;
         if (lane == 0) c.wrong[(bh * c.segments + segment) * c.slices + s.first + slice] = wrong;
     } else if (lane == 0) s.cut[(int64_t)segment * c.batch * c.heads + bh] = any;
@@ -171,18 +177,15 @@ __device__ __forceinline__ void chunk(Kept<KT> &w, const Powers &f, const Part<T
     const int half = lane >> 5, col = lane & 31;
     f32x16(&S)[KT] = w.S;
     bool &none = w.none;
-    float &odd = w.odd;
     Part<T> vf[2];
     vf[0] = column_of<T>(vx, vp, 0, j0, lane);
     vf[1] = column_of<T>(vx, vp, 16, j0, lane);
-    odd = odd_of<T>(vf[1], odd_of<T>(vf[0], odd));
     Part<T> pf[2], pl[2];
     if (WHAT == OUTPUTS) {
         const uint32_t upto = cut & (0xffffffffu >> (31 - col));
         const int since = upto ? 31 - __clz(upto) : 0;  // first step that enters step `col`
 #pragma unroll
         for (int r = 0; r < 16; ++r) p[r] *= f.D[r];
-        // (a score is not finite wherever its q or k is not)
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
             float y[8];
@@ -190,14 +193,10 @@ __device__ __forceinline__ void chunk(Kept<KT> &w, const Powers &f, const Part<T
             for (int r = 0; r < 8; ++r) y[r] = p[8 * x + r];
             if (cut) {
 #pragma unroll
-                for (int r = 0; r < 8; ++r) {
-                    odd = __builtin_fmaf(y[r], 0.0f, odd);
-                    y[r] = 16 * x + 8 * half + r >= since ? y[r] : 0.0f;
-                }
+                for (int r = 0; r < 8; ++r) y[r] = 16 * x + 8 * half + r >= since ? y[r] : 0.0f;
             }
             pf[x] = term_of<T>(y, true);
             if (Part<T>::TERMS) pl[x] = term_of<T>(y, false);
-            odd = odd_of<T>(pf[x], odd);
         }
     }
     if (WHAT == OUTPUTS) {
@@ -220,6 +219,7 @@ __device__ __forceinline__ void chunk(Kept<KT> &w, const Powers &f, const Part<T
             mma<T>(o, vf[x], pf[x]);
             if (Part<T>::TERMS) mma<T>(o, vf[x], pl[x]);
         }
+        w.odd = odd_of(o, w.odd);
     }
     if (goes_on) {
         const int kept = cut ? 31 - __clz(cut) : 0;  // first step that enters the leaving state
@@ -664,7 +664,6 @@ template <typename T, int FIT> __global__ __launch_bounds__(BLOCK, 2) void k_sho
             };
             const uint32_t upto = cut & (0xffffffffu >> (31 - col)), after = col < 31 ? cut >> (col + 1) << (col + 1) : 0;
             const int since = upto ? 31 - __clz(upto) : 0, until = after ? __ffs((int)after) - 1 : 32;
-            float odd = 0.0f;
             Part<T> a[2], b[2], hi[2], lo[2];
             f32x16 p;
             // scores of `a` (rows by swapped lane) and `b` (by lane), times their powers, as operands
@@ -679,21 +678,16 @@ template <typename T, int FIT> __global__ __launch_bounds__(BLOCK, 2) void k_sho
                     for (int r = 0; r < 8; ++r) {
                         const int i = 16 * x + 8 * half + r;
                         y[r] = p[8 * x + r] * w[8 * x + r];
-                        if (cut) {
-                            odd = __builtin_fmaf(y[r], 0.0f, odd);
-                            y[r] = i >= from && i < below ? y[r] : 0.0f;
-                        }
+                        if (cut) y[r] = i >= from && i < below ? y[r] : 0.0f;
                     }
                     hi[x] = term_of<T>(y, true);
                     if (Part<T>::TERMS) lo[x] = term_of<T>(y, false);
-                    odd = odd_of<T>(hi[x], odd);
                 }
             };
             auto times = [&](f32x16 &o, const T *x) {
 #pragma unroll
                 for (int y = 0; y < 2; ++y) {
                     const Part<T> z = column_of<T>(x, P, 16 * y, 0, lane);
-                    odd = odd_of<T>(z, odd);
                     mma<T>(o, z, hi[y]);
                     if (Part<T>::TERMS) mma<T>(o, z, lo[y]);
                 }
@@ -707,7 +701,6 @@ template <typename T, int FIT> __global__ __launch_bounds__(BLOCK, 2) void k_sho
                     for (int r = 0; r < 8; ++r) {
                         const int i = 16 * x + 8 * half + r;
                         z[r] = perm < across && i < along ? m[perm * lane_step + i * step] : 0.0f;
-                        odd = __builtin_fmaf(z[r], 0.0f, odd);
                     }
                     mma<T>(o, term_of<T>(z, true), y[x]);
                     if (Part<T>::TERMS) mma<T>(o, term_of<T>(z, false), y[x]);
@@ -748,17 +741,20 @@ template <typename T, int FIT> __global__ __launch_bounds__(BLOCK, 2) void k_sho
             rows(ox, col, b);
             scores(D, since, 32);
             times(dq, kx);
+            float odd = odd_of(dq, 0.0f);  // (as in chunk())
             __builtin_amdgcn_sched_barrier(0);
             rows(ox, perm, a);
             rows(vx, col, b);
             scores(E, 0, until);
             times(dk_, qx);
+            odd = odd_of(dk_, odd);
             __builtin_amdgcn_sched_barrier(0);
             put(vx, dq);  // (a wave has read what it needs of v: gradients take the rows' place)
             rows(qx, perm, a);
             rows(kx, col, b);
             scores(E, 0, until);
             times(dv_, ox);
+            odd = odd_of(dv_, odd);
             __builtin_amdgcn_sched_barrier(0);
             if (sv.state_out) {  // d S0: columns of q, and of do times their powers
                 f32x16 z = {};
@@ -780,7 +776,11 @@ template <typename T, int FIT> __global__ __launch_bounds__(BLOCK, 2) void k_sho
                 for (int r = 0; r < 16; ++r) {
                     const int i = 16 * (r >> 3) + 8 * half + (r & 7);
                     const int64_t at = bh * c.area + i * dv + perm;
-                    if (i < dk && perm < dv) sv.state_out[at] = z[r] + (sk.state && !cut ? f * sk.state[at] : 0.0f);
+                    if (i < dk && perm < dv) {
+                        const float y = z[r] + (sk.state && !cut ? f * sk.state[at] : 0.0f);
+                        odd = __builtin_fmaf(y, 0.0f, odd);
+                        sv.state_out[at] = y;
+                    }
                 }
             }
             const bool wrong = __ballot(!(odd == 0.0f)) != 0;

@@ -79,22 +79,6 @@ template <typename T> __device__ __forceinline__ Part<T> term_of(float (&x)[8], 
     }
     return p;
 }
-// odd + 0 times what a part holds: not 0 where some of it is not finite.
-template <typename T> __device__ __forceinline__ float odd_of(const Part<T> &p, float odd)
-{
-    if constexpr (Part<T>::TERMS) {
-        typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-        const bf16x2 none = {(bf16)0.0f, (bf16)0.0f};
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-            odd = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, (uint32_t)p.w[k]), none, odd, false);
-    } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) odd = __builtin_fmaf(p.x[k], 0.0f, odd);
-    }
-    return odd;
-}
-
 // How the heads' widths fit the tiles: FULL, dk the tiles' and dv a multiple of 32; EIGHTS, both
 // multiples of 8; ANY, both at least 8; SHORT.
 enum { SHORT, ANY, EIGHTS, FULL };

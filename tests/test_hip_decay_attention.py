@@ -161,6 +161,39 @@ def test_a_start_stops_everything_and_no_step_looks_ahead(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,dk,dv", [(20, 24, 32), (150, 24, 32), (150, 40, 72), (2100, 16, 32)])
+def test_a_start_stops_what_passed_the_largest_float(T, dk, dv, dtype):
+    """Finite parts whose state, or whose products with it, are not: what a start parts from them is as if
+    they had been ordinary.  `clean` has ordinary values in their place."""
+    q, k, v, ld, state, _ = inputs(T, (3,), 2, dk, dv, dtype, T + dk)
+    ld, cut = ld * 0.2, T * 2 // 3
+    s = torch.zeros(T, 3, dtype=torch.bool, device=DEV)
+    s[cut] = True
+    g = gen(2)
+    g_out = torch.randn(v.shape, generator=g, device=DEV).to(dtype)
+    g_state = torch.randn(state.shape, generator=g, device=DEV)
+    large = torch.full_like(state, 3e38)
+    many = [10 * q, k, v, ld, state, s, 10 * g_out, g_state]
+    many_back = [q, 10 * k, 10 * v, ld, state, s, g_out, g_state]
+    late, early = slice(cut, T), slice(0, cut)
+    cases = [("state", many, {4: large}, late), ("gradient of the state", many_back, {7: large}, early)]
+    if dtype != torch.float16:  # (its products stay below 2^32)
+        first, last = torch.ones(T, 1, 1, 1, device=DEV), torch.ones(T, 1, 1, 1, device=DEV)
+        first[:cut], last[cut:] = 1e20, 1e20
+        plain = [q, k, v, ld, state, s, g_out, g_state]
+        cases += [("k and v", plain, {1: (k * first).to(dtype), 2: (v * first).to(dtype)}, late),
+                  ("q and gradients", plain, {0: (q * last).to(dtype), 6: (g_out * last).to(dtype)}, early)]
+    for what, clean, changed, part in cases:
+        want = both(*clean)
+        got = run(*(changed.get(n, x) for n, x in enumerate(clean)))
+        assert not all(bool(x.isfinite().all()) for x in got), what  # (it did pass)
+        keep = [x[part] if n in (0, 2, 3, 4) else x for n, x in enumerate(got)]
+        wanted = [(x[part], y[part]) if n in (0, 2, 3, 4) else (x, y) for n, (x, y) in enumerate(want)]
+        keep[1 if part is early else 5] = wanted[1 if part is early else 5][0]  # (of the other side)
+        check(keep, wanted, T, dk, dv, dtype, f"{what} {T} {dk}x{dv} {dtype}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_padded_ends_reach_nothing_before_them(dtype):
     q, k, v, ld, _, _ = inputs(90, (3,), 2, 32, 48, dtype, 23)
     clean = decay_attention(q, k, v, ld).out
