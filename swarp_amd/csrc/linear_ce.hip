@@ -428,7 +428,8 @@ template <typename T, int ROWS> __global__ __launch_bounds__(BLOCK) void k_join(
         }
         if (how == KEPT2 && mine) c.ref[j] = ref;
     }
-    const bool none = hi == -INFINITY;  // (no logit above -inf)
+    // (no logit above -inf, or no such target: in a second pass its row's exponentials are finite)
+    const bool none = hi == -INFINITY || zt != zt;
     if (none) logp = NAN;
     if (mine && how != SUMS) {
         const int64_t t = c.targets32 ? (int64_t)((const int32_t *)c.targets)[i] : ((const int64_t *)c.targets)[i];

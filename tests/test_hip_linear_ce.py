@@ -247,6 +247,20 @@ def test_what_is_wrong_shows(what, dtype):
         assert all(bool(x.isfinite().all()) for x in got.values())
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D,V", [(16, 300), (400, 300), (16, 25), (200, 20)])
+def test_a_target_that_is_none_shows_beside_a_far_one(D, V, dtype):
+    """A row whose target is e^-400 sends its neighbours through a second pass."""
+    h, w, t, b, _ = inputs(70, D, V, dtype, 22)
+    t = torch.where(t == 5, 6, t)
+    t[3], t[7], b[5] = 5, V, -400.0
+    got = run(h, w, t, b, None)
+    assert got["loss"].isnan() and got["logp"][7].isnan()
+    assert got["hidden"][7].isnan().all() and got["weight"].isnan().all() and got["bias"].isnan().all()
+    rest = torch.arange(70, device=DEV) != 7
+    assert got["logp"][rest].isfinite().all() and got["hidden"][rest].isfinite().all()
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_strides_over_leading_axes(dtype):
     g = gen(0)
