@@ -8,12 +8,15 @@
 // Three matrix products of 2 rows dim width operations each: the logits, which are formed tile by
 // tile in the matrix cores' registers and leave them as exponentials, and the two gradients, which
 // need all of a row's exponentials.  Those are kept for as many rows as 1 GiB holds (a piece); then
-// comes the next piece.  They are relative to the target's logit, which is known beforehand (one dot
+// comes the next piece.  They are relative to the target's logit r, which is known beforehand (one dot
 // product a row):
-//   E_ij = exp(z_j - z_t),  s_i = sum_j E_ij,  logp = -log s_i,  G_ij = E_ij / s_i - [j = t],
+//   E_ij = exp(z_j - r_i),  s_i = sum_j E_ij,  logp = -log(s_i / E_it),  G_ij = E_ij / s_i - [j = t],
 // so that a tile of them can be written before the row's sum is known.  Where some logit of a piece is above
 // its target's by more than REACH the piece is done again, relative to the rows' maxima (the kernels of that
 // second pass are always launched, look at a flag, and mostly end).
+// A dot product adds in another order than the matrix cores: r is off z_t by some 2^-24 of their terms, which
+// may be more than 1 - p.  So the target's own exponential, and G there, come of the logit that its tile has:
+// s_i is a sum with E_it in it, never less, and logp never above 0.
 //
 // float32: 1 / s_i goes into the rows of d h and into E, or into h beside E^T, whichever is less.
 //
@@ -69,9 +72,10 @@ struct Call {
     float *logp, *loss;
     // of all rows
     void *h;
-    float *z_t, *ref, *top;   // target's logit; what E is relative to; largest logit
+    float *z_t, *ref, *top;   // target's logit (NaN: none); what E is relative to; largest logit
     float *inv, *inv_h;       // of d h's rows; what h, or E (16 bits), is multiplied by: k_scale, k_norm
-    int32_t *target;          // 16 bits: or -1
+    float *one;               // normed: G / weight times 2^KEPT_BITS at the target
+    int32_t *target;          // or -1
     double *sums;             // of logp, one for `few` rows
     int few;                  // rows of a workgroup that joins: 1 or 64
     int64_t pieces;
@@ -153,8 +157,8 @@ template <typename T> struct __attribute__((packed, aligned(sizeof(T)))) Eight {
     T e[8];
 };
 
-// Row i of the hidden states, padded with zeros, and its target's logit (NaN if there is no such
-// target).  A wave a row.
+// Row i of the hidden states, padded with zeros, its target, and (of a call that keeps exponentials) what those
+// will be relative to.  A wave a row.
 template <typename T> __global__ __launch_bounds__(BLOCK) void k_rows(const Call c)
 {
     const int lane = threadIdx.x & 63;
@@ -178,12 +182,12 @@ template <typename T> __global__ __launch_bounds__(BLOCK) void k_rows(const Call
             Eight<T> v = {}, y = {};
             if (k + 8 <= c.dim) {
                 v = *(const Eight<T> *)(x + k);
-                y = *(const Eight<T> *)(w + k);
+                if (c.e) y = *(const Eight<T> *)(w + k);
             } else {
                 for (int q = 0; q < 8; ++q)
                     if (k + q < c.dim) {
                         v.e[q] = x[k + q];
-                        y.e[q] = w[k + q];
+                        if (c.e) y.e[q] = w[k + q];
                     }
             }
 #pragma unroll
@@ -193,9 +197,9 @@ template <typename T> __global__ __launch_bounds__(BLOCK) void k_rows(const Call
         z = wave_sum(z);
         if (lane == 0) {
             if (c.bias) z += up(((const T *)c.bias)[in ? t : 0]);
-            z = in ? z : NAN;
-            c.z_t[j] = z;
-            c.ref[j] = z;
+            c.z_t[j] = NAN;  // (k_logits has it where there is such a target)
+            c.ref[j] = in ? z : NAN;
+            c.target[j] = in ? (int32_t)t : -1;
         }
     }
 }
@@ -276,6 +280,16 @@ __global__ __launch_bounds__(C::THREADS) void k_logits(const Call c, int nm, int
         const int row = r0 + (wn * C::TN + j) * 32 + acc_col(lane);
         const bool mine = row < rows;
         float m = -INFINITY, s = 0.0f;
+        // (few tiles of a wide head hold a target of theirs)
+        const uint32_t own = mine ? (uint32_t)(c.target[c.first + row] - (v0 + wm * C::TM * 32)) : ~0u;
+        if (__ballot(own < C::TM * 32u)) {
+            float zt = 0.0f;
+#pragma unroll
+            for (int i = 0; i < C::TM; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) zt = own == (uint32_t)(i * 32 + acc_row(r, lane)) ? t.acc[i][j][r] : zt;
+            if (own < C::TM * 32u && (own >> 2 & 1) == (uint32_t)lane >> 5) c.z_t[c.first + row] = zt;
+        }
 #pragma unroll
         for (int i = 0; i < C::TM; ++i)
 #pragma unroll
@@ -360,7 +374,7 @@ __global__ __launch_bounds__(C::THREADS) void k_logits(const Call c, int nm, int
 
 // How a row's parts are joined.
 enum { SUMS = 0,     // from parts relative to their largest: logp
-       KEPT = 1,     // from parts relative to ref, which E is too: logp, 1 / s, E at the target
+       KEPT = 1,     // from parts relative to ref, which E is too: logp, 1 / s, G at the target
        KEPT2 = 2 };  // the same after a second pass
 
 // A workgroup takes ROWS rows, its threads every (BLOCK / ROWS)-th part of one.
@@ -418,28 +432,29 @@ template <typename T, int ROWS> __global__ __launch_bounds__(BLOCK) void k_join(
     }
     const int64_t i = c.index ? c.index[j] : j;
     float logp;
+    const float et = exp_of(zt - ref);  // as E has it
     if (how == SUMS) {
         logp = (zt - hi) - log_of(s);
     } else {
-        logp = (zt - ref) - log_of(s);
+        // (s is not below et, which is one of its terms)
+        logp = et > 0.5f ? -log_of(s / et) : (zt - ref) - log_of(s);
         if (how == KEPT && mine) {
             if (hi - ref > REACH || ref == -INFINITY) *c.flag = 1;
             c.top[j] = hi;
         }
-        if (how == KEPT2 && mine) c.ref[j] = ref;
     }
     // (no logit above -inf, or no such target: in a second pass its row's exponentials are finite)
     const bool none = hi == -INFINITY || zt != zt;
     if (none) logp = NAN;
     if (mine && how != SUMS) {
-        const int64_t t = c.targets32 ? (int64_t)((const int32_t *)c.targets)[i] : ((const int64_t *)c.targets)[i];
         if (!c.normed) {
             c.inv[j] = c.inv_h[j] = none ? NAN : weight_of(c) / s;
-            if (t >= 0 && t < c.width) ((float *)c.e)[(int64_t)row * c.wide + t] = exp_of(zt - ref) - s;
+            if (c.target[j] >= 0) ((float *)c.e)[(int64_t)row * c.wide + c.target[j]] = et - s;
         } else {
+            const float f = none ? NAN : (1 << KEPT_BITS) / s;
             c.inv[j] = weight_of(c) / (1 << KEPT_BITS);
-            c.inv_h[j] = none ? NAN : (1 << KEPT_BITS) / s;
-            c.target[j] = t >= 0 && t < c.width ? (int32_t)t : -1;
+            c.inv_h[j] = f;
+            c.one[j] = (et - s) * f;
         }
     }
     if (mine) c.logp[i] = logp;
@@ -451,15 +466,11 @@ template <typename T, int ROWS> __global__ __launch_bounds__(BLOCK) void k_join(
     }
 }
 
-// An exponential as it is kept, and G / weight times 2^KEPT_BITS at row j's target (f: of its exponentials).
+// An exponential as it is kept.
 __device__ __forceinline__ float exponential(float e, uint8_t) { return e; }
 template <typename T> __device__ __forceinline__ float exponential(T e, uint8_t low)
 {
     return __builtin_bit_cast(float, (uint32_t)__builtin_bit_cast(uint16_t, e) << 16 | (uint32_t)low << 8);
-}
-__device__ __forceinline__ float one_of(const Call &c, int64_t j, float f)
-{
-    return exp_of(c.z_t[j] - c.ref[j]) * f - (1 << KEPT_BITS);
 }
 
 // G / weight times 2^KEPT_BITS, in E's place.  A thread takes eight neighbours at a time (a row is of whole
@@ -493,7 +504,7 @@ template <typename T> __global__ __launch_bounds__(BLOCK) void k_norm(const Call
 #pragma unroll
         for (int q = 0; q < 8; ++q) z.e[q] = (T)(exponential(x[k].e[q], y[k].e[q]) * f[k]);
         if ((uint32_t)t[k] < 8u) {
-            const T one = (T)one_of(c, c.first + at / eights, f[k]);
+            const T one = (T)c.one[c.first + at / eights];
 #pragma unroll
             for (int q = 0; q < 8; ++q)
                 if (q == t[k]) z.e[q] = one;
@@ -679,7 +690,7 @@ template <typename T> __global__ __launch_bounds__(BLOCK) void k_bias(const Call
             Low low = {};
             if constexpr (sizeof(T) == 2) low = *(const Low *)(c.low + at);
             const float inv = c.inv[j], f = c.normed ? c.inv_h[j] : 1.0f;
-            const float one = c.normed ? one_of(c, j, f) : 0.0f;
+            const float one = c.normed ? c.one[j] : 0.0f;
             const int64_t t = c.normed ? c.target[j] - v : -1;
 #pragma unroll
             for (int k = 0; k < V; ++k) s[k] = __builtin_fmaf(inv, k == t ? one : exponential(y.e[k], low.e[k]) * f, s[k]);
@@ -768,7 +779,7 @@ struct Plan {
     int shape;
     int64_t pieces;
     bool pad_w, grad, normed;
-    uint64_t index, counts, h, z_t, ref, top, inv, inv_h, target, sums, flag, parts, e, low, hs, w, split, bias, bytes;
+    uint64_t index, counts, h, z_t, ref, top, inv, inv_h, one, target, sums, flag, parts, e, low, hs, w, split, bias, bytes;
 };
 
 // Workgroups of a product: one a compute unit with 128 KiB of LDS, two with 64.
@@ -812,7 +823,8 @@ Plan plan_of(const swarp_linear_ce_t *a)
     p.top = room(true, 4 * N);
     p.inv = room(true, 4 * N);
     p.inv_h = room(true, 4 * N);
-    p.target = room(p.grad && p.normed, 4 * N);
+    p.one = room(p.grad && p.normed, 4 * N);
+    p.target = room(true, 4 * N);
     p.sums = room(true, 8 * (N / (piece < FEW_JOINED ? 1 : 64) + 1));
     p.parts = room(true, 8ull * p.n_parts * piece);
     p.w = room(p.pad_w, (uint64_t)V * p.dim_p * p.size);
@@ -911,6 +923,7 @@ template <typename T> int run(const swarp_linear_ce_t *a, hipStream_t st)
     c.top = (float *)(mem + p.top);
     c.inv = (float *)(mem + p.inv);
     c.inv_h = (float *)(mem + p.inv_h);
+    c.one = (float *)(mem + p.one);
     c.target = (int32_t *)(mem + p.target);
     c.sums = (double *)(mem + p.sums);
     c.flag = (int32_t *)(mem + p.flag);

@@ -261,6 +261,48 @@ def test_a_target_that_is_none_shows_beside_a_far_one(D, V, dtype):
     assert got["logp"][rest].isfinite().all() and got["hidden"][rest].isfinite().all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,D,V", [(64, 1024, 1000), (20, 1024, 1000), (300, 1261, 60), (16500, 520, 40), (200, 64, 25)])
+def test_confident_decisions(rows, D, V, dtype):
+    """Where the target's probability is almost 1, 1 - p and log p are what the others leave, and no
+    difference of two roundings of the target's logit.  q = 1 - p is off by the others' relative error, and by
+    what adding terms to a sum near 1 loses: no more than they are, and 2^-24 an addition, of which a
+    logit passes V / 32 + 64 at most; and by 8 2^-24 for quotient, logarithm and the like."""
+    h, w, t, b, _ = inputs(rows, D, V, dtype, rows + V)
+    scale = torch.linspace(6.0, 30.0, rows, device=DEV)[:, None] / w[t].float().square().sum(-1, keepdim=True)
+    h = (w[t].float() * scale + 0.1 * h.float()).to(dtype)
+    # (float16: neither beyond its largest, summed over the rows, nor below its smallest)
+    up, u, kinds = (2.0 ** 14 * min(1.0, 256 / rows) if dtype == torch.float16 else 1.0), half(dtype), (h, w, t, b, None)
+    hd, wd = h.double(), w.double()
+    z = hd @ wd.t() + b.double()
+    dz = (D + 2) * F24 * (hd.abs() @ wd.abs().t() + b.double().abs()).amax(-1, keepdim=True)
+    lse = torch.logsumexp(z, -1, keepdim=True)
+    one = torch.nn.functional.one_hot(t, V).double()
+    p = torch.exp(z - lse) * (1 - one)  # of the others
+    q = p.sum(-1, keepdim=True)
+    assert float(q.median()) < 1e-4
+    relative = 2 * dz + 32 * F24 + 2 * F24 * (z - lse).abs().amax(-1, keepdim=True)
+    dq = q * relative + torch.minimum(q, torch.tensor((V / 32 + 64) * F24)) + 8 * F24
+    logp = torch.log1p(-q)
+    with torch.no_grad():
+        alone = linear_cross_entropy(h, w, t, b, reduction="sum")
+    got = run(*kinds, up, "sum")
+    for y in (alone.logp, got["logp"]):
+        assert bool((y <= 0).all()), float(y.max())
+        close(y, (logp[:, 0], (2 * dq + 4 * F24 * logp.abs())[:, 0]), "logp")
+    G, err = (p - one * q) * up, (p * relative + one * dq) * up
+    mag = G.abs()
+    least = 2.0 ** -39 * up if dtype == torch.float16 else 0.0  # (float16's smallest, over what G is kept times)
+    rounding = 1.02 * u + V * F24
+    dh, db = G @ wd, G.sum(0)
+    tiny = torch.finfo(dtype).tiny
+    close(got["hidden"], (dh, (err + mag * rounding + least) @ wd.abs() + (u + 4 * F24) * dh.abs() + tiny), "hidden")
+    dw = G.t() @ hd
+    close(got["weight"], (dw, (err + mag * (1.02 * u + rows * F24) + least).t() @ hd.abs() + (u + 4 * F24) * dw.abs() + tiny), "weight")
+    # (24 bits of an exponential are kept: 2^-17 of half a step)
+    close(got["bias"], (db, (err + mag * (2.0 ** -16 + rows * F24)).sum(0) + (u + 4 * F24) * db.abs() + tiny), "bias")
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_strides_over_leading_axes(dtype):
     g = gen(0)
