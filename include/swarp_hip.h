@@ -599,7 +599,7 @@ typedef struct swarp_decay {
                                  itself but in swarp_decay_step */
     const void *adj_out;      /* as out, and as state_out, or NULL (zero); read by the _bwd call */
     const float *adj_state;
-    void *d_q, *d_k, *d_v;    /* [steps, batch, heads, dk or dv], or NULL */
+    void *d_q, *d_k, *d_v;    /* [steps, batch, heads, dk or dv]: the _bwd call writes all three */
     float *d_state;           /* as state, or NULL */
     void *work;               /* swarp_decay_work_bytes() bytes, 256-byte aligned */
     uint64_t work_bytes;

@@ -1250,7 +1250,7 @@ int swarp_decay_bwd(const swarp_decay_t *a, void *stream)
     if (!a->batch) return 0;
     if (!a->log_decay || (a->steps && (!a->q || !a->k || !a->v || !a->adj_out)))
         return fail("pointer arguments must be set");
-    if (!a->d_q != !a->d_k || !a->d_q != !a->d_v) return fail("d_q, d_k and d_v are set together");
+    if (a->steps && (!a->d_q || !a->d_k || !a->d_v)) return fail("d_q, d_k and d_v must be set, all three together");
     if (work(a, true)) return -1;
     Call c = call_of(a, true);
     const float scale = (float)a->scale;

@@ -128,6 +128,18 @@ def test_decay_refuses_before_any_launch():
                     "in the state")
 
 
+@pytest.mark.parametrize("missing", ["d_q", "d_k", "d_v", "all"])
+@pytest.mark.parametrize("d_state", [None, 256])
+def test_the_adjoint_of_a_scan_wants_all_three_gradients(missing, d_state):
+    """Its kernels write all of them, also where only the state's is wanted."""
+    lib = _lib.load()
+    outs = {name: None if missing in (name, "all") else 256 for name in ("d_q", "d_k", "d_v")}
+    a = _lib.SwarpDecay(dtype=0, heads=2, dk=8, dv=8, steps=3, batch=4, group=1, scale=1.0, log_decay=256, q=256, k=256,
+                        v=256, state=256, adj_out=256, d_state=d_state, work=256, **outs)
+    a.work_bytes = lib.swarp_decay_work_bytes(ctypes.byref(a))
+    refused(lib.swarp_decay_bwd(ctypes.byref(a), None), "together")
+
+
 @pytest.fixture(autouse=True)
 def no_message_left_behind():
     yield
