@@ -35,6 +35,8 @@ def _strides(x: torch.Tensor, lead: int):
     """(step, batch, head) strides of ``x [*lead, H, D]`` with ``lead`` leading axes, the first of
     them time where there is one more than the batch's; None where one stride does not reach the
     batch or the last axis is not dense."""
+    if x.numel() == 0:  # (nothing to reach)
+        return 0, 0, 0
     if x.shape[-1] > 1 and x.stride(-1) != 1:
         return None
     size, step = 1, 0

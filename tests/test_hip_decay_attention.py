@@ -358,6 +358,21 @@ def test_empty_calls():
         assert not r.state.any()
 
 
+@pytest.mark.parametrize("T", [0, 5])
+@pytest.mark.parametrize("batch", [(4, 0), (0, 4), (3, 0, 2)])
+def test_empty_axes_of_the_batch(T, batch):
+    q, k, v, ld, state, _ = inputs(T, batch, 2, 8, 6, torch.float32, 1)
+    for s in (None, torch.zeros(T, *batch[:1], dtype=torch.bool, device=DEV), torch.zeros(T, *batch, dtype=torch.bool, device=DEV)):
+        x = [t.clone().requires_grad_(True) for t in (q, k, v, state)]
+        r = decay_attention(*x[:3], ld, x[3], s)
+        assert r.out.shape == v.shape and r.state.shape == state.shape
+        d = torch.autograd.grad(r.out.sum() + r.state.sum(), x)
+        assert [t.shape for t in d] == [t.shape for t in x]
+    if T:
+        out = decay_attention_step(q[0], k[0], v[0], ld, state, s[0])
+        assert out.shape == v.shape[1:]
+
+
 def test_one_result_alone_and_parts_that_want_nothing():
     q, k, v, ld, state, s = inputs(40, (2,), 2, 16, 16, torch.float32, 33, 0.1)
     x = [t.requires_grad_(True) for t in (q, k, v, state)]

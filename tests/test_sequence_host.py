@@ -8,7 +8,7 @@ from pathlib import Path
 import pytest
 import torch
 
-from swarp_amd import _lib, decay_attention, decay_attention_step, linear_cross_entropy
+from swarp_amd import _lib, decay_attention, decay_attention_step, linear_cross_entropy, memory
 
 HEADER = Path(__file__).resolve().parents[1] / "include" / "swarp_hip.h"
 
@@ -138,6 +138,15 @@ def test_the_adjoint_of_a_scan_wants_all_three_gradients(missing, d_state):
                         v=256, state=256, adj_out=256, d_state=d_state, work=256, **outs)
     a.work_bytes = lib.swarp_decay_work_bytes(ctypes.byref(a))
     refused(lib.swarp_decay_bwd(ctypes.byref(a), None), "together")
+
+
+@pytest.mark.parametrize("shape", [(5, 4, 0, 2, 8), (5, 0, 4, 2, 8), (0, 4, 3, 2, 8), (5, 3, 0, 2, 2, 8)])
+def test_strides_of_what_is_empty(shape):
+    x = torch.zeros(shape)
+    for y in (x, x[..., ::2], x.transpose(1, 2)):
+        for lead in (1, 0):
+            laid, strides = memory._laid(y, lead)
+            assert laid.numel() == 0 and list(strides) == [0, 0, 0]
 
 
 @pytest.fixture(autouse=True)
