@@ -585,7 +585,7 @@ int swarp_linear_ce_bwd(const swarp_linear_ce_t *a, int32_t skip_unit, const voi
  * t stride[0] + b stride[1] + h stride[2] + i; of the others at ((t batch + b) heads + h) d + i. */
 typedef struct swarp_decay {
     int32_t dtype;            /* of q, k, v, out and their gradients: SWARP_F32, _BF16 or _F16 */
-    int32_t heads, dk, dv;    /* 1 <= dk, dv <= 128 */
+    int32_t heads, dk, dv;    /* 1 <= heads <= 2^22, 1 <= dk, dv <= 128 */
     int64_t steps, batch;
     int64_t group;            /* consecutive batch entries that share their starts */
     int64_t q_stride[3], k_stride[3], v_stride[3]; /* elements */

@@ -28,7 +28,7 @@ using namespace part;
 constexpr int BLOCK = 256, WAVES = BLOCK / 64;
 constexpr int CHUNK = 32;
 constexpr float LOG2E = 1.44269504088896340736f;
-constexpr int MOST_DIM = 128;
+constexpr int MOST_DIM = 128, MOST_HEADS = 1 << 22;
 
 // One of a call's scans.
 struct Scan {
@@ -818,57 +818,59 @@ template <typename T, int FIT> __global__ __launch_bounds__(BLOCK, 2) void k_sho
 template <typename T, int KT> __global__ __launch_bounds__(BLOCK) void k_exact(const Call c, int64_t n)
 {
     const int lane = threadIdx.x & 63, half = lane >> 5;
-    const int64_t first = ((int64_t)blockIdx.x * WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * 64;
-    uint64_t wrong = 0;
-    if (first + lane < n) {
-        const int64_t bh = (first + lane) / c.slices, at = bh * c.segments * c.slices + (first + lane - bh * c.slices);
-        for (int i = 0; i < c.segments; ++i) wrong |= c.wrong[at + (int64_t)i * c.slices];
-    }
-    wrong = __ballot(wrong != 0);
-    for (; wrong; wrong &= wrong - 1) {
-        const int64_t unit = first + __ffsll((unsigned long long)wrong) - 1;
-        const int64_t bh = unit / c.slices, b = bh / c.heads;
-        const int h = (int)(bh - b * c.heads);
-        int slice = (int)(unit - bh * c.slices), which = 0;
-        while (slice >= c.scan[which].slices) slice -= c.scan[which++].slices;
-        const Scan &s = c.scan[which];
-        const int j = 32 * slice + (lane & 31), dk = s.dk;
-        const bool back = s.back, mine = j < s.dv;
-        const uint8_t *const starts = c.starts ? c.starts + b / c.group : nullptr;
-        const int64_t groups = c.batch / c.group;
-        float S[KT * 16];
-#pragma unroll
-        for (int r = 0; r < 16 * KT; ++r) {
-            const int i = 2 * r + half;
-            S[r] = s.state && i < dk && mine ? s.state[bh * c.area + (int64_t)i * s.si + (int64_t)j * s.sj] : 0.0f;
+    const int64_t all = (int64_t)gridDim.x * BLOCK;
+    for (int64_t first = ((int64_t)blockIdx.x * WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * 64; first < n; first += all) {
+        uint64_t wrong = 0;
+        if (first + lane < n) {
+            const int64_t bh = (first + lane) / c.slices, at = bh * c.segments * c.slices + (first + lane - bh * c.slices);
+            for (int i = 0; i < c.segments; ++i) wrong |= c.wrong[at + (int64_t)i * c.slices];
         }
-        const float lambda = __builtin_amdgcn_exp2f(c.log_decay[h] * LOG2E);
-        for (int64_t x = 0; x < c.steps; ++x) {
-            const int64_t t = back ? c.steps - 1 - x : x;
-            const T *const q = (const T *)s.q + t * s.qs[0] + b * s.qs[1] + h * s.qs[2];
-            const T *const k = (const T *)s.k + t * s.ks[0] + b * s.ks[1] + h * s.ks[2];
-            const float v = mine ? (float)((const T *)s.v)[t * s.vs[0] + b * s.vs[1] + h * s.vs[2] + j] * s.grow : 0.0f;
-            const bool fresh = starts && (back ? x > 0 && starts[(t + 1) * groups] : starts[t * groups]);
-            float o = 0.0f;
+        wrong = __ballot(wrong != 0);
+        for (; wrong; wrong &= wrong - 1) {
+            const int64_t unit = first + __ffsll((unsigned long long)wrong) - 1;
+            const int64_t bh = unit / c.slices, b = bh / c.heads;
+            const int h = (int)(bh - b * c.heads);
+            int slice = (int)(unit - bh * c.slices), which = 0;
+            while (slice >= c.scan[which].slices) slice -= c.scan[which++].slices;
+            const Scan &s = c.scan[which];
+            const int j = 32 * slice + (lane & 31), dk = s.dk;
+            const bool back = s.back, mine = j < s.dv;
+            const uint8_t *const starts = c.starts ? c.starts + b / c.group : nullptr;
+            const int64_t groups = c.batch / c.group;
+            float S[KT * 16];
 #pragma unroll
             for (int r = 0; r < 16 * KT; ++r) {
                 const int i = 2 * r + half;
-                if (i < dk) {
-                    const float kv = (float)k[i] * v;
-                    const float y = fresh ? kv : __builtin_fmaf(back ? 1.0f : lambda, S[r], kv);
-                    o = __builtin_fmaf((float)q[i], y, o);
-                    S[r] = back ? lambda * y : y;
-                }
+                S[r] = s.state && i < dk && mine ? s.state[bh * c.area + (int64_t)i * s.si + (int64_t)j * s.sj] : 0.0f;
             }
-            o += __shfl_xor(o, 32, 64);
-            if (half == 0 && mine) ((T *)s.out)[t * s.os[0] + b * s.os[1] + h * s.os[2] + j] = (T)(o * s.carry);
-        }
-        if (s.state_out && mine) {
-            const bool clear = back && starts && c.steps > 0 && starts[0];
+            const float lambda = __builtin_amdgcn_exp2f(c.log_decay[h] * LOG2E);
+            for (int64_t x = 0; x < c.steps; ++x) {
+                const int64_t t = back ? c.steps - 1 - x : x;
+                const T *const q = (const T *)s.q + t * s.qs[0] + b * s.qs[1] + h * s.qs[2];
+                const T *const k = (const T *)s.k + t * s.ks[0] + b * s.ks[1] + h * s.ks[2];
+                const float v = mine ? (float)((const T *)s.v)[t * s.vs[0] + b * s.vs[1] + h * s.vs[2] + j] * s.grow : 0.0f;
+                const bool fresh = starts && (back ? x > 0 && starts[(t + 1) * groups] : starts[t * groups]);
+                float o = 0.0f;
 #pragma unroll
-            for (int r = 0; r < 16 * KT; ++r) {
-                const int i = 2 * r + half;
-                if (i < dk) s.state_out[bh * c.area + (int64_t)i * s.si + (int64_t)j * s.sj] = clear ? 0.0f : S[r];
+                for (int r = 0; r < 16 * KT; ++r) {
+                    const int i = 2 * r + half;
+                    if (i < dk) {
+                        const float kv = (float)k[i] * v;
+                        const float y = fresh ? kv : __builtin_fmaf(back ? 1.0f : lambda, S[r], kv);
+                        o = __builtin_fmaf((float)q[i], y, o);
+                        S[r] = back ? lambda * y : y;
+                    }
+                }
+                o += __shfl_xor(o, 32, 64);
+                if (half == 0 && mine) ((T *)s.out)[t * s.os[0] + b * s.os[1] + h * s.os[2] + j] = (T)(o * s.carry);
+            }
+            if (s.state_out && mine) {
+                const bool clear = back && starts && c.steps > 0 && starts[0];
+#pragma unroll
+                for (int r = 0; r < 16 * KT; ++r) {
+                    const int i = 2 * r + half;
+                    if (i < dk) s.state_out[bh * c.area + (int64_t)i * s.si + (int64_t)j * s.sj] = clear ? 0.0f : S[r];
+                }
             }
         }
     }
@@ -998,7 +1000,8 @@ int check(const swarp_decay_t *a)
     if (a->steps < 0 || a->batch < 0 || a->heads < 1 || a->dk < 1 || a->dk > MOST_DIM || a->dv < 1 ||
         a->dv > MOST_DIM || a->group < 1 || a->batch % a->group)
         return fail("bad sizes");
-    if (a->batch * a->heads > 1ll << 31 || a->steps > 1ll << 40) return fail("bad sizes");
+    // (a launch has fewer than 2^32 threads: a wave, or a share of a workgroup, for every head, slice and scan)
+    if (a->heads > MOST_HEADS || a->batch * a->heads > 1ll << 31 || a->steps > 1ll << 40) return fail("bad sizes");
     return 0;
 }
 
@@ -1094,7 +1097,8 @@ template <typename T, int KT, int WHAT> void scan(Call &c, int fit, hipStream_t 
     else alone<T, KT, WHAT>(c, fit, st);
     if (WHAT == OUTPUTS) {
         const int64_t n = c.units / c.segments;
-        hipLaunchKernelGGL((k_exact<T, KT>), dim3((unsigned)((n + BLOCK - 1) / BLOCK)), dim3(BLOCK), 0, st, c, n);
+        const int64_t blocks = (n + BLOCK - 1) / BLOCK;  // (of up to 2^34 units: a launch has fewer than 2^32 threads)
+        hipLaunchKernelGGL((k_exact<T, KT>), dim3((unsigned)(blocks < 16384 ? blocks : 16384)), dim3(BLOCK), 0, st, c, n);
     }
 }
 

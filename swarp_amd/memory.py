@@ -21,7 +21,7 @@ from . import _lib
 from .policy import (_CODES, _differentiable_once, _guard, _no_tangents, _on_gpu, _plain, _ptr,
                      _same, _untraced)
 
-_MOST_DIM = 128
+_MOST_DIM, _MOST_HEADS = 128, 1 << 22
 
 
 class DecayAttention(NamedTuple):
@@ -82,9 +82,9 @@ def _arguments(what: str, q, k, v, log_decay, state, starts, scale, lead: int):
         raise ValueError(f"v must be {list(q.shape[:-1])} + [Dv]; got {list(v.shape)}")
     T = q.shape[0] if lead else 1
     batch, (H, dk), dv = q.shape[lead:-2], q.shape[-2:], v.shape[-1]
-    if not (1 <= dk <= _MOST_DIM and 1 <= dv <= _MOST_DIM) or H < 1:
-        raise ValueError(f"heads must be 1 to {_MOST_DIM} wide, one at least; got q {list(q.shape)}, "
-                         f"v {list(v.shape)}")
+    if not (1 <= dk <= _MOST_DIM and 1 <= dv <= _MOST_DIM and 1 <= H <= _MOST_HEADS):
+        raise ValueError(f"heads must be 1 to {_MOST_DIM} wide, one to {_MOST_HEADS} of them; got q "
+                         f"{list(q.shape)}, v {list(v.shape)}")
     if batch.numel() * H >= 1 << 31:
         raise ValueError(f"at most 2^31 - 1 heads in all; got {batch.numel() * H}")
     log_decay = _same(log_decay, "log_decay", torch.Size((H,)), torch.float32, dev)

@@ -321,6 +321,25 @@ def test_offsets_beyond_32_bits():
     assert torch.allclose(r.state, want.state, rtol=1e-4, atol=1e-4 * float(want.state.abs().max()))
 
 
+def test_more_than_2_32_units_of_heads():
+    """Three scans of 2^32 / 3 heads of one element (45 GB).  The last head's state, which a start parts it
+    from, is 3e38, and its product with q past the largest float."""
+    n = (1 << 32) // 3 + 99
+    x = torch.randn(1, n, 1, 1, generator=gen(47), device=DEV, dtype=torch.bfloat16)
+    state = torch.zeros(n, 1, 1, 1, device=DEV)
+    starts = torch.zeros(1, n, dtype=torch.bool, device=DEV)
+    x[0, -1], state[-1], starts[0, -1] = 10.0, 3e38, True
+    q = x.requires_grad_(True)
+    r = decay_attention(q, x.detach(), x.detach(), torch.full((1,), -1.0, device=DEV), state, starts)
+    d, = torch.autograd.grad(r.out, q, torch.full_like(r.out, 2.0))
+    assert float(r.out[0, -1]) == 1000.0 and float(d[0, -1]) == 200.0 and float(r.state[-1]) == 100.0
+    for a in range(0, n, 1 << 28):
+        y = x.detach()[0, a:a + (1 << 28), 0, 0].float()
+        # (two terms of a score, and the end's rounding)
+        for got, want in ((r.out, y * y * y), (d, 2 * y * y)):
+            assert bool(((got.detach()[0, a:a + (1 << 28), 0, 0].float() - want).abs() <= 2.0 ** -7 * want.abs() + 1e-30).all())
+
+
 def test_step_under_inference_mode():
     q, k, v, ld, state, s = inputs(1, (3,), 2, 8, 8, torch.float32, 44, 0.3)
     want = decay_attention(q, k, v, ld, state, s)
@@ -507,6 +526,16 @@ def test_refusals():
     g, = torch.autograd.grad(decay_attention(**dict(ok, q=x)).out, x, one, create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         g.sum().backward()
+
+
+def test_more_heads_than_a_launch_takes_are_refused():
+    x = torch.zeros(1, (1 << 22) + 1, 1, device=DEV)
+    with pytest.raises(ValueError, match="4194304 of them"):
+        decay_attention(x, x, x, x[0, :, 0])
+    with pytest.raises(ValueError, match="4194304 of them"):
+        decay_attention_step(x, x, x, x[0, :, 0], x[..., None])
+    y = x[:, 1:]
+    assert decay_attention(y, y, y, y[0, :, 0]).out.shape == y.shape
 
 
 def test_under_compile_the_graph_breaks():

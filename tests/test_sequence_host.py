@@ -140,6 +140,16 @@ def test_the_adjoint_of_a_scan_wants_all_three_gradients(missing, d_state):
     refused(lib.swarp_decay_bwd(ctypes.byref(a), None), "together")
 
 
+def test_heads_beyond_a_launch_are_refused():
+    lib = _lib.load()
+    a = _lib.SwarpDecay(dtype=0, heads=(1 << 22) + 1, dk=8, dv=8, steps=1, batch=1, group=1)
+    for f in (lib.swarp_decay_fwd, lib.swarp_decay_bwd, lib.swarp_decay_step):
+        refused(f(ctypes.byref(a), None), "sizes")
+    assert lib.swarp_decay_work_bytes(ctypes.byref(a)) == 0
+    a.heads -= 1
+    assert lib.swarp_decay_work_bytes(ctypes.byref(a)) > 0
+
+
 @pytest.mark.parametrize("shape", [(5, 4, 0, 2, 8), (5, 0, 4, 2, 8), (0, 4, 3, 2, 8), (5, 3, 0, 2, 2, 8)])
 def test_strides_of_what_is_empty(shape):
     x = torch.zeros(shape)
