@@ -23,7 +23,7 @@
 extern "C" {
 #endif
 
-#define SWARP_ABI_VERSION 18
+#define SWARP_ABI_VERSION 19
 
 #define SWARP_F32 0
 #define SWARP_F64 1
@@ -576,6 +576,10 @@ int swarp_linear_ce(const swarp_linear_ce_t *a, void *stream);
  * mask). */
 int swarp_linear_ce_bwd(const swarp_linear_ce_t *a, int32_t skip_unit, const void *scale, void *d_hidden,
                         void *d_weight, void *d_bias, void *stream);
+
+/* Which graph capture `stream` is part of (0: none).  Gradients that a forward left are there for a
+ * backward of the same capture only: a graph's replays find what the ones before made of them. */
+uint64_t swarp_capture_id(void *stream);
 
 /* Linear attention with a decay for each head, along a rollout.  Per batch entry and head, with
  * the state S [dk, dv] and a step's q, k [dk], v [dv]:

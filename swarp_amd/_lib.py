@@ -13,7 +13,7 @@ from pathlib import Path
 
 import torch
 
-ABI_VERSION = 18
+ABI_VERSION = 19
 F32, F64, BF16, F16 = 0, 1, 2, 3
 EULER, RK4 = 0, 1
 LISTS_BRUTE, LISTS_GRID = 0, 1
@@ -337,6 +337,7 @@ SIGNATURES = {
          ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p],
         ctypes.c_int,
     ),
+    "swarp_capture_id": ([ctypes.c_void_p], ctypes.c_uint64),
     "swarp_decay_work_bytes": ([ctypes.POINTER(SwarpDecay)], ctypes.c_uint64),
     "swarp_decay_fwd": ([ctypes.POINTER(SwarpDecay), ctypes.c_void_p], ctypes.c_int),
     "swarp_decay_bwd": ([ctypes.POINTER(SwarpDecay), ctypes.c_void_p], ctypes.c_int),

@@ -1080,6 +1080,17 @@ int swarp_linear_ce_bwd(const swarp_linear_ce_t *a, int32_t skip_unit, const voi
     return launched();
 }
 
+uint64_t swarp_capture_id(void *stream)
+{
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (hipStreamGetCaptureInfo((hipStream_t)stream, &status, &id) != hipSuccess) {
+        (void)hipGetLastError();
+        return 0;
+    }
+    return status == hipStreamCaptureStatusActive ? id + 1 : 0;
+}
+
 }  // extern "C"
 
 namespace narrow {

@@ -71,7 +71,8 @@ class _LinearCeFn(torch.autograd.Function):
     gradient and rounds them, once.  The others are handed out, once; where the upstream gradient is
     not 1 (the device looks) those of a wide head are multiplied by it and those of a narrow one
     computed again with it.  float16 ones of a narrow head are left to the backward: without the loss
-    scale that comes with it they would vanish.  A second backward computes them again."""
+    scale that comes with it they would vanish.  A second backward computes them again, and so does
+    one that is captured into a graph without its forward."""
 
     @staticmethod
     def forward(ctx, a: _lib.SwarpLinearCe, stream: int, complete: bool, hidden, weight, bias,
@@ -89,6 +90,7 @@ class _LinearCeFn(torch.autograd.Function):
             ctx.save_for_backward(*grads, place)
         else:
             ctx.made = None if late else (grads, place)
+            ctx.capture = _lib.load().swarp_capture_id(stream)
             ctx.work = work if complete else None
             ctx.save_for_backward(hidden, weight, bias, targets, mask)
         ctx.mark_non_differentiable(logp)
@@ -113,6 +115,8 @@ class _LinearCeFn(torch.autograd.Function):
                    for t in out]
         else:
             made, ctx.made = ctx.made, None  # handed out once: the caller may change them
+            if made is not None and ctx.capture != _lib.load().swarp_capture_id(ctx.stream):
+                made = None  # (a graph's replays find them changed, with no forward to leave new ones)
             if not _unmoved(a, ctx.like[0], *saved):
                 a = _lib.SwarpLinearCe.from_buffer_copy(a)
                 keep = _point(a, *saved)

@@ -396,6 +396,60 @@ def test_graphs_of_every_shape(rows, D, V, dtype):
             assert all(torch.equal(y, want[k]) for y, k in zip(grads, ("hidden", "weight", "bias")))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,D,V", [(300, 64, 25), (300, 64, 300)])
+def test_a_backward_captured_without_its_forward(rows, D, V, dtype):
+    """Every replay leaves what an eager backward does, whatever became of the gradients in between."""
+    h, w, t, b, m = inputs(rows, D, V, dtype, 62, True, 0.3)
+    side = torch.cuda.Stream()
+    for up in (1.0, 2.0):
+        want = run(h, w, t, b, m, up)
+        x = [y.clone().requires_grad_(True) for y in (h, w, b)]
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            loss = linear_cross_entropy(x[0], x[1], t, x[2], m).loss
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            grads = torch.autograd.grad(loss * up, x, retain_graph=True)
+        for _ in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(y, want[k]) for y, k in zip(grads, ("hidden", "weight", "bias")))
+            for y in grads:
+                y.zero_()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,D,V", [(300, 64, 25), (300, 64, 300)])
+def test_a_forward_and_its_backward_in_two_graphs(rows, D, V, dtype):
+    """The second graph is replayed twice for a replay of the first."""
+    for up in (1.0, 2.0):
+        h, w, t, b, m = inputs(rows, D, V, dtype, 64, True, 0.3)
+        x = [y.clone().requires_grad_(True) for y in (h, w, b)]
+        run(h, w, t, b, m)
+        torch.cuda.synchronize()
+        one, two, side = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        with torch.cuda.graph(one, stream=side):
+            loss = linear_cross_entropy(x[0], x[1], t, x[2], m).loss
+        with torch.cuda.graph(two, stream=side):
+            grads = torch.autograd.grad(loss * up, x, retain_graph=True)
+        for seed in (65, 66, 67):
+            h, _, t2, _, m2 = inputs(rows, D, V, dtype, seed, True, 0.3)
+            with torch.no_grad():
+                x[0].copy_(h)
+                t.copy_(t2)
+                m.copy_(m2)
+            one.replay()
+            want = run(h, w, t2, b, m2, up)
+            for _ in range(2):
+                two.replay()
+                torch.cuda.synchronize()
+                assert all(torch.equal(y, want[k]) for y, k in zip(grads, ("hidden", "weight", "bias")))
+                for y in grads:
+                    y.zero_()
+
+
 @pytest.mark.parametrize("rows,D,V", [((1 << 24) + 33, 128, 9), ((1 << 21) + 33, 1032, 20)])
 def test_offsets_beyond_32_bits(rows, D, V):
     """2^31 + elements of the hidden states; their last rows."""
