@@ -459,7 +459,8 @@ template <typename T, int ROWS> __global__ __launch_bounds__(BLOCK) void k_join(
     }
     if (mine) c.logp[i] = logp;
     total[lane] = mine ? (double)logp : 0.0;
-    if (lane == 0) {  // (w == 0: one wave at most)
+    __builtin_amdgcn_wave_barrier();  // (w == 0: one wave at most)
+    if (lane == 0) {
         double sum = 0;
         for (int k = 0; k < ROWS; ++k) sum += total[k];
         c.sums[c.first / ROWS + blockIdx.x] = sum;
