@@ -544,7 +544,10 @@ int swarp_grad_norm(const swarp_tensor_t *tensors, int32_t n_tensors, double max
  * gradient of 1.  A head whose weight a workgroup's LDS holds (swarp_linear_ce_complete) is done in
  * one kernel, and they are complete, of `dtype`.  Else they are float, d_hidden with the rows that
  * count moved together; the work memory then holds the exponentials of at most 1 GiB of rows (or of
- * 256 rows; half as much again of 16-bit heads) at a time, copies of hidden and, where its rows are not whole steps of 64 bytes, weight. */
+ * 256 rows) at a time: P bytes.  In all at most 2.1 P (1.5 P in 16 bits; in float32 another P for the rows of
+ * hidden as they go beside them), copies of hidden (rows padded to 64 bytes) and, where its rows are not whole
+ * 16 bytes, of weight, 60 bytes a row, 128 a column with d_bias, and 129 MiB.  Without a gradient: the copies,
+ * 60 bytes a row, and 1 GiB. */
 typedef struct swarp_linear_ce {
     int32_t dtype;            /* of hidden, weight, bias: SWARP_F32, _BF16 or _F16 */
     int32_t sum;              /* 1: loss is the sum, 0: the mean */

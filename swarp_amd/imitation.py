@@ -178,9 +178,10 @@ def linear_cross_entropy(
     them -inf, or with a target outside ``[0, V)`` makes the loss NaN.
 
     Gradients flow to ``hidden``, ``weight`` and ``bias``, once, and backward only.  A loss with
-    float16 heads should be scaled, as mixed precision does.  A call needs, beside copies of
-    ``hidden`` and ``weight``, up to 1.5 GiB of work memory where gradients are wanted, and float32
-    buffers for them until the backward.
+    float16 heads should be scaled, as mixed precision does.  A wide head's call needs work memory:
+    copies of ``hidden`` and of a ``weight`` whose rows are not whole 16 bytes, 60 bytes a decision and
+    up to 1 GiB; where gradients are wanted 2.1 times the exponentials of 1 GiB of rows (or of 256
+    rows), 128 bytes a column and 0.13 GiB, and float32 buffers for them until the backward.
     """
     if is_dynamo_compiling():
         return _untraced(linear_cross_entropy)(hidden, weight, targets, bias, mask,

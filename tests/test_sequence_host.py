@@ -140,6 +140,28 @@ def test_the_adjoint_of_a_scan_wants_all_three_gradients(missing, d_state):
     refused(lib.swarp_decay_bwd(ctypes.byref(a), None), "together")
 
 
+@pytest.mark.parametrize("dtype,size", [(0, 4), (2, 2), (3, 2)])
+def test_linear_ce_work_memory_is_what_is_said(dtype, size):
+    """Of wide heads: copies, 60 bytes a row, and with gradients 2.1 times a piece's exponentials, 128 bytes a
+    column and 129 MiB; without 1 GiB."""
+    lib, pad = _lib.load(), 64 // size
+    for N in (1, 33, 300, 5000, 1 << 17, 1 << 24, (1 << 31) - 1):
+        for D in (65, 129, 333, 2048, 65536):
+            for V in (1, 33, 65, 2048, 32003, 1 << 20, 1 << 21):
+                for grads in (0, 1, 2, 4, 7):
+                    a = _lib.SwarpLinearCe(dtype=dtype, dim=D, width=V, rows=N, inner=1, mask=256, weight=256,
+                                           d_hidden=256 * (grads & 1), d_weight=256 * (grads >> 1 & 1),
+                                           d_bias=256 * (grads >> 2))
+                    if lib.swarp_linear_ce_complete(ctypes.byref(a)):
+                        continue
+                    row = -(-D // pad) * 64
+                    copies = (N + 31) * row + (V * row if D * size % 16 else 0)
+                    piece = max(1 << 30, 256 * -(-V // pad) * 64)
+                    rest = 2.1 * piece + 128 * V + (129 << 20) if grads else 1 << 30
+                    need = lib.swarp_linear_ce_work_bytes(ctypes.byref(a))
+                    assert 0 < need <= copies + 60 * N + rest + 8192, (N, D, V, grads)
+
+
 def test_heads_beyond_a_launch_are_refused():
     lib = _lib.load()
     a = _lib.SwarpDecay(dtype=0, heads=(1 << 22) + 1, dk=8, dv=8, steps=1, batch=1, group=1)
