@@ -6,6 +6,10 @@
 // the softmax is in registers; G = p - [target] is an operand of d h^T = W^T G^T as it lies, and goes
 // through LDS to be one of d W = G^T h, whose sums stay in the wave's registers to the end.  A second
 // kernel adds the workgroups' sums, in their order.
+// bfloat16: G goes into both as two terms, 16 bits, so that what the gradients are off by is their own
+// rounding (256000 x 64 x 25: d h 1.66e-3 of its size, 2.07e-3 with one term, and 1 us of 50).  The biases are in
+// LDS to make room for that: with them in registers the wider heads spilled (256000 x 64 x 60: 89 us,
+// now 76; float16 245, 155).
 // Three products of 2 rows dim width operations: far below what the rows cost to read and write.
 // 256000 rows of 64, 25 outputs, bfloat16: 34 us of the rows' kernel and 5 of adding up 512 workgroups' sums,
 // 69 MB in all (14 us): what is left is a wave's chain through 32 rows, 15 of them each, and its first ones.
@@ -71,10 +75,13 @@ template <typename T, int VT, int KT, int FIT> __global__ __launch_bounds__(BLOC
 {
     typedef typename Mul<T>::type M;
     constexpr int KP = 32 * KT + 16 / (int)sizeof(T), GP = 32 * VT + 16 / (int)sizeof(M);
-    constexpr int SUMS = 32 * VT * 32 * KT * 4, ROOM = WAVES * 32 * (KP * (int)sizeof(T) + GP * (int)sizeof(M));
+    constexpr int TERMS = Part<M>::TERMS ? 2 : 1;  // of G
+    constexpr int EACH = 32 * (KP * (int)sizeof(T) + TERMS * GP * (int)sizeof(M));  // bytes of a wave
+    constexpr int SUMS = 32 * VT * 32 * KT * 4, ROOM = WAVES * EACH;
     __shared__ __align__(16) T wx[32 * VT * KP];
     __shared__ __align__(16) char room[ROOM > SUMS ? ROOM : SUMS];
     __shared__ double red[WAVES];
+    __shared__ __align__(16) float bx[32 * VT];
     if (skipped(c)) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31, perm = swapped(col);
     const int D = c.dim, V = c.width;
@@ -82,23 +89,18 @@ template <typename T, int VT, int KT, int FIT> __global__ __launch_bounds__(BLOC
         const int v = x / KP, d = x % KP;
         wx[x] = v < V && d < D ? ((const T *)c.weight)[v * D + d] : (T)0.0f;
     }
+    // (those past the last output are -inf)
+    if (threadIdx.x < 32 * VT)
+        bx[threadIdx.x] = (int)threadIdx.x >= V ? -INFINITY : c.bias ? up(((const T *)c.bias)[threadIdx.x]) : 0.0f;
     const int64_t n_on = counted(c);
     const float up1 = c.scale ? *c.scale : 1.0f;
     const float weight = c.sum ? up1 : (float)((double)up1 / (double)(n_on > 1 ? n_on : 1));
     __syncthreads();
-    T *const hx = (T *)(room + wave * 32 * (KP * (int)sizeof(T) + GP * (int)sizeof(M)));
+    T *const hx = (T *)(room + wave * EACH);
     M *const gx = (M *)(hx + 32 * KP);
     const bool grads = c.sums != nullptr;
 
-    // register r of tile a is output 32 a + 16 (r / 8) + 8 half + r % 8; those past the last are -inf
-    float bias[VT][16];
-#pragma unroll
-    for (int a = 0; a < VT; ++a)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int v = 32 * a + 16 * (r >> 3) + 8 * half + (r & 7);
-            bias[a][r] = v >= V ? -INFINITY : c.bias ? up(((const T *)c.bias)[v]) : 0.0f;
-        }
+    // register r of tile a is output 32 a + 16 (r / 8) + 8 half + r % 8
     f32x16 dw[VT][KT];
     float db[VT][16];
 #pragma unroll
@@ -151,11 +153,13 @@ template <typename T, int VT, int KT, int FIT> __global__ __launch_bounds__(BLOC
         float m = -INFINITY, s = 0.0f, zt = 0.0f;
         const bool in = at >= 0 && at < V;
         const int own = in ? (int)at - 8 * half : -1;  // this half's place of the target
+        int b0 = 8 * half;
+        asm volatile("" : "+v"(b0));  // (read here, not kept in registers throughout)
 #pragma unroll
         for (int a = 0; a < VT; ++a)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                z[a][r] += bias[a][r];
+                z[a][r] += bx[32 * a + 16 * (r >> 3) + (r & 7) + b0];
                 m = z[a][r] > m ? z[a][r] : m;
             }
         const float m2 = __shfl_xor(m, 32, 64);
@@ -188,7 +192,7 @@ template <typename T, int VT, int KT, int FIT> __global__ __launch_bounds__(BLOC
                 z[a][r] = own == 32 * a + 16 * (r >> 3) + (r & 7) ? p - one : p;
                 db[a][r] += z[a][r];
             }
-        Part<M> gf[VT][2];
+        Part<M> gf[VT][2], gl[VT][2];
 #pragma unroll
         for (int a = 0; a < VT; ++a)
 #pragma unroll
@@ -196,8 +200,12 @@ template <typename T, int VT, int KT, int FIT> __global__ __launch_bounds__(BLOC
                 float y[8];
 #pragma unroll
                 for (int r = 0; r < 8; ++r) y[r] = z[a][8 * x + r];
-                gf[a][x] = term_of<M>(y, false);
-                if (grads) *(Raw<M> *)(gx + col * GP + 32 * a + 16 * x + 8 * half) = __builtin_bit_cast(Raw<M>, gf[a][x]);
+                gf[a][x] = term_of<M>(y, true);
+                if (Part<M>::TERMS) gl[a][x] = term_of<M>(y, false);
+                if (grads) {
+                    *(Raw<M> *)(gx + col * GP + 32 * a + 16 * x + 8 * half) = __builtin_bit_cast(Raw<M>, gf[a][x]);
+                    if (Part<M>::TERMS) *(Raw<M> *)(gx + (32 + col) * GP + 32 * a + 16 * x + 8 * half) = __builtin_bit_cast(Raw<M>, gl[a][x]);
+                }
             }
         if (c.d_hidden) {
 #pragma unroll
@@ -206,8 +214,11 @@ template <typename T, int VT, int KT, int FIT> __global__ __launch_bounds__(BLOC
 #pragma unroll
                 for (int a = 0; a < VT; ++a)
 #pragma unroll
-                    for (int x = 0; x < 2; ++x)
-                        mma<M>(o, mul_of<T>(column_of<T>(wx, KP, 32 * a + 16 * x, 32 * t, lane)), gf[a][x]);
+                    for (int x = 0; x < 2; ++x) {
+                        const Part<M> wc = mul_of<T>(column_of<T>(wx, KP, 32 * a + 16 * x, 32 * t, lane));
+                        mma<M>(o, wc, gf[a][x]);
+                        if (Part<M>::TERMS) mma<M>(o, wc, gl[a][x]);
+                    }
                 if (i < c.rows) {
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
@@ -227,19 +238,22 @@ template <typename T, int VT, int KT, int FIT> __global__ __launch_bounds__(BLOC
             }
         }
         if (grads) {
-            Part<M> gc[VT][2];
 #pragma unroll
-            for (int a = 0; a < VT; ++a)
+            for (int x = 0; x < 2; ++x) {
+                Part<M> gc[VT][TERMS];
 #pragma unroll
-                for (int x = 0; x < 2; ++x) gc[a][x] = column_of<M>(gx, GP, 16 * x, 32 * a, lane);
+                for (int a = 0; a < VT; ++a)
 #pragma unroll
-            for (int t = 0; t < KT; ++t)
+                    for (int n = 0; n < TERMS; ++n) gc[a][n] = column_of<M>(gx, GP, 32 * n + 16 * x, 32 * a, lane);
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
+                for (int t = 0; t < KT; ++t) {
                     const Part<M> hc = mul_of<T>(column_of<T>(hx, KP, 16 * x, 32 * t, lane));
 #pragma unroll
-                    for (int a = 0; a < VT; ++a) mma<M>(dw[a][t], gc[a][x], hc);
+                    for (int a = 0; a < VT; ++a)
+#pragma unroll
+                        for (int n = 0; n < TERMS; ++n) mma<M>(dw[a][t], gc[a][n], hc);
                 }
+            }
         }
     }
     loss = wave_sum(loss);

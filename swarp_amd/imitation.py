@@ -171,8 +171,9 @@ def linear_cross_entropy(
 
         logp = z[target] - log sum exp z,   loss = -mean (or sum) of logp over what counts
 
-    Products and sums are in float32, whatever the type; exponentials go into the gradients' products
-    in the type of ``hidden``.  What a masked decision holds is not looked at, its target included
+    Products and sums are in float32, whatever the type; what comes of exponentials goes into the
+    gradients' products in the type of ``hidden`` (of narrow heads, up to 32 columns of 128 or 64 of 64,
+    with 16 bits at least).  What a masked decision holds is not looked at, its target included
     (-100); with no decision that counts the loss and its gradients are 0.  A bias of -inf is an
     action that is not open.  A decision that counts with NaN or +inf among its logits, with all of
     them -inf, or with a target outside ``[0, V)`` makes the loss NaN.

@@ -202,6 +202,21 @@ def test_the_bias_gradient_is_summed_before_it_is_rounded(rows, D, V, dtype):
     close(run(h, w, t, b, m, up)["bias"], (value, tol), "bias")
 
 
+@pytest.mark.parametrize("rows,D,V", [(1, 64, 9), (200, 64, 25), (300, 30, 60), (70, 128, 31), (33, 9, 40), (4000, 64, 64)])
+def test_gradients_of_narrow_bfloat16_heads_are_rounded_once(rows, D, V):
+    """What a target's probability lacks of 1 and the others' go into the products with 16 bits: a 2^-16 of
+    them where the tolerance of wide heads has a half step of the type."""
+    h, w, t, b, m = inputs(rows, D, V, torch.bfloat16, rows + V, mask=0.2 if rows > 1 else 0.0)
+    want, got = reference(h, w, t, b, m), run(h, w, t, b, m)
+    on = torch.ones(rows, dtype=torch.bool, device=DEV) if m is None else m
+    p = torch.softmax(h.double() @ w.double().t() + b.double(), -1)
+    mag = (p + torch.nn.functional.one_hot(t, V)) * on[:, None] / int(on.sum())
+    less = 1.01 * half(torch.bfloat16) - 2.0 ** -16
+    for name, of in (("hidden", mag @ w.double().abs()), ("weight", mag.t() @ h.double().abs())):
+        value, tol = want[name]
+        close(got[name], (value, tol - less * of), name)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("rows,D,V", [(40, 64, 25), (300, 64, 300), (20, 64, 300)])
 def test_a_row_of_the_lowest_biases(rows, D, V, dtype):
