@@ -967,8 +967,7 @@ template <typename T, int LANES> __global__ __launch_bounds__(BLOCK) void k_step
     }
 }
 
-// The same where dv is no multiple of four: a thread a column of v, all of dk in turn.
-// Few columns, not four: a thread one of them.
+// The same for 1, 2, 3 or 5 columns of v: a thread one of them, all of dk in turn.
 template <typename T> __global__ __launch_bounds__(BLOCK) void k_step_any(const swarp_decay_t a, int64_t n)
 {
     for (int64_t x = (int64_t)blockIdx.x * BLOCK + threadIdx.x; x < n; x += (int64_t)gridDim.x * BLOCK) {

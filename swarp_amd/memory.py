@@ -155,8 +155,7 @@ class _DecayFn(torch.autograd.Function):
         log_decay = _plain(log_decay)
         state = None if state is None else _plain(state)
         starts = None if starts is None else starts.contiguous()
-        like = torch.empty if g_out is not None else torch.zeros
-        g_out = _plain(g_out) if g_out is not None else like(
+        g_out = _plain(g_out) if g_out is not None else torch.zeros(
             (*q.shape[:-1], a.dv), dtype=q.dtype, device=dev)
         g_state = None if g_state is None else _plain(g_state)
         d = [torch.empty(t.shape, dtype=q.dtype, device=dev) for t in (q, k, v)]
