@@ -815,62 +815,132 @@ template <typename T, int FIT> __global__ __launch_bounds__(BLOCK, 2) void k_sho
 
 // The heads (and columns) where something was not finite, step by step, as the definition has it: what
 // a start or the order of the steps keeps from an output does not reach it as a product with 0.
-template <typename T, int KT> __global__ __launch_bounds__(BLOCK) void k_exact(const Call c, int64_t n)
+// A wave takes every `waves`-th unit, since those of one padded sequence are neighbours; lane l looks at the l-th of
+// them.  It does a unit with a column a lane, half of the state's rows in either half of the wave, from 16 steps'
+// rows in LDS; the next 16 are on their way meanwhile.  What bounds it is that chain: 4 operations for every row
+// of the half, 0.65 us a step of 64 rows.  4095 steps of 384 heads of 64, bfloat16, padded with NaN: 3.0 ms, of one sequence
+// of 96 the same (0.35 with nothing to do again; 64 units behind one another in a wave, as neighbours: 991 and 105).
+template <typename T, int KT> __global__ __launch_bounds__(BLOCK, KT <= 2 ? 2 : 1) void k_exact(const Call c, int64_t n)
 {
-    const int lane = threadIdx.x & 63, half = lane >> 5;
-    const int64_t all = (int64_t)gridDim.x * BLOCK;
-    for (int64_t first = ((int64_t)blockIdx.x * WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * 64; first < n; first += all) {
+    constexpr int STEPS = 16, HALF = 16 * KT, WIDE = 2 * HALF, EACH = STEPS * WIDE / 64;
+    struct __align__(16) F4 { float e[4]; };
+    __shared__ F4 room[WAVES][STEPS * (2 * WIDE + 32) / 4];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
+    float *const kx = (float *)room[wave], *const qx = kx + STEPS * WIDE, *const vx = qx + STEPS * WIDE;
+    const int64_t waves = (int64_t)gridDim.x * WAVES;
+    for (int64_t first = (int64_t)blockIdx.x * WAVES + wave; first < n; first += 64 * waves) {
         uint64_t wrong = 0;
-        if (first + lane < n) {
-            const int64_t bh = (first + lane) / c.slices, at = bh * c.segments * c.slices + (first + lane - bh * c.slices);
+        const int64_t own = first + lane * waves;
+        if (own < n) {
+            const int64_t bh = own / c.slices, at = bh * c.segments * c.slices + (own - bh * c.slices);
             for (int i = 0; i < c.segments; ++i) wrong |= c.wrong[at + (int64_t)i * c.slices];
         }
         wrong = __ballot(wrong != 0);
         for (; wrong; wrong &= wrong - 1) {
-            const int64_t unit = first + __ffsll((unsigned long long)wrong) - 1;
+            const int64_t unit = first + (__ffsll((unsigned long long)wrong) - 1) * waves;
             const int64_t bh = unit / c.slices, b = bh / c.heads;
             const int h = (int)(bh - b * c.heads);
             int slice = (int)(unit - bh * c.slices), which = 0;
             while (slice >= c.scan[which].slices) slice -= c.scan[which++].slices;
             const Scan &s = c.scan[which];
-            const int j = 32 * slice + (lane & 31), dk = s.dk;
+            const int j = 32 * slice + col, dk = s.dk, upper = (dk + 1) / 2, lower = dk - upper;  // rows of the halves
+            const int count = half ? lower : upper, row0 = half ? upper : 0;
             const bool back = s.back, mine = j < s.dv;
+            const int64_t steps = c.steps, groups = c.batch / c.group;
+            const T *const q = (const T *)s.q + b * s.qs[1] + h * s.qs[2], *const k = (const T *)s.k + b * s.ks[1] + h * s.ks[2];
+            const T *const v = (const T *)s.v + b * s.vs[1] + h * s.vs[2] + 32 * slice;
+            T *const out = (T *)s.out + b * s.os[1] + h * s.os[2] + j;
             const uint8_t *const starts = c.starts ? c.starts + b / c.group : nullptr;
-            const int64_t groups = c.batch / c.group;
-            float S[KT * 16];
+            const int64_t at = bh * c.area + (int64_t)row0 * s.si + (int64_t)j * s.sj;
+            float S[HALF];
 #pragma unroll
-            for (int r = 0; r < 16 * KT; ++r) {
-                const int i = 2 * r + half;
-                S[r] = s.state && i < dk && mine ? s.state[bh * c.area + (int64_t)i * s.si + (int64_t)j * s.sj] : 0.0f;
-            }
-            const float lambda = __builtin_amdgcn_exp2f(c.log_decay[h] * LOG2E);
-            for (int64_t x = 0; x < c.steps; ++x) {
-                const int64_t t = back ? c.steps - 1 - x : x;
-                const T *const q = (const T *)s.q + t * s.qs[0] + b * s.qs[1] + h * s.qs[2];
-                const T *const k = (const T *)s.k + t * s.ks[0] + b * s.ks[1] + h * s.ks[2];
-                const float v = mine ? (float)((const T *)s.v)[t * s.vs[0] + b * s.vs[1] + h * s.vs[2] + j] * s.grow : 0.0f;
-                const bool fresh = starts && (back ? x > 0 && starts[(t + 1) * groups] : starts[t * groups]);
-                float o = 0.0f;
+            for (int r = 0; r < HALF; ++r) S[r] = s.state && r < count && mine ? s.state[at + (int64_t)r * s.si] : 0.0f;
+            const float lambda = __builtin_amdgcn_exp2f(c.log_decay[h] * LOG2E), pre = back ? 1.0f : lambda, post = back ? lambda : 1.0f;
+            T kr[EACH], qr[EACH], vr[STEPS / 2];
+            uint8_t sr = 0;
+            auto time = [&](int64_t x) { return back ? steps - 1 - x : x; };
+            // (past the end of a row, or of the steps, the last element, or the last row: read, and not used)
+            const int j0 = mine ? col : s.dv - 1 - 32 * slice;
+            auto load = [&](int64_t x0) {
 #pragma unroll
-                for (int r = 0; r < 16 * KT; ++r) {
-                    const int i = 2 * r + half;
-                    if (i < dk) {
-                        const float kv = (float)k[i] * v;
-                        const float y = fresh ? kv : __builtin_fmaf(back ? 1.0f : lambda, S[r], kv);
-                        o = __builtin_fmaf((float)q[i], y, o);
-                        S[r] = back ? lambda * y : y;
-                    }
+                for (int m = 0; m < EACH; ++m) {
+                    const int e = m * 64 + lane, i = e % WIDE < dk ? e % WIDE : dk - 1;
+                    const int64_t t = time(x0 + e / WIDE < steps ? x0 + e / WIDE : steps - 1);
+                    kr[m] = k[t * s.ks[0] + i];
+                    qr[m] = q[t * s.qs[0] + i];
                 }
-                o += __shfl_xor(o, 32, 64);
-                if (half == 0 && mine) ((T *)s.out)[t * s.os[0] + b * s.os[1] + h * s.os[2] + j] = (T)(o * s.carry);
+#pragma unroll
+                for (int m = 0; m < STEPS / 2; ++m) {
+                    const int64_t x = x0 + 2 * m + half;
+                    vr[m] = v[time(x < steps ? x : steps - 1) * s.vs[0] + j0];
+                }
+                const int64_t x = x0 + lane;
+                sr = starts && lane < STEPS && x < steps && (!back || x > 0) ? starts[(back ? steps - x : x) * groups] : 0;
+            };
+            if (steps > 0) load(0);
+            for (int64_t x0 = 0; x0 < steps; x0 += STEPS) {
+#pragma unroll
+                for (int m = 0; m < EACH; ++m) {
+                    const int e = m * 64 + lane, i = e % WIDE;
+                    if (i >= dk) continue;
+                    const int to = e / WIDE * WIDE + (i < upper ? i : HALF + i - upper);
+                    kx[to] = (float)kr[m];
+                    qx[to] = (float)qr[m];
+                }
+#pragma unroll
+                for (int m = 0; m < STEPS / 2; ++m) vx[m * 64 + lane] = (float)vr[m] * s.grow;
+                const uint32_t fresh = (uint32_t)__ballot(sr);
+                __builtin_amdgcn_wave_barrier();
+                if (x0 + STEPS < steps) load(x0 + STEPS);
+                const int L = steps - x0 < STEPS ? (int)(steps - x0) : STEPS;
+#pragma unroll 1
+                for (int x = 0; x < L; ++x) {
+                    // (all asked for together; what lies behind the half's rows is not used)
+                    const F4 *const kk = (const F4 *)(kx + x * WIDE + half * HALF), *const qq = (const F4 *)(qx + x * WIDE + half * HALF);
+                    F4 k4[HALF / 4], q4[HALF / 4];
+#pragma unroll
+                    for (int r = 0; r < HALF / 4; ++r) {
+                        k4[r] = kk[r];
+                        q4[r] = qq[r];
+                    }
+                    const float vj = vx[x * 32 + col];
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (fresh >> x & 1) {
+#pragma unroll
+                        for (int r = 0; r < HALF; ++r) S[r] = 0.0f;
+                    }
+                    float o[4] = {};
+#pragma unroll
+                    for (int r0 = 0; r0 < HALF; r0 += 4) {
+                        // (the same for all lanes, but for the lower half's last row)
+                        if (r0 + 4 <= lower) {
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                const float y = __builtin_fmaf(pre, S[r0 + r], k4[r0 / 4].e[r] * vj);
+                                o[r] = __builtin_fmaf(q4[r0 / 4].e[r], y, o[r]);
+                                S[r0 + r] = post * y;
+                            }
+                        } else {
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                if (r0 + r >= upper) continue;
+                                const float y = __builtin_fmaf(pre, S[r0 + r], k4[r0 / 4].e[r] * vj), z = __builtin_fmaf(q4[r0 / 4].e[r], y, o[r]);
+                                o[r] = r0 + r < lower || half == 0 ? z : o[r];
+                                S[r0 + r] = post * y;
+                            }
+                        }
+                    }
+                    float sum = (o[0] + o[1]) + (o[2] + o[3]);
+                    sum += __shfl_xor(sum, 32, 64);
+                    if (half == 0 && mine) out[time(x0 + x) * s.os[0]] = (T)(sum * s.carry);
+                }
+                __builtin_amdgcn_wave_barrier();
             }
             if (s.state_out && mine) {
-                const bool clear = back && starts && c.steps > 0 && starts[0];
+                const bool clear = back && starts && steps > 0 && starts[0];
 #pragma unroll
-                for (int r = 0; r < 16 * KT; ++r) {
-                    const int i = 2 * r + half;
-                    if (i < dk) s.state_out[bh * c.area + (int64_t)i * s.si + (int64_t)j * s.sj] = clear ? 0.0f : S[r];
-                }
+                for (int r = 0; r < HALF; ++r)
+                    if (r < count) s.state_out[at + (int64_t)r * s.si] = clear ? 0.0f : S[r];
             }
         }
     }
@@ -1096,8 +1166,8 @@ template <typename T, int KT, int WHAT> void scan(Call &c, int fit, hipStream_t 
     else alone<T, KT, WHAT>(c, fit, st);
     if (WHAT == OUTPUTS) {
         const int64_t n = c.units / c.segments;
-        const int64_t blocks = (n + BLOCK - 1) / BLOCK;  // (of up to 2^34 units: a launch has fewer than 2^32 threads)
-        hipLaunchKernelGGL((k_exact<T, KT>), dim3((unsigned)(blocks < 16384 ? blocks : 16384)), dim3(BLOCK), 0, st, c, n);
+        const int64_t blocks = (n + WAVES - 1) / WAVES, most = MOST_WAVES / WAVES;  // (of up to 2^34 units)
+        hipLaunchKernelGGL((k_exact<T, KT>), dim3((unsigned)(blocks < most ? blocks : most)), dim3(BLOCK), 0, st, c, n);
     }
 }
 

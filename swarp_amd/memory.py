@@ -192,7 +192,8 @@ def decay_attention(
 
     ``scale`` is ``Dk ** -0.5`` unless given.  A start stops NaN and infinities as well, and a step
     does not look at later ones: what lies behind the end of a shorter sequence reaches only the
-    outputs there and the state.  Sums and states are float32; with bfloat16 the products are of
+    outputs there and the state.  (A head with something that is not finite is done again step by
+    step, some 0.7 us each: zeros behind the end are quicker.)  Sums and states are float32; with bfloat16 the products are of
     bfloat16 terms that carry 16 bits (24 for the state).
 
     Gradients flow to ``q``, ``k``, ``v`` and ``state`` from both results, once, and backward only.

@@ -161,6 +161,38 @@ def test_a_start_stops_everything_and_no_step_looks_ahead(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,batch,dk,dv", [(1, 9, 5, 7), (16, 3, 1, 1), (17, 3, 2, 33), (53, 3, 31, 100), (70, 20, 32, 32), (53, 3, 64, 65),
+                                           (53, 3, 127, 3), (40, 3, 3, 127), (75, 3, 128, 128), (2100, 1, 20, 24)])
+def test_what_is_not_finite_in_every_shape(T, batch, dk, dv, dtype):
+    """NaN and infinities anywhere, among starts: what the definition has finite is right, and the rest is not finite."""
+    H = 2
+    q, k, v, ld, state, s = inputs(T, (batch,), H, dk, dv, dtype, T + dv, 0.08)
+    g = gen(5)
+    g_out = torch.randn(v.shape, generator=g, device=DEV).to(dtype)
+    g_state = torch.randn(state.shape, generator=g, device=DEV)
+    for n, x in enumerate((q, k, v, state, g_out, g_state)):
+        at = torch.randint(0, x.numel(), (3,), generator=g, device=DEV)
+        x.view(-1)[at[:2]], x.view(-1)[at[2]] = math.nan, math.inf
+    if T > 60:  # a padded end
+        for x in (q, k, v, g_out):
+            x[T - 20:, 0] = math.nan
+    if T > 1000:
+        ld = ld * 0.1
+    x = [t.double().requires_grad_(True) for t in (q, k, v, state)]
+    o, S = recurrence(*x[:3], ld.double(), x[3], s)
+    want = [o.detach(), S.detach(), *torch.autograd.grad((o, S), x, (g_out.double(), g_state.double()))]
+    # (what is finite has none of the others in it: its terms' magnitudes are those without them)
+    clean = [torch.nan_to_num(t, 0.0, 0.0, 0.0) for t in (q, k, v, ld, state, g_out, g_state)]
+    mags = [m for _, m in both(*clean[:5], s, *clean[5:])]
+    got = run(q, k, v, ld, state, s, g_out, g_state)
+    keep = []
+    for name, y, z in zip(("out", "state", "q", "k", "v", "state0"), got, want):
+        assert torch.equal(y.isfinite(), z.isfinite()), name
+        keep.append(torch.where(z.isfinite(), y, 0.0))
+    check(keep, [(torch.where(z.isfinite(), z, 0.0), m) for z, m in zip(want, mags)], T, dk, dv, dtype, f"{T} {dk}x{dv} {dtype}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("T,dk,dv", [(20, 24, 32), (150, 24, 32), (150, 40, 72), (2100, 16, 32)])
 def test_a_start_stops_what_passed_the_largest_float(T, dk, dv, dtype):
     """Finite parts whose state, or whose products with it, are not: what a start parts from them is as if
