@@ -16,8 +16,8 @@ from torch.autograd import forward_ad
 from torch.compiler import is_dynamo_compiling
 
 from . import _lib
-from .policy import (_CODES, _differentiable_once, _guard, _no_tangents, _on_gpu, _plain, _ptr,
-                     _row_strides, _same, _untraced)
+from .policy import (_CODES, _capture_of, _differentiable_once, _guard, _no_tangents, _on_gpu,
+                     _plain, _ptr, _row_strides, _same, _untraced)
 
 _MOST_DIM, _MOST_WIDTH = 65536, 1 << 21
 _TYPES = {code: dtype for dtype, code in _CODES.items()}
@@ -90,7 +90,7 @@ class _LinearCeFn(torch.autograd.Function):
             ctx.save_for_backward(*grads, place)
         else:
             ctx.made = None if late else (grads, place)
-            ctx.capture = _lib.load().swarp_capture_id(stream)
+            ctx.capture = _capture_of(hidden, stream)
             ctx.work = work if complete else None
             ctx.save_for_backward(hidden, weight, bias, targets, mask)
         ctx.mark_non_differentiable(logp)
@@ -115,7 +115,7 @@ class _LinearCeFn(torch.autograd.Function):
                    for t in out]
         else:
             made, ctx.made = ctx.made, None  # handed out once: the caller may change them
-            if made is not None and ctx.capture != _lib.load().swarp_capture_id(ctx.stream):
+            if made is not None and ctx.capture != _capture_of(saved[0], ctx.stream):
                 made = None  # (a graph's replays find them changed, with no forward to leave new ones)
             if not _unmoved(a, ctx.like[0], *saved):
                 a = _lib.SwarpLinearCe.from_buffer_copy(a)

@@ -92,6 +92,12 @@ def _ptr(t: torch.Tensor | None):
     return None if t is None else t.data_ptr()
 
 
+def _capture_of(t: torch.Tensor, stream: int) -> int:
+    """Which graph capture the stream is part of, 0: none.  What a forward left is handed out by a
+    backward of the same one only: replays would find what became of it."""
+    return _lib.load().swarp_capture_id(stream) if t.is_cuda else 0
+
+
 _UNTRACED: dict = {}
 
 
@@ -320,7 +326,8 @@ class _LossFn(torch.autograd.Function):
     at hand: a training step then reads the heads once and writes their gradients once.  The
     backward hands them out; where the upstream gradient is not 1 (the device looks) it computes
     them again with it, so each is rounded once, from the tensors that autograd kept: under a
-    checkpoint or a packing hook the forward's own are gone.  float16 gradients are left to the
+    checkpoint or a packing hook the forward's own are gone.  So does a backward that is captured
+    into a graph without its forward.  float16 gradients are left to the
     backward: without the loss scale that comes with it they would vanish.
     """
 
@@ -333,6 +340,7 @@ class _LossFn(torch.autograd.Function):
         if head.dtype != torch.float16:
             ctx.made = _buffers(head, log_std, ctx.need)
             a.d_head, a.d_log_std = _ptr(ctx.made[0]), _ptr(ctx.made[1])
+            ctx.capture = _capture_of(head, stream)
         loss, stats, logp, ctx.work = _loss_forward(calls[0], a, head, rest[1], stream)
         ctx.like = head.shape, head.stride(), head.dtype, rest[0].dtype
         ctx.save_for_backward(head, log_std, *rest)
@@ -352,6 +360,8 @@ class _LossFn(torch.autograd.Function):
         if g.is_neg():
             g = g.resolve_neg()
         made, ctx.made = ctx.made, None  # handed out once: the caller may change them
+        if made is not None and ctx.capture != _capture_of(saved[0], stream):
+            made = None
         if made is None:
             d = _buffers(saved[0], saved[1], ctx.need)
             a = _lib.SwarpPolicy.from_buffer_copy(a)

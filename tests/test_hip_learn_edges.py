@@ -91,6 +91,42 @@ def test_losses_under_hooks_and_checkpoints(kind, dtype, up, way):
         assert all(same_bits(a, b) for a, b in zip(got, want)), (V, len(taken))
 
 
+@pytest.mark.parametrize("apart", [False, True])
+@pytest.mark.parametrize("up", [1.0, 64.0])
+@pytest.mark.parametrize("kind,dtype", HEADS)
+def test_losses_whose_backward_is_a_graph_of_its_own(kind, dtype, up, apart):
+    """Behind an eager forward, or one in another graph: every replay leaves what an eager backward does,
+    whatever became of the gradients in between."""
+    for V in (9, 300, 9000) if kind == "cat" else (3,):
+        g = gen(V)
+        head = torch.randn(18, V, generator=g, device=DEV).to(dtype)
+        std = (torch.randn(*(() if kind == "shared" else (18,)), V, generator=g, device=DEV) * 0.1).to(dtype)
+        act = torch.randint(0, V, (18,), generator=g, device=DEV) if kind == "cat" else head.float() + 0.3
+        old, adv = (torch.randn(18, generator=g, device=DEV) for _ in range(2))
+
+        def f(head, *std):
+            if kind == "cat":
+                return categorical_policy_loss(head, act, old - 1, adv).loss
+            return gaussian_policy_loss(head, *std, act, old - 1, adv).loss
+        x, y = ([t.clone().requires_grad_(True) for t in ((head,) if kind == "cat" else (head, std))] for _ in range(2))
+        want = torch.autograd.grad(f(*x) * up, x)
+        torch.cuda.synchronize()
+        one, two, side = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        with torch.cuda.graph(one, stream=side) if apart else torch.cuda.stream(side):
+            loss = f(*y)
+        torch.cuda.synchronize()
+        with torch.cuda.graph(two, stream=side):
+            got = torch.autograd.grad(loss * up, y, retain_graph=True)
+        if apart:
+            one.replay()
+        for _ in range(3):
+            two.replay()
+            torch.cuda.synchronize()
+            assert all(same_bits(a, b) for a, b in zip(got, want)), V
+            for t in got:
+                t.zero_()
+
+
 @pytest.mark.parametrize("way", ["pack", "host", "checkpoint"])
 @pytest.mark.parametrize("last", [False, True])
 def test_gae_under_hooks_and_checkpoints(last, way):
