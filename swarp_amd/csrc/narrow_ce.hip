@@ -12,7 +12,7 @@
 // now 76; float16 245, 155).
 // Three products of 2 rows dim width operations: far below what the rows cost to read and write.
 // 256000 rows of 64, 25 outputs, bfloat16: 34 us of the rows' kernel and 5 of adding up 512 workgroups' sums,
-// 69 MB in all (14 us): what is left is a wave's chain through 32 rows, 15 of them each, and its first ones.
+// 69 MB in all (14 us): what is left is a wave's chain through 32 rows, four of them each, and its first ones.
 #include <math.h>
 
 #include "narrow_ce.hpp"

@@ -194,7 +194,7 @@ def decay_attention(
     does not look at later ones: what lies behind the end of a shorter sequence reaches only the
     outputs there and the state.  (A head with something that is not finite is done again step by
     step, some 0.7 us each: zeros behind the end are quicker.)  Sums and states are float32; with bfloat16 the products are of
-    bfloat16 terms that carry 16 bits (24 for the state).
+    bfloat16 terms that carry 16 bits (24 in what enters the state).
 
     Gradients flow to ``q``, ``k``, ``v`` and ``state`` from both results, once, and backward only.
     """
