@@ -607,14 +607,15 @@ typedef struct swarp_decay {
     const void *adj_out;      /* as out, and as state_out, or NULL (zero); read by the _bwd call */
     const float *adj_state;
     void *d_q, *d_k, *d_v;    /* [steps, batch, heads, dk or dv]: the _bwd call writes all three */
-    float *d_state;           /* as state, or NULL */
+    float *d_state;           /* as state, or NULL; not `adj_state` itself */
     void *work;               /* swarp_decay_work_bytes() bytes, 256-byte aligned */
     uint64_t work_bytes;
 } swarp_decay_t;
 uint64_t swarp_decay_work_bytes(const swarp_decay_t *a); /* of either call */
 int swarp_decay_fwd(const swarp_decay_t *a, void *stream);
 int swarp_decay_bwd(const swarp_decay_t *a, void *stream);
-/* One step (steps = 1): state_out is written, `state` itself as a rule; q, k and v lie outside it.
+/* One step (steps = 1): state_out is written, `state` itself as a rule; q, k, v, log_decay and starts
+ * lie outside it.
  * No work memory. */
 int swarp_decay_step(const swarp_decay_t *a, void *stream);
 

@@ -1287,6 +1287,8 @@ int swarp_decay_fwd(const swarp_decay_t *a, void *stream)
     if (check(a)) return -1;
     if (!a->batch) return 0;
     if (!a->log_decay || (a->steps && (!a->q || !a->k || !a->v || !a->out))) return fail("pointer arguments must be set");
+    // (a head that is done again starts from it once more)
+    if (a->state && a->state == a->state_out) return fail("state_out must not be state");
     if (work(a, false)) return -1;
     // One step is mostly its states: 13487 x 4 heads of 32, float32, 81 us, and 282 as a chunk of one step; 3000
     // heads of 128, bfloat16, 79 and 132; 200000 of 4, float32, 82 and 1023.
@@ -1324,6 +1326,8 @@ int swarp_decay_bwd(const swarp_decay_t *a, void *stream)
     if (!a->log_decay || (a->steps && (!a->q || !a->k || !a->v || !a->adj_out)))
         return fail("pointer arguments must be set");
     if (a->steps && (!a->d_q || !a->d_k || !a->d_v)) return fail("d_q, d_k and d_v must be set, all three together");
+    // (the scans of k and of v both start from it)
+    if (a->adj_state && a->adj_state == a->d_state) return fail("d_state must not be adj_state");
     if (work(a, true)) return -1;
     Call c = call_of(a, true);
     const float scale = (float)a->scale;
@@ -1382,7 +1386,7 @@ int swarp_decay_step(const swarp_decay_t *a, void *stream)
     if (a->steps != 1) return fail("a step is one step");
     if (!a->log_decay || !a->q || !a->k || !a->v || !a->out || !a->state_out)
         return fail("pointer arguments must be set");
-    // (the state is changed while others still read q, k and v)
+    // (the state is changed while others still read what the step is made of)
     const uintptr_t size = a->dtype == SWARP_F32 ? 4 : 2, from = (uintptr_t)a->state_out;
     const uintptr_t to = from + (uintptr_t)a->batch * a->heads * a->dk * a->dv * 4;
     auto apart = [&](const void *x, const int64_t *stride, int d) {
@@ -1391,6 +1395,9 @@ int swarp_decay_step(const swarp_decay_t *a, void *stream)
     };
     if (!apart(a->q, a->q_stride, a->dk) || !apart(a->k, a->k_stride, a->dk) || !apart(a->v, a->v_stride, a->dv))
         return fail("q, k and v must not lie in the state");
+    const uintptr_t decay = (uintptr_t)a->log_decay, starts = (uintptr_t)a->starts;
+    if ((decay < to && decay + 4 * (uintptr_t)a->heads > from) || (starts && starts < to && starts + a->batch / a->group > from))
+        return fail("log_decay and starts must not lie in the state");
     step_of(a, (hipStream_t)stream);
     return launched();
 }

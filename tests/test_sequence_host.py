@@ -162,6 +162,27 @@ def test_linear_ce_work_memory_is_what_is_said(dtype, size):
                     assert 0 < need <= copies + 60 * N + rest + 8192, (N, D, V, grads)
 
 
+def test_decay_refuses_states_in_place():
+    lib = _lib.load()
+    a = _lib.SwarpDecay(dtype=0, heads=2, dk=8, dv=8, steps=3, batch=4, group=1, scale=1.0, log_decay=256, q=256, k=256, v=256,
+                        out=256, adj_out=256, d_q=256, d_k=256, d_v=256, work=256)
+    a.work_bytes = lib.swarp_decay_work_bytes(ctypes.byref(a))
+    a.state = a.state_out = 512
+    refused(lib.swarp_decay_fwd(ctypes.byref(a), None), "must not be state")
+    a.adj_state = a.d_state = 512
+    refused(lib.swarp_decay_bwd(ctypes.byref(a), None), "must not be adj_state")
+
+
+def test_a_steps_decay_and_starts_lie_outside_its_state():
+    lib, state, n = _lib.load(), 1 << 20, 4 * 2 * 8 * 8 * 4
+    strides = {x + "_stride": (ctypes.c_int64 * 3)(0, 16, 8) for x in "qkv"}
+    for name, size in (("log_decay", 8), ("starts", 4)):
+        for at in (state, state + n - 1, state - size + 1):
+            a = _lib.SwarpDecay(**{**dict(dtype=0, heads=2, dk=8, dv=8, steps=1, batch=4, group=1, scale=1.0, log_decay=256, q=256,
+                                          k=256, v=256, out=256, state_out=state, **strides), name: at})
+            refused(lib.swarp_decay_step(ctypes.byref(a), None), "in the state")
+
+
 def test_heads_beyond_a_launch_are_refused():
     lib = _lib.load()
     a = _lib.SwarpDecay(dtype=0, heads=(1 << 22) + 1, dk=8, dv=8, steps=1, batch=1, group=1)
